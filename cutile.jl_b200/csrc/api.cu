@@ -63,6 +63,19 @@ int* sched_slot(ctb_ctx* ctx) {
   return ctx->sched_pool + 2 * (n % kSchedSlots);
 }
 
+int check_in_place(const char* who, const void* in, int64_t ld_in, const void* out, int64_t ld_out, int64_t n, int64_t rows,
+                   int64_t elem_size) {
+  const uintptr_t a0 = (uintptr_t)in, a1 = a0 + ((rows - 1) * ld_in + n) * elem_size;
+  const uintptr_t b0 = (uintptr_t)out, b1 = b0 + ((rows - 1) * ld_out + n) * elem_size;
+  if (b0 >= a1 || a0 >= b1 || (b0 == a0 && (ld_in == ld_out || rows == 1))) return CTB_OK;
+  if (ld_in == ld_out && rows > 1) {  // columns of one array side by side
+    const uintptr_t row = (uintptr_t)(n * elem_size), pitch = (uintptr_t)(ld_in * elem_size);
+    const uintptr_t apart = (b0 > a0 ? b0 - a0 : a0 - b0) % pitch;
+    if (apart >= row && pitch - apart >= row) return CTB_OK;
+  }
+  return fail(CTB_BAD_ARG, "%s: the gradient must lie where its rows lie or not overlap them", who);
+}
+
 EncodeTiledFn encode_tiled() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;

@@ -87,6 +87,27 @@ int fmha_decode(ctb_ctx* ctx, cudaStream_t st, const void* Q, const void* K, con
                 int64_t seq_kv, int64_t heads, int64_t kv_heads, int64_t batch, float qk_scale, int input_pos, int64_t keys, bool causal,
                 bool bf16, bool* taken);
 
+// The context's device is the current one while the object lives.
+class CurrentDevice {
+ public:
+  explicit CurrentDevice(const ctb_ctx* ctx) {
+    if (cudaGetDevice(&before_) == cudaSuccess && before_ != ctx->device) cudaSetDevice(ctx->device);
+    else before_ = -1;
+  }
+  ~CurrentDevice() {
+    if (before_ >= 0) cudaSetDevice(before_);
+  }
+  CurrentDevice(const CurrentDevice&) = delete;
+  CurrentDevice& operator=(const CurrentDevice&) = delete;
+
+ private:
+  int before_ = -1;
+};
+
+// A gradient of `rows` rows of n elements may be written over the rows that it is made from, row for row, but not across them.
+int check_in_place(const char* who, const void* in, int64_t ld_in, const void* out, int64_t ld_out, int64_t n, int64_t rows,
+                   int64_t elem_size);
+
 // cuTensorMapEncodeTiled, resolved through the runtime so that the library has
 // no link-time dependency on libcuda and loads on machines without a driver.
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -56,6 +56,11 @@ SIGNATURES = {
     "ctb_set_tf32_rounding": [_p, _i],
     "ctb_validate_hints": [_i, _i, _i, _i],
     "ctb_softmax": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i],
+    "ctb_token_logprobs": [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _f, _i],
+    "ctb_token_logprobs_bwd": [_p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _f, _i],
+    "ctb_distill_fwd": [_p, _p, _p, _p, _i, _p, _i, _p, _p, _p, _i64, _i64, _i64, _i, _f, _i],
+    "ctb_distill_bwd": [_p, _p, _p, _p, _p, _i, _p, _i, _p, _p, _i64, _i64, _i64, _i64, _i, _f, _i],
+    "ctb_distill_fwd_bwd": [_p, _p, _p, _p, _p, _i, _p, _i, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _f, _i],
     "ctb_vadd": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i],
     "ctb_transpose": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i],
     "ctb_tiled_broadcast": [_p, _p, _p, C.POINTER(_i64), C.POINTER(_p), C.POINTER(_i64), _i, C.POINTER(C.c_int32), _i,
@@ -79,6 +84,8 @@ SIGNATURES = {
     "ctb_layernorm_bwd_static_status": [_p],
     "ctb_moe_max_blocks": [_i64, _i64, _i64, _i],
     "ctb_moe_router": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i],
+    "ctb_moe_route": [_p, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i, _f, _i],
+    "ctb_moe_route_bwd": [_p, _p, _p, _p, _p, _i, _p, _i, _i64, _i64, _i64, _i64, _i, _i, _i, _f, _i],
     "ctb_moe_align": [_p, _p, _p, _i, _i64, _i64, _i64, _i, _p, _p, _p, _i64],
     "ctb_moe_fused_gemm": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _i],
     "ctb_moe_silu_and_mul": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i],

@@ -79,3 +79,32 @@ def dtype_code(t):
     if t.dtype == torch.bfloat16:
         return _lib.BF16
     raise _lib.CtbError(_lib.BAD_ARG, f"unsupported element type {t.dtype}")
+
+
+def ids_bits(t, what):
+    """Width of an array of ids."""
+    if t.dtype == torch.int32:
+        return 32
+    if t.dtype == torch.int64:
+        return 64
+    raise _lib.CtbError(_lib.BAD_ARG, f"{what} must be int32 or int64")
+
+
+def dense(t, shape, what, like, dtype=None):
+    """`t` is a dense tensor of this shape (and type) on the device of `like`."""
+    if not isinstance(t, torch.Tensor) or t.device != like.device:
+        raise _lib.CtbError(_lib.BAD_ARG, f"{what}: expected a tensor on {like.device}")
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise _lib.CtbError(_lib.BAD_ARG, f"{what}: expected a dense tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise _lib.CtbError(_lib.BAD_ARG, f"{what}: expected {dtype}, got {t.dtype}")
+    return t
+
+
+def gradient_of(logits, out):
+    """(out, its leading dimension): `out`, or a new dense array like `logits`."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif not isinstance(out, torch.Tensor) or out.device != logits.device or out.shape != logits.shape or out.dtype != logits.dtype:
+        raise _lib.CtbError(_lib.BAD_ARG, "out must have the shape, type and device of the logits")
+    return out, rows(out, "out")[0]

@@ -10,7 +10,7 @@ import ctypes as C
 import torch
 
 from . import _host, _lib
-from ._util import handles, ptr
+from ._util import dense, dtype_code, gradient_of, handles, ids_bits, ptr, rows
 
 
 def _ids_bits(t):
@@ -38,6 +38,50 @@ def moe_router(hidden_states, W_r, topk, return_logits=False):
     _lib.check(_lib.lib.ctb_moe_router(ctx, stream, ptr(hidden_states), ptr(W_r), ptr(ids), ptr(w), ptr(logits), T, H,
                                        E, int(topk)))
     return (w, ids, logits) if return_logits else (w, ids)
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _score(name):
+    if name not in _SCORES:
+        raise _lib.CtbError(_lib.BAD_ARG, f"score must be one of {sorted(_SCORES)}, got {name!r}")
+    return _SCORES[name]
+
+
+def moe_route(logits, topk, bias=None, score="softmax", groups=1, topk_groups=1, group_top=1, renormalize=True, scale=1.0,
+              weights_dtype=torch.float16, **hints):
+    """Routing by given logits (E, T), torch [T, E] in f32, f16 or bf16: the topk experts with the largest score + bias (score =
+    softmax or sigmoid of the logits, bias [E] f32 or None), out of the topk_groups best of `groups` equal runs of experts (a group is as good
+    as its best expert, or with group_top = 2 as the sum of its two best).  Weights are the chosen scores without the bias, divided by their
+    sum with `renormalize`, times `scale`.  Returns (topk_weights [topk, T], topk_ids [topk, T] int32): what cutile_moe takes."""
+    ctx, stream = handles(logits, hints)
+    ld, T, E = rows(logits, "logits")
+    topk, kind = int(topk), _score(score)
+    if bias is not None:
+        dense(bias, (E,), "bias", logits, torch.float32)
+    weights = torch.empty((max(topk, 0), T), dtype=weights_dtype, device=logits.device)
+    ids = torch.empty((max(topk, 0), T), dtype=torch.int32, device=logits.device)
+    _lib.check(_lib.lib.ctb_moe_route(ctx, stream, ptr(logits), ptr(bias), ptr(ids), ptr(weights), dtype_code(weights), T, E, ld, topk,
+                                      kind, int(groups), int(topk_groups), int(group_top), int(bool(renormalize)),
+                                      float(scale), dtype_code(logits)))
+    return weights, ids
+
+
+def moe_route_bwd(logits, topk_ids, d_weights, score="softmax", renormalize=True, scale=1.0, out=None, **hints):
+    """Gradient of the logits, [T, E] in their type, from the gradient d_weights [topk, T] (f32, f16 or bf16) of moe_route's weights
+    and its topk_ids.  `out` may be the logits."""
+    ctx, stream = handles(logits, hints)
+    ld, T, E = rows(logits, "logits")
+    if not isinstance(topk_ids, torch.Tensor) or topk_ids.dim() != 2:
+        raise _lib.CtbError(_lib.BAD_ARG, "moe_route_bwd: topk_ids must have the shape [topk, T]")
+    topk, kind = topk_ids.shape[0], _score(score)
+    bits = ids_bits(dense(topk_ids, (topk, T), "topk_ids", logits), "topk_ids")
+    dense(d_weights, (topk, T), "d_weights", logits)
+    out, ld_out = gradient_of(logits, out)
+    _lib.check(_lib.lib.ctb_moe_route_bwd(ctx, stream, ptr(out), ptr(logits), ptr(topk_ids), bits, ptr(d_weights), dtype_code(d_weights), T, E,
+                                          ld_out, ld, topk, kind, int(bool(renormalize)), float(scale), dtype_code(logits)))
+    return out
 
 
 def moe_align_tile_size(topk_ids, tile_m, num_experts):

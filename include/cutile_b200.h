@@ -96,6 +96,56 @@ int ctb_validate_hints(int num_ctas, int occupancy, int opt_level, int num_worke
 int ctb_softmax(ctb_ctx* ctx, void* stream, void* output, const void* input, int64_t N, int64_t M, int64_t ld_out,
                 int64_t ld_in, int variant, int tile_size, int dtype);
 
+/* ---- Log probabilities of given tokens -------------------------------------- */
+/* (No counterpart in the reference.)  logits (V, T): T rows of V contiguous elements, row stride ld, CTB_F32, CTB_F16 or
+ * CTB_BF16, rows may start at any element; arithmetic and results are f32.  With z = logits / temperature
+ * (1e-6 <= temperature <= 1e6):
+ *   lse      (T) = log sum_v exp(z_v)
+ *   logprobs (T) = z[token] - lse; tokens (T), 1-based, 32- or 64-bit (token_bits)
+ *   entropy  (T) = -sum_v p_v log p_v, p = exp(z - lse)
+ *   top_logprobs, top_ids (top, T) = the `top` most probable elements of a row in descending order, log probabilities
+ *                  and 1-based ids, equal logits by ascending id; 0 <= top <= 32, top <= V.
+ * logprobs comes with tokens; tokens, entropy and lse may be NULL.  A row whose token is 0 is padding: its logits are not
+ * read and its results are 0.  A token outside of 0..V is a bad index (ctb_check_device_status) with log probability NaN.
+ * Masked elements (-inf) have probability 0 and come last among the alternatives; a row that is masked as a whole, or
+ * has NaN or +inf, has NaN results, and its top_ids (0..V) mean nothing.  Bitwise repeatable. */
+int ctb_token_logprobs(ctb_ctx* ctx, void* stream, const void* logits, const void* tokens, int token_bits, float* logprobs,
+                       float* entropy, float* lse, float* top_logprobs, int32_t* top_ids, int64_t V, int64_t T, int64_t ld,
+                       int top, float temperature, int dtype);
+/* Gradient: d_logits (V, T), row stride ld_out, in the type of logits, from the gradients d_logprobs (T), d_entropy (T) and
+ * d_top_logprobs (top, T) of the results (each may be NULL) and the lse, entropy (with d_entropy) and top_ids (with
+ * d_top_logprobs) of the forward call.  Padding rows and rows with a bad token get 0.  An id that occurs more than once
+ * takes the sum.  d_logits may be the logits themselves, and must not overlap them in any other way. */
+int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* tokens, int token_bits,
+                           const float* lse, const float* entropy, const float* d_logprobs, const float* d_entropy,
+                           const int32_t* top_ids, const float* d_top_logprobs, int64_t V, int64_t T, int64_t ld_out,
+                           int64_t ld, int top, float temperature, int dtype);
+
+/* ---- Distillation from a teacher's top logits --------------------------------- */
+/* (No counterpart in the reference.)  logits (V, T) of the student as above; teacher_ids (entries, T), 1-based, 32- or
+ * 64-bit, 0 for an unused entry; teacher_values (entries, T) in f32, f16 or bf16 (values_dtype); both dense, 1 <= entries <=
+ * 256.  With u = teacher_values / temperature, p the student's probabilities at that temperature and the sums over the
+ * used entries:
+ *   teacher_lse NULL: q_j = exp(u_j) / sum_i exp(u_i);     loss = sum_j q_j (log q_j - log p[id_j])
+ *   else:             q_j = exp(u_j - teacher_lse), and what is left, q_r = max(0, 1 - sum_j q_j), stands against the
+ *                     probability p_r that the student gives to all ids that are not listed:
+ *                     loss = sum_j q_j (log q_j - log p[id_j]) + q_r (log q_r - log p_r)
+ * loss (T) f32; saved (4, T) f32, 16-byte aligned, is what the gradient needs.  An id may occur more than once.  A row without a
+ * used entry is padding: its logits are not read, loss and gradient are 0.  An id outside of 0..V is a bad index
+ * (ctb_check_device_status): the row's loss is NaN and its gradient 0. */
+int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
+                    const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved, int64_t V,
+                    int64_t T, int64_t ld, int entries, float temperature, int dtype);
+/* Gradient: d_logits (V, T) from d_loss (T) and saved; d_logits as in ctb_token_logprobs_bwd. */
+int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
+                    const void* teacher_values, int values_dtype, const float* saved, const float* d_loss, int64_t V, int64_t T,
+                    int64_t ld_out, int64_t ld, int entries, float temperature, int dtype);
+/* Both at once, for a d_loss that is known before the loss: the logits are read from memory once. */
+int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
+                        const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
+                        const float* d_loss, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature,
+                        int dtype);
+
 /* ---- Element-wise addition and transpose ----------------------------------- */
 /* vec_add_kernel_1d(a, b, c, tile)                    examples/vadd.jl:10-17
  * vec_add_kernel_2d(a, b, c, tile_x, tile_y)          examples/vadd.jl:20-28
@@ -244,6 +294,25 @@ int64_t ctb_moe_max_blocks(int64_t T, int64_t topk, int64_t E, int tile_m);
  * logits (E, T) f32 or NULL. */
 int ctb_moe_router(ctb_ctx* ctx, void* stream, const void* hidden, const void* W_r, int32_t* topk_ids,
                    void* topk_weights, float* logits, int64_t T, int64_t H, int64_t E, int topk);
+
+/* Routing by given logits (no counterpart in the reference).  logits (E, T), row stride ld, CTB_F32, CTB_F16 or CTB_BF16,
+ * E <= 512.  s = softmax or sigmoid of a token's logits; c = s + bias (E) f32, or s (bias NULL).  With topk_groups <
+ * groups (<= 32, equal runs of experts), a group scores its best c (group_top 1) or the sum of its two best (2), and only
+ * experts of the topk_groups best groups (ties to the first) can be chosen.  The topk (<= 32) experts with the largest c,
+ * compared in f64, are chosen in descending order, ties to the smallest index, c = NaN or -inf last.  Weights: scale * s
+ * of the chosen, divided by max(sum of the chosen s, 1e-20) with renormalize.
+ * Outputs: topk_ids (T, topk) int32, 1-based; topk_weights (T, topk) in weights_dtype: what ctb_moe_ffn takes. */
+enum { CTB_SCORE_SOFTMAX = 0, CTB_SCORE_SIGMOID = 1 };
+int ctb_moe_route(ctb_ctx* ctx, void* stream, const void* logits, const float* bias, int32_t* topk_ids, void* topk_weights,
+                  int weights_dtype, int64_t T, int64_t E, int64_t ld, int topk, int score, int groups, int topk_groups,
+                  int group_top, int renormalize, float scale, int dtype);
+/* Gradient of the logits, (E, T) in their type with row stride ld_out, from d_weights (T, topk) in weights_dtype and the
+ * topk_ids (T, topk), 32- or 64-bit, of the choice; the bias takes none.  An id of 0 is no choice, one outside of 0..E a bad
+ * index (ctb_check_device_status) and no choice either; ids that occur twice take the sum.  d_logits may be the logits
+ * themselves, and must not overlap them in any other way. */
+int ctb_moe_route_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* topk_ids, int ids_bits,
+                      const void* d_weights, int weights_dtype, int64_t T, int64_t E, int64_t ld_out, int64_t ld, int topk,
+                      int score, int renormalize, float scale, int dtype);
 
 /* moe_align_tile_size(topk_ids, tile_m, num_experts)      examples/moe.jl:142-183
  * Runs on the device (the reference copies the ids to the host and sorts there).
