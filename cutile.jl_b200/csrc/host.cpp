@@ -12,6 +12,7 @@
 // (through the Python function installed by setup()).
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -361,6 +362,252 @@ PyObject* moe_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
   if (s != CTB_OK) return done(s, nullptr);
   return THPVariable_Wrap(std::move(out));
+}
+
+// ---- rows of scores -----------------------------------------------------------------------------------------------
+// A tensor or None; false: something else.
+bool maybe_tensor(PyObject* o, const Tensor** t) {
+  *t = nullptr;
+  return o == Py_None || (*t = cuda_tensor(o));
+}
+bool same_device(const Tensor* t, const Tensor& x) { return !t || t->get_device() == x.get_device(); }
+bool maybe_f32(const Tensor* t, const Tensor& x, at::IntArrayRef shape) {
+  return !t || (t->scalar_type() == at::kFloat && t->sizes() == shape && t->is_contiguous() && same_device(t, x));
+}
+int bits_of(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : t.scalar_type() == at::kLong ? 64 : 0; }
+float* f32(const Tensor* t) { return t ? static_cast<float*>(t->data_ptr()) : nullptr; }
+void* data(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
+// logits with contiguous rows and the gradient's array (a new one when none is given)
+struct Rows {
+  const Tensor* x = nullptr;
+  int64_t ld = 0, T = 0, V = 0, ld_out = 0;
+  int dtype = -1;
+  Tensor out;
+  bool take(PyObject* o) { return (x = cuda_tensor(o)) && rows(*x, &ld, &T, &V) && (dtype = dtype_of(*x)) >= 0; }
+  bool take_out(PyObject* o) {
+    const Tensor* t;
+    if (!maybe_tensor(o, &t)) return false;
+    if (t) {
+      int64_t m, k;
+      if (!rows(*t, &ld_out, &m, &k) || m != T || k != V || t->scalar_type() != x->scalar_type() || !same_device(t, *x)) return false;
+      out = *t;
+    }
+    return true;
+  }
+  void make_out() {
+    if (out.defined()) return;
+    out = at::empty({T, V}, x->options());
+    ld_out = V;
+  }
+};
+PyObject* pack(std::initializer_list<Tensor*> list) {  // a tuple; None for undefined tensors
+  PyObject* r = PyTuple_New((Py_ssize_t)list.size());
+  Py_ssize_t i = 0;
+  for (Tensor* t : list) {
+    PyObject* o = !r ? nullptr : t->defined() ? THPVariable_Wrap(std::move(*t)) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_XDECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+// token_logprobs(logits, tokens or None, top, temperature, entropy) -> (logprobs, entropy, lse, top_logprobs, top_ids)
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  const Tensor* tokens;
+  long long top;
+  float temperature;
+  if (n != 5 || !r.take(a[0]) || !maybe_tensor(a[1], &tokens) || !as_int(a[2], &top) || top < 0 || !as_float(a[3], &temperature) ||
+      !PyBool_Check(a[4]))
+    return decline();
+  const int bits = tokens ? bits_of(*tokens) : 64;
+  if (!bits || (tokens && (tokens->dim() != 1 || tokens->size(0) != r.T || !tokens->is_contiguous() || !same_device(tokens, *r.x))))
+    return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  const auto f = r.x->options().dtype(at::kFloat);
+  Tensor lp, h, lse = at::empty({r.T}, f), tlp, tid;
+  if (tokens) lp = at::empty({r.T}, f);
+  if (a[4] == Py_True) h = at::empty({r.T}, f);
+  if (top) {
+    tlp = at::empty({r.T, top}, f);
+    tid = at::empty({r.T, top}, f.dtype(at::kInt));
+  }
+  const int s = without_gil([&] {
+    auto p = [](const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; };
+    return ctb_token_logprobs(c.ctx, c.stream, r.x->data_ptr(), data(tokens), bits, p(lp), p(h), p(lse), p(tlp),
+                              tid.defined() ? static_cast<int32_t*>(tid.data_ptr()) : nullptr, r.V, r.T, r.ld, (int)top, temperature,
+                              r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return pack({&lp, &h, &lse, &tlp, &tid});
+}
+
+// token_logprobs_bwd(logits, tokens, lse, entropy, d_logprobs, d_entropy, top_ids, d_top_logprobs, temperature, out) -> out
+PyObject* token_logprobs_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  const Tensor* t[7];  // tokens, lse, entropy, d_logprobs, d_entropy, top_ids, d_top
+  float temperature;
+  if (n != 10 || !r.take(a[0]) || !as_float(a[8], &temperature) || !r.take_out(a[9])) return decline();
+  for (int i = 0; i < 7; ++i)
+    if (!maybe_tensor(a[1 + i], &t[i])) return decline();
+  const int bits = t[0] ? bits_of(*t[0]) : 64;
+  if (!bits || (t[0] && (t[0]->dim() != 1 || t[0]->size(0) != r.T || !t[0]->is_contiguous() || !same_device(t[0], *r.x))) || !t[1] ||
+      (t[4] && !t[2]) || (t[6] && !t[5]))
+    return decline();
+  for (int i = 1; i < 5; ++i)
+    if (!maybe_f32(t[i], *r.x, {r.T})) return decline();
+  int64_t top = 0;
+  if (t[6]) {
+    if (t[5]->dim() != 2 || t[5]->scalar_type() != at::kInt || !t[5]->is_contiguous() || !same_device(t[5], *r.x)) return decline();
+    top = t[5]->size(1);
+    if (t[5]->size(0) != r.T || !maybe_f32(t[6], *r.x, {r.T, top})) return decline();
+  }
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  r.make_out();
+  const int s = without_gil([&] {
+    return ctb_token_logprobs_bwd(c.ctx, c.stream, r.out.data_ptr(), r.x->data_ptr(), data(t[0]), bits, f32(t[1]), f32(t[2]), f32(t[3]),
+                                  f32(t[4]), top ? static_cast<const int32_t*>(t[5]->data_ptr()) : nullptr, top ? f32(t[6]) : nullptr,
+                                  r.V, r.T, r.ld_out, r.ld, (int)top, temperature, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return THPVariable_Wrap(std::move(r.out));
+}
+
+// a teacher's list: ids [T, entries], values [T, entries]
+struct Teacher {
+  const Tensor *ids = nullptr, *values = nullptr;
+  int bits = 0, dtype = -1, entries = 0;
+  bool take(PyObject* i, PyObject* v, const Rows& r) {
+    if (!(ids = cuda_tensor(i)) || !(values = cuda_tensor(v)) || ids->dim() != 2 || ids->size(0) != r.T || ids->size(1) > 4096 ||
+        values->sizes() != ids->sizes() || !ids->is_contiguous() || !values->is_contiguous() || !same_device(ids, *r.x) ||
+        !same_device(values, *r.x))
+      return false;
+    bits = bits_of(*ids);
+    dtype = dtype_of(*values);
+    entries = (int)ids->size(1);
+    return bits && dtype >= 0;
+  }
+};
+
+// distill_fwd(logits, ids, values, teacher_lse or None, temperature) -> (loss, saved)
+PyObject* distill_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  Teacher t;
+  const Tensor* lse;
+  float temperature;
+  if (n != 5 || !r.take(a[0]) || !t.take(a[1], a[2], r) || !maybe_tensor(a[3], &lse) || !maybe_f32(lse, *r.x, {r.T}) ||
+      !as_float(a[4], &temperature))
+    return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  const auto f = r.x->options().dtype(at::kFloat);
+  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 4}, f);
+  const int s = without_gil([&] {
+    return ctb_distill_fwd(c.ctx, c.stream, r.x->data_ptr(), t.ids->data_ptr(), t.bits, t.values->data_ptr(), t.dtype, f32(lse), f32(&loss),
+                           f32(&saved), r.V, r.T, r.ld, t.entries, temperature, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return pack({&loss, &saved});
+}
+
+// distill_bwd(logits, ids, values, saved, d_loss, temperature, out) -> out
+PyObject* distill_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  Teacher t;
+  const Tensor *saved, *d;
+  float temperature;
+  if (n != 7 || !r.take(a[0]) || !t.take(a[1], a[2], r) || !(saved = cuda_tensor(a[3])) || !maybe_f32(saved, *r.x, {r.T, 4}) ||
+      !(d = cuda_tensor(a[4])) || !maybe_f32(d, *r.x, {r.T}) || !as_float(a[5], &temperature) || !r.take_out(a[6]))
+    return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  r.make_out();
+  const int s = without_gil([&] {
+    return ctb_distill_bwd(c.ctx, c.stream, r.out.data_ptr(), r.x->data_ptr(), t.ids->data_ptr(), t.bits, t.values->data_ptr(), t.dtype,
+                           f32(saved), f32(d), r.V, r.T, r.ld_out, r.ld, t.entries, temperature, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return THPVariable_Wrap(std::move(r.out));
+}
+
+// distill_fwd_bwd(logits, ids, values, d_loss, teacher_lse or None, temperature, out) -> (loss, out)
+PyObject* distill_fwd_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  Teacher t;
+  const Tensor *lse, *d;
+  float temperature;
+  if (n != 7 || !r.take(a[0]) || !t.take(a[1], a[2], r) || !(d = cuda_tensor(a[3])) || !maybe_f32(d, *r.x, {r.T}) ||
+      !maybe_tensor(a[4], &lse) || !maybe_f32(lse, *r.x, {r.T}) || !as_float(a[5], &temperature) || !r.take_out(a[6]))
+    return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  r.make_out();
+  const auto f = r.x->options().dtype(at::kFloat);
+  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 4}, f);
+  const int s = without_gil([&] {
+    return ctb_distill_fwd_bwd(c.ctx, c.stream, r.out.data_ptr(), r.x->data_ptr(), t.ids->data_ptr(), t.bits, t.values->data_ptr(), t.dtype,
+                               f32(lse), f32(&loss), f32(&saved), f32(d), r.V, r.T, r.ld_out, r.ld, t.entries, temperature, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return pack({&loss, &r.out});
+}
+
+int score_of(PyObject* o) {  // -1: neither
+  if (!PyUnicode_Check(o)) return -1;
+  if (PyUnicode_CompareWithASCIIString(o, "softmax") == 0) return CTB_SCORE_SOFTMAX;
+  return PyUnicode_CompareWithASCIIString(o, "sigmoid") == 0 ? CTB_SCORE_SIGMOID : -1;
+}
+
+// moe_route(logits, topk, bias or None, score, groups, topk_groups, group_top, renormalize, scale, weights' dtype) -> (weights, ids)
+PyObject* moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  const Tensor* bias;
+  long long topk, g[3];
+  float scale;
+  if (n != 10 || !r.take(a[0]) || !as_int(a[1], &topk) || topk < 1 || topk > r.V || !maybe_tensor(a[2], &bias) ||
+      !maybe_f32(bias, *r.x, {r.V}) || !ints(a + 4, 3, g) || !PyBool_Check(a[7]) || !as_float(a[8], &scale) || !THPDtype_Check(a[9]))
+    return decline();
+  const int score = score_of(a[3]);
+  const at::ScalarType wt = reinterpret_cast<THPDtype*>(a[9])->scalar_type;
+  const int wdtype = wt == at::kFloat ? CTB_F32 : wt == at::kHalf ? CTB_F16 : wt == at::kBFloat16 ? CTB_BF16 : -1;
+  if (score < 0 || wdtype < 0) return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  Tensor w = at::empty({topk, r.T}, r.x->options().dtype(wt)), ids = at::empty({topk, r.T}, r.x->options().dtype(at::kInt));
+  const int s = without_gil([&] {
+    return ctb_moe_route(c.ctx, c.stream, r.x->data_ptr(), f32(bias), static_cast<int32_t*>(ids.data_ptr()), w.data_ptr(), wdtype, r.T, r.V,
+                         r.ld, (int)topk, score, (int)g[0], (int)g[1], (int)g[2], a[7] == Py_True, scale, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return pack({&w, &ids});
+}
+
+// moe_route_bwd(logits, ids, d_weights, score, renormalize, scale, out) -> out
+PyObject* moe_route_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Rows r;
+  const Tensor *ids, *d;
+  float scale;
+  if (n != 7 || !r.take(a[0]) || !(ids = cuda_tensor(a[1])) || !(d = cuda_tensor(a[2])) || !PyBool_Check(a[4]) || !as_float(a[5], &scale) ||
+      !r.take_out(a[6]))
+    return decline();
+  const int score = score_of(a[3]), bits = bits_of(*ids), wdtype = dtype_of(*d);
+  if (score < 0 || !bits || wdtype < 0 || ids->dim() != 2 || ids->size(1) != r.T || ids->size(0) > r.V || d->sizes() != ids->sizes() ||
+      !ids->is_contiguous() || !d->is_contiguous() || !same_device(ids, *r.x) || !same_device(d, *r.x))
+    return decline();
+  Call c(*r.x);
+  if (!c.ok()) return nullptr;
+  r.make_out();
+  const int s = without_gil([&] {
+    return ctb_moe_route_bwd(c.ctx, c.stream, r.out.data_ptr(), r.x->data_ptr(), ids->data_ptr(), bits, d->data_ptr(), wdtype, r.T, r.V,
+                             r.ld_out, r.ld, (int)ids->size(0), score, a[4] == Py_True, scale, r.dtype);
+  });
+  if (s != CTB_OK) return done(s, nullptr);
+  return THPVariable_Wrap(std::move(r.out));
 }
 
 // ---- host-level array expressions ---------------------------------------------------------------------------------
@@ -748,6 +995,9 @@ PyMethodDef kMethods[] = {CTB_METHOD(setup),         CTB_METHOD(softmax),       
                           CTB_METHOD(fmha),          CTB_METHOD(moe_router),     CTB_METHOD(moe_ffn),
                           CTB_METHOD(unary),         CTB_METHOD(binary),         CTB_METHOD(assign),
                           CTB_METHOD(mapreduce),     CTB_METHOD(fft),
+                          CTB_METHOD(token_logprobs), CTB_METHOD(token_logprobs_bwd), CTB_METHOD(distill_fwd),
+                          CTB_METHOD(distill_bwd),   CTB_METHOD(distill_fwd_bwd), CTB_METHOD(moe_route),
+                          CTB_METHOD(moe_route_bwd),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Native call path of cutile_b200.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

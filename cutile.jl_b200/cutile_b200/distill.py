@@ -10,7 +10,7 @@ leaves of the teacher's probability stands against what the student gives to all
 """
 import torch
 
-from . import _lib
+from . import _host, _lib
 from ._util import dense, dtype_code, gradient_of, handles, ids_bits, ptr, rows
 
 
@@ -28,6 +28,10 @@ def _teacher(logits, T, ids, values, lse):
 
 def distill_fwd(logits, teacher_ids, teacher_values, teacher_lse=None, temperature=1.0, **hints):
     """Returns (loss [T] f32, saved [T, 4] f32); saved is what distill_bwd needs."""
+    if not hints:
+        r = _host.distill_fwd(logits, teacher_ids, teacher_values, teacher_lse, temperature)
+        if r is not None:
+            return r
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
     entries, bits, values_code = _teacher(logits, T, teacher_ids, teacher_values, teacher_lse)
@@ -41,6 +45,10 @@ def distill_fwd(logits, teacher_ids, teacher_values, teacher_lse=None, temperatu
 
 def distill_bwd(logits, teacher_ids, teacher_values, saved, d_loss, temperature=1.0, out=None, **hints):
     """Gradient of the logits, [T, V] in their type, from d_loss [T] f32 and what distill_fwd saved.  `out` may be the logits."""
+    if not hints:
+        r = _host.distill_bwd(logits, teacher_ids, teacher_values, saved, d_loss, temperature, out)
+        if r is not None:
+            return r if out is None else out
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
     entries, bits, values_code = _teacher(logits, T, teacher_ids, teacher_values, None)
@@ -55,6 +63,10 @@ def distill_bwd(logits, teacher_ids, teacher_values, saved, d_loss, temperature=
 def distill_fwd_bwd(logits, teacher_ids, teacher_values, d_loss, teacher_lse=None, temperature=1.0, out=None, **hints):
     """Loss and gradient at once, for a d_loss [T] f32 that is known beforehand (the rows' weights): the logits are read once.
     Returns (loss [T] f32, gradient [T, V]); `out` may be the logits."""
+    if not hints:
+        r = _host.distill_fwd_bwd(logits, teacher_ids, teacher_values, d_loss, teacher_lse, temperature, out)
+        if r is not None:
+            return r if out is None else (r[0], out)
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
     entries, bits, values_code = _teacher(logits, T, teacher_ids, teacher_values, teacher_lse)

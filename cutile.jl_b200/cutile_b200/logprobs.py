@@ -7,7 +7,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib
+from . import _host, _lib
 from ._util import dense, dtype_code, gradient_of, handles, ids_bits, ptr, rows
 
 
@@ -24,6 +24,10 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, entropy=True, **
     """Log probabilities under softmax(logits / temperature) of `tokens` ([T] int32 or int64; a row with token 0 is padding:
     it is not read and its results are 0), the entropies, and the `top` (up to 32) most probable elements of every row, equal ones
     by ascending id.  Returns a TokenLogprobs."""
+    if not hints:
+        r = _host.token_logprobs(logits, tokens, top, temperature, entropy)
+        if r is not None:
+            return TokenLogprobs._make(r)
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
 
@@ -42,6 +46,10 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, d_logprobs=None, d_entropy=
                        out=None, **hints):
     """Gradient of the logits, [T, V] in their type, from the gradients of the results of token_logprobs (any of them None) and
     its lse, entropy (needed with d_entropy) and top_ids (needed with d_top_logprobs).  `out` may be the logits themselves."""
+    if not hints:
+        r = _host.token_logprobs_bwd(logits, tokens, lse, entropy, d_logprobs, d_entropy, top_ids, d_top_logprobs, temperature, out)
+        if r is not None:
+            return r if out is None else out
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
     bits = 64 if tokens is None else ids_bits(dense(tokens, (T,), "tokens", logits), "tokens")

@@ -55,6 +55,10 @@ def moe_route(logits, topk, bias=None, score="softmax", groups=1, topk_groups=1,
     softmax or sigmoid of the logits, bias [E] f32 or None), out of the topk_groups best of `groups` equal runs of experts (a group is as good
     as its best expert, or with group_top = 2 as the sum of its two best).  Weights are the chosen scores without the bias, divided by their
     sum with `renormalize`, times `scale`.  Returns (topk_weights [topk, T], topk_ids [topk, T] int32): what cutile_moe takes."""
+    if not hints:
+        r = _host.moe_route(logits, topk, bias, score, groups, topk_groups, group_top, renormalize, scale, weights_dtype)
+        if r is not None:
+            return r
     ctx, stream = handles(logits, hints)
     ld, T, E = rows(logits, "logits")
     topk, kind = int(topk), _score(score)
@@ -71,6 +75,10 @@ def moe_route(logits, topk, bias=None, score="softmax", groups=1, topk_groups=1,
 def moe_route_bwd(logits, topk_ids, d_weights, score="softmax", renormalize=True, scale=1.0, out=None, **hints):
     """Gradient of the logits, [T, E] in their type, from the gradient d_weights [topk, T] (f32, f16 or bf16) of moe_route's weights
     and its topk_ids.  `out` may be the logits."""
+    if not hints:
+        r = _host.moe_route_bwd(logits, topk_ids, d_weights, score, renormalize, scale, out)
+        if r is not None:
+            return r if out is None else out
     ctx, stream = handles(logits, hints)
     ld, T, E = rows(logits, "logits")
     if not isinstance(topk_ids, torch.Tensor) or topk_ids.dim() != 2:
