@@ -46,28 +46,6 @@ __device__ __forceinline__ void unpack_row(const uint4& q, float (&f)[16 / sizeo
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ uint4 pack_row(const float (&f)[16 / sizeof(T)]) {
-  uint32_t w[4];
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
-  } else if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // A vector of -inf.
 template <typename T>
 __device__ __forceinline__ uint4 empty_row_vec() {
@@ -75,41 +53,105 @@ __device__ __forceinline__ uint4 empty_row_vec() {
   return make_uint4(w, w, w, w);
 }
 
-// Element i of vector v is an element of the row.
-template <int V>
-__device__ __forceinline__ bool in_row(int off, int n, int v, int i) {
-  const int e = v * V - off + i;
-  return e >= 0 && e < n;
+// A 32-bit word of a row is one f32 or two 16-bit elements.  Larger of two words, element by element; NEVER_NAN: a number where one of
+// them is NaN, else NaN.
+template <typename T, bool NEVER_NAN>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (NEVER_NAN) asm("max.f32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.f32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    if constexpr (NEVER_NAN) asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  } else {
+    if constexpr (NEVER_NAN) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  }
+  return d;
+}
+// The elements of a 16-bit word.
+template <typename T>
+__device__ __forceinline__ float2 word_pair(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// The larger element of a word.
+template <typename T>
+__device__ __forceinline__ float word_max(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else {
+    const float2 f = word_pair<T>(w);
+    return fmaxf(f.x, f.y);
+  }
+}
+// Pair i of a vector's elements.
+template <typename T>
+__device__ __forceinline__ float2 vec_pair(const uint32_t (&w)[4], int i) {
+  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else return word_pair<T>(w[i]);
 }
 
-// KEEP: the row is read again, from L2.
-template <typename T, bool KEEP = false>
-__device__ __forceinline__ uint4 load_row_vec(const T* src, int off, int n, int v) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int e0 = v * V - off;
-  if (e0 >= 0 && e0 + V <= n) {
-    const uint4* p = reinterpret_cast<const uint4*>(src + e0);
-    return KEEP ? __ldcg(p) : __ldcs(p);
-  }
-  uint4 q = empty_row_vec<T>();
-  T* f = reinterpret_cast<T*>(&q);
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (e0 + i >= 0 && e0 + i < n) f[i] = src[e0 + i];
-  return q;
-}
-// aligned: the row that is written lies off elements behind a vector boundary, like the one that was read.
 template <typename T>
-__device__ __forceinline__ void store_row_vec(T* dst, int off, int n, int v, const float (&f)[16 / sizeof(T)], bool aligned) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int e0 = v * V - off;
-  if (aligned && e0 >= 0 && e0 + V <= n) {
-    __stcs(reinterpret_cast<uint4*>(dst + e0), pack_row<T>(f));
-    return;
+__device__ __forceinline__ void put_pair(uint32_t (&w)[4], int i, float2 f) {
+  if constexpr (sizeof(T) == 4) {
+    w[2 * i] = __float_as_uint(f.x);
+    w[2 * i + 1] = __float_as_uint(f.y);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
+}
+
+// A row and the vectors [v0, v1) of it.
+template <typename T>
+struct Range {
+  static constexpr int V = 16 / (int)sizeof(T);
+  const T* src;
+  int off, n, v0, v1;
+
+  __device__ __forceinline__ bool has(int v, int i) const {  // element i of vector v is one of the row
+    const int e = v * V - off + i;
+    return e >= 0 && e < n;
+  }
+  // Vectors [v, v + count) lie wholly inside of the row and the range.
+  __device__ __forceinline__ bool inside(int v, int count) const {
+    return (v > 0 || off == 0) && v + count <= v1 && (v + count) * V - off <= n;
+  }
+  __device__ __forceinline__ const uint4* at(int v) const { return reinterpret_cast<const uint4*>(src - off) + v; }
+};
+
+// A vector that may be partly outside of the row; -inf there, and beyond the range.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T* src, int off, int n, int v) {
+  constexpr int V = 16 / (int)sizeof(T);
+  uint4 q = empty_row_vec<T>();
+  T f[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (e0 + i >= 0 && e0 + i < n) dst[e0 + i] = from_float<T>(f[i]);
+  for (int i = 0; i < V; ++i) {
+    const int e = v * V - off + i;
+    f[i] = e >= 0 && e < n ? src[e] : reinterpret_cast<const T*>(&q)[0];
+  }
+  return *reinterpret_cast<const uint4*>(f);
+}
+template <typename T, bool KEEP = false>
+__device__ __forceinline__ uint4 load_vec(const Range<T>& r, int v) {
+  if (v >= r.v1) return empty_row_vec<T>();
+  if (r.inside(v, 1)) return KEEP ? __ldcg(r.at(v)) : __ldcs(r.at(v));
+  return load_edge<T>(r.src, r.off, r.n, v);
+}
+// Writes a vector to a row that starts like r; what is outside of the row is left as it is.
+template <typename T>
+__device__ __noinline__ void store_edge(T* dst, int off, int n, int v, uint4 q) {
+  constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = v * V - off + i;
+    if (e >= 0 && e < n) dst[e] = reinterpret_cast<const T*>(&q)[i];
+  }
 }
 
 // Two f32 operations in one instruction.
