@@ -12,6 +12,7 @@
 #include <float.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "ctx.h"
@@ -23,23 +24,31 @@ using namespace ctb_internal;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;            // that stream
 constexpr int kWarps = kThreads / 32;
+constexpr int kAllThreads = kThreads + 32;  // and the clerk
 constexpr int kUnroll = 4;               // vectors of 16 bytes per thread and tile
 constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
 constexpr int kMaxEntries = kThreads;    // of a teacher's list
 constexpr int kCand = 1024;
-constexpr int kMaxParts = 32;
-constexpr int kPlainPerSm = 5, kTopPerSm = 4, kDistillPerSm = 4, kBackwardPerSm = 4;  // CTAs on an SM
+template <bool TOP>
+constexpr int kLogprobsPerSm = TOP ? 3 : 5;  // CTAs on an SM
+constexpr int kDistillPerSm = 4;
+template <bool DISTILL>
+constexpr int kBackwardPerSm = DISTILL ? 4 : 5;
 constexpr int kMostHoles = 512 * 1024;  // elements of a part that have a bit (in two sets) in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Exponents (base 2) are held above this where they are multiplied by their power, which is 0 there: 0 * -inf would be NaN.
 constexpr float kLowest = -16384.f;
-// A thread's reference follows its maximum only when an element is 2^kSlack above it: powers up to 2^kSlack are harmless in f32.
-constexpr float kSlack = 64.f;
+// A thread's reference follows its maximum only when an element is 2^kSlack above it.
+constexpr float kSlack = 4.f;
 constexpr float kFar = 1e30f;  // rows with a maximum beyond +-kFar (masked as a whole, or infinite) are summed in another way
+
+__device__ __forceinline__ void bar_stream() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the streaming threads
+__device__ __forceinline__ void bar_row() { asm volatile("bar.sync 2, 288;" ::: "memory"); }         // and the clerk
+static_assert(kThreads == 256, "the barriers name the numbers of threads");
 
 // ------------------------------------------------------------------ the best k of a row
 // One pass, every element compared with a threshold that at least k earlier elements reach:
@@ -65,14 +74,14 @@ struct Best {
   int out_index[kMaxTop];
 };
 
-// The k-th largest of the 64 group maxima; the whole CTA.
+// The k-th largest of the 64 group maxima; all streaming threads.
 __device__ __forceinline__ float group_threshold(float mine, int k, Best& b) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float g = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
   g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
   const int i = warp * 8 + (lane >> 2);
   if ((lane & 3) == 0) b.group[i] = g;
-  __syncthreads();
+  bar_stream();
   int rank = 0;  // among a quarter of the groups per lane
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
@@ -83,12 +92,12 @@ __device__ __forceinline__ float group_threshold(float mine, int k, Best& b) {
   rank += __shfl_xor_sync(0xffffffffu, rank, 1);
   rank += __shfl_xor_sync(0xffffffffu, rank, 2);
   if (rank == k - 1 && (lane & 3) == 0) b.theta = g;
-  __syncthreads();
+  bar_stream();
   return b.theta;
 }
 
-// Writes the best k of the n listed elements to out_*, in order; what is missing gets index -1.  The whole CTA; the list is complete and
-// visible.
+// Writes the best k of the n listed elements to out_*, in order; what is missing gets index -1.  All streaming threads; the list is
+// complete and visible.
 __device__ void select_list(int n, int k, Best& b) {
   const int tid = threadIdx.x;
   const float* value = b.value;
@@ -107,10 +116,10 @@ __device__ void select_list(int n, int k, Best& b) {
       }
     value = b.value2;
     index = b.index2;
-    __syncthreads();
+    bar_stream();
     n = b.count2;
   } else {
-    __syncthreads();
+    bar_stream();
   }
   for (int i = tid; i < n; i += kThreads) {
     const float v = value[i];
@@ -122,7 +131,7 @@ __device__ void select_list(int n, int k, Best& b) {
       b.out_index[rank] = id;
     }
   }
-  __syncthreads();
+  bar_stream();
 }
 
 // Adds the first `need` elements that equal `value`, in the order of their indices, to the `have` listed ones; returns how many are listed.
@@ -148,7 +157,7 @@ __device__ int append_equal(const Range<T>& r, float value, int have, int need, 
       if (lane >= o) upto += x;
     }
     if (lane == 31) b.warp_n[warp] = upto;
-    __syncthreads();
+    bar_stream();
     int at = upto - mine, total = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) at += b.warp_n[w];
@@ -160,7 +169,7 @@ __device__ int append_equal(const Range<T>& r, float value, int have, int need, 
     }
     have += min(total, need);
     need -= min(total, need);
-    __syncthreads();
+    bar_stream();
   }
   return have;
 }
@@ -182,7 +191,7 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
   int want = k;
   for (int shift = 24; shift >= 0; shift -= 8) {
     hist[tid] = 0;
-    __syncthreads();
+    bar_stream();
     for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
       float f[V];
       unpack_row<T>(load_vec(r, v), f);
@@ -192,22 +201,22 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
         if (f[i] == f[i] && r.has(v, i) && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
       }
     }
-    __syncthreads();
+    bar_stream();
     if (tid == 0) {
       int bin = 255, above = 0;
       while (bin > 0 && above + hist[bin] < want) above += hist[bin--];
       b.bin = bin;
       b.above = above;
     }
-    __syncthreads();
+    bar_stream();
     prefix |= (uint32_t)b.bin << shift;
     mask |= 255u << shift;
     want -= b.above;
-    __syncthreads();
+    bar_stream();
   }
   const float kth = key_value(prefix);
   if (tid == 0) b.count = 0;
-  __syncthreads();
+  bar_stream();
   for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
     float f[V];
     unpack_row<T>(load_vec(r, v), f);
@@ -219,86 +228,128 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
         b.index[at] = v * V - r.off + i;
       }
   }
-  __syncthreads();
+  bar_stream();
   return append_equal(r, kth, b.count, want, b);
 }
 
 // ------------------------------------------------------------------ sums of a row
+// Exponents t = x c - m2, with c = log2(e) / temperature: one fused multiply-add gives them with one rounding, whatever the magnitude of x, and
+// the rounding of c is that of a temperature, the same for the whole row.
+//
+// A thread's share of s = sum 2^t and w = sum 2^t t.  Its reference m2 follows its maximum, or t 2^t of a likely element would carry a
+// rounding that the entropy, a difference of two such sums, shows.  Masked elements (-inf) make w NaN (0 * -inf); the tile's share is
+// then taken again with exponents held above kLowest.  Valid for rows whose maximum is `plain`; the others take slow_sums.
 template <typename T>
-__device__ __forceinline__ void load_tile(uint4 (&q)[kUnroll], const Range<T>& r, int v, bool keep) {
-  const int tid = threadIdx.x;
-  if (r.inside(v, kTile)) {
-    const uint4* p = r.at(v) + tid;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = keep ? __ldcg(p + u * kThreads) : __ldcs(p + u * kThreads);
-  } else {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = load_vec(r, v + u * kThreads + tid);
-  }
-}
-
-// A thread's share of s = sum 2^(x c - m2) and w = sum 2^(x c - m2) (x c - m2), with c = log2(e) / temperature: one fused multiply-add gives
-// an exponent with one rounding, whatever the magnitude of x, and the rounding of c is that of a temperature, the same for the whole row.
-// Masked elements (-inf) would make w NaN (0 * -inf): with ENTROPY words are raised to a floor whose power is 0.  Valid for rows whose
-// maximum is `plain`; the others take slow_sums.
-template <typename T, bool ENTROPY>
 struct Sums {
-  [[maybe_unused]] static constexpr uint32_t kFloor = sizeof(T) == 4 ? 0xf149f2cau : std::is_same<T, __half>::value ? 0xfbfffbffu : 0xf14af14au;
-  // -1e30 (bf16: the next one below), -65504
   float m2 = 0.f, limit = -FLT_MAX;  // elements above limit move the reference
   uint32_t top = empty_row_vec<T>().x;
-  float2 s = make_float2(0.f, 0.f), w = make_float2(0.f, 0.f);
+  Pair s = pair(0.f, 0.f), w = pair(0.f, 0.f);
 
-  static __device__ __forceinline__ bool plain(float maximum, float c) {
-    if (!(maximum <= kFar && maximum >= -0.1f * kFar)) return false;
-    return !(ENTROPY && std::is_same<T, __half>::value) || (maximum + 65504.f) * c > 256.f;
+  static __device__ __forceinline__ bool plain(float maximum) { return maximum <= kFar && maximum >= -kFar; }
+  __device__ __forceinline__ void move(float t, float c) {
+    const float x = fminf(fmaxf(t, -kFar), kFar), to = x * c, d = fmaxf(fminf(m2 - to, 0.f), kLowest), r = ex2_approx_ftz(d);
+    const Pair rr = pair(r, r);
+    w = mul2(rr, fma2(s, pair(d, d), w));
+    s = mul2(rr, s);
+    m2 = to;
+    limit = x + kSlack / c;
   }
   // Returns the largest element of the tile.
   __device__ __forceinline__ float add(const uint4 (&q)[kUnroll], float c) {
     uint32_t all = 0;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t a = max_word<T, true>(max_word<T, true>(q[u].x, q[u].y), max_word<T, true>(q[u].z, q[u].w));
-      all = u == 0 ? a : max_word<T, true>(all, a);
+      const uint32_t a = max_word<T>(max_word<T>(q[u].x, q[u].y), max_word<T>(q[u].z, q[u].w));
+      all = u == 0 ? a : max_word<T>(all, a);
     }
-    top = max_word<T, true>(top, all);
-    const float t = word_max<T>(all);
-    if (t > limit) {
-      const float x = fminf(fmaxf(t, -kFar), kFar), to = x * c, d = fmaxf(fminf(m2 - to, 0.f), kLowest), r = ex2_approx_ftz(d);
-      if constexpr (ENTROPY) {
-        w.x = r * fmaf(s.x, d, w.x);
-        w.y = r * fmaf(s.y, d, w.y);
-      }
-      s.x *= r;
-      s.y *= r;
-      m2 = to;
-      limit = x + kSlack / c;
-    }
-    const float2 cc = make_float2(c, c), minus = make_float2(-m2, -m2);
-    float2 ts = make_float2(0.f, 0.f), tw = ts;
+    top = max_word<T>(top, all);
+    const float most = word_max<T>(all);
+    if (most > limit) move(most, c);
+    const Pair cc = pair(c, c), minus = pair(-m2, -m2);
+    Pair ts = pair(0.f, 0.f), tw = ts;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-      if constexpr (ENTROPY)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word[i] = max_word<T, false>(word[i], kFloor);
+      const uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
       for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
-        const float2 t2 = fma_pair(vec_pair<T>(word, i), cc, minus);
-        const float2 e = make_float2(ex2_approx_ftz(t2.x), ex2_approx_ftz(t2.y));
-        ts = add_pair(ts, e);
-        if constexpr (ENTROPY) tw = fma_pair(e, t2, tw);
+        const Pair t = fma2(vec_pair<T>(word, i), cc, minus), e = exp2_pair(t);
+        ts = add2(ts, e);
+        tw = fma2(e, t, tw);
       }
     }
-    s = add_pair(s, ts);
-    if constexpr (ENTROPY) w = add_pair(w, tw);
-    return t;
+    s = add2(s, ts);
+    if (sum_of(tw) != sum_of(tw)) tw = pair((again(q[0], m2, c) + again(q[1], m2, c)) + (again(q[2], m2, c) + again(q[3], m2, c)), 0.f);
+    w = add2(w, tw);
+    return most;
+  }
+  static __device__ __noinline__ float again(uint4 q, float m2, float c) {
+    static_assert(kUnroll == 4, "add() calls this for each vector of a tile");
+    float f[16 / sizeof(T)], a = 0.f;
+    unpack_row<T>(q, f);
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+      const float t = fmaf(f[i], c, -m2);
+      a = fmaf(ex2_approx_ftz(t), fmaxf(t, kLowest), a);
+    }
+    return a;
+  }
+  // One element more.
+  __device__ __forceinline__ void add_one(float x, float c) {
+    const T e = from_float<T>(x);
+    top = max_word<T>(top, sizeof(T) == 4 ? __float_as_uint(x) : 0x10001u * *reinterpret_cast<const unsigned short*>(&e));
+    if (x > limit) move(x, c);
+    const float t = fmaf(x, c, -m2), v = ex2_approx_ftz(t);
+    s = add2(s, pair(v, 0.f));
+    w = add2(w, pair(v * fmaxf(t, kLowest), 0.f));
   }
   // The warp's (maximum, s, w), the sums relative to that maximum.
   __device__ __forceinline__ float3 over_warp(float c) const {
     const float most = warp_max(word_max<T>(top)), to = fminf(fmaxf(most, -kFar), kFar);
-    const float d = fminf(fmaf(-to, c, m2), 1.f), r = ex2_approx_ftz(d), sum = s.x + s.y;  // a thread without elements has m2 = sum = 0
-    return make_float3(most, warp_sum(sum * r), ENTROPY ? warp_sum(r * fmaf(sum, fmaxf(d, kLowest), w.x + w.y)) : 0.f);
+    const float d = fminf(fmaf(-to, c, m2), 1.f), r = ex2_approx_ftz(d), sum = sum_of(s);  // a thread without elements has m2 = sum = 0
+    return make_float3(most, warp_sum(sum * r), warp_sum(r * fmaf(sum, fmaxf(d, kLowest), sum_of(w))));
+  }
+};
+
+// s alone, for the warp: the reference is the largest element of the warp's first tile that has one above -inf, and stays.  What is
+// more than 2^127 above it, or all of it below f32, shows as a sum that is not finite and positive; the row then takes slow_sums.
+template <typename T>
+struct LeanSums {
+  float ref = -INFINITY, m2 = 0.f;  // m2 = ref c
+  Pair s = pair(0.f, 0.f);
+
+  __device__ __forceinline__ void add(const uint4 (&q)[kUnroll], float c) {
+    if (ref == -INFINITY) {  // the same in the whole warp
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        most = max_nan(most, max_nan(max_nan(word_nan<T>(q[u].x), word_nan<T>(q[u].y)), max_nan(word_nan<T>(q[u].z), word_nan<T>(q[u].w))));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (most == -INFINITY) return;
+      ref = fminf(fmaxf(most, -kFar), kFar);  // of NaN: any number, the sum will be NaN
+      m2 = ref * c;
+    }
+    const Pair cc = pair(c, c), minus = pair(-m2, -m2);
+    Pair ts = pair(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+      for (int i = 0; i < 8 / (int)sizeof(T); ++i) ts = add2(ts, exp2_pair(fma2(vec_pair<T>(word, i), cc, minus)));
+    }
+    s = add2(s, ts);
+  }
+  // One element more of each lane (-inf: none).
+  __device__ __forceinline__ void add_one(float x, float c) {
+    uint4 q[kUnroll] = {empty_row_vec<T>(), empty_row_vec<T>(), empty_row_vec<T>(), empty_row_vec<T>()};
+    const T e = from_float<T>(x);
+    q[0].x = sizeof(T) == 4 ? __float_as_uint(x) : (q[0].x & 0xffff0000u) | *reinterpret_cast<const unsigned short*>(&e);
+    add(q, c);
+  }
+  // The warp's (reference, s), s relative to that reference.
+  __device__ __forceinline__ float2 over_warp(float c) const {
+    const float sum = warp_sum(sum_of(s));
+    return make_float2(ref, ref == -INFINITY ? 0.f : sum * ex2_approx_ftz(fmaf(-ref, c, m2)));
   }
 };
 
@@ -323,41 +374,72 @@ __device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
   }
 }
 
-// The sums of a warp's threads relative to a maximum that is not `plain`, from differences (x - maximum).
+// (maximum, s, w) of a range whose sums above are not valid, relative to its maximum, from differences (x - maximum); without the elements
+// that the `entries` ids name.  All streaming threads; `red` is theirs.
 template <typename T>
-__device__ __noinline__ float2 slow_sums(const Range<T>& r, const unsigned* holes, float maximum, float c) {
+__device__ __noinline__ float3 slow_sums(const Range<T>& r, const int* entry, int entries, float c, float (&red)[3][kWarps]) {
   constexpr int V = 16 / (int)sizeof(T);
-  float s = 0.f, w = 0.f;
-  for (int v = r.v0 + (int)threadIdx.x; v < r.v1; v += kThreads) {
-    uint4 q = load_vec(r, v);
-    if (holes) mask_holes<T>(q, hole_bits<T>(holes, v - r.v0));
-    float f[V];
-    unpack_row<T>(q, f);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float most = -FLT_MAX, s = 0.f, w = 0.f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
+      uint4 q = load_vec(r, v);
+      unsigned bits = 0;
+      for (int j = 0; j < entries; ++j) {
+        const int i = entry[j] - 1 + r.off - v * V;
+        if (entry[j] && i >= 0 && i < V) bits |= 1u << i;
+      }
+      if (bits) mask_holes<T>(q, bits);
+      float f[V];
+      unpack_row<T>(q, f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float t = (f[i] - maximum) * c, e = ex2_approx_ftz(t);
-      s += e;
-      w = fmaf(e, fmaxf(t, kLowest), w);
+      for (int i = 0; i < V; ++i) {
+        if (pass == 0) {
+          most = fmaxf(most, f[i]);
+        } else {
+          const float t = (f[i] - most) * c, e = ex2_approx_ftz(t);
+          s += e;
+          w = fmaf(e, fmaxf(t, kLowest), w);
+        }
+      }
+    }
+    bar_stream();  // red has been read
+    if (pass == 0) {
+      most = warp_max(most);
+      if (lane == 0) red[0][warp] = most;
+    } else {
+      s = warp_sum(s);
+      w = warp_sum(w);
+      if (lane == 0) {
+        red[1][warp] = s;
+        red[2][warp] = w;
+      }
+    }
+    bar_stream();
+    if (pass == 0) {
+      for (int i = 0; i < kWarps; ++i) most = fmaxf(most, red[0][i]);
     }
   }
-  return make_float2(warp_sum(s), warp_sum(w));
+  s = w = 0.f;
+  for (int i = 0; i < kWarps; ++i) {
+    s += red[1][i];
+    w += red[2][i];
+  }
+  return make_float3(most, s, w);
 }
 
-// (s, w) of the eight warps, each relative to its own maximum and held by lanes w, w + 8, ..., relative to the maximum of them all.
-__device__ __forceinline__ float2 join(float maximum, float s, float w, float most, float c) {
-  const float d = (maximum - most) * c, r = ex2_approx_ftz(d);
-  float a = s * r, b = r * fmaf(s, fmaxf(d, kLowest), w);
+// (s, w) of up to 8 or 16 sets of sums, held by lanes i, i + 8 (16), ..., each relative to a maximum of its own, relative to `most`.
+// apart: of the set's maximum below `most`, in units of log2.
+template <int OF>
+__device__ __forceinline__ float2 join(float apart, float s, float w) {
+  const float r = ex2_approx_ftz(apart);
+  float a = s * r, b = r * fmaf(s, fmaxf(apart, kLowest), w);
 #pragma unroll
-  for (int o = kWarps / 2; o > 0; o >>= 1) {
+  for (int o = OF / 2; o > 0; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     b += __shfl_xor_sync(0xffffffffu, b, o);
   }
   return make_float2(a, b);
-}
-// The same for the records of a row's parts, whose maxima are finite; one per lane.
-__device__ __forceinline__ float2 join_parts(float4 record, float most, float c) {
-  const float d = (record.x - most) * c, r = ex2_approx_ftz(d);
-  return make_float2(warp_sum(record.y * r), warp_sum(r * fmaf(record.y, fmaxf(d, kLowest), record.z)));
 }
 __device__ __forceinline__ float red_max(const float (&v)[kWarps]) {
   float m = v[0];
@@ -374,31 +456,184 @@ __device__ __forceinline__ float load_value(const void* p, long long i, int dtyp
   if (dtype == CTB_F16) return __half2float(static_cast<const __half*>(p)[i]);
   return __uint_as_float((uint32_t) static_cast<const unsigned short*>(p)[i] << 16);
 }
-template <typename T>
-__device__ __forceinline__ Range<T> range_of(const void* x, long long ld, int n, long long row, int part, int per) {
-  constexpr int V = 16 / (int)sizeof(T);
-  Range<T> r;
-  r.src = static_cast<const T*>(x) + row * ld;
-  r.off = (int)(((uintptr_t)r.src & 15) / sizeof(T));
-  r.n = n;
-  const int nvec = (r.off + n + V - 1) / V;
-  r.v0 = min(nvec, part * per);
-  r.v1 = min(nvec, r.v0 + per);
-  return r;
-}
-
 // What the kernels below have in common: the logits, and how their rows are cut.
 struct Rows {
   const void* x;
   long long ld;
   int n, rows, parts, per;  // per: vectors of a part
+  int cluster;              // the parts of a row are the CTAs of a cluster, which meet; else they have nothing to do with each other
   float c, temperature;     // c = log2(e) / temperature
   int* status;
-  float* scratch;           // records of the parts: maximum, s, w, -, then the best values and their indices
-  unsigned* tickets;        // a counter per row
 };
-// Floats of a part's record.
-__host__ __device__ constexpr int record_floats(int top) { return 4 + (2 * top + 3) / 4 * 4; }
+// The (row, part) of an item.
+__device__ __forceinline__ long long row_of(const Rows& p, long long item) { return p.cluster ? item : item / p.parts; }
+__device__ __forceinline__ int part_of(const Rows& p, long long item) {
+  return p.cluster ? (int)cluster_ctarank() : (int)(item - item / p.parts * p.parts);
+}
+template <typename T>
+__device__ __forceinline__ Range<T> range_of(const Rows& p, long long item) {
+  constexpr int V = 16 / (int)sizeof(T);
+  Range<T> r;
+  r.src = static_cast<const T*>(p.x) + row_of(p, item) * p.ld;
+  r.off = (int)(((uintptr_t)r.src & 15) / sizeof(T));
+  r.n = p.n;
+  const int nvec = (r.off + p.n + V - 1) / V;
+  r.v0 = (int)min((long long)nvec, (long long)part_of(p, item) * p.per);
+  r.v1 = min(nvec, r.v0 + p.per);
+  return r;
+}
+
+// ------------------------------------------------------------------ rows through a CTA
+// A CTA takes row after row, or parts of rows, with two roles:
+//   stream   eight warps read the row, four vectors of 16 bytes per thread at a time; five CTAs on an SM keep HBM busy while one of them
+//            computes or ends a row (a ring of bulk copies ahead of the warps was no faster: what it saved in waiting it took in
+//            instructions, 10.7 per element instead of 7.4, for its barriers)
+//   clerk    a warp prepares the next row: whether it is padding, what the operator needs besides its logits (loads that
+//            depend on loads, f64 exponentials), so that a row ends with one barrier and a handful of operations
+// The row's first and last elements, up to a vector boundary, are loaded one by one.
+//
+// Where a row is cut into parts whose sums have to meet, the parts are the CTAs of a cluster: they send their sums to each other's
+// shared memory.  Few rows are spread over the GPU that way.
+constexpr int kMaxCluster = 16;
+
+// Whole vectors of a range, [a, b), and the elements before and behind them.
+struct Inner {
+  int a, b, head, tail;
+  template <typename T>
+  __device__ __forceinline__ explicit Inner(const Range<T>& r) {
+    constexpr int V = Range<T>::V;
+    const int nvec = (r.off + r.n + V - 1) / V;
+    a = r.v0;
+    head = 0;
+    if (r.off > 0 && r.v0 == 0 && r.v1 > 0) {
+      a = 1;
+      head = min(r.n, V - r.off);
+    }
+    b = r.v1;
+    if (r.v1 == nvec && nvec * V - r.off > r.n) --b;
+    b = max(a, b);
+    tail = r.v1 == nvec && r.v1 > r.v0 ? r.n - (b * V - r.off) : 0;
+    if (tail < 0) tail = 0;  // all of the row lies before its first vector boundary
+  }
+};
+// The element that thread tid < 16 holds: of the head (tid < 8) or the tail, or -1.
+template <typename T>
+__device__ __forceinline__ int edge_index(const Range<T>& r, const Inner& in, int tid) {
+  if (tid < in.head) return tid;
+  if (tid >= 8 && tid - 8 < in.tail) return r.n - in.tail + tid - 8;
+  return -1;
+}
+
+// A streaming thread's vectors of the tile at v; beyond the range -inf.  KEEP: the row is read again, from L2.
+template <typename T, bool KEEP = false>
+__device__ __forceinline__ void load_tile(uint4 (&q)[kUnroll], const Range<T>& r, const Inner& in, int v) {
+  const int tid = threadIdx.x;
+  const uint4* p = r.at(v) + tid;
+  if (v + kTile <= in.b) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kThreads) : __ldcs(p + u * kThreads);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) q[u] = v + tid + u * kThreads < in.b ? (KEEP ? __ldcg(p + u * kThreads) : __ldcs(p + u * kThreads)) : empty_row_vec<T>();
+  }
+}
+
+// Sums of a row's parts in the shared memory of every CTA of the cluster, for even and odd meetings.  A peer sends to the meeting after
+// the next one only when this CTA has sent to the next, that is, has read this one.
+struct Meeting {
+  float4 part[2][kMaxCluster];
+  uint64_t bar[2];
+  volatile int abort;  // a wait ran out: no further message or wait
+};
+
+// The frame of the kernels below.  Op has
+//   Lesson                     what the clerk prepares; .at is the item, -1 behind the last one; .zero: its gradient is 0 and its logits are not read
+//   prepare(lesson, item)      the clerk: false for padding whose results it has written
+//   before(turn, lessons), after(turn, lessons)             the clerk, before and after a lesson is made
+//   stream(turn, lesson, range, inner)                      the streaming threads, up to the row's barrier
+//   finish(turn, lesson, range, inner)                      the streaming threads behind it
+template <typename T, typename Op>
+__device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Lesson* lessons, Meeting* meeting) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool cluster = p.cluster && p.parts > 1;
+  if (cluster) {
+    if (tid == 0) {
+      for (int i = 0; i < 2; ++i) mbar_init(&meeting->bar[i], 1);
+      meeting->abort = 0;
+      fence_mbar_init();
+    }
+    __syncthreads();
+    cluster_arrive();  // the peers' shared memory and barriers exist
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  grid_dependency_sync();
+  const long long items = p.cluster ? p.rows : (long long)p.rows * p.parts;
+  if (warp == kWarps) {
+    const int step = p.cluster ? gridDim.x / p.parts : gridDim.x;
+    long long at = (long long)(p.cluster ? blockIdx.x / p.parts : blockIdx.x) - step;
+    for (int turn = -1;; ++turn) {  // while row `turn` streams, the next one is prepared
+      if (turn >= 0 && lessons[turn % 3].at < 0) break;
+      typename Op::Lesson& l = lessons[(turn + 1) % 3];
+      op.before(turn + 1, lessons);
+      __syncwarp();
+      if (lane == 0) l.zero = false;
+      do at += step;
+      while (at < items && !op.prepare(l, at));
+      if (lane == 0) l.at = at < items ? at : -1;
+      __syncwarp();
+      op.after(turn + 1, lessons);
+      __syncwarp();
+      bar_row();
+    }
+  } else {
+    bar_row();
+    for (int turn = 0;; ++turn) {
+      const typename Op::Lesson& l = lessons[turn % 3];
+      if (l.at < 0) break;
+      const Range<T> r = range_of<T>(p, l.at);
+      const Inner in(r);
+      op.stream(turn, l, r, in);
+      bar_row();
+      op.finish(turn, l, r, in);
+    }
+  }
+  if (cluster) {  // no peer sends any more, and what they have sent is there unless a wait ran out
+    __syncthreads();
+    cluster_arrive_relaxed();
+    cluster_wait();
+    let_copies_land(&meeting->abort);
+  }
+}
+
+// Sends (maximum, s, w) of this CTA's part to its row's CTAs; warp 0.  extra: bytes that come besides.
+__device__ __forceinline__ void send_part(const Rows& p, Meeting& m, int turn, float3 mine, uint32_t extra) {
+  const int lane = threadIdx.x & 31;
+  if (m.abort) return;
+  __syncwarp();
+  if (lane == 0) mbar_expect_tx(&m.bar[turn & 1], p.parts * (uint32_t)sizeof(float4) + extra);
+  if (lane < p.parts) send4_to_cta(&m.part[turn & 1][cluster_ctarank()], make_float4(mine.x, mine.y, mine.z, 0.f), &m.bar[turn & 1], lane);
+}
+// Waits for all parts; a warp.
+__device__ __forceinline__ void await_parts(const Rows& p, Meeting& m, int turn) {
+  if (m.abort) return;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) (void)mbar_wait<true>(&m.bar[turn & 1], (turn >> 1) & 1, p.status, DEV_TIMEOUT_TMA, &m.abort);
+  __syncwarp();
+  (void)mbar_try_wait<true>(&m.bar[turn & 1], (turn >> 1) & 1);  // every lane acquires what the peers sent
+}
+// (maximum, s, w) of all parts, in all lanes of a warp.
+__device__ __forceinline__ float3 join_parts(const Rows& p, const Meeting& m, int turn) {
+  const int i = threadIdx.x & (kMaxCluster - 1);
+  const float4 one = i < p.parts ? m.part[turn & 1][i] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  float most = one.x;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  most = fmaxf(most, -FLT_MAX);
+  const float2 sum = join<kMaxCluster>((one.x - most) * p.c, one.y, one.z);
+  return make_float3(most, sum.x, sum.y);
+}
 
 // ------------------------------------------------------------------ log probabilities, forward
 struct Logprobs : Rows {
@@ -407,95 +642,118 @@ struct Logprobs : Rows {
   float *logprobs, *entropy, *lse, *top_logprobs;
   int* top_ids;
 };
+struct LogprobsLesson {
+  long long at, token;
+  float x;  // the token's logit
+  bool zero;
+};
+struct Lists {  // of the parts, in the first CTA of a row
+  float2 entry[2][kMaxCluster * kMaxTop];
+};
 
-// A CTA takes (row, part) after (row, part).  Rows are cut into parts where there are fewer rows than room for CTAs; the CTA that
-// finishes a row's last part puts the parts together.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? kTopPerSm : kPlainPerSm) logprobs_kernel(const __grid_constant__ Logprobs p) {
-  __shared__ float red[2][3][kWarps];
-  __shared__ int last;
-  __shared__ typename std::conditional<TOP, Best, int>::type best_store;
-  Best& best = reinterpret_cast<Best&>(best_store);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_dependency_sync();
-  const long long items = (long long)p.rows * p.parts;
-  auto token_of = [&](long long at) { return at < items && p.tokens ? load_id(p.tokens, at / p.parts, p.token_bits) : -1ll; };
-  long long next_token = token_of(blockIdx.x);
-  int turn = 0;
-  for (long long at = blockIdx.x; at < items; at += gridDim.x) {
-    const long long row = at / p.parts, token = next_token;
-    const int part = (int)(at - row * p.parts);
-    next_token = token_of(at + gridDim.x);
-    if (token == 0) {
-      if (part == 0) {
-        if (tid == 0) {
-          if (p.logprobs) p.logprobs[row] = 0.f;
-          if (p.entropy) p.entropy[row] = 0.f;
-          if (p.lse) p.lse[row] = 0.f;
-        }
-        if (TOP && tid < p.top) {
-          p.top_logprobs[row * p.top + tid] = 0.f;
-          p.top_ids[row * p.top + tid] = 0;
-        }
+struct LogprobsOp {
+  using Lesson = LogprobsLesson;
+  const Logprobs& p;
+  Best& best;
+  Lists& lists;
+  float (&red)[2][3][kWarps];
+  Meeting& meeting;
+  float theta;
+
+  __device__ __forceinline__ void before(int, const Lesson*) {}
+  __device__ __forceinline__ void after(int, const Lesson*) {}
+  __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
+    const int lane = threadIdx.x & 31;
+    const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
+    if (token != 0) {
+      if (lane == 0) {
+        l.token = token;
+        l.x = token > 0 && token <= p.n ? to_float((static_cast<const T*>(p.x) + row * p.ld)[token - 1]) : 0.f;
       }
-      continue;
+      return true;
     }
-    const Range<T> r = range_of<T>(p.x, p.ld, p.n, row, part, p.per);
-    Sums<T, true> sums;
-    float theta = -INFINITY;
+    if (p.parts == 1 || cluster_ctarank() == 0) {
+      if (lane == 0) {
+        if (p.logprobs) p.logprobs[row] = 0.f;
+        if (p.entropy) p.entropy[row] = 0.f;
+        if (p.lse) p.lse[row] = 0.f;
+      }
+      if (TOP && lane < p.top) {
+        p.top_logprobs[row * p.top + lane] = 0.f;
+        p.top_ids[row * p.top + lane] = 0;
+      }
+    }
+    return false;
+  }
+
+  __device__ __forceinline__ void list(float x, int index) {
+    if (x > theta) {
+      const int pos = atomicAdd(&best.count, 1);
+      if (pos < kCand) {
+        best.value[pos] = x;
+        best.index[pos] = index;
+      }
+    }
+  }
+  __device__ __forceinline__ void stream(int turn, const Lesson&, const Range<T>& r, const Inner& in) {
+    constexpr int V = Range<T>::V;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, edge = edge_index(r, in, tid);
+    const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
+    Sums<T> sums;
     if constexpr (TOP) {
       if (tid == 0) best.count = 0;  // ahead of the barriers of the first threshold
+      theta = -INFINITY;
+      if (edge >= 0 && tid < 8) sums.add_one(x, p.c);
     }
     int tile = 0;
 #pragma unroll 1
-    for (int v = r.v0; v < r.v1 || tile == 0; v += kTile, ++tile) {
+    for (int v = in.a; v < in.b || (TOP && tile == 0); v += kTile, ++tile) {
       uint4 q[kUnroll];
-      load_tile(q, r, v, false);
-      const float most = sums.add(q, p.c);
+      float most = -INFINITY;
+      if (v < in.b) {
+        load_tile(q, r, in, v);
+        most = sums.add(q, p.c);
+      }
       if constexpr (TOP) {
-        if (tile == 0) theta = group_threshold(word_max<T>(sums.top), p.top, best);
+        if (tile == 0) {
+          theta = group_threshold(word_max<T>(sums.top), p.top, best);
+          if (edge >= 0 && tid < 8) list(x, edge);
+        }
         if (most > theta) {
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) {
-            constexpr int V = 16 / (int)sizeof(T);
             float f[V];
             unpack_row<T>(q[u], f);
             const int e0 = (v + u * kThreads + tid) * V - r.off;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (f[i] > theta) {
-                const int pos = atomicAdd(&best.count, 1);
-                if (pos < kCand) {
-                  best.value[pos] = f[i];
-                  best.index[pos] = e0 + i;
-                }
-              }
+            for (int i = 0; i < V; ++i) list(f[i], e0 + i);
           }
         }
-        if (tile > 0 && (tile & (tile + 1)) == 0 && v + kTile < r.v1) theta = group_threshold(word_max<T>(sums.top), p.top, best);
+        if (tile > 0 && (tile & (tile + 1)) == 0 && v + kTile < in.b) theta = group_threshold(word_max<T>(sums.top), p.top, best);
       }
     }
-
-    float(&mine)[3][kWarps] = red[turn++ & 1];
-    {
-      const float3 of_warp = sums.over_warp(p.c);
-      if (lane == 0) {
-        mine[0][warp] = of_warp.x;
-        mine[1][warp] = of_warp.y;
-        mine[2][warp] = of_warp.z;
-      }
+    if (edge >= 0 && (!TOP || tid >= 8)) {
+      sums.add_one(x, p.c);
+      if constexpr (TOP) list(x, edge);
     }
-    __syncthreads();
-    float top_max = red_max(mine[0]);
-    const bool plain = Sums<T, true>::plain(top_max, p.c);
-    if (!plain) {
-      top_max = fmaxf(top_max, -FLT_MAX);
-      const float2 of_warp = slow_sums(r, nullptr, top_max, p.c);
-      if (lane == 0) {
-        mine[1][warp] = of_warp.x;
-        mine[2][warp] = of_warp.y;
-      }
-      __syncthreads();
+    const float3 of_warp = sums.over_warp(p.c);
+    if (lane == 0) {
+      red[turn & 1][0][warp] = of_warp.x;
+      red[turn & 1][1][warp] = of_warp.y;
+      red[turn & 1][2][warp] = of_warp.z;
+    }
+  }
+  __device__ __forceinline__ void finish(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float(&mine)[3][kWarps] = red[turn & 1];
+    const long long row = l.at;
+    float3 sum = make_float3(red_max(mine[0]), 0.f, 0.f);
+    if (!Sums<T>::plain(sum.x)) {
+      sum = slow_sums(r, nullptr, 0, p.c, mine);
+    } else if (warp == 0) {
+      const float2 s = join<kWarps>((mine[0][lane & 7] - sum.x) * p.c, mine[1][lane & 7], mine[2][lane & 7]);
+      sum = make_float3(sum.x, s.x, s.y);
     }
     if constexpr (TOP) {
       int n = best.count;
@@ -504,154 +762,140 @@ __global__ void __launch_bounds__(kThreads, TOP ? kTopPerSm : kPlainPerSm) logpr
       } else if (n < p.top) {
         // theta of the first tile: with fewer than k above it, it is also the last one
         Range<T> first = r;
-        first.v1 = min(r.v1, r.v0 + kTile);
+        first.v1 = min(r.v1, in.a + kTile);
         n = append_equal(first, theta, n, p.top - n, best);
       }
       select_list(n, p.top, best);
     }
-    float2 sum = make_float2(0.f, 0.f);
-    if (warp == 0) {
-      const int w = lane & 7;
-      sum = join(plain ? mine[0][w] : top_max, mine[1][w], mine[2][w], top_max, p.c);
-    }
-
-    bool finish = true;
     if (p.parts > 1) {
-      const int stride = record_floats(p.top);
-      float* record = p.scratch + at * stride;
-      if (tid == 0) *reinterpret_cast<float4*>(record) = make_float4(top_max, sum.x, sum.y, 0.f);
+      const int rank = cluster_ctarank();
+      if (warp == 0) {
+        send_part(p, meeting, turn, sum, TOP && rank == 0 ? p.parts * p.top * (uint32_t)sizeof(float2) : 0);
+        if (TOP && lane < p.top && !meeting.abort)
+          send_to_cta(&lists.entry[turn & 1][rank * p.top + lane], best.out_value[lane], __int_as_float(best.out_index[lane]),
+                      &meeting.bar[turn & 1], 0);
+      }
+      if (warp == 0 || (TOP && rank == 0)) {
+        await_parts(p, meeting, turn);
+        sum = join_parts(p, meeting, turn);
+      }
+      if (rank != 0) return;
       if constexpr (TOP) {
-        if (tid < p.top) {
-          const int id = best.out_index[tid];
-          record[4 + tid] = id >= 0 ? best.out_value[tid] : -INFINITY;
-          reinterpret_cast<int*>(record)[4 + p.top + tid] = id;
-        }
-      }
-      if (warp == 0) {  // it alone has written
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) last = atomicInc(p.tickets + row, p.parts - 1) == (unsigned)p.parts - 1;
-      }
-      __syncthreads();
-      finish = last;
-      if (finish) {
-        __threadfence();
-        const float* all = p.scratch + row * p.parts * stride;
-        const float4 one = lane < p.parts ? __ldcg(reinterpret_cast<const float4*>(all + (long long)lane * stride))
-                                          : make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
-        top_max = warp_max(one.x);
-        sum = join_parts(one, top_max, p.c);
-        if constexpr (TOP) {
-          if (tid == 0) best.count = 0;
-          __syncthreads();
-          for (int i = tid; i < p.parts * p.top; i += kThreads) {
-            const float* rec = all + (long long)(i / p.top) * stride + 4 + i % p.top;
-            const int id = __ldcg(reinterpret_cast<const int*>(rec) + p.top);
-            if (id >= 0) {
-              const int pos = atomicAdd(&best.count, 1);
-              best.value[pos] = __ldcg(rec);
-              best.index[pos] = id;
-            }
+        if (tid == 0) best.count = 0;
+        bar_stream();
+        for (int i = tid; i < p.parts * p.top; i += kThreads) {
+          const float2 e = lists.entry[turn & 1][i];
+          const int id = __float_as_int(e.y);
+          if (id >= 0) {
+            const int pos = atomicAdd(&best.count, 1);
+            best.value[pos] = e.x;
+            best.index[pos] = id;
           }
-          __syncthreads();
-          select_list(best.count, p.top, best);
         }
+        bar_stream();
+        select_list(best.count, p.top, best);
       }
-      __syncthreads();  // `last` has been read
     }
-
-    if (finish && warp == 0) {
-      const float log_sum = logf(sum.x);
+    if (warp == 0) {
+      const float log_sum = logf(sum.y);
       if (lane == 0) {
-        if (p.lse) p.lse[row] = top_max / p.temperature + log_sum;
-        if (p.entropy) p.entropy[row] = log_sum - kLn2 * (sum.y / sum.x);
+        if (p.lse) p.lse[row] = sum.x / p.temperature + log_sum;
+        if (p.entropy) p.entropy[row] = log_sum - kLn2 * (sum.z / sum.y);
         if (p.logprobs) {
-          float lp = NAN;
-          if (token < 0 || token > p.n) atomicMax(p.status, DEV_BAD_INDEX);
-          else lp = (to_float(r.src[token - 1]) - top_max) / p.temperature - log_sum;
-          p.logprobs[row] = lp;
+          const bool bad = l.token < 0 || l.token > p.n;
+          if (bad) atomicMax(p.status, DEV_BAD_INDEX);
+          p.logprobs[row] = bad ? NAN : (l.x - sum.x) / p.temperature - log_sum;
         }
       }
-      if constexpr (TOP) {
-        if (lane < p.top) {
-          const int id = best.out_index[lane];
-          p.top_logprobs[row * p.top + lane] = id >= 0 ? (best.out_value[lane] - top_max) / p.temperature - log_sum : NAN;
-          p.top_ids[row * p.top + lane] = id + 1;
-        }
+      if (TOP && lane < p.top) {
+        const int id = best.out_index[lane];
+        p.top_logprobs[row * p.top + lane] = id >= 0 ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
+        p.top_ids[row * p.top + lane] = id + 1;
       }
     }
   }
+};
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kAllThreads, kLogprobsPerSm<TOP>) logprobs_kernel(const __grid_constant__ Logprobs p) {
+  __shared__ Meeting meeting;
+  __shared__ LogprobsLesson lessons[3];
+  __shared__ float red[2][3][kWarps];
+  __shared__ typename std::conditional<TOP, Best, int>::type best;
+  __shared__ typename std::conditional<TOP, Lists, int>::type lists;
+  LogprobsOp<T, TOP> op{p, reinterpret_cast<Best&>(best), reinterpret_cast<Lists&>(lists), red, meeting, 0.f};
+  run_rows<T>(p, op, lessons, &meeting);
 }
 
 // ------------------------------------------------------------------ gradients
-// d = p (a + b t), t = log2 p, over vectors of a row; KEPT: they are in L2.
+// d = p (a + b t), t = log2 p, over a range.
 template <typename T, bool ENTROPY>
-__device__ __forceinline__ void stream_gradient(const Range<T>& r, T* dst, float c, float lse2, float a, float b) {
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void stream_gradient(const Range<T>& r, const Inner& in, T* dst, float c, float lse2, float a, float b) {
+  const int tid = threadIdx.x, edge = edge_index(r, in, tid);
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
-  const float2 cc = make_float2(c, c), minus = make_float2(-lse2, -lse2), aa = make_float2(a, a), bb = make_float2(b, b);
+  const Pair cc = pair(c, c), minus = pair(-lse2, -lse2), aa = pair(a, a), bb = pair(b, b);
+  const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
 #pragma unroll 1
-  for (int v = r.v0; v < r.v1; v += kTile) {
+  for (int v = in.a; v < in.b; v += kTile) {
     uint4 q[kUnroll];
-    load_tile(q, r, v, false);
+    load_tile(q, r, in, v);
+    uint4* to = reinterpret_cast<uint4*>(dst - r.off) + v + tid;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
       for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
-        float2 t = fma_pair(vec_pair<T>(word, i), cc, minus);
-        float2 e = make_float2(ex2_approx_ftz(t.x), ex2_approx_ftz(t.y));
+        const Pair t = fma2(vec_pair<T>(word, i), cc, minus), e = exp2_pair(t);
         if constexpr (ENTROPY) {
-          t = make_float2(fmaxf(t.x, kLowest), fmaxf(t.y, kLowest));
-          e = mul_pair(e, fma_pair(bb, t, aa));
+          const float2 h = halves(t);
+          put_pair<T>(word, i, mul2(e, fma2(bb, pair(fmaxf(h.x, kLowest), fmaxf(h.y, kLowest)), aa)));
         } else {
-          e = mul_pair(e, aa);
+          put_pair<T>(word, i, mul2(e, aa));
         }
-        put_pair<T>(word, i, e);
       }
-      q[u] = make_uint4(word[0], word[1], word[2], word[3]);
-    }
-    if (aligned && r.inside(v, kTile)) {
-      uint4* to = reinterpret_cast<uint4*>(dst - r.off) + v + tid;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) __stcs(to + u * kThreads, q[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int at = v + u * kThreads + tid;
-        if (at >= r.v1) continue;
-        if (aligned && r.inside(at, 1)) __stcs(reinterpret_cast<uint4*>(dst - r.off) + at, q[u]);
-        else store_edge<T>(dst, r.off, r.n, at, q[u]);
+      const uint4 d = make_uint4(word[0], word[1], word[2], word[3]);
+      if (v + u * kThreads + tid < in.b) {
+        if (aligned) __stcs(to + u * kThreads, d);
+        else store_edge<T>(dst, r.off, r.n, v + u * kThreads + tid, d);
       }
     }
   }
+  if (edge >= 0) {
+    const float t = fmaf(x, c, -lse2), e = ex2_approx_ftz(t);
+    dst[edge] = from_float<T>(ENTROPY ? e * fmaf(b, fmaxf(t, kLowest), a) : e * a);
+  }
 }
-// Zeros over vectors of a row, by `threads` threads of which this is the i-th.
+// Zeros over a range, by the streaming threads.
 template <typename T>
-__device__ __noinline__ void stream_zeros(const Range<T>& r, T* dst, int i, int threads) {
+__device__ __noinline__ void stream_zeros(const Range<T>& r, T* dst) {
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int v = r.v0 + i; v < r.v1; v += threads) {
+  for (int v = r.v0 + threadIdx.x; v < r.v1; v += kThreads) {
     if (aligned && r.inside(v, 1)) __stcs(reinterpret_cast<uint4*>(dst - r.off) + v, zero);
     else store_edge<T>(dst, r.off, r.n, v, zero);
   }
 }
 
-// Gradient at what a teacher lists: g (all p - sum of the q of this id), once per id.  Thread j has entry j and its logit x.
+// Id of an entry if it lies in this range, else 0.
 template <typename T>
-__device__ __forceinline__ void patch_entries(T* dst, const int* entry, const float* q, int entries, float x, float c, float lse2, float g,
-                                              float all, long long lo, long long hi) {
+__device__ __forceinline__ int in_range(const Range<T>& r, long long id) {
+  const long long v = (id - 1 + r.off) / Range<T>::V;
+  return id > 0 && v >= r.v0 && v < r.v1 ? (int)id : 0;
+}
+// Gradient at what a teacher lists: g (all p - sum of the q of this id), once per id.  Thread j has entry j; 0: unused or in another part.
+template <typename T>
+__device__ __forceinline__ void patch_entries(const Range<T>& r, T* dst, const int* entry, const float* q, const float* x, int entries, float c,
+                                              float lse2, float g, float all) {
   const int j = threadIdx.x;
   if (j >= entries) return;
   const int id = entry[j];
-  if (id <= lo || id > hi) return;
+  if (!in_range(r, id)) return;
   float sum = 0.f;
   for (int i = 0; i < entries; ++i)
     if (entry[i] == id) {
       if (i < j) return;
       sum += q[i];
     }
-  dst[id - 1] = from_float<T>(g * (all * ex2_approx_ftz(fmaf(x, c, -lse2)) - sum));
+  dst[id - 1] = from_float<T>(g * (all * ex2_approx_ftz(fmaf(x[j], c, -lse2)) - sum));
 }
 
 // ------------------------------------------------------------------ distillation, forward, and the gradient at once
@@ -680,226 +924,196 @@ __device__ __forceinline__ double max_lanes(double v) {
 }
 
 // The teacher's side of a row, in f64: what its list leaves over is a difference from one.
-struct Lesson {
-  long long at;              // row * parts + part; -1: no more
+struct DistillLesson {
+  long long at;
   double terms, all, norm;   // sum q (log q - z), sum q
   float listed_max, listed;  // what the student gives to the listed ids, each once: maximum, sum of powers relative to it
+  float g;                   // upstream gradient / temperature
+  bool zero;
   int entry[kMaxEntries];    // ids, 0: unused
   float q[kMaxEntries], x[kMaxEntries];
 };
 
-__device__ __forceinline__ void bar_stream() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // the streaming warps alone
-static_assert(kThreads == 256, "bar_stream names the number of threads");
-
-// Eight warps stream rows; a ninth one prepares the teacher's side of the next row meanwhile (loads that depend on loads, f64
-// exponentials), so that a row ends with one barrier and a handful of operations.  HOLES: teacher_lse is given; what the teacher lists is left out of
-// the row's sum by a bit per element and added apart, since the rest's probability from a difference would lose all digits where it
-// is small.  GRAD: the same CTA reads the row again, from L2, and writes the gradient.
+// HOLES: teacher_lse is given; what the teacher lists is left out of the row's sum by a bit per element and added apart, since the rest's
+// probability from a difference would lose all digits where it is small.  GRAD: the row is read a second time, out of L2, for the
+// gradient.
 template <typename T, bool GRAD, bool HOLES>
-__global__ void __launch_bounds__(kThreads + 32, kDistillPerSm) distill_kernel(const __grid_constant__ Distill p) {
-  constexpr int V = 16 / (int)sizeof(T);
-  extern __shared__ __align__(16) unsigned hole_store[];  // HOLES: two sets of bits
-  __shared__ Lesson lessons[3];
-  __shared__ double power[kMaxEntries];  // the ninth warp's
-  __shared__ float red[2][3][kWarps];
-  __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hole_words = HOLES ? (p.per * V + 31) / 32 : 0;
-  if constexpr (HOLES)
-    for (int i = tid; i < 2 * hole_words; i += kThreads + 32) hole_store[i] = 0;
-  grid_dependency_sync();
-  const long long items = (long long)p.rows * p.parts;
-  long long at = (long long)blockIdx.x - gridDim.x;
+struct DistillOp {
+  using Lesson = DistillLesson;
+  static constexpr int V = Range<T>::V;
+  const Distill& p;
+  double (&power)[kMaxEntries];  // the clerk's
+  float (&red)[2][3][kWarps];
+  unsigned* holes;  // two sets of hole_words
+  int hole_words;
+  Meeting& meeting;
+  int meetings;
 
-  // Ninth warp: the next row that is not padding, or -1; results of padding rows are written on the way.
-  auto prepare = [&](Lesson& l) {
-    for (;;) {
-      at += gridDim.x;
-      if (at >= items) {
-        if (lane == 0) l.at = -1;
-        return;
-      }
-      const long long row = at / p.parts;
-      const int part = (int)(at - row * p.parts);
-      const T* src = static_cast<const T*>(p.x) + row * p.ld;
-      bool used = false, bad = false;
-      double most = -INFINITY;
-      for (int j = lane; j < p.entries; j += 32) {
-        const long long id = load_id(p.ids, row * p.entries + j, p.id_bits);
-        const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
-        const bool out = id < 0 || id > p.n;
-        bad |= out;
-        used |= id != 0;
-        l.entry[j] = out ? 0 : (int)id;
-        power[j] = u;
-        if (id) most = fmax(most, u);
-      }
-      used = __any_sync(0xffffffffu, used);
-      bad = __any_sync(0xffffffffu, bad);
-      if (!used || bad) {
-        if (part == 0) {
-          if (lane == 0) {
-            if (bad) atomicMax(p.status, DEV_BAD_INDEX);
-            p.loss[row] = bad ? NAN : 0.f;
-            reinterpret_cast<float4*>(p.saved)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-          if constexpr (GRAD)
-            stream_zeros<T>(range_of<T>(p.x, p.ld, p.n, row, 0, p.per), static_cast<T*>(p.dx) + row * p.ld_dx, lane, 32);
-        }
-        continue;
-      }
-      __syncwarp();
-      float x_most = -INFINITY;
-      for (int j = lane; j < p.entries; j += 32) {
-        const int id = l.entry[j];
-        const float x = id ? to_float(src[id - 1]) : -INFINITY;
-        l.x[j] = x;
-        x_most = fmaxf(x_most, x);
-      }
-      double sum = 1, norm;
-      if constexpr (HOLES) {
-        norm = p.teacher_lse[row];
-      } else {
-        most = max_lanes(most);
-        sum = 0;
-        for (int j = lane; j < p.entries; j += 32)
-          if (l.entry[j]) sum += exp(power[j] - most);
-        norm = most + log(sum_lanes(sum));
-      }
-      double all = 0, terms = 0;
-      for (int j = lane; j < p.entries; j += 32) {
-        if (l.entry[j] == 0) continue;
-        const double log_q = power[j] - norm, q = exp(log_q);
-        if (q != 0) terms += q * (log_q - (double)l.x[j] / (double)p.temperature);
-        all += q;
-        l.q[j] = (float)q;
-      }
-      all = sum_lanes(all);
-      terms = sum_lanes(terms);
-      float listed = 0.f;
-      if constexpr (HOLES) {
-        x_most = fmaxf(warp_max(x_most), -FLT_MAX);
-        for (int j = lane; j < p.entries; j += 32) {
-          const int id = l.entry[j];
-          bool again = id == 0;
-          for (int i = 0; i < j; ++i) again |= l.entry[i] == id;
-          if (!again) listed += ex2_approx_ftz((l.x[j] - x_most) * p.c);
-        }
-        listed = warp_sum(listed);
-      }
-      if (lane == 0) {
-        l.at = at;
-        l.terms = terms;
-        l.all = all;
-        l.norm = norm;
-        l.listed_max = x_most;
-        l.listed = listed;
-      }
-      return;
+  __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
+    const int lane = threadIdx.x & 31;
+    const T* src = static_cast<const T*>(p.x) + row * p.ld;
+    bool used = false, bad = false;
+    double most = -INFINITY;
+    for (int j = lane; j < p.entries; j += 32) {
+      const long long id = load_id(p.ids, row * p.entries + j, p.id_bits);
+      const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
+      const bool out = id < 0 || id > p.n;
+      bad |= out;
+      used |= id != 0;
+      l.entry[j] = out ? 0 : (int)id;
+      power[j] = u;
+      if (id) most = fmax(most, u);
     }
-  };
-  // Ninth warp: sets or clears the bits of a lesson's entries in its part.
-  auto punch = [&](const Lesson& l, unsigned* holes, bool set) {
-    if (l.at < 0) return;
-    const long long row = l.at / p.parts;
-    const Range<T> r = range_of<T>(p.x, p.ld, p.n, row, (int)(l.at - row * p.parts), p.per);
+    used = __any_sync(0xffffffffu, used);
+    bad = __any_sync(0xffffffffu, bad);
+    if (!used || bad) {
+      if ((p.parts == 1 || cluster_ctarank() == 0) && lane == 0) {
+        if (bad) atomicMax(p.status, DEV_BAD_INDEX);
+        p.loss[row] = bad ? NAN : 0.f;
+        reinterpret_cast<float4*>(p.saved)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (GRAD && lane == 0) l.zero = true;
+      return GRAD;
+    }
+    float x_most = -INFINITY;
     for (int j = lane; j < p.entries; j += 32) {
       const int id = l.entry[j];
-      const long long e = (long long)id - 1 + r.off - (long long)r.v0 * V;
-      if (id == 0 || e < 0 || e >= (long long)(r.v1 - r.v0) * V) continue;
-      if (set) atomicOr(holes + (e >> 5), 1u << (e & 31));
-      else holes[e >> 5] = 0;
+      const float x = id ? to_float(src[id - 1]) : -INFINITY;
+      l.x[j] = x;
+      x_most = fmaxf(x_most, x);
     }
-    __syncwarp();
-  };
-
-  if (warp == kWarps) {
-    prepare(lessons[0]);
-    __syncwarp();
-    if constexpr (HOLES) punch(lessons[0], hole_store, true);
-  }
-  __syncthreads();
-  for (int turn = 0;; ++turn) {
-    const Lesson& l = lessons[turn % 3];
-    if (l.at < 0) break;
-    const long long row = l.at / p.parts;
-    const int part = (int)(l.at - row * p.parts);
-    const Range<T> r = range_of<T>(p.x, p.ld, p.n, row, part, p.per);
-    const unsigned* holes = HOLES ? hole_store + (turn & 1) * hole_words : nullptr;
-    float(&mine)[3][kWarps] = red[turn & 1];
-    if (warp == kWarps) {
-      // The row before this one has been summed, and its bits lie where the next row's go.
-      unsigned* next_holes = hole_store + (~turn & 1) * hole_words;
-      if constexpr (HOLES)
-        if (turn > 0) punch(lessons[(turn + 2) % 3], next_holes, false);
-      prepare(lessons[(turn + 1) % 3]);
-      __syncwarp();
-      if constexpr (HOLES) punch(lessons[(turn + 1) % 3], next_holes, true);
-    } else {
-      Sums<T, false> sums;
-#pragma unroll 1
-      for (int v = r.v0; v < r.v1; v += kTile) {
-        uint4 q[kUnroll];
-        load_tile(q, r, v, GRAD);
-        if constexpr (HOLES)
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u) {
-            const int of = v - r.v0 + u * kThreads + tid;
-            const unsigned bits = of < r.v1 - r.v0 ? hole_bits<T>(holes, of) : 0u;
-            if (bits) mask_holes<T>(q[u], bits);
-          }
-        (void)sums.add(q, p.c);
-      }
-      const float3 of_warp = sums.over_warp(p.c);
-      if (lane == 0) {
-        mine[0][warp] = of_warp.x;
-        mine[1][warp] = of_warp.y;
-      }
-    }
-    __syncthreads();
-    if (warp == kWarps) continue;
-
-    float top_max = red_max(mine[0]);
-    const bool plain = Sums<T, false>::plain(top_max, p.c);
-    if (!plain) {
-      top_max = fmaxf(top_max, -FLT_MAX);
-      const float2 of_warp = slow_sums(r, holes, top_max, p.c);
-      if (lane == 0) mine[1][warp] = of_warp.x;
-      bar_stream();
-    }
-    float sum = join(plain ? mine[0][lane & 7] : top_max, mine[1][lane & 7], 0.f, top_max, p.c).x;
-    bool finish = true;
-    if (p.parts > 1) {
-      float* record = p.scratch + l.at * record_floats(0);
-      if (tid == 0) {
-        *reinterpret_cast<float4*>(record) = make_float4(top_max, sum, 0.f, 0.f);
-        __threadfence();
-        last = atomicInc(p.tickets + row, p.parts - 1) == (unsigned)p.parts - 1;
-      }
-      bar_stream();
-      finish = last;
-      if (finish) {
-        __threadfence();
-        const float4 one = lane < p.parts ? __ldcg(reinterpret_cast<const float4*>(p.scratch + (row * p.parts + lane) * record_floats(0)))
-                                          : make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
-        top_max = warp_max(one.x);
-        sum = join_parts(one, top_max, p.c).x;
-      }
-      bar_stream();  // `last` has been read
-    }
-    if (!finish) continue;
-    float total = sum, rest = sum, all = 1.f, outside = 1.f;
+    double norm;
     if constexpr (HOLES) {
-      const float both = fmaxf(top_max, l.listed_max);
-      rest = sum * ex2_approx_ftz((top_max - both) * p.c);
+      norm = p.teacher_lse[row];
+    } else {
+      most = max_lanes(most);
+      double sum = 0;
+      for (int j = lane; j < p.entries; j += 32)
+        if (l.entry[j]) sum += exp(power[j] - most);
+      norm = most + log(sum_lanes(sum));
+    }
+    double all = 0, terms = 0;
+    for (int j = lane; j < p.entries; j += 32) {
+      if (l.entry[j] == 0) continue;
+      const double log_q = power[j] - norm, q = exp(log_q);
+      if (q != 0) terms += q * (log_q - (double)l.x[j] / (double)p.temperature);
+      all += q;
+      l.q[j] = (float)q;
+    }
+    all = sum_lanes(all);
+    terms = sum_lanes(terms);
+    float listed = 0.f;
+    if constexpr (HOLES) {
+      __syncwarp();
+      x_most = fmaxf(warp_max(x_most), -FLT_MAX);
+      for (int j = lane; j < p.entries; j += 32) {
+        const int id = l.entry[j];
+        bool again = id == 0;
+        for (int i = 0; i < j; ++i) again |= l.entry[i] == id;
+        if (!again) listed += ex2_approx_ftz((l.x[j] - x_most) * p.c);
+      }
+      listed = warp_sum(listed);
+    }
+    if (lane == 0) {
+      l.terms = terms;
+      l.all = all;
+      l.norm = norm;
+      l.listed_max = x_most;
+      l.listed = listed;
+      if constexpr (GRAD) l.g = p.d_loss[row] / p.temperature;
+    }
+    return true;
+  }
+  // Sets or clears the bits of a lesson's entries in its part.
+  __device__ __forceinline__ void punch(const Lesson& l, unsigned* set, bool on) {
+    if (l.at < 0 || l.zero) return;
+    const Range<T> r = range_of<T>(p, l.at);
+    for (int j = threadIdx.x & 31; j < p.entries; j += 32) {
+      const int id = in_range(r, l.entry[j]);
+      if (id == 0) continue;
+      const long long e = (long long)id - 1 + r.off - (long long)r.v0 * V;
+      if (on) atomicOr(set + (e >> 5), 1u << (e & 31));
+      else set[e >> 5] = 0;
+    }
+    __syncwarp();
+  }
+  // The row two before has been summed: its bits lie where the next row's go.
+  __device__ __forceinline__ void before(int turn, const Lesson* lessons) {
+    if constexpr (HOLES)
+      if (turn >= 2) punch(lessons[(turn + 1) % 3], holes + (turn & 1) * hole_words, false);
+  }
+  __device__ __forceinline__ void after(int turn, const Lesson* lessons) {
+    if constexpr (HOLES) punch(lessons[turn % 3], holes + (turn & 1) * hole_words, true);
+  }
+
+  __device__ __forceinline__ void stream(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
+    if (GRAD && l.zero) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, edge = edge_index(r, in, tid);
+    const unsigned* mine = holes + (turn & 1) * hole_words;
+    float x = edge >= 0 ? to_float(r.src[edge]) : -INFINITY;
+    LeanSums<T> sums;
+#pragma unroll 1
+    for (int v = in.a; v < in.b; v += kTile) {
+      uint4 q[kUnroll];
+      load_tile<T, GRAD>(q, r, in, v);
+      if constexpr (HOLES)
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int of = v + u * kThreads + tid;
+          const unsigned bits = of < in.b ? hole_bits<T>(mine, of - r.v0) : 0u;
+          if (bits) mask_holes<T>(q[u], bits);
+        }
+      sums.add(q, p.c);
+    }
+    if (warp == 0 && in.head + in.tail > 0) {
+      if (HOLES && edge >= 0) {
+        const int e = edge + r.off - r.v0 * V;
+        if (mine[e >> 5] >> (e & 31) & 1) x = -INFINITY;
+      }
+      sums.add_one(x, p.c);
+    }
+    const float2 of_warp = sums.over_warp(p.c);
+    if (lane == 0) {
+      red[turn & 1][0][warp] = of_warp.x;
+      red[turn & 1][1][warp] = of_warp.y;
+    }
+  }
+  __device__ __forceinline__ void finish(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long row = l.at;
+    if (GRAD && l.zero) {
+      stream_zeros<T>(r, static_cast<T*>(p.dx) + row * p.ld_dx);
+      return;
+    }
+    float(&mine)[3][kWarps] = red[turn & 1];
+    float3 sum;
+    sum.x = red_max(mine[0]);
+    sum.y = join<kWarps>((mine[0][lane & 7] - sum.x) * p.c, mine[1][lane & 7], 0.f).x;
+    // A part of which nothing is left (all of it masked, or listed) counts as -inf, unless the row has no other.
+    const bool nothing = sum.x == -INFINITY && p.parts > 1;
+    if (!nothing && !(sum.y > 0.f && sum.y < INFINITY)) sum = slow_sums(r, l.entry, HOLES ? p.entries : 0, p.c, mine);
+    if (nothing) sum.y = 0.f;
+    if (p.parts > 1) {
+      const int meet = meetings++;
+      if (warp == 0) send_part(p, meeting, meet, make_float3(sum.x, sum.y, 0.f), 0);
+      if (GRAD || warp == 0) {
+        await_parts(p, meeting, meet);
+        sum = join_parts(p, meeting, meet);
+      }
+    }
+    if (!GRAD && warp != 0) return;
+    float total = sum.y, rest = sum.y, all = 1.f, outside = 1.f;
+    if constexpr (HOLES) {
+      const float both = fmaxf(sum.x, l.listed_max);
+      rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
       total = rest + l.listed * ex2_approx_ftz((l.listed_max - both) * p.c);
-      top_max = both;
+      sum.x = both;
       const double left = l.all > 1 ? 0 : 1 - l.all;
       all = (float)(l.all + left);
       outside = rest == 0.f ? all : (float)(l.all + left - left * ((double)total / (double)rest));
     }
-    if (tid == 0) {
-      const double log_total = log((double)total), lse = (double)top_max / (double)p.temperature + log_total;
+    if (tid == 0 && (p.parts == 1 || cluster_ctarank() == 0)) {
+      const double log_total = log((double)total), lse = (double)sum.x / (double)p.temperature + log_total;
       double loss = l.terms + l.all * lse;
       if constexpr (HOLES) {
         const double left = l.all > 1 ? 0 : 1 - l.all;
@@ -911,25 +1125,33 @@ __global__ void __launch_bounds__(kThreads + 32, kDistillPerSm) distill_kernel(c
       reinterpret_cast<float4*>(p.saved)[row] = HOLES ? make_float4((float)lse, outside, all, high)
                                                       : make_float4((float)lse, (float)(l.norm - (double)high), -1.f, high);
     }
-    if constexpr (GRAD) {  // one part
+    if constexpr (GRAD) {
       T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
-      const float g = p.d_loss[row] / p.temperature;
-      const float lse2 = fmaf(top_max, p.c, log2f(total));
-      stream_gradient<T, false>(r, dst, p.c, lse2, g * outside, 0.f);
+      int k;  // the logarithm's whole part joins the reference before it is rounded
+      const float m = frexpf(total, &k), lse2 = fmaf(sum.x, p.c, (float)k) + log2f(m);
+      stream_gradient<T, false>(r, in, dst, p.c, lse2, l.g * outside, 0.f);
       bar_stream();
-      patch_entries<T>(dst, l.entry, l.q, p.entries, tid < p.entries ? l.x[tid] : 0.f, p.c, lse2, g, all, 0, p.n);
+      patch_entries<T>(r, dst, l.entry, l.q, l.x, p.entries, p.c, lse2, l.g, all);
     }
   }
+};
+template <typename T, bool GRAD, bool HOLES>
+__global__ void __launch_bounds__(kAllThreads, kDistillPerSm) distill_kernel(const __grid_constant__ Distill p) {
+  __shared__ Meeting meeting;
+  __shared__ DistillLesson lessons[3];
+  __shared__ double power[kMaxEntries];
+  __shared__ float red[2][3][kWarps];
+  extern __shared__ unsigned holes[];  // two sets
+  const int hole_words = HOLES ? (p.per * Range<T>::V + 31) / 32 : 0;
+  for (int i = threadIdx.x; i < 2 * hole_words; i += kAllThreads) holes[i] = 0;
+  DistillOp<T, GRAD, HOLES> op{p, power, red, holes, hole_words, meeting, 0};
+  run_rows<T>(p, op, lessons, &meeting);
 }
 
 // ------------------------------------------------------------------ backward
-struct Backward {
-  const void* x;
+struct Backward : Rows {
   void* dx;
-  long long ld, ld_dx;
-  int n, rows, parts, per;
-  float c, temperature;
-  int* status;
+  long long ld_dx;
   // log probabilities
   const void* tokens;
   int token_bits, top;
@@ -943,95 +1165,111 @@ struct Backward {
   const float *saved, *d_loss;
 };
 
+// A row's gradient is p (a + b log2 p) but where an entry (an alternative, the token, what the teacher lists) meets it.
+template <int ENTRIES>
+struct BackwardLesson {
+  long long at;
+  float lse2, a, b, all, g;
+  int entries;
+  bool zero;
+  int entry[ENTRIES];
+  float weight[ENTRIES], x[ENTRIES];
+};
+
 // Gradient of the log probabilities, the entropy and the alternatives of a row:
 //   dx_v = 1/temperature [ sum of the gradients that meet at v - p_v (G + g_H (log p_v + H)) ],  G = the sum of all but g_H
 // and of the distillation loss (DISTILL): g/temperature p_v outside, or g/temperature (all p_v - q_v) where the teacher lists v.
-// A CTA takes part after part; the few places that a gradient meets directly are written behind the part's stream.
-template <typename T, bool DISTILL>
-__global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kernel(const __grid_constant__ Backward p) {
-  constexpr int V = 16 / (int)sizeof(T);
-  __shared__ int entry[kMaxEntries];
-  __shared__ float weight[kMaxEntries];
-  const int tid = threadIdx.x, lane = tid & 31;
-  grid_dependency_sync();
-  const long long items = (long long)p.rows * p.parts;
-  for (long long at = blockIdx.x; at < items; at += gridDim.x) {
-    const long long row = at / p.parts;
-    const Range<T> r = range_of<T>(p.x, p.ld, p.n, row, (int)(at - row * p.parts), p.per);
-    T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
-    const long long lo = max(0ll, (long long)r.v0 * V - r.off), hi = min((long long)p.n, (long long)r.v1 * V - r.off);  // ids (lo, hi] lie in this part
+template <typename T, bool DISTILL, bool ENTROPY>
+struct BackwardOp {
+  using Lesson = BackwardLesson<DISTILL ? kMaxEntries : kMaxTop + 1>;
+  const Backward& p;
+
+  __device__ __forceinline__ void before(int, const Lesson*) {}
+  __device__ __forceinline__ void after(int, const Lesson*) {}
+  // dx may be the logits themselves: the entries' logits are read before their row is streamed.
+  __device__ __forceinline__ void enter(Lesson& l, int j, long long id, float weight, const Range<T>& r) {
+    if (id < 0 || id > p.n) {
+      atomicMax(p.status, DEV_BAD_INDEX);
+      id = 0;
+    }
+    const int mine = in_range(r, id);
+    l.entry[j] = mine;
+    l.weight[j] = weight;
+    l.x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
+  }
+  __device__ __forceinline__ bool prepare(Lesson& l, long long item) {
+    const int lane = threadIdx.x & 31;
+    const long long row = row_of(p, item);
+    const Range<T> r = range_of<T>(p, item);
     if constexpr (!DISTILL) {
       const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
       const bool bad = p.tokens && (token < 0 || token > p.n);
       if (token == 0 || bad) {
-        if (bad && tid == 0) atomicMax(p.status, DEV_BAD_INDEX);
-        stream_zeros<T>(r, dst, tid, kThreads);
-        continue;
+        if (bad && lane == 0) atomicMax(p.status, DEV_BAD_INDEX);
+        if (lane == 0) l.zero = true;
+        return true;
       }
-      const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gh = p.d_entropy ? p.d_entropy[row] : 0.f;
-      const float h = p.d_entropy ? p.entropy[row] : 0.f, lse2 = p.lse[row] * kLog2e;
-      float all = lane < p.top ? p.d_top[row * p.top + lane] : 0.f;
-      all = g0 + warp_sum(all);
-      // entries: the alternatives, then the token
-      const int entries = p.top + (p.d_logprobs ? 1 : 0);
-      __syncthreads();
-      if (tid < entries) {
-        long long id = tid < p.top ? p.top_ids[row * p.top + tid] : token;
-        if (id < 0 || id > p.n) {
-          atomicMax(p.status, DEV_BAD_INDEX);
-          id = 0;
-        }
-        entry[tid] = (int)id;
-        weight[tid] = tid < p.top ? p.d_top[row * p.top + tid] : g0;
-      }
-      __syncthreads();
-      const int id = tid < entries ? entry[tid] : 0;
-      const float x = id > lo && id <= hi ? to_float(r.src[id - 1]) : 0.f;
-      const float a = -(all + gh * h) / p.temperature, b = -gh * kLn2 / p.temperature;
-      __syncthreads();  // dst may be the logits themselves
-      if (p.d_entropy) stream_gradient<T, true>(r, dst, p.c, lse2, a, b);
-      else stream_gradient<T, false>(r, dst, p.c, lse2, a, 0.f);
-      __syncthreads();
-      if (id > lo && id <= hi) {
-        float g = 0.f;
-        bool again = false;
-        for (int i = 0; i < entries; ++i)
-          if (entry[i] == id) {
-            again |= i < tid;
-            g += weight[i];
-          }
-        const float t = fmaf(x, p.c, -lse2);
-        if (!again) dst[id - 1] = from_float<T>(g / p.temperature + ex2_approx_ftz(t) * fmaf(b, fmaxf(t, kLowest), a));
+      const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
+      const float gt = lane < p.top ? p.d_top[row * p.top + lane] : 0.f, all = g0 + warp_sum(gt);
+      if (lane < p.top) enter(l, lane, p.top_ids[row * p.top + lane], gt, r);
+      if (lane == 0) {
+        if (p.d_logprobs) enter(l, p.top, token, g0, r);
+        l.entries = p.top + (p.d_logprobs ? 1 : 0);
+        l.lse2 = p.lse[row] * kLog2e;
+        l.a = -(all + gh * h) / p.temperature;
+        l.b = -gh * kLn2 / p.temperature;
       }
     } else {
       const float4 saved = reinterpret_cast<const float4*>(p.saved)[row];
       if (saved.z == 0.f) {
-        stream_zeros<T>(r, dst, tid, kThreads);
-        continue;
+        if (lane == 0) l.zero = true;
+        return true;
       }
       const bool whole = saved.z < 0.f;  // the teacher's list is all of its distribution
-      const float outside = whole ? 1.f : saved.y, all = whole ? 1.f : saved.z;
       const double norm = (double)saved.w + (whole ? (double)saved.y : 0.);
-      const float g = p.d_loss[row] / p.temperature, lse2 = saved.x * kLog2e;
-      __syncthreads();
-      if (tid < p.entries) {
-        long long id = load_id(p.ids, row * p.entries + tid, p.id_bits);
-        if (id < 0 || id > p.n) {
-          atomicMax(p.status, DEV_BAD_INDEX);
-          id = 0;
-        }
-        entry[tid] = (int)id;
-        weight[tid] = (float)exp((double)load_value(p.values, row * p.entries + tid, p.values_dtype) / (double)p.temperature - norm);
+      for (int j = lane; j < p.entries; j += 32) {
+        const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
+        enter(l, j, load_id(p.ids, row * p.entries + j, p.id_bits), (float)exp(u - norm), r);
       }
-      __syncthreads();
-      const int id = tid < p.entries ? entry[tid] : 0;
-      const float x = id > lo && id <= hi ? to_float(r.src[id - 1]) : 0.f;
-      __syncthreads();  // dst may be the logits themselves
-      stream_gradient<T, false>(r, dst, p.c, lse2, g * outside, 0.f);
-      __syncthreads();
-      patch_entries<T>(dst, entry, weight, p.entries, x, p.c, lse2, g, all, lo, hi);
+      if (lane == 0) {
+        l.g = p.d_loss[row] / p.temperature;
+        l.entries = p.entries;
+        l.lse2 = saved.x * kLog2e;
+        l.a = l.g * (whole ? 1.f : saved.y);
+        l.all = whole ? 1.f : saved.z;
+      }
+    }
+    return true;
+  }
+  __device__ __forceinline__ void stream(int, const Lesson& l, const Range<T>& r, const Inner& in) {
+    T* dst = static_cast<T*>(p.dx) + row_of(p, l.at) * p.ld_dx;
+    if (l.zero) stream_zeros<T>(r, dst);
+    else stream_gradient<T, ENTROPY>(r, in, dst, p.c, l.lse2, l.a, l.b);
+  }
+  __device__ __forceinline__ void finish(int, const Lesson& l, const Range<T>& r, const Inner&) {
+    if (l.zero) return;
+    T* dst = static_cast<T*>(p.dx) + row_of(p, l.at) * p.ld_dx;
+    if constexpr (DISTILL) {
+      patch_entries<T>(r, dst, l.entry, l.weight, l.x, l.entries, p.c, l.lse2, l.g, l.all);
+    } else {
+      const int j = threadIdx.x;
+      if (j >= l.entries || l.entry[j] == 0) return;
+      float g = 0.f;
+      for (int i = 0; i < l.entries; ++i)
+        if (l.entry[i] == l.entry[j]) {
+          if (i < j) return;
+          g += l.weight[i];
+        }
+      const float t = fmaf(l.x[j], p.c, -l.lse2);
+      dst[l.entry[j] - 1] = from_float<T>(g / p.temperature + ex2_approx_ftz(t) * fmaf(l.b, fmaxf(t, kLowest), l.a));
     }
   }
+};
+template <typename T, bool DISTILL, bool ENTROPY>
+__global__ void __launch_bounds__(kAllThreads, kBackwardPerSm<DISTILL>) logits_backward_kernel(const __grid_constant__ Backward p) {
+  __shared__ typename BackwardOp<T, DISTILL, ENTROPY>::Lesson lessons[3];
+  BackwardOp<T, DISTILL, ENTROPY> op{p};
+  run_rows<T>(p, op, lessons, nullptr);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1060,67 +1298,123 @@ int check_gradient(const char* who, const void* x, void* dx, int64_t V, int64_t 
     if (!is_device_ptr(p)) return fail(CTB_BAD_ARG, "%s: argument %s is not a device pointer", who, #p); \
   } while (0)
 
-// Parts of a row in a forward pass, and vectors per part: as many parts as bring work to every place for a CTA, none below one tile.
-void cut_rows(int64_t places, int64_t rows, int64_t nvec, int64_t least, int most, int* parts, int* per) {
-  int64_t n = rows >= places ? 1 : places / rows;
-  n = std::min<int64_t>(n, (nvec + kTile - 1) / kTile);
-  n = std::min<int64_t>(std::max(n, least), most);
-  int64_t v = (nvec + n - 1) / n;
-  v = (v + 31) / 32 * 32;
-  *per = (int)v;
-  *parts = (int)((nvec + v - 1) / v);
+// Clusters of C CTAs of a kernel that run at once.
+template <auto KERNEL>
+int most_teams(ctb_ctx* ctx, int C, int per_sm, size_t smem, bool keep) {
+  static std::atomic<int> cached[16][kMaxCluster + 1];
+  std::atomic<int>& known = cached[ctx->device & 15][C];
+  if (keep && known.load(std::memory_order_relaxed) > 0) return known.load(std::memory_order_relaxed);
+  int n = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctx->sm_count * per_sm / C * C);
+  cfg.blockDim = dim3(kAllThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  if (keep && n > 0) known.store(n, std::memory_order_relaxed);
+  return n;
 }
 
-// Launches a forward kernel: rows whole or in parts.  `most` parts at most; holes: of the bits per element that a part may have in shared
-// memory.
-template <typename T, typename P>
-int launch_forward(ctb_ctx* ctx, cudaStream_t st, P p, void (*kernel)(P), int threads, int per_sm, int top, bool whole, bool holes, const char* who) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int64_t nvec = (p.n + V - 1) / V + 1;  // a row that starts off a vector boundary touches one more
-  int most = kMaxParts;
-  if (p.rows > kTickets || whole) most = 1;
-  else most = std::max<int>(1, std::min<int64_t>(most, kStreamScratchBytes / sizeof(float) / record_floats(top) / p.rows));
-  if (top) most = std::min(most, kCand / top);
-  cut_rows(per_sm * ctx->sm_count, p.rows, nvec, holes ? (nvec * V + kMostHoles - 1) / kMostHoles : 1, most, &p.parts, &p.per);
-  auto go = [&] {
-    const size_t smem = holes ? 2 * 4 * (((size_t)p.per * V + 31) / 32) : 0;
-    if (holes) {
-      if ((int64_t)p.per * V > kMostHoles + 1024)
-        return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
-      cudaError_t e = allow_smem(kernel, 2 * (kMostHoles + 1024) / 8);
-      if (e != cudaSuccess) return cuda_fail(e, who);
+// How the rows are cut: for the kernels whose parts meet, into the 1, 2, 4, 8 or 16 CTAs of a cluster.  Rows go over the teams in rounds;
+// a round takes the time of its bytes at the rate of HBM, but no less than a part at the rate that a CTA reaches alone, and what begins
+// and ends a row (`ends`, and a meeting).  Times in us, rates in bytes per us.
+struct Cut {
+  int parts, teams;
+};
+template <auto KERNEL>
+Cut cut_rows(ctb_ctx* ctx, int64_t rows, int64_t row_bytes, int per_sm, int least, double ends) {
+  constexpr double kAlone = 20e3, kAll = 6500e3, kMeeting = 1.0;
+  Cut best = {0, 0};
+  double best_time = 0;
+  for (int C = 1; C <= kMaxCluster; C *= 2) {
+    if (C < least) continue;
+    if (row_bytes / C < 4096 && C > least) break;
+    const int most = C == 1 ? ctx->sm_count * per_sm : most_teams<KERNEL>(ctx, C, per_sm, 0, true);
+    if (most < 1) continue;
+    const int teams = (int)std::min<int64_t>(rows, most);
+    const double part = (double)row_bytes / C / kAlone + ends + (C > 1 ? kMeeting : 0.);
+    const int64_t full = rows / teams, rest = rows % teams;
+    const double time = (double)full * std::max((double)teams * (double)row_bytes / kAll, part) +
+                        (rest ? std::max((double)rest * (double)row_bytes / kAll, part) : 0.);
+    if (best.parts == 0 || time < best_time) {
+      best = {C, teams};
+      best_time = time;
     }
-    int fit = per_sm;  // more shared memory may leave room for fewer
-    if (holes) cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, smem);
-    const int grid = (int)std::min<int64_t>((int64_t)p.rows * p.parts, (int64_t)std::max(1, std::min(fit, per_sm)) * ctx->sm_count);
-    launch_kernel(kernel, grid, threads, smem, st, 0, p);
-    CTB_CHECK_LAUNCH(who);
-    return (int)CTB_OK;
-  };
-  if (p.parts > 1) {
-    StreamScratch scratch(ctx, st);
-    if (scratch.data) {
-      p.scratch = scratch.data;
-      p.tickets = scratch.tickets;
-      return go();
-    }
-    p.parts = 1;
-    p.per = (int)((nvec + 31) / 32 * 32);
   }
-  return go();
+  return best;
+}
+
+template <typename T>
+int64_t vectors(const Rows& p) {  // of a row, wherever it starts
+  constexpr int V = 16 / (int)sizeof(T);
+  return (p.n + V - 1) / V + 1;
+}
+void cut_into(Rows& p, int64_t nvec, int64_t parts) {
+  p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
+  p.parts = (int)parts;
+}
+// Launches a forward kernel.  holes: two bits of shared memory for each element of a part.
+template <auto KERNEL, typename T, typename P>
+int launch_forward(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool holes, double ends, const char* who) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int64_t nvec = vectors<T>(p);
+  p.cluster = 1;
+  cudaError_t e = holes ? allow_smem(KERNEL, (kMostHoles + 1024) / 4) : cudaSuccess;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  int least = 1;
+  if (holes)
+    while (least < kMaxCluster && nvec * V > (int64_t)least * kMostHoles) least *= 2;
+  Cut cut = cut_rows<KERNEL>(ctx, p.rows, nvec * 16, per_sm, least, ends);
+  if (cut.parts == 0) return fail(CTB_UNSUPPORTED, "%s: no room for a row's CTAs on this device", who);
+  cut_into(p, nvec, cut.parts);
+  size_t smem = 0;
+  if (holes) {  // more shared memory may leave room for fewer
+    if ((int64_t)p.per * V > kMostHoles + 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, rows of %d elements are too long", who, p.n);
+    smem = 2 * 4 * (((size_t)p.per * V + 31) / 32);
+    int fit = 0;
+    if (p.parts > 1) {
+      fit = most_teams<KERNEL>(ctx, p.parts, per_sm, smem, false);
+    } else {
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, KERNEL, kAllThreads, smem);
+      fit *= ctx->sm_count;
+    }
+    cut.teams = std::max(1, std::min(cut.teams, fit));
+  }
+  launch_kernel(KERNEL, cut.teams * p.parts, kAllThreads, smem, st, p.parts, p);
+  CTB_CHECK_LAUNCH(who);
+  return CTB_OK;
 }
 
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
-  return launch_forward<T>(ctx, st, p, p.top ? logprobs_kernel<T, true> : logprobs_kernel<T, false>, kThreads, p.top ? kTopPerSm : kPlainPerSm, p.top, false,
-                           false, who);
+  return p.top ? launch_forward<logprobs_kernel<T, true>, T>(ctx, st, p, kLogprobsPerSm<true>, false, 3.0, who)
+               : launch_forward<logprobs_kernel<T, false>, T>(ctx, st, p, kLogprobsPerSm<false>, false, 1.0, who);
 }
-template <typename T>
+template <typename T, bool GRAD>
 int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* who) {
-  const bool grad = p.dx, holes = p.teacher_lse;
-  auto kernel = grad ? holes ? distill_kernel<T, true, true> : distill_kernel<T, true, false>
-                     : holes ? distill_kernel<T, false, true> : distill_kernel<T, false, false>;
-  return launch_forward<T>(ctx, st, p, kernel, kThreads + 32, kDistillPerSm, 0, grad, holes, who);
+  return p.teacher_lse ? launch_forward<distill_kernel<T, GRAD, true>, T>(ctx, st, p, kDistillPerSm, true, 2.5, who)
+                       : launch_forward<distill_kernel<T, GRAD, false>, T>(ctx, st, p, kDistillPerSm, false, 2.5, who);
+}
+template <typename T, bool DISTILL>
+int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
+  auto kernel = p.d_entropy ? logits_backward_kernel<T, DISTILL, !DISTILL> : logits_backward_kernel<T, DISTILL, false>;
+  // Parts have nothing to do with each other: of at most four tiles, or one where that brings work to more places.
+  const int64_t nvec = vectors<T>(p), places = (int64_t)kBackwardPerSm<DISTILL> * ctx->sm_count;
+  const int64_t tiles = (nvec + kTile - 1) / kTile, each = p.rows * tiles >= 16 * places ? 4 : 1;
+  cut_into(p, nvec, (tiles + each - 1) / each);
+  launch_kernel(kernel, (int)std::min<int64_t>((int64_t)p.rows * p.parts, places), kAllThreads, 0, st, 0, p);
+  CTB_CHECK_LAUNCH(who);
+  return CTB_OK;
 }
 template <typename F>
 int by_type(int dtype, F f) {
@@ -1129,21 +1423,6 @@ int by_type(int dtype, F f) {
   return f(__nv_bfloat16());
 }
 
-template <typename T, bool DISTILL>
-int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int64_t nvec = (p.n + V - 1) / V + 1;
-  // parts of at most four tiles, and of one where that spreads the work over more SMs
-  const int64_t tiles = p.rows * ((nvec + kTile - 1) / kTile);
-  const int64_t want = tiles >= 16ll * ctx->sm_count ? 4 : 1;
-  const int64_t parts = (nvec + want * kTile - 1) / (want * kTile);
-  p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
-  p.parts = (int)((nvec + p.per - 1) / p.per);
-  const int grid = (int)std::min<int64_t>((int64_t)p.rows * p.parts, (int64_t)kBackwardPerSm * ctx->sm_count);
-  launch_kernel(logits_backward_kernel<T, DISTILL>, grid, kThreads, 0, st, 0, p);
-  CTB_CHECK_LAUNCH(who);
-  return CTB_OK;
-}
 int check_bits(const char* who, int bits) {
   return bits == 32 || bits == 64 ? CTB_OK : fail(CTB_BAD_ARG, "%s: ids must be 32- or 64-bit integers", who);
 }
@@ -1218,7 +1497,7 @@ extern "C" int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits
     CTB_CHECK_PTR(who, d_top_logprobs);
   }
   Backward p = {};
-  p.x = logits; p.dx = d_logits; p.ld = ld; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
+  p.x = logits; p.ld = ld; p.dx = d_logits; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
   p.c = (float)(1.4426950408889634 / (double)temperature);
   p.temperature = temperature;
   p.status = ctx->dev_status;
@@ -1247,7 +1526,8 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   p.teacher_lse = teacher_lse; p.loss = loss; p.saved = saved;
   p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(ctx, st, p, who); });
+  if (d_logits) return by_type(dtype, [&](auto t) { return launch_distill<decltype(t), true>(ctx, st, p, who); });
+  return by_type(dtype, [&](auto t) { return launch_distill<decltype(t), false>(ctx, st, p, who); });
 }
 
 extern "C" int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
@@ -1257,19 +1537,6 @@ extern "C" int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, c
   CurrentDevice current(ctx);
   return distill_forward("ctb_distill_fwd", ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved,
                          nullptr, nullptr, V, T, 0, ld, entries, temperature, dtype);
-}
-
-static int distill_backward(const char* who, ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids,
-                            int id_bits, const void* teacher_values, int values_dtype, const float* saved, const float* d_loss, int64_t V,
-                            int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature, int dtype) {
-  Backward p = {};
-  p.x = logits; p.dx = d_logits; p.ld = ld; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
-  p.c = (float)(1.4426950408889634 / (double)temperature);
-  p.temperature = temperature;
-  p.status = ctx->dev_status;
-  p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
-  p.saved = saved; p.d_loss = d_loss;
-  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t), true>(ctx, static_cast<cudaStream_t>(stream), p, who); });
 }
 
 extern "C" int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
@@ -1285,8 +1552,14 @@ extern "C" int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const
   CTB_CHECK_PTR(who, saved);
   CTB_CHECK_PTR(who, d_loss);
   if ((uintptr_t)saved % 16) return fail(CTB_BAD_ALIGN, "%s: saved must be 16-byte aligned", who);
-  return distill_backward(who, ctx, stream, d_logits, logits, teacher_ids, id_bits, teacher_values, values_dtype, saved, d_loss, V, T, ld_out,
-                          ld, entries, temperature, dtype);
+  Backward p = {};
+  p.x = logits; p.ld = ld; p.dx = d_logits; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
+  p.c = (float)(1.4426950408889634 / (double)temperature);
+  p.temperature = temperature;
+  p.status = ctx->dev_status;
+  p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
+  p.saved = saved; p.d_loss = d_loss;
+  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t), true>(ctx, static_cast<cudaStream_t>(stream), p, who); });
 }
 
 extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
@@ -1300,13 +1573,6 @@ extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, c
   if (T == 0) return CTB_OK;
   if (int s = check_gradient(who, logits, d_logits, V, T, ld, ld_out, dtype)) return s;
   CTB_CHECK_PTR(who, d_loss);
-    // One kernel where there are rows enough to give every SM its own, else the two halves, which cut rows into parts.
-  if (T >= 2 * ctx->sm_count && !(teacher_lse && V > kMostHoles))
     return distill_forward(who, ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved, d_loss,
-                           d_logits, V, T, ld_out, ld, entries, temperature, dtype);
-  if (int s = distill_forward(who, ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved, nullptr,
-                              nullptr, V, T, 0, ld, entries, temperature, dtype))
-    return s;
-  return distill_backward(who, ctx, stream, d_logits, logits, teacher_ids, id_bits, teacher_values, values_dtype, saved, d_loss, V, T, ld_out,
-                          ld, entries, temperature, dtype);
+                         d_logits, V, T, ld_out, ld, entries, temperature, dtype);
 }

@@ -272,6 +272,13 @@ __device__ __forceinline__ void send_to_cta(const void* slot, float a, float b, 
                "f"(a), "f"(b), "r"(map_to_cta(bar, rank))
                : "memory");
 }
+// The same with four values, 16 bytes.
+__device__ __forceinline__ void send4_to_cta(const void* slot, float4 v, const void* bar, uint32_t rank) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(map_to_cta(slot, rank)),
+      "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(map_to_cta(bar, rank))
+      : "memory");
+}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 // Meets the cluster without making stores visible to it (a release waits for those of the thread).
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }

@@ -53,21 +53,18 @@ __device__ __forceinline__ uint4 empty_row_vec() {
   return make_uint4(w, w, w, w);
 }
 
-// A 32-bit word of a row is one f32 or two 16-bit elements.  Larger of two words, element by element; NEVER_NAN: a number where one of
-// them is NaN, else NaN.
-template <typename T, bool NEVER_NAN>
+// A 32-bit word of a row is one f32 or two 16-bit elements.  Larger of two words, element by element; a number where one of them is NaN.
+template <typename T>
 __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
   uint32_t d;
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (NEVER_NAN) asm("max.f32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    else asm("max.NaN.f32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  } else if constexpr (std::is_same<T, __half>::value) {
-    if constexpr (NEVER_NAN) asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  } else {
-    if constexpr (NEVER_NAN) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  }
+  if constexpr (sizeof(T) == 4) asm("max.f32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else if constexpr (std::is_same<T, __half>::value) asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 // The elements of a 16-bit word.
@@ -85,15 +82,66 @@ __device__ __forceinline__ float word_max(uint32_t w) {
     return fmaxf(f.x, f.y);
   }
 }
-// Pair i of a vector's elements.
 template <typename T>
-__device__ __forceinline__ float2 vec_pair(const uint32_t (&w)[4], int i) {
-  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-  else return word_pair<T>(w[i]);
+__device__ __forceinline__ float word_nan(uint32_t w) {  // the same, NaN where one of them is
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else {
+    const float2 f = word_pair<T>(w);
+    return max_nan(f.x, f.y);
+  }
 }
 
+// Two f32 values in a 64-bit register, and operations that take one instruction for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 halves(Pair a) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
+  return f;
+}
+__device__ __forceinline__ float sum_of(Pair a) {
+  const float2 f = halves(a);
+  return f.x + f.y;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair exp2_pair(Pair t) {
+  const float2 f = halves(t);
+  float a, b;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(f.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(f.y));
+  return pair(a, b);
+}
+
+// Pair i of a vector's elements.
 template <typename T>
-__device__ __forceinline__ void put_pair(uint32_t (&w)[4], int i, float2 f) {
+__device__ __forceinline__ Pair vec_pair(const uint32_t (&w)[4], int i) {
+  if constexpr (sizeof(T) == 4) return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else {
+    const float2 f = word_pair<T>(w[i]);
+    return pair(f.x, f.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put_pair(uint32_t (&w)[4], int i, Pair d) {
+  const float2 f = halves(d);
   if constexpr (sizeof(T) == 4) {
     w[2 * i] = __float_as_uint(f.x);
     w[2 * i + 1] = __float_as_uint(f.y);
@@ -152,30 +200,6 @@ __device__ __noinline__ void store_edge(T* dst, int off, int n, int v, uint4 q) 
     const int e = v * V - off + i;
     if (e >= 0 && e < n) dst[e] = reinterpret_cast<const T*>(&q)[i];
   }
-}
-
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 w, x, y, z;\n\tmov.b64 w, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tmov.b64 y, {%6, %7};\n\tfma.rn.f32x2 z, w, x, y;\n\t"
-      "mov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
 }
 
 }  // namespace ctb
