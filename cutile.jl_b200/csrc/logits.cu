@@ -26,17 +26,13 @@ namespace {
 
 constexpr int kThreads = 256;            // that stream
 constexpr int kWarps = kThreads / 32;
-constexpr int kAllThreads = kThreads + 32;  // and the clerk
+constexpr int kAllThreads = kThreads + 32;  // with a clerk
 constexpr int kUnroll = 4;               // vectors of 16 bytes per thread and tile
 constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
 constexpr int kMaxEntries = kThreads;    // of a teacher's list
 constexpr int kCand = 1024;
-template <bool TOP>
-constexpr int kLogprobsPerSm = TOP ? 3 : 5;  // CTAs on an SM
-constexpr int kDistillPerSm = 4;
-template <bool DISTILL>
-constexpr int kBackwardPerSm = DISTILL ? 4 : 5;
+constexpr int kPlainPerSm = 6, kTopPerSm = 3, kDistillPerSm = 4, kBackwardPerSm = 5;  // CTAs on an SM
 constexpr int kMostHoles = 512 * 1024;  // elements of a part that have a bit (in two sets) in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -44,11 +40,19 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -16384.f;
 // A thread's reference follows its maximum only when an element is 2^kSlack above it.
 constexpr float kSlack = 4.f;
-constexpr float kFar = 1e30f;  // rows with a maximum beyond +-kFar (masked as a whole, or infinite) are summed in another way
+constexpr float kFar = 1e30f;  // beyond, x log2(e) / temperature may overflow
 
-__device__ __forceinline__ void bar_stream() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the streaming threads
-__device__ __forceinline__ void bar_row() { asm volatile("bar.sync 2, 288;" ::: "memory"); }         // and the clerk
-static_assert(kThreads == 256, "the barriers name the numbers of threads");
+__device__ __forceinline__ void bar_stream() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // the streaming warps
+__device__ __forceinline__ bool all_stream(bool ok) {  // true in all of them when it is in all of them
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)ok)
+      : "memory");
+  return r != 0;
+}
+static_assert(kThreads == 256, "bar_stream names the number of threads");
 
 // ------------------------------------------------------------------ the best k of a row
 // One pass, every element compared with a threshold that at least k earlier elements reach:
@@ -236,29 +240,34 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
 // Exponents t = x c - m2, with c = log2(e) / temperature: one fused multiply-add gives them with one rounding, whatever the magnitude of x, and
 // the rounding of c is that of a temperature, the same for the whole row.
 //
-// A thread's share of s = sum 2^t and w = sum 2^t t.  Its reference m2 follows its maximum, or t 2^t of a likely element would carry a
-// rounding that the entropy, a difference of two such sums, shows.  Masked elements (-inf) make w NaN (0 * -inf); the tile's share is
-// then taken again with exponents held above kLowest.  Valid for rows whose maximum is `plain`; the others take slow_sums.
-template <typename T>
+// A thread's share of s = sum 2^t and, with ENTROPY, w = sum 2^t t.  Its reference follows its maximum, or t 2^t of a likely element would
+// carry a rounding that the entropy, a difference of two such sums, shows.  Masked elements (-inf) make w NaN (0 * -inf): the tile's
+// share is then taken again with exponents held above kLowest.  Where the maximum is beyond +-kFar (all that is left is masked by the
+// lowest number; infinities) x c would overflow, and exponents are taken from differences, (x - maximum) c.
+template <typename T, bool ENTROPY>
 struct Sums {
-  float m2 = 0.f, limit = -FLT_MAX;  // elements above limit move the reference
+  float ref = 0.f, m2 = 0.f, limit = -INFINITY;  // m2 = ref c; elements above limit move the reference
   uint32_t top = empty_row_vec<T>().x;
   Pair s = pair(0.f, 0.f), w = pair(0.f, 0.f);
 
-  static __device__ __forceinline__ bool plain(float maximum) { return maximum <= kFar && maximum >= -kFar; }
-  __device__ __forceinline__ void move(float t, float c) {
-    const float x = fminf(fmaxf(t, -kFar), kFar), to = x * c, d = fmaxf(fminf(m2 - to, 0.f), kLowest), r = ex2_approx_ftz(d);
+  __device__ __forceinline__ bool far() const { return fabsf(ref) > kFar; }
+  __device__ __forceinline__ void move(float x, float c) {
+    const float to = x * c;
+    const bool jump = fabsf(x) > kFar || far();
+    const float d = fmaxf(fminf(jump ? (ref - x) * c : m2 - to, 0.f), kLowest), r = ex2_approx_ftz(d);  // s = w = 0 until there is a reference
     const Pair rr = pair(r, r);
-    w = mul2(rr, fma2(s, pair(d, d), w));
+    if constexpr (ENTROPY) w = mul2(rr, fma2(s, pair(d, d), w));
     s = mul2(rr, s);
-    m2 = to;
+    ref = x;
+    m2 = fabsf(x) > kFar ? 0.f : to;
     limit = x + kSlack / c;
   }
-  // Returns the largest element of the tile.
-  __device__ __forceinline__ float add(const uint4 (&q)[kUnroll], float c) {
+  // Returns the largest element.
+  template <int N>
+  __device__ __forceinline__ float add(const uint4 (&q)[N], float c) {
     uint32_t all = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < N; ++u) {
       const uint32_t a = max_word<T>(max_word<T>(q[u].x, q[u].y), max_word<T>(q[u].z, q[u].w));
       all = u == 0 ? a : max_word<T>(all, a);
     }
@@ -268,88 +277,57 @@ struct Sums {
     const Pair cc = pair(c, c), minus = pair(-m2, -m2);
     Pair ts = pair(0.f, 0.f), tw = ts;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < N; ++u) {
       const uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
       for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
         const Pair t = fma2(vec_pair<T>(word, i), cc, minus), e = exp2_pair(t);
         ts = add2(ts, e);
-        tw = fma2(e, t, tw);
+        if constexpr (ENTROPY) tw = fma2(e, t, tw);
+      }
+    }
+    if (far() || (ENTROPY && sum_of(tw) != sum_of(tw))) {
+      ts = tw = pair(0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const float2 one = apart(q[u], ref, m2, c);
+        ts = add2(ts, pair(one.x, 0.f));
+        tw = add2(tw, pair(one.y, 0.f));
       }
     }
     s = add2(s, ts);
-    if (sum_of(tw) != sum_of(tw)) tw = pair((again(q[0], m2, c) + again(q[1], m2, c)) + (again(q[2], m2, c) + again(q[3], m2, c)), 0.f);
-    w = add2(w, tw);
+    if constexpr (ENTROPY) w = add2(w, tw);
     return most;
   }
-  static __device__ __noinline__ float again(uint4 q, float m2, float c) {
-    static_assert(kUnroll == 4, "add() calls this for each vector of a tile");
-    float f[16 / sizeof(T)], a = 0.f;
+  // (s, w) of a vector, exponents held above kLowest in w.
+  static __device__ __noinline__ float2 apart(uint4 q, float ref, float m2, float c) {
+    float f[16 / sizeof(T)], s = 0.f, w = 0.f;
     unpack_row<T>(q, f);
+    const bool far = fabsf(ref) > kFar;
 #pragma unroll
     for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
-      const float t = fmaf(f[i], c, -m2);
-      a = fmaf(ex2_approx_ftz(t), fmaxf(t, kLowest), a);
+      const float t = far ? (f[i] - ref) * c : fmaf(f[i], c, -m2), e = ex2_approx_ftz(t);
+      s += e;
+      w = fmaf(e, fmaxf(t, kLowest), w);
     }
-    return a;
+    return make_float2(s, w);
   }
   // One element more.
   __device__ __forceinline__ void add_one(float x, float c) {
     const T e = from_float<T>(x);
     top = max_word<T>(top, sizeof(T) == 4 ? __float_as_uint(x) : 0x10001u * *reinterpret_cast<const unsigned short*>(&e));
     if (x > limit) move(x, c);
-    const float t = fmaf(x, c, -m2), v = ex2_approx_ftz(t);
+    const float t = far() ? (x - ref) * c : fmaf(x, c, -m2), v = ex2_approx_ftz(t);
     s = add2(s, pair(v, 0.f));
-    w = add2(w, pair(v * fmaxf(t, kLowest), 0.f));
+    if constexpr (ENTROPY) w = add2(w, pair(v * fmaxf(t, kLowest), 0.f));
   }
   // The warp's (maximum, s, w), the sums relative to that maximum.
   __device__ __forceinline__ float3 over_warp(float c) const {
-    const float most = warp_max(word_max<T>(top)), to = fminf(fmaxf(most, -kFar), kFar);
-    const float d = fminf(fmaf(-to, c, m2), 1.f), r = ex2_approx_ftz(d), sum = sum_of(s);  // a thread without elements has m2 = sum = 0
-    return make_float3(most, warp_sum(sum * r), warp_sum(r * fmaf(sum, fmaxf(d, kLowest), sum_of(w))));
-  }
-};
-
-// s alone, for the warp: the reference is the largest element of the warp's first tile that has one above -inf, and stays.  What is
-// more than 2^127 above it, or all of it below f32, shows as a sum that is not finite and positive; the row then takes slow_sums.
-template <typename T>
-struct LeanSums {
-  float ref = -INFINITY, m2 = 0.f;  // m2 = ref c
-  Pair s = pair(0.f, 0.f);
-
-  __device__ __forceinline__ void add(const uint4 (&q)[kUnroll], float c) {
-    if (ref == -INFINITY) {  // the same in the whole warp
-      float most = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        most = max_nan(most, max_nan(max_nan(word_nan<T>(q[u].x), word_nan<T>(q[u].y)), max_nan(word_nan<T>(q[u].z), word_nan<T>(q[u].w))));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (most == -INFINITY) return;
-      ref = fminf(fmaxf(most, -kFar), kFar);  // of NaN: any number, the sum will be NaN
-      m2 = ref * c;
-    }
-    const Pair cc = pair(c, c), minus = pair(-m2, -m2);
-    Pair ts = pair(0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-      for (int i = 0; i < 8 / (int)sizeof(T); ++i) ts = add2(ts, exp2_pair(fma2(vec_pair<T>(word, i), cc, minus)));
-    }
-    s = add2(s, ts);
-  }
-  // One element more of each lane (-inf: none).
-  __device__ __forceinline__ void add_one(float x, float c) {
-    uint4 q[kUnroll] = {empty_row_vec<T>(), empty_row_vec<T>(), empty_row_vec<T>(), empty_row_vec<T>()};
-    const T e = from_float<T>(x);
-    q[0].x = sizeof(T) == 4 ? __float_as_uint(x) : (q[0].x & 0xffff0000u) | *reinterpret_cast<const unsigned short*>(&e);
-    add(q, c);
-  }
-  // The warp's (reference, s), s relative to that reference.
-  __device__ __forceinline__ float2 over_warp(float c) const {
-    const float sum = warp_sum(sum_of(s));
-    return make_float2(ref, ref == -INFINITY ? 0.f : sum * ex2_approx_ftz(fmaf(-ref, c, m2)));
+    const float most = warp_max(word_max<T>(top));
+    float d = fabsf(most) > kFar || far() ? (ref - most) * c : fmaf(-most, c, m2);
+    if (limit == -INFINITY) d = 0.f;  // nothing but masked elements, or NaN: its sums are 0, or NaN
+    const float r = ex2_approx_ftz(d), sum = sum_of(s);
+    return make_float3(most, warp_sum(sum * r), ENTROPY ? warp_sum(r * fmaf(sum, fmaxf(d, kLowest), sum_of(w))) : 0.f);
   }
 };
 
@@ -374,60 +352,6 @@ __device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
   }
 }
 
-// (maximum, s, w) of a range whose sums above are not valid, relative to its maximum, from differences (x - maximum); without the elements
-// that the `entries` ids name.  All streaming threads; `red` is theirs.
-template <typename T>
-__device__ __noinline__ float3 slow_sums(const Range<T>& r, const int* entry, int entries, float c, float (&red)[3][kWarps]) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float most = -FLT_MAX, s = 0.f, w = 0.f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
-      uint4 q = load_vec(r, v);
-      unsigned bits = 0;
-      for (int j = 0; j < entries; ++j) {
-        const int i = entry[j] - 1 + r.off - v * V;
-        if (entry[j] && i >= 0 && i < V) bits |= 1u << i;
-      }
-      if (bits) mask_holes<T>(q, bits);
-      float f[V];
-      unpack_row<T>(q, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (pass == 0) {
-          most = fmaxf(most, f[i]);
-        } else {
-          const float t = (f[i] - most) * c, e = ex2_approx_ftz(t);
-          s += e;
-          w = fmaf(e, fmaxf(t, kLowest), w);
-        }
-      }
-    }
-    bar_stream();  // red has been read
-    if (pass == 0) {
-      most = warp_max(most);
-      if (lane == 0) red[0][warp] = most;
-    } else {
-      s = warp_sum(s);
-      w = warp_sum(w);
-      if (lane == 0) {
-        red[1][warp] = s;
-        red[2][warp] = w;
-      }
-    }
-    bar_stream();
-    if (pass == 0) {
-      for (int i = 0; i < kWarps; ++i) most = fmaxf(most, red[0][i]);
-    }
-  }
-  s = w = 0.f;
-  for (int i = 0; i < kWarps; ++i) {
-    s += red[1][i];
-    w += red[2][i];
-  }
-  return make_float3(most, s, w);
-}
-
 // (s, w) of up to 8 or 16 sets of sums, held by lanes i, i + 8 (16), ..., each relative to a maximum of its own, relative to `most`.
 // apart: of the set's maximum below `most`, in units of log2.
 template <int OF>
@@ -441,11 +365,16 @@ __device__ __forceinline__ float2 join(float apart, float s, float w) {
   }
   return make_float2(a, b);
 }
-__device__ __forceinline__ float red_max(const float (&v)[kWarps]) {
-  float m = v[0];
+// (maximum, s, w) of the warps' sums, in all lanes of a warp.
+template <int W>
+__device__ __forceinline__ float3 join_warps(const float (&red)[3][kWarps], float c) {
+  const int w = threadIdx.x & (W - 1);
+  float most = red[0][w];
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) m = fmaxf(m, v[i]);
-  return m;
+  for (int o = W / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  most = fmaxf(most, -FLT_MAX);
+  const float2 sum = join<W>((red[0][w] - most) * c, red[1][w], red[2][w]);
+  return make_float3(most, sum.x, sum.y);
 }
 
 __device__ __forceinline__ long long load_id(const void* p, long long i, int bits) {
@@ -461,39 +390,24 @@ struct Rows {
   const void* x;
   long long ld;
   int n, rows, parts, per;  // per: vectors of a part
-  int cluster;              // the parts of a row are the CTAs of a cluster, which meet; else they have nothing to do with each other
   float c, temperature;     // c = log2(e) / temperature
   int* status;
+  float4* records;          // (maximum, s, w) of the parts of rows that warps have cut among them
+  unsigned* tickets;        // a counter per row
 };
-// The (row, part) of an item.
-__device__ __forceinline__ long long row_of(const Rows& p, long long item) { return p.cluster ? item : item / p.parts; }
-__device__ __forceinline__ int part_of(const Rows& p, long long item) {
-  return p.cluster ? (int)cluster_ctarank() : (int)(item - item / p.parts * p.parts);
-}
 template <typename T>
-__device__ __forceinline__ Range<T> range_of(const Rows& p, long long item) {
+__device__ __forceinline__ Range<T> range_of(const Rows& p, long long row, int part) {
   constexpr int V = 16 / (int)sizeof(T);
   Range<T> r;
-  r.src = static_cast<const T*>(p.x) + row_of(p, item) * p.ld;
+  r.src = static_cast<const T*>(p.x) + row * p.ld;
   r.off = (int)(((uintptr_t)r.src & 15) / sizeof(T));
   r.n = p.n;
   const int nvec = (r.off + p.n + V - 1) / V;
-  r.v0 = (int)min((long long)nvec, (long long)part_of(p, item) * p.per);
+  r.v0 = (int)min((long long)nvec, (long long)part * p.per);
   r.v1 = min(nvec, r.v0 + p.per);
   return r;
 }
 
-// ------------------------------------------------------------------ rows through a CTA
-// A CTA takes row after row, or parts of rows, with two roles:
-//   stream   eight warps read the row, four vectors of 16 bytes per thread at a time; five CTAs on an SM keep HBM busy while one of them
-//            computes or ends a row (a ring of bulk copies ahead of the warps was no faster: what it saved in waiting it took in
-//            instructions, 10.7 per element instead of 7.4, for its barriers)
-//   clerk    a warp prepares the next row: whether it is padding, what the operator needs besides its logits (loads that
-//            depend on loads, f64 exponentials), so that a row ends with one barrier and a handful of operations
-// The row's first and last elements, up to a vector boundary, are loaded one by one.
-//
-// Where a row is cut into parts whose sums have to meet, the parts are the CTAs of a cluster: they send their sums to each other's
-// shared memory.  Few rows are spread over the GPU that way.
 constexpr int kMaxCluster = 16;
 
 // Whole vectors of a range, [a, b), and the elements before and behind them.
@@ -524,20 +438,82 @@ __device__ __forceinline__ int edge_index(const Range<T>& r, const Inner& in, in
   return -1;
 }
 
-// A streaming thread's vectors of the tile at v; beyond the range -inf.  KEEP: the row is read again, from L2.
-template <typename T, bool KEEP = false>
-__device__ __forceinline__ void load_tile(uint4 (&q)[kUnroll], const Range<T>& r, const Inner& in, int v) {
-  const int tid = threadIdx.x;
-  const uint4* p = r.at(v) + tid;
-  if (v + kTile <= in.b) {
+// Calls f(q, v) for a streaming thread's vectors, four at a time; v: the tile's first one.  What is left over comes one vector at a time, in
+// the warps that have some of it; lanes beyond the end get -inf.  KEEP: the row is read again, from L2.  Lanes that
+// took a rare branch in f would go on by themselves up to the next shuffle, behind the row: they meet before every tile.
+// W warps stream the row.
+template <typename T, bool KEEP, int W, typename F>
+__device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F f) {
+  constexpr int kWide = W * 32;
+  const int tid = threadIdx.x % kWide;
+  const uint4* p = r.at(in.a) + tid;
+  int v = in.a;
+#pragma unroll 1
+  for (; v + kWide * kUnroll <= in.b; v += kWide * kUnroll, p += kWide * kUnroll) {
+    __syncwarp();
+    uint4 q[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kThreads) : __ldcs(p + u * kThreads);
-  } else {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = v + tid + u * kThreads < in.b ? (KEEP ? __ldcg(p + u * kThreads) : __ldcs(p + u * kThreads)) : empty_row_vec<T>();
+    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kWide) : __ldcs(p + u * kWide);
+    f(q, v);
+  }
+#pragma unroll 1
+  for (; v + (tid & ~31) < in.b; v += kWide, p += kWide) {
+    __syncwarp();
+    uint4 q[1] = {empty_row_vec<T>()};
+    if (v + tid < in.b) q[0] = KEEP ? __ldcg(p) : __ldcs(p);
+    f(q, v);
   }
 }
 
+// ------------------------------------------------------------------ rows cut among warps
+// Where nothing but sums has to meet, a warp takes a part of a row (2 to 16 KB) after another, without a barrier and without a thought for the
+// other warps of its CTA: (maximum, s, w) go to a record in scratch memory, and the warp that finishes a row's last part joins the
+// records in their order and writes the results.  48 such warps on an SM keep 16-bit logits, whose exponentials take 70 % of the ex2
+// unit, as close to HBM's rate as a loop without rows; eight warps that meet at the end of every row left them at 78 %.
+constexpr int kMaxParts = 256;
+struct Items {  // of a warp
+  const Rows& p;
+  long long at, step, end;
+  __device__ __forceinline__ explicit Items(const Rows& rows) : p(rows) {
+    at = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    step = (long long)gridDim.x * kWarps;
+    end = (long long)p.rows * p.parts;
+  }
+  __device__ __forceinline__ long long row(long long item) const { return p.parts == 1 ? item : item / p.parts; }
+};
+// After a warp has summed a part: true for the row's last one, with the row's (maximum, s, w).
+__device__ __forceinline__ bool join_records(const Rows& p, long long row, int part, float3& sum) {
+  if (p.parts == 1) return true;
+  const int lane = threadIdx.x & 31;
+  float4* records = p.records + row * p.parts;
+  unsigned order = 0;
+  if (lane == 0) {
+    __stcg(records + part, make_float4(sum.x, sum.y, sum.z, 0.f));
+    __threadfence();
+    order = atomicInc(p.tickets + row, p.parts - 1);
+  }
+  if (__shfl_sync(0xffffffffu, order, 0) != (unsigned)p.parts - 1) return false;
+  __threadfence();
+  float most = -FLT_MAX;
+  for (int i = lane; i < p.parts; i += 32) most = fmaxf(most, __ldcg(&records[i].x));
+  most = warp_max(most);
+  float s = 0.f, w = 0.f;
+  for (int i = lane; i < p.parts; i += 32) {
+    const float4 one = __ldcg(records + i);
+    const float d = (one.x - most) * p.c, r = ex2_approx_ftz(d);
+    s = fmaf(one.y, r, s);
+    w += r * fmaf(one.y, fmaxf(d, kLowest), one.z);
+  }
+  sum = make_float3(most, warp_sum(s), warp_sum(w));
+  return true;
+}
+
+// ------------------------------------------------------------------ rows through a CTA
+// Where a row's warps have to meet (thresholds of a list; a gradient that follows the sum), a CTA takes row after row, with two roles:
+//   stream   eight warps read the row
+//   clerk    a warp prepares the rows to come: whether they are padding, what the operator needs besides the logits (loads that
+//            depend on loads, f64 exponentials), and joins the sums of rows that have been read
+// and the parts of a row are the CTAs of a cluster, whose sums go to each other's shared memory.
 // Sums of a row's parts in the shared memory of every CTA of the cluster, for even and odd meetings.  A peer sends to the meeting after
 // the next one only when this CTA has sent to the next, that is, has read this one.
 struct Meeting {
@@ -546,61 +522,99 @@ struct Meeting {
   volatile int abort;  // a wait ran out: no further message or wait
 };
 
-// The frame of the kernels below.  Op has
-//   Lesson                     what the clerk prepares; .at is the item, -1 behind the last one; .zero: its gradient is 0 and its logits are not read
-//   prepare(lesson, item)      the clerk: false for padding whose results it has written
-//   before(turn, lessons), after(turn, lessons)             the clerk, before and after a lesson is made
-//   stream(turn, lesson, range, inner)                      the streaming threads, up to the row's barrier
-//   finish(turn, lesson, range, inner)                      the streaming threads behind it
+// What passes between the roles: lesson n is posted by the clerk in slot n % 4, summed by the eight warps, answered by the clerk.
+struct Pipe {
+  uint64_t posted[4], summed[4], answered[4];
+  float red[4][3][kWarps];
+  volatile int abort;
+};
+
+// The frame of the kernels.  Op has
+//   Lesson                          what the clerk prepares for a row; .at is the row, -1 behind the last one
+//   prepare(lesson, row)            the clerk: false for padding whose results it has written
+//   before(n, lessons), after(n, lessons)   the clerk, before and after lesson n is made
+//   stream(n, lesson, range, inner, red)    the streaming warps
+//   answer(n, lesson, red)          the clerk, when all warps have streamed
+//   MEETS                           the streaming warps meet at barriers of their own
+//   AGAIN, again(lesson, range, inner)      the streaming warps, once the row has been answered and the next row has been streamed
 template <typename T, typename Op>
-__device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Lesson* lessons, Meeting* meeting) {
+__device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Lesson* lessons, Pipe& pipe, Meeting* meeting) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool cluster = p.cluster && p.parts > 1;
-  if (cluster) {
-    if (tid == 0) {
+  const bool cluster = p.parts > 1;
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&pipe.posted[i], 1);
+      mbar_init(&pipe.summed[i], kWarps);
+      mbar_init(&pipe.answered[i], 1);
+    }
+    pipe.abort = 0;
+    if (cluster) {
       for (int i = 0; i < 2; ++i) mbar_init(&meeting->bar[i], 1);
       meeting->abort = 0;
-      fence_mbar_init();
     }
-    __syncthreads();
-    cluster_arrive();  // the peers' shared memory and barriers exist
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (cluster) {  // the peers' shared memory and barriers exist
+    cluster_arrive();
     cluster_wait();
-  } else {
-    __syncthreads();
   }
-  grid_dependency_sync();
-  const long long items = p.cluster ? p.rows : (long long)p.rows * p.parts;
+  grid_dependency_wait();
+  const int step = gridDim.x / p.parts, rank = cluster ? (int)cluster_ctarank() : 0;
+  auto wait = [&](uint64_t* bar, int n) {
+    const int ok = lane == 0 ? (int)mbar_watch(bar, (n >> 2) & 1, p.status, DEV_TIMEOUT_SLOT, &pipe.abort) : 1;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  };
   if (warp == kWarps) {
-    const int step = p.cluster ? gridDim.x / p.parts : gridDim.x;
-    long long at = (long long)(p.cluster ? blockIdx.x / p.parts : blockIdx.x) - step;
-    for (int turn = -1;; ++turn) {  // while row `turn` streams, the next one is prepared
-      if (turn >= 0 && lessons[turn % 3].at < 0) break;
-      typename Op::Lesson& l = lessons[(turn + 1) % 3];
-      op.before(turn + 1, lessons);
-      __syncwarp();
-      if (lane == 0) l.zero = false;
+    long long at = (long long)(blockIdx.x / p.parts) - step;
+    auto make = [&](int n) {  // lesson n - 4 has been read by all, lesson n - 2 has been answered
+      typename Op::Lesson& l = lessons[n & 3];
+      op.before(n, lessons);
       do at += step;
-      while (at < items && !op.prepare(l, at));
-      if (lane == 0) l.at = at < items ? at : -1;
+      while (at < p.rows && !op.prepare(l, at));
+      if (lane == 0) l.at = at < p.rows ? at : -1;
       __syncwarp();
-      op.after(turn + 1, lessons);
+      op.after(n, lessons);
       __syncwarp();
-      bar_row();
+      if (lane == 0) mbar_arrive(&pipe.posted[n & 3]);
+    };
+    make(0);
+    make(1);
+    for (int n = 0; lessons[n & 3].at >= 0; ++n) {
+      if (!wait(&pipe.summed[n & 3], n)) break;
+      op.answer(n, lessons[n & 3], pipe.red[n & 3]);
+      __syncwarp();
+      if (Op::AGAIN && lane == 0) mbar_arrive(&pipe.answered[n & 3]);
+      make(n + 2);
     }
   } else {
-    bar_row();
-    for (int turn = 0;; ++turn) {
-      const typename Op::Lesson& l = lessons[turn % 3];
+    auto again = [&](int n) {
+      if (!wait(&pipe.answered[n & 3], n)) return false;
+      const typename Op::Lesson& l = lessons[n & 3];
+      const Range<T> r = range_of<T>(p, l.at, rank);
+      op.again(l, r, Inner(r));
+      return true;
+    };
+    for (int n = 0;; ++n) {
+      bool posted = wait(&pipe.posted[n & 3], n);
+      if constexpr (Op::MEETS) posted = all_stream(posted);  // none stays behind at a barrier of the others
+      if (!posted) break;
+      const typename Op::Lesson& l = lessons[n & 3];
+      if (l.at >= 0) {
+        const Range<T> r = range_of<T>(p, l.at, rank);
+        op.stream(n, l, r, Inner(r), pipe.red[n & 3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pipe.summed[n & 3]);
+      }
+      if (Op::AGAIN && n > 0 && !again(n - 1)) break;
       if (l.at < 0) break;
-      const Range<T> r = range_of<T>(p, l.at);
-      const Inner in(r);
-      op.stream(turn, l, r, in);
-      bar_row();
-      op.finish(turn, l, r, in);
     }
   }
+  __syncthreads();
+  // The next kernel's CTAs come now: those that come while others of this one still run gather where rows happen to end first, and then share
+  // an SM among more rows than elsewhere (2220 x 100000 bf16: 110 us for 85).
+  grid_dependency_launch();
   if (cluster) {  // no peer sends any more, and what they have sent is there unless a wait ran out
-    __syncthreads();
     cluster_arrive_relaxed();
     cluster_wait();
     let_copies_land(&meeting->abort);
@@ -643,48 +657,103 @@ struct Logprobs : Rows {
   int* top_ids;
 };
 struct LogprobsLesson {
-  long long at, token;
+  long long at;
+  int token;
   float x;  // the token's logit
-  bool zero;
 };
 struct Lists {  // of the parts, in the first CTA of a row
   float2 entry[2][kMaxCluster * kMaxTop];
 };
 
-template <typename T, bool TOP>
-struct LogprobsOp {
+// A warp writes a row's results from its (maximum, s, w).  token: of the row, or -1 for one out of range; x: its logit.
+__device__ __forceinline__ void write_results(const Logprobs& p, long long row, int token, float x, float3 sum) {
+  if ((threadIdx.x & 31) != 0) return;
+  const float log_sum = logf(sum.y);
+  if (p.lse) p.lse[row] = sum.x / p.temperature + log_sum;
+  if (p.entropy) p.entropy[row] = log_sum - kLn2 * (sum.z / sum.y);
+  if (p.logprobs) {
+    if (token < 0) atomicMax(p.status, DEV_BAD_INDEX);
+    p.logprobs[row] = token < 0 ? NAN : (x - sum.x) / p.temperature - log_sum;
+  }
+}
+// Token of a row: 0 for padding, -1 when it is out of range (or there are no tokens).
+__device__ __forceinline__ int token_of(const Logprobs& p, long long row) {
+  if (!p.tokens) return -1;
+  const long long t = load_id(p.tokens, row, p.token_bits);
+  return t < 0 || t > p.n ? -1 : (int)t;
+}
+__device__ __forceinline__ void write_padding(const Logprobs& p, long long row) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    if (p.logprobs) p.logprobs[row] = 0.f;
+    if (p.entropy) p.entropy[row] = 0.f;
+    if (p.lse) p.lse[row] = 0.f;
+  }
+  if (lane < p.top) {
+    p.top_logprobs[row * p.top + lane] = 0.f;
+    p.top_ids[row * p.top + lane] = 0;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kPlainPerSm) logprobs_kernel(const __grid_constant__ Logprobs p) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const Items items(p);
+  int tokens = 0;  // lane i: token of the i-th item of a batch of 32, and its logit
+  float logits = 0.f;
+  int n = 0;
+  for (long long item = items.at; item < items.end; item += items.step, ++n) {
+    if ((n & 31) == 0) {
+      const long long mine = item + lane * items.step, row = items.row(mine);
+      tokens = mine < items.end ? token_of(p, row) : 0;
+      logits = tokens > 0 ? to_float((static_cast<const T*>(p.x) + row * p.ld)[tokens - 1]) : 0.f;
+    }
+    const long long row = items.row(item);
+    const int part = (int)(item - row * p.parts), token = __shfl_sync(0xffffffffu, tokens, n & 31);
+    const float x = __shfl_sync(0xffffffffu, logits, n & 31);
+    if (token == 0) {
+      if (part == 0) write_padding(p, row);
+      continue;
+    }
+    const Range<T> r = range_of<T>(p, row, part);
+    const Inner in(r);
+    const int edge = edge_index(r, in, lane);
+    const float at_edge = edge >= 0 ? to_float(r.src[edge]) : 0.f;
+    Sums<T, true> sums;
+    each_tile<T, false, 1>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
+    if (edge >= 0) sums.add_one(at_edge, p.c);
+    __syncwarp();
+    float3 sum = sums.over_warp(p.c);
+    if (join_records(p, row, part, sum)) write_results(p, row, token, x, sum);
+  }
+  grid_dependency_launch();
+}
+
+// With alternatives the eight warps meet at barriers of their own, for the thresholds of the list.
+template <typename T>
+struct TopOp {
   using Lesson = LogprobsLesson;
+  static constexpr bool AGAIN = false, MEETS = true;
   const Logprobs& p;
   Best& best;
   Lists& lists;
-  float (&red)[2][3][kWarps];
   Meeting& meeting;
   float theta;
 
   __device__ __forceinline__ void before(int, const Lesson*) {}
   __device__ __forceinline__ void after(int, const Lesson*) {}
   __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
-    const int lane = threadIdx.x & 31;
-    const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
-    if (token != 0) {
-      if (lane == 0) {
-        l.token = token;
-        l.x = token > 0 && token <= p.n ? to_float((static_cast<const T*>(p.x) + row * p.ld)[token - 1]) : 0.f;
-      }
-      return true;
+    const int token = token_of(p, row);
+    if (token == 0) {
+      if (p.parts == 1 || cluster_ctarank() == 0) write_padding(p, row);
+      return false;
     }
-    if (p.parts == 1 || cluster_ctarank() == 0) {
-      if (lane == 0) {
-        if (p.logprobs) p.logprobs[row] = 0.f;
-        if (p.entropy) p.entropy[row] = 0.f;
-        if (p.lse) p.lse[row] = 0.f;
-      }
-      if (TOP && lane < p.top) {
-        p.top_logprobs[row * p.top + lane] = 0.f;
-        p.top_ids[row * p.top + lane] = 0;
-      }
+    if ((threadIdx.x & 31) == 0) {
+      l.token = token;
+      l.x = token > 0 ? to_float((static_cast<const T*>(p.x) + row * p.ld)[token - 1]) : 0.f;
     }
-    return false;
+    return true;
   }
 
   __device__ __forceinline__ void list(float x, int index) {
@@ -696,151 +765,124 @@ struct LogprobsOp {
       }
     }
   }
-  __device__ __forceinline__ void stream(int turn, const Lesson&, const Range<T>& r, const Inner& in) {
+  __device__ __forceinline__ void stream(int n, const Lesson& l, const Range<T>& r, const Inner& in, float (&red)[3][kWarps]) {
     constexpr int V = Range<T>::V;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, edge = edge_index(r, in, tid);
     const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
-    Sums<T> sums;
-    if constexpr (TOP) {
-      if (tid == 0) best.count = 0;  // ahead of the barriers of the first threshold
-      theta = -INFINITY;
-      if (edge >= 0 && tid < 8) sums.add_one(x, p.c);
-    }
+    Sums<T, true> sums;
+    if (tid == 0) best.count = 0;  // ahead of the barriers of the first threshold
+    theta = -INFINITY;
+    if (edge >= 0 && tid < 8) sums.add_one(x, p.c);
     int tile = 0;
 #pragma unroll 1
-    for (int v = in.a; v < in.b || (TOP && tile == 0); v += kTile, ++tile) {
+    for (int v = in.a; v < in.b || tile == 0; v += kTile, ++tile) {
       uint4 q[kUnroll];
-      float most = -INFINITY;
-      if (v < in.b) {
-        load_tile(q, r, in, v);
-        most = sums.add(q, p.c);
-      }
-      if constexpr (TOP) {
-        if (tile == 0) {
-          theta = group_threshold(word_max<T>(sums.top), p.top, best);
-          if (edge >= 0 && tid < 8) list(x, edge);
-        }
-        if (most > theta) {
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u) {
-            float f[V];
-            unpack_row<T>(q[u], f);
-            const int e0 = (v + u * kThreads + tid) * V - r.off;
-#pragma unroll
-            for (int i = 0; i < V; ++i) list(f[i], e0 + i);
-          }
-        }
-        if (tile > 0 && (tile & (tile + 1)) == 0 && v + kTile < in.b) theta = group_threshold(word_max<T>(sums.top), p.top, best);
+      for (int u = 0; u < kUnroll; ++u) q[u] = v + u * kThreads + tid < in.b ? __ldcs(r.at(v) + u * kThreads + tid) : empty_row_vec<T>();
+      const float most = sums.add(q, p.c);
+      if (tile == 0) {
+        theta = group_threshold(word_max<T>(sums.top), p.top, best);
+        if (edge >= 0 && tid < 8) list(x, edge);
       }
+      if (most > theta) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          float f[V];
+          unpack_row<T>(q[u], f);
+          const int e0 = (v + u * kThreads + tid) * V - r.off;
+#pragma unroll
+          for (int i = 0; i < V; ++i) list(f[i], e0 + i);
+        }
+      }
+      if (tile > 0 && (tile & (tile + 1)) == 0 && v + kTile < in.b) theta = group_threshold(word_max<T>(sums.top), p.top, best);
     }
-    if (edge >= 0 && (!TOP || tid >= 8)) {
+    if (edge >= 0 && tid >= 8) {
       sums.add_one(x, p.c);
-      if constexpr (TOP) list(x, edge);
+      list(x, edge);
     }
     const float3 of_warp = sums.over_warp(p.c);
     if (lane == 0) {
-      red[turn & 1][0][warp] = of_warp.x;
-      red[turn & 1][1][warp] = of_warp.y;
-      red[turn & 1][2][warp] = of_warp.z;
+      red[0][warp] = of_warp.x;
+      red[1][warp] = of_warp.y;
+      red[2][warp] = of_warp.z;
     }
-  }
-  __device__ __forceinline__ void finish(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float(&mine)[3][kWarps] = red[turn & 1];
-    const long long row = l.at;
-    float3 sum = make_float3(red_max(mine[0]), 0.f, 0.f);
-    if (!Sums<T>::plain(sum.x)) {
-      sum = slow_sums(r, nullptr, 0, p.c, mine);
-    } else if (warp == 0) {
-      const float2 s = join<kWarps>((mine[0][lane & 7] - sum.x) * p.c, mine[1][lane & 7], mine[2][lane & 7]);
-      sum = make_float3(sum.x, s.x, s.y);
+    bar_stream();
+    int count = best.count;
+    if (count > kCand) {
+      count = radix_list(r, p.top, best);
+    } else if (count < p.top) {
+      // theta of the first tile: with fewer than k above it, it is also the last one
+      Range<T> first = r;
+      first.v1 = min(r.v1, in.a + kTile);
+      count = append_equal(first, theta, count, p.top - count, best);
     }
-    if constexpr (TOP) {
-      int n = best.count;
-      if (n > kCand) {
-        n = radix_list(r, p.top, best);
-      } else if (n < p.top) {
-        // theta of the first tile: with fewer than k above it, it is also the last one
-        Range<T> first = r;
-        first.v1 = min(r.v1, in.a + kTile);
-        n = append_equal(first, theta, n, p.top - n, best);
-      }
-      select_list(n, p.top, best);
-    }
+    select_list(count, p.top, best);
+    float3 sum = make_float3(0.f, 0.f, 0.f);
+    const int rank = p.parts > 1 ? cluster_ctarank() : 0;
+    if (warp == 0 || (p.parts > 1 && rank == 0)) sum = join_warps<kWarps>(red, p.c);
     if (p.parts > 1) {
-      const int rank = cluster_ctarank();
       if (warp == 0) {
-        send_part(p, meeting, turn, sum, TOP && rank == 0 ? p.parts * p.top * (uint32_t)sizeof(float2) : 0);
-        if (TOP && lane < p.top && !meeting.abort)
-          send_to_cta(&lists.entry[turn & 1][rank * p.top + lane], best.out_value[lane], __int_as_float(best.out_index[lane]),
-                      &meeting.bar[turn & 1], 0);
+        send_part(p, meeting, n, sum, rank == 0 ? p.parts * p.top * (uint32_t)sizeof(float2) : 0);
+        if (lane < p.top && !meeting.abort)
+          send_to_cta(&lists.entry[n & 1][rank * p.top + lane], best.out_value[lane], __int_as_float(best.out_index[lane]),
+                      &meeting.bar[n & 1], 0);
       }
-      if (warp == 0 || (TOP && rank == 0)) {
-        await_parts(p, meeting, turn);
-        sum = join_parts(p, meeting, turn);
+      if (warp == 0 || rank == 0) {
+        await_parts(p, meeting, n);
+        sum = join_parts(p, meeting, n);
       }
       if (rank != 0) return;
-      if constexpr (TOP) {
-        if (tid == 0) best.count = 0;
-        bar_stream();
-        for (int i = tid; i < p.parts * p.top; i += kThreads) {
-          const float2 e = lists.entry[turn & 1][i];
-          const int id = __float_as_int(e.y);
-          if (id >= 0) {
-            const int pos = atomicAdd(&best.count, 1);
-            best.value[pos] = e.x;
-            best.index[pos] = id;
-          }
+      if (tid == 0) best.count = 0;
+      bar_stream();
+      for (int i = tid; i < p.parts * p.top; i += kThreads) {
+        const float2 e = lists.entry[n & 1][i];
+        const int id = __float_as_int(e.y);
+        if (id >= 0) {
+          const int pos = atomicAdd(&best.count, 1);
+          best.value[pos] = e.x;
+          best.index[pos] = id;
         }
-        bar_stream();
-        select_list(best.count, p.top, best);
       }
+      bar_stream();
+      select_list(best.count, p.top, best);
     }
     if (warp == 0) {
       const float log_sum = logf(sum.y);
-      if (lane == 0) {
-        if (p.lse) p.lse[row] = sum.x / p.temperature + log_sum;
-        if (p.entropy) p.entropy[row] = log_sum - kLn2 * (sum.z / sum.y);
-        if (p.logprobs) {
-          const bool bad = l.token < 0 || l.token > p.n;
-          if (bad) atomicMax(p.status, DEV_BAD_INDEX);
-          p.logprobs[row] = bad ? NAN : (l.x - sum.x) / p.temperature - log_sum;
-        }
-      }
-      if (TOP && lane < p.top) {
+      write_results(p, l.at, l.token, l.x, sum);
+      if (lane < p.top) {
         const int id = best.out_index[lane];
-        p.top_logprobs[row * p.top + lane] = id >= 0 ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
-        p.top_ids[row * p.top + lane] = id + 1;
+        p.top_logprobs[l.at * p.top + lane] = id >= 0 ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
+        p.top_ids[l.at * p.top + lane] = id + 1;
       }
     }
   }
+  __device__ __forceinline__ void answer(int, const Lesson&, const float (&)[3][kWarps]) {}
+  __device__ __forceinline__ void again(const Lesson&, const Range<T>&, const Inner&) {}
 };
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kAllThreads, kLogprobsPerSm<TOP>) logprobs_kernel(const __grid_constant__ Logprobs p) {
+template <typename T>
+__global__ void __launch_bounds__(kAllThreads, kTopPerSm) top_logprobs_kernel(const __grid_constant__ Logprobs p) {
+  __shared__ Pipe pipe;
   __shared__ Meeting meeting;
-  __shared__ LogprobsLesson lessons[3];
-  __shared__ float red[2][3][kWarps];
-  __shared__ typename std::conditional<TOP, Best, int>::type best;
-  __shared__ typename std::conditional<TOP, Lists, int>::type lists;
-  LogprobsOp<T, TOP> op{p, reinterpret_cast<Best&>(best), reinterpret_cast<Lists&>(lists), red, meeting, 0.f};
-  run_rows<T>(p, op, lessons, &meeting);
+  __shared__ LogprobsLesson lessons[4];
+  __shared__ Best best;
+  __shared__ Lists lists;
+  TopOp<T> op{p, best, lists, meeting, 0.f};
+  run_rows<T>(p, op, lessons, pipe, &meeting);
 }
 
 // ------------------------------------------------------------------ gradients
-// d = p (a + b t), t = log2 p, over a range.
-template <typename T, bool ENTROPY>
+// d = p (a + b t), t = log2 p, over a range, by W warps.
+template <typename T, bool ENTROPY, int W>
 __device__ __forceinline__ void stream_gradient(const Range<T>& r, const Inner& in, T* dst, float c, float lse2, float a, float b) {
-  const int tid = threadIdx.x, edge = edge_index(r, in, tid);
+  const int tid = threadIdx.x % (W * 32), edge = edge_index(r, in, tid);
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
   const Pair cc = pair(c, c), minus = pair(-lse2, -lse2), aa = pair(a, a), bb = pair(b, b);
   const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
-#pragma unroll 1
-  for (int v = in.a; v < in.b; v += kTile) {
-    uint4 q[kUnroll];
-    load_tile(q, r, in, v);
+  each_tile<T, false, W>(r, in, [&](auto& q, int v) {
+    constexpr int N = sizeof(q) / sizeof(uint4);
     uint4* to = reinterpret_cast<uint4*>(dst - r.off) + v + tid;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < N; ++u) {
       uint32_t word[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
       for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
@@ -853,23 +895,23 @@ __device__ __forceinline__ void stream_gradient(const Range<T>& r, const Inner& 
         }
       }
       const uint4 d = make_uint4(word[0], word[1], word[2], word[3]);
-      if (v + u * kThreads + tid < in.b) {
-        if (aligned) __stcs(to + u * kThreads, d);
-        else store_edge<T>(dst, r.off, r.n, v + u * kThreads + tid, d);
+      if (N > 1 || v + tid < in.b) {
+        if (aligned) __stcs(to + u * W * 32, d);
+        else store_edge<T>(dst, r.off, r.n, v + u * W * 32 + tid, d);
       }
     }
-  }
+  });
   if (edge >= 0) {
     const float t = fmaf(x, c, -lse2), e = ex2_approx_ftz(t);
     dst[edge] = from_float<T>(ENTROPY ? e * fmaf(b, fmaxf(t, kLowest), a) : e * a);
   }
 }
-// Zeros over a range, by the streaming threads.
-template <typename T>
+// Zeros over a range, by W warps.
+template <typename T, int W>
 __device__ __noinline__ void stream_zeros(const Range<T>& r, T* dst) {
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int v = r.v0 + threadIdx.x; v < r.v1; v += kThreads) {
+  for (int v = r.v0 + threadIdx.x % (W * 32); v < r.v1; v += W * 32) {
     if (aligned && r.inside(v, 1)) __stcs(reinterpret_cast<uint4*>(dst - r.off) + v, zero);
     else store_edge<T>(dst, r.off, r.n, v, zero);
   }
@@ -881,21 +923,26 @@ __device__ __forceinline__ int in_range(const Range<T>& r, long long id) {
   const long long v = (id - 1 + r.off) / Range<T>::V;
   return id > 0 && v >= r.v0 && v < r.v1 ? (int)id : 0;
 }
-// Gradient at what a teacher lists: g (all p - sum of the q of this id), once per id.  Thread j has entry j; 0: unused or in another part.
-template <typename T>
-__device__ __forceinline__ void patch_entries(const Range<T>& r, T* dst, const int* entry, const float* q, const float* x, int entries, float c,
-                                              float lse2, float g, float all) {
-  const int j = threadIdx.x;
-  if (j >= entries) return;
-  const int id = entry[j];
-  if (!in_range(r, id)) return;
-  float sum = 0.f;
-  for (int i = 0; i < entries; ++i)
-    if (entry[i] == id) {
-      if (i < j) return;
-      sum += q[i];
-    }
-  dst[id - 1] = from_float<T>(g * (all * ex2_approx_ftz(fmaf(x[j], c, -lse2)) - sum));
+// Calls f(id, j, sum of the weights of this id) for the entries of this range that the calling warp, of W, has streamed, once per id: the
+// lane writes over what the warp has written there.
+template <int W, typename T, typename F>
+__device__ __forceinline__ void patch_entries(const Range<T>& r, const Inner& in, const int* entry, const float* weight, int entries, F f) {
+  __syncwarp();
+  const int warp = threadIdx.x >> 5;
+  for (int j = threadIdx.x & 31; j < entries; j += 32) {
+    const int id = in_range(r, entry[j]);
+    if (id == 0) continue;
+    const int v = (id - 1 + r.off) / Range<T>::V;
+    if (W > 1 && (v < in.a || v >= in.b ? 0 : (v - in.a) % kThreads >> 5) != warp) continue;
+    float sum = 0.f;
+    bool first = true;
+    for (int i = 0; i < entries; ++i)
+      if (entry[i] == id) {
+        first &= i >= j;
+        sum += weight[i];
+      }
+    if (first) f(id, j, sum);
+  }
 }
 
 // ------------------------------------------------------------------ distillation, forward, and the gradient at once
@@ -924,228 +971,284 @@ __device__ __forceinline__ double max_lanes(double v) {
 }
 
 // The teacher's side of a row, in f64: what its list leaves over is a difference from one.
-struct DistillLesson {
-  long long at;
+struct Teacher {
   double terms, all, norm;   // sum q (log q - z), sum q
   float listed_max, listed;  // what the student gives to the listed ids, each once: maximum, sum of powers relative to it
-  float g;                   // upstream gradient / temperature
-  bool zero;
   int entry[kMaxEntries];    // ids, 0: unused
   float q[kMaxEntries], x[kMaxEntries];
 };
+enum Row { PADDING, BAD, LIVE };
 
-// HOLES: teacher_lse is given; what the teacher lists is left out of the row's sum by a bit per element and added apart, since the rest's
-// probability from a difference would lose all digits where it is small.  GRAD: the row is read a second time, out of L2, for the
-// gradient.
-template <typename T, bool GRAD, bool HOLES>
+// Whether a row has used entries, and ids in range only; a warp.
+__device__ __forceinline__ Row look_at(const Distill& p, long long row) {
+  bool used = false, bad = false;
+  for (int j = threadIdx.x & 31; j < p.entries; j += 32) {
+    const long long id = load_id(p.ids, row * p.entries + j, p.id_bits);
+    used |= id != 0;
+    bad |= id < 0 || id > p.n;
+  }
+  used = __any_sync(0xffffffffu, used);
+  return __any_sync(0xffffffffu, bad) ? BAD : used ? LIVE : PADDING;
+}
+__device__ __forceinline__ void write_unused(const Distill& p, long long row, Row kind) {
+  if ((threadIdx.x & 31) != 0) return;
+  if (kind == BAD) atomicMax(p.status, DEV_BAD_INDEX);
+  p.loss[row] = kind == BAD ? NAN : 0.f;
+  reinterpret_cast<float4*>(p.saved)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+// The teacher's side of a live row; a warp.  power: kMaxEntries of its own.
+template <typename T, bool TAIL>
+__device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t, double* power) {
+  const int lane = threadIdx.x & 31;
+  const T* src = static_cast<const T*>(p.x) + row * p.ld;
+  double most = -INFINITY;
+  float x_most = -INFINITY;
+  __syncwarp();
+  for (int j = lane; j < p.entries; j += 32) {
+    const int id = (int)load_id(p.ids, row * p.entries + j, p.id_bits);
+    const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
+    const float x = id ? to_float(src[id - 1]) : -INFINITY;
+    t.entry[j] = id;
+    t.x[j] = x;
+    power[j] = u;
+    x_most = fmaxf(x_most, x);
+    if (id) most = fmax(most, u);
+  }
+  double norm;
+  if constexpr (TAIL) {
+    norm = p.teacher_lse[row];
+  } else {
+    most = max_lanes(most);
+    double sum = 0;
+    for (int j = lane; j < p.entries; j += 32)
+      if (t.entry[j]) sum += exp(power[j] - most);
+    norm = most + log(sum_lanes(sum));
+  }
+  double all = 0, terms = 0;
+  for (int j = lane; j < p.entries; j += 32) {
+    if (t.entry[j] == 0) continue;
+    const double log_q = power[j] - norm, q = exp(log_q);
+    if (q != 0) terms += q * (log_q - (double)t.x[j] / (double)p.temperature);
+    all += q;
+    t.q[j] = (float)q;
+  }
+  all = sum_lanes(all);
+  terms = sum_lanes(terms);
+  float listed = 0.f;
+  if constexpr (TAIL) {
+    __syncwarp();
+    x_most = fmaxf(warp_max(x_most), -FLT_MAX);
+    for (int j = lane; j < p.entries; j += 32) {
+      const int id = t.entry[j];
+      bool again = id == 0;
+      for (int i = 0; i < j; ++i) again |= t.entry[i] == id;
+      if (!again) listed += ex2_approx_ftz((t.x[j] - x_most) * p.c);
+    }
+    listed = warp_sum(listed);
+  }
+  if (lane == 0) {
+    t.terms = terms;
+    t.all = all;
+    t.norm = norm;
+    t.listed_max = x_most;
+    t.listed = listed;
+  }
+  __syncwarp();
+}
+// What the gradient needs of a row: where the teacher lists nothing it is p a, else g (whole p - q).
+struct Answer {
+  float lse2, a, g, whole;
+};
+// Loss and saved values of a row from (maximum, s), which with TAIL leave out what the teacher lists; one lane.
+template <bool TAIL>
+__device__ __noinline__ Answer close_row(const Distill& p, long long row, const Teacher& t, float3 sum, bool write) {
+  float total = sum.y, rest = sum.y, whole = 1.f, outside = 1.f;
+  double left = 0;
+  if constexpr (TAIL) {
+    const float both = fmaxf(sum.x, t.listed_max);
+    rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
+    total = rest + t.listed * ex2_approx_ftz((t.listed_max - both) * p.c);
+    sum.x = both;
+    left = t.all > 1 ? 0 : 1 - t.all;
+    whole = (float)(t.all + left);
+    outside = rest == 0.f ? whole : (float)(t.all + left - left * ((double)total / (double)rest));
+  }
+  if (write) {
+    const double log_total = log((double)total), lse = (double)sum.x / (double)p.temperature + log_total;
+    double loss = t.terms + t.all * lse;
+    if (left != 0) loss += left * (log(left) - (log((double)rest) - log_total));
+    // (lse, outside, whole, norm) with teacher_lse; else outside and whole are 1, and the norm keeps 48 bits: (lse, low part, -1, norm)
+    const float high = (float)t.norm;
+    p.loss[row] = (float)loss;
+    reinterpret_cast<float4*>(p.saved)[row] = TAIL ? make_float4((float)lse, outside, whole, high)
+                                                   : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
+  }
+  Answer answer;
+  int k;  // the logarithm's whole part joins the reference before it is rounded
+  const float m = frexpf(total, &k);
+  answer.lse2 = fmaf(sum.x, p.c, (float)k) + log2f(m);
+  answer.g = p.d_loss ? p.d_loss[row] / p.temperature : 0.f;
+  answer.a = answer.g * outside;
+  answer.whole = whole;
+  return answer;
+}
+// TAIL: teacher_lse is given, and what the teacher lists is left out of the row's sum, by a bit per element, and added apart: the rest's
+// probability from a difference would lose all digits where it is small.  Sets or clears the bits of a part's entries; a warp.
+template <typename T>
+__device__ __forceinline__ void punch(const Range<T>& r, const int* entry, int entries, unsigned* bits, bool set) {
+  for (int j = threadIdx.x & 31; j < entries; j += 32) {
+    const int id = in_range(r, entry[j]);
+    if (id == 0) continue;
+    const int e = id - 1 + r.off - r.v0 * Range<T>::V;
+    if (set) atomicOr(bits + (e >> 5), 1u << (e & 31));
+    else bits[e >> 5] = 0;
+  }
+  __syncwarp();
+}
+// A range's elements but for those with a bit, by W warps.
+template <typename T, bool KEEP, bool TAIL, int W>
+__device__ __forceinline__ float3 sum_range(const Range<T>& r, const unsigned* bits, float c) {
+  const Inner in(r);
+  const int tid = threadIdx.x % (W * 32), edge = edge_index(r, in, tid);
+  const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
+  Sums<T, false> sums;
+  each_tile<T, KEEP, W>(r, in, [&](auto& q, int v) {
+    if constexpr (TAIL) {
+#pragma unroll
+      for (int u = 0; u < (int)(sizeof(q) / sizeof(uint4)); ++u) {
+        const int of = v + u * W * 32 + tid;
+        const unsigned hole = of < in.b ? hole_bits<T>(bits, of - r.v0) : 0u;
+        if (hole) mask_holes<T>(q[u], hole);
+      }
+    }
+    (void)sums.add(q, c);
+  });
+  if (edge >= 0) {
+    const int e = edge + r.off - r.v0 * Range<T>::V;
+    if (!(TAIL && (bits[e >> 5] >> (e & 31) & 1))) sums.add_one(x, c);
+  }
+  __syncwarp();
+  return sums.over_warp(c);
+}
+
+// The loss alone: rows cut among warps.
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __grid_constant__ Distill p) {
+  extern __shared__ __align__(16) unsigned char store[];
+  __shared__ Teacher teachers[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Teacher& t = teachers[warp];
+  double* power = reinterpret_cast<double*>(store) + warp * kMaxEntries;
+  const int words = TAIL ? p.per * Range<T>::V / 32 : 0;  // per is a multiple of 32 vectors
+  unsigned* bits = reinterpret_cast<unsigned*>(store + sizeof(double) * kWarps * kMaxEntries) + warp * words;
+  for (int i = lane; i < words; i += 32) bits[i] = 0;
+  grid_dependency_wait();
+  __syncwarp();
+  const Items items(p);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item);
+    const int part = (int)(item - row * p.parts);
+    const Row kind = look_at(p, row);
+    if (kind != LIVE) {
+      if (part == 0) write_unused(p, row, kind);
+      continue;
+    }
+    const Range<T> r = range_of<T>(p, row, part);
+    if constexpr (TAIL) {
+      for (int j = lane; j < p.entries; j += 32) t.entry[j] = (int)load_id(p.ids, row * p.entries + j, p.id_bits);
+      punch(r, t.entry, p.entries, bits, true);
+    }
+    float3 sum = sum_range<T, false, TAIL, 1>(r, bits, p.c);
+    if constexpr (TAIL) punch(r, t.entry, p.entries, bits, false);
+    if (!join_records(p, row, part, sum)) continue;
+    learn<T, TAIL>(p, row, t, power);
+    if (lane == 0) (void)close_row<TAIL>(p, row, t, sum, true);
+    __syncwarp();
+  }
+  grid_dependency_launch();
+}
+
+// Loss and gradient at once: the row is read a second time, out of L2, for the gradient, while the clerk joins the sums of the row behind it.
+struct DistillLesson {
+  long long at;
+  bool zero;  // its gradient is 0 and its logits are not read
+  Answer answer;
+  Teacher teacher;
+};
+template <typename T, bool TAIL>
 struct DistillOp {
   using Lesson = DistillLesson;
-  static constexpr int V = Range<T>::V;
+  static constexpr bool AGAIN = true, MEETS = false;
   const Distill& p;
   double (&power)[kMaxEntries];  // the clerk's
-  float (&red)[2][3][kWarps];
-  unsigned* holes;  // two sets of hole_words
-  int hole_words;
+  unsigned* bits;                // two sets of `words`
+  int words;
   Meeting& meeting;
   int meetings;
 
+  __device__ __forceinline__ int rank() const { return p.parts > 1 ? (int)cluster_ctarank() : 0; }
   __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
-    const int lane = threadIdx.x & 31;
-    const T* src = static_cast<const T*>(p.x) + row * p.ld;
-    bool used = false, bad = false;
-    double most = -INFINITY;
-    for (int j = lane; j < p.entries; j += 32) {
-      const long long id = load_id(p.ids, row * p.entries + j, p.id_bits);
-      const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
-      const bool out = id < 0 || id > p.n;
-      bad |= out;
-      used |= id != 0;
-      l.entry[j] = out ? 0 : (int)id;
-      power[j] = u;
-      if (id) most = fmax(most, u);
-    }
-    used = __any_sync(0xffffffffu, used);
-    bad = __any_sync(0xffffffffu, bad);
-    if (!used || bad) {
-      if ((p.parts == 1 || cluster_ctarank() == 0) && lane == 0) {
-        if (bad) atomicMax(p.status, DEV_BAD_INDEX);
-        p.loss[row] = bad ? NAN : 0.f;
-        reinterpret_cast<float4*>(p.saved)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      if (GRAD && lane == 0) l.zero = true;
-      return GRAD;
-    }
-    float x_most = -INFINITY;
-    for (int j = lane; j < p.entries; j += 32) {
-      const int id = l.entry[j];
-      const float x = id ? to_float(src[id - 1]) : -INFINITY;
-      l.x[j] = x;
-      x_most = fmaxf(x_most, x);
-    }
-    double norm;
-    if constexpr (HOLES) {
-      norm = p.teacher_lse[row];
-    } else {
-      most = max_lanes(most);
-      double sum = 0;
-      for (int j = lane; j < p.entries; j += 32)
-        if (l.entry[j]) sum += exp(power[j] - most);
-      norm = most + log(sum_lanes(sum));
-    }
-    double all = 0, terms = 0;
-    for (int j = lane; j < p.entries; j += 32) {
-      if (l.entry[j] == 0) continue;
-      const double log_q = power[j] - norm, q = exp(log_q);
-      if (q != 0) terms += q * (log_q - (double)l.x[j] / (double)p.temperature);
-      all += q;
-      l.q[j] = (float)q;
-    }
-    all = sum_lanes(all);
-    terms = sum_lanes(terms);
-    float listed = 0.f;
-    if constexpr (HOLES) {
-      __syncwarp();
-      x_most = fmaxf(warp_max(x_most), -FLT_MAX);
-      for (int j = lane; j < p.entries; j += 32) {
-        const int id = l.entry[j];
-        bool again = id == 0;
-        for (int i = 0; i < j; ++i) again |= l.entry[i] == id;
-        if (!again) listed += ex2_approx_ftz((l.x[j] - x_most) * p.c);
-      }
-      listed = warp_sum(listed);
-    }
-    if (lane == 0) {
-      l.terms = terms;
-      l.all = all;
-      l.norm = norm;
-      l.listed_max = x_most;
-      l.listed = listed;
-      if constexpr (GRAD) l.g = p.d_loss[row] / p.temperature;
-    }
+    const Row kind = look_at(p, row);
+    if (kind != LIVE && rank() == 0) write_unused(p, row, kind);
+    if ((threadIdx.x & 31) == 0) l.zero = kind != LIVE;
+    if (kind == LIVE) learn<T, TAIL>(p, row, l.teacher, power);
     return true;
   }
-  // Sets or clears the bits of a lesson's entries in its part.
-  __device__ __forceinline__ void punch(const Lesson& l, unsigned* set, bool on) {
-    if (l.at < 0 || l.zero) return;
-    const Range<T> r = range_of<T>(p, l.at);
-    for (int j = threadIdx.x & 31; j < p.entries; j += 32) {
-      const int id = in_range(r, l.entry[j]);
-      if (id == 0) continue;
-      const long long e = (long long)id - 1 + r.off - (long long)r.v0 * V;
-      if (on) atomicOr(set + (e >> 5), 1u << (e & 31));
-      else set[e >> 5] = 0;
-    }
-    __syncwarp();
-  }
   // The row two before has been summed: its bits lie where the next row's go.
-  __device__ __forceinline__ void before(int turn, const Lesson* lessons) {
-    if constexpr (HOLES)
-      if (turn >= 2) punch(lessons[(turn + 1) % 3], holes + (turn & 1) * hole_words, false);
+  __device__ __forceinline__ void before(int n, const Lesson* lessons) {
+    if (TAIL && n >= 2) mark(lessons[(n - 2) & 3], n, false);
   }
-  __device__ __forceinline__ void after(int turn, const Lesson* lessons) {
-    if constexpr (HOLES) punch(lessons[turn % 3], holes + (turn & 1) * hole_words, true);
+  __device__ __forceinline__ void after(int n, const Lesson* lessons) {
+    if (TAIL) mark(lessons[n & 3], n, true);
   }
-
-  __device__ __forceinline__ void stream(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
-    if (GRAD && l.zero) return;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, edge = edge_index(r, in, tid);
-    const unsigned* mine = holes + (turn & 1) * hole_words;
-    float x = edge >= 0 ? to_float(r.src[edge]) : -INFINITY;
-    LeanSums<T> sums;
-#pragma unroll 1
-    for (int v = in.a; v < in.b; v += kTile) {
-      uint4 q[kUnroll];
-      load_tile<T, GRAD>(q, r, in, v);
-      if constexpr (HOLES)
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int of = v + u * kThreads + tid;
-          const unsigned bits = of < in.b ? hole_bits<T>(mine, of - r.v0) : 0u;
-          if (bits) mask_holes<T>(q[u], bits);
-        }
-      sums.add(q, p.c);
-    }
-    if (warp == 0 && in.head + in.tail > 0) {
-      if (HOLES && edge >= 0) {
-        const int e = edge + r.off - r.v0 * V;
-        if (mine[e >> 5] >> (e & 31) & 1) x = -INFINITY;
-      }
-      sums.add_one(x, p.c);
-    }
-    const float2 of_warp = sums.over_warp(p.c);
-    if (lane == 0) {
-      red[turn & 1][0][warp] = of_warp.x;
-      red[turn & 1][1][warp] = of_warp.y;
+  __device__ __forceinline__ void mark(const Lesson& l, int n, bool set) {
+    if (l.at >= 0 && !l.zero) punch(range_of<T>(p, l.at, rank()), l.teacher.entry, p.entries, bits + (n & 1) * words, set);
+  }
+  __device__ __forceinline__ void stream(int n, const Lesson& l, const Range<T>& r, const Inner&, float (&red)[3][kWarps]) {
+    if (l.zero) return;
+    const float3 sum = sum_range<T, true, TAIL, kWarps>(r, bits + (n & 1) * words, p.c);
+    if ((threadIdx.x & 31) == 0) {
+      red[0][threadIdx.x >> 5] = sum.x;
+      red[1][threadIdx.x >> 5] = sum.y;
+      red[2][threadIdx.x >> 5] = 0.f;
     }
   }
-  __device__ __forceinline__ void finish(int turn, const Lesson& l, const Range<T>& r, const Inner& in) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long row = l.at;
-    if (GRAD && l.zero) {
-      stream_zeros<T>(r, static_cast<T*>(p.dx) + row * p.ld_dx);
-      return;
-    }
-    float(&mine)[3][kWarps] = red[turn & 1];
-    float3 sum;
-    sum.x = red_max(mine[0]);
-    sum.y = join<kWarps>((mine[0][lane & 7] - sum.x) * p.c, mine[1][lane & 7], 0.f).x;
-    // A part of which nothing is left (all of it masked, or listed) counts as -inf, unless the row has no other.
-    const bool nothing = sum.x == -INFINITY && p.parts > 1;
-    if (!nothing && !(sum.y > 0.f && sum.y < INFINITY)) sum = slow_sums(r, l.entry, HOLES ? p.entries : 0, p.c, mine);
-    if (nothing) sum.y = 0.f;
+  __device__ __forceinline__ void answer(int, Lesson& l, const float (&red)[3][kWarps]) {
+    if (l.zero) return;
+    float3 sum = join_warps<kWarps>(red, p.c);
     if (p.parts > 1) {
       const int meet = meetings++;
-      if (warp == 0) send_part(p, meeting, meet, make_float3(sum.x, sum.y, 0.f), 0);
-      if (GRAD || warp == 0) {
-        await_parts(p, meeting, meet);
-        sum = join_parts(p, meeting, meet);
-      }
+      send_part(p, meeting, meet, sum, 0);
+      await_parts(p, meeting, meet);
+      sum = join_parts(p, meeting, meet);
     }
-    if (!GRAD && warp != 0) return;
-    float total = sum.y, rest = sum.y, all = 1.f, outside = 1.f;
-    if constexpr (HOLES) {
-      const float both = fmaxf(sum.x, l.listed_max);
-      rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
-      total = rest + l.listed * ex2_approx_ftz((l.listed_max - both) * p.c);
-      sum.x = both;
-      const double left = l.all > 1 ? 0 : 1 - l.all;
-      all = (float)(l.all + left);
-      outside = rest == 0.f ? all : (float)(l.all + left - left * ((double)total / (double)rest));
+    if ((threadIdx.x & 31) == 0) l.answer = close_row<TAIL>(p, l.at, l.teacher, sum, rank() == 0);
+  }
+  __device__ __forceinline__ void again(const Lesson& l, const Range<T>& r, const Inner& in) {
+    T* dst = static_cast<T*>(p.dx) + l.at * p.ld_dx;
+    if (l.zero) {
+      stream_zeros<T, kWarps>(r, dst);
+      return;
     }
-    if (tid == 0 && (p.parts == 1 || cluster_ctarank() == 0)) {
-      const double log_total = log((double)total), lse = (double)sum.x / (double)p.temperature + log_total;
-      double loss = l.terms + l.all * lse;
-      if constexpr (HOLES) {
-        const double left = l.all > 1 ? 0 : 1 - l.all;
-        if (left != 0) loss += left * (log(left) - (log((double)rest) - log_total));
-      }
-      // (lse, outside, all, norm) with teacher_lse; else outside and all are 1, and the norm keeps 48 bits: (lse, low part, -1, norm)
-      const float high = (float)l.norm;
-      p.loss[row] = (float)loss;
-      reinterpret_cast<float4*>(p.saved)[row] = HOLES ? make_float4((float)lse, outside, all, high)
-                                                      : make_float4((float)lse, (float)(l.norm - (double)high), -1.f, high);
-    }
-    if constexpr (GRAD) {
-      T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
-      int k;  // the logarithm's whole part joins the reference before it is rounded
-      const float m = frexpf(total, &k), lse2 = fmaf(sum.x, p.c, (float)k) + log2f(m);
-      stream_gradient<T, false>(r, in, dst, p.c, lse2, l.g * outside, 0.f);
-      bar_stream();
-      patch_entries<T>(r, dst, l.entry, l.q, l.x, p.entries, p.c, lse2, l.g, all);
-    }
+    const Answer a = l.answer;
+    stream_gradient<T, false, kWarps>(r, in, dst, p.c, a.lse2, a.a, 0.f);
+    patch_entries<kWarps>(r, in, l.teacher.entry, l.teacher.q, p.entries, [&](int id, int j, float q) {
+      dst[id - 1] = from_float<T>(a.g * (a.whole * ex2_approx_ftz(fmaf(l.teacher.x[j], p.c, -a.lse2)) - q));
+    });
   }
 };
-template <typename T, bool GRAD, bool HOLES>
-__global__ void __launch_bounds__(kAllThreads, kDistillPerSm) distill_kernel(const __grid_constant__ Distill p) {
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kAllThreads, kDistillPerSm) distill_both_kernel(const __grid_constant__ Distill p) {
+  extern __shared__ __align__(16) unsigned char store[];
+  __shared__ Pipe pipe;
   __shared__ Meeting meeting;
-  __shared__ DistillLesson lessons[3];
+  __shared__ DistillLesson lessons[4];
   __shared__ double power[kMaxEntries];
-  __shared__ float red[2][3][kWarps];
-  extern __shared__ unsigned holes[];  // two sets
-  const int hole_words = HOLES ? (p.per * Range<T>::V + 31) / 32 : 0;
-  for (int i = threadIdx.x; i < 2 * hole_words; i += kAllThreads) holes[i] = 0;
-  DistillOp<T, GRAD, HOLES> op{p, power, red, holes, hole_words, meeting, 0};
-  run_rows<T>(p, op, lessons, &meeting);
+  unsigned* bits = reinterpret_cast<unsigned*>(store);
+  const int words = TAIL ? p.per * Range<T>::V / 32 : 0;
+  for (int i = threadIdx.x; i < 2 * words; i += kAllThreads) bits[i] = 0;
+  DistillOp<T, TAIL> op{p, power, bits, words, meeting, 0};
+  run_rows<T>(p, op, lessons, pipe, &meeting);
 }
 
 // ------------------------------------------------------------------ backward
@@ -1165,111 +1268,84 @@ struct Backward : Rows {
   const float *saved, *d_loss;
 };
 
-// A row's gradient is p (a + b log2 p) but where an entry (an alternative, the token, what the teacher lists) meets it.
-template <int ENTRIES>
-struct BackwardLesson {
-  long long at;
-  float lse2, a, b, all, g;
-  int entries;
-  bool zero;
-  int entry[ENTRIES];
-  float weight[ENTRIES], x[ENTRIES];
-};
-
 // Gradient of the log probabilities, the entropy and the alternatives of a row:
 //   dx_v = 1/temperature [ sum of the gradients that meet at v - p_v (G + g_H (log p_v + H)) ],  G = the sum of all but g_H
-// and of the distillation loss (DISTILL): g/temperature p_v outside, or g/temperature (all p_v - q_v) where the teacher lists v.
+// and of the distillation loss (DISTILL): g/temperature p_v outside, or g/temperature (whole p_v - q_v) where the teacher lists v.
+// A warp takes a part of a row after another; the few places that a gradient meets directly are written behind the part's stream.
 template <typename T, bool DISTILL, bool ENTROPY>
-struct BackwardOp {
-  using Lesson = BackwardLesson<DISTILL ? kMaxEntries : kMaxTop + 1>;
-  const Backward& p;
-
-  __device__ __forceinline__ void before(int, const Lesson*) {}
-  __device__ __forceinline__ void after(int, const Lesson*) {}
-  // dx may be the logits themselves: the entries' logits are read before their row is streamed.
-  __device__ __forceinline__ void enter(Lesson& l, int j, long long id, float weight, const Range<T>& r) {
-    if (id < 0 || id > p.n) {
-      atomicMax(p.status, DEV_BAD_INDEX);
-      id = 0;
-    }
-    const int mine = in_range(r, id);
-    l.entry[j] = mine;
-    l.weight[j] = weight;
-    l.x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
-  }
-  __device__ __forceinline__ bool prepare(Lesson& l, long long item) {
-    const int lane = threadIdx.x & 31;
-    const long long row = row_of(p, item);
-    const Range<T> r = range_of<T>(p, item);
+__global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kernel(const __grid_constant__ Backward p) {
+  constexpr int kEntries = DISTILL ? kMaxEntries : kMaxTop + 1;
+  __shared__ int entries_of[kWarps][kEntries];
+  __shared__ float weights_of[kWarps][kEntries], logits_of[kWarps][kEntries];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int* entry = entries_of[warp];
+  float *weight = weights_of[warp], *x = logits_of[warp];
+  const Items items(p);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item);
+    const Range<T> r = range_of<T>(p, row, (int)(item - row * p.parts));
+    const Inner in(r);
+    T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
+    __syncwarp();
+    // dx may be the logits themselves: the entries' logits are read before the part is streamed
+    auto enter = [&](int j, long long id, float w) {
+      if (id < 0 || id > p.n) {
+        atomicMax(p.status, DEV_BAD_INDEX);
+        id = 0;
+      }
+      const int mine = in_range(r, id);
+      entry[j] = mine;
+      weight[j] = w;
+      x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
+    };
+    float lse2, a, b = 0.f, g = 0.f, whole = 1.f;
+    int entries;
     if constexpr (!DISTILL) {
       const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
       const bool bad = p.tokens && (token < 0 || token > p.n);
       if (token == 0 || bad) {
         if (bad && lane == 0) atomicMax(p.status, DEV_BAD_INDEX);
-        if (lane == 0) l.zero = true;
-        return true;
+        stream_zeros<T, 1>(r, dst);
+        continue;
       }
       const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
       const float gt = lane < p.top ? p.d_top[row * p.top + lane] : 0.f, all = g0 + warp_sum(gt);
-      if (lane < p.top) enter(l, lane, p.top_ids[row * p.top + lane], gt, r);
-      if (lane == 0) {
-        if (p.d_logprobs) enter(l, p.top, token, g0, r);
-        l.entries = p.top + (p.d_logprobs ? 1 : 0);
-        l.lse2 = p.lse[row] * kLog2e;
-        l.a = -(all + gh * h) / p.temperature;
-        l.b = -gh * kLn2 / p.temperature;
-      }
+      if (lane < p.top) enter(lane, p.top_ids[row * p.top + lane], gt);
+      if (lane == 0 && p.d_logprobs) enter(p.top, token, g0);
+      entries = p.top + (p.d_logprobs ? 1 : 0);
+      lse2 = p.lse[row] * kLog2e;
+      a = -(all + gh * h) / p.temperature;
+      b = -gh * kLn2 / p.temperature;
     } else {
       const float4 saved = reinterpret_cast<const float4*>(p.saved)[row];
       if (saved.z == 0.f) {
-        if (lane == 0) l.zero = true;
-        return true;
+        stream_zeros<T, 1>(r, dst);
+        continue;
       }
-      const bool whole = saved.z < 0.f;  // the teacher's list is all of its distribution
-      const double norm = (double)saved.w + (whole ? (double)saved.y : 0.);
-      for (int j = lane; j < p.entries; j += 32) {
-        const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
-        enter(l, j, load_id(p.ids, row * p.entries + j, p.id_bits), (float)exp(u - norm), r);
+      const bool list_is_all = saved.z < 0.f;  // of the teacher's distribution
+      const double norm = (double)saved.w + (list_is_all ? (double)saved.y : 0.);
+      entries = p.entries;
+      for (int j = lane; j < entries; j += 32) {
+        const long long id = load_id(p.ids, row * entries + j, p.id_bits);
+        float q = 0.f;
+        if (in_range(r, id))
+          q = (float)exp((double)load_value(p.values, row * entries + j, p.values_dtype) / (double)p.temperature - norm);
+        enter(j, id, q);
       }
-      if (lane == 0) {
-        l.g = p.d_loss[row] / p.temperature;
-        l.entries = p.entries;
-        l.lse2 = saved.x * kLog2e;
-        l.a = l.g * (whole ? 1.f : saved.y);
-        l.all = whole ? 1.f : saved.z;
-      }
+      g = p.d_loss[row] / p.temperature;
+      lse2 = saved.x * kLog2e;
+      a = g * (list_is_all ? 1.f : saved.y);
+      whole = list_is_all ? 1.f : saved.z;
     }
-    return true;
+    __syncwarp();
+    stream_gradient<T, ENTROPY, 1>(r, in, dst, p.c, lse2, a, b);
+    patch_entries<1>(r, in, entry, weight, entries, [&](int id, int j, float sum) {
+      const float t = fmaf(x[j], p.c, -lse2), e = ex2_approx_ftz(t);
+      dst[id - 1] = from_float<T>(DISTILL ? g * (whole * e - sum) : sum / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
+    });
   }
-  __device__ __forceinline__ void stream(int, const Lesson& l, const Range<T>& r, const Inner& in) {
-    T* dst = static_cast<T*>(p.dx) + row_of(p, l.at) * p.ld_dx;
-    if (l.zero) stream_zeros<T>(r, dst);
-    else stream_gradient<T, ENTROPY>(r, in, dst, p.c, l.lse2, l.a, l.b);
-  }
-  __device__ __forceinline__ void finish(int, const Lesson& l, const Range<T>& r, const Inner&) {
-    if (l.zero) return;
-    T* dst = static_cast<T*>(p.dx) + row_of(p, l.at) * p.ld_dx;
-    if constexpr (DISTILL) {
-      patch_entries<T>(r, dst, l.entry, l.weight, l.x, l.entries, p.c, l.lse2, l.g, l.all);
-    } else {
-      const int j = threadIdx.x;
-      if (j >= l.entries || l.entry[j] == 0) return;
-      float g = 0.f;
-      for (int i = 0; i < l.entries; ++i)
-        if (l.entry[i] == l.entry[j]) {
-          if (i < j) return;
-          g += l.weight[i];
-        }
-      const float t = fmaf(l.x[j], p.c, -l.lse2);
-      dst[l.entry[j] - 1] = from_float<T>(g / p.temperature + ex2_approx_ftz(t) * fmaf(l.b, fmaxf(t, kLowest), l.a));
-    }
-  }
-};
-template <typename T, bool DISTILL, bool ENTROPY>
-__global__ void __launch_bounds__(kAllThreads, kBackwardPerSm<DISTILL>) logits_backward_kernel(const __grid_constant__ Backward p) {
-  __shared__ typename BackwardOp<T, DISTILL, ENTROPY>::Lesson lessons[3];
-  BackwardOp<T, DISTILL, ENTROPY> op{p};
-  run_rows<T>(p, op, lessons, nullptr);
+  grid_dependency_launch();
 }
 
 // ------------------------------------------------------------------ host side
@@ -1332,7 +1408,7 @@ struct Cut {
 };
 template <auto KERNEL>
 Cut cut_rows(ctb_ctx* ctx, int64_t rows, int64_t row_bytes, int per_sm, int least, double ends) {
-  constexpr double kAlone = 20e3, kAll = 6500e3, kMeeting = 1.0;
+  constexpr double kAlone = 20e3, kAll = 6500e3, kMeeting = 2.5;
   Cut best = {0, 0};
   double best_time = 0;
   for (int C = 1; C <= kMaxCluster; C *= 2) {
@@ -1362,25 +1438,81 @@ void cut_into(Rows& p, int64_t nvec, int64_t parts) {
   p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
   p.parts = (int)parts;
 }
-// Launches a forward kernel.  holes: two bits of shared memory for each element of a part.
+// Rows cut among warps: into the parts for which rounds of parts take the least time.  A warp reads `alone` bytes per ns when nobody else reads
+// and shares what HBM gives otherwise, and a part costs `ends` besides (us); measured with 1 to 2220 rows of 50000 to 128000 elements.
+void cut_among_warps(Rows& p, int64_t nvec, int elem, int passes, int64_t places, int64_t most, double ends) {
+  const double alone = elem == 4 ? 5.1 : 3.5, all = 7600, bytes = (double)(passes * nvec) * 16e-3;  // of a row, in 1000
+  double best = 0;
+  int64_t parts = 1;
+  most = std::min({most, std::max<int64_t>(1, nvec / 128), std::max<int64_t>(1, 16 * places / std::max(1, p.rows))});  // 2 KB; 16 rounds
+  for (int64_t n = 1; n <= most; n = n < 64 ? n + 1 : n + n / 8) {
+    const int64_t items = p.rows * n, full = items / places, rest = items % places;
+    auto round = [&](int64_t active) { return bytes / (double)n * (1 / alone + (double)active / all) + ends; };
+    const double time = (double)full * round(places) + (rest ? round(rest) : 0) + 0.01 * (double)n;
+    if (n == 1 || time < best) {
+      best = time;
+      parts = n;
+    }
+  }
+  p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
+  p.parts = (int)((nvec + p.per - 1) / p.per);
+}
+// Parts that a row may have whose sums meet in scratch memory: as many as their records and counters have room for.
+int64_t most_parts(const Rows& p) {
+  if (p.rows > kTickets) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows));
+}
+
+// Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element, besides `fixed` bytes.
 template <auto KERNEL, typename T, typename P>
-int launch_forward(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool holes, double ends, const char* who) {
+int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, size_t fixed, bool bits, double ends, const char* who) {
+  const int64_t places = (int64_t)kPlainPerSm * ctx->sm_count * kWarps, nvec = vectors<T>(p);
+  auto go = [&] {
+    const size_t smem = fixed + (bits ? (size_t)kWarps * 4 * (p.per * (16 / sizeof(T)) / 32) : 0);
+    int per_sm = kPlainPerSm;
+    if (smem > 0) {
+      if (smem > 200 * 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
+      cudaError_t e = allow_smem(KERNEL, 200 * 1024);
+      if (e != cudaSuccess) return cuda_fail(e, who);
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, kThreads, smem);
+      per_sm = std::max(1, std::min(kPlainPerSm, per_sm));
+    }
+    const int64_t ctas = ((int64_t)p.rows * p.parts + kWarps - 1) / kWarps;
+    launch_kernel(KERNEL, (int)std::min<int64_t>(ctas, (int64_t)per_sm * ctx->sm_count), kThreads, smem, st, 0, p);
+    CTB_CHECK_LAUNCH(who);
+    return (int)CTB_OK;
+  };
+  cut_among_warps(p, nvec, sizeof(T), 1, places, most_parts(p), ends);
+  if (p.parts > 1) {
+    StreamScratch scratch(ctx, st);
+    if (scratch.data) {
+      p.records = reinterpret_cast<float4*>(scratch.data);
+      p.tickets = scratch.tickets;
+      return go();
+    }
+    cut_into(p, nvec, 1);
+  }
+  return go();
+}
+
+// Launches a kernel of run_rows.  bits: two sets of a bit per element of a part in shared memory.
+template <auto KERNEL, typename T, typename P>
+int launch_rows(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool bits, double ends, const char* who) {
   constexpr int V = 16 / (int)sizeof(T);
   const int64_t nvec = vectors<T>(p);
-  p.cluster = 1;
-  cudaError_t e = holes ? allow_smem(KERNEL, (kMostHoles + 1024) / 4) : cudaSuccess;
+  cudaError_t e = bits ? allow_smem(KERNEL, (kMostHoles + 1024) / 4) : cudaSuccess;
   if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return cuda_fail(e, who);
   int least = 1;
-  if (holes)
+  if (bits)
     while (least < kMaxCluster && nvec * V > (int64_t)least * kMostHoles) least *= 2;
   Cut cut = cut_rows<KERNEL>(ctx, p.rows, nvec * 16, per_sm, least, ends);
   if (cut.parts == 0) return fail(CTB_UNSUPPORTED, "%s: no room for a row's CTAs on this device", who);
   cut_into(p, nvec, cut.parts);
   size_t smem = 0;
-  if (holes) {  // more shared memory may leave room for fewer
+  if (bits) {  // more shared memory may leave room for fewer
     if ((int64_t)p.per * V > kMostHoles + 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, rows of %d elements are too long", who, p.n);
-    smem = 2 * 4 * (((size_t)p.per * V + 31) / 32);
+    smem = 2 * 4 * ((size_t)p.per * V / 32);
     int fit = 0;
     if (p.parts > 1) {
       fit = most_teams<KERNEL>(ctx, p.parts, per_sm, smem, false);
@@ -1397,22 +1529,24 @@ int launch_forward(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool holes, d
 
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
-  return p.top ? launch_forward<logprobs_kernel<T, true>, T>(ctx, st, p, kLogprobsPerSm<true>, false, 3.0, who)
-               : launch_forward<logprobs_kernel<T, false>, T>(ctx, st, p, kLogprobsPerSm<false>, false, 1.0, who);
+  if (p.top) return launch_rows<top_logprobs_kernel<T>, T>(ctx, st, p, kTopPerSm, false, 3.0, who);
+  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, 0, false, 3.0, who);
 }
-template <typename T, bool GRAD>
+template <typename T>
 int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* who) {
-  return p.teacher_lse ? launch_forward<distill_kernel<T, GRAD, true>, T>(ctx, st, p, kDistillPerSm, true, 2.5, who)
-                       : launch_forward<distill_kernel<T, GRAD, false>, T>(ctx, st, p, kDistillPerSm, false, 2.5, who);
+  constexpr size_t kPowers = sizeof(double) * kWarps * kMaxEntries;
+  if (p.dx)
+    return p.teacher_lse ? launch_rows<distill_both_kernel<T, true>, T>(ctx, st, p, kDistillPerSm, true, 2.5, who)
+                         : launch_rows<distill_both_kernel<T, false>, T>(ctx, st, p, kDistillPerSm, false, 2.5, who);
+  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, kPowers, true, 5.0, who)
+                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, kPowers, false, 5.0, who);
 }
 template <typename T, bool DISTILL>
 int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
   auto kernel = p.d_entropy ? logits_backward_kernel<T, DISTILL, !DISTILL> : logits_backward_kernel<T, DISTILL, false>;
-  // Parts have nothing to do with each other: of at most four tiles, or one where that brings work to more places.
-  const int64_t nvec = vectors<T>(p), places = (int64_t)kBackwardPerSm<DISTILL> * ctx->sm_count;
-  const int64_t tiles = (nvec + kTile - 1) / kTile, each = p.rows * tiles >= 16 * places ? 4 : 1;
-  cut_into(p, nvec, (tiles + each - 1) / each);
-  launch_kernel(kernel, (int)std::min<int64_t>((int64_t)p.rows * p.parts, places), kAllThreads, 0, st, 0, p);
+  const int64_t most = (int64_t)kBackwardPerSm * ctx->sm_count;
+  cut_among_warps(p, vectors<T>(p), sizeof(T), 2, most * kWarps, INT32_MAX, DISTILL ? 2.0 : 1.0);
+  launch_kernel(kernel, (int)std::min<int64_t>(((int64_t)p.rows * p.parts + kWarps - 1) / kWarps, most), kThreads, 0, st, 0, p);
   CTB_CHECK_LAUNCH(who);
   return CTB_OK;
 }
@@ -1526,8 +1660,7 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   p.teacher_lse = teacher_lse; p.loss = loss; p.saved = saved;
   p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d_logits) return by_type(dtype, [&](auto t) { return launch_distill<decltype(t), true>(ctx, st, p, who); });
-  return by_type(dtype, [&](auto t) { return launch_distill<decltype(t), false>(ctx, st, p, who); });
+  return by_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(ctx, st, p, who); });
 }
 
 extern "C" int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,

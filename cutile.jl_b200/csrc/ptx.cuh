@@ -125,6 +125,36 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   }
 }
 
+// The same for a warp that waits for long beside others that work: it looks (test_wait does not suspend) and sleeps in turn.  A suspended
+// try_wait holds up other warps' shuffles and shared-memory accesses: five shuffles of a streaming warp took 16000 clocks beside one.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_watch(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort) {
+  if (mbar_test(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 1;; ++i) {
+    __nanosleep(40);
+    if (mbar_test(bar, parity)) return true;
+    if ((i & 15u) == 0) {
+      if (*abort) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (status) atomicMax(status, code);
+        *abort = 1;
+        return false;
+      }
+    }
+  }
+}
+
 // End of a kernel whose roles share an abort flag, behind a barrier of the CTA: after an abort, copies that were requested and
 // that nobody waits for any more get 10 ms to land (they take microseconds) before the CTA gives its shared memory back.
 __device__ __forceinline__ void let_copies_land(const volatile int* abort) {
