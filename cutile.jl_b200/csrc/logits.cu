@@ -471,12 +471,12 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
 // records in their order and writes the results.  48 such warps on an SM keep 16-bit logits, whose exponentials take 70 % of the ex2
 // unit, as close to HBM's rate as a loop without rows; eight warps that meet at the end of every row left them at 78 %.
 constexpr int kMaxParts = 256;
-struct Items {  // of a warp
+struct Items {  // of a warp (or, with W = 8, of the warps of a CTA, which share a part's tiles)
   const Rows& p;
   long long at, step, end;
-  __device__ __forceinline__ explicit Items(const Rows& rows) : p(rows) {
-    at = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    step = (long long)gridDim.x * kWarps;
+  __device__ __forceinline__ explicit Items(const Rows& rows, int W = 1) : p(rows) {
+    at = W == 1 ? (long long)blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+    step = W == 1 ? (long long)gridDim.x * kWarps : gridDim.x;
     end = (long long)p.rows * p.parts;
   }
   __device__ __forceinline__ long long row(long long item) const { return p.parts == 1 ? item : item / p.parts; }
@@ -536,7 +536,8 @@ struct Pipe {
 //   stream(n, lesson, range, inner, red)    the streaming warps
 //   answer(n, lesson, red)          the clerk, when all warps have streamed
 //   MEETS                           the streaming warps meet at barriers of their own
-//   AGAIN, again(lesson, range, inner)      the streaming warps, once the row has been answered and the next row has been streamed
+//   close(lesson)                   the clerk, behind it
+//   AGAIN, again(lesson, range, inner)      the streaming warps, once the row has been answered
 template <typename T, typename Op>
 __device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Lesson* lessons, Pipe& pipe, Meeting* meeting) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -585,6 +586,8 @@ __device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Les
       op.answer(n, lessons[n & 3], pipe.red[n & 3]);
       __syncwarp();
       if (Op::AGAIN && lane == 0) mbar_arrive(&pipe.answered[n & 3]);
+      op.close(lessons[n & 3]);
+      __syncwarp();
       make(n + 2);
     }
   } else {
@@ -606,8 +609,8 @@ __device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Les
         __syncwarp();
         if (lane == 0) mbar_arrive(&pipe.summed[n & 3]);
       }
-      if (Op::AGAIN && n > 0 && !again(n - 1)) break;
       if (l.at < 0) break;
+      if (Op::AGAIN && !again(n)) break;
     }
   }
   __syncthreads();
@@ -857,6 +860,7 @@ struct TopOp {
     }
   }
   __device__ __forceinline__ void answer(int, const Lesson&, const float (&)[3][kWarps]) {}
+  __device__ __forceinline__ void close(const Lesson&) {}
   __device__ __forceinline__ void again(const Lesson&, const Range<T>&, const Inner&) {}
 };
 template <typename T>
@@ -952,6 +956,7 @@ struct Distill : Rows {
   const void* values;
   int values_dtype;
   const float* teacher_lse;
+  double per_temperature;  // 1 / temperature
   float *loss, *saved;
   // with the gradient
   const float* d_loss;
@@ -962,11 +967,6 @@ struct Distill : Rows {
 __device__ __forceinline__ double sum_lanes(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ double max_lanes(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -996,46 +996,63 @@ __device__ __forceinline__ void write_unused(const Distill& p, long long row, Ro
   p.loss[row] = kind == BAD ? NAN : 0.f;
   reinterpret_cast<float4*>(p.saved)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
-// The teacher's side of a live row; a warp.  power: kMaxEntries of its own.
+// log v, absolutely exact to 2^-24 whatever the magnitude.
+__device__ __forceinline__ double log_of(float v) {
+  int k;
+  const float m = frexpf(v, &k);
+  return fma((double)k, 0.69314718055994531, (double)logf(m));
+}
+// e^v for v <= 0 or so, to a relative 2^-22: expf of v's leading bits, and the rest's first order.
+__device__ __forceinline__ float exp_of(double v) {
+  if (v < -200) return 0.f;
+  const float high = (float)v, e = expf(high);
+  return fmaf(e, (float)(v - (double)high), e);
+}
+// The teacher's side of a live row; a warp.  Sums and differences are in f64, of values that f32 functions give to a relative 2^-22;
+// with TAIL the q themselves are f64, for their difference from one.
 template <typename T, bool TAIL>
-__device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t, double* power) {
+__device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t) {
   const int lane = threadIdx.x & 31;
   const T* src = static_cast<const T*>(p.x) + row * p.ld;
-  double most = -INFINITY;
-  float x_most = -INFINITY;
+  float most = -INFINITY, x_most = -INFINITY;
   __syncwarp();
   for (int j = lane; j < p.entries; j += 32) {
     const int id = (int)load_id(p.ids, row * p.entries + j, p.id_bits);
-    const double u = (double)load_value(p.values, row * p.entries + j, p.values_dtype) / (double)p.temperature;
-    const float x = id ? to_float(src[id - 1]) : -INFINITY;
+    const float v = load_value(p.values, row * p.entries + j, p.values_dtype), x = id ? to_float(src[id - 1]) : -INFINITY;
     t.entry[j] = id;
+    t.q[j] = v;
     t.x[j] = x;
-    power[j] = u;
     x_most = fmaxf(x_most, x);
-    if (id) most = fmax(most, u);
+    if (id) most = fmaxf(most, v);
   }
   double norm;
   if constexpr (TAIL) {
     norm = p.teacher_lse[row];
   } else {
-    most = max_lanes(most);
-    double sum = 0;
+    most = warp_max(most);
+    float sum = 0.f;
     for (int j = lane; j < p.entries; j += 32)
-      if (t.entry[j]) sum += exp(power[j] - most);
-    norm = most + log(sum_lanes(sum));
+      if (t.entry[j]) sum += exp_of(((double)t.q[j] - (double)most) * p.per_temperature);
+    norm = fma((double)most, p.per_temperature, log_of(warp_sum(sum)));
   }
   double all = 0, terms = 0;
   for (int j = lane; j < p.entries; j += 32) {
     if (t.entry[j] == 0) continue;
-    const double log_q = power[j] - norm, q = exp(log_q);
-    if (q != 0) terms += q * (log_q - (double)t.x[j] / (double)p.temperature);
-    all += q;
+    const double log_q = fma((double)t.q[j], p.per_temperature, -norm);
+    double q;
+    if constexpr (TAIL) {
+      q = exp(log_q);
+      all += q;
+    } else {
+      q = (double)exp_of(log_q);
+    }
+    if (q != 0) terms = fma(q, log_q - (double)t.x[j] * p.per_temperature, terms);
     t.q[j] = (float)q;
   }
-  all = sum_lanes(all);
   terms = sum_lanes(terms);
   float listed = 0.f;
   if constexpr (TAIL) {
+    all = sum_lanes(all);
     __syncwarp();
     x_most = fmaxf(warp_max(x_most), -FLT_MAX);
     for (int j = lane; j < p.entries; j += 32) {
@@ -1048,7 +1065,7 @@ __device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t, 
   }
   if (lane == 0) {
     t.terms = terms;
-    t.all = all;
+    t.all = TAIL ? all : 1;
     t.norm = norm;
     t.listed_max = x_most;
     t.listed = listed;
@@ -1059,38 +1076,41 @@ __device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t, 
 struct Answer {
   float lse2, a, g, whole;
 };
-// Loss and saved values of a row from (maximum, s), which with TAIL leave out what the teacher lists; one lane.
+// A row's (maximum, s) with what the teacher lists, which with TAIL they leave out: maximum, total, and the rest's share of it.
 template <bool TAIL>
-__device__ __noinline__ Answer close_row(const Distill& p, long long row, const Teacher& t, float3 sum, bool write) {
-  float total = sum.y, rest = sum.y, whole = 1.f, outside = 1.f;
-  double left = 0;
-  if constexpr (TAIL) {
-    const float both = fmaxf(sum.x, t.listed_max);
-    rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
-    total = rest + t.listed * ex2_approx_ftz((t.listed_max - both) * p.c);
-    sum.x = both;
-    left = t.all > 1 ? 0 : 1 - t.all;
-    whole = (float)(t.all + left);
-    outside = rest == 0.f ? whole : (float)(t.all + left - left * ((double)total / (double)rest));
-  }
-  if (write) {
-    const double log_total = log((double)total), lse = (double)sum.x / (double)p.temperature + log_total;
-    double loss = t.terms + t.all * lse;
-    if (left != 0) loss += left * (log(left) - (log((double)rest) - log_total));
-    // (lse, outside, whole, norm) with teacher_lse; else outside and whole are 1, and the norm keeps 48 bits: (lse, low part, -1, norm)
-    const float high = (float)t.norm;
-    p.loss[row] = (float)loss;
-    reinterpret_cast<float4*>(p.saved)[row] = TAIL ? make_float4((float)lse, outside, whole, high)
-                                                   : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
-  }
+__device__ __forceinline__ float3 with_listed(const Distill& p, const Teacher& t, float3 sum) {
+  if constexpr (!TAIL) return make_float3(sum.x, sum.y, sum.y);
+  const float both = fmaxf(sum.x, t.listed_max), rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
+  return make_float3(both, rest + t.listed * ex2_approx_ftz((t.listed_max - both) * p.c), rest);
+}
+// What the teacher's list leaves over, and the factor of p outside of the list.
+__device__ __forceinline__ double left_over(const Teacher& t) { return t.all > 1 ? 0 : 1 - t.all; }
+__device__ __forceinline__ float outside_of(const Teacher& t, float3 sum) {
+  const double left = left_over(t), whole = t.all + left;
+  return (float)(sum.z == 0.f ? whole : whole - left * ((double)sum.y / (double)sum.z));
+}
+template <bool TAIL>
+__device__ __forceinline__ Answer answer_of(const Distill& p, const Teacher& t, float3 sum, float d_loss) {
   Answer answer;
   int k;  // the logarithm's whole part joins the reference before it is rounded
-  const float m = frexpf(total, &k);
+  const float m = frexpf(sum.y, &k);
   answer.lse2 = fmaf(sum.x, p.c, (float)k) + log2f(m);
-  answer.g = p.d_loss ? p.d_loss[row] / p.temperature : 0.f;
-  answer.a = answer.g * outside;
-  answer.whole = whole;
+  answer.g = d_loss / p.temperature;
+  answer.a = TAIL ? answer.g * outside_of(t, sum) : answer.g;
+  answer.whole = TAIL ? (float)(t.all + left_over(t)) : 1.f;
   return answer;
+}
+// Loss and saved values of a row; one lane.
+template <bool TAIL>
+__device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, float3 sum) {
+  const double log_total = log_of(sum.y), lse = fma((double)sum.x, p.per_temperature, log_total);
+  double loss = t.terms + t.all * lse;
+  if (TAIL && left_over(t) != 0) loss += left_over(t) * (log(left_over(t)) - (log_of(sum.z) - log_total));
+  // (lse, outside, whole, norm) with teacher_lse; else outside and whole are 1, and the norm keeps 48 bits: (lse, low part, -1, norm)
+  const float high = (float)t.norm;
+  p.loss[row] = (float)loss;
+  reinterpret_cast<float4*>(p.saved)[row] = TAIL ? make_float4((float)lse, outside_of(t, sum), (float)(t.all + left_over(t)), high)
+                                                 : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
 }
 // TAIL: teacher_lse is given, and what the teacher lists is left out of the row's sum, by a bit per element, and added apart: the rest's
 // probability from a difference would lose all digits where it is small.  Sets or clears the bits of a part's entries; a warp.
@@ -1138,9 +1158,8 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __
   __shared__ Teacher teachers[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Teacher& t = teachers[warp];
-  double* power = reinterpret_cast<double*>(store) + warp * kMaxEntries;
   const int words = TAIL ? p.per * Range<T>::V / 32 : 0;  // per is a multiple of 32 vectors
-  unsigned* bits = reinterpret_cast<unsigned*>(store + sizeof(double) * kWarps * kMaxEntries) + warp * words;
+  unsigned* bits = reinterpret_cast<unsigned*>(store) + warp * words;
   for (int i = lane; i < words; i += 32) bits[i] = 0;
   grid_dependency_wait();
   __syncwarp();
@@ -1161,17 +1180,20 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __
     float3 sum = sum_range<T, false, TAIL, 1>(r, bits, p.c);
     if constexpr (TAIL) punch(r, t.entry, p.entries, bits, false);
     if (!join_records(p, row, part, sum)) continue;
-    learn<T, TAIL>(p, row, t, power);
-    if (lane == 0) (void)close_row<TAIL>(p, row, t, sum, true);
+    learn<T, TAIL>(p, row, t);
+    if (lane == 0) close_row<TAIL>(p, row, t, with_listed<TAIL>(p, t, sum));
     __syncwarp();
   }
   grid_dependency_launch();
 }
 
-// Loss and gradient at once: the row is read a second time, out of L2, for the gradient, while the clerk joins the sums of the row behind it.
+// Loss and gradient at once: the row is read a second time, out of L2, for the gradient.  Rows are few enough at a time (CTAs on the device
+// times a row) to stay there: with the next row streamed between the two, or five CTAs on an SM, HBM was read twice.
 struct DistillLesson {
   long long at;
   bool zero;  // its gradient is 0 and its logits are not read
+  float d_loss;
+  float3 sum;  // with what the teacher lists
   Answer answer;
   Teacher teacher;
 };
@@ -1180,7 +1202,6 @@ struct DistillOp {
   using Lesson = DistillLesson;
   static constexpr bool AGAIN = true, MEETS = false;
   const Distill& p;
-  double (&power)[kMaxEntries];  // the clerk's
   unsigned* bits;                // two sets of `words`
   int words;
   Meeting& meeting;
@@ -1190,8 +1211,11 @@ struct DistillOp {
   __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
     const Row kind = look_at(p, row);
     if (kind != LIVE && rank() == 0) write_unused(p, row, kind);
-    if ((threadIdx.x & 31) == 0) l.zero = kind != LIVE;
-    if (kind == LIVE) learn<T, TAIL>(p, row, l.teacher, power);
+    if ((threadIdx.x & 31) == 0) {
+      l.zero = kind != LIVE;
+      l.d_loss = p.d_loss[row];
+    }
+    if (kind == LIVE) learn<T, TAIL>(p, row, l.teacher);
     return true;
   }
   // The row two before has been summed: its bits lie where the next row's go.
@@ -1222,7 +1246,13 @@ struct DistillOp {
       await_parts(p, meeting, meet);
       sum = join_parts(p, meeting, meet);
     }
-    if ((threadIdx.x & 31) == 0) l.answer = close_row<TAIL>(p, l.at, l.teacher, sum, rank() == 0);
+    if ((threadIdx.x & 31) == 0) {
+      l.sum = with_listed<TAIL>(p, l.teacher, sum);
+      l.answer = answer_of<TAIL>(p, l.teacher, l.sum, l.d_loss);
+    }
+  }
+  __device__ __forceinline__ void close(const Lesson& l) {
+    if (!l.zero && rank() == 0 && (threadIdx.x & 31) == 0) close_row<TAIL>(p, l.at, l.teacher, l.sum);
   }
   __device__ __forceinline__ void again(const Lesson& l, const Range<T>& r, const Inner& in) {
     T* dst = static_cast<T*>(p.dx) + l.at * p.ld_dx;
@@ -1243,11 +1273,10 @@ __global__ void __launch_bounds__(kAllThreads, kDistillPerSm) distill_both_kerne
   __shared__ Pipe pipe;
   __shared__ Meeting meeting;
   __shared__ DistillLesson lessons[4];
-  __shared__ double power[kMaxEntries];
   unsigned* bits = reinterpret_cast<unsigned*>(store);
   const int words = TAIL ? p.per * Range<T>::V / 32 : 0;
   for (int i = threadIdx.x; i < 2 * words; i += kAllThreads) bits[i] = 0;
-  DistillOp<T, TAIL> op{p, power, bits, words, meeting, 0};
+  DistillOp<T, TAIL> op{p, bits, words, meeting, 0};
   run_rows<T>(p, op, lessons, pipe, &meeting);
 }
 
@@ -1271,7 +1300,9 @@ struct Backward : Rows {
 // Gradient of the log probabilities, the entropy and the alternatives of a row:
 //   dx_v = 1/temperature [ sum of the gradients that meet at v - p_v (G + g_H (log p_v + H)) ],  G = the sum of all but g_H
 // and of the distillation loss (DISTILL): g/temperature p_v outside, or g/temperature (whole p_v - q_v) where the teacher lists v.
-// A warp takes a part of a row after another; the few places that a gradient meets directly are written behind the part's stream.
+// A CTA takes a part of a row after another; its warps share the tiles, so that 16 KB are read and written side by side (parts of a warp's
+// own left HBM at 85 %), but do not wait for each other: each has the few places in its tiles that a gradient meets directly, and writes
+// them behind its stream.  What a warp needs of a row the others need as well, and each loads it.
 template <typename T, bool DISTILL, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kernel(const __grid_constant__ Backward p) {
   constexpr int kEntries = DISTILL ? kMaxEntries : kMaxTop + 1;
@@ -1281,7 +1312,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int* entry = entries_of[warp];
   float *weight = weights_of[warp], *x = logits_of[warp];
-  const Items items(p);
+  const Items items(p, kWarps);
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item);
     const Range<T> r = range_of<T>(p, row, (int)(item - row * p.parts));
@@ -1306,7 +1337,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
       const bool bad = p.tokens && (token < 0 || token > p.n);
       if (token == 0 || bad) {
         if (bad && lane == 0) atomicMax(p.status, DEV_BAD_INDEX);
-        stream_zeros<T, 1>(r, dst);
+        stream_zeros<T, kWarps>(r, dst);
         continue;
       }
       const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
@@ -1320,7 +1351,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
     } else {
       const float4 saved = reinterpret_cast<const float4*>(p.saved)[row];
       if (saved.z == 0.f) {
-        stream_zeros<T, 1>(r, dst);
+        stream_zeros<T, kWarps>(r, dst);
         continue;
       }
       const bool list_is_all = saved.z < 0.f;  // of the teacher's distribution
@@ -1330,7 +1361,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
         const long long id = load_id(p.ids, row * entries + j, p.id_bits);
         float q = 0.f;
         if (in_range(r, id))
-          q = (float)exp((double)load_value(p.values, row * entries + j, p.values_dtype) / (double)p.temperature - norm);
+          q = exp_of((double)load_value(p.values, row * entries + j, p.values_dtype) / (double)p.temperature - norm);
         enter(j, id, q);
       }
       g = p.d_loss[row] / p.temperature;
@@ -1339,8 +1370,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
       whole = list_is_all ? 1.f : saved.z;
     }
     __syncwarp();
-    stream_gradient<T, ENTROPY, 1>(r, in, dst, p.c, lse2, a, b);
-    patch_entries<1>(r, in, entry, weight, entries, [&](int id, int j, float sum) {
+    stream_gradient<T, ENTROPY, kWarps>(r, in, dst, p.c, lse2, a, b);
+    patch_entries<kWarps>(r, in, entry, weight, entries, [&](int id, int j, float sum) {
       const float t = fmaf(x[j], p.c, -lse2), e = ex2_approx_ftz(t);
       dst[id - 1] = from_float<T>(DISTILL ? g * (whole * e - sum) : sum / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
     });
@@ -1440,8 +1471,8 @@ void cut_into(Rows& p, int64_t nvec, int64_t parts) {
 }
 // Rows cut among warps: into the parts for which rounds of parts take the least time.  A warp reads `alone` bytes per ns when nobody else reads
 // and shares what HBM gives otherwise, and a part costs `ends` besides (us); measured with 1 to 2220 rows of 50000 to 128000 elements.
-void cut_among_warps(Rows& p, int64_t nvec, int elem, int passes, int64_t places, int64_t most, double ends) {
-  const double alone = elem == 4 ? 5.1 : 3.5, all = 7600, bytes = (double)(passes * nvec) * 16e-3;  // of a row, in 1000
+void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t most, double ends) {
+  const double alone = elem == 4 ? 5.1 : 3.5, all = 7600, bytes = (double)nvec * 16e-3;  // of a row, in 1000
   double best = 0;
   int64_t parts = 1;
   most = std::min({most, std::max<int64_t>(1, nvec / 128), std::max<int64_t>(1, 16 * places / std::max(1, p.rows))});  // 2 KB; 16 rounds
@@ -1457,18 +1488,23 @@ void cut_among_warps(Rows& p, int64_t nvec, int elem, int passes, int64_t places
   p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
   p.parts = (int)((nvec + p.per - 1) / p.per);
 }
+// Rows cut among CTAs that share nothing: parts of up to four tiles (64 KB), of one where that brings work to more SMs.
+void cut_rows_into_parts(Rows& p, int64_t nvec, int64_t places) {
+  const int64_t tiles = (nvec + kTile - 1) / kTile, each = p.rows * tiles >= 16 * places ? 4 : p.rows * tiles >= 8 * places ? 2 : 1;
+  cut_into(p, nvec, (tiles + each - 1) / each);
+}
 // Parts that a row may have whose sums meet in scratch memory: as many as their records and counters have room for.
 int64_t most_parts(const Rows& p) {
   if (p.rows > kTickets) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows));
 }
 
-// Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element, besides `fixed` bytes.
+// Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element.
 template <auto KERNEL, typename T, typename P>
-int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, size_t fixed, bool bits, double ends, const char* who) {
+int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, double ends, const char* who) {
   const int64_t places = (int64_t)kPlainPerSm * ctx->sm_count * kWarps, nvec = vectors<T>(p);
   auto go = [&] {
-    const size_t smem = fixed + (bits ? (size_t)kWarps * 4 * (p.per * (16 / sizeof(T)) / 32) : 0);
+    const size_t smem = (bits ? (size_t)kWarps * 4 * (p.per * (16 / sizeof(T)) / 32) : 0);
     int per_sm = kPlainPerSm;
     if (smem > 0) {
       if (smem > 200 * 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
@@ -1482,7 +1518,7 @@ int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, size_t fixed, bool bits, do
     CTB_CHECK_LAUNCH(who);
     return (int)CTB_OK;
   };
-  cut_among_warps(p, nvec, sizeof(T), 1, places, most_parts(p), ends);
+  cut_among_warps(p, nvec, sizeof(T), places, most_parts(p), ends);
   if (p.parts > 1) {
     StreamScratch scratch(ctx, st);
     if (scratch.data) {
@@ -1530,23 +1566,22 @@ int launch_rows(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool bits, doubl
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
   if (p.top) return launch_rows<top_logprobs_kernel<T>, T>(ctx, st, p, kTopPerSm, false, 3.0, who);
-  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, 0, false, 3.0, who);
+  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, 3.0, who);
 }
 template <typename T>
 int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* who) {
-  constexpr size_t kPowers = sizeof(double) * kWarps * kMaxEntries;
   if (p.dx)
     return p.teacher_lse ? launch_rows<distill_both_kernel<T, true>, T>(ctx, st, p, kDistillPerSm, true, 2.5, who)
                          : launch_rows<distill_both_kernel<T, false>, T>(ctx, st, p, kDistillPerSm, false, 2.5, who);
-  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, kPowers, true, 5.0, who)
-                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, kPowers, false, 5.0, who);
+  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, true, 5.0, who)
+                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, false, 5.0, who);
 }
 template <typename T, bool DISTILL>
 int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
   auto kernel = p.d_entropy ? logits_backward_kernel<T, DISTILL, !DISTILL> : logits_backward_kernel<T, DISTILL, false>;
   const int64_t most = (int64_t)kBackwardPerSm * ctx->sm_count;
-  cut_among_warps(p, vectors<T>(p), sizeof(T), 2, most * kWarps, INT32_MAX, DISTILL ? 2.0 : 1.0);
-  launch_kernel(kernel, (int)std::min<int64_t>(((int64_t)p.rows * p.parts + kWarps - 1) / kWarps, most), kThreads, 0, st, 0, p);
+  cut_rows_into_parts(p, vectors<T>(p), most);
+  launch_kernel(kernel, (int)std::min<int64_t>((int64_t)p.rows * p.parts, most), kThreads, 0, st, 0, p);
   CTB_CHECK_LAUNCH(who);
   return CTB_OK;
 }
@@ -1657,7 +1692,7 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   p.temperature = temperature;
   p.status = ctx->dev_status;
   p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
-  p.teacher_lse = teacher_lse; p.loss = loss; p.saved = saved;
+  p.teacher_lse = teacher_lse; p.per_temperature = 1 / (double)temperature; p.loss = loss; p.saved = saved;
   p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(ctx, st, p, who); });
