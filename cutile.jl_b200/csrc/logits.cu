@@ -32,8 +32,8 @@ constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
 constexpr int kMaxEntries = kThreads;    // of a teacher's list
 constexpr int kCand = 1024;
-constexpr int kPlainPerSm = 6, kTopPerSm = 3, kDistillPerSm = 4, kBackwardPerSm = 5;  // CTAs on an SM
-constexpr int kMostHoles = 512 * 1024;  // elements of a part that have a bit (in two sets) in shared memory
+constexpr int kPlainPerSm = 6, kTopPerSm = 3, kBackwardPerSm = 5;  // CTAs on an SM
+constexpr size_t kMostShared = 220 * 1024;  // dynamic shared memory of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Exponents (base 2) are held above this where they are multiplied by their power, which is 0 there: 0 * -inf would be NaN.
@@ -331,26 +331,6 @@ struct Sums {
   }
 };
 
-// Listed elements of a range: a bit for each element from vector v0 on, or nothing.
-template <typename T>
-__device__ __forceinline__ unsigned hole_bits(const unsigned* holes, int v) {  // of the range's vector v
-  if constexpr (sizeof(T) == 4) return holes[v >> 3] >> (v & 7) * 4 & 15;
-  else return reinterpret_cast<const unsigned char*>(holes)[v];
-}
-template <typename T>
-__device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      if (bits >> i & 1) w[i] = 0xff800000u;
-    } else {
-      const uint32_t low = empty_row_vec<T>().x;
-      if (bits >> 2 * i & 1) w[i] = (w[i] & 0xffff0000u) | (low & 0xffffu);
-      if (bits >> 2 * i & 2) w[i] = (w[i] & 0xffffu) | (low & 0xffff0000u);
-    }
-  }
-}
 
 // (s, w) of up to 8 or 16 sets of sums, held by lanes i, i + 8 (16), ..., each relative to a maximum of its own, relative to `most`.
 // apart: of the set's maximum below `most`, in units of log2.
@@ -437,12 +417,42 @@ __device__ __forceinline__ int edge_index(const Range<T>& r, const Inner& in, in
   if (tid >= 8 && tid - 8 < in.tail) return r.n - in.tail + tid - 8;
   return -1;
 }
+// A bit per element of a warp's part, in the order in which the lanes take its vectors, kUnroll at a time; the last word: head, then tail.
+__host__ __device__ constexpr int hole_words(int per, int elem) { return (per + 32 * kUnroll - 1) / (32 * kUnroll) * kUnroll * (16 / elem) + 1; }
+template <typename T>
+__device__ __forceinline__ unsigned hole_bits(const unsigned* holes, int v) {  // of a lane's vectors from v on, v counted from the first inner one
+  const int at = (v / (32 * kUnroll)) * 32 + (threadIdx.x & 31), u = v / 32 % kUnroll;
+  if constexpr (sizeof(T) == 4) return reinterpret_cast<const unsigned short*>(holes)[at] >> 4 * u;
+  else return holes[at] >> 8 * u;
+}
+template <typename T>
+__device__ __forceinline__ void punch(const Range<T>& r, const Inner& in, int id, unsigned* holes, int words) {
+  constexpr int V = Range<T>::V;
+  const int e = id - 1 + r.off, v = e / V - in.a;
+  int bit = (words - 1) * 32 + (e & (V - 1)) + (v < 0 ? 0 : 16);
+  if (v >= 0 && e / V < in.b) bit = (((v / (32 * kUnroll)) * 32 + v % 32) * kUnroll + v / 32 % kUnroll) * V + (e & (V - 1));
+  atomicOr(holes + (bit >> 5), 1u << (bit & 31));
+}
+template <typename T>
+__device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      if (bits >> i & 1) w[i] = 0xff800000u;
+    } else {
+      const uint32_t low = empty_row_vec<T>().x;
+      if (bits >> 2 * i & 1) w[i] = (w[i] & 0xffff0000u) | (low & 0xffffu);
+      if (bits >> 2 * i & 2) w[i] = (w[i] & 0xffffu) | (low & 0xffff0000u);
+    }
+  }
+}
 
 // Calls f(q, v) for a streaming thread's vectors, four at a time; v: the tile's first one.  What is left over comes one vector at a time, in
 // the warps that have some of it; lanes beyond the end get -inf.  KEEP: the row is read again, from L2.  Lanes that
 // took a rare branch in f would go on by themselves up to the next shuffle, behind the row: they meet before every tile.
 // W warps stream the row.
-template <typename T, bool KEEP, int W, typename F>
+template <typename T, int W, typename F>
 __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F f) {
   constexpr int kWide = W * 32;
   const int tid = threadIdx.x % kWide;
@@ -453,14 +463,14 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
     __syncwarp();
     uint4 q[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kWide) : __ldcs(p + u * kWide);
+    for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(p + u * kWide);
     f(q, v);
   }
 #pragma unroll 1
   for (; v + (tid & ~31) < in.b; v += kWide, p += kWide) {
     __syncwarp();
     uint4 q[1] = {empty_row_vec<T>()};
-    if (v + tid < in.b) q[0] = KEEP ? __ldcg(p) : __ldcs(p);
+    if (v + tid < in.b) q[0] = __ldcs(p);
     f(q, v);
   }
 }
@@ -473,38 +483,43 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
 constexpr int kMaxParts = 256;
 struct Items {  // of a warp (or, with W = 8, of the warps of a CTA, which share a part's tiles)
   const Rows& p;
+  int parts;
   long long at, step, end;
-  __device__ __forceinline__ explicit Items(const Rows& rows, int W = 1) : p(rows) {
+  __device__ __forceinline__ explicit Items(const Rows& rows, int W = 1, int each = 0) : p(rows), parts(each ? each : rows.parts) {
     at = W == 1 ? (long long)blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
     step = W == 1 ? (long long)gridDim.x * kWarps : gridDim.x;
-    end = (long long)p.rows * p.parts;
+    end = (long long)p.rows * parts;
   }
-  __device__ __forceinline__ long long row(long long item) const { return p.parts == 1 ? item : item / p.parts; }
+  __device__ __forceinline__ long long row(long long item) const { return parts == 1 ? item : item / parts; }
 };
 // After a warp has summed a part: true for the row's last one, with the row's (maximum, s, w).
+// A row's (maximum, s, w) from those of its parts.
+__device__ __forceinline__ float3 gather_records(const float4* records, int parts, float c) {
+  const int lane = threadIdx.x & 31;
+  float most = -FLT_MAX;
+  for (int i = lane; i < parts; i += 32) most = fmaxf(most, __ldcg(&records[i].x));
+  most = warp_max(most);
+  float s = 0.f, w = 0.f;
+  for (int i = lane; i < parts; i += 32) {
+    const float4 one = __ldcg(records + i);
+    const float d = (one.x - most) * c, r = ex2_approx_ftz(d);
+    s = fmaf(one.y, r, s);
+    w += r * fmaf(one.y, fmaxf(d, kLowest), one.z);
+  }
+  return make_float3(most, warp_sum(s), warp_sum(w));
+}
 __device__ __forceinline__ bool join_records(const Rows& p, long long row, int part, float3& sum) {
   if (p.parts == 1) return true;
-  const int lane = threadIdx.x & 31;
   float4* records = p.records + row * p.parts;
   unsigned order = 0;
-  if (lane == 0) {
+  if ((threadIdx.x & 31) == 0) {
     __stcg(records + part, make_float4(sum.x, sum.y, sum.z, 0.f));
     __threadfence();
     order = atomicInc(p.tickets + row, p.parts - 1);
   }
   if (__shfl_sync(0xffffffffu, order, 0) != (unsigned)p.parts - 1) return false;
   __threadfence();
-  float most = -FLT_MAX;
-  for (int i = lane; i < p.parts; i += 32) most = fmaxf(most, __ldcg(&records[i].x));
-  most = warp_max(most);
-  float s = 0.f, w = 0.f;
-  for (int i = lane; i < p.parts; i += 32) {
-    const float4 one = __ldcg(records + i);
-    const float d = (one.x - most) * p.c, r = ex2_approx_ftz(d);
-    s = fmaf(one.y, r, s);
-    w += r * fmaf(one.y, fmaxf(d, kLowest), one.z);
-  }
-  sum = make_float3(most, warp_sum(s), warp_sum(w));
+  sum = gather_records(records, p.parts, p.c);
   return true;
 }
 
@@ -724,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) logprobs_kernel(const _
     const int edge = edge_index(r, in, lane);
     const float at_edge = edge >= 0 ? to_float(r.src[edge]) : 0.f;
     Sums<T, true> sums;
-    each_tile<T, false, 1>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
+    each_tile<T, 1>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
     if (edge >= 0) sums.add_one(at_edge, p.c);
     __syncwarp();
     float3 sum = sums.over_warp(p.c);
@@ -882,7 +897,7 @@ __device__ __forceinline__ void stream_gradient(const Range<T>& r, const Inner& 
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
   const Pair cc = pair(c, c), minus = pair(-lse2, -lse2), aa = pair(a, a), bb = pair(b, b);
   const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
-  each_tile<T, false, W>(r, in, [&](auto& q, int v) {
+  each_tile<T, W>(r, in, [&](auto& q, int v) {
     constexpr int N = sizeof(q) / sizeof(uint4);
     uint4* to = reinterpret_cast<uint4*>(dst - r.off) + v + tid;
 #pragma unroll
@@ -958,10 +973,6 @@ struct Distill : Rows {
   const float* teacher_lse;
   double per_temperature;  // 1 / temperature
   float *loss, *saved;
-  // with the gradient
-  const float* d_loss;
-  void* dx;
-  long long ld_dx;
 };
 
 __device__ __forceinline__ double sum_lanes(double v) {
@@ -974,18 +985,30 @@ __device__ __forceinline__ double sum_lanes(double v) {
 struct Teacher {
   double terms, all, norm;   // sum q (log q - z), sum q
   float listed_max, listed;  // what the student gives to the listed ids, each once: maximum, sum of powers relative to it
-  int entry[kMaxEntries];    // ids, 0: unused
-  float q[kMaxEntries], x[kMaxEntries];
 };
+static_assert(sizeof(Teacher) == 2 * sizeof(float4), "a teacher takes two records");
+// A warp's lists of `entries` each, in dynamic shared memory: ids (0: unused), q, the student's logits.
+struct Listed {
+  int* entry;
+  float *q, *x;
+  __device__ __forceinline__ Listed(unsigned char* store, int entries) {
+    entry = reinterpret_cast<int*>(store) + (threadIdx.x >> 5) * 3 * entries;
+    q = reinterpret_cast<float*>(entry + entries);
+    x = q + entries;
+  }
+};
+__host__ __device__ constexpr int lists_words(int entries) { return kWarps * 3 * entries; }
 enum Row { PADDING, BAD, LIVE };
 
-// Whether a row has used entries, and ids in range only; a warp.
-__device__ __forceinline__ Row look_at(const Distill& p, long long row) {
+// Whether a row has used entries, and ids in range only; a warp.  f(id) for each id in range.
+template <typename F>
+__device__ __forceinline__ Row look_at(const Distill& p, long long row, F f) {
   bool used = false, bad = false;
   for (int j = threadIdx.x & 31; j < p.entries; j += 32) {
     const long long id = load_id(p.ids, row * p.entries + j, p.id_bits);
     used |= id != 0;
-    bad |= id < 0 || id > p.n;
+    if (id < 0 || id > p.n) bad = true;
+    else if (id > 0) f((int)id);
   }
   used = __any_sync(0xffffffffu, used);
   return __any_sync(0xffffffffu, bad) ? BAD : used ? LIVE : PADDING;
@@ -1011,19 +1034,32 @@ __device__ __forceinline__ float exp_of(double v) {
 // The teacher's side of a live row; a warp.  Sums and differences are in f64, of values that f32 functions give to a relative 2^-22;
 // with TAIL the q themselves are f64, for their difference from one.
 template <typename T, bool TAIL>
-__device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t) {
+__device__ __noinline__ Teacher learn(const Distill& p, long long row, const Listed& t, unsigned* seen, int words) {
   const int lane = threadIdx.x & 31;
   const T* src = static_cast<const T*>(p.x) + row * p.ld;
   float most = -INFINITY, x_most = -INFINITY;
   __syncwarp();
-  for (int j = lane; j < p.entries; j += 32) {
-    const int id = (int)load_id(p.ids, row * p.entries + j, p.id_bits);
-    const float v = load_value(p.values, row * p.entries + j, p.values_dtype), x = id ? to_float(src[id - 1]) : -INFINITY;
-    t.entry[j] = id;
-    t.q[j] = v;
-    t.x[j] = x;
-    x_most = fmaxf(x_most, x);
-    if (id) most = fmaxf(most, v);
+  for (int j0 = 0; j0 < p.entries; j0 += 64) {
+    int id[2];
+    float v[2], x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = j0 + 32 * i + lane;
+      id[i] = j < p.entries ? (int)load_id(p.ids, row * p.entries + j, p.id_bits) : 0;
+      v[i] = j < p.entries ? load_value(p.values, row * p.entries + j, p.values_dtype) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = id[i] ? to_float(src[id[i] - 1]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = j0 + 32 * i + lane;
+      if (j >= p.entries) break;
+      t.entry[j] = id[i];
+      t.q[j] = v[i];
+      t.x[j] = x[i];
+      x_most = fmaxf(x_most, x[i]);
+      if (id[i]) most = fmaxf(most, v[i]);
+    }
   }
   double norm;
   if constexpr (TAIL) {
@@ -1055,27 +1091,32 @@ __device__ __noinline__ void learn(const Distill& p, long long row, Teacher& t) 
     all = sum_lanes(all);
     __syncwarp();
     x_most = fmaxf(warp_max(x_most), -FLT_MAX);
-    for (int j = lane; j < p.entries; j += 32) {
-      const int id = t.entry[j];
-      bool again = id == 0;
-      for (int i = 0; i < j; ++i) again |= t.entry[i] == id;
-      if (!again) listed += ex2_approx_ftz((t.x[j] - x_most) * p.c);
+    // Ids that meet in a small table are looked for in the list, and all but the first of those alike marked.
+    const unsigned mask = (32u << (31 - __clz(words))) - 1;
+    for (int j0 = 0; j0 < p.entries; j0 += 32) {
+      const int id = j0 + lane < p.entries ? t.entry[j0 + lane] : 0, own = max(id, 0);
+      const bool met = id > 0 && (atomicOr(seen + ((own & mask) >> 5), 1u << (own & 31)) >> (own & 31) & 1);
+      for (unsigned left = __ballot_sync(0xffffffffu, met); left; left &= left - 1) {
+        const int like = __shfl_sync(0xffffffffu, id, __ffs(left) - 1);
+        int first = kMaxEntries;
+        for (int i = lane; i < p.entries; i += 32)
+          if (abs(t.entry[i]) == like) first = min(first, i);
+        first = __reduce_min_sync(0xffffffffu, first);
+        for (int i = lane; i < p.entries; i += 32)
+          if (i != first && t.entry[i] == like) t.entry[i] = -like;
+        __syncwarp();
+      }
     }
+    for (int j = lane; j < p.entries; j += 32)
+      if (t.entry[j] > 0) {
+        listed += ex2_approx_ftz((t.x[j] - x_most) * p.c);
+        seen[(t.entry[j] & mask) >> 5] = 0;
+      }
     listed = warp_sum(listed);
   }
-  if (lane == 0) {
-    t.terms = terms;
-    t.all = TAIL ? all : 1;
-    t.norm = norm;
-    t.listed_max = x_most;
-    t.listed = listed;
-  }
   __syncwarp();
+  return {terms, TAIL ? all : 1, norm, x_most, listed};
 }
-// What the gradient needs of a row: where the teacher lists nothing it is p a, else g (whole p - q).
-struct Answer {
-  float lse2, a, g, whole;
-};
 // A row's (maximum, s) with what the teacher lists, which with TAIL they leave out: maximum, total, and the rest's share of it.
 template <bool TAIL>
 __device__ __forceinline__ float3 with_listed(const Distill& p, const Teacher& t, float3 sum) {
@@ -1089,17 +1130,6 @@ __device__ __forceinline__ float outside_of(const Teacher& t, float3 sum) {
   const double left = left_over(t), whole = t.all + left;
   return (float)(sum.z == 0.f ? whole : whole - left * ((double)sum.y / (double)sum.z));
 }
-template <bool TAIL>
-__device__ __forceinline__ Answer answer_of(const Distill& p, const Teacher& t, float3 sum, float d_loss) {
-  Answer answer;
-  int k;  // the logarithm's whole part joins the reference before it is rounded
-  const float m = frexpf(sum.y, &k);
-  answer.lse2 = fmaf(sum.x, p.c, (float)k) + log2f(m);
-  answer.g = d_loss / p.temperature;
-  answer.a = TAIL ? answer.g * outside_of(t, sum) : answer.g;
-  answer.whole = TAIL ? (float)(t.all + left_over(t)) : 1.f;
-  return answer;
-}
 // Loss and saved values of a row; one lane.
 template <bool TAIL>
 __device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, float3 sum) {
@@ -1112,174 +1142,6 @@ __device__ __noinline__ void close_row(const Distill& p, long long row, const Te
   reinterpret_cast<float4*>(p.saved)[row] = TAIL ? make_float4((float)lse, outside_of(t, sum), (float)(t.all + left_over(t)), high)
                                                  : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
 }
-// TAIL: teacher_lse is given, and what the teacher lists is left out of the row's sum, by a bit per element, and added apart: the rest's
-// probability from a difference would lose all digits where it is small.  Sets or clears the bits of a part's entries; a warp.
-template <typename T>
-__device__ __forceinline__ void punch(const Range<T>& r, const int* entry, int entries, unsigned* bits, bool set) {
-  for (int j = threadIdx.x & 31; j < entries; j += 32) {
-    const int id = in_range(r, entry[j]);
-    if (id == 0) continue;
-    const int e = id - 1 + r.off - r.v0 * Range<T>::V;
-    if (set) atomicOr(bits + (e >> 5), 1u << (e & 31));
-    else bits[e >> 5] = 0;
-  }
-  __syncwarp();
-}
-// A range's elements but for those with a bit, by W warps.
-template <typename T, bool KEEP, bool TAIL, int W>
-__device__ __forceinline__ float3 sum_range(const Range<T>& r, const unsigned* bits, float c) {
-  const Inner in(r);
-  const int tid = threadIdx.x % (W * 32), edge = edge_index(r, in, tid);
-  const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
-  Sums<T, false> sums;
-  each_tile<T, KEEP, W>(r, in, [&](auto& q, int v) {
-    if constexpr (TAIL) {
-#pragma unroll
-      for (int u = 0; u < (int)(sizeof(q) / sizeof(uint4)); ++u) {
-        const int of = v + u * W * 32 + tid;
-        const unsigned hole = of < in.b ? hole_bits<T>(bits, of - r.v0) : 0u;
-        if (hole) mask_holes<T>(q[u], hole);
-      }
-    }
-    (void)sums.add(q, c);
-  });
-  if (edge >= 0) {
-    const int e = edge + r.off - r.v0 * Range<T>::V;
-    if (!(TAIL && (bits[e >> 5] >> (e & 31) & 1))) sums.add_one(x, c);
-  }
-  __syncwarp();
-  return sums.over_warp(c);
-}
-
-// The loss alone: rows cut among warps.
-template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __grid_constant__ Distill p) {
-  extern __shared__ __align__(16) unsigned char store[];
-  __shared__ Teacher teachers[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Teacher& t = teachers[warp];
-  const int words = TAIL ? p.per * Range<T>::V / 32 : 0;  // per is a multiple of 32 vectors
-  unsigned* bits = reinterpret_cast<unsigned*>(store) + warp * words;
-  for (int i = lane; i < words; i += 32) bits[i] = 0;
-  grid_dependency_wait();
-  __syncwarp();
-  const Items items(p);
-  for (long long item = items.at; item < items.end; item += items.step) {
-    const long long row = items.row(item);
-    const int part = (int)(item - row * p.parts);
-    const Row kind = look_at(p, row);
-    if (kind != LIVE) {
-      if (part == 0) write_unused(p, row, kind);
-      continue;
-    }
-    const Range<T> r = range_of<T>(p, row, part);
-    if constexpr (TAIL) {
-      for (int j = lane; j < p.entries; j += 32) t.entry[j] = (int)load_id(p.ids, row * p.entries + j, p.id_bits);
-      punch(r, t.entry, p.entries, bits, true);
-    }
-    float3 sum = sum_range<T, false, TAIL, 1>(r, bits, p.c);
-    if constexpr (TAIL) punch(r, t.entry, p.entries, bits, false);
-    if (!join_records(p, row, part, sum)) continue;
-    learn<T, TAIL>(p, row, t);
-    if (lane == 0) close_row<TAIL>(p, row, t, with_listed<TAIL>(p, t, sum));
-    __syncwarp();
-  }
-  grid_dependency_launch();
-}
-
-// Loss and gradient at once: the row is read a second time, out of L2, for the gradient.  Rows are few enough at a time (CTAs on the device
-// times a row) to stay there: with the next row streamed between the two, or five CTAs on an SM, HBM was read twice.
-struct DistillLesson {
-  long long at;
-  bool zero;  // its gradient is 0 and its logits are not read
-  float d_loss;
-  float3 sum;  // with what the teacher lists
-  Answer answer;
-  Teacher teacher;
-};
-template <typename T, bool TAIL>
-struct DistillOp {
-  using Lesson = DistillLesson;
-  static constexpr bool AGAIN = true, MEETS = false;
-  const Distill& p;
-  unsigned* bits;                // two sets of `words`
-  int words;
-  Meeting& meeting;
-  int meetings;
-
-  __device__ __forceinline__ int rank() const { return p.parts > 1 ? (int)cluster_ctarank() : 0; }
-  __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
-    const Row kind = look_at(p, row);
-    if (kind != LIVE && rank() == 0) write_unused(p, row, kind);
-    if ((threadIdx.x & 31) == 0) {
-      l.zero = kind != LIVE;
-      l.d_loss = p.d_loss[row];
-    }
-    if (kind == LIVE) learn<T, TAIL>(p, row, l.teacher);
-    return true;
-  }
-  // The row two before has been summed: its bits lie where the next row's go.
-  __device__ __forceinline__ void before(int n, const Lesson* lessons) {
-    if (TAIL && n >= 2) mark(lessons[(n - 2) & 3], n, false);
-  }
-  __device__ __forceinline__ void after(int n, const Lesson* lessons) {
-    if (TAIL) mark(lessons[n & 3], n, true);
-  }
-  __device__ __forceinline__ void mark(const Lesson& l, int n, bool set) {
-    if (l.at >= 0 && !l.zero) punch(range_of<T>(p, l.at, rank()), l.teacher.entry, p.entries, bits + (n & 1) * words, set);
-  }
-  __device__ __forceinline__ void stream(int n, const Lesson& l, const Range<T>& r, const Inner&, float (&red)[3][kWarps]) {
-    if (l.zero) return;
-    const float3 sum = sum_range<T, true, TAIL, kWarps>(r, bits + (n & 1) * words, p.c);
-    if ((threadIdx.x & 31) == 0) {
-      red[0][threadIdx.x >> 5] = sum.x;
-      red[1][threadIdx.x >> 5] = sum.y;
-      red[2][threadIdx.x >> 5] = 0.f;
-    }
-  }
-  __device__ __forceinline__ void answer(int, Lesson& l, const float (&red)[3][kWarps]) {
-    if (l.zero) return;
-    float3 sum = join_warps<kWarps>(red, p.c);
-    if (p.parts > 1) {
-      const int meet = meetings++;
-      send_part(p, meeting, meet, sum, 0);
-      await_parts(p, meeting, meet);
-      sum = join_parts(p, meeting, meet);
-    }
-    if ((threadIdx.x & 31) == 0) {
-      l.sum = with_listed<TAIL>(p, l.teacher, sum);
-      l.answer = answer_of<TAIL>(p, l.teacher, l.sum, l.d_loss);
-    }
-  }
-  __device__ __forceinline__ void close(const Lesson& l) {
-    if (!l.zero && rank() == 0 && (threadIdx.x & 31) == 0) close_row<TAIL>(p, l.at, l.teacher, l.sum);
-  }
-  __device__ __forceinline__ void again(const Lesson& l, const Range<T>& r, const Inner& in) {
-    T* dst = static_cast<T*>(p.dx) + l.at * p.ld_dx;
-    if (l.zero) {
-      stream_zeros<T, kWarps>(r, dst);
-      return;
-    }
-    const Answer a = l.answer;
-    stream_gradient<T, false, kWarps>(r, in, dst, p.c, a.lse2, a.a, 0.f);
-    patch_entries<kWarps>(r, in, l.teacher.entry, l.teacher.q, p.entries, [&](int id, int j, float q) {
-      dst[id - 1] = from_float<T>(a.g * (a.whole * ex2_approx_ftz(fmaf(l.teacher.x[j], p.c, -a.lse2)) - q));
-    });
-  }
-};
-template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kAllThreads, kDistillPerSm) distill_both_kernel(const __grid_constant__ Distill p) {
-  extern __shared__ __align__(16) unsigned char store[];
-  __shared__ Pipe pipe;
-  __shared__ Meeting meeting;
-  __shared__ DistillLesson lessons[4];
-  unsigned* bits = reinterpret_cast<unsigned*>(store);
-  const int words = TAIL ? p.per * Range<T>::V / 32 : 0;
-  for (int i = threadIdx.x; i < 2 * words; i += kAllThreads) bits[i] = 0;
-  DistillOp<T, TAIL> op{p, bits, words, meeting, 0};
-  run_rows<T>(p, op, lessons, pipe, &meeting);
-}
-
 // ------------------------------------------------------------------ backward
 struct Backward : Rows {
   void* dx;
@@ -1294,6 +1156,7 @@ struct Backward : Rows {
   int id_bits, entries;
   const void* values;
   int values_dtype;
+  double per_temperature;
   const float *saved, *d_loss;
 };
 
@@ -1303,9 +1166,181 @@ struct Backward : Rows {
 // A CTA takes a part of a row after another; its warps share the tiles, so that 16 KB are read and written side by side (parts of a warp's
 // own left HBM at 85 %), but do not wait for each other: each has the few places in its tiles that a gradient meets directly, and writes
 // them behind its stream.  What a warp needs of a row the others need as well, and each loads it.
-template <typename T, bool DISTILL, bool ENTROPY>
+// TAIL: teacher_lse is given, and what the teacher lists is left out of the row's sum, by a bit per element, and added apart: the rest's
+// probability from a difference would lose all digits where it is small.
+// A part's elements but for those with a bit.
+template <typename T, bool TAIL>
+__device__ __forceinline__ float3 sum_range(const Range<T>& r, const Inner& in, const unsigned* holes, int words, float c) {
+  constexpr int V = Range<T>::V;
+  const int lane = threadIdx.x & 31, edge = edge_index(r, in, lane);
+  const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
+  Sums<T, false> sums;
+  each_tile<T, 1>(r, in, [&](auto& q, int v) {
+    if constexpr (TAIL) {
+      const unsigned hole = hole_bits<T>(holes, v - in.a);
+      if (__any_sync(0xffffffffu, hole != 0)) {
+#pragma unroll
+        for (int u = 0; u < (int)(sizeof(q) / sizeof(uint4)); ++u) mask_holes<T>(q[u], hole >> u * V);
+      }
+    }
+    (void)sums.add(q, c);
+  });
+  if (edge >= 0) {
+    const int bit = (edge + r.off & V - 1) + (lane < 8 ? 0 : 16);
+    if (!(TAIL && (holes[words - 1] >> bit & 1))) sums.add_one(x, c);
+  }
+  __syncwarp();
+  return sums.over_warp(c);
+}
+__device__ __forceinline__ void clear_holes(unsigned* holes, int words) {
+  __syncwarp();
+  for (int i = threadIdx.x & 31; i < words; i += 32) holes[i] = 0;
+  __syncwarp();
+}
+// What a row needs, by a warp each: the sums of its parts, and (part -1) the teacher's side, which takes as long as a part of 20 KB or so: latencies
+// and f64.  Each is left as a record, the teacher's in the first two; the last warp to come closes the row.  holes: zero before and after.
+template <typename T, bool TAIL>
+__device__ __forceinline__ void distill_part(const Distill& p, long long row, int part, const Listed& lists, unsigned* holes, int words) {
+  const int lane = threadIdx.x & 31;
+  const bool whole = p.parts == 1;  // one warp does it all
+  const Range<T> r = range_of<T>(p, row, max(part, 0));
+  const Inner in(r);
+  const Row kind = look_at(p, row, [&](int id) {
+    if (TAIL && part >= 0 && in_range(r, id)) punch(r, in, id, holes, words);
+  });
+  float4* records = p.records + row * (p.parts + 2);
+  bool last = whole || part < 0, clean = false;
+  if (kind != LIVE) {
+    if (last) write_unused(p, row, kind);
+  } else {
+    __syncwarp();
+    float3 sum;
+    Teacher t;
+    if (part >= 0) sum = sum_range<T, TAIL>(r, in, holes, words, p.c);
+    if (whole || part < 0) {
+      if (TAIL && whole) clear_holes(holes, words);
+      clean = whole;
+      t = learn<T, TAIL>(p, row, lists, holes, words);
+    }
+    if (!whole) {
+      unsigned order = 0;
+      if (lane == 0) {
+        if (part < 0) {
+          __stcg(reinterpret_cast<double2*>(records), make_double2(t.terms, t.all));
+          __stcg(reinterpret_cast<double2*>(records + 1), make_double2(t.norm, __hiloint2double(__float_as_int(t.listed), __float_as_int(t.listed_max))));
+        } else {
+          __stcg(records + 2 + part, make_float4(sum.x, sum.y, sum.z, 0.f));
+        }
+        __threadfence();
+        order = atomicInc(p.tickets + row, p.parts);
+      }
+      last = __shfl_sync(0xffffffffu, order, 0) == (unsigned)p.parts;
+      if (last) {
+        __threadfence();
+        const double2 a = __ldcg(reinterpret_cast<const double2*>(records)), b = __ldcg(reinterpret_cast<const double2*>(records + 1));
+        t = {a.x, a.y, b.x, __int_as_float(__double2loint(b.y)), __int_as_float(__double2hiint(b.y))};
+        sum = gather_records(records + 2, p.parts, p.c);
+      }
+    }
+    if (last && lane == 0) close_row<TAIL>(p, row, t, with_listed<TAIL>(p, t, sum));
+  }
+  if (TAIL && part >= 0 && !clean) clear_holes(holes, words);
+  __syncwarp();
+}
+
+// The loss alone: rows cut among warps.
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __grid_constant__ Distill p) {
+  extern __shared__ __align__(16) unsigned char store[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Listed lists(store, p.entries);
+  const int words = TAIL ? hole_words(p.per, sizeof(T)) : 0;
+  unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) + warp * words;
+  for (int i = lane; i < words; i += 32) holes[i] = 0;
+  grid_dependency_wait();
+  __syncwarp();
+  const int each = p.parts > 1 ? p.parts + 1 : 1;
+  const Items items(p, 1, each);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item);
+    distill_part<T, TAIL>(p, row, (int)(item - row * each) - (each > 1), lists, holes, words);
+  }
+  grid_dependency_launch();
+}
+
+// A part of a row's gradient, by W warps that own each their vectors of it, and the listed elements in those: g (whole p - q), elsewhere a p.
+// The listed logits are read before the part is streamed (dx may be the logits themselves).  entry, q, x: lists of the warp's own.
+template <typename T, int W, typename P>
+__device__ __forceinline__ void distill_gradient(const P& p, long long row, int part, const float4 saved, int* entry, float* weight, float* x) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Range<T> r = range_of<T>(p, row, part);
+  const Inner in(r);
+  T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
+  if (saved.z == 0.f) {
+    stream_zeros<T, W>(r, dst);
+    return;
+  }
+  const bool list_is_all = saved.z < 0.f;  // of the teacher's distribution
+  const double norm = (double)saved.w + (list_is_all ? (double)saved.y : 0.);
+  int own = 0;
+  __syncwarp();
+  for (int j0 = 0; j0 < p.entries; j0 += 32) {
+    const int j = j0 + lane;
+    const long long id = j < p.entries ? load_id(p.ids, row * p.entries + j, p.id_bits) : 0;
+    if (id < 0 || id > p.n) atomicMax(p.status, DEV_BAD_INDEX);
+    bool mine = id <= p.n && in_range(r, id) != 0;
+    if (W > 1 && mine) {
+      const int v = (int)((id - 1 + r.off) / Range<T>::V);
+      mine = (v < in.a || v >= in.b ? 0 : (v - in.a) % (W * 32) >> 5) == warp;
+    }
+    const unsigned all = __ballot_sync(0xffffffffu, mine);
+    if (mine) {
+      const int at = own + __popc(all & ((1u << lane) - 1));
+      entry[at] = (int)id;
+      weight[at] = __int_as_float(j);
+    }
+    own += __popc(all);
+  }
+  __syncwarp();
+  for (int k = lane; k < own; k += 32) {
+    const float value = load_value(p.values, row * p.entries + __float_as_int(weight[k]), p.values_dtype);
+    x[k] = to_float(r.src[entry[k] - 1]);
+    weight[k] = exp_of(fma((double)value, p.per_temperature, -norm));
+  }
+  const float g = p.d_loss[row] / p.temperature, lse2 = saved.x * kLog2e;
+  const float a = g * (list_is_all ? 1.f : saved.y), whole = list_is_all ? 1.f : saved.z;
+  __syncwarp();
+  stream_gradient<T, false, W>(r, in, dst, p.c, lse2, a, 0.f);
+  __syncwarp();
+  for (int k = lane; k < own; k += 32) {
+    const int id = entry[k];
+    float q = 0.f;
+    bool first = true;
+    for (int i = 0; i < own; ++i)
+      if (entry[i] == id) {
+        first &= i >= k;
+        q += weight[i];
+      }
+    if (first) dst[id - 1] = from_float<T>(g * (whole * ex2_approx_ftz(fmaf(x[k], p.c, -lse2)) - q));
+  }
+  __syncwarp();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kBackwardPerSm) distill_backward_kernel(const __grid_constant__ Backward p) {
+  extern __shared__ __align__(16) unsigned char store[];
+  const Listed lists(store, p.entries);
+  grid_dependency_wait();
+  const Items items(p, kWarps);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item);
+    distill_gradient<T, kWarps>(p, row, (int)(item - row * p.parts), reinterpret_cast<const float4*>(p.saved)[row], lists.entry, lists.q, lists.x);
+  }
+  grid_dependency_launch();
+}
+template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kernel(const __grid_constant__ Backward p) {
-  constexpr int kEntries = DISTILL ? kMaxEntries : kMaxTop + 1;
+  constexpr int kEntries = kMaxTop + 1;
   __shared__ int entries_of[kWarps][kEntries];
   __shared__ float weights_of[kWarps][kEntries], logits_of[kWarps][kEntries];
   grid_dependency_wait();
@@ -1330,9 +1365,9 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
       weight[j] = w;
       x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
     };
-    float lse2, a, b = 0.f, g = 0.f, whole = 1.f;
+    float lse2, a, b = 0.f;
     int entries;
-    if constexpr (!DISTILL) {
+    {
       const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
       const bool bad = p.tokens && (token < 0 || token > p.n);
       if (token == 0 || bad) {
@@ -1348,32 +1383,12 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
       lse2 = p.lse[row] * kLog2e;
       a = -(all + gh * h) / p.temperature;
       b = -gh * kLn2 / p.temperature;
-    } else {
-      const float4 saved = reinterpret_cast<const float4*>(p.saved)[row];
-      if (saved.z == 0.f) {
-        stream_zeros<T, kWarps>(r, dst);
-        continue;
-      }
-      const bool list_is_all = saved.z < 0.f;  // of the teacher's distribution
-      const double norm = (double)saved.w + (list_is_all ? (double)saved.y : 0.);
-      entries = p.entries;
-      for (int j = lane; j < entries; j += 32) {
-        const long long id = load_id(p.ids, row * entries + j, p.id_bits);
-        float q = 0.f;
-        if (in_range(r, id))
-          q = exp_of((double)load_value(p.values, row * entries + j, p.values_dtype) / (double)p.temperature - norm);
-        enter(j, id, q);
-      }
-      g = p.d_loss[row] / p.temperature;
-      lse2 = saved.x * kLog2e;
-      a = g * (list_is_all ? 1.f : saved.y);
-      whole = list_is_all ? 1.f : saved.z;
     }
     __syncwarp();
     stream_gradient<T, ENTROPY, kWarps>(r, in, dst, p.c, lse2, a, b);
     patch_entries<kWarps>(r, in, entry, weight, entries, [&](int id, int j, float sum) {
       const float t = fmaf(x[j], p.c, -lse2), e = ex2_approx_ftz(t);
-      dst[id - 1] = from_float<T>(DISTILL ? g * (whole * e - sum) : sum / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
+      dst[id - 1] = from_float<T>(sum / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
     });
   }
   grid_dependency_launch();
@@ -1438,13 +1453,12 @@ struct Cut {
   int parts, teams;
 };
 template <auto KERNEL>
-Cut cut_rows(ctb_ctx* ctx, int64_t rows, int64_t row_bytes, int per_sm, int least, double ends) {
+Cut cut_rows(ctb_ctx* ctx, int64_t rows, int64_t row_bytes, int per_sm, double ends) {
   constexpr double kAlone = 20e3, kAll = 6500e3, kMeeting = 2.5;
   Cut best = {0, 0};
   double best_time = 0;
   for (int C = 1; C <= kMaxCluster; C *= 2) {
-    if (C < least) continue;
-    if (row_bytes / C < 4096 && C > least) break;
+    if (row_bytes / C < 4096 && C > 1) break;
     const int most = C == 1 ? ctx->sm_count * per_sm : most_teams<KERNEL>(ctx, C, per_sm, 0, true);
     if (most < 1) continue;
     const int teams = (int)std::min<int64_t>(rows, most);
@@ -1471,16 +1485,18 @@ void cut_into(Rows& p, int64_t nvec, int64_t parts) {
 }
 // Rows cut among warps: into the parts for which rounds of parts take the least time.  A warp reads `alone` bytes per ns when nobody else reads
 // and shares what HBM gives otherwise, and a part costs `ends` besides (us); measured with 1 to 2220 rows of 50000 to 128000 elements.
-void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t most, double ends) {
+void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t least, int64_t most, int more,
+                     double ends) {
   const double alone = elem == 4 ? 5.1 : 3.5, all = 7600, bytes = (double)nvec * 16e-3;  // of a row, in 1000
   double best = 0;
   int64_t parts = 1;
   most = std::min({most, std::max<int64_t>(1, nvec / 128), std::max<int64_t>(1, 16 * places / std::max(1, p.rows))});  // 2 KB; 16 rounds
-  for (int64_t n = 1; n <= most; n = n < 64 ? n + 1 : n + n / 8) {
-    const int64_t items = p.rows * n, full = items / places, rest = items % places;
+  least = std::min(least, most);
+  for (int64_t n = least; n <= most; n = n < 64 ? n + 1 : n + n / 8) {
+    const int64_t items = p.rows * (n + (n > 1 ? more : 0)), full = items / places, rest = items % places;
     auto round = [&](int64_t active) { return bytes / (double)n * (1 / alone + (double)active / all) + ends; };
     const double time = (double)full * round(places) + (rest ? round(rest) : 0) + 0.01 * (double)n;
-    if (n == 1 || time < best) {
+    if (n == least || time < best) {
       best = time;
       parts = n;
     }
@@ -1488,37 +1504,50 @@ void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t mo
   p.per = (int)(((nvec + parts - 1) / parts + 31) / 32 * 32);
   p.parts = (int)((nvec + p.per - 1) / p.per);
 }
-// Rows cut among CTAs that share nothing: parts of up to four tiles (64 KB), of one where that brings work to more SMs.
+// Rows cut among CTAs that share nothing, in parts of whole tiles: those for which rounds of parts, with half a tile for what begins and ends
+// one, take the least time.
 void cut_rows_into_parts(Rows& p, int64_t nvec, int64_t places) {
-  const int64_t tiles = (nvec + kTile - 1) / kTile, each = p.rows * tiles >= 16 * places ? 4 : p.rows * tiles >= 8 * places ? 2 : 1;
-  cut_into(p, nvec, (tiles + each - 1) / each);
+  const int64_t tiles = (nvec + kTile - 1) / kTile;
+  double best = 0;
+  int64_t per = 1;
+  for (int64_t each = std::min<int64_t>(tiles, 16); each >= 1; --each) {
+    const int64_t items = p.rows * ((tiles + each - 1) / each);
+    const double time = (double)((items + places - 1) / places) * ((double)each + 0.5);
+    if (best == 0 || time < best) {
+      best = time;
+      per = each;
+    }
+  }
+  p.per = (int)(per * kTile);
+  p.parts = (int)((nvec + p.per - 1) / p.per);
 }
 // Parts that a row may have whose sums meet in scratch memory: as many as their records and counters have room for.
-int64_t most_parts(const Rows& p) {
+int64_t most_parts(const Rows& p, int more) {
   if (p.rows > kTickets) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows));
+  return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows - more));
 }
 
 // Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element.
 template <auto KERNEL, typename T, typename P>
-int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, double ends, const char* who) {
+int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, bool taught, double ends, const char* who) {
   const int64_t places = (int64_t)kPlainPerSm * ctx->sm_count * kWarps, nvec = vectors<T>(p);
+  size_t lists = 0;
+  if constexpr (std::is_same<P, Distill>::value) lists = 4 * (size_t)lists_words(p.entries);
   auto go = [&] {
-    const size_t smem = (bits ? (size_t)kWarps * 4 * (p.per * (16 / sizeof(T)) / 32) : 0);
+    const size_t smem = lists + (bits ? (size_t)kWarps * 4 * hole_words(p.per, sizeof(T)) : 0);
     int per_sm = kPlainPerSm;
     if (smem > 0) {
-      if (smem > 200 * 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
-      cudaError_t e = allow_smem(KERNEL, 200 * 1024);
+      if (smem > kMostShared) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
+      cudaError_t e = smem > 48 * 1024 ? allow_smem(KERNEL, kMostShared) : cudaSuccess;
       if (e != cudaSuccess) return cuda_fail(e, who);
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, kThreads, smem);
-      per_sm = std::max(1, std::min(kPlainPerSm, per_sm));
+      per_sm = std::max(1, std::min(kPlainPerSm, (int)(kMostShared / (smem + 1024))));
     }
-    const int64_t ctas = ((int64_t)p.rows * p.parts + kWarps - 1) / kWarps;
+    const int64_t ctas = ((int64_t)p.rows * (p.parts + (taught && p.parts > 1)) + kWarps - 1) / kWarps;
     launch_kernel(KERNEL, (int)std::min<int64_t>(ctas, (int64_t)per_sm * ctx->sm_count), kThreads, smem, st, 0, p);
     CTB_CHECK_LAUNCH(who);
     return (int)CTB_OK;
   };
-  cut_among_warps(p, nvec, sizeof(T), places, most_parts(p), ends);
+  cut_among_warps(p, nvec, sizeof(T), places, bits ? p.n / 16384 + 1 : 1, most_parts(p, taught ? 2 : 0), taught, ends);
   if (p.parts > 1) {
     StreamScratch scratch(ctx, st);
     if (scratch.data) {
@@ -1531,59 +1560,39 @@ int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, double ends, con
   return go();
 }
 
-// Launches a kernel of run_rows.  bits: two sets of a bit per element of a part in shared memory.
+// Launches a kernel of run_rows.
 template <auto KERNEL, typename T, typename P>
-int launch_rows(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, bool bits, double ends, const char* who) {
-  constexpr int V = 16 / (int)sizeof(T);
+int launch_rows(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, double ends, const char* who) {
   const int64_t nvec = vectors<T>(p);
-  cudaError_t e = bits ? allow_smem(KERNEL, (kMostHoles + 1024) / 4) : cudaSuccess;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return cuda_fail(e, who);
-  int least = 1;
-  if (bits)
-    while (least < kMaxCluster && nvec * V > (int64_t)least * kMostHoles) least *= 2;
-  Cut cut = cut_rows<KERNEL>(ctx, p.rows, nvec * 16, per_sm, least, ends);
+  const Cut cut = cut_rows<KERNEL>(ctx, p.rows, nvec * 16, per_sm, ends);
   if (cut.parts == 0) return fail(CTB_UNSUPPORTED, "%s: no room for a row's CTAs on this device", who);
   cut_into(p, nvec, cut.parts);
-  size_t smem = 0;
-  if (bits) {  // more shared memory may leave room for fewer
-    if ((int64_t)p.per * V > kMostHoles + 1024) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, rows of %d elements are too long", who, p.n);
-    smem = 2 * 4 * ((size_t)p.per * V / 32);
-    int fit = 0;
-    if (p.parts > 1) {
-      fit = most_teams<KERNEL>(ctx, p.parts, per_sm, smem, false);
-    } else {
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, KERNEL, kAllThreads, smem);
-      fit *= ctx->sm_count;
-    }
-    cut.teams = std::max(1, std::min(cut.teams, fit));
-  }
-  launch_kernel(KERNEL, cut.teams * p.parts, kAllThreads, smem, st, p.parts, p);
+  launch_kernel(KERNEL, cut.teams * p.parts, kAllThreads, 0, st, p.parts, p);
   CTB_CHECK_LAUNCH(who);
   return CTB_OK;
 }
 
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
-  if (p.top) return launch_rows<top_logprobs_kernel<T>, T>(ctx, st, p, kTopPerSm, false, 3.0, who);
-  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, 3.0, who);
+  if (p.top) return launch_rows<top_logprobs_kernel<T>, T>(ctx, st, p, kTopPerSm, 3.0, who);
+  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, false, 3.0, who);
+}
+template <typename T>
+int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
+  auto kernel = p.ids ? distill_backward_kernel<T> : p.d_entropy ? logits_backward_kernel<T, true> : logits_backward_kernel<T, false>;
+  const int64_t most = (int64_t)kBackwardPerSm * ctx->sm_count;
+  cut_rows_into_parts(p, vectors<T>(p), most);
+  launch_kernel(kernel, (int)std::min<int64_t>((int64_t)p.rows * p.parts, most), kThreads,
+                p.ids ? 4 * (size_t)lists_words(p.entries) : 0, st, 0, p);
+  CTB_CHECK_LAUNCH(who);
+  return CTB_OK;
 }
 template <typename T>
 int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* who) {
-  if (p.dx)
-    return p.teacher_lse ? launch_rows<distill_both_kernel<T, true>, T>(ctx, st, p, kDistillPerSm, true, 2.5, who)
-                         : launch_rows<distill_both_kernel<T, false>, T>(ctx, st, p, kDistillPerSm, false, 2.5, who);
-  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, true, 5.0, who)
-                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, false, 5.0, who);
-}
-template <typename T, bool DISTILL>
-int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
-  auto kernel = p.d_entropy ? logits_backward_kernel<T, DISTILL, !DISTILL> : logits_backward_kernel<T, DISTILL, false>;
-  const int64_t most = (int64_t)kBackwardPerSm * ctx->sm_count;
-  cut_rows_into_parts(p, vectors<T>(p), most);
-  launch_kernel(kernel, (int)std::min<int64_t>((int64_t)p.rows * p.parts, most), kThreads, 0, st, 0, p);
-  CTB_CHECK_LAUNCH(who);
-  return CTB_OK;
+  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, true, true, 3.0, who)
+                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, false, true, 3.0, who);
 }
 template <typename F>
 int by_type(int dtype, F f) {
@@ -1672,13 +1681,12 @@ extern "C" int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits
   p.status = ctx->dev_status;
   p.tokens = tokens; p.token_bits = token_bits; p.top = top;
   p.lse = lse; p.entropy = entropy; p.d_logprobs = d_logprobs; p.d_entropy = d_entropy; p.d_top = d_top_logprobs; p.top_ids = top_ids;
-  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t), false>(ctx, static_cast<cudaStream_t>(stream), p, who); });
+  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t)>(ctx, static_cast<cudaStream_t>(stream), p, who); });
 }
 
 static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
                            const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
-                           const float* d_loss, void* d_logits, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries,
-                           float temperature, int dtype) {
+                           int64_t V, int64_t T, int64_t ld, int entries, float temperature, int dtype) {
   if (int s = check_rows(who, logits, V, T, ld, temperature, dtype)) return s;
   if (T == 0) return CTB_OK;
   if (int s = check_teacher(who, teacher_ids, id_bits, teacher_values, values_dtype, entries)) return s;
@@ -1693,9 +1701,21 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   p.status = ctx->dev_status;
   p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
   p.teacher_lse = teacher_lse; p.per_temperature = 1 / (double)temperature; p.loss = loss; p.saved = saved;
-  p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(ctx, st, p, who); });
+}
+
+static int distill_backward(const char* who, ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
+                            const void* teacher_values, int values_dtype, const float* saved, const float* d_loss, int64_t V, int64_t T,
+                            int64_t ld_out, int64_t ld, int entries, float temperature, int dtype) {
+  Backward p = {};
+  p.x = logits; p.ld = ld; p.dx = d_logits; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
+  p.c = (float)(1.4426950408889634 / (double)temperature);
+  p.temperature = temperature;
+  p.status = ctx->dev_status;
+  p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
+  p.saved = saved; p.d_loss = d_loss; p.per_temperature = 1 / (double)temperature;
+  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t)>(ctx, static_cast<cudaStream_t>(stream), p, who); });
 }
 
 extern "C" int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
@@ -1704,7 +1724,7 @@ extern "C" int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, c
   CTB_CHECK_CTX(ctx);
   CurrentDevice current(ctx);
   return distill_forward("ctb_distill_fwd", ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved,
-                         nullptr, nullptr, V, T, 0, ld, entries, temperature, dtype);
+                         V, T, ld, entries, temperature, dtype);
 }
 
 extern "C" int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
@@ -1720,16 +1740,13 @@ extern "C" int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const
   CTB_CHECK_PTR(who, saved);
   CTB_CHECK_PTR(who, d_loss);
   if ((uintptr_t)saved % 16) return fail(CTB_BAD_ALIGN, "%s: saved must be 16-byte aligned", who);
-  Backward p = {};
-  p.x = logits; p.ld = ld; p.dx = d_logits; p.ld_dx = ld_out; p.n = (int)V; p.rows = (int)T;
-  p.c = (float)(1.4426950408889634 / (double)temperature);
-  p.temperature = temperature;
-  p.status = ctx->dev_status;
-  p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
-  p.saved = saved; p.d_loss = d_loss;
-  return by_type(dtype, [&](auto t) { return launch_backward<decltype(t), true>(ctx, static_cast<cudaStream_t>(stream), p, who); });
+  return distill_backward(who, ctx, stream, d_logits, logits, teacher_ids, id_bits, teacher_values, values_dtype, saved, d_loss, V, T, ld_out,
+                          ld, entries, temperature, dtype);
 }
 
+// The loss, then its gradient.  One launch for both (warps that drew sums and, some rows behind, gradients from one counter; before that, CTAs
+// that streamed their row twice) gained 0 to 6 % on large batches and lost half on small ones: what is in flight at HBM's rate does not stay in
+// L2 until a row's sum is known.
 extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                                    const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
                                    const float* d_loss, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature,
@@ -1741,6 +1758,9 @@ extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, c
   if (T == 0) return CTB_OK;
   if (int s = check_gradient(who, logits, d_logits, V, T, ld, ld_out, dtype)) return s;
   CTB_CHECK_PTR(who, d_loss);
-    return distill_forward(who, ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved, d_loss,
-                         d_logits, V, T, ld_out, ld, entries, temperature, dtype);
+  if (int s = distill_forward(who, ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved, V, T, ld,
+                              entries, temperature, dtype))
+    return s;
+  return distill_backward(who, ctx, stream, d_logits, logits, teacher_ids, id_bits, teacher_values, values_dtype, saved, d_loss, V, T, ld_out,
+                          ld, entries, temperature, dtype);
 }
