@@ -26,13 +26,12 @@ namespace {
 
 constexpr int kThreads = 256;            // that stream
 constexpr int kWarps = kThreads / 32;
-constexpr int kAllThreads = kThreads + 32;  // with a clerk
 constexpr int kUnroll = 4;               // vectors of 16 bytes per thread and tile
 constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
 constexpr int kMaxEntries = kThreads;    // of a teacher's list
 constexpr int kCand = 1024;
-constexpr int kPlainPerSm = 6, kTopPerSm = 3, kBackwardPerSm = 5;  // CTAs on an SM
+constexpr int kPlainPerSm = 6, kTopPerSm = 4, kBackwardPerSm = 5;  // CTAs on an SM
 constexpr size_t kMostShared = 220 * 1024;  // dynamic shared memory of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -42,17 +41,6 @@ constexpr float kLowest = -16384.f;
 constexpr float kSlack = 4.f;
 constexpr float kFar = 1e30f;  // beyond, x log2(e) / temperature may overflow
 
-__device__ __forceinline__ void bar_stream() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // the streaming warps
-__device__ __forceinline__ bool all_stream(bool ok) {  // true in all of them when it is in all of them
-  int r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((int)ok)
-      : "memory");
-  return r != 0;
-}
-static_assert(kThreads == 256, "bar_stream names the number of threads");
 
 // ------------------------------------------------------------------ the best k of a row
 // One pass, every element compared with a threshold that at least k earlier elements reach:
@@ -85,7 +73,7 @@ __device__ __forceinline__ float group_threshold(float mine, int k, Best& b) {
   g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
   const int i = warp * 8 + (lane >> 2);
   if ((lane & 3) == 0) b.group[i] = g;
-  bar_stream();
+  __syncthreads();
   int rank = 0;  // among a quarter of the groups per lane
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
@@ -96,7 +84,7 @@ __device__ __forceinline__ float group_threshold(float mine, int k, Best& b) {
   rank += __shfl_xor_sync(0xffffffffu, rank, 1);
   rank += __shfl_xor_sync(0xffffffffu, rank, 2);
   if (rank == k - 1 && (lane & 3) == 0) b.theta = g;
-  bar_stream();
+  __syncthreads();
   return b.theta;
 }
 
@@ -120,22 +108,26 @@ __device__ void select_list(int n, int k, Best& b) {
       }
     value = b.value2;
     index = b.index2;
-    bar_stream();
+    __syncthreads();
     n = b.count2;
   } else {
-    bar_stream();
+    __syncthreads();
   }
-  for (int i = tid; i < n; i += kThreads) {
+  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {  // four threads rank an element
+    const int i = min(i0 + (tid >> 2), n - 1);
     const float v = value[i];
     const int id = index[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += value[j] > v || (value[j] == v && index[j] < id);
-    if (rank < k) {
+#pragma unroll 4
+    for (int j = tid & 3; j < n; j += 4) rank += value[j] > v || (value[j] == v && index[j] < id);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (rank < k && i == i0 + (tid >> 2)) {
       b.out_value[rank] = v;
       b.out_index[rank] = id;
     }
   }
-  bar_stream();
+  __syncthreads();
 }
 
 // Adds the first `need` elements that equal `value`, in the order of their indices, to the `have` listed ones; returns how many are listed.
@@ -161,7 +153,7 @@ __device__ int append_equal(const Range<T>& r, float value, int have, int need, 
       if (lane >= o) upto += x;
     }
     if (lane == 31) b.warp_n[warp] = upto;
-    bar_stream();
+    __syncthreads();
     int at = upto - mine, total = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) at += b.warp_n[w];
@@ -173,7 +165,7 @@ __device__ int append_equal(const Range<T>& r, float value, int have, int need, 
     }
     have += min(total, need);
     need -= min(total, need);
-    bar_stream();
+    __syncthreads();
   }
   return have;
 }
@@ -195,7 +187,7 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
   int want = k;
   for (int shift = 24; shift >= 0; shift -= 8) {
     hist[tid] = 0;
-    bar_stream();
+    __syncthreads();
     for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
       float f[V];
       unpack_row<T>(load_vec(r, v), f);
@@ -205,22 +197,22 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
         if (f[i] == f[i] && r.has(v, i) && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
       }
     }
-    bar_stream();
+    __syncthreads();
     if (tid == 0) {
       int bin = 255, above = 0;
       while (bin > 0 && above + hist[bin] < want) above += hist[bin--];
       b.bin = bin;
       b.above = above;
     }
-    bar_stream();
+    __syncthreads();
     prefix |= (uint32_t)b.bin << shift;
     mask |= 255u << shift;
     want -= b.above;
-    bar_stream();
+    __syncthreads();
   }
   const float kth = key_value(prefix);
   if (tid == 0) b.count = 0;
-  bar_stream();
+  __syncthreads();
   for (int v = r.v0 + tid; v < r.v1; v += kThreads) {
     float f[V];
     unpack_row<T>(load_vec(r, v), f);
@@ -232,7 +224,7 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
         b.index[at] = v * V - r.off + i;
       }
   }
-  bar_stream();
+  __syncthreads();
   return append_equal(r, kth, b.count, want, b);
 }
 
@@ -388,7 +380,6 @@ __device__ __forceinline__ Range<T> range_of(const Rows& p, long long row, int p
   return r;
 }
 
-constexpr int kMaxCluster = 16;
 
 // Whole vectors of a range, [a, b), and the elements before and behind them.
 struct Inner {
@@ -418,7 +409,10 @@ __device__ __forceinline__ int edge_index(const Range<T>& r, const Inner& in, in
   return -1;
 }
 // A bit per element of a warp's part, in the order in which the lanes take its vectors, kUnroll at a time; the last word: head, then tail.
-__host__ __device__ constexpr int hole_words(int per, int elem) { return (per + 32 * kUnroll - 1) / (32 * kUnroll) * kUnroll * (16 / elem) + 1; }
+__host__ __device__ constexpr int hole_words(int per, int elem) {
+  const int words = (per + 32 * kUnroll - 1) / (32 * kUnroll) * kUnroll * (16 / elem);
+  return (words > 256 ? words : 256) + 1;  // 256: the table in which equal ids meet
+}
 template <typename T>
 __device__ __forceinline__ unsigned hole_bits(const unsigned* holes, int v) {  // of a lane's vectors from v on, v counted from the first inner one
   const int at = (v / (32 * kUnroll)) * 32 + (threadIdx.x & 31), u = v / 32 % kUnroll;
@@ -494,14 +488,14 @@ struct Items {  // of a warp (or, with W = 8, of the warps of a CTA, which share
 };
 // After a warp has summed a part: true for the row's last one, with the row's (maximum, s, w).
 // A row's (maximum, s, w) from those of its parts.
-__device__ __forceinline__ float3 gather_records(const float4* records, int parts, float c) {
+__device__ __forceinline__ float3 gather_records(const float4* records, int parts, int size, float c) {
   const int lane = threadIdx.x & 31;
   float most = -FLT_MAX;
-  for (int i = lane; i < parts; i += 32) most = fmaxf(most, __ldcg(&records[i].x));
+  for (int i = lane; i < parts; i += 32) most = fmaxf(most, __ldcg(&records[i * size].x));
   most = warp_max(most);
   float s = 0.f, w = 0.f;
   for (int i = lane; i < parts; i += 32) {
-    const float4 one = __ldcg(records + i);
+    const float4 one = __ldcg(records + i * size);
     const float d = (one.x - most) * c, r = ex2_approx_ftz(d);
     s = fmaf(one.y, r, s);
     w += r * fmaf(one.y, fmaxf(d, kLowest), one.z);
@@ -519,152 +513,8 @@ __device__ __forceinline__ bool join_records(const Rows& p, long long row, int p
   }
   if (__shfl_sync(0xffffffffu, order, 0) != (unsigned)p.parts - 1) return false;
   __threadfence();
-  sum = gather_records(records, p.parts, p.c);
+  sum = gather_records(records, p.parts, 1, p.c);
   return true;
-}
-
-// ------------------------------------------------------------------ rows through a CTA
-// Where a row's warps have to meet (thresholds of a list; a gradient that follows the sum), a CTA takes row after row, with two roles:
-//   stream   eight warps read the row
-//   clerk    a warp prepares the rows to come: whether they are padding, what the operator needs besides the logits (loads that
-//            depend on loads, f64 exponentials), and joins the sums of rows that have been read
-// and the parts of a row are the CTAs of a cluster, whose sums go to each other's shared memory.
-// Sums of a row's parts in the shared memory of every CTA of the cluster, for even and odd meetings.  A peer sends to the meeting after
-// the next one only when this CTA has sent to the next, that is, has read this one.
-struct Meeting {
-  float4 part[2][kMaxCluster];
-  uint64_t bar[2];
-  volatile int abort;  // a wait ran out: no further message or wait
-};
-
-// What passes between the roles: lesson n is posted by the clerk in slot n % 4, summed by the eight warps, answered by the clerk.
-struct Pipe {
-  uint64_t posted[4], summed[4], answered[4];
-  float red[4][3][kWarps];
-  volatile int abort;
-};
-
-// The frame of the kernels.  Op has
-//   Lesson                          what the clerk prepares for a row; .at is the row, -1 behind the last one
-//   prepare(lesson, row)            the clerk: false for padding whose results it has written
-//   before(n, lessons), after(n, lessons)   the clerk, before and after lesson n is made
-//   stream(n, lesson, range, inner, red)    the streaming warps
-//   answer(n, lesson, red)          the clerk, when all warps have streamed
-//   MEETS                           the streaming warps meet at barriers of their own
-//   close(lesson)                   the clerk, behind it
-//   AGAIN, again(lesson, range, inner)      the streaming warps, once the row has been answered
-template <typename T, typename Op>
-__device__ __forceinline__ void run_rows(const Rows& p, Op& op, typename Op::Lesson* lessons, Pipe& pipe, Meeting* meeting) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool cluster = p.parts > 1;
-  if (tid == 0) {
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&pipe.posted[i], 1);
-      mbar_init(&pipe.summed[i], kWarps);
-      mbar_init(&pipe.answered[i], 1);
-    }
-    pipe.abort = 0;
-    if (cluster) {
-      for (int i = 0; i < 2; ++i) mbar_init(&meeting->bar[i], 1);
-      meeting->abort = 0;
-    }
-    fence_mbar_init();
-  }
-  __syncthreads();
-  if (cluster) {  // the peers' shared memory and barriers exist
-    cluster_arrive();
-    cluster_wait();
-  }
-  grid_dependency_wait();
-  const int step = gridDim.x / p.parts, rank = cluster ? (int)cluster_ctarank() : 0;
-  auto wait = [&](uint64_t* bar, int n) {
-    const int ok = lane == 0 ? (int)mbar_watch(bar, (n >> 2) & 1, p.status, DEV_TIMEOUT_SLOT, &pipe.abort) : 1;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
-  };
-  if (warp == kWarps) {
-    long long at = (long long)(blockIdx.x / p.parts) - step;
-    auto make = [&](int n) {  // lesson n - 4 has been read by all, lesson n - 2 has been answered
-      typename Op::Lesson& l = lessons[n & 3];
-      op.before(n, lessons);
-      do at += step;
-      while (at < p.rows && !op.prepare(l, at));
-      if (lane == 0) l.at = at < p.rows ? at : -1;
-      __syncwarp();
-      op.after(n, lessons);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pipe.posted[n & 3]);
-    };
-    make(0);
-    make(1);
-    for (int n = 0; lessons[n & 3].at >= 0; ++n) {
-      if (!wait(&pipe.summed[n & 3], n)) break;
-      op.answer(n, lessons[n & 3], pipe.red[n & 3]);
-      __syncwarp();
-      if (Op::AGAIN && lane == 0) mbar_arrive(&pipe.answered[n & 3]);
-      op.close(lessons[n & 3]);
-      __syncwarp();
-      make(n + 2);
-    }
-  } else {
-    auto again = [&](int n) {
-      if (!wait(&pipe.answered[n & 3], n)) return false;
-      const typename Op::Lesson& l = lessons[n & 3];
-      const Range<T> r = range_of<T>(p, l.at, rank);
-      op.again(l, r, Inner(r));
-      return true;
-    };
-    for (int n = 0;; ++n) {
-      bool posted = wait(&pipe.posted[n & 3], n);
-      if constexpr (Op::MEETS) posted = all_stream(posted);  // none stays behind at a barrier of the others
-      if (!posted) break;
-      const typename Op::Lesson& l = lessons[n & 3];
-      if (l.at >= 0) {
-        const Range<T> r = range_of<T>(p, l.at, rank);
-        op.stream(n, l, r, Inner(r), pipe.red[n & 3]);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pipe.summed[n & 3]);
-      }
-      if (l.at < 0) break;
-      if (Op::AGAIN && !again(n)) break;
-    }
-  }
-  __syncthreads();
-  // The next kernel's CTAs come now: those that come while others of this one still run gather where rows happen to end first, and then share
-  // an SM among more rows than elsewhere (2220 x 100000 bf16: 110 us for 85).
-  grid_dependency_launch();
-  if (cluster) {  // no peer sends any more, and what they have sent is there unless a wait ran out
-    cluster_arrive_relaxed();
-    cluster_wait();
-    let_copies_land(&meeting->abort);
-  }
-}
-
-// Sends (maximum, s, w) of this CTA's part to its row's CTAs; warp 0.  extra: bytes that come besides.
-__device__ __forceinline__ void send_part(const Rows& p, Meeting& m, int turn, float3 mine, uint32_t extra) {
-  const int lane = threadIdx.x & 31;
-  if (m.abort) return;
-  __syncwarp();
-  if (lane == 0) mbar_expect_tx(&m.bar[turn & 1], p.parts * (uint32_t)sizeof(float4) + extra);
-  if (lane < p.parts) send4_to_cta(&m.part[turn & 1][cluster_ctarank()], make_float4(mine.x, mine.y, mine.z, 0.f), &m.bar[turn & 1], lane);
-}
-// Waits for all parts; a warp.
-__device__ __forceinline__ void await_parts(const Rows& p, Meeting& m, int turn) {
-  if (m.abort) return;
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) (void)mbar_wait<true>(&m.bar[turn & 1], (turn >> 1) & 1, p.status, DEV_TIMEOUT_TMA, &m.abort);
-  __syncwarp();
-  (void)mbar_try_wait<true>(&m.bar[turn & 1], (turn >> 1) & 1);  // every lane acquires what the peers sent
-}
-// (maximum, s, w) of all parts, in all lanes of a warp.
-__device__ __forceinline__ float3 join_parts(const Rows& p, const Meeting& m, int turn) {
-  const int i = threadIdx.x & (kMaxCluster - 1);
-  const float4 one = i < p.parts ? m.part[turn & 1][i] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  float most = one.x;
-#pragma unroll
-  for (int o = kMaxCluster / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  most = fmaxf(most, -FLT_MAX);
-  const float2 sum = join<kMaxCluster>((one.x - most) * p.c, one.y, one.z);
-  return make_float3(most, sum.x, sum.y);
 }
 
 // ------------------------------------------------------------------ log probabilities, forward
@@ -674,16 +524,6 @@ struct Logprobs : Rows {
   float *logprobs, *entropy, *lse, *top_logprobs;
   int* top_ids;
 };
-struct LogprobsLesson {
-  long long at;
-  int token;
-  float x;  // the token's logit
-};
-struct Lists {  // of the parts, in the first CTA of a row
-  float2 entry[2][kMaxCluster * kMaxTop];
-};
-
-// A warp writes a row's results from its (maximum, s, w).  token: of the row, or -1 for one out of range; x: its logit.
 __device__ __forceinline__ void write_results(const Logprobs& p, long long row, int token, float x, float3 sum) {
   if ((threadIdx.x & 31) != 0) return;
   const float log_sum = logf(sum.y);
@@ -749,48 +589,55 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) logprobs_kernel(const _
 }
 
 // With alternatives the eight warps meet at barriers of their own, for the thresholds of the list.
+__device__ __forceinline__ void list_one(float value, int index, float theta, Best& best) {
+  if (value > theta) {
+    const int at = atomicAdd(&best.count, 1);
+    if (at < kCand) {
+      best.value[at] = value;
+      best.index[at] = index;
+    }
+  }
+}
+// A call: in line it takes registers that the loop over tiles needs.
 template <typename T>
-struct TopOp {
-  using Lesson = LogprobsLesson;
-  static constexpr bool AGAIN = false, MEETS = true;
-  const Logprobs& p;
-  Best& best;
-  Lists& lists;
-  Meeting& meeting;
-  float theta;
+__device__ __noinline__ void list_vector(uint4 q, int index, float theta, Best& best) {
+  float f[16 / sizeof(T)];
+  unpack_row<T>(q, f);
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) list_one(f[i], index + i, theta, best);
+}
+// What a part leaves, in float4s: its sums, and a list of values and indices.
+__host__ __device__ constexpr int record_size(int top) { return 1 + (top + 1) / 2; }
 
-  __device__ __forceinline__ void before(int, const Lesson*) {}
-  __device__ __forceinline__ void after(int, const Lesson*) {}
-  __device__ __forceinline__ bool prepare(Lesson& l, long long row) {
-    const int token = token_of(p, row);
+// With alternatives: rows, or parts of rows, a CTA each, whose threads meet for thresholds and lists.  The last CTA of a row joins the lists of
+// its parts.  A list per warp, over parts of 16 KB, took twice as long: thresholds over so little are low, and choosing from lists is
+// a chain of reductions.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kTopPerSm) top_logprobs_kernel(const __grid_constant__ Logprobs p) {
+  __shared__ Best best;
+  __shared__ float red[3][kWarps];
+  __shared__ bool shared_last;
+  constexpr int V = Range<T>::V;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_wait();
+  const Items items(p, kWarps);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item);
+    const int part = (int)(item - row * p.parts), token = token_of(p, row);
     if (token == 0) {
-      if (p.parts == 1 || cluster_ctarank() == 0) write_padding(p, row);
-      return false;
+      if (part == 0 && warp == 0) write_padding(p, row);
+      continue;
     }
-    if ((threadIdx.x & 31) == 0) {
-      l.token = token;
-      l.x = token > 0 ? to_float((static_cast<const T*>(p.x) + row * p.ld)[token - 1]) : 0.f;
-    }
-    return true;
-  }
-
-  __device__ __forceinline__ void list(float x, int index) {
-    if (x > theta) {
-      const int pos = atomicAdd(&best.count, 1);
-      if (pos < kCand) {
-        best.value[pos] = x;
-        best.index[pos] = index;
-      }
-    }
-  }
-  __device__ __forceinline__ void stream(int n, const Lesson& l, const Range<T>& r, const Inner& in, float (&red)[3][kWarps]) {
-    constexpr int V = Range<T>::V;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, edge = edge_index(r, in, tid);
-    const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
+    const float x = token > 0 ? to_float((static_cast<const T*>(p.x) + row * p.ld)[token - 1]) : 0.f;
+    __syncthreads();  // the item before is done with
+    const Range<T> r = range_of<T>(p, row, part);
+    const Inner in(r);
+    const int edge = edge_index(r, in, tid);
+    const float at_edge = edge >= 0 ? to_float(r.src[edge]) : 0.f;
     Sums<T, true> sums;
     if (tid == 0) best.count = 0;  // ahead of the barriers of the first threshold
-    theta = -INFINITY;
-    if (edge >= 0 && tid < 8) sums.add_one(x, p.c);
+    float theta = -INFINITY;
+    if (edge >= 0 && tid < 8) sums.add_one(at_edge, p.c);
     int tile = 0;
 #pragma unroll 1
     for (int v = in.a; v < in.b || tile == 0; v += kTile, ++tile) {
@@ -800,23 +647,20 @@ struct TopOp {
       const float most = sums.add(q, p.c);
       if (tile == 0) {
         theta = group_threshold(word_max<T>(sums.top), p.top, best);
-        if (edge >= 0 && tid < 8) list(x, edge);
+        if (edge >= 0 && tid < 8) list_one(at_edge, edge, theta, best);
       }
       if (most > theta) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          float f[V];
-          unpack_row<T>(q[u], f);
-          const int e0 = (v + u * kThreads + tid) * V - r.off;
-#pragma unroll
-          for (int i = 0; i < V; ++i) list(f[i], e0 + i);
+          const uint32_t largest = max_word<T>(max_word<T>(q[u].x, q[u].y), max_word<T>(q[u].z, q[u].w));
+          if (word_max<T>(largest) > theta) list_vector<T>(q[u], (v + u * kThreads + tid) * V - r.off, theta, best);
         }
       }
       if (tile > 0 && (tile & (tile + 1)) == 0 && v + kTile < in.b) theta = group_threshold(word_max<T>(sums.top), p.top, best);
     }
     if (edge >= 0 && tid >= 8) {
-      sums.add_one(x, p.c);
-      list(x, edge);
+      sums.add_one(at_edge, p.c);
+      list_one(at_edge, edge, theta, best);
     }
     const float3 of_warp = sums.over_warp(p.c);
     if (lane == 0) {
@@ -824,7 +668,7 @@ struct TopOp {
       red[1][warp] = of_warp.y;
       red[2][warp] = of_warp.z;
     }
-    bar_stream();
+    __syncthreads();
     int count = best.count;
     if (count > kCand) {
       count = radix_list(r, p.top, best);
@@ -836,57 +680,49 @@ struct TopOp {
     }
     select_list(count, p.top, best);
     float3 sum = make_float3(0.f, 0.f, 0.f);
-    const int rank = p.parts > 1 ? cluster_ctarank() : 0;
-    if (warp == 0 || (p.parts > 1 && rank == 0)) sum = join_warps<kWarps>(red, p.c);
+    if (warp == 0) sum = join_warps<kWarps>(red, p.c);
     if (p.parts > 1) {
+      const int size = record_size(p.top);
+      float4* records = p.records + row * p.parts * size;
       if (warp == 0) {
-        send_part(p, meeting, n, sum, rank == 0 ? p.parts * p.top * (uint32_t)sizeof(float2) : 0);
-        if (lane < p.top && !meeting.abort)
-          send_to_cta(&lists.entry[n & 1][rank * p.top + lane], best.out_value[lane], __int_as_float(best.out_index[lane]),
-                      &meeting.bar[n & 1], 0);
-      }
-      if (warp == 0 || rank == 0) {
-        await_parts(p, meeting, n);
-        sum = join_parts(p, meeting, n);
-      }
-      if (rank != 0) return;
-      if (tid == 0) best.count = 0;
-      bar_stream();
-      for (int i = tid; i < p.parts * p.top; i += kThreads) {
-        const float2 e = lists.entry[n & 1][i];
-        const int id = __float_as_int(e.y);
-        if (id >= 0) {
-          const int pos = atomicAdd(&best.count, 1);
-          best.value[pos] = e.x;
-          best.index[pos] = id;
+        if (lane < p.top)
+          __stcg(reinterpret_cast<float2*>(records + part * size + 1) + lane, make_float2(best.out_value[lane], __int_as_float(best.out_index[lane])));
+        if (lane == 0) __stcg(records + part * size, make_float4(sum.x, sum.y, sum.z, 0.f));
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          shared_last = atomicInc(p.tickets + row, p.parts - 1) == p.parts - 1;
+          best.count = 0;
         }
       }
-      bar_stream();
+      __syncthreads();
+      if (!shared_last) continue;
+      __threadfence();
+      for (int i = tid; i < p.parts * p.top; i += kThreads) {
+        const int of = i / p.top;
+        const float2 e = __ldcg(reinterpret_cast<const float2*>(records + of * size + 1) + (i - of * p.top));
+        const int index = __float_as_int(e.y);
+        if (index >= 0) {
+          const int at = atomicAdd(&best.count, 1);
+          best.value[at] = e.x;
+          best.index[at] = index;
+        }
+      }
+      if (warp == 0) sum = gather_records(records, p.parts, size, p.c);
+      __syncthreads();
       select_list(best.count, p.top, best);
     }
     if (warp == 0) {
       const float log_sum = logf(sum.y);
-      write_results(p, l.at, l.token, l.x, sum);
+      write_results(p, row, token, x, sum);
       if (lane < p.top) {
         const int id = best.out_index[lane];
-        p.top_logprobs[l.at * p.top + lane] = id >= 0 ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
-        p.top_ids[l.at * p.top + lane] = id + 1;
+        p.top_logprobs[row * p.top + lane] = id >= 0 ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
+        p.top_ids[row * p.top + lane] = id + 1;
       }
     }
   }
-  __device__ __forceinline__ void answer(int, const Lesson&, const float (&)[3][kWarps]) {}
-  __device__ __forceinline__ void close(const Lesson&) {}
-  __device__ __forceinline__ void again(const Lesson&, const Range<T>&, const Inner&) {}
-};
-template <typename T>
-__global__ void __launch_bounds__(kAllThreads, kTopPerSm) top_logprobs_kernel(const __grid_constant__ Logprobs p) {
-  __shared__ Pipe pipe;
-  __shared__ Meeting meeting;
-  __shared__ LogprobsLesson lessons[4];
-  __shared__ Best best;
-  __shared__ Lists lists;
-  TopOp<T> op{p, best, lists, meeting, 0.f};
-  run_rows<T>(p, op, lessons, pipe, &meeting);
+  grid_dependency_launch();
 }
 
 // ------------------------------------------------------------------ gradients
@@ -1239,7 +1075,7 @@ __device__ __forceinline__ void distill_part(const Distill& p, long long row, in
         __threadfence();
         const double2 a = __ldcg(reinterpret_cast<const double2*>(records)), b = __ldcg(reinterpret_cast<const double2*>(records + 1));
         t = {a.x, a.y, b.x, __int_as_float(__double2loint(b.y)), __int_as_float(__double2hiint(b.y))};
-        sum = gather_records(records + 2, p.parts, p.c);
+        sum = gather_records(records + 2, p.parts, 1, p.c);
       }
     }
     if (last && lane == 0) close_row<TAIL>(p, row, t, with_listed<TAIL>(p, t, sum));
@@ -1420,60 +1256,6 @@ int check_gradient(const char* who, const void* x, void* dx, int64_t V, int64_t 
     if (!is_device_ptr(p)) return fail(CTB_BAD_ARG, "%s: argument %s is not a device pointer", who, #p); \
   } while (0)
 
-// Clusters of C CTAs of a kernel that run at once.
-template <auto KERNEL>
-int most_teams(ctb_ctx* ctx, int C, int per_sm, size_t smem, bool keep) {
-  static std::atomic<int> cached[16][kMaxCluster + 1];
-  std::atomic<int>& known = cached[ctx->device & 15][C];
-  if (keep && known.load(std::memory_order_relaxed) > 0) return known.load(std::memory_order_relaxed);
-  int n = 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctx->sm_count * per_sm / C * C);
-  cfg.blockDim = dim3(kAllThreads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
-    (void)cudaGetLastError();
-    n = 0;
-  }
-  if (keep && n > 0) known.store(n, std::memory_order_relaxed);
-  return n;
-}
-
-// How the rows are cut: for the kernels whose parts meet, into the 1, 2, 4, 8 or 16 CTAs of a cluster.  Rows go over the teams in rounds;
-// a round takes the time of its bytes at the rate of HBM, but no less than a part at the rate that a CTA reaches alone, and what begins
-// and ends a row (`ends`, and a meeting).  Times in us, rates in bytes per us.
-struct Cut {
-  int parts, teams;
-};
-template <auto KERNEL>
-Cut cut_rows(ctb_ctx* ctx, int64_t rows, int64_t row_bytes, int per_sm, double ends) {
-  constexpr double kAlone = 20e3, kAll = 6500e3, kMeeting = 2.5;
-  Cut best = {0, 0};
-  double best_time = 0;
-  for (int C = 1; C <= kMaxCluster; C *= 2) {
-    if (row_bytes / C < 4096 && C > 1) break;
-    const int most = C == 1 ? ctx->sm_count * per_sm : most_teams<KERNEL>(ctx, C, per_sm, 0, true);
-    if (most < 1) continue;
-    const int teams = (int)std::min<int64_t>(rows, most);
-    const double part = (double)row_bytes / C / kAlone + ends + (C > 1 ? kMeeting : 0.);
-    const int64_t full = rows / teams, rest = rows % teams;
-    const double time = (double)full * std::max((double)teams * (double)row_bytes / kAll, part) +
-                        (rest ? std::max((double)rest * (double)row_bytes / kAll, part) : 0.);
-    if (best.parts == 0 || time < best_time) {
-      best = {C, teams};
-      best_time = time;
-    }
-  }
-  return best;
-}
-
 template <typename T>
 int64_t vectors(const Rows& p) {  // of a row, wherever it starts
   constexpr int V = 16 / (int)sizeof(T);
@@ -1522,9 +1304,9 @@ void cut_rows_into_parts(Rows& p, int64_t nvec, int64_t places) {
   p.parts = (int)((nvec + p.per - 1) / p.per);
 }
 // Parts that a row may have whose sums meet in scratch memory: as many as their records and counters have room for.
-int64_t most_parts(const Rows& p, int more) {
+int64_t most_parts(const Rows& p, int record, int more) {
   if (p.rows > kTickets) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows - more));
+  return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kStreamScratchBytes / (int64_t)sizeof(float4) / p.rows / record - more));
 }
 
 // Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element.
@@ -1547,7 +1329,7 @@ int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, bool taught, dou
     CTB_CHECK_LAUNCH(who);
     return (int)CTB_OK;
   };
-  cut_among_warps(p, nvec, sizeof(T), places, bits ? p.n / 16384 + 1 : 1, most_parts(p, taught ? 2 : 0), taught, ends);
+  cut_among_warps(p, nvec, sizeof(T), places, bits ? p.n / 16384 + 1 : 1, most_parts(p, 1, taught ? 2 : 0), taught, ends);
   if (p.parts > 1) {
     StreamScratch scratch(ctx, st);
     if (scratch.data) {
@@ -1560,24 +1342,46 @@ int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, bool taught, dou
   return go();
 }
 
-// Launches a kernel of run_rows.
-template <auto KERNEL, typename T, typename P>
-int launch_rows(ctb_ctx* ctx, cudaStream_t st, P p, int per_sm, double ends, const char* who) {
-  const int64_t nvec = vectors<T>(p);
-  cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  const Cut cut = cut_rows<KERNEL>(ctx, p.rows, nvec * 16, per_sm, ends);
-  if (cut.parts == 0) return fail(CTB_UNSUPPORTED, "%s: no room for a row's CTAs on this device", who);
-  cut_into(p, nvec, cut.parts);
-  launch_kernel(KERNEL, cut.teams * p.parts, kAllThreads, 0, st, p.parts, p);
-  CTB_CHECK_LAUNCH(who);
-  return CTB_OK;
+// With alternatives: parts of whole tiles, a CTA each, those for which rounds of parts take the least time.  A CTA reads 20 bytes per ns when
+// nobody else reads, a part costs 3 us besides, and lists that are joined 2.5 (measured with 1 to 2220 rows of 32000 to 128000 elements).
+template <typename T>
+int launch_top(ctb_ctx* ctx, cudaStream_t st, Logprobs p, const char* who) {
+  const int64_t nvec = vectors<T>(p), tiles = (nvec + kTile - 1) / kTile, places = (int64_t)kTopPerSm * ctx->sm_count;
+  const int64_t most = std::min<int64_t>(most_parts(p, record_size(p.top), 0), kCand / p.top);
+  double best = 0;
+  p.per = (int)(tiles * kTile);
+  p.parts = 1;
+  for (int64_t n = 1; n <= std::min(most, tiles); ++n) {
+    const int64_t each = (tiles + n - 1) / n, parts = (tiles + each - 1) / each, items = p.rows * parts;
+    const double bytes = (double)each * kTile * 16;
+    auto round = [&](int64_t active) { return std::max((double)active * bytes / 6500e3, bytes / 20e3 + 3.0); };
+    const double time = (double)(items / places) * round(places) + (items % places ? round(items % places) : 0) + (parts > 1 ? 2.5 : 0);
+    if (n == 1 || time < best) {
+      best = time;
+      p.per = (int)(each * kTile);
+      p.parts = (int)parts;
+    }
+  }
+  auto go = [&] {
+    launch_kernel(top_logprobs_kernel<T>, (int)std::min<int64_t>((int64_t)p.rows * p.parts, places), kThreads, 0, st, 0, p);
+    CTB_CHECK_LAUNCH(who);
+    return (int)CTB_OK;
+  };
+  if (p.parts > 1) {
+    StreamScratch scratch(ctx, st);
+    if (scratch.data) {
+      p.records = reinterpret_cast<float4*>(scratch.data);
+      p.tickets = scratch.tickets;
+      return go();
+    }
+    p.per = (int)(tiles * kTile);
+    p.parts = 1;
+  }
+  return go();
 }
-
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
-  if (p.top) return launch_rows<top_logprobs_kernel<T>, T>(ctx, st, p, kTopPerSm, 3.0, who);
-  return launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, false, 3.0, who);
+  return p.top ? launch_top<T>(ctx, st, p, who) : launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, false, 3.0, who);
 }
 template <typename T>
 int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
