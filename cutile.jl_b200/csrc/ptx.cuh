@@ -55,12 +55,6 @@ __device__ __forceinline__ void grid_dependency_sync() {
 __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -125,36 +119,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         if (status) atomicMax(status, code);
         if (abort) *abort = 1;
-        return false;
-      }
-    }
-  }
-}
-
-// The same for a warp that waits for long beside others that work: it looks (test_wait does not suspend) and sleeps in turn.  A suspended
-// try_wait holds up other warps' shuffles and shared-memory accesses: five shuffles of a streaming warp took 16000 clocks beside one.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_watch(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort) {
-  if (mbar_test(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t i = 1;; ++i) {
-    __nanosleep(40);
-    if (mbar_test(bar, parity)) return true;
-    if ((i & 15u) == 0) {
-      if (*abort) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        if (status) atomicMax(status, code);
-        *abort = 1;
         return false;
       }
     }
@@ -307,13 +271,6 @@ __device__ __forceinline__ void send_to_cta(const void* slot, float a, float b, 
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(map_to_cta(slot, rank)),
                "f"(a), "f"(b), "r"(map_to_cta(bar, rank))
                : "memory");
-}
-// The same with four values, 16 bytes.
-__device__ __forceinline__ void send4_to_cta(const void* slot, float4 v, const void* bar, uint32_t rank) {
-  asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(map_to_cta(slot, rank)),
-      "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(map_to_cta(bar, rank))
-      : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 // Meets the cluster without making stores visible to it (a release waits for those of the thread).
