@@ -354,7 +354,7 @@ __device__ __noinline__ void route_exactly(const Route& p, int t, void* scratch)
 }
 
 template <typename T, int EPL>
-__global__ void __launch_bounds__(kThreads, EPL <= 8 ? 4 : 2) route_kernel(const __grid_constant__ Route p) {
+__global__ void __launch_bounds__(kThreads, EPL <= 4 ? 6 : EPL <= 8 ? 5 : 2) route_kernel(const __grid_constant__ Route p) {
   extern __shared__ double scratch[];  // with groups that are not lanes' chunks
   const int warp = threadIdx.x >> 5;
   grid_dependency_wait();
@@ -389,22 +389,25 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
   for (int t = blockIdx.x * kWarps + warp; t < p.tokens; t += gridDim.x * kWarps) {
     const T* src = static_cast<const T*>(p.x) + (long long)t * p.ld;
     T* dst = static_cast<T*>(p.dx) + (long long)t * p.ld_dx;
+    float s[EPL], most = -INFINITY;
+    load_chunk<T, EPL>(src, first, p.experts, p.wide, s);
     int id = 0;
-    float dw = 0.f, xj = 0.f;
+    float dw = 0.f;
     if (lane < p.topk) {
       const long long at = (long long)lane * p.tokens + t;
+      dw = load_weight(p.d_weights, at, p.weights_dtype);
       const long long e = p.id_bits == 64 ? static_cast<const long long*>(p.ids)[at] : static_cast<const int*>(p.ids)[at];
       if (e < 0 || e > p.experts) atomicMax(p.status, DEV_BAD_INDEX);
       else id = (int)e;
-      if (id) {
-        dw = load_weight(p.d_weights, at, p.weights_dtype);
-        xj = to_float(src[id - 1]);
-      }
+      if (!id) dw = 0.f;
     }
-    float s[EPL], most = -INFINITY;
-    load_chunk<T, EPL>(src, first, p.experts, p.wide, s);
+    float xj = 0.f;  // logit of this lane's choice, from the lane that holds it
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) most = fmaxf(most, s[i]);
+    for (int i = 0; i < EPL; ++i) {
+      const float x = __shfl_sync(0xffffffffu, s[i], max(id - 1, 0) / EPL);
+      if (max(id - 1, 0) % EPL == i) xj = x;
+      most = fmaxf(most, s[i]);
+    }
     float sj;  // score of this lane's choice
     if (p.sigmoid) {
 #pragma unroll
@@ -419,9 +422,10 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
         if (first + i < p.experts) sum += s[i];
       }
       sum = warp_sum(sum);
+      sum = 1.f / sum;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) s[i] /= sum;
-      sj = expf(xj - most) / sum;
+      for (int i = 0; i < EPL; ++i) s[i] *= sum;
+      sj = expf(xj - most) * sum;
     }
     if (!id) sj = 0.f;
     float u = p.scale * dw;
@@ -442,7 +446,6 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
       for (int i = 0; i < EPL; ++i)
         if (e == first + i) d[i] += v;
     }
-    __syncwarp();  // dst may be the logits themselves: the choices' logits have been read
 #pragma unroll
     for (int i = 0; i < EPL; ++i) d[i] *= s[i] * (p.sigmoid ? 1.f - s[i] : 1.f);
     store_chunk<T, EPL>(dst, first, p.experts, p.wide, d);
