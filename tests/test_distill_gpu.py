@@ -207,6 +207,58 @@ def test_teacher_from_token_logprobs(cuda):
     cuda.check_device_status(0)
 
 
+@pytest.mark.parametrize("T,V,K", [(1, 70001, 256), (70, 9001, 256), (4100, 17001, 33)])
+def test_many_entries_and_rows(cuda, T, V, K):
+    """Long lists with ids many times over (more alike than a small table keeps apart), and more rows than there are counters."""
+    import torch
+    x = make(T, V, "bfloat16", seed=3, shift=5)
+    ids, values, all_values = teacher(T, V, K, seed=4)
+    ids[:, K // 2:] = ids[:, :K - K // 2]
+    ids[0, 1:] = ids[0, :1]
+    if T > 60:
+        ids[50:] = 0
+    for lse in (None, torch.logsumexp(all_values, 1) + 2.0):
+        check(cuda, x, ids, values, lse)
+
+
+def test_repeatable_and_on_streams(cuda):
+    """Bitwise the same on every call, on several streams at once and from replayed graphs beside eager calls."""
+    import torch
+    ops = cuda.distill
+    cases = []
+    for T, V, K, dtype in ((2, 120001, 60, "bfloat16"), (64, 30000, 256, "float32"), (700, 5000, 17, "float16")):
+        x = make(T, V, dtype, seed=T)
+        ids, values, all_values = teacher(T, V, K, seed=V)
+        ids[:, K // 2] = ids[:, 0]
+        cases.append((x, ids, values, torch.logsumexp(all_values, 1) + 0.5, torch.rand(T, device="cuda")))
+
+    def run(i):
+        x, ids, values, lse, g = cases[i]
+        loss, saved = ops.distill_fwd(x, ids, values)
+        return [loss, saved, ops.distill_bwd(x, ids, values, saved, g), *ops.distill_fwd_bwd(x, ids, values, g, lse)]
+    want = [run(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    graphs, captured = [], []
+    for i in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            captured.append(run(i))
+        graphs.append(g)
+    got = []
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                if k < 3:
+                    got.append((k, run(k)))
+                else:
+                    graphs[k - 3].replay()
+    torch.cuda.synchronize()
+    for k, r in got + list(enumerate(captured)):
+        assert all(a.equal(b) for a, b in zip(r, want[k]))
+    cuda.check_device_status(0)
+
+
 def test_refusals(cuda):
     import torch
     ops, lib = cuda.distill, cuda._lib

@@ -306,6 +306,38 @@ def test_repeatable_and_on_streams(cuda):
     cuda.check_device_status(0)
 
 
+@pytest.mark.parametrize("top", [0, 5])
+def test_more_rows_than_counters(cuda, top):
+    """Beyond 4096 rows there is no counter per row: rows in several launches, or whole."""
+    import torch
+    T, V = 4100, 17001
+    x = make(T, V, "bfloat16", seed=8, shift=1)
+    tokens = torch.randint(0, V + 1, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    tokens[::7] = 0
+    check(cuda, x, tokens, top)
+    x = make(9000, 40, "float32", seed=9)
+    check(cuda, x, tokens[:1].clamp(min=1, max=40).expand(9000).contiguous(), top)
+
+
+@pytest.mark.parametrize("T,V", [(1, 262144), (8, 131073), (40, 33333)])
+@pytest.mark.parametrize("top", [1, 19, 31, 32])
+def test_lists_of_parts(cuda, T, V, top):
+    """Rows cut into many parts: the best elements in one part, in the last elements, spread, alike, or fewer than `top` at all."""
+    import torch
+    for dtype in TYPES:
+        x = make(T, V, dtype, seed=top, shift=3)
+        tokens = torch.full((T,), V, device="cuda", dtype=torch.int32)
+        check(cuda, x, tokens, top)
+        x[:, V // 2:V // 2 + 40] += 16
+        x[0, -7:] += 40
+        check(cuda, x, tokens, top)
+        x[:, ::V // 64] = 60.0  # alike, in every part
+        check(cuda, x, tokens, top)
+        x.fill_(-float("inf"))
+        x[:, V - 3:] = 1.0
+        check(cuda, x, tokens, top)
+
+
 def test_refusals(cuda):
     import torch
     ops, lib = cuda.logprobs, cuda._lib

@@ -245,6 +245,31 @@ def test_router_of_an_expert_layer(cuda):
     cuda.check_device_status(0)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_doubtful_orders(cuda, score):
+    """Scores with a bias so close that f32 cannot order them, next to each other, at the last choice and at the last group; scores beyond f32."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(11)
+    for T, E, topk, kw in ((3000, 256, 8, dict(groups=8, topk_groups=4, group_top=2)), (3000, 64, 30, dict()), (3000, 64, 31, dict()),
+                           (500, 60, 32, dict()), (3000, 384, 6, dict(groups=8, topk_groups=3, group_top=1))):
+        x = torch.randn(T, E, device="cuda", generator=g)
+        bias = torch.randn(E, device="cuda", generator=g) * 0.1
+        scores = torch.softmax(x.double(), 1) if score == "softmax" else torch.sigmoid(x.double())
+        a, b = torch.randperm(E, device="cuda", generator=g)[:2]
+        step = torch.randint(-3, 4, (E,), device="cuda", generator=g) * 2.0 ** -25
+        bias[b] = 0.7
+        bias[a] = (scores[0, b] + 0.7 - scores[0, a]).float()  # the two best of the first token, a rounding apart
+        check(cuda, x, topk, torch.float32, score=score, bias=bias, **kw)
+        close_x = x.clone()
+        close_x[:, 1::2] = close_x[:, ::2]
+        check(cuda, close_x, topk, torch.float32, score=score, bias=bias, **kw)
+        check(cuda, close_x, topk, torch.float32, score=score, bias=(bias.view(-1, 2)[:, :1].expand(-1, 2).reshape(-1) + step).float(), **kw)
+        check(cuda, close_x, topk, torch.float32, score=score, bias=(bias.view(-1, 2)[:, :1].expand(-1, 2).reshape(-1) + step).float() * 1e4, **kw)
+        check(cuda, x * 12, topk, torch.float32, score=score, renormalize=False, **kw)
+        check(cuda, x * 12, topk, torch.float32, score=score, bias=bias, renormalize=False, **kw)
+        check(cuda, x * 12 + 18, topk, torch.float32, score=score, bias=bias, **kw)
+
+
 def test_refusals(cuda):
     import torch
     ops, lib = cuda.moe, cuda._lib
