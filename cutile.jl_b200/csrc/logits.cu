@@ -32,7 +32,7 @@ constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
 constexpr int kMaxEntries = kThreads;    // of a teacher's list
 constexpr int kCand = 1024;
-constexpr int kPlainPerSm = 6, kTopPerSm = 4, kBackwardPerSm = 5;  // CTAs on an SM
+constexpr int kPlainPerSm = 6, kTopPerSm = 4, kBackwardPerSm = 5, kBothPerSm = 4;  // CTAs on an SM
 constexpr size_t kMostShared = 220 * 1024;  // dynamic shared memory of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -442,8 +442,9 @@ __device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
 
 // Calls f(q, v) for a thread's vectors, four at a time; v: the tile's first one.  What is left over comes one vector at a time, in
 // the warps that have some of it; lanes beyond the end get -inf.  Lanes that took a rare branch in f would go on by
-// themselves up to the next shuffle, behind the row: they meet before every tile (2220 x 100000 bf16: 110 -> 82 us).  W warps stream the row.
-template <typename T, int W, typename F>
+// themselves up to the next shuffle, behind the row: they meet before every tile (2220 x 100000 bf16: 110 -> 82 us).  W warps stream the row.  KEEP: it is read again,
+// from L2.
+template <typename T, int W, bool KEEP = false, typename F>
 __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F f) {
   constexpr int kWide = W * 32;
   const int tid = threadIdx.x % kWide;
@@ -454,14 +455,14 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
     __syncwarp();
     uint4 q[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = __ldcs(p + u * kWide);
+    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kWide) : __ldcs(p + u * kWide);
     f(q, v);
   }
 #pragma unroll 1
   for (; v + (tid & ~31) < in.b; v += kWide, p += kWide) {
     __syncwarp();
     uint4 q[1] = {empty_row_vec<T>()};
-    if (v + tid < in.b) q[0] = __ldcs(p);
+    if (v + tid < in.b) q[0] = KEEP ? __ldcg(p) : __ldcs(p);
     f(q, v);
   }
 }
@@ -959,19 +960,31 @@ __device__ __forceinline__ float outside_of(const Teacher& t, float3 sum) {
   const double left = left_over(t), whole = t.all + left;
   return (float)(sum.z == 0.f ? whole : whole - left * ((double)sum.y / (double)sum.z));
 }
+// What the gradient needs to know of a row: (lse, outside, whole, norm) with teacher_lse; else outside and whole are 1, and the norm keeps 48
+// bits: (lse, low part, -1, norm).  log_total: log sum.y.
+template <bool TAIL>
+__device__ __forceinline__ float4 saved_of(const Distill& p, const Teacher& t, float3 sum, double log_total) {
+  const double lse = fma((double)sum.x, p.per_temperature, log_total);
+  const float high = (float)t.norm;
+  return TAIL ? make_float4((float)lse, outside_of(t, sum), (float)(t.all + left_over(t)), high)
+              : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
+}
 // Loss and saved values of a row; one lane.
 template <bool TAIL>
 __device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, float3 sum) {
-  const double log_total = log_of(sum.y), lse = fma((double)sum.x, p.per_temperature, log_total);
-  double loss = t.terms + t.all * lse;
+  const double log_total = log_of(sum.y);
+  double loss = t.terms + t.all * fma((double)sum.x, p.per_temperature, log_total);
   if (TAIL && left_over(t) != 0) loss += left_over(t) * (log(left_over(t)) - (log_of(sum.z) - log_total));
-  // (lse, outside, whole, norm) with teacher_lse; else outside and whole are 1, and the norm keeps 48 bits: (lse, low part, -1, norm)
-  const float high = (float)t.norm;
   p.loss[row] = (float)loss;
-  reinterpret_cast<float4*>(p.saved)[row] = TAIL ? make_float4((float)lse, outside_of(t, sum), (float)(t.all + left_over(t)), high)
-                                                 : make_float4((float)lse, (float)(t.norm - (double)high), -1.f, high);
+  reinterpret_cast<float4*>(p.saved)[row] = saved_of<TAIL>(p, t, sum, log_total);
 }
+
 // ------------------------------------------------------------------ backward
+struct Both : Distill {
+  void* dx;
+  long long ld_dx;
+  const float* d_loss;
+};
 struct Backward : Rows {
   void* dx;
   long long ld_dx;
@@ -998,13 +1011,13 @@ struct Backward : Rows {
 // TAIL: teacher_lse is given, and what the teacher lists is left out of the row's sum, by a bit per element, and added apart: the rest's
 // probability from a difference would lose all digits where it is small.
 // A part's elements but for those with a bit.
-template <typename T, bool TAIL>
+template <typename T, bool TAIL, bool KEEP>
 __device__ __forceinline__ float3 sum_range(const Range<T>& r, const Inner& in, const unsigned* holes, int words, float c) {
   constexpr int V = Range<T>::V;
   const int lane = threadIdx.x & 31, edge = edge_index(r, in, lane);
   const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
   Sums<T, false> sums;
-  each_tile<T, 1>(r, in, [&](auto& q, int v) {
+  each_tile<T, 1, KEEP>(r, in, [&](auto& q, int v) {
     if constexpr (TAIL) {
       const unsigned hole = hole_bits<T>(holes, v - in.a);
       if (__any_sync(0xffffffffu, hole != 0)) {
@@ -1045,7 +1058,7 @@ __device__ __forceinline__ void distill_part(const Distill& p, long long row, in
     __syncwarp();
     float3 sum;
     Teacher t;
-    if (part >= 0) sum = sum_range<T, TAIL>(r, in, holes, words, p.c);
+    if (part >= 0) sum = sum_range<T, TAIL, false>(r, in, holes, words, p.c);
     if (whole || part < 0) {
       if (TAIL && whole) clear_holes(holes, words);
       clean = whole;
@@ -1153,6 +1166,61 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
     if (first) dst[id - 1] = from_float<T>(g * (whole * ex2_approx_ftz(fmaf(x[k], p.c, -lse2)) - q));
   }
   __syncwarp();
+}
+
+// Loss and gradient at once, a row at a time by a CTA: eight warps sum an eighth each while a ninth learns the teacher's side, they meet, and
+// each writes the gradient of its eighth, which comes out of L2.  The rows that are under way (four per SM) have to stay there: with five per
+// SM 4096 x 65536 bf16 takes 274 us for 250, with three 254.  Two forms with more to them were slower: clusters with a warp that
+// learns ahead (267), and warps that draw sums and, some rows behind, gradients from one counter (255, small batches twice as long).
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel(const __grid_constant__ Both p) {
+  extern __shared__ __align__(16) unsigned char store[];
+  __shared__ float red[2][3][kWarps];
+  __shared__ Teacher teachers[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Listed lists(store, p.entries);
+  const int words = TAIL ? hole_words(p.per, sizeof(T)) : 0;
+  unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) / kWarps * (kWarps + 1) + warp * words;
+  for (int i = lane; i < words; i += 32) holes[i] = 0;
+  grid_dependency_wait();
+  __syncwarp();
+  int turn = 0;  // what a warp leaves for the others is not written over before they have all come to the next meeting
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const Range<T> r = range_of<T>(p, row, warp);
+    const Inner in(r);
+    const Row kind = look_at(p, row, [&](int id) {
+      if (TAIL && warp < kWarps && in_range(r, id)) punch(r, in, id, holes, words);
+    });
+    if (kind != LIVE) {
+      if (warp == kWarps) write_unused(p, row, kind);
+      else stream_zeros<T, 1>(r, static_cast<T*>(p.dx) + row * p.ld_dx);
+      if (TAIL) clear_holes(holes, words);
+      continue;
+    }
+    __syncwarp();
+    if (warp == kWarps) {
+      const Teacher t = learn<T, TAIL>(p, row, lists, holes, words);
+      if (lane == 0) teachers[turn] = t;
+    } else {
+      const float3 sum = sum_range<T, TAIL, true>(r, in, holes, words, p.c);
+      if (lane == 0) {
+        red[turn][0][warp] = sum.x;
+        red[turn][1][warp] = sum.y;
+        red[turn][2][warp] = 0.f;
+      }
+      if (TAIL) clear_holes(holes, words);
+    }
+    __syncthreads();
+    const Teacher t = teachers[turn];
+    const float3 sum = with_listed<TAIL>(p, t, join_warps<kWarps>(red[turn], p.c));
+    if (warp == kWarps) {
+      if (lane == 0) close_row<TAIL>(p, row, t, sum);
+    } else {
+      distill_gradient<T, 1>(p, row, warp, saved_of<TAIL>(p, t, sum, log_of(sum.y)), lists.entry, lists.q, lists.x);
+    }
+    __syncwarp();
+  }
+  grid_dependency_launch();
 }
 
 template <typename T>
@@ -1423,6 +1491,30 @@ int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* 
   return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, true, true, 3.0, who)
                        : launch_items<distill_kernel<T, false>, T>(ctx, st, p, false, true, 3.0, who);
 }
+template <typename T>
+size_t both_shared(const Both& p) {
+  const int per = (int)((vectors<T>(p) + kWarps - 1) / kWarps + 31) / 32 * 32;
+  return 4 * ((size_t)lists_words(p.entries) / kWarps + (p.teacher_lse ? (size_t)hole_words(per, sizeof(T)) : 0)) * (kWarps + 1);
+}
+// Loss and gradient at once, or one after the other?  In us, one after the other and at once: 4096 x 65536 bf16 298, 250; 1500 x 50001 f32 178, 151;
+// 8000 x 32000 bf16 318, 228.  Where the teacher's side takes longer than a row (20000 x 8000 bf16, with a rest: 305, 362), where the rows
+// under way do not stay in L2 (1024 x 128000 f32: 281, 278), and for few long rows, one after the other.
+template <typename T>
+bool at_once(const Both& p) {
+  const int64_t bytes = (int64_t)p.n * sizeof(T);
+  return bytes >= 32 * 1024 && bytes <= 512 * 1024 && (bytes <= 128 * 1024 || p.rows >= 148) && both_shared<T>(p) <= kMostShared / kBothPerSm - 2048;
+}
+template <typename T>
+int launch_both(ctb_ctx* ctx, cudaStream_t st, Both p, const char* who) {
+  auto kernel = p.teacher_lse ? distill_both_kernel<T, true> : distill_both_kernel<T, false>;
+  cut_into(p, vectors<T>(p), kWarps);
+  const size_t smem = both_shared<T>(p);
+  cudaError_t e = smem > 48 * 1024 ? allow_smem(kernel, kMostShared) : cudaSuccess;
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  launch_kernel(kernel, (int)std::min<int64_t>(p.rows, (int64_t)kBothPerSm * ctx->sm_count), kThreads + 32, smem, st, 0, p);
+  CTB_CHECK_LAUNCH(who);
+  return CTB_OK;
+}
 template <typename F>
 int by_type(int dtype, F f) {
   if (dtype == CTB_F32) return f(float());
@@ -1515,7 +1607,8 @@ extern "C" int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits
 
 static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
                            const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
-                           int64_t V, int64_t T, int64_t ld, int entries, float temperature, int dtype) {
+                           int64_t V, int64_t T, int64_t ld, int entries, float temperature, int dtype, const float* d_loss = nullptr,
+                           void* d_logits = nullptr, int64_t ld_out = 0, bool* both = nullptr) {
   if (int s = check_rows(who, logits, V, T, ld, temperature, dtype)) return s;
   if (T == 0) return CTB_OK;
   if (int s = check_teacher(who, teacher_ids, id_bits, teacher_values, values_dtype, entries)) return s;
@@ -1523,7 +1616,7 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   CTB_CHECK_PTR(who, loss);
   CTB_CHECK_PTR(who, saved);
   if ((uintptr_t)saved % 16) return fail(CTB_BAD_ALIGN, "%s: saved must be 16-byte aligned", who);
-  Distill p = {};
+  Both p = {};
   p.x = logits; p.ld = ld; p.n = (int)V; p.rows = (int)T;
   p.c = (float)(1.4426950408889634 / (double)temperature);
   p.temperature = temperature;
@@ -1531,7 +1624,11 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   p.ids = teacher_ids; p.id_bits = id_bits; p.entries = entries; p.values = teacher_values; p.values_dtype = values_dtype;
   p.teacher_lse = teacher_lse; p.per_temperature = 1 / (double)temperature; p.loss = loss; p.saved = saved;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(ctx, st, p, who); });
+  p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
+  return by_type(dtype, [&](auto t) {
+    if (both) *both = at_once<decltype(t)>(p);
+    return both && *both ? launch_both<decltype(t)>(ctx, st, p, who) : launch_distill<decltype(t)>(ctx, st, p, who);
+  });
 }
 
 static int distill_backward(const char* who, ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
@@ -1573,9 +1670,6 @@ extern "C" int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const
                           ld, entries, temperature, dtype);
 }
 
-// The loss, then its gradient.  One launch for both (warps that drew sums and, some rows behind, gradients from one counter; before that, CTAs
-// that streamed their row twice) gained 0 to 6 % on large batches and lost half on small ones: what is in flight at HBM's rate does not stay in
-// L2 until a row's sum is known.
 extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                                    const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
                                    const float* d_loss, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature,
@@ -1587,9 +1681,11 @@ extern "C" int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, c
   if (T == 0) return CTB_OK;
   if (int s = check_gradient(who, logits, d_logits, V, T, ld, ld_out, dtype)) return s;
   CTB_CHECK_PTR(who, d_loss);
+  bool both = true;
   if (int s = distill_forward(who, ctx, stream, logits, teacher_ids, id_bits, teacher_values, values_dtype, teacher_lse, loss, saved, V, T, ld,
-                              entries, temperature, dtype))
+                              entries, temperature, dtype, d_loss, d_logits, ld_out, &both))
     return s;
+  if (both) return CTB_OK;
   return distill_backward(who, ctx, stream, d_logits, logits, teacher_ids, id_bits, teacher_values, values_dtype, saved, d_loss, V, T, ld_out,
                           ld, entries, temperature, dtype);
 }

@@ -207,7 +207,7 @@ def test_teacher_from_token_logprobs(cuda):
     cuda.check_device_status(0)
 
 
-@pytest.mark.parametrize("T,V,K", [(1, 70001, 256), (70, 9001, 256), (4100, 17001, 33)])
+@pytest.mark.parametrize("T,V,K", [(1, 70001, 256), (70, 9001, 256), (5, 40001, 256), (149, 70001, 40), (4100, 17001, 33)])
 def test_many_entries_and_rows(cuda, T, V, K):
     """Long lists with ids many times over (more alike than a small table keeps apart), and more rows than there are counters."""
     import torch
