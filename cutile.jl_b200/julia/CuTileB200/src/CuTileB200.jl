@@ -180,6 +180,93 @@ function moe_router(hidden_states::CuArray{Float16,2}, W_r::CuArray{Float16,2}, 
     return w, ids
 end
 
+"Routing by given logits (E, T): returns (topk_weights (T, topk), topk_ids::CuArray{Int32}(T, topk)); `score` is :softmax or :sigmoid."
+function moe_route(logits::CuArray{X,2}, topk::Int; bias::Union{CuArray{Float32},Nothing}=nothing, score::Symbol=:softmax, groups::Int=1,
+                   topk_groups::Int=1, group_top::Int=1, renormalize::Bool=true, scale::Real=1, weights_type::Type=Float16) where {X}
+    E, T = size(logits)
+    ids = CuArray{Int32}(undef, T, topk); w = CuArray{weights_type}(undef, T, topk)
+    check(ccall((:ctb_moe_route, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Int64, Int64, Int64, Cint, Cint, Cint, Cint, Cint,
+         Cint, Cfloat, Cint),
+        context(), stream(), dptr(logits), bias === nothing ? C_NULL : dptr(bias), dptr(ids), dptr(w), dtype(weights_type), T, E,
+        stride(logits, 2), topk, score_code(score), groups, topk_groups, group_top, renormalize, scale, dtype(X)))
+    return w, ids
+end
+score_code(s::Symbol) = s === :softmax ? Cint(0) : s === :sigmoid ? Cint(1) : throw(ArgumentError("score must be :softmax or :sigmoid"))
+
+function moe_route_bwd(logits::CuArray{X,2}, topk_ids::CuArray, d_weights::CuArray{D}; score::Symbol=:softmax, renormalize::Bool=true,
+                       scale::Real=1) where {X,D}
+    E, T = size(logits); d = similar(logits)
+    check(ccall((:ctb_moe_route_bwd, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Int64, Int64, Int64, Int64, Cint, Cint, Cint,
+         Cfloat, Cint),
+        context(), stream(), dptr(d), dptr(logits), dptr(topk_ids), ids_bits(topk_ids), dptr(d_weights), dtype(D), T, E, stride(d, 2),
+        stride(logits, 2), size(topk_ids, 2), score_code(score), renormalize, scale, dtype(X)))
+    return d
+end
+
+# ---- log probabilities and distillation (no example in the reference) -------
+"Log probabilities of `tokens` (1-based, 0: padding) under softmax(logits ./ temperature), logits (V, T): a named tuple."
+function token_logprobs(logits::CuArray{X,2}, tokens::CuArray; top::Int=0, temperature::Real=1) where {X}
+    V, T = size(logits)
+    logprobs = CuArray{Float32}(undef, T); entropy = similar(logprobs); lse = similar(logprobs)
+    top_logprobs = CuArray{Float32}(undef, top, T); top_ids = CuArray{Int32}(undef, top, T)
+    check(ccall((:ctb_token_logprobs, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64,
+         Int64, Cint, Cfloat, Cint),
+        context(), stream(), dptr(logits), dptr(tokens), ids_bits(tokens), dptr(logprobs), dptr(entropy), dptr(lse),
+        top == 0 ? C_NULL : dptr(top_logprobs), top == 0 ? C_NULL : dptr(top_ids), V, T, stride(logits, 2), top, temperature, dtype(X)))
+    return (; logprobs, entropy, lse, top_logprobs, top_ids)
+end
+
+"Gradient of the logits from those of log probabilities and entropies."
+function token_logprobs_bwd(logits::CuArray{X,2}, tokens::CuArray, lse, entropy, d_logprobs, d_entropy; temperature::Real=1) where {X}
+    V, T = size(logits); d = similar(logits)
+    check(ccall((:ctb_token_logprobs_bwd, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+         Ptr{Cvoid}, Int64, Int64, Int64, Int64, Cint, Cfloat, Cint),
+        context(), stream(), dptr(d), dptr(logits), dptr(tokens), ids_bits(tokens), dptr(lse), dptr(entropy), dptr(d_logprobs),
+        d_entropy === nothing ? C_NULL : dptr(d_entropy), C_NULL, C_NULL, V, T, stride(d, 2), stride(logits, 2), 0, temperature, dtype(X)))
+    return d
+end
+
+"Distillation from a teacher's list (entries, T): returns (loss, saved) for `distill_bwd`."
+function distill_fwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_values::CuArray{Q}; teacher_lse=nothing, temperature::Real=1) where {X,Q}
+    V, T = size(logits)
+    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 4, T)
+    check(ccall((:ctb_distill_fwd, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64,
+         Cint, Cfloat, Cint),
+        context(), stream(), dptr(logits), dptr(teacher_ids), ids_bits(teacher_ids), dptr(teacher_values), dtype(Q),
+        teacher_lse === nothing ? C_NULL : dptr(teacher_lse), dptr(loss), dptr(saved), V, T, stride(logits, 2), size(teacher_ids, 1),
+        temperature, dtype(X)))
+    return loss, saved
+end
+
+function distill_bwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_values::CuArray{Q}, saved, d_loss; temperature::Real=1) where {X,Q}
+    V, T = size(logits); d = similar(logits)
+    check(ccall((:ctb_distill_bwd, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64,
+         Int64, Cint, Cfloat, Cint),
+        context(), stream(), dptr(d), dptr(logits), dptr(teacher_ids), ids_bits(teacher_ids), dptr(teacher_values), dtype(Q), dptr(saved),
+        dptr(d_loss), V, T, stride(d, 2), stride(logits, 2), size(teacher_ids, 1), temperature, dtype(X)))
+    return d
+end
+
+"Loss and gradient in one call: (loss, gradient)."
+function distill_fwd_bwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_values::CuArray{Q}, d_loss; teacher_lse=nothing,
+                         temperature::Real=1) where {X,Q}
+    V, T = size(logits); d = similar(logits)
+    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 4, T)
+    check(ccall((:ctb_distill_fwd_bwd, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+         Int64, Int64, Int64, Int64, Cint, Cfloat, Cint),
+        context(), stream(), dptr(d), dptr(logits), dptr(teacher_ids), ids_bits(teacher_ids), dptr(teacher_values), dtype(Q),
+        teacher_lse === nothing ? C_NULL : dptr(teacher_lse), dptr(loss), dptr(saved), dptr(d_loss), V, T, stride(d, 2), stride(logits, 2),
+        size(teacher_ids, 1), temperature, dtype(X)))
+    return loss, d
+end
+
 function moe_align_tile_size(topk_ids::CuArray, tile_m::Int, num_experts::Int)
     T, topk = size(topk_ids)
     cap = ccall((:ctb_moe_max_blocks, LIB), Int64, (Int64, Int64, Int64, Cint), T, topk, num_experts, tile_m)
