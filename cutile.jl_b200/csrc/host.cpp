@@ -429,9 +429,18 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Call c(*r.x);
   if (!c.ok()) return nullptr;
   const auto f = r.x->options().dtype(at::kFloat);
-  Tensor lp, h, lse = at::empty({r.T}, f), tlp, tid;
-  if (tokens) lp = at::empty({r.T}, f);
-  if (a[4] == Py_True) h = at::empty({r.T}, f);
+  // one allocation for the vectors: each of its own would be 1.3 us of a call of 11
+  const int64_t step = (r.T + 3) / 4 * 4;
+  const Tensor all = at::empty({3 * step}, f);
+  auto vector = [&](int i) {
+    Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), all.dtype());
+    v.unsafeGetTensorImpl()->set_sizes_contiguous({r.T});
+    v.unsafeGetTensorImpl()->set_storage_offset(i * step);
+    return v;
+  };
+  Tensor lp, h, lse = vector(0), tlp, tid;
+  if (tokens) lp = vector(1);
+  if (a[4] == Py_True) h = vector(2);
   if (top) {
     tlp = at::empty({r.T, top}, f);
     tid = at::empty({r.T, top}, f.dtype(at::kInt));

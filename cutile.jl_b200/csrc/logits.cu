@@ -1184,8 +1184,8 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
   for (int i = lane; i < words; i += 32) holes[i] = 0;
   grid_dependency_wait();
   __syncwarp();
-  int turn = 0;  // what a warp leaves for the others is not written over before they have all come to the next meeting
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+  int turn = 0;  // of two places: what a warp leaves for the others is not written over before they have all come to the next meeting
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const Range<T> r = range_of<T>(p, row, warp);
     const Inner in(r);
     const Row kind = look_at(p, row, [&](int id) {
@@ -1218,6 +1218,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
     } else {
       distill_gradient<T, 1>(p, row, warp, saved_of<TAIL>(p, t, sum, log_of(sum.y)), lists.entry, lists.q, lists.x);
     }
+    turn ^= 1;
     __syncwarp();
   }
   grid_dependency_launch();

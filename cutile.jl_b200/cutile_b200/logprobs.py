@@ -12,7 +12,7 @@ from ._util import dense, dtype_code, gradient_of, handles, ids_bits, ptr, rows
 
 
 class TokenLogprobs(NamedTuple):
-    """Results of token_logprobs, f32; None for what was not asked for."""
+    """Results of token_logprobs, f32; None for what was not asked for.  The three vectors may share an allocation."""
     logprobs: Optional[torch.Tensor]      # [T] of the given tokens
     entropy: Optional[torch.Tensor]       # [T]
     lse: torch.Tensor                     # [T] log of the sum of exponentials
