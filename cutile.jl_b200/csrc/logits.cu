@@ -13,7 +13,6 @@
 #include <limits.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "ctx.h"
@@ -30,7 +29,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;               // vectors of 16 bytes per thread and tile
 constexpr int kTile = kThreads * kUnroll;  // vectors
 constexpr int kMaxTop = 32;
-constexpr int kMaxEntries = kThreads;    // of a teacher's list
+constexpr int kMaxEntries = 256;         // of a teacher's list
 constexpr int kCand = 1024;
 constexpr int kPlainPerSm = 6, kTopPerSm = 4, kBackwardPerSm = 5, kBothPerSm = 4;  // CTAs on an SM
 constexpr size_t kMostShared = 220 * 1024;  // dynamic shared memory of a CTA
@@ -821,8 +820,8 @@ static_assert(sizeof(Teacher) == 2 * sizeof(float4), "a teacher takes two record
 struct Listed {
   int* entry;
   float *q, *x;
-  __device__ __forceinline__ Listed(unsigned char* store, int entries) {
-    entry = reinterpret_cast<int*>(store) + (threadIdx.x >> 5) * 3 * entries;
+  __device__ __forceinline__ Listed(unsigned char* store, int entries, int which) {
+    entry = reinterpret_cast<int*>(store) + which * 3 * entries;
     q = reinterpret_cast<float*>(entry + entries);
     x = q + entries;
   }
@@ -1095,7 +1094,7 @@ template <typename T, bool TAIL>
 __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __grid_constant__ Distill p) {
   extern __shared__ __align__(16) unsigned char store[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Listed lists(store, p.entries);
+  const Listed lists(store, p.entries, threadIdx.x >> 5);
   const int words = TAIL ? hole_words(p.per, sizeof(T)) : 0;
   unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) + warp * words;
   for (int i = lane; i < words; i += 32) holes[i] = 0;
@@ -1112,8 +1111,12 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __
 
 // A part of a row's gradient, by W warps that own each their vectors of it, and the listed elements in those: g (whole p - q), elsewhere a p.
 // The listed logits are read before the part is streamed (dx may be the logits themselves).  entry, q, x: lists of the warp's own.
-template <typename T, int W, typename P>
-__device__ __forceinline__ void distill_gradient(const P& p, long long row, int part, const float4 saved, int* entry, float* weight, float* x) {
+// given: the entries as learn has left them, if it has.
+template <typename T, int W, bool GIVEN, typename P>
+__device__ __forceinline__ void distill_gradient(const P& p, long long row, int part, const float4 saved, const Listed& own_list,
+                                                 const Listed& given) {
+  int* entry = own_list.entry;
+  float *weight = own_list.q, *x = own_list.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Range<T> r = range_of<T>(p, row, part);
   const Inner in(r);
@@ -1128,8 +1131,8 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
   __syncwarp();
   for (int j0 = 0; j0 < p.entries; j0 += 32) {
     const int j = j0 + lane;
-    const long long id = j < p.entries ? load_id(p.ids, row * p.entries + j, p.id_bits) : 0;
-    if (id < 0 || id > p.n) atomicMax(p.status, DEV_BAD_INDEX);
+    const long long id = j >= p.entries ? 0 : GIVEN ? abs(given.entry[j]) : load_id(p.ids, row * p.entries + j, p.id_bits);
+    if (!GIVEN && (id < 0 || id > p.n)) atomicMax(p.status, DEV_BAD_INDEX);
     bool mine = id <= p.n && in_range(r, id) != 0;
     if (W > 1 && mine) {
       const int v = (int)((id - 1 + r.off) / Range<T>::V);
@@ -1145,9 +1148,14 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
   }
   __syncwarp();
   for (int k = lane; k < own; k += 32) {
-    const float value = load_value(p.values, row * p.entries + __float_as_int(weight[k]), p.values_dtype);
-    x[k] = to_float(r.src[entry[k] - 1]);
-    weight[k] = exp_of(fma((double)value, p.per_temperature, -norm));
+    const int j = __float_as_int(weight[k]);
+    if constexpr (GIVEN) {
+      x[k] = given.x[j];
+      weight[k] = given.q[j];
+    } else {
+      x[k] = to_float(r.src[entry[k] - 1]);
+      weight[k] = exp_of(fma((double)load_value(p.values, row * p.entries + j, p.values_dtype), p.per_temperature, -norm));
+    }
   }
   const float g = p.d_loss[row] / p.temperature, lse2 = saved.x * kLog2e;
   const float a = g * (list_is_all ? 1.f : saved.y), whole = list_is_all ? 1.f : saved.z;
@@ -1178,9 +1186,9 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
   __shared__ float red[2][3][kWarps];
   __shared__ Teacher teachers[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Listed lists(store, p.entries);
+  const Listed lists(store, p.entries, threadIdx.x >> 5);
   const int words = TAIL ? hole_words(p.per, sizeof(T)) : 0;
-  unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) / kWarps * (kWarps + 1) + warp * words;
+  unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) / kWarps * (kWarps + 2) + warp * words;
   for (int i = lane; i < words; i += 32) holes[i] = 0;
   grid_dependency_wait();
   __syncwarp();
@@ -1198,8 +1206,9 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
       continue;
     }
     __syncwarp();
+    const Listed taught(store, p.entries, kWarps + turn);
     if (warp == kWarps) {
-      const Teacher t = learn<T, TAIL>(p, row, lists, holes, words);
+      const Teacher t = learn<T, TAIL>(p, row, taught, holes, words);
       if (lane == 0) teachers[turn] = t;
     } else {
       const float3 sum = sum_range<T, TAIL, true>(r, in, holes, words, p.c);
@@ -1216,7 +1225,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
     if (warp == kWarps) {
       if (lane == 0) close_row<TAIL>(p, row, t, sum);
     } else {
-      distill_gradient<T, 1>(p, row, warp, saved_of<TAIL>(p, t, sum, log_of(sum.y)), lists.entry, lists.q, lists.x);
+      distill_gradient<T, 1, true>(p, row, warp, saved_of<TAIL>(p, t, sum, log_of(sum.y)), lists, taught);
     }
     turn ^= 1;
     __syncwarp();
@@ -1227,12 +1236,12 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBackwardPerSm) distill_backward_kernel(const __grid_constant__ Backward p) {
   extern __shared__ __align__(16) unsigned char store[];
-  const Listed lists(store, p.entries);
+  const Listed lists(store, p.entries, threadIdx.x >> 5);
   grid_dependency_wait();
   const Items items(p, kWarps);
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item);
-    distill_gradient<T, kWarps>(p, row, (int)(item - row * p.parts), reinterpret_cast<const float4*>(p.saved)[row], lists.entry, lists.q, lists.x);
+    distill_gradient<T, kWarps, false>(p, row, (int)(item - row * p.parts), reinterpret_cast<const float4*>(p.saved)[row], lists, lists);
   }
   grid_dependency_launch();
 }
@@ -1339,7 +1348,7 @@ void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t le
   for (int64_t n = least; n <= most; n = n < 64 ? n + 1 : n + n / 8) {
     const int64_t items = p.rows * (n + (n > 1 ? more : 0)), full = items / places, rest = items % places;
     auto round = [&](int64_t active) { return bytes / (double)n * (1 / alone + (double)active / all) + ends; };
-    const double time = (double)full * round(places) + (rest ? round(rest) : 0) + 0.01 * (double)n;
+    const double time = (double)full * round(places) + (rest ? round(rest) : 0) + 0.05 * (double)n;
     if (n == least || time < best) {
       best = time;
       parts = n;
@@ -1495,7 +1504,7 @@ int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* 
 template <typename T>
 size_t both_shared(const Both& p) {
   const int per = (int)((vectors<T>(p) + kWarps - 1) / kWarps + 31) / 32 * 32;
-  return 4 * ((size_t)lists_words(p.entries) / kWarps + (p.teacher_lse ? (size_t)hole_words(per, sizeof(T)) : 0)) * (kWarps + 1);
+  return 4 * ((size_t)lists_words(p.entries) / kWarps * (kWarps + 2) + (p.teacher_lse ? (size_t)hole_words(per, sizeof(T)) * (kWarps + 1) : 0));
 }
 // Loss and gradient at once, or one after the other?  In us, one after the other and at once: 4096 x 65536 bf16 298, 250; 1500 x 50001 f32 178, 151;
 // 8000 x 32000 bf16 318, 228.  Where the teacher's side takes longer than a row (20000 x 8000 bf16, with a rest: 305, 362), where the rows

@@ -62,11 +62,6 @@ __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
   else asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 // The elements of a 16-bit word.
 template <typename T>
 __device__ __forceinline__ float2 word_pair(uint32_t w) {
@@ -80,14 +75,6 @@ __device__ __forceinline__ float word_max(uint32_t w) {
   else {
     const float2 f = word_pair<T>(w);
     return fmaxf(f.x, f.y);
-  }
-}
-template <typename T>
-__device__ __forceinline__ float word_nan(uint32_t w) {  // the same, NaN where one of them is
-  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
-  else {
-    const float2 f = word_pair<T>(w);
-    return max_nan(f.x, f.y);
   }
 }
 
