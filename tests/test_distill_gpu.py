@@ -221,6 +221,28 @@ def test_many_entries_and_rows(cuda, T, V, K):
         check(cuda, x, ids, values, lse)
 
 
+@pytest.mark.parametrize("V,dtype", [(17001, "bfloat16"), (8300, "float32"), (9000, "float16")])
+def test_padding_and_bad_rows_between(cuda, V, dtype):
+    """Several rows per CTA, some of them padding (not read), some with a bad id; loss and gradient in one call and in two."""
+    import torch
+    T, K = 1900, 9
+    x = make(T, V, dtype, seed=6, shift=1)
+    ids, values, all_values = teacher(T, V, K, seed=7)
+    kind = torch.randint(0, 5, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    ids[kind == 0] = 0
+    x[kind == 0] = float("nan")
+    check(cuda, x, ids, values)
+    lse = torch.logsumexp(all_values, 1) + 0.25
+    check(cuda, x, ids, values, lse)
+    cuda.check_device_status(0)
+    ids[kind == 1, 4] = V + 1
+    loss, d = cuda.distill.distill_fwd_bwd(x, ids, values, torch.ones(T, device="cuda"), lse)
+    with pytest.raises(cuda.CtbError, match="out-of-range index"):
+        cuda.check_device_status(0)
+    assert loss[kind == 1].isnan().all() and (loss[kind == 0] == 0).all() and loss[kind > 1].isfinite().all()
+    assert (d[kind < 2] == 0).all() and d.isfinite().all()
+
+
 def test_repeatable_and_on_streams(cuda):
     """Bitwise the same on every call, on several streams at once and from replayed graphs beside eager calls."""
     import torch
