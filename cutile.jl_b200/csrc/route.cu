@@ -302,10 +302,20 @@ __device__ __forceinline__ bool route_token(const Route& p, int t, void* scratch
     if (!sure) {
       const bool there = lane < rounds && my_word > 1;
       const float my_bias = there ? p.bias[my_id] : 0.f, c = there ? number_of(my_word) : -INFINITY;
-      const float next = __shfl_down_sync(0xffffffffu, c, 1), next_x = __shfl_down_sync(0xffffffffu, my_x, 1);
+      float next = __shfl_down_sync(0xffffffffu, c, 1);
+      const float next_x = __shfl_down_sync(0xffffffffu, my_x, 1);
       const float next_bias = __shfl_down_sync(0xffffffffu, my_bias, 1);
+      if (p.topk == 32) {  // no lane holds what comes after the last choice
+        Word best = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) best = max(best, word[i]);
+        int who;
+        best = top_word(best, who);
+        if (lane == 31) next = best > 1 ? number_of(best) : -INFINITY;
+      }
       auto close = [&](float below) { return there && below > -INFINITY && !(c - below > 2 * error + (fabsf(c) + fabsf(below)) * 0x1p-22f); };
-      const bool doubt = mine && close(next) && !(my_x == next_x && my_bias == next_bias);
+      // Alike in both, two choices are in order.  What comes after the last one is not: behind it there may be one that is only close.
+      const bool doubt = mine && close(next) && (lane == p.topk - 1 || !(my_x == next_x && my_bias == next_bias));
       if (__any_sync(0xffffffffu, doubt)) {
         // The choices and the one after them in f64, where the next one cannot be among the best either.
         const float second = __shfl_sync(0xffffffffu, c, (p.topk + 1) & 31);

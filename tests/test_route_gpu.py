@@ -270,6 +270,19 @@ def test_doubtful_orders(cuda, score):
         check(cuda, x * 12 + 18, topk, torch.float32, score=score, bias=bias, **kw)
 
 
+@pytest.mark.parametrize("topk", [1, 29, 30, 31, 32])
+def test_doubt_at_the_last_choice(cuda, topk):
+    """Every score within a few f32 roundings of every other, whatever the number of choices."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(topk)
+    for E in (40, 64, 250):
+        x = 0.5 + torch.randint(0, 40, (400, E), device="cuda", generator=g).float() * 2.0 ** -24
+        bias = 0.25 + torch.randint(0, 40, (E,), device="cuda", generator=g).float() * 2.0 ** -25
+        for score in ("softmax", "sigmoid"):
+            check(cuda, x, topk, torch.float32, score=score, bias=bias)
+            check(cuda, x, topk, torch.float32, score=score)
+
+
 def test_refusals(cuda):
     import torch
     ops, lib = cuda.moe, cuda._lib
