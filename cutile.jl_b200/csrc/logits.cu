@@ -854,14 +854,7 @@ __device__ __forceinline__ double log_of(float v) {
   const float m = frexpf(v, &k);
   return fma((double)k, 0.69314718055994531, (double)logf(m));
 }
-// e^v for v <= 0 or so, to a relative 2^-22: expf of v's leading bits, and the rest's first order.
-__device__ __forceinline__ float exp_of(double v) {
-  if (v < -200) return 0.f;
-  const float high = (float)v, e = expf(high);
-  return fmaf(e, (float)(v - (double)high), e);
-}
-// The teacher's side of a live row; a warp.  Sums and differences are in f64, of values that f32 functions give to a relative 2^-22;
-// with TAIL the q themselves are f64, for their difference from one.
+// The teacher's side of a live row; a warp.  All of it is f64: a gradient q is off by the roundings of q, of g and of their product alone.
 template <typename T, bool TAIL>
 __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Listed& t, unsigned* seen, int words) {
   const int lane = threadIdx.x & 31;
@@ -895,22 +888,17 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
     norm = p.teacher_lse[row];
   } else {
     most = warp_max(most);
-    float sum = 0.f;
+    double sum = 0;
     for (int j = lane; j < p.entries; j += 32)
-      if (t.entry[j]) sum += exp_of(((double)t.q[j] - (double)most) * p.per_temperature);
-    norm = fma((double)most, p.per_temperature, log_of(warp_sum(sum)));
+      if (t.entry[j]) sum += exp(((double)t.q[j] - (double)most) * p.per_temperature);
+    norm = fma((double)most, p.per_temperature, log(sum_lanes(sum)));
   }
   double all = 0, terms = 0;
   for (int j = lane; j < p.entries; j += 32) {
     if (t.entry[j] == 0) continue;
     const double log_q = fma((double)t.q[j], p.per_temperature, -norm);
-    double q;
-    if constexpr (TAIL) {
-      q = exp(log_q);
-      all += q;
-    } else {
-      q = (double)exp_of(log_q);
-    }
+    const double q = exp(log_q);
+    all += q;
     if (q != 0) terms = fma(q, log_q - (double)t.x[j] * p.per_temperature, terms);
     t.q[j] = (float)q;
   }
@@ -1154,7 +1142,7 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
       weight[k] = given.q[j];
     } else {
       x[k] = to_float(r.src[entry[k] - 1]);
-      weight[k] = exp_of(fma((double)load_value(p.values, row * p.entries + j, p.values_dtype), p.per_temperature, -norm));
+      weight[k] = (float)exp(fma((double)load_value(p.values, row * p.entries + j, p.values_dtype), p.per_temperature, -norm));
     }
   }
   const float g = p.d_loss[row] / p.temperature, lse2 = saved.x * kLog2e;
