@@ -38,7 +38,8 @@ struct Route {
   void* weights;
   int weights_dtype;
   long long ld;
-  int tokens, experts, topk, sigmoid, groups, topk_groups, group_top, renormalize;
+  unsigned tokens;
+  int experts, topk, sigmoid, groups, topk_groups, group_top, renormalize;
   float scale;
   int wide;           // rows (and bias) can be read as vectors
   int lanes_a_group;  // a power of two where the lanes' chunks make up groups, else 0
@@ -134,7 +135,7 @@ __device__ __forceinline__ void store_chunk(T* dst, int at, int end, bool wide, 
 // A token; a warp.  scratch: a word per expert of its own, where lanes' chunks do not make up groups.  True: nothing has been written, the
 // order is in doubt (never with EXACT).
 template <typename T, int EPL, bool EXACT>
-__device__ __forceinline__ bool route_token(const Route& p, int t, void* scratch) {
+__device__ __forceinline__ bool route_token(const Route& p, unsigned t, void* scratch) {
   using Word = typename std::conditional<EXACT, uint64_t, uint32_t>::type;
   using Number = typename std::conditional<EXACT, double, float>::type;
   const int lane = threadIdx.x & 31, first = lane * EPL;
@@ -359,7 +360,7 @@ __device__ __forceinline__ bool route_token(const Route& p, int t, void* scratch
   return false;
 }
 template <typename T, int EPL>
-__device__ __noinline__ void route_exactly(const Route& p, int t, void* scratch) {
+__device__ __noinline__ void route_exactly(const Route& p, unsigned t, void* scratch) {
   route_token<T, EPL, true>(p, t, scratch);
 }
 
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, EPL <= 4 ? 6 : EPL <= 8 ? 5 : 2) rou
   extern __shared__ double scratch[];  // with groups that are not lanes' chunks
   const int warp = threadIdx.x >> 5;
   grid_dependency_wait();
-  for (int t = blockIdx.x * kWarps + warp; t < p.tokens; t += gridDim.x * kWarps) {
+  for (unsigned t = blockIdx.x * kWarps + warp; t < p.tokens; t += gridDim.x * kWarps) {  // 2^31 and a round more at most
     if (route_token<T, EPL, false>(p, t, scratch + warp * p.experts)) route_exactly<T, EPL>(p, t, scratch + warp * p.experts);
     __syncwarp();
   }
@@ -383,7 +384,8 @@ struct RouteBackward {
   const void* d_weights;
   int weights_dtype;
   long long ld, ld_dx;
-  int tokens, experts, topk, sigmoid, renormalize;
+  unsigned tokens;
+  int experts, topk, sigmoid, renormalize;
   float scale;
   int* status;
   int wide;
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = lane * EPL;
   grid_dependency_wait();
-  for (int t = blockIdx.x * kWarps + warp; t < p.tokens; t += gridDim.x * kWarps) {
+  for (unsigned t = blockIdx.x * kWarps + warp; t < p.tokens; t += gridDim.x * kWarps) {  // 2^31 and a round more at most
     const T* src = static_cast<const T*>(p.x) + (long long)t * p.ld;
     T* dst = static_cast<T*>(p.dx) + (long long)t * p.ld_dx;
     float s[EPL], most = -INFINITY;
@@ -541,7 +543,7 @@ extern "C" int ctb_moe_route(ctb_ctx* ctx, void* stream, const void* logits, con
   if (bias) CTB_CHECK_DEV(bias);
   CTB_CHECK_DEV(topk_ids);
   CTB_CHECK_DEV(topk_weights);
-  const Route p = {logits, bias, topk_ids, topk_weights, weights_dtype, ld, (int)T, (int)E, topk, score == CTB_SCORE_SIGMOID, groups, topk_groups,
+  const Route p = {logits, bias, topk_ids, topk_weights, weights_dtype, ld, (unsigned)T, (int)E, topk, score == CTB_SCORE_SIGMOID, groups, topk_groups,
                    group_top, renormalize != 0, scale, 0, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == CTB_F32) return launch_route<float>(ctx, st, p);
@@ -564,7 +566,7 @@ extern "C" int ctb_moe_route_bwd(ctb_ctx* ctx, void* stream, void* d_logits, con
   CTB_CHECK_DEV(d_weights);
   if ((uintptr_t)d_logits % (dtype == CTB_F32 ? 4 : 2)) return fail(CTB_BAD_ALIGN, "%s: d_logits must be aligned to their element size", who);
   if (int s = check_in_place(who, logits, ld, d_logits, ld_out, E, T, dtype == CTB_F32 ? 4 : 2)) return s;
-  const RouteBackward p = {logits, d_logits, topk_ids, ids_bits, d_weights, weights_dtype, ld, ld_out, (int)T, (int)E, topk,
+  const RouteBackward p = {logits, d_logits, topk_ids, ids_bits, d_weights, weights_dtype, ld, ld_out, (unsigned)T, (int)E, topk,
                            score == CTB_SCORE_SIGMOID, renormalize != 0, scale, ctx->dev_status, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == CTB_F32) return launch_route_backward<float>(ctx, st, p);
