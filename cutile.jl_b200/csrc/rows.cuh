@@ -163,19 +163,19 @@ struct Range {
 template <typename T>
 __device__ __noinline__ uint4 load_edge(const T* src, int off, int n, int v) {
   constexpr int V = 16 / (int)sizeof(T);
-  uint4 q = empty_row_vec<T>();
-  T f[V];
+  const uint4 empty = empty_row_vec<T>();
+  alignas(uint4) T f[V];  // read as one vector below
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = v * V - off + i;
-    f[i] = e >= 0 && e < n ? src[e] : reinterpret_cast<const T*>(&q)[0];
+    f[i] = e >= 0 && e < n ? src[e] : reinterpret_cast<const T*>(&empty)[0];
   }
   return *reinterpret_cast<const uint4*>(f);
 }
-template <typename T, bool KEEP = false>
+template <typename T>
 __device__ __forceinline__ uint4 load_vec(const Range<T>& r, int v) {
   if (v >= r.v1) return empty_row_vec<T>();
-  if (r.inside(v, 1)) return KEEP ? __ldcg(r.at(v)) : __ldcs(r.at(v));
+  if (r.inside(v, 1)) return __ldcs(r.at(v));
   return load_edge<T>(r.src, r.off, r.n, v);
 }
 // Writes a vector to a row that starts like r; what is outside of the row is left as it is.
