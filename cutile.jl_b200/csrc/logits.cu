@@ -39,7 +39,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -16384.f;
 // A thread's reference follows its maximum only when an element is 2^kSlack above it.
 constexpr float kSlack = 4.f;
-constexpr float kFar = 1e30f;  // beyond, x log2(e) / temperature may overflow
+// Beyond, the rounding of an exponent's reference is no small fraction (2^-4 here) of a power of two any more, or it overflows.
+constexpr float kFar = 0x1p20f;
 
 // ------------------------------------------------------------------ the best k of a row
 // One pass, every element compared with a threshold that at least k earlier elements reach:
@@ -233,24 +234,28 @@ __device__ int radix_list(const Range<T>& r, int k, Best& b) {
 //
 // A thread's share of s = sum 2^t and, with ENTROPY, w = sum 2^t t.  Its reference follows its maximum, or t 2^t of a likely element would
 // carry a rounding that the entropy, a difference of two such sums, shows.  Masked elements (-inf) make w NaN (0 * -inf): the tile's
-// share is then taken again with exponents held above kLowest.  Where the maximum is beyond +-kFar (all that is left is masked by the
-// lowest number; infinities) x c would overflow, and exponents are taken from differences, (x - maximum) c.
+// share is then taken again with exponents held above kLowest.  m2 is maximum c rounded, and t is off by what that lost, until the sums are
+// put relative to the maximum itself.  Where m2 is beyond kFar (a small temperature, all that is left is masked by a number, infinities) that
+// may be more than an exponent holds, and exponents are taken from differences, (x - maximum) c.
 template <typename T, bool ENTROPY>
 struct Sums {
   float ref = 0.f, m2 = 0.f, limit = -INFINITY;  // m2 = ref c; elements above limit move the reference
   uint32_t top = empty_row_vec<T>().x;
   Pair s = pair(0.f, 0.f), w = pair(0.f, 0.f);
 
-  __device__ __forceinline__ bool far() const { return fabsf(ref) > kFar; }
+  static __device__ __forceinline__ bool far(float m2) { return !(fabsf(m2) <= kFar); }
+  __device__ __forceinline__ bool far() const { return far(m2); }
+  // What the rounding of m2 has added to the exponents.
+  static __device__ __forceinline__ float added(float ref, float m2, float c) { return far(m2) ? 0.f : fmaf(ref, c, -m2); }
   __device__ __forceinline__ void move(float x, float c) {
     const float to = x * c;
-    const bool jump = fabsf(x) > kFar || far();
-    const float d = fmaxf(fminf(jump ? (ref - x) * c : m2 - to, 0.f), kLowest), r = ex2_approx_ftz(d);  // s = w = 0 until there is a reference
+    const float apart = far(to) || far() ? (ref - x) * c - added(ref, m2, c) + added(x, to, c) : m2 - to;
+    const float d = fmaxf(fminf(apart, 0.f), kLowest), r = ex2_approx_ftz(d);  // s = w = 0 until there is a reference
     const Pair rr = pair(r, r);
     if constexpr (ENTROPY) w = mul2(rr, fma2(s, pair(d, d), w));
     s = mul2(rr, s);
     ref = x;
-    m2 = fabsf(x) > kFar ? 0.f : to;
+    m2 = to;
     limit = x + kSlack / c;
   }
   // Returns the largest element.
@@ -294,10 +299,9 @@ struct Sums {
   static __device__ __noinline__ float2 apart(uint4 q, float ref, float m2, float c) {
     float f[16 / sizeof(T)], s = 0.f, w = 0.f;
     unpack_row<T>(q, f);
-    const bool far = fabsf(ref) > kFar;
 #pragma unroll
     for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
-      const float t = far ? (f[i] - ref) * c : fmaf(f[i], c, -m2), e = ex2_approx_ftz(t);
+      const float t = far(m2) ? (f[i] - ref) * c : fmaf(f[i], c, -m2), e = ex2_approx_ftz(t);
       s += e;
       w = fmaf(e, fmaxf(t, kLowest), w);
     }
@@ -315,7 +319,7 @@ struct Sums {
   // The warp's (maximum, s, w), the sums relative to that maximum.
   __device__ __forceinline__ float3 over_warp(float c) const {
     const float most = warp_max(word_max<T>(top));
-    float d = fabsf(most) > kFar || far() ? (ref - most) * c : fmaf(-most, c, m2);
+    float d = far() || far(most * c) ? (ref - most) * c - added(ref, m2, c) : fmaf(-most, c, m2);
     if (limit == -INFINITY) d = 0.f;  // nothing but masked elements, or NaN: its sums are 0, or NaN
     const float r = ex2_approx_ftz(d), sum = sum_of(s);
     return make_float3(most, warp_sum(sum * r), ENTROPY ? warp_sum(r * fmaf(sum, fmaxf(d, kLowest), sum_of(w))) : 0.f);
@@ -521,6 +525,8 @@ struct Logprobs : Rows {
   float *logprobs, *entropy, *lse, *top_logprobs;
   int* top_ids;
 };
+// (x - most) / temperature; the difference by itself may be beyond f32.
+__device__ __forceinline__ float scaled_apart(float x, float most, float temperature) { return 2 * ((0.5f * x - 0.5f * most) / temperature); }
 __device__ __forceinline__ void write_results(const Logprobs& p, long long row, int token, float x, float3 sum) {
   if ((threadIdx.x & 31) != 0) return;
   const float log_sum = logf(sum.y);
@@ -528,7 +534,7 @@ __device__ __forceinline__ void write_results(const Logprobs& p, long long row, 
   if (p.entropy) p.entropy[row] = log_sum - kLn2 * (sum.z / sum.y);
   if (p.logprobs) {
     if (token < 0) atomicMax(p.status, DEV_BAD_INDEX);
-    p.logprobs[row] = token < 0 ? NAN : (x - sum.x) / p.temperature - log_sum;
+    p.logprobs[row] = token < 0 ? NAN : scaled_apart(x, sum.x, p.temperature) - log_sum;
   }
 }
 // Token of a row: 0 for padding, -1 when it is out of range (or there are no tokens).
@@ -710,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, kTopPerSm) top_logprobs_kernel(const
       if (lane < p.top) {
         const int id = best.out_index[lane];
         const bool there = id >= 0 && id != INT_MAX;
-        p.top_logprobs[row * p.top + lane] = there ? (best.out_value[lane] - sum.x) / p.temperature - log_sum : NAN;
+        p.top_logprobs[row * p.top + lane] = there ? scaled_apart(best.out_value[lane], sum.x, p.temperature) - log_sum : NAN;
         p.top_ids[row * p.top + lane] = there ? id + 1 : 0;
       }
     }

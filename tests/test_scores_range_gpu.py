@@ -1,10 +1,15 @@
 """Operators over rows of logits at the ends of their range: rows that start anywhere, large logits, small temperatures, rows that a mask
-of any kind leaves empty."""
+of any kind leaves empty.
+
+Temperatures here are powers of two, the same number in f32 and f64.  What a row's shift or a temperature does to the exponents cancels
+in differences from the row's maximum, which f32 holds to 2^-24 of themselves: the tolerances of test_logprobs_gpu.py and
+test_distill_gpu.py hold whatever the magnitude.  Results beyond f32 are its infinities.
+"""
 import pytest
 
 pytestmark = pytest.mark.gpu
 
-from test_logprobs_gpu import TYPES, check, make  # noqa: E402
+from test_logprobs_gpu import TYPES, check, close, make, reference  # noqa: E402
 
 
 @pytest.mark.parametrize("shift", range(8))
@@ -17,3 +22,52 @@ def test_lists_made_again_from_rows_that_start_anywhere(cuda, shift, dtype):
     x[:2] = torch.linspace(-20, 20, V, device="cuda").to(x.dtype)
     x[2:] = 1.5
     check(cuda, x, torch.tensor([1, V, 1, V], device="cuda"), 32)
+
+
+MAGNITUDES = (3e4, 1e9, 1e10, 3e12, 1e20, 1e29, 2e30, 3e38)
+
+
+def shifted_rows(T, V, dtype, seed=0, shift=0):
+    """Rows whose maximum is a large number: equal throughout, one element or half of the row above the rest, random but for a shift."""
+    import torch
+    x = make(T, V, dtype, seed=seed, shift=shift)
+    most = torch.finfo(x.dtype).max
+    row = 0
+    for m in MAGNITUDES:
+        for a in (m, -m):
+            if m > most:
+                a = most if a > 0 else -most
+            x[row] = a
+            x[row + 1] = -abs(a)
+            x[row + 1, V // 3] = a
+            x[row + 2] = a
+            x[row + 2, V // 2:] = a * 2 if a < 0 and abs(a) * 2 < most else -abs(a)
+            row += 3
+    for a in (1e3, 1e4, -1e3, -1e4):
+        x[row] += a
+        row += 1
+    x[row] = -float("inf")
+    x[row, V // 2:] = -1e4
+    x[row + 1] = -float("inf")
+    x[row + 1, V - 1] = most
+    return x, row + 2
+
+
+@pytest.mark.parametrize("T,V", [(54, 1), (54, 70), (54, 9001), (900, 1025), (54, 70001)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_logits(cuda, T, V, dtype):
+    import torch
+    for temperature in (1.0, 2.0 ** -5, 2.0 ** -19, 2.0 ** 19):
+        x, rows = shifted_rows(T, V, dtype, seed=V, shift=1)
+        assert rows <= T
+        tokens = torch.randint(1, V + 1, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+        for top in (0, min(V, 5)):
+            r = cuda.logprobs.token_logprobs(x, tokens, top=top, temperature=temperature)
+            want = reference(x, tokens, top, temperature)
+            for got, w in zip(r[:3 if top == 0 else 4], want):
+                inside = w.abs() < 3.4e38
+                close(torch.where(inside, got, torch.zeros_like(got)), torch.where(inside, w, torch.zeros_like(w)))
+                assert (inside | (got == torch.sign(w) * float("inf")) | (got.double().abs() > 3.3e38)).all()
+            if top:
+                assert r.top_ids.equal(want[4])
+    cuda.check_device_status(0)
