@@ -818,8 +818,8 @@ __device__ __forceinline__ double sum_lanes(double v) {
 
 // The teacher's side of a row, in f64: what its list leaves over is a difference from one.
 struct Teacher {
-  double terms, all, norm;   // sum q (log q - z), sum q
-  float listed_max, listed;  // what the student gives to the listed ids, each once: maximum, sum of powers relative to it
+  double terms, all, norm;   // sum q (log q - (z - listed_max / temperature)), sum q
+  float listed_max, listed;  // the student's largest listed logit, and the sum of powers, relative to it, of the listed ids, each once
 };
 static_assert(sizeof(Teacher) == 2 * sizeof(float4), "a teacher takes two records");
 // A warp's lists of `entries` each, in dynamic shared memory: ids (0: unused), q, the student's logits.
@@ -889,6 +889,7 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
       if (id[i]) most = fmaxf(most, v[i]);
     }
   }
+  x_most = fmaxf(warp_max(x_most), -FLT_MAX);
   double norm;
   if constexpr (TAIL) {
     norm = p.teacher_lse[row];
@@ -905,7 +906,7 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
     const double log_q = fma((double)t.q[j], p.per_temperature, -norm);
     const double q = exp(log_q);
     all += q;
-    if (q != 0) terms = fma(q, log_q - (double)t.x[j] * p.per_temperature, terms);
+    if (q != 0) terms = fma(q, log_q - ((double)t.x[j] - (double)x_most) * p.per_temperature, terms);
     t.q[j] = (float)q;
   }
   terms = sum_lanes(terms);
@@ -913,7 +914,6 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
   if constexpr (TAIL) {
     all = sum_lanes(all);
     __syncwarp();
-    x_most = fmaxf(warp_max(x_most), -FLT_MAX);
     // Ids that meet in a small table are looked for in the list, and all but the first of those alike marked.
     const unsigned mask = (32u << (31 - __clz(words))) - 1;
     for (int j0 = 0; j0 < p.entries; j0 += 32) {
@@ -966,7 +966,7 @@ __device__ __forceinline__ float4 saved_of(const Distill& p, const Teacher& t, f
 template <bool TAIL>
 __device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, float3 sum) {
   const double log_total = log_of(sum.y);
-  double loss = t.terms + t.all * fma((double)sum.x, p.per_temperature, log_total);
+  double loss = t.terms + t.all * fma((double)sum.x - (double)t.listed_max, p.per_temperature, log_total);  // differences: z may be large
   if (TAIL && left_over(t) != 0) loss += left_over(t) * (log(left_over(t)) - (log_of(sum.z) - log_total));
   p.loss[row] = (float)loss;
   reinterpret_cast<float4*>(p.saved)[row] = saved_of<TAIL>(p, t, sum, log_total);

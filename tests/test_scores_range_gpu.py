@@ -9,6 +9,7 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
+from test_distill_gpu import close_loss, teacher  # noqa: E402
 from test_logprobs_gpu import TYPES, check, close, make, reference  # noqa: E402
 
 
@@ -70,4 +71,44 @@ def test_large_logits(cuda, T, V, dtype):
                 assert (inside | (got == torch.sign(w) * float("inf")) | (got.double().abs() > 3.3e38)).all()
             if top:
                 assert r.top_ids.equal(want[4])
+    cuda.check_device_status(0)
+
+
+def distillation_loss(x, ids, values, lse, temperature):
+    """In f64; what the teacher's list leaves over by logarithms."""
+    import torch
+    used = ids > 0
+    at = (ids.long() - 1).clamp(min=0)
+    z = x.double() / temperature
+    u = torch.where(used, values.double() / temperature, -float("inf"))
+    log_q = u - (torch.logsumexp(u, 1, keepdim=True) if lse is None else lse.double()[:, None])
+    q = log_q.exp()
+    log_p = torch.log_softmax(z, 1)
+    loss = torch.where(q > 0, q * (log_q - log_p.gather(1, at)), 0.0).sum(1)
+    if lse is not None:
+        listed = torch.zeros_like(log_p).scatter_add_(1, at, used.double()) > 0
+        left = (1 - q.sum(1, keepdim=True)).clamp(min=0)
+        log_rest = torch.logsumexp(log_p.masked_fill(listed, -float("inf")), 1, keepdim=True)
+        loss = loss + (torch.xlogy(left, left) - torch.where(left > 0, left * log_rest, 0.0))[:, 0]
+    return loss
+
+
+@pytest.mark.parametrize("T,V", [(54, 3), (54, 9001), (900, 20003), (54, 70001), (160, 70001)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_loss_of_large_logits(cuda, T, V, dtype):
+    """Terms of a loss that are large beside the loss."""
+    import torch
+    inf = float("inf")
+    for temperature in (1.0, 2.0 ** -5, 2.0 ** (-13 if dtype == "float16" else -19)):  # f16 does not hold 2^19 times a gradient
+        x, rows = shifted_rows(T, V, dtype, seed=V + 1, shift=3)
+        x[x == -inf] = -1.0  # what a list gives to a masked id is an infinite loss
+        ids, values, _ = teacher(T, V, min(V, 30), dtype, seed=V)
+        ids[:, 0] = V // 3 + 1
+        z = x.double() / temperature
+        small = (torch.logsumexp(z, 1) - z.gather(1, ids.long() - 1).amin(1)) < 1e30  # or the loss is beyond f32
+        x, ids, values = x[small], ids[small], values[small] * temperature
+        assert len(x) >= 30
+        want = distillation_loss(x, ids, values.to(x.dtype), None, temperature)
+        close_loss(cuda.distill.distill_fwd(x, ids, values.to(x.dtype), None, temperature)[0], want)
+        close_loss(cuda.distill.distill_fwd_bwd(x, ids, values.to(x.dtype), torch.ones(len(x), device="cuda"), None, temperature)[0], want)
     cuda.check_device_status(0)
