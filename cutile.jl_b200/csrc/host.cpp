@@ -515,7 +515,7 @@ PyObject* distill_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Call c(*r.x);
   if (!c.ok()) return nullptr;
   const auto f = r.x->options().dtype(at::kFloat);
-  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 4}, f);
+  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 8}, f);
   const int s = without_gil([&] {
     return ctb_distill_fwd(c.ctx, c.stream, r.x->data_ptr(), t.ids->data_ptr(), t.bits, t.values->data_ptr(), t.dtype, f32(lse), f32(&loss),
                            f32(&saved), r.V, r.T, r.ld, t.entries, temperature, r.dtype);
@@ -530,7 +530,7 @@ PyObject* distill_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Teacher t;
   const Tensor *saved, *d;
   float temperature;
-  if (n != 7 || !r.take(a[0]) || !t.take(a[1], a[2], r) || !(saved = cuda_tensor(a[3])) || !maybe_f32(saved, *r.x, {r.T, 4}) ||
+  if (n != 7 || !r.take(a[0]) || !t.take(a[1], a[2], r) || !(saved = cuda_tensor(a[3])) || !maybe_f32(saved, *r.x, {r.T, 8}) ||
       !(d = cuda_tensor(a[4])) || !maybe_f32(d, *r.x, {r.T}) || !as_float(a[5], &temperature) || !r.take_out(a[6]))
     return decline();
   Call c(*r.x);
@@ -557,7 +557,7 @@ PyObject* distill_fwd_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!c.ok()) return nullptr;
   r.make_out();
   const auto f = r.x->options().dtype(at::kFloat);
-  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 4}, f);
+  Tensor loss = at::empty({r.T}, f), saved = at::empty({r.T, 8}, f);
   const int s = without_gil([&] {
     return ctb_distill_fwd_bwd(c.ctx, c.stream, r.out.data_ptr(), r.x->data_ptr(), t.ids->data_ptr(), t.bits, t.values->data_ptr(), t.dtype,
                                f32(lse), f32(&loss), f32(&saved), f32(d), r.V, r.T, r.ld_out, r.ld, t.entries, temperature, r.dtype);

@@ -27,7 +27,7 @@ def _teacher(logits, T, ids, values, lse):
 
 
 def distill_fwd(logits, teacher_ids, teacher_values, teacher_lse=None, temperature=1.0, **hints):
-    """Returns (loss [T] f32, saved [T, 4] f32); saved is what distill_bwd needs."""
+    """Returns (loss [T] f32, saved [T, 8] f32); saved is what distill_bwd needs."""
     if not hints:
         r = _host.distill_fwd(logits, teacher_ids, teacher_values, teacher_lse, temperature)
         if r is not None:
@@ -36,7 +36,7 @@ def distill_fwd(logits, teacher_ids, teacher_values, teacher_lse=None, temperatu
     ld, T, V = rows(logits, "logits")
     entries, bits, values_code = _teacher(logits, T, teacher_ids, teacher_values, teacher_lse)
     loss = torch.empty(T, dtype=torch.float32, device=logits.device)
-    saved = torch.empty((T, 4), dtype=torch.float32, device=logits.device)
+    saved = torch.empty((T, 8), dtype=torch.float32, device=logits.device)
     _lib.check(_lib.lib.ctb_distill_fwd(ctx, stream, ptr(logits), ptr(teacher_ids), bits, ptr(teacher_values), values_code,
                                         ptr(teacher_lse), ptr(loss), ptr(saved), V, T, ld, entries, float(temperature),
                                         dtype_code(logits)))
@@ -52,7 +52,7 @@ def distill_bwd(logits, teacher_ids, teacher_values, saved, d_loss, temperature=
     ctx, stream = handles(logits, hints)
     ld, T, V = rows(logits, "logits")
     entries, bits, values_code = _teacher(logits, T, teacher_ids, teacher_values, None)
-    dense(saved, (T, 4), "saved", logits, torch.float32)
+    dense(saved, (T, 8), "saved", logits, torch.float32)
     dense(d_loss, (T,), "d_loss", logits, torch.float32)
     out, ld_out = gradient_of(logits, out)
     _lib.check(_lib.lib.ctb_distill_bwd(ctx, stream, ptr(out), ptr(logits), ptr(teacher_ids), bits, ptr(teacher_values), values_code,
@@ -73,7 +73,7 @@ def distill_fwd_bwd(logits, teacher_ids, teacher_values, d_loss, teacher_lse=Non
     dense(d_loss, (T,), "d_loss", logits, torch.float32)
     out, ld_out = gradient_of(logits, out)
     loss = torch.empty(T, dtype=torch.float32, device=logits.device)
-    saved = torch.empty((T, 4), dtype=torch.float32, device=logits.device)
+    saved = torch.empty((T, 8), dtype=torch.float32, device=logits.device)
     _lib.check(_lib.lib.ctb_distill_fwd_bwd(ctx, stream, ptr(out), ptr(logits), ptr(teacher_ids), bits, ptr(teacher_values), values_code,
                                             ptr(teacher_lse), ptr(loss), ptr(saved), ptr(d_loss), V, T, ld_out, ld, entries,
                                             float(temperature), dtype_code(logits)))

@@ -233,7 +233,7 @@ end
 "Distillation from a teacher's list (entries, T): returns (loss, saved) for `distill_bwd`."
 function distill_fwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_values::CuArray{Q}; teacher_lse=nothing, temperature::Real=1) where {X,Q}
     V, T = size(logits)
-    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 4, T)
+    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 8, T)
     check(ccall((:ctb_distill_fwd, LIB), Cint,
         (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64,
          Cint, Cfloat, Cint),
@@ -257,7 +257,7 @@ end
 function distill_fwd_bwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_values::CuArray{Q}, d_loss; teacher_lse=nothing,
                          temperature::Real=1) where {X,Q}
     V, T = size(logits); d = similar(logits)
-    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 4, T)
+    loss = CuArray{Float32}(undef, T); saved = CuArray{Float32}(undef, 8, T)
     check(ccall((:ctb_distill_fwd_bwd, LIB), Cint,
         (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
          Int64, Int64, Int64, Int64, Cint, Cfloat, Cint),

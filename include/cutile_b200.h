@@ -130,7 +130,7 @@ int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const voi
  *   else:             q_j = exp(u_j - teacher_lse), and what is left, q_r = max(0, 1 - sum_j q_j), stands against the
  *                     probability p_r that the student gives to all ids that are not listed:
  *                     loss = sum_j q_j (log q_j - log p[id_j]) + q_r (log q_r - log p_r)
- * loss (T) f32; saved (4, T) f32, 16-byte aligned, is what the gradient needs.  An id may occur more than once.  A row without a
+ * loss (T) f32; saved (8, T) f32, 16-byte aligned, is what the gradient needs.  An id may occur more than once.  A row without a
  * used entry is padding: its logits are not read, loss and gradient are 0.  An id outside of 0..V is a bad index
  * (ctb_check_device_status): the row's loss is NaN and its gradient 0. */
 int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,

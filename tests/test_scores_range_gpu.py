@@ -10,7 +10,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 from test_distill_gpu import close_loss, teacher  # noqa: E402
-from test_logprobs_gpu import TYPES, check, close, make, reference  # noqa: E402
+from test_logprobs_gpu import TYPES, check, close, close_gradient, make, reference  # noqa: E402
 
 
 @pytest.mark.parametrize("shift", range(8))
@@ -74,8 +74,8 @@ def test_large_logits(cuda, T, V, dtype):
     cuda.check_device_status(0)
 
 
-def distillation_loss(x, ids, values, lse, temperature):
-    """In f64; what the teacher's list leaves over by logarithms."""
+def distillation(x, ids, values, lse, temperature, d_loss):
+    """(loss, gradient, tolerance of the gradient) in f64; what the teacher's list leaves over by logarithms."""
     import torch
     used = ids > 0
     at = (ids.long() - 1).clamp(min=0)
@@ -84,19 +84,48 @@ def distillation_loss(x, ids, values, lse, temperature):
     log_q = u - (torch.logsumexp(u, 1, keepdim=True) if lse is None else lse.double()[:, None])
     q = log_q.exp()
     log_p = torch.log_softmax(z, 1)
+    p = log_p.exp()
     loss = torch.where(q > 0, q * (log_q - log_p.gather(1, at)), 0.0).sum(1)
+    g = (d_loss.double() / temperature)[:, None]
+    qv = torch.zeros_like(p).scatter_add_(1, at, q)
+    whole = torch.ones_like(g)
+    rest = torch.zeros_like(p)
     if lse is not None:
-        listed = torch.zeros_like(log_p).scatter_add_(1, at, used.double()) > 0
+        listed = torch.zeros_like(p).scatter_add_(1, at, used.double()) > 0
         left = (1 - q.sum(1, keepdim=True)).clamp(min=0)
+        whole = q.sum(1, keepdim=True) + left
         log_rest = torch.logsumexp(log_p.masked_fill(listed, -float("inf")), 1, keepdim=True)
         loss = loss + (torch.xlogy(left, left) - torch.where(left > 0, left * log_rest, 0.0))[:, 0]
-    return loss
+        rest = torch.where(listed, 0.0, left * (log_p - log_rest).exp())
+    d = g * (whole * p - rest - qv)
+    # see test_distill_gpu.py; and a power below 2^-126 is 0
+    tol = g.abs() * (2.0 ** -16 * (whole * p + rest) + 2.0 ** -22 * qv + 2.0 ** -125)
+    return loss, d, tol
+
+
+def check_distillation(cuda, x, ids, values, lse, temperature):
+    """By two calls, by one, and over the logits."""
+    import torch
+    ops = cuda.distill
+    g = torch.rand(len(x), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) + 0.1
+    want_loss, want, tol = distillation(x, ids, values, lse, temperature, g)
+    loss, saved = ops.distill_fwd(x, ids, values, lse, temperature)
+    close_loss(loss, want_loss)
+    d = ops.distill_bwd(x, ids, values, saved, g, temperature)
+    close_gradient(d, want, tol)
+    both_loss, both = ops.distill_fwd_bwd(x, ids, values, g, lse, temperature)
+    close_loss(both_loss, want_loss)
+    close_gradient(both, want, tol)
+    over = x.clone()
+    assert ops.distill_bwd(over, ids, values, saved, g, temperature, out=over).equal(d)
+    over = x.clone()
+    assert ops.distill_fwd_bwd(over, ids, values, g, lse, temperature, out=over)[1].equal(both)
 
 
 @pytest.mark.parametrize("T,V", [(54, 3), (54, 9001), (900, 20003), (54, 70001), (160, 70001)])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_distillation_loss_of_large_logits(cuda, T, V, dtype):
-    """Terms of a loss that are large beside the loss."""
+def test_distillation_of_large_logits(cuda, T, V, dtype):
+    """Loss and gradient where the logarithm of a row's sum is large beside what the sum's last digit says."""
     import torch
     inf = float("inf")
     for temperature in (1.0, 2.0 ** -5, 2.0 ** (-13 if dtype == "float16" else -19)):  # f16 does not hold 2^19 times a gradient
@@ -108,7 +137,5 @@ def test_distillation_loss_of_large_logits(cuda, T, V, dtype):
         small = (torch.logsumexp(z, 1) - z.gather(1, ids.long() - 1).amin(1)) < 1e30  # or the loss is beyond f32
         x, ids, values = x[small], ids[small], values[small] * temperature
         assert len(x) >= 30
-        want = distillation_loss(x, ids, values.to(x.dtype), None, temperature)
-        close_loss(cuda.distill.distill_fwd(x, ids, values.to(x.dtype), None, temperature)[0], want)
-        close_loss(cuda.distill.distill_fwd_bwd(x, ids, values.to(x.dtype), torch.ones(len(x), device="cuda"), None, temperature)[0], want)
+        check_distillation(cuda, x, ids, values.to(x.dtype), None, temperature)
     cuda.check_device_status(0)
