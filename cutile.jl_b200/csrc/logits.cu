@@ -803,11 +803,14 @@ __device__ __forceinline__ void patch_entries(const Range<T>& r, const Inner& in
 // ------------------------------------------------------------------ distillation, forward, and the gradient at once
 // What the gradient needs to know of a row.  Maximum and sum apart, as p = 2^((x - most) c) / sum: one f32 for the logarithm of the sum of powers
 // would leave p off by 2^-24 of that logarithm, and at -1e9 (a row that is masked by a number, a small temperature) nothing of the sum.
+//   listed elements: d = g (whole p - q)      others: d = g outside r, r = 2^((x - rest_most) c) / rest_sum
+// With a rest, r is its share of the rest's probability p_r, and outside = whole p_r - (what the list leaves over): p is 0 in f32 where the
+// gradient of a small rest is not.  Else r = p, outside = 1.
 struct alignas(16) Saved {
   float most, sum;       // of the row
-  float outside, whole;  // d = g outside p where the teacher lists nothing, g (whole p - q) elsewhere; whole 0: the row has no gradient
+  float outside, whole;  // whole 0: the row has no gradient
   float norm, norm_low;  // q = exp(value / temperature - norm - norm_low); norm_low 0 with teacher_lse
-  float none[2];
+  float rest_most, rest_sum;
 };
 static_assert(sizeof(Saved) == 32, "a row's saved values are eight f32");
 struct Distill : Rows {
@@ -951,32 +954,38 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
   __syncwarp();
   return {terms, TAIL ? all : 1, norm, x_most, listed};
 }
-// A row's (maximum, s) with what the teacher lists, which with TAIL they leave out: maximum, total, and the rest's share of it.
+// The maximum and the sum of powers of a row, and of what it has besides the teacher's list.  The two do not share a maximum: a student that is
+// sure of what is listed leaves the rest less than f32 holds beside it.
+struct Sides {
+  float most, sum, rest_most, rest_sum;
+};
+// sum: of the row, with TAIL without what is listed.
 template <bool TAIL>
-__device__ __forceinline__ float3 with_listed(const Distill& p, const Teacher& t, float3 sum) {
-  if constexpr (!TAIL) return make_float3(sum.x, sum.y, sum.y);
-  const float both = fmaxf(sum.x, t.listed_max), rest = sum.y * ex2_approx_ftz((sum.x - both) * p.c);
-  return make_float3(both, rest + t.listed * ex2_approx_ftz((t.listed_max - both) * p.c), rest);
+__device__ __forceinline__ Sides with_listed(const Distill& p, const Teacher& t, float3 sum) {
+  if constexpr (!TAIL) return {sum.x, sum.y, sum.x, sum.y};
+  const float most = fmaxf(sum.x, t.listed_max);
+  return {most, sum.y * ex2_approx_ftz((sum.x - most) * p.c) + t.listed * ex2_approx_ftz((t.listed_max - most) * p.c), sum.x, sum.y};
 }
-// What the teacher's list leaves over, and the factor of p outside of the list.
+// What the teacher's list leaves over.
 __device__ __forceinline__ double left_over(const Teacher& t) { return t.all > 1 ? 0 : 1 - t.all; }
-__device__ __forceinline__ float outside_of(const Teacher& t, float3 sum) {
-  const double left = left_over(t), whole = t.all + left;
-  return (float)(sum.z == 0.f ? whole : whole - left * ((double)sum.y / (double)sum.z));
-}
 template <bool TAIL>
-__device__ __forceinline__ Saved saved_of(const Teacher& t, float3 sum) {
+__device__ __forceinline__ Saved saved_of(const Distill& p, const Teacher& t, const Sides& of) {
   const float norm = (float)t.norm;
-  return {sum.x, sum.y, TAIL ? outside_of(t, sum) : 1.f, TAIL ? (float)(t.all + left_over(t)) : 1.f, norm, TAIL ? 0.f : (float)(t.norm - (double)norm), {0.f, 0.f}};
+  if constexpr (!TAIL) return {of.most, of.sum, 1.f, 1.f, norm, (float)(t.norm - (double)norm), of.most, of.sum};
+  const double left = left_over(t), whole = t.all + left;
+  if (of.rest_sum == 0.f) return {of.most, of.sum, (float)whole, (float)whole, norm, 0.f, of.most, of.sum};  // all else is masked, and gets 0
+  const double share = exp(((double)of.rest_most - (double)of.most) * p.per_temperature) * (double)of.rest_sum / (double)of.sum;
+  return {of.most, of.sum, (float)(whole * share - left), (float)whole, norm, 0.f, of.rest_most, of.rest_sum};
 }
 // Loss and saved values of a row; one lane.
 template <bool TAIL>
-__device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, float3 sum) {
-  const double log_total = log_of(sum.y);
-  double loss = t.terms + t.all * fma((double)sum.x - (double)t.listed_max, p.per_temperature, log_total);  // differences: z may be large
-  if (TAIL && left_over(t) != 0) loss += left_over(t) * (log(left_over(t)) - (log_of(sum.z) - log_total));
+__device__ __noinline__ void close_row(const Distill& p, long long row, const Teacher& t, const Sides& of) {
+  const double log_total = log_of(of.sum);
+  double loss = t.terms + t.all * fma((double)of.most - (double)t.listed_max, p.per_temperature, log_total);  // differences: z may be large
+  if (TAIL && left_over(t) != 0)
+    loss += left_over(t) * (log(left_over(t)) - fma((double)of.rest_most - (double)of.most, p.per_temperature, log_of(of.rest_sum) - log_total));
   p.loss[row] = (float)loss;
-  p.saved[row] = saved_of<TAIL>(t, sum);
+  p.saved[row] = saved_of<TAIL>(p, t, of);
 }
 
 // ------------------------------------------------------------------ backward
@@ -1111,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __
   grid_dependency_launch();
 }
 
-// A part of a row's gradient, by W warps that own each their vectors of it, and the listed elements in those: g (whole p - q), elsewhere a p.
+// A part of a row's gradient, by W warps that own each their vectors of it, and the listed elements in those.
 // What the listed logits give is taken from them before the part is streamed (dx may be the logits themselves).  own_list: of the warp.
 // given: the entries as learn has left them, if it has.
 template <typename T, int W, bool GIVEN, typename P>
@@ -1161,7 +1170,7 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
   }
   const float g = p.d_loss[row] / p.temperature;
   __syncwarp();
-  stream_gradient<T, false, true, W>(r, in, dst, p.c, saved.most, g * saved.outside * per_sum, 0.f);
+  stream_gradient<T, false, true, W>(r, in, dst, p.c, saved.rest_most, g * saved.outside / saved.rest_sum, 0.f);
   __syncwarp();
   for (int k = lane; k < own; k += 32) {
     const int id = entry[k];
@@ -1222,11 +1231,11 @@ __global__ void __launch_bounds__(kThreads + 32, kBothPerSm) distill_both_kernel
     }
     __syncthreads();
     const Teacher t = teachers[turn];
-    const float3 sum = with_listed<TAIL>(p, t, join_warps<kWarps>(red[turn], p.c));
+    const Sides sides = with_listed<TAIL>(p, t, join_warps<kWarps>(red[turn], p.c));
     if (warp == kWarps) {
-      if (lane == 0) close_row<TAIL>(p, row, t, sum);
+      if (lane == 0) close_row<TAIL>(p, row, t, sides);
     } else {
-      distill_gradient<T, 1, true>(p, row, warp, saved_of<TAIL>(t, sum), lists, taught);
+      distill_gradient<T, 1, true>(p, row, warp, saved_of<TAIL>(p, t, sides), lists, taught);
     }
     turn ^= 1;
     __syncwarp();

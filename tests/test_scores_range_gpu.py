@@ -98,8 +98,8 @@ def distillation(x, ids, values, lse, temperature, d_loss):
         loss = loss + (torch.xlogy(left, left) - torch.where(left > 0, left * log_rest, 0.0))[:, 0]
         rest = torch.where(listed, 0.0, left * (log_p - log_rest).exp())
     d = g * (whole * p - rest - qv)
-    # see test_distill_gpu.py; and a power below 2^-126 is 0
-    tol = g.abs() * (2.0 ** -16 * (whole * p + rest) + 2.0 ** -22 * qv + 2.0 ** -125)
+    # see test_distill_gpu.py; and a power below 2^-126 counts as 0, of which the gradient takes at most g whole
+    tol = g.abs() * (2.0 ** -16 * (whole * p + rest) + 2.0 ** -22 * qv + 2.0 ** -125 * whole)
     return loss, d, tol
 
 
@@ -117,9 +117,11 @@ def check_distillation(cuda, x, ids, values, lse, temperature):
     close_loss(both_loss, want_loss)
     close_gradient(both, want, tol)
     over = x.clone()
-    assert ops.distill_bwd(over, ids, values, saved, g, temperature, out=over).equal(d)
+    want = ops.distill_bwd(over, ids, values, saved, g, temperature)
+    assert ops.distill_bwd(over, ids, values, saved, g, temperature, out=over).equal(want)
     over = x.clone()
-    assert ops.distill_fwd_bwd(over, ids, values, g, lse, temperature, out=over)[1].equal(both)
+    want = ops.distill_fwd_bwd(over, ids, values, g, lse, temperature)[1]
+    assert ops.distill_fwd_bwd(over, ids, values, g, lse, temperature, out=over)[1].equal(want)
 
 
 @pytest.mark.parametrize("T,V", [(54, 3), (54, 9001), (900, 20003), (54, 70001), (160, 70001)])
@@ -138,4 +140,25 @@ def test_distillation_of_large_logits(cuda, T, V, dtype):
         x, ids, values = x[small], ids[small], values[small] * temperature
         assert len(x) >= 30
         check_distillation(cuda, x, ids, values.to(x.dtype), None, temperature)
+    cuda.check_device_status(0)
+
+
+@pytest.mark.parametrize("T,V,K", [(12, 1000, 4), (12, 9001, 256), (700, 20003, 20), (12, 70001, 30)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rest_that_is_far_below_the_list(cuda, T, V, K, dtype):
+    """A student whose listed logits stand above all else by more than an f32 power holds: the loss is finite, and what the teacher leaves
+    over still pulls at all else."""
+    import torch
+    for k, (gap, temperature) in enumerate(((20, 1.0), (80, 1.0), (86, 1.0), (87, 1.0), (90, 1.0), (103, 1.0), (1000, 1.0), (10000, 1.0), (4.5, 2.0 ** -4),
+                                            (6, 2.0 ** -4), (30000, 2.0 ** -7), (-90, 1.0), (-1000, 1.0))):
+        x = make(T, V, dtype, seed=V + k, shift=k % 8, scale=1.0)
+        ids, values, all_values = teacher(T, V, K, seed=K)
+        ids[1, K // 2:] = 0
+        ids[2, 1:] = ids[2, :1]
+        values[2, 1:] = -float("inf")
+        x.scatter_(1, (ids.long() - 1).clamp(min=0), (x.gather(1, (ids.long() - 1).clamp(min=0)).float() + gap).to(x.dtype))
+        x[3] = x[3].round()
+        for over in (1.0, 1e-3, 0.0, -1.0):  # in logarithms, of what the list leaves over: much, little, next to nothing, less than nothing
+            lse = torch.logsumexp(values.double() / temperature, 1).float() + over
+            check_distillation(cuda, x, ids, values, lse, temperature)
     cuda.check_device_status(0)
