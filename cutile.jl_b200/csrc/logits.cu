@@ -806,11 +806,13 @@ __device__ __forceinline__ void patch_entries(const Range<T>& r, const Inner& in
 //   listed elements: d = g (whole p - q)      others: d = g outside r, r = 2^((x - rest_most) c) / rest_sum
 // With a rest, r is its share of the rest's probability p_r, and outside = whole p_r - (what the list leaves over): p is 0 in f32 where the
 // gradient of a small rest is not.  Else r = p, outside = 1.
+// The teacher's maximum and log of its sum are apart as well, q = exp((value - largest value) / temperature - norm - norm_low); with teacher_lse
+// q = exp(value / temperature - norm).
 struct alignas(16) Saved {
   float most, sum;       // of the row
-  float outside, whole;  // whole 0: the row has no gradient
-  float norm, norm_low;  // q = exp(value / temperature - norm - norm_low); norm_low 0 with teacher_lse
   float rest_most, rest_sum;
+  float whole, outside;  // whole 0: the row has no gradient; -1: there is no rest, whole = outside = 1, and in `outside` lies the largest value
+  float norm, norm_low;
 };
 static_assert(sizeof(Saved) == 32, "a row's saved values are eight f32");
 struct Distill : Rows {
@@ -832,8 +834,12 @@ __device__ __forceinline__ double sum_lanes(double v) {
 
 // The teacher's side of a row, in f64: what its list leaves over is a difference from one.
 struct Teacher {
-  double terms, all, norm;   // sum q (log q - (z - listed_max / temperature)), sum q
-  float listed_max, listed;  // the student's largest listed logit, and the sum of powers, relative to it, of the listed ids, each once
+  double terms, all, norm;   // sum q (log q - (z - listed_max / temperature)), sum q; norm: see Saved
+  float listed_max;          // the student's largest listed logit
+  union {
+    float listed;            // with a rest: the sum of powers, relative to it, of the listed ids, each once
+    float most;              // without: the teacher's largest value
+  };
 };
 static_assert(sizeof(Teacher) == 2 * sizeof(float4), "a teacher takes two records");
 // A warp's lists of `entries` each, in dynamic shared memory: ids (0: unused), q, the student's logits.
@@ -904,20 +910,21 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
     }
   }
   x_most = fmaxf(warp_max(x_most), -FLT_MAX);
-  double norm;
+  double norm, base = 0;
   if constexpr (TAIL) {
     norm = p.teacher_lse[row];
   } else {
     most = warp_max(most);
+    base = most;
     double sum = 0;
     for (int j = lane; j < p.entries; j += 32)
-      if (t.entry[j]) sum += exp(((double)t.q[j] - (double)most) * p.per_temperature);
-    norm = fma((double)most, p.per_temperature, log(sum_lanes(sum)));
+      if (t.entry[j]) sum += exp(((double)t.q[j] - base) * p.per_temperature);
+    norm = log(sum_lanes(sum));
   }
   double all = 0, terms = 0;
   for (int j = lane; j < p.entries; j += 32) {
     if (t.entry[j] == 0) continue;
-    const double log_q = fma((double)t.q[j], p.per_temperature, -norm);
+    const double log_q = fma((double)t.q[j] - base, p.per_temperature, -norm);
     const double q = exp(log_q);
     all += q;
     if (q != 0) terms = fma(q, log_q - ((double)t.x[j] - (double)x_most) * p.per_temperature, terms);
@@ -952,7 +959,7 @@ __device__ __noinline__ Teacher learn(const Distill& p, long long row, const Lis
     listed = warp_sum(listed);
   }
   __syncwarp();
-  return {terms, TAIL ? all : 1, norm, x_most, listed};
+  return {terms, TAIL ? all : 1, norm, x_most, {TAIL ? listed : most}};
 }
 // The maximum and the sum of powers of a row, and of what it has besides the teacher's list.  The two do not share a maximum: a student that is
 // sure of what is listed leaves the rest less than f32 holds beside it.
@@ -971,11 +978,11 @@ __device__ __forceinline__ double left_over(const Teacher& t) { return t.all > 1
 template <bool TAIL>
 __device__ __forceinline__ Saved saved_of(const Distill& p, const Teacher& t, const Sides& of) {
   const float norm = (float)t.norm;
-  if constexpr (!TAIL) return {of.most, of.sum, 1.f, 1.f, norm, (float)(t.norm - (double)norm), of.most, of.sum};
+  if constexpr (!TAIL) return {of.most, of.sum, of.most, of.sum, -1.f, t.most, norm, (float)(t.norm - (double)norm)};
   const double left = left_over(t), whole = t.all + left;
-  if (of.rest_sum == 0.f) return {of.most, of.sum, (float)whole, (float)whole, norm, 0.f, of.most, of.sum};  // all else is masked, and gets 0
+  if (of.rest_sum == 0.f) return {of.most, of.sum, of.most, of.sum, (float)whole, (float)whole, norm, 0.f};  // all else is masked, and gets 0
   const double share = exp(((double)of.rest_most - (double)of.most) * p.per_temperature) * (double)of.rest_sum / (double)of.sum;
-  return {of.most, of.sum, (float)(whole * share - left), (float)whole, norm, 0.f, of.rest_most, of.rest_sum};
+  return {of.most, of.sum, of.rest_most, of.rest_sum, (float)whole, (float)(whole * share - left), norm, 0.f};
 }
 // Loss and saved values of a row; one lane.
 template <bool TAIL>
@@ -1090,7 +1097,7 @@ __device__ __forceinline__ void distill_part(const Distill& p, long long row, in
       if (last) {
         __threadfence();
         const double2 a = __ldcg(reinterpret_cast<const double2*>(records)), b = __ldcg(reinterpret_cast<const double2*>(records + 1));
-        t = {a.x, a.y, b.x, __int_as_float(__double2loint(b.y)), __int_as_float(__double2hiint(b.y))};
+        t = {a.x, a.y, b.x, __int_as_float(__double2loint(b.y)), {__int_as_float(__double2hiint(b.y))}};
         sum = gather_records(records + 2, p.parts, 1, p.c);
       }
     }
@@ -1136,7 +1143,6 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
     stream_zeros<T, W>(r, dst);
     return;
   }
-  const double norm = (double)saved.norm + (double)saved.norm_low;
   int own = 0;
   __syncwarp();
   for (int j0 = 0; j0 < p.entries; j0 += 32) {
@@ -1157,20 +1163,22 @@ __device__ __forceinline__ void distill_gradient(const P& p, long long row, int 
     own += __popc(all);
   }
   __syncwarp();
-  const float per_sum = 1.f / saved.sum;
+  const bool list_is_all = saved.whole < 0.f;
+  const float whole = list_is_all ? 1.f : saved.whole, per_sum = 1.f / saved.sum;
   for (int k = lane; k < own; k += 32) {
     const int j = __float_as_int(weight[k]);
     const float of = GIVEN ? given.x[j] : to_float(r.src[entry[k] - 1]);
-    p_all[k] = saved.whole * (ex2_approx_ftz((of - saved.most) * p.c) * per_sum);
+    p_all[k] = whole * (ex2_approx_ftz((of - saved.most) * p.c) * per_sum);
     if constexpr (GIVEN) {
       weight[k] = given.q[j];
     } else {
-      weight[k] = (float)exp(fma((double)load_value(p.values, row * p.entries + j, p.values_dtype), p.per_temperature, -norm));
+      const double norm = (double)saved.norm + (double)saved.norm_low, base = list_is_all ? (double)saved.outside : 0.;
+      weight[k] = (float)exp(fma((double)load_value(p.values, row * p.entries + j, p.values_dtype) - base, p.per_temperature, -norm));
     }
   }
-  const float g = p.d_loss[row] / p.temperature;
+  const float g = p.d_loss[row] / p.temperature, outside = list_is_all ? 1.f : saved.outside;
   __syncwarp();
-  stream_gradient<T, false, true, W>(r, in, dst, p.c, saved.rest_most, g * saved.outside / saved.rest_sum, 0.f);
+  stream_gradient<T, false, true, W>(r, in, dst, p.c, saved.rest_most, g * outside / saved.rest_sum, 0.f);
   __syncwarp();
   for (int k = lane; k < own; k += 32) {
     const int id = entry[k];

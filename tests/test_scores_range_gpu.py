@@ -162,3 +162,33 @@ def test_rest_that_is_far_below_the_list(cuda, T, V, K, dtype):
             lse = torch.logsumexp(values.double() / temperature, 1).float() + over
             check_distillation(cuda, x, ids, values, lse, temperature)
     cuda.check_device_status(0)
+
+
+@pytest.mark.parametrize("T,V,K", [(8, 40, 5), (8, 9001, 256), (600, 20003, 40)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_values_of_the_teacher(cuda, T, V, K, dtype):
+    """A list is a distribution whatever its values' magnitude: equal ones of any size, a large shift, a small temperature."""
+    import torch
+    x = make(T, V, "float32", seed=V)
+    ids, values, _ = teacher(T, V, K, dtype, seed=K)
+    low = torch.finfo(values.dtype).min
+    values[0] = low
+    values[1] = -low
+    values[2] = low
+    values[2, K // 2:] = 0.5
+    values[3] += 6e4 if dtype == "float16" else 1e5
+    values[4] = 0.0 if dtype == "float16" else -1e30
+    for temperature in (1.0, 2.0 ** -5, 2.0 ** -19, 2.0 ** 19):
+        u = values.double() / temperature
+        got, saved = cuda.distill.distill_fwd(x, ids, values, None, temperature)
+        q = torch.softmax(u - u.amax(1, keepdim=True), 1)
+        log_p = torch.log_softmax(x.double() / temperature, 1)
+        want = (torch.xlogy(q, q) - q * log_p.gather(1, ids.long() - 1)).sum(1)
+        close_loss(got, want)
+        g = torch.ones(T, device="cuda")
+        d = (log_p.exp().scatter_add(1, ids.long() - 1, -q)) / temperature
+        tol = (2.0 ** -16 * log_p.exp() + torch.zeros_like(log_p).scatter_add(1, ids.long() - 1, 2.0 ** -22 * q) + 2.0 ** -125) / temperature
+        close_gradient(cuda.distill.distill_bwd(x, ids, values, saved, g, temperature), d, tol)
+        loss, both = cuda.distill.distill_fwd_bwd(x, ids, values, g, None, temperature)
+        close_loss(loss, want)
+        close_gradient(both, d, tol)
