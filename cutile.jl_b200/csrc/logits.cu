@@ -1008,6 +1008,7 @@ struct Backward : Rows {
   const void* tokens;
   int token_bits, top;
   const float *lse, *entropy, *d_logprobs, *d_entropy, *d_top;
+  float lse_c, lse_c_low;  // temperature c: what lse is in units of the exponents
   const int* top_ids;
   // distillation
   const void* ids;
@@ -1263,59 +1264,126 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) distill_backward_ker
   }
   grid_dependency_launch();
 }
+// The ids that gradients of a row meet directly, in the range r, with those gradients and with the logits: dx may be the logits themselves.
+// Returns how many, and the sum of the gradients; a warp, for itself.
+struct Meeting {
+  int entry[kMaxTop + 1];
+  float weight[kMaxTop + 1], x[kMaxTop + 1];
+  int others;  // whether a row is left for whole_rows_gradient
+};
+template <typename T>
+__device__ __forceinline__ int meet(const Backward& p, long long row, long long token, const Range<T>& r, Meeting& m, float& all) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  auto enter = [&](int j, long long id, float w) {
+    if (id < 0 || id > p.n) {
+      atomicMax(p.status, DEV_BAD_INDEX);
+      id = 0;
+    }
+    const int mine = in_range(r, id);
+    m.entry[j] = mine;
+    m.weight[j] = w;
+    m.x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
+  };
+  const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gt = lane < p.top ? p.d_top[row * p.top + lane] : 0.f;
+  all = g0 + warp_sum(gt);
+  if (lane < p.top) enter(lane, p.top_ids[row * p.top + lane], gt);
+  if (lane == 0 && p.d_logprobs) enter(p.top, token, g0);
+  __syncwarp();
+  return p.top + (p.d_logprobs ? 1 : 0);
+}
+
+// p = e^(z - lse) is off by the rounding of lse, 2^-24 of it at most.  Up to this |lse| that is no more than 2^-17 of p (f32), or 2^-16, less
+// than a tenth of a step of f16 and a hundredth of one of bf16.
+template <typename T>
+__device__ __forceinline__ bool lse_will_do(float lse) { return fabsf(lse) <= (sizeof(T) == 4 ? 128.f : 256.f); }
+// The other rows (large logits, small temperatures, rows masked by a number): a CTA takes one as a whole, for what it writes over others may not
+// read, and reads it twice, first for its maximum and sum.  Logits around 1000: 2048 x 100003 bf16 221 us (157 around 0), 512 x 50001 f32 59
+// (41), 64 x 128000 bf16 33 (11).
+template <typename T, bool ENTROPY>
+__device__ __forceinline__ void whole_row_gradient(const Backward& p, long long row, long long token, Meeting& m) {
+  __shared__ float red[3][kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Range<T> r = range_of<T>(p, row, 0);
+  r.v1 = (r.off + r.n + Range<T>::V - 1) / Range<T>::V;
+  const Inner in(r);
+  T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
+  float all;
+  const int entries = meet(p, row, token, r, m, all), edge = edge_index(r, in, threadIdx.x);
+  Sums<T, false> sums;
+  each_tile<T, kWarps, true>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
+  if (edge >= 0) sums.add_one(to_float(r.src[edge]), p.c);
+  __syncwarp();
+  const float3 of_warp = sums.over_warp(p.c);
+  __syncthreads();  // the row before is done with
+  if (lane == 0) {
+    red[0][warp] = of_warp.x;
+    red[1][warp] = of_warp.y;
+    red[2][warp] = 0.f;
+  }
+  __syncthreads();
+  const float3 sum = join_warps<kWarps>(red, p.c);
+  // lse says no more than these, unless it is not the row's own (a part of a vocabulary, with the lse of all)
+  const float lse = p.lse[row], own = sum.x / p.temperature + logf(sum.y);
+  const float per = (own == lse || fabsf(own - lse) <= 0x1p-21f * fabsf(lse) ? 1.f : expf(own - lse)) / sum.y;
+  const float gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
+  const float b = -gh * kLn2 / p.temperature * per;
+  const float a = -(all + gh * h) / p.temperature * per + (ENTROPY ? b * log2f(per) : 0.f);
+  stream_gradient<T, ENTROPY, true, kWarps>(r, in, dst, p.c, sum.x, a, b);
+  patch_entries<kWarps>(r, in, m.entry, m.weight, entries, [&](int id, int j, float direct) {
+    const float t = (m.x[j] - sum.x) * p.c, e = ex2_approx_ftz(t);
+    dst[id - 1] = from_float<T>(direct / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
+  });
+}
+// A call behind the loop over the other rows: in line, or within that loop, it takes registers that they need.
+template <typename T, bool ENTROPY>
+__device__ __noinline__ void whole_rows_gradient(const Backward& p, Meeting* lists) {
+  const Items items(p, kWarps);
+  for (long long item = items.at; item < items.end; item += items.step) {
+    const long long row = items.row(item), token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
+    if (item != row * p.parts || token == 0 || (p.tokens && (token < 0 || token > p.n)) || lse_will_do<T>(p.lse[row])) continue;
+    whole_row_gradient<T, ENTROPY>(p, row, token, lists[threadIdx.x >> 5]);
+  }
+}
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kernel(const __grid_constant__ Backward p) {
-  constexpr int kEntries = kMaxTop + 1;
-  __shared__ int entries_of[kWarps][kEntries];
-  __shared__ float weights_of[kWarps][kEntries], logits_of[kWarps][kEntries];
+  __shared__ Meeting lists[kWarps];
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int* entry = entries_of[warp];
-  float *weight = weights_of[warp], *x = logits_of[warp];
+  const int lane = threadIdx.x & 31;
+  Meeting& m = lists[threadIdx.x >> 5];
   const Items items(p, kWarps);
+  if (lane == 0) m.others = 0;
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item);
     const Range<T> r = range_of<T>(p, row, (int)(item - row * p.parts));
-    const Inner in(r);
     T* dst = static_cast<T*>(p.dx) + row * p.ld_dx;
-    __syncwarp();
-    // dx may be the logits themselves: the entries' logits are read before the part is streamed
-    auto enter = [&](int j, long long id, float w) {
-      if (id < 0 || id > p.n) {
-        atomicMax(p.status, DEV_BAD_INDEX);
-        id = 0;
-      }
-      const int mine = in_range(r, id);
-      entry[j] = mine;
-      weight[j] = w;
-      x[j] = mine ? to_float(r.src[mine - 1]) : 0.f;
-    };
-    float lse2, a, b = 0.f;
-    int entries;
-    {
-      const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
-      const bool bad = p.tokens && (token < 0 || token > p.n);
-      if (token == 0 || bad) {
-        if (bad && lane == 0) atomicMax(p.status, DEV_BAD_INDEX);
-        stream_zeros<T, kWarps>(r, dst);
-        continue;
-      }
-      const float g0 = p.d_logprobs ? p.d_logprobs[row] : 0.f, gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
-      const float gt = lane < p.top ? p.d_top[row * p.top + lane] : 0.f, all = g0 + warp_sum(gt);
-      if (lane < p.top) enter(lane, p.top_ids[row * p.top + lane], gt);
-      if (lane == 0 && p.d_logprobs) enter(p.top, token, g0);
-      entries = p.top + (p.d_logprobs ? 1 : 0);
-      lse2 = p.lse[row] * kLog2e;
-      a = -(all + gh * h) / p.temperature;
-      b = -gh * kLn2 / p.temperature;
+    const long long token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
+    const float lse = p.lse[row];
+    const bool bad = p.tokens && (token < 0 || token > p.n);
+    if (token == 0 || bad) {
+      if (bad && lane == 0) atomicMax(p.status, DEV_BAD_INDEX);
+      stream_zeros<T, kWarps>(r, dst);
+      continue;
     }
-    __syncwarp();
-    stream_gradient<T, ENTROPY, false, kWarps>(r, in, dst, p.c, lse2, a, b);
-    patch_entries<kWarps>(r, in, entry, weight, entries, [&](int id, int j, float sum) {
-      const float t = fmaf(x[j], p.c, -lse2), e = ex2_approx_ftz(t);
-      dst[id - 1] = from_float<T>(sum / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
+    if (!lse_will_do<T>(lse)) {
+      if (lane == 0) m.others = 1;
+      continue;
+    }
+    const Inner in(r);
+    float all;
+    const int entries = meet(p, row, token, r, m, all);
+    const float gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
+    // log2 p = t - lost: lse in units of c as it is, and what its f32 loses goes into a and b
+    const float base = lse * p.lse_c, lost = fmaf(lse, p.lse_c, -base) + lse * p.lse_c_low, more = ex2_approx_ftz(-lost);
+    const float b = -gh * kLn2 / p.temperature * more, a = -(all + gh * h) / p.temperature * more - b * lost;
+    stream_gradient<T, ENTROPY, false, kWarps>(r, in, dst, p.c, base, a, b);
+    patch_entries<kWarps>(r, in, m.entry, m.weight, entries, [&](int id, int j, float direct) {
+      const float t = fmaf(m.x[j], p.c, -base), e = ex2_approx_ftz(t);
+      dst[id - 1] = from_float<T>(direct / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
     });
   }
+  __syncwarp();
+  if (m.others) whole_rows_gradient<T, ENTROPY>(p, lists);  // all warps of a CTA have found the same
   grid_dependency_launch();
 }
 
@@ -1629,6 +1697,8 @@ extern "C" int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits
   p.temperature = temperature;
   p.status = ctx->dev_status;
   p.tokens = tokens; p.token_bits = token_bits; p.top = top;
+  const double lse_c = (double)temperature * (double)p.c;
+  p.lse_c = (float)lse_c; p.lse_c_low = (float)(lse_c - (double)p.lse_c);
   p.lse = lse; p.entropy = entropy; p.d_logprobs = d_logprobs; p.d_entropy = d_entropy; p.d_top = d_top_logprobs; p.top_ids = top_ids;
   return by_type(dtype, [&](auto t) { return launch_backward<decltype(t)>(ctx, static_cast<cudaStream_t>(stream), p, who); });
 }

@@ -10,7 +10,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 from test_distill_gpu import close_loss, teacher  # noqa: E402
-from test_logprobs_gpu import TYPES, check, close, close_gradient, make, reference  # noqa: E402
+from test_logprobs_gpu import TYPES, check, close, close_gradient, gradients, make, reference  # noqa: E402
 
 
 @pytest.mark.parametrize("shift", range(8))
@@ -192,3 +192,47 @@ def test_large_values_of_the_teacher(cuda, T, V, K, dtype):
         loss, both = cuda.distill.distill_fwd_bwd(x, ids, values, g, None, temperature)
         close_loss(loss, want)
         close_gradient(both, d, tol)
+
+
+@pytest.mark.parametrize("T,V", [(54, 1), (54, 70), (54, 9001), (900, 1025), (54, 70001), (160, 70001)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_large_logits(cuda, T, V, dtype):
+    """Gradients where half a step of an f32 lse is much of an exponent, or all of it; also over the logits, and into other columns."""
+    import torch
+    ops = cuda.logprobs
+    for k, temperature in enumerate((1.0, 2.0 ** -5, 2.0 ** (-13 if dtype == "float16" else -19), 8.0)):  # f16 does not hold 2^19 times a gradient
+        x, rows = shifted_rows(T, V, dtype, seed=V + 2, shift=k)
+        generator = torch.Generator(device="cuda").manual_seed(V)
+        tokens = torch.randint(1, V + 1, (T,), device="cuda", generator=generator)
+        tokens[1::7] = 0
+        top = min(V, 5)
+        r = ops.token_logprobs(x, tokens, top=top, temperature=temperature)
+        g0, gh, gt = (torch.randn(*s, device="cuda", generator=generator) for s in ((T,), (T,), (T, top)))
+        for a, b, c in ((g0, gh, gt), (g0, None, None), (None, gh, None)):
+            want, tol = gradients(x.double(), tokens, r.top_ids, a, b, c, temperature)
+            # a power below 2^-126 (log p of -88) counts as 0
+            lost = sum((t.abs() * w).view(T, -1).sum(1) for t, w in ((a, 1), (c, 1), (b, 100 + r.entropy)) if t is not None)
+            tol = tol + 2.0 ** -125 * lost.double()[:, None] / temperature
+            got = ops.token_logprobs_bwd(x, tokens, r.lse, r.entropy, a, b, r.top_ids, c, temperature)
+            close_gradient(got, want, tol)
+        over = x.clone()
+        want = ops.token_logprobs_bwd(over, tokens, r.lse, r.entropy, g0, gh, r.top_ids, gt, temperature)
+        wide = torch.full((T, V + 9), 7.0, device="cuda", dtype=x.dtype)
+        ops.token_logprobs_bwd(over, tokens, r.lse, r.entropy, g0, gh, r.top_ids, gt, temperature, out=wide[:, 2:2 + V])
+        assert wide[:, 2:2 + V].equal(want) and (wide[:, :2] == 7).all() and (wide[:, 2 + V:] == 7).all()
+        assert ops.token_logprobs_bwd(over, tokens, r.lse, r.entropy, g0, gh, r.top_ids, gt, temperature, out=over).equal(want)
+    cuda.check_device_status(0)
+
+
+@pytest.mark.parametrize("shift", [0.0, 500.0])
+def test_gradient_of_a_part_of_a_vocabulary(cuda, shift):
+    """The lse and the entropy of all parts make each part's gradient that of its columns."""
+    import torch
+    T, V, cut = 30, 5000, 1999
+    ops = cuda.logprobs
+    x = make(T, V, "float32", seed=3) + shift
+    tokens = torch.randint(1, cut + 1, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    r = ops.token_logprobs(x, tokens)
+    g0, gh = torch.randn(T, device="cuda"), torch.randn(T, device="cuda")
+    want, tol = gradients(x.double(), tokens, None, g0, gh, None, 1.0)
+    close_gradient(ops.token_logprobs_bwd(x[:, :cut], tokens, r.lse, r.entropy, g0, gh), want[:, :cut], tol[:, :cut] * 4)  # lse to 2^-15
