@@ -393,6 +393,7 @@ struct RouteBackward {
 
 // With u_j the gradient that reaches s_j of the j-th choice (0 for the others):
 //   sigmoid: dx_e = u_e s_e (1 - s_e)        softmax: dx_e = s_e (u_e - sum_j u_j s_j), a sum that is 0 for renormalised weights
+// s (1 - s) comes from e^-|x|, without a difference: 1 - s has no digits left in f32 from a logit of 17 on.
 template <typename T, int EPL>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBackward p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -423,8 +424,12 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
     float sj;  // score of this lane's choice
     if (p.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) s[i] = 1.f / (1.f + expf(-s[i]));
-      sj = 1.f / (1.f + expf(-xj));
+      for (int i = 0; i < EPL; ++i) {  // s (1 - s) in its place
+        const float e = expf(-fabsf(s[i])), inverse = 1.f / (1.f + e);
+        s[i] = e * inverse * inverse;
+      }
+      const float e = expf(-fabsf(xj));
+      sj = (xj < 0.f ? e : 1.f) / (1.f + e);
     } else {
       most = warp_max(most);
       float sum = 0.f;
@@ -459,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
         if (e == first + i) d[i] += v;
     }
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) d[i] *= s[i] * (p.sigmoid ? 1.f - s[i] : 1.f);
+    for (int i = 0; i < EPL; ++i) d[i] *= s[i];
     store_chunk<T, EPL>(dst, first, p.experts, p.wide, d);
   }
   grid_dependency_launch();

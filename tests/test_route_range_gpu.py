@@ -20,3 +20,23 @@ def test_as_many_tokens_as_there_are(cuda):
     assert ((x[at].double() - want).abs() <= 2.0 ** -10 * want).all()
     assert int((x != 0.125).sum()) == 3
     cuda.check_device_status(0)
+
+
+TYPES = ("float32", "float16", "bfloat16")
+
+
+@pytest.mark.parametrize("E,topk", [(4, 1), (30, 3), (64, 8), (128, 4), (250, 6), (512, 32)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_large_sigmoid_logits(cuda, E, topk, dtype):
+    """s (1 - s) where s is near 1 and near 0.  An exponential is off by 2^-22, its sum with 1, the quotient and four products by 2^-24 each: 2^-20."""
+    import torch
+    T = 40
+    generator = torch.Generator(device="cuda").manual_seed(E)
+    x = ((torch.rand(T, E, device="cuda", generator=generator) - 0.5) * 60).to(getattr(torch, dtype))
+    dw = torch.randn(topk, T, device="cuda", generator=generator)
+    ids = cuda.moe.moe_route(x, topk, score="sigmoid", renormalize=False)[1]
+    got = cuda.moe.moe_route_bwd(x, ids, dw, score="sigmoid", renormalize=False, scale=2.5)
+    want = torch.sigmoid(x.double()) * torch.sigmoid(-x.double()) * 2.5
+    want = want * torch.zeros_like(want).scatter_(1, ids.long().t() - 1, dw.double().t())
+    info = torch.finfo(got.dtype)
+    assert ((got.double() - want).abs() <= (2.0 ** -20 + info.eps / 2) * want.abs() + info.smallest_normal * info.eps).all()
