@@ -395,7 +395,7 @@ struct RouteBackward {
 // the chosen e, C that of dw_j e_j, and s' = s (1 - s) of a sigmoid:
 //   softmax: dx_v = scale / S e_v (dw_v - C / S)      renormalised: dx_v = scale / R e_v (dw_v - C / R) for the chosen, else 0
 //   sigmoid: dx_v = scale s'_v dw_v                   renormalised: dx_v = scale / R s'_v (dw_v - C / R)
-// (a chosen sum below 1e-20 is a constant).  s' comes from e^-|x| without a difference.  The
+// (a chosen sum below 1e-20 is a constant, and the gradient that without renormalisation).  s' comes from e^-|x| without a difference.  The
 // brackets are the sum of e_w (dw_v - dw_w), of which little is left where one expert has nearly all of it or the gradients are alike:
 //   - renormalised, dw is taken relative to that of the largest chosen e: f32 is then off by (2 topk + 1) 2^-23 of the sum of sizes;
 //   - else f32 is off by 17 * 2^-23 of it while an eighth of S is not chosen, and beyond S and C are f64 (f64 for all tokens: 16384 x 128 bf16
@@ -467,8 +467,8 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
         dw = id ? fmaf(dw - of, chosen, -mean) * per : 0.f;
         factor *= per;
       } else if (p.renormalize) {
-        apart = false;
-        factor *= 1e20f / all;
+        factor *= 1e20f;
+        mean = fmaf(of, chosen, mean);
       } else if (chosen > 0.875f * all) {
         double a = 0, b = (double)dw * (double)ej;
 #pragma unroll

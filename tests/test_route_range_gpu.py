@@ -103,3 +103,26 @@ def test_gradient_of_sure_choices(cuda, E, topk, dtype):
                 got = cuda.moe.moe_route_bwd(x, ids, dw, score=score, renormalize=renormalize, scale=2.5)
                 close(got, *gradient(x, ids, dw, score, renormalize, 2.5))
     cuda.check_device_status(0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gradient_of_a_sum_that_is_held(cuda, score):
+    """Chosen scores whose sum is below 1e-20 are divided by 1e-20: no gradient flows through that sum, and all else stays."""
+    import torch
+    T, E, topk, scale = 6, 16, 3, 1.5
+    x = torch.randn(T, E, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    bias = torch.zeros(E, device="cuda")
+    bias[[2, 7, 11]] = 4.0
+    x[:, bias > 0] -= 55
+    w, ids = cuda.moe.moe_route(x, topk, bias=bias, score=score, scale=scale, weights_dtype=torch.float32)
+    dw = torch.randn(topk, T, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))
+    x64 = x.double().requires_grad_()
+    s = torch.softmax(x64, 1) if score == "softmax" else torch.sigmoid(x64)
+    s = s.gather(1, ids.long().t() - 1)
+    assert (s.sum(1) < 1e-20).all()
+    (s / s.sum(1, keepdim=True).clamp(min=1e-20) * scale * dw.double().t()).sum().backward()
+    got = cuda.moe.moe_route_bwd(x, ids, dw, score=score, scale=scale)
+    # a sum of three products that may cancel, each off by 2^-22 and by 2^-24 of an argument of up to 60
+    size = (s.detach() * 1e20 * scale * dw.double().t().abs()).sum(1, keepdim=True)
+    assert ((got.double() - x64.grad).abs() <= 2.0 ** -17 * size).all()
+    assert (x64.grad[:, bias == 0].abs() > 2.0 ** -10 * size).any() == (score == "softmax")
