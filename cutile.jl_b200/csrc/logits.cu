@@ -1057,17 +1057,29 @@ __device__ __forceinline__ void clear_holes(unsigned* holes, int words) {
   for (int i = threadIdx.x & 31; i < words; i += 32) holes[i] = 0;
   __syncwarp();
 }
+// (maximum, s) of two stretches of a row.
+__device__ __forceinline__ float3 join_two(float3 a, float3 b, float c) {
+  const float most = fmaxf(fmaxf(a.x, b.x), -FLT_MAX);
+  return make_float3(most, fmaf(a.y, ex2_approx_ftz((a.x - most) * c), b.y * ex2_approx_ftz((b.x - most) * c)), 0.f);
+}
+// A warp has bits for this many elements, and takes a longer part in stretches (LONG).  Parts are that long only where rows of 300000 elements and
+// more have few counters, or none.
+constexpr int kStretch = 16384;
+__host__ __device__ constexpr int stretch(int elem) { return kStretch * elem / 16; }  // vectors
+__host__ __device__ constexpr int part_words(int per, int elem) { return hole_words(per < stretch(elem) ? per : stretch(elem), elem); }
 // What a row needs, by a warp each: the sums of its parts, and (part -1) the teacher's side, which takes as long as a part of 20 KB or so: latencies
 // and f64.  Each is left as a record, the teacher's in the first two; the last warp to come closes the row.  holes: zero before and after.
-template <typename T, bool TAIL>
+template <typename T, bool TAIL, bool LONG>
 __device__ __forceinline__ void distill_part(const Distill& p, long long row, int part, const Listed& lists, unsigned* holes, int words) {
   const int lane = threadIdx.x & 31;
   const bool whole = p.parts == 1;  // one warp does it all
-  const Range<T> r = range_of<T>(p, row, max(part, 0));
-  const Inner in(r);
-  const Row kind = look_at(p, row, [&](int id) {
-    if (TAIL && part >= 0 && in_range(r, id)) punch(r, in, id, holes, words);
-  });
+  Range<T> r = range_of<T>(p, row, max(part, 0));
+  const int end = r.v1;
+  if (LONG) r.v1 = min(end, r.v0 + stretch(sizeof(T)));
+  auto leave_out = [&](int id) {
+    if (TAIL && part >= 0 && in_range(r, id)) punch(r, Inner(r), id, holes, words);
+  };
+  const Row kind = look_at(p, row, leave_out);
   float4* records = p.records + row * (p.parts + 2);
   bool last = whole || part < 0, clean = false;
   if (kind != LIVE) {
@@ -1076,7 +1088,20 @@ __device__ __forceinline__ void distill_part(const Distill& p, long long row, in
     __syncwarp();
     float3 sum;
     Teacher t;
-    if (part >= 0) sum = sum_range<T, TAIL, false>(r, in, holes, words, p.c);
+    if constexpr (LONG) {
+      sum = make_float3(-INFINITY, 0.f, 0.f);
+      while (part >= 0) {
+        sum = join_two(sum, sum_range<T, TAIL, false>(r, Inner(r), holes, words, p.c), p.c);
+        if (r.v1 == end) break;
+        clear_holes(holes, words);
+        r.v0 = r.v1;
+        r.v1 = min(end, r.v0 + stretch(sizeof(T)));
+        (void)look_at(p, row, leave_out);
+        __syncwarp();
+      }
+    } else if (part >= 0) {
+      sum = sum_range<T, TAIL, false>(r, Inner(r), holes, words, p.c);
+    }
     if (whole || part < 0) {
       if (TAIL && whole) clear_holes(holes, words);
       clean = whole;
@@ -1109,12 +1134,12 @@ __device__ __forceinline__ void distill_part(const Distill& p, long long row, in
 }
 
 // The loss alone: rows cut among warps.
-template <typename T, bool TAIL>
+template <typename T, bool TAIL, bool LONG>
 __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __grid_constant__ Distill p) {
   extern __shared__ __align__(16) unsigned char store[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Listed lists(store, p.entries, threadIdx.x >> 5);
-  const int words = TAIL ? hole_words(p.per, sizeof(T)) : 0;
+  const int words = TAIL ? part_words(p.per, sizeof(T)) : 0;
   unsigned* holes = reinterpret_cast<unsigned*>(store) + lists_words(p.entries) + warp * words;
   for (int i = lane; i < words; i += 32) holes[i] = 0;
   grid_dependency_wait();
@@ -1123,7 +1148,7 @@ __global__ void __launch_bounds__(kThreads, kPlainPerSm) distill_kernel(const __
   const Items items(p, 1, each);
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item);
-    distill_part<T, TAIL>(p, row, (int)(item - row * each) - (each > 1), lists, holes, words);
+    distill_part<T, TAIL, LONG>(p, row, (int)(item - row * each) - (each > 1), lists, holes, words);
   }
   grid_dependency_launch();
 }
@@ -1494,33 +1519,32 @@ Distill rows_of(Distill p, int64_t first, int rows) {
   return p;
 }
 
-// Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element.
-template <auto KERNEL, typename T, typename P>
+// Launches a forward kernel whose warps cut the rows among them.  bits: dynamic shared memory for a bit per element; LONG: for parts that have more of
+// them than that has room for.
+template <auto KERNEL, auto LONG, typename T, typename P>
 int launch_items(ctb_ctx* ctx, cudaStream_t st, P p, bool bits, bool taught, double ends, const char* who) {
   const int64_t places = (int64_t)kPlainPerSm * ctx->sm_count * kWarps, nvec = vectors<T>(p);
   if (p.rows > kTickets && nvec >= 2048 && (bits || p.rows < 8 * places)) {  // rows that there are no counters for, and too few to go whole
     const int64_t launches = (p.rows + kTickets - 1) / kTickets, each = (p.rows + launches - 1) / launches;
     for (int64_t first = 0; first < p.rows; first += each)
-      if (int s = launch_items<KERNEL, T>(ctx, st, rows_of<T>(p, first, (int)std::min<int64_t>(each, p.rows - first)), bits, taught, ends, who)) return s;
+      if (int s = launch_items<KERNEL, LONG, T>(ctx, st, rows_of<T>(p, first, (int)std::min<int64_t>(each, p.rows - first)), bits, taught, ends, who)) return s;
     return CTB_OK;
   }
   size_t lists = 0;
   if constexpr (std::is_same<P, Distill>::value) lists = 4 * (size_t)lists_words(p.entries);
   auto go = [&] {
-    const size_t smem = lists + (bits ? (size_t)kWarps * 4 * hole_words(p.per, sizeof(T)) : 0);
+    const size_t smem = lists + (bits ? (size_t)kWarps * 4 * part_words(p.per, sizeof(T)) : 0);  // 41 KB at most
     int per_sm = kPlainPerSm;
     if (smem > 0) {
-      if (smem > kMostShared) return fail(CTB_UNSUPPORTED, "%s: with teacher_lse, %d rows of %d elements are too long", who, p.rows, p.n);
-      cudaError_t e = smem > 48 * 1024 ? allow_smem(KERNEL, kMostShared) : cudaSuccess;
-      if (e != cudaSuccess) return cuda_fail(e, who);
       per_sm = std::max(1, std::min(kPlainPerSm, (int)(kMostShared / (smem + 1024))));
     }
     const int64_t ctas = ((int64_t)p.rows * (p.parts + (taught && p.parts > 1)) + kWarps - 1) / kWarps;
-    launch_kernel(KERNEL, (int)std::min<int64_t>(ctas, (int64_t)per_sm * ctx->sm_count), kThreads, smem, st, 0, p);
+    const bool stretches = bits && p.per > stretch(sizeof(T));
+    launch_kernel(stretches ? LONG : KERNEL, (int)std::min<int64_t>(ctas, (int64_t)per_sm * ctx->sm_count), kThreads, smem, st, 0, p);
     CTB_CHECK_LAUNCH(who);
     return (int)CTB_OK;
   };
-  cut_among_warps(p, nvec, sizeof(T), places, bits ? p.n / 16384 + 1 : 1, most_parts(p, 1, taught ? 2 : 0), taught, ends);
+  cut_among_warps(p, nvec, sizeof(T), places, bits ? p.n / kStretch + 1 : 1, most_parts(p, 1, taught ? 2 : 0), taught, ends);
   if (p.parts > 1) {
     StreamScratch scratch(ctx, st);
     if (scratch.data) {
@@ -1572,7 +1596,7 @@ int launch_top(ctb_ctx* ctx, cudaStream_t st, Logprobs p, const char* who) {
 }
 template <typename T>
 int launch_logprobs(ctb_ctx* ctx, cudaStream_t st, const Logprobs& p, const char* who) {
-  return p.top ? launch_top<T>(ctx, st, p, who) : launch_items<logprobs_kernel<T>, T>(ctx, st, p, false, false, 3.0, who);
+  return p.top ? launch_top<T>(ctx, st, p, who) : launch_items<logprobs_kernel<T>, logprobs_kernel<T>, T>(ctx, st, p, false, false, 3.0, who);
 }
 template <typename T>
 int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) {
@@ -1584,8 +1608,8 @@ int launch_backward(ctb_ctx* ctx, cudaStream_t st, Backward p, const char* who) 
 }
 template <typename T>
 int launch_distill(ctb_ctx* ctx, cudaStream_t st, const Distill& p, const char* who) {
-  return p.teacher_lse ? launch_items<distill_kernel<T, true>, T>(ctx, st, p, true, true, 3.0, who)
-                       : launch_items<distill_kernel<T, false>, T>(ctx, st, p, false, true, 3.0, who);
+  return p.teacher_lse ? launch_items<distill_kernel<T, true, false>, distill_kernel<T, true, true>, T>(ctx, st, p, true, true, 3.0, who)
+                       : launch_items<distill_kernel<T, false, false>, distill_kernel<T, false, false>, T>(ctx, st, p, false, true, 3.0, who);
 }
 template <typename T>
 size_t both_shared(const Both& p) {

@@ -140,8 +140,7 @@ int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* 
 int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                     const void* teacher_values, int values_dtype, const float* saved, const float* d_loss, int64_t V, int64_t T,
                     int64_t ld_out, int64_t ld, int entries, float temperature, int dtype);
-/* Both in one call, for a d_loss that is known before the loss: rows of 32 to 512 KB are read from memory once.
- * (With teacher_lse, rows of millions of elements are CTB_UNSUPPORTED: a bit per element of a part lies in shared memory.) */
+/* Both in one call, for a d_loss that is known before the loss: rows of 32 to 512 KB are read from memory once. */
 int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                         const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
                         const float* d_loss, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature,

@@ -236,3 +236,27 @@ def test_gradient_of_a_part_of_a_vocabulary(cuda, shift):
     g0, gh = torch.randn(T, device="cuda"), torch.randn(T, device="cuda")
     want, tol = gradients(x.double(), tokens, None, g0, gh, None, 1.0)
     close_gradient(ops.token_logprobs_bwd(x[:, :cut], tokens, r.lse, r.entropy, g0, gh), want[:, :cut], tol[:, :cut] * 4)  # lse to 2^-15
+
+
+@pytest.mark.parametrize("V", [400003, 4000003])
+def test_long_rows_with_a_rest(cuda, V):
+    """As many rows as there are counters: parts are longer than a warp has bits for.  All rows but three are padding, which is not read."""
+    import torch
+    T, K, live = 4096, 40, [0, 1777, 4095]
+    x = torch.empty(T, V, device="cuda", dtype=torch.bfloat16)
+    x[live] = make(3, V, "bfloat16", seed=V)
+    some_ids, some_values, all_values = teacher(3, V, K, seed=1)
+    some_ids[1, 3:] = some_ids[1, :1]
+    ids, values = torch.zeros(T, K, device="cuda", dtype=torch.int32), torch.zeros(T, K, device="cuda")
+    ids[live], values[live] = some_ids, some_values
+    lse = torch.zeros(T, device="cuda")
+    lse[live] = torch.logsumexp(all_values, 1) + 1
+    g = torch.ones(T, device="cuda")
+    want_loss, want, tol = distillation(x[live], some_ids, some_values, lse[live], 1.0, g[live])
+    loss, saved = cuda.distill.distill_fwd(x, ids, values, lse)
+    close_loss(loss[live], want_loss)
+    assert loss.count_nonzero() == 3
+    cuda.distill.distill_bwd(x, ids, values, saved, g, out=x)
+    close_gradient(x[live], want, tol)
+    assert all(not x[r].any() for r in (1, 1776, 4094))
+    cuda.check_device_status(0)
