@@ -87,11 +87,12 @@ int fmha_decode(ctb_ctx* ctx, cudaStream_t st, const void* Q, const void* K, con
                 int64_t seq_kv, int64_t heads, int64_t kv_heads, int64_t batch, float qk_scale, int input_pos, int64_t keys, bool causal,
                 bool bf16, bool* taken);
 
-// The context's device is the current one while the object lives.
+// A device (the context's) is the current one while the object lives.
 class CurrentDevice {
  public:
-  explicit CurrentDevice(const ctb_ctx* ctx) {
-    if (cudaGetDevice(&before_) == cudaSuccess && before_ != ctx->device) cudaSetDevice(ctx->device);
+  explicit CurrentDevice(const ctb_ctx* ctx) : CurrentDevice(ctx->device) {}
+  explicit CurrentDevice(int device) {
+    if (cudaGetDevice(&before_) == cudaSuccess && before_ != device) cudaSetDevice(device);
     else before_ = -1;
   }
   ~CurrentDevice() {

@@ -826,12 +826,6 @@ struct Distill : Rows {
   Saved* saved;
 };
 
-__device__ __forceinline__ double sum_lanes(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // The teacher's side of a row, in f64: what its list leaves over is a difference from one.
 struct Teacher {
   double terms, all, norm;   // sum q (log q - (z - listed_max / temperature)), sum q; norm: see Saved
@@ -1448,7 +1442,7 @@ void cut_into(Rows& p, int64_t nvec, int64_t parts) {
   p.parts = (int)parts;
 }
 // Rows cut among warps: into the parts for which rounds of parts take the least time.  A warp reads `alone` bytes per ns when nobody else reads
-// and shares what HBM gives otherwise, a part costs `ends` besides and one more of a row 0.03 in the join (us); measured with 1 to 2220 rows of 50000 to 128000 elements.
+// and shares what HBM gives otherwise, a part costs `ends` besides and one more of a row 0.05 in the join (us); measured with 1 to 2220 rows of 50000 to 128000 elements.
 void cut_among_warps(Rows& p, int64_t nvec, int elem, int64_t places, int64_t least, int64_t most, int more,
                      double ends) {
   const double alone = elem == 4 ? 5.1 : 3.5, all = 7600, bytes = (double)nvec * 16e-3;  // of a row, in 1000
@@ -1616,13 +1610,13 @@ size_t both_shared(const Both& p) {
   const int per = (int)((vectors<T>(p) + kWarps - 1) / kWarps + 31) / 32 * 32;
   return 4 * ((size_t)lists_words(p.entries) / kWarps * (kWarps + 2) + (p.teacher_lse ? (size_t)hole_words(per, sizeof(T)) * (kWarps + 1) : 0));
 }
-// Loss and gradient at once, or one after the other?  In us, one after the other and at once: 4096 x 65536 bf16 298, 250; 1500 x 50001 f32 178, 151;
+// Loss and gradient at once, or one after the other?  sms: above 128 KB a row takes a CTA so long that each SM wants one.  In us, one after the other and at once: 4096 x 65536 bf16 298, 250; 1500 x 50001 f32 178, 151;
 // 8000 x 32000 bf16 318, 228.  Where the teacher's side takes longer than a row (20000 x 8000 bf16, with a rest: 305, 362), where the rows
 // under way do not stay in L2 (1024 x 128000 f32: 281, 278), and for few long rows, one after the other.
 template <typename T>
-bool at_once(const Both& p) {
+bool at_once(const Both& p, int sms) {
   const int64_t bytes = (int64_t)p.n * sizeof(T);
-  return bytes >= 32 * 1024 && bytes <= 512 * 1024 && (bytes <= 128 * 1024 || p.rows >= 148) && both_shared<T>(p) <= kMostShared / kBothPerSm - 2048;
+  return bytes >= 32 * 1024 && bytes <= 512 * 1024 && (bytes <= 128 * 1024 || p.rows >= sms) && both_shared<T>(p) <= kMostShared / kBothPerSm - 2048;
 }
 template <typename T>
 int launch_both(ctb_ctx* ctx, cudaStream_t st, Both p, const char* who) {
@@ -1748,7 +1742,7 @@ static int distill_forward(const char* who, ctb_ctx* ctx, void* stream, const vo
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   p.d_loss = d_loss; p.dx = d_logits; p.ld_dx = ld_out;
   return by_type(dtype, [&](auto t) {
-    if (both) *both = at_once<decltype(t)>(p);
+    if (both) *both = at_once<decltype(t)>(p, ctx->sm_count);
     return both && *both ? launch_both<decltype(t)>(ctx, st, p, who) : launch_distill<decltype(t)>(ctx, st, p, who);
   });
 }

@@ -45,12 +45,6 @@ struct Route {
   int lanes_a_group;  // a power of two where the lanes' chunks make up groups, else 0
 };
 
-__device__ __forceinline__ double sum_lanes(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 __device__ __forceinline__ void store_weight(void* p, long long i, int dtype, float v) {
   if (dtype == CTB_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == CTB_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
@@ -523,7 +517,7 @@ int check_route(const char* who, const void* logits, int64_t T, int64_t E, int64
   return CTB_OK;
 }
 
-template <typename T, typename F>
+template <typename F>
 void by_experts(int E, F f) {
   if (E <= 32) f(std::integral_constant<int, 1>());
   else if (E <= 64) f(std::integral_constant<int, 2>());
@@ -540,7 +534,7 @@ bool wide_rows(const void* p, long long ld, int experts, int epl, int elem) {
 template <typename T>
 int launch_route(ctb_ctx* ctx, cudaStream_t st, Route p) {
   const int grid = (int)std::min<int64_t>((p.tokens + kWarps - 1) / kWarps, 16ll * ctx->sm_count);
-  by_experts<T>(p.experts, [&](auto epl) {
+  by_experts(p.experts, [&](auto epl) {
     constexpr int kEach = decltype(epl)::value;
     const int size = p.experts / p.groups, lanes = size % kEach == 0 ? size / kEach : 0;
     p.lanes_a_group = (lanes & (lanes - 1)) == 0 ? lanes : 0;
@@ -554,7 +548,7 @@ int launch_route(ctb_ctx* ctx, cudaStream_t st, Route p) {
 template <typename T>
 int launch_route_backward(ctb_ctx* ctx, cudaStream_t st, RouteBackward p) {
   const int grid = (int)std::min<int64_t>((p.tokens + kWarps - 1) / kWarps, 16ll * ctx->sm_count);
-  by_experts<T>(p.experts, [&](auto epl) {
+  by_experts(p.experts, [&](auto epl) {
     constexpr int kEach = decltype(epl)::value;
     p.wide = wide_rows(p.x, p.ld, p.experts, kEach, sizeof(T)) && wide_rows(p.dx, p.ld_dx, p.experts, kEach, sizeof(T));
     launch_kernel(route_backward_kernel<T, kEach>, grid, kThreads, 0, st, 0, p);

@@ -78,6 +78,12 @@ __device__ __forceinline__ float word_max(uint32_t w) {
   }
 }
 
+__device__ __forceinline__ double sum_lanes(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Two f32 values in a 64-bit register, and operations that take one instruction for both.
 using Pair = unsigned long long;
 __device__ __forceinline__ Pair pair(float a, float b) {

@@ -43,16 +43,6 @@ struct RelaxedCapture {
   RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
   ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
-struct OnDevice {
-  int before = -1;
-  explicit OnDevice(int device) {
-    if (cudaGetDevice(&before) == cudaSuccess && before != device) cudaSetDevice(device);
-    else before = -1;
-  }
-  ~OnDevice() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
 
 }  // namespace
 
@@ -92,7 +82,7 @@ void scratch_pool_destroy(ScratchPool* p) {
 namespace {
 
 bool allocate(ScratchPool* p, ScratchSlot* s) {
-  OnDevice on(p->device);
+  CurrentDevice on(p->device);
   RelaxedCapture relaxed;
   constexpr size_t ticket_bytes = kTickets * sizeof(unsigned);
   cudaStream_t st = nullptr;

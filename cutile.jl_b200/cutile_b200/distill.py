@@ -61,8 +61,8 @@ def distill_bwd(logits, teacher_ids, teacher_values, saved, d_loss, temperature=
 
 
 def distill_fwd_bwd(logits, teacher_ids, teacher_values, d_loss, teacher_lse=None, temperature=1.0, out=None, **hints):
-    """Loss and gradient in one call, for a d_loss [T] f32 that is known beforehand (the rows' weights); rows of 32 to 512 KB are read once.
-    Returns (loss [T] f32, gradient [T, V]); `out` may be the logits."""
+    """Loss and gradient in one call, for a d_loss [T] f32 that is known beforehand (the rows' weights); rows of 32 to 128 KB, or
+    of up to 512 KB when there are many, are read once.  Returns (loss [T] f32, gradient [T, V]); `out` may be the logits."""
     if not hints:
         r = _host.distill_fwd_bwd(logits, teacher_ids, teacher_values, d_loss, teacher_lse, temperature, out)
         if r is not None:

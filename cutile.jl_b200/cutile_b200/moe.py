@@ -13,14 +13,6 @@ from . import _host, _lib
 from ._util import dense, dtype_code, gradient_of, handles, ids_bits, ptr, rows
 
 
-def _ids_bits(t):
-    if t.dtype == torch.int32:
-        return 32
-    if t.dtype == torch.int64:
-        return 64
-    raise _lib.CtbError(_lib.BAD_ARG, "expert ids must be int32 or int64")
-
-
 def moe_router(hidden_states, W_r, topk, return_logits=False):
     """Router of the benchmark configuration: returns (topk_weights [topk, T] f16, topk_ids [topk, T] int32)."""
     if not return_logits:
@@ -105,7 +97,7 @@ def moe_align_tile_size(topk_ids, tile_m, num_experts):
     tok = torch.empty(max(cap, 1) * tile_m, dtype=torch.int32, device=topk_ids.device)
     exp = torch.empty(max(cap, 1), dtype=torch.int32, device=topk_ids.device)
     nb = torch.zeros(1, dtype=torch.int32, device=topk_ids.device)
-    _lib.check(_lib.lib.ctb_moe_align(ctx, stream, ptr(topk_ids), _ids_bits(topk_ids), T, topk, num_experts,
+    _lib.check(_lib.lib.ctb_moe_align(ctx, stream, ptr(topk_ids), ids_bits(topk_ids, "expert ids"), T, topk, num_experts,
                                       int(tile_m), ptr(tok), ptr(exp), ptr(nb), cap))
     n = int(nb.item())
     _lib.check_device_status(topk_ids.device.index or 0, stream.value or 0)
@@ -165,7 +157,7 @@ def cutile_moe(hidden_states, w1, w2, topk_weights, topk_ids, tile_m, tile_n, ti
         raise _lib.CtbError(_lib.BAD_ARG, "cutile_moe: only Float16 is implemented")
     out = torch.empty((T, H), dtype=torch.float16, device=hidden_states.device)
     _lib.check(_lib.lib.ctb_moe_ffn(ctx, stream, ptr(hidden_states), ptr(w1), ptr(w2), ptr(topk_weights),
-                                    ptr(topk_ids), _ids_bits(topk_ids), ptr(out), T, H, I, E, topk, int(tile_m),
+                                    ptr(topk_ids), ids_bits(topk_ids, "expert ids"), ptr(out), T, H, I, E, topk, int(tile_m),
                                     int(tile_n), int(tile_k)))
     return out
 

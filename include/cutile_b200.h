@@ -107,15 +107,19 @@ int ctb_softmax(ctb_ctx* ctx, void* stream, void* output, const void* input, int
  *                  and 1-based ids, equal logits by ascending id; 0 <= top <= 32, top <= V.
  * logprobs comes with tokens; tokens, entropy and lse may be NULL.  A row whose token is 0 is padding: its logits are not
  * read and its results are 0.  A token outside of 0..V is a bad index (ctb_check_device_status) with log probability NaN.
- * Masked elements (-inf) have probability 0 and come last among the alternatives; a row that is masked as a whole, or
- * has NaN or +inf, has NaN results, and its top_ids (0..V) mean nothing.  Bitwise repeatable. */
+ * Masked elements (-inf) have probability 0 and come last among the alternatives.  A row that is masked as a whole, or
+ * has NaN or +inf, has NaN results (but an lse of -inf where all is masked), and its top_ids (0..V) mean nothing.
+ * lse, log probabilities and entropy are within 2^-17 + 2^-23 |result| of their exact values, whatever the magnitude of the
+ * logits; results beyond f32 are infinite.  Bitwise repeatable. */
 int ctb_token_logprobs(ctb_ctx* ctx, void* stream, const void* logits, const void* tokens, int token_bits, float* logprobs,
                        float* entropy, float* lse, float* top_logprobs, int32_t* top_ids, int64_t V, int64_t T, int64_t ld,
                        int top, float temperature, int dtype);
 /* Gradient: d_logits (V, T), row stride ld_out, in the type of logits, from the gradients d_logprobs (T), d_entropy (T) and
  * d_top_logprobs (top, T) of the results (each may be NULL) and the lse, entropy (with d_entropy) and top_ids (with
  * d_top_logprobs) of the forward call.  Padding rows and rows with a bad token get 0.  An id that occurs more than once
- * takes the sum.  d_logits may be the logits themselves, and must not overlap them in any other way. */
+ * takes the sum.  d_logits may be the logits themselves, and must not overlap them in any other way.  Probabilities in it are
+ * within 2^-16 of themselves (and 0 below 2^-126): where |lse| is above 128 (f32 logits) or 256, one f32 does not say that
+ * much, and the row is read twice.  lse and entropy may be those of more columns than the logits have. */
 int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* tokens, int token_bits,
                            const float* lse, const float* entropy, const float* d_logprobs, const float* d_entropy,
                            const int32_t* top_ids, const float* d_top_logprobs, int64_t V, int64_t T, int64_t ld_out,
@@ -132,7 +136,8 @@ int ctb_token_logprobs_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const voi
  *                     loss = sum_j q_j (log q_j - log p[id_j]) + q_r (log q_r - log p_r)
  * loss (T) f32; saved (8, T) f32, 16-byte aligned, is what the gradient needs.  An id may occur more than once.  A row without a
  * used entry is padding: its logits are not read, loss and gradient are 0.  An id outside of 0..V is a bad index
- * (ctb_check_device_status): the row's loss is NaN and its gradient 0. */
+ * (ctb_check_device_status): the row's loss is NaN and its gradient 0.  Where the student masks (-inf) an id with q_j > 0, or
+ * all that is not listed with q_r > 0, the loss is +inf; the gradient has p = 0 there. */
 int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* teacher_ids, int id_bits,
                     const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved, int64_t V,
                     int64_t T, int64_t ld, int entries, float temperature, int dtype);
@@ -140,7 +145,9 @@ int ctb_distill_fwd(ctb_ctx* ctx, void* stream, const void* logits, const void* 
 int ctb_distill_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                     const void* teacher_values, int values_dtype, const float* saved, const float* d_loss, int64_t V, int64_t T,
                     int64_t ld_out, int64_t ld, int entries, float temperature, int dtype);
-/* Both in one call, for a d_loss that is known before the loss: rows of 32 to 512 KB are read from memory once. */
+/* Both in one call, for a d_loss that is known before the loss.  Rows of 32 to 128 KB, and from as many rows on as there are SMs
+ * of up to 512 KB, are read from memory once (not so with long lists and a rest in the longest of them: their bits need
+ * the room); others as by the two calls. */
 int ctb_distill_fwd_bwd(ctb_ctx* ctx, void* stream, void* d_logits, const void* logits, const void* teacher_ids, int id_bits,
                         const void* teacher_values, int values_dtype, const float* teacher_lse, float* loss, float* saved,
                         const float* d_loss, int64_t V, int64_t T, int64_t ld_out, int64_t ld, int entries, float temperature,
