@@ -443,22 +443,22 @@ __device__ __forceinline__ void mask_holes(uint4& q, unsigned bits) {
   }
 }
 
-// Calls f(q, v) for a thread's vectors, four at a time; v: the tile's first one.  What is left over comes one vector at a time, in
+// Calls f(q, v) for a thread's vectors, UNROLL at a time; v: the tile's first one.  What is left over comes one vector at a time, in
 // the warps that have some of it; lanes beyond the end get -inf.  Lanes that took a rare branch in f would go on by
 // themselves up to the next shuffle, behind the row: they meet before every tile (2220 x 100000 bf16: 110 -> 82 us).  W warps stream the row.  KEEP: it is read again,
 // from L2.
-template <typename T, int W, bool KEEP = false, typename F>
+template <typename T, int W, bool KEEP = false, int UNROLL = kUnroll, typename F>
 __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F f) {
   constexpr int kWide = W * 32;
   const int tid = threadIdx.x % kWide;
   const uint4* p = r.at(in.a) + tid;
   int v = in.a;
 #pragma unroll 1
-  for (; v + kWide * kUnroll <= in.b; v += kWide * kUnroll, p += kWide * kUnroll) {
+  for (; v + kWide * UNROLL <= in.b; v += kWide * UNROLL, p += kWide * UNROLL) {
     __syncwarp();
-    uint4 q[kUnroll];
+    uint4 q[UNROLL];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = KEEP ? __ldcg(p + u * kWide) : __ldcs(p + u * kWide);
+    for (int u = 0; u < UNROLL; ++u) q[u] = KEEP ? __ldcg(p + u * kWide) : __ldcs(p + u * kWide);
     f(q, v);
   }
 #pragma unroll 1
@@ -727,13 +727,13 @@ __global__ void __launch_bounds__(kThreads, kTopPerSm) top_logprobs_kernel(const
 // ------------------------------------------------------------------ gradients
 // d = e (a + b t), e = 2^t, over a range, by W warps.  t = (x - base) c with APART, which keeps its digits whatever the magnitude of x (and
 // costs a loop that HBM bounds nothing: 4096 x 65536 bf16 240.5 us for 240.4), else x c - base.
-template <typename T, bool ENTROPY, bool APART, int W>
+template <typename T, bool ENTROPY, bool APART, int W, int UNROLL = kUnroll>
 __device__ __forceinline__ void stream_gradient(const Range<T>& r, const Inner& in, T* dst, float c, float base, float a, float b) {
   const int tid = threadIdx.x % (W * 32), edge = edge_index(r, in, tid);
   const bool aligned = ((uintptr_t)(dst - r.off) & 15) == 0;
   const Pair cc = pair(c, c), minus = pair(-base, -base), aa = pair(a, a), bb = pair(b, b);
   const float x = edge >= 0 ? to_float(r.src[edge]) : 0.f;
-  each_tile<T, W>(r, in, [&](auto& q, int v) {
+  each_tile<T, W, false, UNROLL>(r, in, [&](auto& q, int v) {
     constexpr int N = sizeof(q) / sizeof(uint4);
     uint4* to = reinterpret_cast<uint4*>(dst - r.off) + v + tid;
 #pragma unroll
@@ -1317,8 +1317,9 @@ __device__ __forceinline__ int meet(const Backward& p, long long row, long long 
 template <typename T>
 __device__ __forceinline__ bool lse_will_do(float lse) { return fabsf(lse) <= (sizeof(T) == 4 ? 128.f : 256.f); }
 // The other rows (large logits, small temperatures, rows masked by a number): a CTA takes one as a whole, for what it writes over others may not
-// read, and reads it twice, first for its maximum and sum.  Logits around 1000: 2048 x 100003 bf16 221 us (157 around 0), 512 x 50001 f32 59
-// (41), 64 x 128000 bf16 33 (11).
+// read, and reads it twice, first for its maximum and sum.  Logits around 1000: 2048 x 100003 bf16 219 us (156 around 0), 512 x 50001 f32 60
+// (40), 64 x 128000 bf16 38 (10).
+constexpr int kWholeUnroll = 2;
 template <typename T, bool ENTROPY>
 __device__ __forceinline__ void whole_row_gradient(const Backward& p, long long row, long long token, Meeting& m) {
   __shared__ float red[3][kWarps];
@@ -1330,7 +1331,7 @@ __device__ __forceinline__ void whole_row_gradient(const Backward& p, long long 
   float all;
   const int entries = meet(p, row, token, r, m, all), edge = edge_index(r, in, threadIdx.x);
   Sums<T, false> sums;
-  each_tile<T, kWarps, true>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
+  each_tile<T, kWarps, true, kWholeUnroll>(r, in, [&](auto& q, int) { (void)sums.add(q, p.c); });
   if (edge >= 0) sums.add_one(to_float(r.src[edge]), p.c);
   __syncwarp();
   const float3 of_warp = sums.over_warp(p.c);
@@ -1348,15 +1349,16 @@ __device__ __forceinline__ void whole_row_gradient(const Backward& p, long long 
   const float gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
   const float b = -gh * kLn2 / p.temperature * per;
   const float a = -(all + gh * h) / p.temperature * per + (ENTROPY ? b * log2f(per) : 0.f);
-  stream_gradient<T, ENTROPY, true, kWarps>(r, in, dst, p.c, sum.x, a, b);
+  stream_gradient<T, ENTROPY, true, kWarps, kWholeUnroll>(r, in, dst, p.c, sum.x, a, b);
   patch_entries<kWarps>(r, in, m.entry, m.weight, entries, [&](int id, int j, float direct) {
     const float t = (m.x[j] - sum.x) * p.c, e = ex2_approx_ftz(t);
     dst[id - 1] = from_float<T>(direct / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
   });
 }
-// A call behind the loop over the other rows: in line, or within that loop, it takes registers that they need.
+// Behind the loop over the other rows, and two vectors at a time: as a call, in that loop, or four vectors at a time it slows the other rows down
+// (2048 x 100003 bf16, forward and gradient 228.5 us; as a call 232).
 template <typename T, bool ENTROPY>
-__device__ __noinline__ void whole_rows_gradient(const Backward& p, Meeting* lists) {
+__device__ __forceinline__ void whole_rows_gradient(const Backward& p, Meeting* lists) {
   const Items items(p, kWarps);
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item), token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
