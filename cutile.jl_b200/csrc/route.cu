@@ -442,34 +442,34 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
       ej = expf(xj - most);
     }
     if (!id) ej = 0.f;
-    float factor = p.scale, chosen = 0.f, mean = 0.f, all_low = 0.f, mean_low = 0.f;  // mean: C
-    bool apart = !p.sigmoid;  // from dw S - C, once what meets at an expert is added up
-    if (p.renormalize || !p.sigmoid) {
-      float of = 0.f;  // what dw is relative to
-      if (p.renormalize) {
-        const uint32_t bits = __float_as_uint(ej), top = __reduce_max_sync(0xffffffffu, bits);
-        of = __shfl_sync(0xffffffffu, dw, __ffs(__ballot_sync(0xffffffffu, bits == top)) - 1);
-      }
-      Pair sums = pair(ej, (id ? dw - of : 0.f) * ej);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sums = add2(sums, __shfl_xor_sync(0xffffffffu, sums, o));
-      chosen = halves(sums).x;
-      mean = halves(sums).y;
-      if (p.renormalize && !(chosen < 1e-20f * all)) {
+    float factor = p.scale, mean = 0.f, all_low = 0.f, mean_low = 0.f;  // mean: C
+    bool apart = !p.sigmoid, exact = false;  // apart: from dw S - C, once what meets at an expert is added up
+    if (p.renormalize) {
+      const uint32_t bits = __float_as_uint(ej), top = __reduce_max_sync(0xffffffffu, bits);
+      const float of = __shfl_sync(0xffffffffu, dw, __ffs(__ballot_sync(0xffffffffu, bits == top)) - 1);
+      const float chosen = warp_sum(ej);
+      mean = warp_sum((id ? dw - of : 0.f) * ej);
+      if (chosen < 1e-20f * all) {
+        factor *= 1e20f;
+        mean = fmaf(of, chosen, mean);
+      } else {
         apart = false;
         const float per = 1.f / chosen;
         dw = id ? fmaf(dw - of, chosen, -mean) * per : 0.f;
         factor *= per;
-      } else if (p.renormalize) {
-        factor *= 1e20f;
-        mean = fmaf(of, chosen, mean);
-      } else if (chosen > 0.875f * all) {
-        double a = 0, b = (double)dw * (double)ej;
+      }
+    } else if (!p.sigmoid) {
+      const unsigned chosen = __reduce_add_sync(0xffffffffu, (unsigned)(ej * 0x1p24f));  // near enough
+      exact = (float)chosen > 0.875f * 0x1p24f * all;
+      if (!exact) {
+        mean = warp_sum(dw * ej);
+      } else {
+        double a = 0;
 #pragma unroll
         for (int i = 0; i < EPL; ++i)
           if (first + i < p.experts) a += (double)s[i];
         a = sum_lanes(a);
-        b = sum_lanes(b);
+        const double b = sum_lanes((double)dw * (double)ej);
         all = (float)a;
         all_low = (float)(a - (double)all);
         mean = (float)b;
@@ -489,8 +489,8 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteBac
     if (apart) {
       const float per = 1.f / all;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) d[i] = (fmaf(d[i], all, -mean) + fmaf(d[i], all_low, -mean_low)) * per;
-      factor *= per;
+      for (int i = 0; i < EPL; ++i) d[i] = fmaf(d[i], all, -mean) + (exact ? fmaf(d[i], all_low, -mean_low) : 0.f);
+      factor *= per * per;
     }
 #pragma unroll
     for (int i = 0; i < EPL; ++i) d[i] *= factor * s[i];
