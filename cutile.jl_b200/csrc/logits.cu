@@ -248,7 +248,7 @@ struct Sums {
   // What the rounding of m2 has added to the exponents.
   static __device__ __forceinline__ float added(float ref, float m2, float c) { return far(m2) ? 0.f : fmaf(ref, c, -m2); }
   __device__ __forceinline__ void move(float x, float c) {
-    const float to = x * c;
+    const float to = __fmul_rn(x, c);  // rounded: as part of a fused m2 - x c it would not be what m2 becomes
     const float apart = far(to) || far() ? (ref - x) * c - added(ref, m2, c) + added(x, to, c) : m2 - to;
     const float d = fmaxf(fminf(apart, 0.f), kLowest), r = ex2_approx_ftz(d);  // s = w = 0 until there is a reference
     const Pair rr = pair(r, r);

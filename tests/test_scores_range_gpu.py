@@ -74,6 +74,23 @@ def test_large_logits(cuda, T, V, dtype):
     cuda.check_device_status(0)
 
 
+@pytest.mark.parametrize("shift", [3e3, -2e4, 1e5, 3e5, -6e5, 7e5, 1e6])
+def test_shifted_rows_whose_maximum_rises(cuda, shift):
+    """A thread's sums follow its maximum: what they are relative to is off by the rounding of a large product, and must be so throughout."""
+    import torch
+    for T, V in ((24, 39812), (700, 12001)):
+        x = make(T, V, "float32", seed=5, scale=3.0) + shift
+        x[::3] = x[::3].sort(dim=1).values
+        tokens = torch.argmax(x, 1) + 1
+        check(cuda, x, tokens, 0)
+        check(cuda, x, tokens, 7)
+        ids = torch.topk(x, 20, 1).indices.int() + 1
+        values = torch.zeros(T, 20, device="cuda")
+        for lse in (None, torch.full((T,), 4.0, device="cuda")):
+            want = distillation(x, ids, values, lse, 1.0, tokens.float())[0]
+            close_loss(cuda.distill.distill_fwd(x, ids, values, lse)[0], want)
+
+
 def distillation(x, ids, values, lse, temperature, d_loss):
     """(loss, gradient, tolerance of the gradient) in f64; what the teacher's list leaves over by logarithms."""
     import torch
@@ -94,9 +111,11 @@ def distillation(x, ids, values, lse, temperature, d_loss):
         listed = torch.zeros_like(p).scatter_add_(1, at, used.double()) > 0
         left = (1 - q.sum(1, keepdim=True)).clamp(min=0)
         whole = q.sum(1, keepdim=True) + left
-        log_rest = torch.logsumexp(log_p.masked_fill(listed, -float("inf")), 1, keepdim=True)
+        others = z.masked_fill(listed, -float("inf"))
+        most = others.amax(1, keepdim=True)  # apart from the sum, which f64 would lose beside 1e38 as well
+        log_rest = (most - z.amax(1, keepdim=True)) + (others - most).exp().sum(1, keepdim=True).log() - (z - z.amax(1, keepdim=True)).exp().sum(1, keepdim=True).log()
         loss = loss + (torch.xlogy(left, left) - torch.where(left > 0, left * log_rest, 0.0))[:, 0]
-        rest = torch.where(listed, 0.0, left * (log_p - log_rest).exp())
+        rest = left * torch.softmax(others, 1).nan_to_num(0.0)
     d = g * (whole * p - rest - qv)
     # see test_distill_gpu.py; and a power below 2^-126 counts as 0, of which the gradient takes at most g whole
     tol = g.abs() * (2.0 ** -16 * (whole * p + rest) + 2.0 ** -22 * qv + 2.0 ** -125 * whole)
