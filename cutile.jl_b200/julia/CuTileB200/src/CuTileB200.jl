@@ -206,27 +206,32 @@ function moe_route_bwd(logits::CuArray{X,2}, topk_ids::CuArray, d_weights::CuArr
 end
 
 # ---- log probabilities and distillation (no example in the reference) -------
-"Log probabilities of `tokens` (1-based, 0: padding) under softmax(logits ./ temperature), logits (V, T): a named tuple."
-function token_logprobs(logits::CuArray{X,2}, tokens::CuArray; top::Int=0, temperature::Real=1) where {X}
+or_null(a) = a === nothing ? C_NULL : dptr(a)
+"Log probabilities of `tokens` (1-based, 0: padding; or none) under softmax(logits ./ temperature), logits (V, T): a named tuple."
+function token_logprobs(logits::CuArray{X,2}, tokens::Union{CuArray,Nothing}=nothing; top::Int=0, temperature::Real=1) where {X}
     V, T = size(logits)
-    logprobs = CuArray{Float32}(undef, T); entropy = similar(logprobs); lse = similar(logprobs)
+    entropy = CuArray{Float32}(undef, T); lse = similar(entropy); logprobs = tokens === nothing ? nothing : similar(entropy)
     top_logprobs = CuArray{Float32}(undef, top, T); top_ids = CuArray{Int32}(undef, top, T)
     check(ccall((:ctb_token_logprobs, LIB), Cint,
         (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64,
          Int64, Cint, Cfloat, Cint),
-        context(), stream(), dptr(logits), dptr(tokens), ids_bits(tokens), dptr(logprobs), dptr(entropy), dptr(lse),
-        top == 0 ? C_NULL : dptr(top_logprobs), top == 0 ? C_NULL : dptr(top_ids), V, T, stride(logits, 2), top, temperature, dtype(X)))
+        context(), stream(), dptr(logits), or_null(tokens), tokens === nothing ? 64 : ids_bits(tokens), or_null(logprobs), dptr(entropy),
+        dptr(lse), top == 0 ? C_NULL : dptr(top_logprobs), top == 0 ? C_NULL : dptr(top_ids), V, T, stride(logits, 2), top, temperature,
+        dtype(X)))
     return (; logprobs, entropy, lse, top_logprobs, top_ids)
 end
 
-"Gradient of the logits from those of log probabilities and entropies."
-function token_logprobs_bwd(logits::CuArray{X,2}, tokens::CuArray, lse, entropy, d_logprobs, d_entropy; temperature::Real=1) where {X}
+"Gradient of the logits from those of log probabilities, entropies (either may be nothing) and alternatives."
+function token_logprobs_bwd(logits::CuArray{X,2}, tokens::Union{CuArray,Nothing}, lse, entropy, d_logprobs, d_entropy; top_ids=nothing,
+                            d_top_logprobs=nothing, temperature::Real=1) where {X}
     V, T = size(logits); d = similar(logits)
+    top = d_top_logprobs === nothing ? 0 : size(d_top_logprobs, 1)
     check(ccall((:ctb_token_logprobs_bwd, LIB), Cint,
         (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
          Ptr{Cvoid}, Int64, Int64, Int64, Int64, Cint, Cfloat, Cint),
-        context(), stream(), dptr(d), dptr(logits), dptr(tokens), ids_bits(tokens), dptr(lse), dptr(entropy), dptr(d_logprobs),
-        d_entropy === nothing ? C_NULL : dptr(d_entropy), C_NULL, C_NULL, V, T, stride(d, 2), stride(logits, 2), 0, temperature, dtype(X)))
+        context(), stream(), dptr(d), dptr(logits), or_null(tokens), tokens === nothing ? 64 : ids_bits(tokens), dptr(lse), or_null(entropy),
+        or_null(d_logprobs), or_null(d_entropy), or_null(top_ids), or_null(d_top_logprobs), V, T, stride(d, 2), stride(logits, 2), top,
+        temperature, dtype(X)))
     return d
 end
 
