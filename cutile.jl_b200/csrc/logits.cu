@@ -474,7 +474,7 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
 // Where nothing but sums has to meet, a warp takes a part of a row (2 KB with few rows, 30 to 130 KB with thousands) after another, without a barrier and without a thought for the
 // other warps of its CTA: (maximum, s, w) go to a record in scratch memory, and the warp that finishes a row's last part joins the
 // records in their order and writes the results.  48 such warps on an SM keep 16-bit logits, whose exponentials keep the ex2 unit
-// busy 55 % of the time, as close to HBM's rate as a loop without rows (2048 x 100003 bf16 78 us, 0.80 of the copy rate; 512 x 50001 f32 24.8); eight warps that meet at the end of every row left them at 78 %.
+// busy 55 % of the time, as close to HBM's rate as a loop without rows (2048 x 100003 bf16 81 us, 0.77 of the copy rate; 512 x 50001 f32 24.8); eight warps that meet at the end of every row left them at 78 %.
 constexpr int kMaxParts = 256;
 struct Items {  // of a warp (or, with W = 8, of the warps of a CTA, which share a part's tiles)
   const Rows& p;

@@ -109,7 +109,7 @@ int ctb_softmax(ctb_ctx* ctx, void* stream, void* output, const void* input, int
  * read and its results are 0.  A token outside of 0..V is a bad index (ctb_check_device_status) with log probability NaN.
  * Masked elements (-inf) have probability 0 and come last among the alternatives.  A row that is masked as a whole, or
  * has NaN or +inf, has NaN results (but an lse of -inf where all is masked), and its top_ids (0..V) mean nothing.
- * lse, log probabilities and entropy are within 2^-17 + 2^-23 |result| of their exact values, whatever the magnitude of the
+ * lse, log probabilities and entropy are within 2^-17 + 2^-22 |result| of their exact values, whatever the magnitude of the
  * logits; results beyond f32 are infinite.  Bitwise repeatable. */
 int ctb_token_logprobs(ctb_ctx* ctx, void* stream, const void* logits, const void* tokens, int token_bits, float* logprobs,
                        float* entropy, float* lse, float* top_logprobs, int32_t* top_ids, int64_t V, int64_t T, int64_t ld,
