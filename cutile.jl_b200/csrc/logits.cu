@@ -1016,7 +1016,7 @@ struct Backward : Rows {
 
 // Gradient of the log probabilities, the entropy and the alternatives of a row:
 //   dx_v = 1/temperature [ sum of the gradients that meet at v - p_v (G + g_H (log p_v + H)) ],  G = the sum of all but g_H
-// and of the distillation loss (DISTILL): g/temperature p_v outside, or g/temperature (whole p_v - q_v) where the teacher lists v.
+// and of the distillation loss: see Saved.
 // A CTA takes a part of a row after another; its warps share the tiles, so that 16 KB are read and written side by side (parts of a warp's
 // own left HBM at 85 %), but do not wait for each other: each has the few places in its tiles that a gradient meets directly, and writes
 // them behind its stream.  What a warp needs of a row the others need as well, and each loads it.
@@ -1355,6 +1355,7 @@ __device__ __forceinline__ void whole_row_gradient(const Backward& p, long long 
     dst[id - 1] = from_float<T>(direct / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
   });
 }
+// The warps of a CTA agree on the rows by votes, whatever each has read.
 // Behind the loop over the other rows, and two vectors at a time: as a call, in that loop, or four vectors at a time it slows the other rows down
 // (2048 x 100003 bf16, forward and gradient 228.5 us; as a call 232).
 template <typename T, bool ENTROPY>
@@ -1362,7 +1363,8 @@ __device__ __forceinline__ void whole_rows_gradient(const Backward& p, Meeting* 
   const Items items(p, kWarps);
   for (long long item = items.at; item < items.end; item += items.step) {
     const long long row = items.row(item), token = p.tokens ? load_id(p.tokens, row, p.token_bits) : -1;
-    if (item != row * p.parts || token == 0 || (p.tokens && (token < 0 || token > p.n)) || lse_will_do<T>(p.lse[row])) continue;
+    const bool skip = item != row * p.parts || token == 0 || (p.tokens && (token < 0 || token > p.n)) || lse_will_do<T>(p.lse[row]);
+    if (!__syncthreads_or(!skip)) continue;
     whole_row_gradient<T, ENTROPY>(p, row, token, lists[threadIdx.x >> 5]);
   }
 }
@@ -1395,7 +1397,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
     const int entries = meet(p, row, token, r, m, all);
     const float gh = ENTROPY ? p.d_entropy[row] : 0.f, h = ENTROPY ? p.entropy[row] : 0.f;
     // log2 p = t - lost: lse in units of c as it is, and what its f32 loses goes into a and b
-    const float base = lse * p.lse_c, lost = fmaf(lse, p.lse_c, -base) + lse * p.lse_c_low, more = ex2_approx_ftz(-lost);
+    const float base = __fmul_rn(lse, p.lse_c), lost = fmaf(lse, p.lse_c, -base) + lse * p.lse_c_low, more = ex2_approx_ftz(-lost);
     const float b = -gh * kLn2 / p.temperature * more, a = -(all + gh * h) / p.temperature * more - b * lost;
     stream_gradient<T, ENTROPY, false, kWarps>(r, in, dst, p.c, base, a, b);
     patch_entries<kWarps>(r, in, m.entry, m.weight, entries, [&](int id, int j, float direct) {
@@ -1403,9 +1405,9 @@ __global__ void __launch_bounds__(kThreads, kBackwardPerSm) logits_backward_kern
       dst[id - 1] = from_float<T>(direct / p.temperature + e * fmaf(b, fmaxf(t, kLowest), a));
     });
   }
-  __syncwarp();
-  if (m.others) whole_rows_gradient<T, ENTROPY>(p, lists);  // all warps of a CTA have found the same
   grid_dependency_launch();
+  __syncwarp();
+  if (__syncthreads_or(m.others)) whole_rows_gradient<T, ENTROPY>(p, lists);
 }
 
 // ------------------------------------------------------------------ host side
