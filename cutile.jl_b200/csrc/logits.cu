@@ -249,7 +249,7 @@ struct Sums {
   static __device__ __forceinline__ float added(float ref, float m2, float c) { return far(m2) ? 0.f : fmaf(ref, c, -m2); }
   __device__ __forceinline__ void move(float x, float c) {
     const float to = __fmul_rn(x, c);  // rounded: as part of a fused m2 - x c it would not be what m2 becomes
-    const float apart = far(to) || far() ? (ref - x) * c - added(ref, m2, c) + added(x, to, c) : m2 - to;
+    const float apart = (ref - x) * c - added(ref, m2, c) + added(x, to, c);  // m2 - to, but for what is far
     const float d = fmaxf(fminf(apart, 0.f), kLowest), r = ex2_approx_ftz(d);  // s = w = 0 until there is a reference
     const Pair rr = pair(r, r);
     if constexpr (ENTROPY) w = mul2(rr, fma2(s, pair(d, d), w));
@@ -319,7 +319,7 @@ struct Sums {
   // The warp's (maximum, s, w), the sums relative to that maximum.
   __device__ __forceinline__ float3 over_warp(float c) const {
     const float most = warp_max(word_max<T>(top));
-    float d = far() || far(most * c) ? (ref - most) * c - added(ref, m2, c) : fmaf(-most, c, m2);
+    float d = (ref - most) * c - added(ref, m2, c);
     if (limit == -INFINITY) d = 0.f;  // nothing but masked elements, or NaN: its sums are 0, or NaN
     const float r = ex2_approx_ftz(d), sum = sum_of(s);
     return make_float3(most, warp_sum(sum * r), ENTROPY ? warp_sum(r * fmaf(sum, fmaxf(d, kLowest), sum_of(w))) : 0.f);
@@ -474,7 +474,7 @@ __device__ __forceinline__ void each_tile(const Range<T>& r, const Inner& in, F 
 // Where nothing but sums has to meet, a warp takes a part of a row (2 KB with few rows, 30 to 130 KB with thousands) after another, without a barrier and without a thought for the
 // other warps of its CTA: (maximum, s, w) go to a record in scratch memory, and the warp that finishes a row's last part joins the
 // records in their order and writes the results.  48 such warps on an SM keep 16-bit logits, whose exponentials keep the ex2 unit
-// busy 55 % of the time, as close to HBM's rate as a loop without rows (2048 x 100003 bf16 81 us, 0.77 of the copy rate; 512 x 50001 f32 24.8); eight warps that meet at the end of every row left them at 78 %.
+// busy 55 % of the time, as close to HBM's rate as a loop without rows (2048 x 100003 bf16 80 us, 0.78 of the copy rate; 512 x 50001 f32 24.8); eight warps that meet at the end of every row left them at 78 %.
 constexpr int kMaxParts = 256;
 struct Items {  // of a warp (or, with W = 8, of the warps of a CTA, which share a part's tiles)
   const Rows& p;
