@@ -56,7 +56,8 @@ size_t moe_ffn_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top
 int moe_check_tile(const char* who, int tile_m, int tile_n, int tile_k);
 constexpr int kSchedSlots = 256;
 constexpr int kTickets = 4096;
-constexpr size_t kStreamScratchBytes = 1280 * 1024;
+constexpr size_t kStreamScratchBytes = 1280 * 1024;  // what the sizes of parts go by, but for those of ctb_fmha_paged
+constexpr size_t kSlotBytes = 2560 * 1024;           // what there is
 // Scratch of a launch whose last CTA adds up the parts that the others leave, and its arrival counters (zero between
 // launches: they are counted by atomicInc, which wraps at the last arrival).  No other launch that may run at the same time has
 // it, captured ones included (scratch.cu).  The object lives until the kernel is launched.  data is null when none can be
@@ -67,7 +68,7 @@ class StreamScratch {
   ~StreamScratch();
   StreamScratch(const StreamScratch&) = delete;
   StreamScratch& operator=(const StreamScratch&) = delete;
-  float* data = nullptr;        // kStreamScratchBytes
+  float* data = nullptr;        // kSlotBytes
   unsigned* tickets = nullptr;  // kTickets
 
  private:
@@ -108,6 +109,12 @@ class CurrentDevice {
 // A gradient of `rows` rows of n elements may be written over the rows that it is made from, row for row, but not across them.
 int check_in_place(const char* who, const void* in, int64_t ld_in, const void* out, int64_t ld_out, int64_t n, int64_t rows,
                    int64_t elem_size);
+
+// The same for rows of D elements in three strides (rope.cu).
+int check_turned_in_place(const char* who, const void* in, const int64_t* in_strides, const void* out, const int64_t* out_strides,
+                          const int64_t* extents, int64_t D, int64_t elem_size);
+// A paged cache is well formed (kvcache.cu).
+int check_kv_cache(const char* who, const ctb_kv_cache* cache);
 
 // cuTensorMapEncodeTiled, resolved through the runtime so that the library has
 // no link-time dependency on libcuda and loads on machines without a driver.

@@ -314,6 +314,208 @@ PyObject* fmha(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(made));
 }
 
+// Three strides of [batch, seq, heads, D], or of [tokens, heads, D] as one batch.
+bool token_strides(const Tensor& t, int64_t* s) {
+  const int64_t n = t.dim();
+  if ((n != 3 && n != 4) || t.stride(n - 1) != 1) return false;
+  s[0] = n == 4 ? t.stride(0) : 0;
+  s[1] = t.stride(n - 3);
+  s[2] = t.stride(n - 2);
+  return true;
+}
+int index_bits(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : t.scalar_type() == at::kLong ? 64 : 0; }
+bool frequencies_of(const Tensor* f, const Tensor& like) {
+  return f && f->scalar_type() == at::kDouble && f->dim() == 1 && f->is_contiguous() && f->device() == like.device();
+}
+// A result where one is given, else a new array with the strides of its input.
+const Tensor* result_like(PyObject* given, const Tensor& x, Tensor* made) {
+  if (given == Py_None) {
+    *made = at::empty_like(x);
+    return made;
+  }
+  const Tensor* out = cuda_tensor(given);
+  return out && out->device() == x.device() && out->scalar_type() == x.scalar_type() && out->sizes() == x.sizes() ? out : nullptr;
+}
+PyObject* given_or(PyObject* given, Tensor& made) { return given != Py_None ? Py_NewRef(given) : THPVariable_Wrap(std::move(made)); }
+
+// rope(q, k or None, positions, frequencies, interleaved, scale, out_q or None, out_k or None, inverse) -> (out_q, out_k or None)
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9) return decline();
+  const Tensor *q = cuda_tensor(a[0]), *k = a[1] == Py_None ? nullptr : cuda_tensor(a[1]), *pos = cuda_tensor(a[2]), *f = cuda_tensor(a[3]);
+  float scale;
+  int64_t s[12] = {};
+  if (!q || (!k && a[1] != Py_None) || !pos || !PyBool_Check(a[4]) || !as_float(a[5], &scale) || !PyBool_Check(a[8]) || dtype_of(*q) < 0 ||
+      !token_strides(*q, s + 3) || !frequencies_of(f, *q) || pos->device() != q->device() || !pos->is_contiguous() || !index_bits(*pos))
+    return decline();
+  const int64_t d = q->dim();
+  if (pos->dim() != d - 2 || pos->sizes() != q->sizes().slice(0, d - 2)) return decline();
+  if (k && (k->device() != q->device() || k->scalar_type() != q->scalar_type() || k->dim() != d || k->size(d - 1) != q->size(d - 1) ||
+            k->sizes().slice(0, d - 2) != q->sizes().slice(0, d - 2) || !token_strides(*k, s + 9)))
+    return decline();
+  Call c(*q);
+  if (!c.ok()) return nullptr;
+  Tensor made[2];
+  const Tensor* out[2] = {result_like(a[6], *q, &made[0]), nullptr};
+  if (!out[0] || !token_strides(*out[0], s)) return decline();
+  if (k && (!(out[1] = result_like(a[7], *k, &made[1])) || !token_strides(*out[1], s + 6))) return decline();
+  const int r = without_gil([&] {
+    return ctb_rope(c.ctx, c.stream, out[0]->data_ptr(), q->data_ptr(), k ? out[1]->data_ptr() : nullptr, k ? k->data_ptr() : nullptr,
+                    pos->data_ptr(), index_bits(*pos), static_cast<const double*>(f->data_ptr()), d == 4 ? q->size(0) : 1, q->size(d - 3),
+                    q->size(d - 2), k ? k->size(d - 2) : 0, q->size(d - 1), 2 * f->size(0), s, a[4] == Py_True, a[8] == Py_True, scale,
+                    dtype_of(*q));
+  });
+  if (r != CTB_OK) return done(r, nullptr);
+  return Py_BuildValue("(NN)", given_or(a[6], made[0]), k ? given_or(a[7], made[1]) : Py_NewRef(Py_None));
+}
+
+// A kvcache.KvCache (a tuple of k, v, k_scale or None, v_scale or None) in its ordinary form.
+bool cache_of(PyObject* o, const Tensor& like, ctb_kv_cache* c) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const Tensor* t[4];
+  for (int i = 0; i < 4; ++i) {
+    PyObject* x = PyTuple_GET_ITEM(o, i);
+    t[i] = x == Py_None ? nullptr : cuda_tensor(x);
+    if ((!t[i] && (i < 2 || x != Py_None)) || (t[i] && t[i]->device() != like.device())) return false;
+  }
+  const Tensor &k = *t[0], &v = *t[1];
+  if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type()) return false;
+  switch (k.scalar_type()) {
+    case at::kHalf: c->dtype = CTB_F16; break;
+    case at::kBFloat16: c->dtype = CTB_BF16; break;
+    case at::kFloat8_e4m3fn: c->dtype = CTB_E4M3; break;
+    case at::kChar: c->dtype = CTB_I8; break;
+    default: return false;
+  }
+  const bool bytes = c->dtype == CTB_E4M3 || c->dtype == CTB_I8;
+  const int64_t D = k.size(3), page = k.size(2);
+  for (const Tensor* x : {&k, &v})
+    if (x->stride(3) != 1 || x->stride(2) != D || x->stride(1) != page * D) return false;
+  for (int i = 2; i < 4; ++i) {
+    if ((t[i] != nullptr) != bytes) return false;
+    if (bytes && (t[i]->scalar_type() != at::kFloat || t[i]->sizes() != k.sizes().slice(0, 3) || t[i]->stride(2) != 1 || t[i]->stride(1) != page))
+      return false;
+  }
+  c->k = k.data_ptr();
+  c->v = v.data_ptr();
+  c->k_scale = bytes ? static_cast<float*>(t[2]->data_ptr()) : nullptr;
+  c->v_scale = bytes ? static_cast<float*>(t[3]->data_ptr()) : nullptr;
+  c->pages = k.size(0);
+  c->kv_heads = k.size(1);
+  c->page_size = page;
+  c->head_dim = D;
+  c->k_page_stride = k.stride(0);
+  c->v_page_stride = v.stride(0);
+  c->k_scale_page_stride = bytes ? t[2]->stride(0) : 0;
+  c->v_scale_page_stride = bytes ? t[3]->stride(0) : 0;
+  return true;
+}
+// [tokens, heads, D] of the type and device of `like`, heads contiguous.
+bool token_rows(const Tensor* t, const Tensor& like, int64_t T, int64_t D, int64_t* s) {
+  if (!t || t->dim() != 3 || t->size(0) != T || t->size(2) != D || t->stride(2) != 1 || t->scalar_type() != like.scalar_type() ||
+      t->device() != like.device())
+    return false;
+  s[0] = t->stride(0);
+  s[1] = t->stride(1);
+  return true;
+}
+
+// kv_write(cache, slots, k, v, q, positions, frequencies, interleaved, scale, out_q) -> (out_q or None,); q .. frequencies, out_q: or None
+PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) return decline();
+  const Tensor *slots = cuda_tensor(a[1]), *k = cuda_tensor(a[2]), *v = cuda_tensor(a[3]);
+  const Tensor *q = a[4] == Py_None ? nullptr : cuda_tensor(a[4]), *pos = a[5] == Py_None ? nullptr : cuda_tensor(a[5]);
+  const Tensor* f = a[6] == Py_None ? nullptr : cuda_tensor(a[6]);
+  ctb_kv_cache cache;
+  float scale;
+  int64_t s[8] = {};
+  if (!slots || !k || !v || (!q && a[4] != Py_None) || (!pos && a[5] != Py_None) || (!f && a[6] != Py_None) || !PyBool_Check(a[7]) ||
+      !as_float(a[8], &scale) || dtype_of(*k) < 0 || k->dim() != 3 || !cache_of(a[0], *k, &cache))
+    return decline();
+  const int64_t T = k->size(0), D = cache.head_dim;
+  auto list = [&](const Tensor& t) { return t.dim() == 1 && t.size(0) == T && t.is_contiguous() && t.device() == k->device() && index_bits(t); };
+  if (!list(*slots) || !token_rows(k, *k, T, D, s + 4) || !token_rows(v, *k, T, D, s + 6) || k->size(1) != cache.kv_heads ||
+      v->size(1) != cache.kv_heads || (pos != nullptr) != (f != nullptr) || (f && (!frequencies_of(f, *k) || !list(*pos))) ||
+      (q && (!f || !token_rows(q, *k, T, D, s + 2))) || (!q && a[9] != Py_None))
+    return decline();
+  Call c(*k);
+  if (!c.ok()) return nullptr;
+  Tensor made;
+  const Tensor* out = nullptr;
+  if (q && (!(out = result_like(a[9], *q, &made)) || !token_rows(out, *k, T, D, s))) return decline();
+  const int r = without_gil([&] {
+    return ctb_kv_write(c.ctx, c.stream, &cache, slots->data_ptr(), index_bits(*slots), q ? out->data_ptr() : nullptr, q ? q->data_ptr() : nullptr,
+                        k->data_ptr(), v->data_ptr(), s, pos ? pos->data_ptr() : nullptr, pos ? index_bits(*pos) : 32,
+                        f ? static_cast<const double*>(f->data_ptr()) : nullptr, T, q ? q->size(1) : 0, f ? 2 * f->size(0) : 0, a[7] == Py_True,
+                        scale, dtype_of(*k));
+  });
+  if (r != CTB_OK) return done(r, nullptr);
+  return Py_BuildValue("(N)", q ? given_or(a[9], made) : Py_NewRef(Py_None));
+}
+
+bool page_table_of(const Tensor* table, const Tensor* lengths, const Tensor& like, int64_t* ld) {
+  if (!table || !lengths || table->device() != like.device() || lengths->device() != like.device() || table->scalar_type() != at::kInt ||
+      lengths->scalar_type() != at::kInt || table->dim() != 2 || lengths->dim() != 1 || lengths->size(0) != table->size(0) ||
+      !lengths->is_contiguous() || (table->size(1) > 1 && table->stride(1) != 1))
+    return false;
+  *ld = table->size(0) > 1 ? table->stride(0) : std::max(table->size(1), table->stride(0));
+  return true;
+}
+
+// kv_read(cache, page_table, lengths, max_length, dtype or None) -> (K, V)
+PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) return decline();
+  const Tensor *table = cuda_tensor(a[1]), *lengths = cuda_tensor(a[2]);
+  ctb_kv_cache cache;
+  long long seq;
+  int64_t ld;
+  if (!table || !page_table_of(table, lengths, *table, &ld) || !as_int(a[3], &seq) || seq < 0 || !cache_of(a[0], *table, &cache)) return decline();
+  at::ScalarType type;
+  if (THPDtype_Check(a[4])) type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+  else if (a[4] == Py_None && cache.dtype == CTB_F16) type = at::kHalf;
+  else if (a[4] == Py_None && cache.dtype == CTB_BF16) type = at::kBFloat16;
+  else return decline();
+  if (type != at::kHalf && type != at::kBFloat16) return decline();
+  Call c(*table);
+  if (!c.ok()) return nullptr;
+  const auto options = table->options().dtype(type);
+  Tensor K = at::empty({table->size(0), cache.kv_heads, seq, cache.head_dim}, options), V = at::empty_like(K);
+  const int r = without_gil([&] {
+    return ctb_kv_read(c.ctx, c.stream, K.data_ptr(), V.data_ptr(), &cache, static_cast<const int32_t*>(table->data_ptr()),
+                       static_cast<const int32_t*>(lengths->data_ptr()), table->size(0), seq, table->size(1), ld,
+                       type == at::kHalf ? CTB_F16 : CTB_BF16);
+  });
+  if (r != CTB_OK) return done(r, nullptr);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(K)), THPVariable_Wrap(std::move(V)));
+}
+
+// fmha_paged(Q, cache, page_table, lengths, qk_scale or None, return_lse) -> Out or (Out, lse)
+PyObject* fmha_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) return decline();
+  const Tensor *q = cuda_tensor(a[0]), *table = cuda_tensor(a[2]), *lengths = cuda_tensor(a[3]);
+  ctb_kv_cache cache;
+  int64_t ld, s[2];
+  float scale;
+  if (!q || q->dim() != 3 || dtype_of(*q) < 0 || !PyBool_Check(a[5]) || !page_table_of(table, lengths, *q, &ld) || !cache_of(a[1], *q, &cache) ||
+      !token_rows(q, *q, table->size(0), cache.head_dim, s))
+    return decline();
+  if (a[4] == Py_None) scale = (float)(1.0 / std::sqrt((double)cache.head_dim));
+  else if (!as_float(a[4], &scale)) return decline();
+  Call c(*q);
+  if (!c.ok()) return nullptr;
+  const int64_t B = q->size(0), H = q->size(1);
+  Tensor out = at::empty({B, H, cache.head_dim}, q->options()), lse;
+  const bool with_lse = a[5] == Py_True;
+  if (with_lse) lse = at::empty({B, H}, q->options().dtype(at::kFloat));
+  const int r = without_gil([&] {
+    return ctb_fmha_paged(c.ctx, c.stream, out.data_ptr(), with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, q->data_ptr(), &cache,
+                          static_cast<const int32_t*>(table->data_ptr()), static_cast<const int32_t*>(lengths->data_ptr()), B, H, s[0], s[1],
+                          table->size(1), ld, scale, dtype_of(*q));
+  });
+  if (r != CTB_OK) return done(r, nullptr);
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+}
+
 // moe_router(hidden, W_r, topk) -> (gates [topk, T] f16, ids [topk, T] int32)
 PyObject* moe_router(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *x, *w;
@@ -1006,7 +1208,8 @@ PyMethodDef kMethods[] = {CTB_METHOD(setup),         CTB_METHOD(softmax),       
                           CTB_METHOD(mapreduce),     CTB_METHOD(fft),
                           CTB_METHOD(token_logprobs), CTB_METHOD(token_logprobs_bwd), CTB_METHOD(distill_fwd),
                           CTB_METHOD(distill_bwd),   CTB_METHOD(distill_fwd_bwd), CTB_METHOD(moe_route),
-                          CTB_METHOD(moe_route_bwd),
+                          CTB_METHOD(moe_route_bwd), CTB_METHOD(rope),           CTB_METHOD(kv_write),
+                          CTB_METHOD(kv_read),       CTB_METHOD(fmha_paged),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Native call path of cutile_b200.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -47,7 +47,7 @@ struct RelaxedCapture {
 }  // namespace
 
 struct ScratchSlot {
-  void* memory = nullptr;  // kStreamScratchBytes, then kTickets counters
+  void* memory = nullptr;  // kSlotBytes, then kTickets counters
   bool owned = false;      // by (stream, capture); capture 0: eager launches
   unsigned long long stream = 0, capture = 0;
   int users = 0;           // calls that have it and have not launched yet
@@ -86,10 +86,10 @@ bool allocate(ScratchPool* p, ScratchSlot* s) {
   RelaxedCapture relaxed;
   constexpr size_t ticket_bytes = kTickets * sizeof(unsigned);
   cudaStream_t st = nullptr;
-  cudaError_t e = cudaMalloc(&s->memory, kStreamScratchBytes + ticket_bytes);
+  cudaError_t e = cudaMalloc(&s->memory, kSlotBytes + ticket_bytes);
   if (e != cudaSuccess) s->memory = nullptr;
   if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
-  if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(s->memory) + kStreamScratchBytes, 0, ticket_bytes, st);
+  if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(s->memory) + kSlotBytes, 0, ticket_bytes, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&s->event, cudaEventDisableTiming);
   if (st) cudaStreamDestroy(st);
@@ -198,7 +198,7 @@ StreamScratch::StreamScratch(ctb_ctx* ctx, cudaStream_t stream) : pool_(ctx->scr
   slot_->marked = false;
   mark_ = !captured && held >= kMarkFrom;
   data = static_cast<float*>(slot_->memory);
-  tickets = reinterpret_cast<unsigned*>(static_cast<char*>(slot_->memory) + kStreamScratchBytes);
+  tickets = reinterpret_cast<unsigned*>(static_cast<char*>(slot_->memory) + kSlotBytes);
 }
 
 StreamScratch::~StreamScratch() {

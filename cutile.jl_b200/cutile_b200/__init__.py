@@ -15,4 +15,4 @@ if _host.TORCH_VERSION != torch.__version__:  # it reads tensors by the layout o
     raise ImportError(f"_host.so was built for torch {_host.TORCH_VERSION}, this is torch {torch.__version__}: "
                       "build it again with `python cutile.jl_b200/csrc/build.py`")
 from ._lib import CtbError, version_info, check_device_status  # noqa: F401
-from . import softmax, layernorm, matmul, batchmatmul, fmha, moe, multi, vadd, transpose, fft, tiled, logprobs, distill  # noqa: F401
+from . import softmax, layernorm, matmul, batchmatmul, fmha, moe, multi, vadd, transpose, fft, tiled, logprobs, distill, rope, kvcache  # noqa: F401

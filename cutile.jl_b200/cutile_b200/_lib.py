@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcutile_b200.so")
 
 OK, BAD_ARG, BAD_ALIGN, UNSUPPORTED_TILE, UNSUPPORTED, CUDA_ERROR, NCCL_ERROR, TIMEOUT, NO_DEVICE = range(9)
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3, I8 = 0, 1, 2, 3, 4
 
 
 class CtbError(RuntimeError):
@@ -42,6 +42,13 @@ class EpBuffers(C.Structure):
     _fields_ = [("world", _i), ("rank", _i), ("recv_rows", _p * EP_MAX_RANKS), ("recv_ids", _p * EP_MAX_RANKS),
                 ("recv_gates", _p * EP_MAX_RANKS), ("slot_out", _p * EP_MAX_RANKS), ("flags", _p * EP_MAX_RANKS),
                 ("epoch", _p)]
+
+
+class KvCacheArrays(C.Structure):
+    """ctb_kv_cache: the arrays of a paged key-value cache."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64),
+                ("head_dim", _i64), ("k_page_stride", _i64), ("v_page_stride", _i64), ("k_scale_page_stride", _i64),
+                ("v_scale_page_stride", _i64), ("dtype", _i)]
 
 
 # name -> argument types (return type is int unless listed in _RESTYPES)
@@ -80,6 +87,10 @@ SIGNATURES = {
                          _i],
     "ctb_fmha_fwd": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, C.c_int32, _i, _i, _i, _i,
                      _i],
+    "ctb_rope": [_p, _p, _p, _p, _p, _p, _p, _i, _p, _i64, _i64, _i64, _i64, _i64, _i64, C.POINTER(_i64), _i, _i, _f, _i],
+    "ctb_kv_write": [_p, _p, C.POINTER(KvCacheArrays), _p, _i, _p, _p, _p, _p, C.POINTER(_i64), _p, _i, _p, _i64, _i64, _i64, _i, _f, _i],
+    "ctb_kv_read": [_p, _p, _p, _p, C.POINTER(KvCacheArrays), _p, _p, _i64, _i64, _i64, _i64, _i],
+    "ctb_fmha_paged": [_p, _p, _p, _p, _p, C.POINTER(KvCacheArrays), _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f, _i],
     "ctb_layernorm_bwd_static": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64],
     "ctb_layernorm_bwd_static_status": [_p],
     "ctb_moe_max_blocks": [_i64, _i64, _i64, _i],

@@ -44,7 +44,7 @@ typedef enum ctb_status {
   CTB_NO_DEVICE = 8         /* no sm_100 device / driver                           */
 } ctb_status;
 
-typedef enum ctb_dtype { CTB_F32 = 0, CTB_F16 = 1, CTB_BF16 = 2 } ctb_dtype;
+typedef enum ctb_dtype { CTB_F32 = 0, CTB_F16 = 1, CTB_BF16 = 2, CTB_E4M3 = 3, CTB_I8 = 4 } ctb_dtype; /* the last two: caches only */
 
 typedef struct ctb_ctx ctb_ctx;
 
@@ -283,6 +283,60 @@ int ctb_fmha_fwd(ctb_ctx* ctx, void* stream, const void* Q, const void* K, const
                  int64_t d_v, int64_t seq_q, int64_t seq_kv, int64_t heads, int64_t kv_heads, int64_t batch,
                  float qk_scale, int32_t input_pos, int tile_m, int tile_n, int query_group_size, int causal,
                  int dtype);
+
+/* ---- Rotary positions ---------------------------------------------------------- */
+/* (No counterpart in the reference.)  Turns pairs of the first `rotary` dimensions (even, at most D) of every head by an angle
+ * that grows with the token's position: pair i of a token at position n by a = n * frequencies[i],
+ *   (x1, x2) -> scale * (x1 cos a - x2 sin a, x1 sin a + x2 cos a),
+ * and by -a with `inverse`, which is the gradient.  Pairs are elements (2i, 2i + 1) with `interleaved`, else (i, i + rotary / 2); the
+ * other dimensions are copied.  Up to two arrays of one call (queries and keys; k may be NULL): q (D, q_heads, seq, batch), k (D,
+ * k_heads, seq, batch) in CTB_F32, CTB_F16 or CTB_BF16, dimensions contiguous, with strides[12] (elements) of q_out, q, k_out, k:
+ * batch, seq, head each.  positions (seq, batch), dense, 32- or 64-bit; frequencies (rotary / 2) f64, both device arrays.  Angles are
+ * formed and reduced in f64 (|n| < 2^31), cosines and sines are within 2^-22, and results are rounded once.  A result may lie
+ * where its rows lie (the same address and strides), and must not overlap them, or the other array, in any other way. */
+int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, void* k_out, const void* k, const void* positions,
+             int position_bits, const double* frequencies, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t D,
+             int64_t rotary, const int64_t* strides, int interleaved, int inverse, float scale, int dtype);
+
+/* ---- Paged key-value cache -------------------------------------------------------- */
+/* (No counterpart in the reference.)  Keys and values of sequences in pages of page_size tokens (a power of two from 16 to 1024):
+ * k and v (head_dim, page_size, kv_heads, pages), dense but for the strides from page to page (elements, multiples of 16 bytes), 16-byte
+ * aligned; head_dim 64 or 128.  dtype CTB_F16 or CTB_BF16, or 8 bits with a scale per token and head in k_scale and v_scale
+ * (page_size, kv_heads, pages) f32: CTB_I8 (codes -127..127) and CTB_E4M3 (up to 448); the value is code * scale.  A page of a
+ * sequence is named by its 1-based number in a page table (table_width, batch) int32 (0: none); lengths (batch) int32 says how
+ * many tokens a sequence has.  A token's slot is its 1-based place in the whole cache, (page - 1) * page_size + place in the page + 1. */
+typedef struct ctb_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale; /* NULL with 16 bits */
+  int64_t pages, kv_heads, page_size, head_dim;
+  int64_t k_page_stride, v_page_stride, k_scale_page_stride, v_scale_page_stride;
+  int dtype;
+} ctb_kv_cache;
+/* Writes k and v (head_dim, kv_heads, tokens), CTB_F16 or CTB_BF16 (the cache's type, or any of the two for 8 bits), to slots
+ * (tokens) 32- or 64-bit; slot 0 writes nothing, a slot outside of the cache is a bad index (ctb_check_device_status) and writes
+ * nothing either; slots that are not 0 must differ.  With frequencies, keys are turned by their positions as by ctb_rope before
+ * they are stored (rounded once, when stored), and so are the queries q (head_dim, heads, tokens), if given, into q_out, for all tokens.
+ * strides[8] (elements): of q_out, q, k, v: token, head each.
+ * 8 bits: with a the largest magnitude of a row and c the largest code, scale = a / c and code = x c / a, rounded to the
+ * nearest, ties to even.  Rows with a < 2^-100 are stored as zeros, rows with an infinity or NaN with a scale that is one. */
+int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cache, const void* slots, int slot_bits, void* q_out,
+                 const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int position_bits,
+                 const double* frequencies, int64_t tokens, int64_t heads, int64_t rotary, int interleaved, float scale, int dtype);
+/* Reads sequences back: K, V (head_dim, seq, kv_heads, batch) dense, CTB_F16 or CTB_BF16 (of a 16-bit cache its type): what
+ * ctb_fmha_fwd takes.  Tokens behind a sequence's length are zeros.  A length outside of 0..table_width * page_size, or a page that a
+ * length needs outside of 1..pages, is a bad index, and the tokens in question are NaN. */
+int ctb_kv_read(ctb_ctx* ctx, void* stream, void* K, void* V, const ctb_kv_cache* cache, const int32_t* page_table,
+                const int32_t* lengths, int64_t batch, int64_t seq, int64_t table_width, int64_t table_stride, int dtype);
+/* Attention of one query row per head and sequence over the cache: with s_j = qk_scale q.k_j for the tokens j of the sequence,
+ * Out = sum_j exp(s_j) v_j / sum_j exp(s_j), lse = log sum_j exp(s_j) (may be NULL).  Q (head_dim, heads, batch), CTB_F16 or CTB_BF16 (the
+ * cache's type if that has 16 bits), with strides from sequence to sequence and head to head (multiples of 8); Out (head_dim,
+ * heads, batch) in the type of Q and lse (heads, batch) f32, dense.  heads is a multiple of kv_heads, and head h has the keys of
+ * h / (heads / kv_heads).  A length of 0 gives zeros and -inf; bad lengths and pages as above make the sequence's (for a page, the
+ * heads') results NaN.  What the cache holds behind a sequence's length does not matter.  Scores, sums and outputs are f32,
+ * probabilities enter the product with values as the sum of two 16-bit numbers.  Bitwise repeatable. */
+int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse, const void* Q, const ctb_kv_cache* cache,
+                   const int32_t* page_table, const int32_t* lengths, int64_t batch, int64_t heads, int64_t q_seq_stride,
+                   int64_t q_head_stride, int64_t table_width, int64_t table_stride, float qk_scale, int dtype);
 
 /* ---- Mixture of experts -------------------------------------------------------- */
 /* Upper bound on the number of tile_m-slot blocks moe_align can emit:
