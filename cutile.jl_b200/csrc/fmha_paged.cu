@@ -19,8 +19,9 @@ namespace {
 
 enum Store { F16 = 0, BF16 = 1, E4M3 = 2, I8 = 3 };
 
-constexpr int kMaxBatch = 4096;  // sequences of a launch (their prefix sums lie in shared memory)
+constexpr int kMaxBatch = 1024;  // sequences of a launch (their lengths lie in shared memory)
 constexpr int kMinTiles = 2;     // of a warp, where there is that much work
+constexpr unsigned kWholeItems = 40;  // tiles of the longest item up to which CTAs have whole items
 // Exponents' reference (in powers of two): it moves once a score stands kLazy above the largest that it knows.  What goes to f16 is lifted
 // by kLift, so that the largest is at most 2^(kLazy + kLift + 1) and what f16 pairs cannot tell from 0 is 2^-(25 + kLift) of it.
 constexpr int kLazy = 6, kLift = 8;
@@ -51,21 +52,55 @@ struct Shape {
   static constexpr int QW = D / 8;                   // words that a lane has of a query row
   static constexpr int R = 8 * NT;
   static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = kWarps * 32;
+  static constexpr int kEntry = 4096;                // bytes of keys or values of a tile
+  static constexpr int kRing = NT == 1 ? 3 : 4;      // entries that a warp has or has asked for
   static constexpr int kPitch = D + 4;               // floats between rows of partial results in shared memory
   static constexpr int kSlotFloats = R * kPitch + 2 * R;
   static constexpr int kPartFloats = R * D + 2 * R;
-  static constexpr size_t kSmem = sizeof(float) * 2 * kWarps * kSlotFloats + sizeof(unsigned) * (kMaxBatch + 1);
+  static constexpr int kScales = kBytes ? 16 * KT : 0;  // of an entry
+  static constexpr size_t kSmem =
+      128 + (size_t)kWarps * (kRing * (kEntry + kScales * 4) + kSlotFloats * 4) + (2 * kMaxBatch + 1) * 4;
 };
 
-__device__ __forceinline__ uint4 load16(const void* p) {
+template <int OFFSET>
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFFSET));
   return v;
 }
-__device__ __forceinline__ uint2 load8(const void* p) {
+template <int OFFSET>
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at), "n"(OFFSET)
+               : "memory");
+}
+template <int OFFSET>
+__device__ __forceinline__ uint2 lds8(uint32_t at) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(at), "n"(OFFSET));
   return v;
+}
+template <int SRC, int DST>
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {  // all but the last N groups of every lane have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  __syncwarp();
+}
+template <class F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F f) {  // f(std::integral_constant<int, i>()) for i = 0 .. N - 1
+  each(f, std::make_integer_sequence<int, N>());
 }
 template <bool BF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -140,46 +175,67 @@ struct Cursor {
 };
 
 template <int STORE, int D, int NT>
-__global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_kernel(const Params p, int* status) {
+__global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
+    fmha_paged_kernel(const Params p, int* status) {
   using S = Shape<STORE, D, NT>;
   constexpr int KC = S::KC, KT = S::KT, VW = S::VW, MT = S::MT, QW = S::QW, R = S::R, kWarps = S::kWarps, kThreads = S::kThreads;
-  constexpr int kTileKeys = 16 * KT;
+  constexpr int kTileKeys = 16 * KT, kRow = S::kRow, kRing = S::kRing;
   constexpr bool BF = STORE == BF16;
   constexpr float kAbove = STORE == F16 ? kLift : 0;  // what the known largest score stands above m
-  extern __shared__ __align__(16) float smem[];
-  float* slots = smem;  // [warp][first, last item of its range][R rows, maxima, sums]
-  unsigned* prefix = reinterpret_cast<unsigned*>(smem + 2 * kWarps * S::kSlotFloats);
-  __shared__ unsigned warp_sum[kWarps], seg_lo[2 * kWarps], seg_hi[2 * kWarps];
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  // [warp][entries], [warp][entries' scales], [warp][R rows, maxima, sums], lengths, tiles before
+  float* all_scales = reinterpret_cast<float*>(smem + kWarps * kRing * S::kEntry);
+  float* firsts = all_scales + kWarps * kRing * S::kScales;
+  int* lens = reinterpret_cast<int*>(firsts + kWarps * S::kSlotFloats);
+  unsigned* prefix = reinterpret_cast<unsigned*>(lens + kMaxBatch);
+  __shared__ unsigned warp_sum[kWarps], warp_most[kWarps], seg_lo[2 * kWarps], seg_hi[2 * kWarps];
   __shared__ int seg_item[2 * kWarps];
   __shared__ int last_s[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  // Results of a warp's part of an item: of the first item of its range beside the ring, of the last one in the ring, which is empty by then.
+  auto slot_at = [&](int slot) {
+    return slot & 1 ? reinterpret_cast<float*>(smem + (slot >> 1) * (kRing * S::kEntry)) : firsts + (slot >> 1) * S::kSlotFloats;
+  };
   grid_dependency_sync();
 
   // ---- tiles before every sequence
   const int most = p.width << p.page_log2;
   const unsigned per_tile = (unsigned)p.kv_heads * p.row_tiles;
+  unsigned longest;
   {
-    const int per = (p.batch + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(p.batch, b0 + per);
-    auto tiles = [&](int b) {
+    const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+    auto tiles = [&](int n) { return (unsigned)(n + kTileKeys - 1) / kTileKeys; };
+    unsigned sum = 0, top = 0;
+    for (int b = b0; b < b1; ++b) {
       const int n = min(max(__ldg(p.lengths + b), 0), most);
-      return (unsigned)((n + kTileKeys - 1) / kTileKeys) * per_tile;
-    };
-    unsigned sum = 0;
-    for (int b = b0; b < b1; ++b) sum += tiles(b);
+      lens[b] = n;
+      sum += tiles(n) * per_tile;
+      top = max(top, tiles(n));
+    }
     unsigned up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned v = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += v;
     }
-    if (lane == 31) warp_sum[warp] = up;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 31) {
+      warp_sum[warp] = up;
+      warp_most[warp] = top;
+    }
     if (tid < 2 * kWarps) seg_item[tid] = -1;
     __syncthreads();
     unsigned before = up - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    longest = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? warp_sum[w] : 0;
+      longest = max(longest, warp_most[w]);
+    }
     for (int b = b0; b < b1; ++b) {
       prefix[b] = before;
-      before += tiles(b);
+      before += tiles(lens[b]) * per_tile;
     }
     if (tid == kThreads - 1) prefix[p.batch] = before;
     __syncthreads();
@@ -187,145 +243,177 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
   const unsigned total = prefix[p.batch];
   // sequences without keys
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    const int n = __ldg(p.lengths + b);
-    if (min(n, most) > 0) continue;
-    if (n != 0 && tid == 0) atomicMax(status, (int)DEV_BAD_INDEX);
+    if (lens[b] > 0) continue;
+    const bool wrong = __ldg(p.lengths + b) != 0;
+    if (wrong && tid == 0) atomicMax(status, (int)DEV_BAD_INDEX);
     uint32_t* out = static_cast<uint32_t*>(p.Out) + (int64_t)b * p.heads * (D / 2);
-    for (int i = tid; i < p.heads * (D / 2); i += kThreads) out[i] = n != 0 ? 0x7fff7fffu : 0u;
+    for (int i = tid; i < p.heads * (D / 2); i += kThreads) out[i] = wrong ? 0x7fff7fffu : 0u;
     if (p.lse)
-      for (int i = tid; i < p.heads; i += kThreads) p.lse[(int64_t)b * p.heads + i] = n != 0 ? NAN : -INFINITY;
+      for (int i = tid; i < p.heads; i += kThreads) p.lse[(int64_t)b * p.heads + i] = wrong ? NAN : -INFINITY;
   }
   if (total == 0) return;
-  const unsigned all = gridDim.x * kWarps, workers = min(all, (total + kMinTiles - 1) / kMinTiles);
-  const unsigned me = blockIdx.x * kWarps + warp;
-  auto range_of = [&](unsigned w) { return first_tile(min(w, workers), total, workers); };
-  const unsigned lo = range_of(me), hi = range_of(me + 1);
-
-  auto write_row = [&](int b, int head, int row, int d, const float (&v)[8]) {  // eight dimensions of a head of the group
-    uint16_t* out = static_cast<uint16_t*>(p.Out) + ((int64_t)b * p.heads + (int64_t)head * p.group + row) * D + d;
-    uint4 w;
-    if (p.q_bf16) w = make_uint4(pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3]), pack2<true>(v[4], v[5]), pack2<true>(v[6], v[7]));
-    else w = make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]), pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
-    *reinterpret_cast<uint4*>(out) = w;
+  auto sequence_of = [&](unsigned x) {  // that has tile x: the last one that begins at or before it
+    int a = 0, z = p.batch - 1;
+    while (a < z) {
+      const int mid = (a + z + 1) >> 1;
+      if (prefix[mid] <= x) a = mid;
+      else z = mid - 1;
+    }
+    return a;
   };
+  // Ranges of the line of tiles: equal ones for all warps of the grid, or, where items are short, for the warps of a CTA, whose range
+  // ends where an item ends.
+  const bool whole_items = longest <= kWholeItems;
+  const unsigned all = gridDim.x * kWarps, workers = min(all, (total + kMinTiles - 1) / kMinTiles);
+  auto range_of = [&](unsigned w) { return first_tile(min(w, workers), total, workers); };
+  unsigned cta_lo, cta_hi, lo, hi;
+  if (whole_items) {
+    auto end_of = [&](unsigned i) {  // the end of an item that is next to the end of an equal range
+      const unsigned x = first_tile(i, total, gridDim.x);
+      if (x >= total) return total;
+      const int b = sequence_of(x);
+      const unsigned tiles = (unsigned)(lens[b] + kTileKeys - 1) / kTileKeys;
+      return prefix[b] + (x - prefix[b] + tiles / 2) / tiles * tiles;
+    };
+    cta_lo = end_of(blockIdx.x);
+    cta_hi = end_of(blockIdx.x + 1);
+    lo = cta_lo + first_tile(warp, cta_hi - cta_lo, kWarps);
+    hi = cta_lo + first_tile(warp + 1, cta_hi - cta_lo, kWarps);
+  } else {
+    cta_lo = range_of(blockIdx.x * kWarps);
+    cta_hi = range_of((blockIdx.x + 1) * kWarps);
+    lo = range_of(blockIdx.x * kWarps + warp);
+    hi = range_of(blockIdx.x * kWarps + warp + 1);
+  }
+
   auto write_lse = [&](int b, int head, int row, float m, float l) {
     if (p.lse) p.lse[(int64_t)b * p.heads + (int64_t)head * p.group + row] = (m + log2f(l)) * 0.6931471805599453f;
   };
 
+  auto next = [&](Cursor& t) {
+    t.key += kTileKeys;
+    if (t.key < t.len) return;
+    t.key = 0;
+    if (++t.rt < p.row_tiles) return;
+    t.rt = 0;
+    if (++t.head < p.kv_heads) return;
+    t.head = 0;
+    do ++t.b;
+    while (t.b < p.batch && (t.len = lens[t.b]) <= 0);
+  };
+  auto cursor_at = [&](unsigned x) {
+    Cursor t;
+    t.b = sequence_of(x);
+    t.len = lens[t.b];
+    const unsigned tiles = (unsigned)(t.len + kTileKeys - 1) / kTileKeys, at = x - prefix[t.b], item = at / tiles;
+    t.head = item / p.row_tiles;
+    t.rt = item - t.head * p.row_tiles;
+    t.key = (int)(at - item * tiles) * kTileKeys;
+    return t;
+  };
   if (lo < hi) {
-    const int page_keys = 1 << p.page_log2;
+    const int page_mask = (1 << p.page_log2) - 1;
+    Cursor now = cursor_at(lo);  // the tile at hand
+    // Tiles are asked for ahead of it: keys and values in turn, an entry of the warp's ring each; the numbers of their pages are read
+    // two tiles before that.
+    Cursor ahead = now, numbers = now;
+    unsigned ahead_x = lo, numbers_x = lo;
+    uint32_t bad_pages = 0;  // a bit per tile that has been asked for
     bool seen_bad = false;
-    auto length_of = [&](int b) { return min(__ldg(p.lengths + b), most); };
-    auto next = [&](Cursor& t) {
-      t.key += kTileKeys;
-      if (t.key < t.len) return;
-      t.key = 0;
-      if (++t.rt < p.row_tiles) return;
-      t.rt = 0;
-      if (++t.head < p.kv_heads) return;
-      t.head = 0;
-      do ++t.b;
-      while (t.b < p.batch && (t.len = length_of(t.b)) <= 0);
-    };
-    auto page_ids = [&](const Cursor& t, int (&id)[KT]) {
+    int id[3][KT] = {};
+    auto more_ids = [&](int (&to)[KT]) {
+      if (numbers_x >= hi) return;
+      const int32_t* row = p.table + (int64_t)numbers.b * p.table_ld;
 #pragma unroll
       for (int s = 0; s < KT; ++s) {
-        const int key = t.key + 16 * s;
-        id[s] = key < t.len ? __ldg(p.table + (int64_t)t.b * p.table_ld + (key >> p.page_log2)) : 0;
+        const int key = numbers.key + 16 * s;
+        to[s] = key < numbers.len ? __ldg(row + (key >> p.page_log2)) : 0;
       }
+      if (++numbers_x < hi) next(numbers);
     };
-    // the page that is read for an id: the first one where there is none
-    auto page = [&](int id) { return (unsigned)(id - 1) < (unsigned)p.pages ? id - 1 : 0; };
-    auto load_k = [&](const Cursor& t, const int (&id)[KT], uint4 (&k)[KT][2][KC], float (&ks)[KT][2]) {
 #pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const int key = t.key + 16 * s;
-        if (KT > 1 && key >= t.len) continue;
-        const int64_t row = ((int64_t)t.head << p.page_log2) + (key & (page_keys - 1)) + g;
-        const char* src = static_cast<const char*>(p.K) + (page(id[s]) * p.k_page + row * D) * (S::kBytes ? 1 : 2) + c * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < KC; ++i) k[s][h][i] = load16(src + h * 8 * S::kRow + i * 64);
-        if constexpr (S::kBytes) {
-          const float* sc = p.Ks + page(id[s]) * p.ks_page + row;
-          ks[s][0] = __ldg(sc);
-          ks[s][1] = __ldg(sc + 8);
-        }
-      }
-    };
-    // keys 2c, 2c + 1, 2c + 8, 2c + 9 of each sixteen; a word has the dimensions that stand in it
-    auto load_v = [&](const Cursor& t, const int (&id)[KT], uint32_t (&v)[KT][4][VW], float (&vs)[KT][2]) {
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const int key = t.key + 16 * s;
-        const int64_t row = ((int64_t)t.head << p.page_log2) + (key & (page_keys - 1));
-        const char* src = static_cast<const char*>(p.V) + (page(id[s]) * p.v_page + row * D) * (S::kBytes ? 1 : 2);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int j = 2 * c + (h & 1) + 8 * (h >> 1);
-          const bool live = key + j < t.len;  // rows behind the last key may hold anything: 0 x NaN is NaN
-          const char* at = src + j * S::kRow;
-          if constexpr (S::kRow == 64) {
-            const uint2 w = live ? load8(at + g * 8) : make_uint2(0, 0);
-            v[s][h][0] = w.x;
-            v[s][h][1] = w.y;
-          } else {
-#pragma unroll
-            for (int l = 0; l < S::kRow / 128; ++l) {
-              const uint4 w = live ? load16(at + g * 16 + l * 128) : make_uint4(0, 0, 0, 0);
-              v[s][h][4 * l] = w.x;
-              v[s][h][4 * l + 1] = w.y;
-              v[s][h][4 * l + 2] = w.z;
-              v[s][h][4 * l + 3] = w.w;
+    for (int i = 0; i < 3; ++i) more_ids(id[i]);
+
+    const uint32_t ring = smem_u32(smem) + warp * (kRing * S::kEntry);
+    float* scales = all_scales + warp * (kRing * S::kScales);
+    int put = 0, slot = 0;
+    // Where a lane's 16 bytes of 512 go: rows in 128-byte lines whose chunks are exchanged by the line's number (in 64-byte rows by that
+    // of every second one); lines of 256-byte rows' second halves behind those of the first of 16 rows.
+    const uint32_t to = kRow == 256   ? ((lane >> 3) & 1) * 2048 + (lane >> 4) * 128 + ((lane & 7) ^ (lane >> 4)) * 16
+                        : kRow == 128 ? (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16
+                                      : (lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
+    auto ask = [&](auto values) {
+      constexpr bool V = decltype(values)::value;
+      if (ahead_x < hi) {
+        const uint32_t dst = ring + put * S::kEntry + to;
+        bool wrong = false;
+        unrolled<KT>([&](auto s_tag) {
+          constexpr int s = decltype(s_tag)::value;
+          const int key = ahead.key + 16 * s;
+          if (KT == 1 || key < ahead.len) {
+            const bool good = (unsigned)(id[0][s] - 1) < (unsigned)p.pages;
+            wrong |= !good;
+            const int64_t page = good ? id[0][s] - 1 : 0;  // the first one where there is none
+            const int row = (ahead.head << p.page_log2) + (key & page_mask);
+            const char* src = static_cast<const char*>(V ? p.V : p.K) + (page * (V ? p.v_page : p.k_page) + (int64_t)row * D) * (S::kBytes ? 1 : 2) + lane * 16;
+            unrolled<8 / KT>([&](auto i_tag) {
+              constexpr int i = decltype(i_tag)::value;
+              constexpr int kFlip = kRow == 256 ? 32 * (i & 3) : kRow == 128 ? 64 * (i & 1) : 0, kRows = 512 / kRow * i;
+              copy16<i * 512, s * 16 * kRow + kRows * (kRow == 64 ? 64 : 128)>(dst ^ kFlip, src);
+            });
+            if constexpr (S::kBytes) {
+              const float* from = (V ? p.Vs + page * p.vs_page : p.Ks + page * p.ks_page) + row + (lane & 15);
+              if (lane < 16) copy4(smem_u32(scales + put * S::kScales + 16 * s + lane), from);
             }
           }
-        }
-        if constexpr (S::kBytes) {
-          const float* sc = p.Vs + page(id[s]) * p.vs_page + row + g;
-          vs[s][0] = key + g < t.len ? __ldg(sc) : 0.f;
-          vs[s][1] = key + g + 8 < t.len ? __ldg(sc + 8) : 0.f;
+        });
+        if constexpr (!V) {
+          const uint32_t bit = 1u << (ahead_x & 31);
+          bad_pages = wrong ? bad_pages | bit : bad_pages & ~bit;
+        } else {
+          if (++ahead_x < hi) next(ahead);
+#pragma unroll
+          for (int s = 0; s < KT; ++s) {
+            id[0][s] = id[1][s];
+            id[1][s] = id[2][s];
+          }
+          more_ids(id[2]);
         }
       }
+      copies_commit();
+      if (++put == kRing) put = 0;
     };
-    // first dimension of instruction j's pair in this lane
-    auto dim_of = [&](int j) {
-      if constexpr (S::kRow == 256) return (j >> 2) * 64 + g * 8 + 2 * (j & 3);
-      else return g * (D / 8) + 2 * j;
-    };
-
-    Cursor now;  // the tile at hand
-    {
-      int a = 0, z = p.batch - 1;  // the sequence that has tile lo: the last one that begins at or before it and has keys
-      while (a < z) {
-        const int mid = (a + z + 1) >> 1;
-        if (prefix[mid] <= lo) a = mid;
-        else z = mid - 1;
-      }
-      now.b = a;
-      now.len = length_of(a);
-      const unsigned tiles = (unsigned)(now.len + kTileKeys - 1) / kTileKeys, at = lo - prefix[a], item = at / tiles;
-      now.head = item / p.row_tiles;
-      now.rt = item - now.head * p.row_tiles;
-      now.key = (int)(at - item * tiles) * kTileKeys;
+    constexpr std::false_type keys;
+    constexpr std::true_type values;
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      if (i & 1) ask(values);
+      else ask(keys);
     }
-    Cursor ahead = now;  // the tile whose keys are asked for
-    int id[KT], id1[KT];
-    uint4 k[KT][2][KC];
-    float ks[KT][2] = {};
-    page_ids(ahead, id1);
-    load_k(ahead, id1, k, ks);
-    next(ahead);
-    int id2[KT] = {};
-    if (lo + 1 < hi) page_ids(ahead, id2);
+    auto leave_entry = [&](auto next_is) {
+      __syncwarp();  // every lane has read it
+      ask(next_is);
+      if (++slot == kRing) slot = 0;
+    };
+    using AfterKeys = std::integral_constant<bool, (kRing & 1) != 0>;
+    using AfterValues = std::integral_constant<bool, (kRing & 1) == 0>;
+    // Dimensions of a lane in instruction j's output: with 16 bits 16 j + g and 16 j + g + 8, with 8 bits the pair at
+    auto pair_of = [&](int j) { return g * (D / 8) + 2 * j; };
+    // This lane's places in an entry.  Its chunks of a key are 2c and 2c + 1 of a line (c where a row is half a line): with the swizzle,
+    // the eight lanes that a 16-byte load serves at a time (two keys) are in different banks.  16-bit values are read as matrices of
+    // eight keys' chunks and transposed on the way, 8-bit ones as chunk g (half a chunk where a row is half a line) of four keys.
+    const uint32_t k_at = kRow == 64 ? g * 64 + ((c ^ (g >> 1)) & 3) * 16 : g * 128 + ((2 * c) ^ g) * 16;
+    const uint32_t v_at = !S::kBytes ? ((lane >> 4) * 8 + (lane & 7)) * 128 + (((lane >> 3) & 1) ^ (lane & 7)) * 16
+                          : kRow == 64 ? c * 128 + ((g >> 1) ^ c) * 16 + (g & 1) * 8
+                                       : c * 256 + (g ^ (2 * c)) * 16;
 
     for (unsigned x = lo; x < hi;) {
       // ---- an item or the part of it that is this warp's
       const int b = now.b, head = now.head, rt = now.rt, len = now.len;
       const unsigned tiles = (unsigned)(len + kTileKeys - 1) / kTileKeys;
       const unsigned item_lo = x - (unsigned)now.key / kTileKeys, item_hi = item_lo + tiles, end = min(hi, item_hi);
-      bool bad = __ldg(p.lengths + b) > most;
       const int rows = p.group - rt * R;  // live rows, at least one
+      bool bad = __ldg(p.lengths + b) > most;
       uint32_t q[NT][QW];
       float mult[NT][2];  // score in powers of two of the rows 2c, 2c + 1
 #pragma unroll
@@ -338,7 +426,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
         for (int i = 0; i < KC; ++i)
 #pragma unroll
           for (int h = 0; h < kDims / 8; ++h) {
-            const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src + (i * 4 + c) * kDims + 8 * h)) : make_uint4(0, 0, 0, 0);
+            const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src + (kRow == 64 ? c : (i >> 1) * 8 + 2 * c + (i & 1)) * kDims + 8 * h)) : make_uint4(0, 0, 0, 0);
             const int at = (i * kDims / 8 + h) * 4;
             q[n][at] = w.x;
             q[n][at + 1] = w.y;
@@ -369,6 +457,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
         mult[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
       }
       float o[MT][NT][4], m[NT][2], ref[NT][2], l[NT][2], unit[NT][2], peak[NT][2];
+      bool fresh = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -383,77 +472,83 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-
       for (; x < end; ++x) {
+        copies_wait<kRing - 1>();
+        bad |= (bad_pages >> (x & 31)) & 1;
+        float sc[KT][NT][4], ks[KT][2];
+        const uint32_t k_even = ring + slot * S::kEntry + k_at, k_odd = k_even ^ 16;
+        if constexpr (S::kBytes) {
 #pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          id[s] = id1[s];
-          id1[s] = id2[s];
-          bad |= now.key + 16 * s < len && (unsigned)(id[s] - 1) >= (unsigned)p.pages;
+          for (int s = 0; s < KT; ++s) {
+            ks[s][0] = scales[slot * S::kScales + 16 * s + g];
+            ks[s][1] = scales[slot * S::kScales + 16 * s + g + 8];
+          }
         }
-        uint32_t v[KT][4][VW];
-        float vs[KT][2] = {};
-        load_v(now, id, v, vs);
-        float sc[KT][NT][4];
+        unrolled<KT>([&](auto tag) {
+          constexpr int s = decltype(tag)::value;
+          uint4 k[2][KC];
+          unrolled<2 * KC>([&](auto hi_tag) {
+            constexpr int h = decltype(hi_tag)::value / KC, i = decltype(hi_tag)::value % KC;
+            constexpr int kAt = s * 16 * kRow + (i >> 1) * 2048 + h * 8 * (kRow == 64 ? 64 : 128);
+            k[h][i] = lds16<kAt>(i & 1 ? k_odd : k_even);
+          });
 #pragma unroll
-        for (int s = 0; s < KT; ++s)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[s][n][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < KC; ++i) {
-              const uint32_t w0[4] = {k[s][0][i].x, k[s][0][i].y, k[s][0][i].z, k[s][0][i].w};
-              const uint32_t w1[4] = {k[s][1][i].x, k[s][1][i].y, k[s][1][i].z, k[s][1][i].w};
-              if constexpr (S::kBytes) {
+          for (int i = 0; i < KC; ++i) {
+            const uint32_t w0[4] = {k[0][i].x, k[0][i].y, k[0][i].z, k[0][i].w};
+            const uint32_t w1[4] = {k[1][i].x, k[1][i].y, k[1][i].z, k[1][i].w};
+            if constexpr (S::kBytes) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  uint32_t a0, a1, a2, a3;
-                  codes4<STORE>(w0[j], a0, a2);
-                  codes4<STORE>(w1[j], a1, a3);
-                  mma<false>(sc[s][n], a0, a1, a2, a3, q[n][8 * i + 2 * j], q[n][8 * i + 2 * j + 1]);
-                }
-              } else {
+              for (int j = 0; j < 4; ++j) {
+                uint32_t a0, a1, a2, a3;
+                codes4<STORE>(w0[j], a0, a2);
+                codes4<STORE>(w1[j], a1, a3);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  mma<BF>(sc[s][n], w0[2 * j], w1[2 * j], w0[2 * j + 1], w1[2 * j + 1], q[n][4 * i + 2 * j], q[n][4 * i + 2 * j + 1]);
+                for (int n = 0; n < NT; ++n) mma<false>(sc[s][n], a0, a1, a2, a3, q[n][8 * i + 2 * j], q[n][8 * i + 2 * j + 1]);
               }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma<BF>(sc[s][n], w0[2 * j], w1[2 * j], w0[2 * j + 1], w1[2 * j + 1], q[n][4 * i + 2 * j], q[n][4 * i + 2 * j + 1]);
             }
           }
-        float ks_now[KT][2];
-#pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          ks_now[s][0] = ks[s][0];
-          ks_now[s][1] = ks[s][1];
-        }
-        if (x + 1 < hi) {
-          load_k(ahead, id1, k, ks);
-          next(ahead);
-          if (x + 2 < hi) page_ids(ahead, id2);
-        }
-        // ---- scores in powers of two; e = 0, 1: key g, rows 2c, 2c + 1; e = 2, 3: key g + 8
-        bool grown = false;
+        });
+        leave_entry(AfterKeys());
+        // ---- Scores in powers of two: e = 0, 1: key g, rows 2c, 2c + 1; e = 2, 3: key g + 8.  d is their distance from the reference.
+        const bool tail = now.key + kTileKeys > len;
+        auto hidden = [&](int s, int e) { return tail && now.key + 16 * s + g + 8 * (e >> 1) >= len; };
+        auto times = [&](int s, int n, int e) {
+          if constexpr (S::kBytes) return mult[n][e & 1] * ks[s][e >> 1];
+          else return mult[n][e & 1];
+        };
+        float d[KT][NT][4], top_d = -INFINITY;
 #pragma unroll
         for (int s = 0; s < KT; ++s)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float t = sc[s][n][e] * mult[n][e & 1];
-              if constexpr (S::kBytes) t *= ks_now[s][e >> 1];
-              if (now.key + kTileKeys > len && now.key + 16 * s + g + 8 * (e >> 1) >= len) t = -INFINITY;
-              sc[s][n][e] = t;
-              grown |= t > m[n][e & 1] + (kAbove + kLazy);
+              d[s][n][e] = hidden(s, e) ? -INFINITY : fmaf(sc[s][n][e], times(s, n, e), -ref[n][e & 1]);
+              top_d = fmaxf(top_d, d[s][n][e]);
             }
-        grown = __any_sync(0xffffffffu, grown);
+        const bool grown = fresh || __any_sync(0xffffffffu, top_d > kAbove + kLazy);
         if (grown) {
+          fresh = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               float top = -INFINITY;
 #pragma unroll
-              for (int s = 0; s < KT; ++s) top = fmaxf(top, fmaxf(sc[s][n][r], sc[s][n][r + 2]));
+              for (int s = 0; s < KT; ++s)
+#pragma unroll
+                for (int e = r; e < 4; e += 2)
+                  if (!hidden(s, e)) top = fmaxf(top, sc[s][n][e] * times(s, n, e));
               const float m_new = fmaxf(m[n][r], max_over_keys(top) - kAbove);
               ref[n][r] = from_minus_inf(m_new);
               const float alpha = ex2_approx_ftz(m[n][r] - ref[n][r]);
@@ -465,36 +560,54 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
                 o[j][n][r] *= alpha;
                 o[j][n][r + 2] *= alpha;
               }
+#pragma unroll
+              for (int s = 0; s < KT; ++s)
+#pragma unroll
+                for (int e = r; e < 4; e += 2)
+                  if (!hidden(s, e)) d[s][n][e] = fmaf(sc[s][n][e], times(s, n, e), -ref[n][r]);
             }
         }
+        copies_wait<kRing - 1>();
 #pragma unroll
         for (int s = 0; s < KT; ++s)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float w = ex2_approx_ftz(sc[s][n][e] - ref[n][e & 1]);
-              l[n][e & 1] += w;
-              sc[s][n][e] = S::kBytes ? w * vs[s][e >> 1] : w;
+              d[s][n][e] = ex2_approx_ftz(d[s][n][e]);
+              l[n][e & 1] += d[s][n][e];
             }
         if constexpr (S::kBytes) {
           // A probability times its value's scale goes to f16 in units of (about) the largest so far: scales differ from key to key by
           // any factor.
-          bool off = grown;
+          float vs[KT][2];
+#pragma unroll
+          for (int s = 0; s < KT; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float v = scales[slot * S::kScales + 16 * s + g + 8 * h];
+              vs[s][h] = hidden(s, 2 * h) ? 0.f : v;
+            }
+          float top_w = 0.f;
 #pragma unroll
           for (int s = 0; s < KT; ++s)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) off |= sc[s][n][e] > (1 << kLazy) * peak[n][e & 1];
-          if (__any_sync(0xffffffffu, off)) {
+              for (int e = 0; e < 4; ++e) {
+                sc[s][n][e] = d[s][n][e] * (vs[s][e >> 1] * unit[n][e & 1]);
+                top_w = fmaxf(top_w, sc[s][n][e]);
+              }
+          if (grown || __any_sync(0xffffffffu, top_w > (float)(2 << (kLift + kLazy)))) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 float top = peak[n][r];
 #pragma unroll
-                for (int s = 0; s < KT; ++s) top = fmaxf(top, fmaxf(sc[s][n][r], sc[s][n][r + 2]));
+                for (int s = 0; s < KT; ++s)
+#pragma unroll
+                  for (int e = r; e < 4; e += 2) top = fmaxf(top, d[s][n][e] * vs[s][e >> 1]);
                 top = max_over_keys(top);
                 peak[n][r] = top;
                 const int e = (int)(__float_as_uint(top) >> 23);
@@ -506,88 +619,103 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
                   o[j][n][r] *= f;
                   o[j][n][r + 2] *= f;
                 }
+#pragma unroll
+                for (int s = 0; s < KT; ++s)
+#pragma unroll
+                  for (int e2 = r; e2 < 4; e2 += 2) sc[s][n][e2] = d[s][n][e2] * vs[s][e2 >> 1] * u;
               }
           }
-#pragma unroll
-          for (int s = 0; s < KT; ++s)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[s][n][e] *= unit[n][e & 1];
         }
-        // ---- O += V P, probabilities as two 16-bit numbers
-#pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          uint32_t hi_[NT][2], lo_[NT][2];
+        // ---- O += V P.  Probabilities are the sum of two 16-bit numbers beside 16-bit values, one f16 beside 8-bit ones.
+        const uint32_t v_even = ring + slot * S::kEntry + v_at, v_odd = v_even ^ 16;
+        unrolled<KT>([&](auto tag) {
+          constexpr int s = decltype(tag)::value;
+          uint32_t hi_[NT][2];
+          [[maybe_unused]] uint32_t lo_[NT][2];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float a = sc[s][n][2 * h], z = sc[s][n][2 * h + 1];
-              const uint32_t w = pack2<BF>(a, z);
-              const float2 f = unpack2<BF>(w);
-              hi_[n][h] = transposed(w);
-              lo_[n][h] = transposed(pack2<BF>(a - f.x, z - f.y));
+              if constexpr (S::kBytes) hi_[n][h] = transposed(pack2<false>(sc[s][n][2 * h], sc[s][n][2 * h + 1]));
+              else {
+                const uint32_t w = pack2<BF>(d[s][n][2 * h], d[s][n][2 * h + 1]);
+                const float2 f = unpack2<BF>(w);
+                hi_[n][h] = transposed(w);
+                lo_[n][h] = transposed(pack2<BF>(d[s][n][2 * h] - f.x, d[s][n][2 * h + 1] - f.y));
+              }
             }
+          // rows behind the last key may hold anything: 0 x NaN is NaN
+          const int left = len - now.key - 16 * s;
           if constexpr (S::kBytes) {
+            uint32_t v[4][VW];
+            unrolled<4>([&](auto h_tag) {
+              constexpr int h = decltype(h_tag)::value;
+              constexpr int kLine = kRow == 64 ? 64 : 128, kAt = s * 16 * kRow + (8 * (h >> 1) + (h & 1)) * kLine;
+              if constexpr (kRow == 64) {
+                const uint2 w = lds8<kAt>(v_even);
+                v[h][0] = w.x;
+                v[h][1] = w.y;
+              } else {
+                const uint4 w = lds16<kAt>(h & 1 ? v_odd : v_even);
+                v[h][0] = w.x;
+                v[h][1] = w.y;
+                v[h][2] = w.z;
+                v[h][3] = w.w;
+              }
+              if (tail && 2 * c + (h & 1) + 8 * (h >> 1) >= left) {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) v[h][i] = 0;
+              }
+            });
 #pragma unroll
             for (int i = 0; i < VW; ++i) {  // four dimensions
               uint32_t a[2][4];
-              codes4<STORE>(__byte_perm(v[s][0][i], v[s][1][i], 0x5140), a[0][0], a[0][1]);
-              codes4<STORE>(__byte_perm(v[s][2][i], v[s][3][i], 0x5140), a[0][2], a[0][3]);
-              codes4<STORE>(__byte_perm(v[s][0][i], v[s][1][i], 0x7362), a[1][0], a[1][1]);
-              codes4<STORE>(__byte_perm(v[s][2][i], v[s][3][i], 0x7362), a[1][2], a[1][3]);
+              codes4<STORE>(__byte_perm(v[0][i], v[1][i], 0x5140), a[0][0], a[0][1]);
+              codes4<STORE>(__byte_perm(v[2][i], v[3][i], 0x5140), a[0][2], a[0][3]);
+              codes4<STORE>(__byte_perm(v[0][i], v[1][i], 0x7362), a[1][0], a[1][1]);
+              codes4<STORE>(__byte_perm(v[2][i], v[3][i], 0x7362), a[1][2], a[1][3]);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], hi_[n][0], hi_[n][1]);
-                  mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], lo_[n][0], lo_[n][1]);
-                }
+                for (int n = 0; n < NT; ++n) mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], hi_[n][0], hi_[n][1]);
             }
           } else {
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {  // two dimensions
-              const uint32_t a0 = __byte_perm(v[s][0][i], v[s][1][i], 0x5410), a1 = __byte_perm(v[s][0][i], v[s][1][i], 0x7632);
-              const uint32_t a2 = __byte_perm(v[s][2][i], v[s][3][i], 0x5410), a3 = __byte_perm(v[s][2][i], v[s][3][i], 0x7632);
+            const uint32_t mask0 = (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
+            const uint32_t mask1 = (2 * c + 8 < left ? 0xffffu : 0u) | (2 * c + 9 < left ? 0xffff0000u : 0u);
+            unrolled<MT>([&](auto j_tag) {
+              constexpr int j = decltype(j_tag)::value;
+              uint32_t a[4];
+              ldmatrix4_trans<s * 16 * kRow + (j >> 2) * 2048>(a, v_even ^ (32 * (j & 3)));
+              if (tail) {
+                a[0] &= mask0;
+                a[1] &= mask0;
+                a[2] &= mask1;
+                a[3] &= mask1;
+              }
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma<BF>(o[i][n], a0, a1, a2, a3, hi_[n][0], hi_[n][1]);
-                mma<BF>(o[i][n], a0, a1, a2, a3, lo_[n][0], lo_[n][1]);
+                mma<BF>(o[j][n], a[0], a[1], a[2], a[3], hi_[n][0], hi_[n][1]);
+                mma<BF>(o[j][n], a[0], a[1], a[2], a[3], lo_[n][0], lo_[n][1]);
               }
-            }
+            });
           }
-        }
+        });
+        leave_entry(AfterValues());
         next(now);
       }
       // ---- leaving the item
       seen_bad |= bad;
       const bool whole = item_lo >= lo && item_hi <= hi;
-      const int slot = warp * 2 + (item_lo <= lo ? 0 : 1);
-      float* mine = slots + slot * S::kSlotFloats;
+      const int part_slot = warp * 2 + (item_lo <= lo ? 0 : 1);
+      float* mine = slot_at(part_slot);
+      float f[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float sum = bad ? NAN : sum_over_keys(l[n][r]);
           const int row = n * 8 + 2 * c + r;
-          const float f = (whole ? 1.f / sum : 1.f) / unit[n][r];
-#pragma unroll
-          for (int j = 0; j < MT; j += 4) {
-            float d[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              d[2 * i] = o[j + i][n][r] * f;
-              d[2 * i + 1] = o[j + i][n][r + 2] * f;
-            }
-            if (whole) {
-              if (row < rows) write_row(b, head, rt * R + row, dim_of(j), d);
-            } else {
-              float4* at = reinterpret_cast<float4*>(mine + row * S::kPitch + dim_of(j));
-              at[0] = make_float4(d[0], d[1], d[2], d[3]);
-              at[1] = make_float4(d[4], d[5], d[6], d[7]);
-            }
-          }
+          f[n][r] = (whole ? 1.f / sum : 1.f) / unit[n][r];
           if (g == 0) {
             if (whole) {
               if (row < rows) write_lse(b, head, rt * R + row, m[n][r], sum);
@@ -597,56 +725,82 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
             }
           }
         }
-      if (!whole && lane == 0) {
-        seg_item[slot] = (b * p.kv_heads + head) * p.row_tiles + rt;
-        seg_lo[slot] = item_lo;
-        seg_hi[slot] = item_hi;
+      if (whole) {  // outputs in pairs of dimensions of a row: those of 16-bit values by a transposition
+        uint16_t* out = static_cast<uint16_t*>(p.Out) + ((int64_t)b * p.heads + (int64_t)head * p.group + rt * R) * D;
+        auto pack = [&](float x, float y) { return p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y); };
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if constexpr (S::kBytes) {
+                const int row = n * 8 + 2 * c + h;
+                const uint32_t w = pack(o[j][n][h] * f[n][h], o[j][n][h + 2] * f[n][h]);
+                if (row < rows) *reinterpret_cast<uint32_t*>(out + row * D + pair_of(j)) = w;
+              } else {
+                const int row = n * 8 + g;
+                const uint32_t w = transposed(pack(o[j][n][2 * h] * f[n][0], o[j][n][2 * h + 1] * f[n][1]));
+                if (row < rows) *reinterpret_cast<uint32_t*>(out + row * D + 16 * j + 8 * h + 2 * c) = w;
+              }
+            }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int dim = S::kBytes ? pair_of(j) + (e >> 1) : 16 * j + g + 8 * (e >> 1);
+              mine[(n * 8 + 2 * c + (e & 1)) * S::kPitch + dim] = o[j][n][e] * f[n][e & 1];
+            }
+        if (lane == 0) {
+          seg_item[part_slot] = (b * p.kv_heads + head) * p.row_tiles + rt;
+          seg_lo[part_slot] = item_lo;
+          seg_hi[part_slot] = item_hi;
+        }
       }
     }
     if (seen_bad && lane == 0) atomicMax(status, (int)DEV_BAD_INDEX);
   }
   __syncthreads();
 
-  // ---- items that several warps had
-  const unsigned cta_lo = range_of(blockIdx.x * kWarps), cta_hi = range_of((blockIdx.x + 1) * kWarps);
-  // The parts in slots [s0, s1) (those that are marked), added in ascending order: to the output, or to a part of the item in memory.
-  auto join = [&](int s0, int s1, int item, float* part) {
+  // The parts in slots [s0, s1) (those that are `marked`), added in ascending order: to the output, or to a part of the item in memory.
+  auto join = [&](int s0, int s1, auto marked, int item, float* part) {
     const int rt = item % p.row_tiles, pair = item / p.row_tiles, head = pair % p.kv_heads, b = pair / p.kv_heads;
     const int rows = min(R, p.group - rt * R);
-    for (int i = tid; i < rows * (D / 8); i += kThreads) {
-      const int row = i / (D / 8), d = (i - row * (D / 8)) * 8;
-      float M = -INFINITY, L = 0.f, acc[8] = {};
+    for (int i = tid; i < rows * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int s = s0; s < s1; ++s)
-        if (seg_item[s] >= 0) M = fmaxf(M, slots[s * S::kSlotFloats + R * S::kPitch + row]);
+        if (marked(s)) M = fmaxf(M, slot_at(s)[R * S::kPitch + row]);
       const float ref = from_minus_inf(M);
       for (int s = s0; s < s1; ++s) {
-        if (seg_item[s] < 0) continue;
-        const float* from = slots + s * S::kSlotFloats;
+        if (!marked(s)) continue;
+        const float* from = slot_at(s);
         const float f = ex2_approx_ftz(from[R * S::kPitch + row] - ref);
-        const float4 u = *reinterpret_cast<const float4*>(from + row * S::kPitch + d), w = *reinterpret_cast<const float4*>(from + row * S::kPitch + d + 4);
+        const float4 u = *reinterpret_cast<const float4*>(from + row * S::kPitch + d);
         L += from[R * S::kPitch + R + row] * f;
-        acc[0] += u.x * f; acc[1] += u.y * f; acc[2] += u.z * f; acc[3] += u.w * f;
-        acc[4] += w.x * f; acc[5] += w.y * f; acc[6] += w.z * f; acc[7] += w.w * f;
+        acc.x += u.x * f; acc.y += u.y * f; acc.z += u.z * f; acc.w += u.w * f;
       }
       if (part) {
-        float4* to = reinterpret_cast<float4*>(part + row * D + d);
-        to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        *reinterpret_cast<float4*>(part + row * D + d) = acc;
         if (d == 0) {
           part[R * D + row] = M;
           part[R * D + R + row] = L;
         }
       } else {
         const float inv = 1.f / L;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] *= inv;
-        write_row(b, head, rt * R + row, d, acc);
+        uint2 w;
+        if (p.q_bf16) w = make_uint2(pack2<true>(acc.x * inv, acc.y * inv), pack2<true>(acc.z * inv, acc.w * inv));
+        else w = make_uint2(pack2<false>(acc.x * inv, acc.y * inv), pack2<false>(acc.z * inv, acc.w * inv));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.Out) + ((int64_t)b * p.heads + (int64_t)head * p.group + rt * R + row) * D + d) = w;
         if (d == 0) write_lse(b, head, rt * R + row, M, L);
       }
     }
   };
-  int shared_item[2] = {-1, -1};  // of several CTAs: the first and the last of the range
-  unsigned shared_lo[2] = {}, shared_hi[2] = {};
+  int first_shared = -1, last_shared = -1;  // slots of the items that other CTAs have a part of: the first and the last of the range
   for (int s = 0; s < 2 * kWarps;) {
     const int item = seg_item[s];
     int z = s + 1;
@@ -654,71 +808,73 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1) fmha_paged_k
       while (z < 2 * kWarps && (seg_item[z] < 0 || seg_item[z] == item)) ++z;
       const bool inside = seg_lo[s] >= cta_lo && seg_hi[s] <= cta_hi;
       const int which = seg_lo[s] < cta_lo ? 0 : 1;
-      join(s, z, item, inside ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + which) * S::kPartFloats);
-      if (!inside) {
-        shared_item[which] = item;
-        shared_lo[which] = seg_lo[s];
-        shared_hi[which] = seg_hi[s];
-      }
+      join(s, z, [&](int i) { return seg_item[i] >= 0; }, item, inside ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + which) * S::kPartFloats);
+      if (!inside) (which ? last_shared : first_shared) = s;
     }
     s = z;
   }
-  if (shared_item[0] < 0 && shared_item[1] < 0) return;
+  if (first_shared < 0 && last_shared < 0) return;
+  auto cta_of = [&](unsigned x) { return (int)(worker_of(x, total, workers) / kWarps); };
   __syncthreads();
   if (tid < 2) {
     last_s[tid] = 0;
-    const int which = tid;
-    if (shared_item[which] >= 0) {
-      const unsigned c0 = worker_of(shared_lo[which], total, workers) / kWarps, c1 = worker_of(shared_hi[which] - 1, total, workers) / kWarps;
+    const int s = tid ? last_shared : first_shared;
+    if (s >= 0) {
+      const int c0 = cta_of(seg_lo[s]), parts = cta_of(seg_hi[s] - 1) - c0;
       __threadfence();
-      last_s[which] = atomicInc(&p.tickets[c0], c1 - c0) == c1 - c0;  // back to zero by the last
+      last_s[tid] = atomicInc(&p.tickets[c0], parts) == parts;  // back to zero by the last
       __threadfence();
     }
   }
   __syncthreads();
+  const bool last[2] = {last_s[0] != 0, last_s[1] != 0};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    if (!last_s[which]) continue;
-    // warp w takes the parts c0 + w, c0 + w + kWarps, ...; a lane has eight (D = 64: four) rows' share of the dimensions
-    const int c0 = worker_of(shared_lo[which], total, workers) / kWarps, c1 = worker_of(shared_hi[which] - 1, total, workers) / kWarps;
-    auto part_of = [&](int i) { return p.part + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * S::kPartFloats; };
-    constexpr int kVecs = R * D / 4 / 32;  // of a lane; vector i is number i * 32 + lane
+    if (!last[which]) continue;
+    const int s = which ? last_shared : first_shared, item = seg_item[s];
+    // warp w takes the parts c0 + w, c0 + w + kWarps, ...: vector i of a lane is number i * 32 + lane of the part's rows
+    const int c0 = cta_of(seg_lo[s]), c1 = cta_of(seg_hi[s] - 1), rows = min(R, p.group - item % p.row_tiles * R);
+    constexpr int kVecs = R * D / 4 / 32;
     const int row = lane & (R - 1);
     float M = -INFINITY, L = 0.f;
-    for (int i = c0 + warp; i <= c1; i += kWarps) M = fmaxf(M, __ldcg(part_of(i) + R * D + row));
-    const float ref = from_minus_inf(M);
     float4 acc[kVecs];
 #pragma unroll
     for (int e = 0; e < kVecs; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int rows = min(R, p.group - shared_item[which] % p.row_tiles * R);
+#pragma unroll 2
     for (int i = c0 + warp; i <= c1; i += kWarps) {
-      const float* from = part_of(i);
-      const float f = ex2_approx_ftz(__ldcg(from + R * D + row) - ref);
-      L += __ldcg(from + R * D + R + row) * f;
+      const float* from = p.part + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * S::kPartFloats;
+      float4 u[kVecs];
+#pragma unroll
+      for (int e = 0; e < kVecs; ++e) u[e] = __ldcg(reinterpret_cast<const float4*>(from) + e * 32 + lane);
+      const float m = __ldcg(from + R * D + row), l = __ldcg(from + R * D + R + row);
+      const float top = fmaxf(M, m), ref = from_minus_inf(top), old = ex2_approx_ftz(M - ref), f = ex2_approx_ftz(m - ref);
+      M = top;
+      L = L * old + l * f;
 #pragma unroll
       for (int e = 0; e < kVecs; ++e) {
-        const int at = e * 32 + lane, r = at / (D / 4);
-        const float fr = __shfl_sync(0xffffffffu, f, r);
-        if (r < rows) {
-          const float4 u = __ldcg(reinterpret_cast<const float4*>(from) + at);
-          acc[e].x += u.x * fr; acc[e].y += u.y * fr; acc[e].z += u.z * fr; acc[e].w += u.w * fr;
+        const int r = (e * 32 + lane) / (D / 4);
+        const float fr = __shfl_sync(0xffffffffu, f, r), of = __shfl_sync(0xffffffffu, old, r);
+        if (r < rows) {  // rows behind the group's last are not written
+          acc[e].x = acc[e].x * of + u[e].x * fr;
+          acc[e].y = acc[e].y * of + u[e].y * fr;
+          acc[e].z = acc[e].z * of + u[e].z * fr;
+          acc[e].w = acc[e].w * of + u[e].w * fr;
         }
       }
     }
     __syncthreads();  // the slots are free
-    float* mine = slots + warp * S::kSlotFloats;
+    float* to = slot_at(2 * warp);
 #pragma unroll
     for (int e = 0; e < kVecs; ++e) {
       const int at = e * 32 + lane, r = at / (D / 4);
-      *reinterpret_cast<float4*>(mine + r * S::kPitch + (at - r * (D / 4)) * 4) = acc[e];
+      *reinterpret_cast<float4*>(to + r * S::kPitch + (at - r * (D / 4)) * 4) = acc[e];
     }
     if (lane < R) {
-      mine[R * S::kPitch + lane] = M;
-      mine[R * S::kPitch + R + lane] = L;
+      to[R * S::kPitch + lane] = M;
+      to[R * S::kPitch + R + lane] = L;
     }
-    if (tid < 2 * kWarps) seg_item[tid] = tid < kWarps ? 0 : -1;
     __syncthreads();
-    join(0, kWarps, shared_item[which], nullptr);
+    join(0, 2 * kWarps, [](int s) { return (s & 1) == 0; }, item, nullptr);
   }
 }
 

@@ -300,8 +300,8 @@ int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, void* k_out
 
 /* ---- Paged key-value cache -------------------------------------------------------- */
 /* (No counterpart in the reference.)  Keys and values of sequences in pages of page_size tokens (a power of two from 16 to 1024):
- * k and v (head_dim, page_size, kv_heads, pages), dense but for the strides from page to page (elements, multiples of 16 bytes), 16-byte
- * aligned; head_dim 64 or 128.  dtype CTB_F16 or CTB_BF16, or 8 bits with a scale per token and head in k_scale and v_scale
+ * k and v (head_dim, page_size, kv_heads, pages), dense but for the strides from page to page (elements); head_dim 64 or 128; all
+ * pages begin on 16 bytes.  dtype CTB_F16 or CTB_BF16, or 8 bits with a scale per token and head in k_scale and v_scale
  * (page_size, kv_heads, pages) f32: CTB_I8 (codes -127..127) and CTB_E4M3 (up to 448); the value is code * scale.  A page of a
  * sequence is named by its 1-based number in a page table (table_width, batch) int32 (0: none); lengths (batch) int32 says how
  * many tokens a sequence has.  A token's slot is its 1-based place in the whole cache, (page - 1) * page_size + place in the page + 1. */
@@ -333,7 +333,8 @@ int ctb_kv_read(ctb_ctx* ctx, void* stream, void* K, void* V, const ctb_kv_cache
  * heads, batch) in the type of Q and lse (heads, batch) f32, dense.  heads is a multiple of kv_heads, and head h has the keys of
  * h / (heads / kv_heads).  A length of 0 gives zeros and -inf; bad lengths and pages as above make the sequence's (for a page, the
  * heads') results NaN.  What the cache holds behind a sequence's length does not matter.  Scores, sums and outputs are f32,
- * probabilities enter the product with values as the sum of two 16-bit numbers.  Bitwise repeatable. */
+ * probabilities enter the product with 16-bit values as the sum of two 16-bit numbers, with 8-bit codes (times the values' scales)
+ * as one f16.  Bitwise repeatable. */
 int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse, const void* Q, const ctb_kv_cache* cache,
                    const int32_t* page_table, const int32_t* lengths, int64_t batch, int64_t heads, int64_t q_seq_stride,
                    int64_t q_head_stride, int64_t table_width, int64_t table_stride, float qk_scale, int dtype);
