@@ -252,14 +252,12 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       for (int i = tid; i < p.heads; i += kThreads) p.lse[(int64_t)b * p.heads + i] = wrong ? NAN : -INFINITY;
   }
   if (total == 0) return;
-  auto sequence_of = [&](unsigned x) {  // that has tile x: the last one that begins at or before it
-    int a = 0, z = p.batch - 1;
-    while (a < z) {
-      const int mid = (a + z + 1) >> 1;
-      if (prefix[mid] <= x) a = mid;
-      else z = mid - 1;
-    }
-    return a;
+  // The sequence that has tile x: the last one that begins at or before it.  All lanes of a warp ask together.
+  auto sequence_of = [&](unsigned x) {
+    const int stride = (p.batch + 31) / 32;
+    auto count = [&](int at, int end) { return __popc(__ballot_sync(0xffffffffu, at < end && prefix[at] <= x)); };
+    const int start = (count(lane * stride, p.batch) - 1) * stride;
+    return start + count(start + lane, min(start + stride, p.batch)) - 1;
   };
   // Ranges of the line of tiles: equal ones for all warps of the grid, or, where items are short, for the warps of a CTA, whose range
   // ends where an item ends.
@@ -312,72 +310,67 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     return t;
   };
   if (lo < hi) {
-    const int page_mask = (1 << p.page_log2) - 1;
     Cursor now = cursor_at(lo);  // the tile at hand
-    // Tiles are asked for ahead of it: keys and values in turn, an entry of the warp's ring each; the numbers of their pages are read
-    // two tiles before that.
-    Cursor ahead = now, numbers = now;
-    unsigned ahead_x = lo, numbers_x = lo;
+    // Tiles are asked for ahead of it: keys and values in turn, an entry of the warp's ring each.  A tile's groups of 16 keys are shared
+    // out over the lanes; the number of a lane's page is read two tiles before that: (number, row in the page, -1 behind the last key).
+    constexpr int kLanes = 32 / KT;  // of a group
+    const int mine = lane / kLanes * 16;
+    Cursor ahead = now;
+    unsigned ahead_x = lo, asked_x = lo;
+    int id[3] = {}, row[3] = {};
     uint32_t bad_pages = 0;  // a bit per tile that has been asked for
     bool seen_bad = false;
-    int id[3][KT] = {};
-    auto more_ids = [&](int (&to)[KT]) {
-      if (numbers_x >= hi) return;
-      const int32_t* row = p.table + (int64_t)numbers.b * p.table_ld;
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const int key = numbers.key + 16 * s;
-        to[s] = key < numbers.len ? __ldg(row + (key >> p.page_log2)) : 0;
+    auto look_ahead = [&](int& to_id, int& to_row) {
+      if (ahead_x >= hi) return;
+      const int key = ahead.key + mine;
+      to_id = to_row = -1;
+      if (key < ahead.len) {
+        to_id = __ldg(p.table + ahead.b * p.table_ld + (key >> p.page_log2));
+        to_row = (ahead.head << p.page_log2) + (key & ((1 << p.page_log2) - 1));
       }
-      if (++numbers_x < hi) next(numbers);
+      if (++ahead_x < hi) next(ahead);
     };
 #pragma unroll
-    for (int i = 0; i < 3; ++i) more_ids(id[i]);
+    for (int i = 0; i < 3; ++i) look_ahead(id[i], row[i]);
 
     const uint32_t ring = smem_u32(smem) + warp * (kRing * S::kEntry);
     float* scales = all_scales + warp * (kRing * S::kScales);
     int put = 0, slot = 0;
-    // Where a lane's 16 bytes of 512 go: rows in 128-byte lines whose chunks are exchanged by the line's number (in 64-byte rows by that
-    // of every second one); lines of 256-byte rows' second halves behind those of the first of 16 rows.
+    // Where a lane's 16 bytes go: rows in 128-byte lines whose chunks are exchanged by the line's number (in 64-byte rows by that of every
+    // second one); the second halves of 256-byte rows in lines behind those of the first.
+    const int l = lane % kLanes;
     const uint32_t to = kRow == 256   ? ((lane >> 3) & 1) * 2048 + (lane >> 4) * 128 + ((lane & 7) ^ (lane >> 4)) * 16
-                        : kRow == 128 ? (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16
-                                      : (lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
+                        : kRow == 128 ? (lane >> 4) * 2048 + (l >> 3) * 128 + ((l & 7) ^ (l >> 3)) * 16
+                                      : (lane >> 3) * 1024 + l * 16;
     auto ask = [&](auto values) {
       constexpr bool V = decltype(values)::value;
-      if (ahead_x < hi) {
-        const uint32_t dst = ring + put * S::kEntry + to;
-        bool wrong = false;
-        unrolled<KT>([&](auto s_tag) {
-          constexpr int s = decltype(s_tag)::value;
-          const int key = ahead.key + 16 * s;
-          if (KT == 1 || key < ahead.len) {
-            const bool good = (unsigned)(id[0][s] - 1) < (unsigned)p.pages;
-            wrong |= !good;
-            const int64_t page = good ? id[0][s] - 1 : 0;  // the first one where there is none
-            const int row = (ahead.head << p.page_log2) + (key & page_mask);
-            const char* src = static_cast<const char*>(V ? p.V : p.K) + (page * (V ? p.v_page : p.k_page) + (int64_t)row * D) * (S::kBytes ? 1 : 2) + lane * 16;
-            unrolled<8 / KT>([&](auto i_tag) {
-              constexpr int i = decltype(i_tag)::value;
-              constexpr int kFlip = kRow == 256 ? 32 * (i & 3) : kRow == 128 ? 64 * (i & 1) : 0, kRows = 512 / kRow * i;
-              copy16<i * 512, s * 16 * kRow + kRows * (kRow == 64 ? 64 : 128)>(dst ^ kFlip, src);
-            });
-            if constexpr (S::kBytes) {
-              const float* from = (V ? p.Vs + page * p.vs_page : p.Ks + page * p.ks_page) + row + (lane & 15);
-              if (lane < 16) copy4(smem_u32(scales + put * S::kScales + 16 * s + lane), from);
-            }
-          }
-        });
-        if constexpr (!V) {
-          const uint32_t bit = 1u << (ahead_x & 31);
-          bad_pages = wrong ? bad_pages | bit : bad_pages & ~bit;
-        } else {
-          if (++ahead_x < hi) next(ahead);
+      if (asked_x < hi) {
+        const bool good = (unsigned)(id[0] - 1) < (unsigned)p.pages;
+        const int64_t page = good ? id[0] - 1 : 0;  // the first one where there is none
+        if (KT == 1 || row[0] >= 0) {
+          const uint32_t dst = ring + put * S::kEntry + to;
+          const char* src = static_cast<const char*>(V ? p.V : p.K) + (page * (V ? p.v_page : p.k_page) + (int64_t)row[0] * D) * (S::kBytes ? 1 : 2) + l * 16;
+          unrolled<8>([&](auto i_tag) {
+            constexpr int i = decltype(i_tag)::value;
+            copy16<i * 512 / KT, i * (kRow == 64 ? 128 : 256)>(dst ^ ((kRow == 64 ? 16 : 32) * (i & 3)), src);
+          });
+          if constexpr (S::kBytes) {
+            const float* from = (V ? p.Vs + page * p.vs_page : p.Ks + page * p.ks_page) + row[0] + l;
+            const uint32_t s_dst = smem_u32(scales + put * S::kScales + mine + l);
 #pragma unroll
-          for (int s = 0; s < KT; ++s) {
-            id[0][s] = id[1][s];
-            id[1][s] = id[2][s];
+            for (int i = 0; i < 16; i += kLanes) copy4(s_dst + 4 * i, from + i);
           }
-          more_ids(id[2]);
+        }
+        if constexpr (!V) {
+          const bool wrong = __any_sync(0xffffffffu, row[0] >= 0 && !good);
+          bad_pages = (bad_pages & ~(1u << (asked_x & 31))) | ((uint32_t)wrong << (asked_x & 31));
+        } else {
+          ++asked_x;
+          id[0] = id[1];
+          id[1] = id[2];
+          row[0] = row[1];
+          row[1] = row[2];
+          look_ahead(id[2], row[2]);
         }
       }
       copies_commit();
@@ -472,7 +465,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-      for (; x < end; ++x) {
+      auto tile = [&](auto tail_tag) {  // TAIL: some of its keys are behind the last one
+        constexpr bool tail = decltype(tail_tag)::value;
         copies_wait<kRing - 1>();
         bad |= (bad_pages >> (x & 31)) & 1;
         float sc[KT][NT][4], ks[KT][2];
@@ -520,7 +514,6 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         });
         leave_entry(AfterKeys());
         // ---- Scores in powers of two: e = 0, 1: key g, rows 2c, 2c + 1; e = 2, 3: key g + 8.  d is their distance from the reference.
-        const bool tail = now.key + kTileKeys > len;
         auto hidden = [&](int s, int e) { return tail && now.key + 16 * s + g + 8 * (e >> 1) >= len; };
         auto times = [&](int s, int n, int e) {
           if constexpr (S::kBytes) return mult[n][e & 1] * ks[s][e >> 1];
@@ -701,8 +694,14 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
           }
         });
         leave_entry(AfterValues());
-        next(now);
+      };
+      for (; x < end; ++x) {
+        if (now.key + kTileKeys <= len) tile(std::false_type());
+        else tile(std::true_type());
+        now.key += kTileKeys;
       }
+      now.key -= kTileKeys;
+      next(now);
       // ---- leaving the item
       seen_bad |= bad;
       const bool whole = item_lo >= lo && item_hi <= hi;
