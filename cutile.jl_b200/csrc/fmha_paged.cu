@@ -161,13 +161,16 @@ __device__ __forceinline__ float sum_over_keys(float v) {
 }
 __device__ __forceinline__ float from_minus_inf(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Range of a worker among `workers` that share out `n` tiles, and the worker that has tile x.
-__device__ __forceinline__ unsigned first_tile(unsigned w, unsigned n, unsigned workers) {
-  return (unsigned)((unsigned long long)w * n / workers);
-}
-__device__ __forceinline__ unsigned worker_of(unsigned x, unsigned n, unsigned workers) {
-  return (unsigned)((((unsigned long long)x + 1) * workers - 1) / n);
-}
+// `n` tiles shared out among `workers`: the first ones have one more.
+struct Shares {
+  unsigned least, more;
+  __device__ __forceinline__ Shares(unsigned n, unsigned workers) : least(n / workers), more(n - least * workers) {}
+  __device__ __forceinline__ unsigned first(unsigned w) const { return w * least + min(w, more); }
+  __device__ __forceinline__ unsigned owner(unsigned x) const {  // of tile x
+    const unsigned large = more * (least + 1);
+    return x < large ? x / (least + 1) : more + (x - large) / least;
+  }
+};
 
 // A tile: the sequence, the row of heads, and the keys.
 struct Cursor {
@@ -189,8 +192,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   float* firsts = all_scales + kWarps * kRing * S::kScales;
   int* lens = reinterpret_cast<int*>(firsts + kWarps * S::kSlotFloats);
   unsigned* prefix = reinterpret_cast<unsigned*>(lens + kMaxBatch);
-  __shared__ unsigned warp_sum[kWarps], warp_most[kWarps], seg_lo[2 * kWarps], seg_hi[2 * kWarps];
-  __shared__ int seg_item[2 * kWarps];
+  __shared__ unsigned warp_sum[kWarps], warp_most[kWarps];
+  __shared__ uint4 segs[2 * kWarps];  // parts of items: first output row of the item (-1: no part), its live rows, its first tile, its last one's end
   __shared__ int last_s[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   // Results of a warp's part of an item: of the first item of its range beside the ring, of the last one in the ring, which is empty by then.
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       warp_sum[warp] = up;
       warp_most[warp] = top;
     }
-    if (tid < 2 * kWarps) seg_item[tid] = -1;
+    if (tid < 2 * kWarps) segs[tid].x = ~0u;
     __syncthreads();
     unsigned before = up - sum;
     longest = 0;
@@ -262,12 +265,11 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   // Ranges of the line of tiles: equal ones for all warps of the grid, or, where items are short, for the warps of a CTA, whose range
   // ends where an item ends.
   const bool whole_items = longest <= kWholeItems;
-  const unsigned all = gridDim.x * kWarps, workers = min(all, (total + kMinTiles - 1) / kMinTiles);
-  auto range_of = [&](unsigned w) { return first_tile(min(w, workers), total, workers); };
+  const Shares shares(total, whole_items ? gridDim.x : min(gridDim.x * kWarps, (total + kMinTiles - 1) / kMinTiles));
   unsigned cta_lo, cta_hi, lo, hi;
   if (whole_items) {
     auto end_of = [&](unsigned i) {  // the end of an item that is next to the end of an equal range
-      const unsigned x = first_tile(i, total, gridDim.x);
+      const unsigned x = shares.first(i);
       if (x >= total) return total;
       const int b = sequence_of(x);
       const unsigned tiles = (unsigned)(lens[b] + kTileKeys - 1) / kTileKeys;
@@ -275,19 +277,21 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     };
     cta_lo = end_of(blockIdx.x);
     cta_hi = end_of(blockIdx.x + 1);
-    lo = cta_lo + first_tile(warp, cta_hi - cta_lo, kWarps);
-    hi = cta_lo + first_tile(warp + 1, cta_hi - cta_lo, kWarps);
+    const unsigned n = cta_hi - cta_lo;
+    lo = cta_lo + warp * n / kWarps;
+    hi = cta_lo + (warp + 1) * n / kWarps;
   } else {
+    auto range_of = [&](unsigned w) { return min(shares.first(w), total); };
     cta_lo = range_of(blockIdx.x * kWarps);
     cta_hi = range_of((blockIdx.x + 1) * kWarps);
     lo = range_of(blockIdx.x * kWarps + warp);
     hi = range_of(blockIdx.x * kWarps + warp + 1);
   }
 
-  auto write_lse = [&](int b, int head, int row, float m, float l) {
-    if (p.lse) p.lse[(int64_t)b * p.heads + (int64_t)head * p.group + row] = (m + log2f(l)) * 0.6931471805599453f;
+  auto write_lse = [&](int at, float m, float l) {
+    if (p.lse) p.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
   };
-
+  auto pack = [&](float x, float y) { return p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y); };
   auto next = [&](Cursor& t) {
     t.key += kTileKeys;
     if (t.key < t.len) return;
@@ -469,7 +473,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         constexpr bool tail = decltype(tail_tag)::value;
         copies_wait<kRing - 1>();
         bad |= (bad_pages >> (x & 31)) & 1;
-        float sc[KT][NT][4], ks[KT][2];
+        float sc[KT][NT][4];
+        [[maybe_unused]] float ks[KT][2];
         const uint32_t k_even = ring + slot * S::kEntry + k_at, k_odd = k_even ^ 16;
         if constexpr (S::kBytes) {
 #pragma unroll
@@ -620,7 +625,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
           }
         }
         // ---- O += V P.  Probabilities are the sum of two 16-bit numbers beside 16-bit values, one f16 beside 8-bit ones.
-        const uint32_t v_even = ring + slot * S::kEntry + v_at, v_odd = v_even ^ 16;
+        const uint32_t v_even = ring + slot * S::kEntry + v_at;
+        [[maybe_unused]] const uint32_t v_odd = v_even ^ 16;
         unrolled<KT>([&](auto tag) {
           constexpr int s = decltype(tag)::value;
           uint32_t hi_[NT][2];
@@ -707,6 +713,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       const bool whole = item_lo >= lo && item_hi <= hi;
       const int part_slot = warp * 2 + (item_lo <= lo ? 0 : 1);
       float* mine = slot_at(part_slot);
+      const int out_row = b * p.heads + head * p.group + rt * R;
       float f[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -717,7 +724,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
           f[n][r] = (whole ? 1.f / sum : 1.f) / unit[n][r];
           if (g == 0) {
             if (whole) {
-              if (row < rows) write_lse(b, head, rt * R + row, m[n][r], sum);
+              if (row < rows) write_lse(out_row + row, m[n][r], sum);
             } else {
               mine[R * S::kPitch + row] = m[n][r];
               mine[R * S::kPitch + R + row] = sum;
@@ -725,8 +732,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
           }
         }
       if (whole) {  // outputs in pairs of dimensions of a row: those of 16-bit values by a transposition
-        uint16_t* out = static_cast<uint16_t*>(p.Out) + ((int64_t)b * p.heads + (int64_t)head * p.group + rt * R) * D;
-        auto pack = [&](float x, float y) { return p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y); };
+        uint16_t* out = static_cast<uint16_t*>(p.Out) + (int64_t)out_row * D;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -753,73 +759,83 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
               const int dim = S::kBytes ? pair_of(j) + (e >> 1) : 16 * j + g + 8 * (e >> 1);
               mine[(n * 8 + 2 * c + (e & 1)) * S::kPitch + dim] = o[j][n][e] * f[n][e & 1];
             }
-        if (lane == 0) {
-          seg_item[part_slot] = (b * p.kv_heads + head) * p.row_tiles + rt;
-          seg_lo[part_slot] = item_lo;
-          seg_hi[part_slot] = item_hi;
-        }
+        if (lane == 0) segs[part_slot] = make_uint4(out_row, min(rows, R), item_lo, item_hi);
       }
     }
     if (seen_bad && lane == 0) atomicMax(status, (int)DEV_BAD_INDEX);
   }
   __syncthreads();
 
-  // The parts in slots [s0, s1) (those that are `marked`), added in ascending order: to the output, or to a part of the item in memory.
-  auto join = [&](int s0, int s1, auto marked, int item, float* part) {
-    const int rt = item % p.row_tiles, pair = item / p.row_tiles, head = pair % p.kv_heads, b = pair / p.kv_heads;
-    const int rows = min(R, p.group - rt * R);
-    for (int i = tid; i < rows * (D / 4); i += kThreads) {
-      const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-      float M = -INFINITY, L = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int s = s0; s < s1; ++s)
-        if (marked(s)) M = fmaxf(M, slot_at(s)[R * S::kPitch + row]);
-      const float ref = from_minus_inf(M);
-      for (int s = s0; s < s1; ++s) {
-        if (!marked(s)) continue;
-        const float* from = slot_at(s);
-        const float f = ex2_approx_ftz(from[R * S::kPitch + row] - ref);
-        const float4 u = *reinterpret_cast<const float4*>(from + row * S::kPitch + d);
-        L += from[R * S::kPitch + R + row] * f;
-        acc.x += u.x * f; acc.y += u.y * f; acc.z += u.z * f; acc.w += u.w * f;
-      }
-      if (part) {
-        *reinterpret_cast<float4*>(part + row * D + d) = acc;
-        if (d == 0) {
-          part[R * D + row] = M;
-          part[R * D + R + row] = L;
-        }
+  // ---- Items that several warps had.  A lane looks at a slot; neighbouring parts of one item are joined.
+  constexpr int kEach = D / 32;  // dimensions of a lane
+  static_assert(2 * kWarps <= 32, "a lane per slot");
+  // One row of the parts in the slots of `members`, in ascending order: to the output, or to a part of the item in memory.
+  auto join_row = [&](uint32_t members, int out_row, int row, float* part) {
+    const bool member = (members >> lane) & 1;
+    const float* stats = slot_at(member ? lane : 0) + R * S::kPitch + row;
+    const float m = member ? stats[0] : -INFINITY;
+    float M = m, L = member ? stats[R] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float f = ex2_approx_ftz(m - from_minus_inf(M));
+    L *= f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    float acc[kEach] = {};
+#pragma unroll 4
+    for (uint32_t left = members; left; left &= left - 1) {
+      const int s = __ffs(left) - 1;
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      const float* from = slot_at(s) + row * S::kPitch + lane * kEach;
+      if constexpr (kEach == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(from);
+        acc[0] += u.x * fs; acc[1] += u.y * fs; acc[2] += u.z * fs; acc[3] += u.w * fs;
       } else {
-        const float inv = 1.f / L;
-        uint2 w;
-        if (p.q_bf16) w = make_uint2(pack2<true>(acc.x * inv, acc.y * inv), pack2<true>(acc.z * inv, acc.w * inv));
-        else w = make_uint2(pack2<false>(acc.x * inv, acc.y * inv), pack2<false>(acc.z * inv, acc.w * inv));
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.Out) + ((int64_t)b * p.heads + (int64_t)head * p.group + rt * R + row) * D + d) = w;
-        if (d == 0) write_lse(b, head, rt * R + row, M, L);
+        const float2 u = *reinterpret_cast<const float2*>(from);
+        acc[0] += u.x * fs; acc[1] += u.y * fs;
       }
+    }
+    if (part) {
+#pragma unroll
+      for (int i = 0; i < kEach; i += 2) *reinterpret_cast<float2*>(part + row * D + lane * kEach + i) = make_float2(acc[i], acc[i + 1]);
+      if (lane == 0) {
+        part[R * D + row] = M;
+        part[R * D + R + row] = L;
+      }
+    } else {
+      const float inv = 1.f / L;
+      uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.Out) + (int64_t)(out_row + row) * D + lane * kEach);
+      if constexpr (kEach == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack(acc[0] * inv, acc[1] * inv), pack(acc[2] * inv, acc[3] * inv));
+      else *out = pack(acc[0] * inv, acc[1] * inv);
+      if (lane == 0) write_lse(out_row + row, M, L);
     }
   };
-  int first_shared = -1, last_shared = -1;  // slots of the items that other CTAs have a part of: the first and the last of the range
-  for (int s = 0; s < 2 * kWarps;) {
-    const int item = seg_item[s];
-    int z = s + 1;
-    if (item >= 0) {
-      while (z < 2 * kWarps && (seg_item[z] < 0 || seg_item[z] == item)) ++z;
-      const bool inside = seg_lo[s] >= cta_lo && seg_hi[s] <= cta_hi;
-      const int which = seg_lo[s] < cta_lo ? 0 : 1;
-      join(s, z, [&](int i) { return seg_item[i] >= 0; }, item, inside ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + which) * S::kPartFloats);
-      if (!inside) (which ? last_shared : first_shared) = s;
-    }
-    s = z;
+  const uint4 seg = lane < 2 * kWarps ? segs[lane] : make_uint4(~0u, 0, 0, 0);
+  const uint32_t marked = __ballot_sync(0xffffffffu, seg.x != ~0u), below = marked & ((1u << lane) - 1);
+  const uint32_t item_below = __shfl_sync(0xffffffffu, seg.x, below ? 31 - __clz(below) : 0);
+  uint32_t leaders = __ballot_sync(0xffffffffu, seg.x != ~0u && (!below || item_below != seg.x));
+  uint4 shared_item[2] = {make_uint4(~0u, 0, 0, 0), make_uint4(~0u, 0, 0, 0)};  // that other CTAs have a part of: the first and the last of the range
+  for (int task = 0; leaders; leaders &= leaders - 1) {
+    const int s = __ffs(leaders) - 1;
+    const uint32_t later = leaders & (leaders - 1), members = marked & ~((1u << s) - 1) & (later ? (later & -later) - 1 : ~0u);
+    const uint4 item = make_uint4(__shfl_sync(0xffffffffu, seg.x, s), __shfl_sync(0xffffffffu, seg.y, s), __shfl_sync(0xffffffffu, seg.z, s),
+                                  __shfl_sync(0xffffffffu, seg.w, s));
+    const bool inside = item.z >= cta_lo && item.w <= cta_hi;
+    const int which = item.z < cta_lo ? 0 : 1;
+    if (!inside) shared_item[which] = item;
+    float* part = inside ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + which) * S::kPartFloats;
+    for (int row = (warp + kWarps - task % kWarps) % kWarps; row < (int)item.y; row += kWarps) join_row(members, item.x, row, part);
+    task += item.y;
   }
-  if (first_shared < 0 && last_shared < 0) return;
-  auto cta_of = [&](unsigned x) { return (int)(worker_of(x, total, workers) / kWarps); };
+  if (shared_item[0].x == ~0u && shared_item[1].x == ~0u) return;
+  // ---- Items that several CTAs had: the one that is done last adds the parts.
+  auto cta_of = [&](unsigned x) { return (int)(shares.owner(x) / kWarps); };
   __syncthreads();
   if (tid < 2) {
     last_s[tid] = 0;
-    const int s = tid ? last_shared : first_shared;
-    if (s >= 0) {
-      const int c0 = cta_of(seg_lo[s]), parts = cta_of(seg_hi[s] - 1) - c0;
+    const uint4 item = tid ? shared_item[1] : shared_item[0];
+    if (item.x != ~0u) {
+      const int c0 = cta_of(item.z), parts = cta_of(item.w - 1) - c0;
       __threadfence();
       last_s[tid] = atomicInc(&p.tickets[c0], parts) == parts;  // back to zero by the last
       __threadfence();
@@ -830,22 +846,23 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (!last[which]) continue;
-    const int s = which ? last_shared : first_shared, item = seg_item[s];
+    const uint4 item = shared_item[which];
     // warp w takes the parts c0 + w, c0 + w + kWarps, ...: vector i of a lane is number i * 32 + lane of the part's rows
-    const int c0 = cta_of(seg_lo[s]), c1 = cta_of(seg_hi[s] - 1), rows = min(R, p.group - item % p.row_tiles * R);
+    const int c0 = cta_of(item.z), c1 = cta_of(item.w - 1), rows = item.y;
     constexpr int kVecs = R * D / 4 / 32;
     const int row = lane & (R - 1);
     float M = -INFINITY, L = 0.f;
     float4 acc[kVecs];
 #pragma unroll
     for (int e = 0; e < kVecs; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
     for (int i = c0 + warp; i <= c1; i += kWarps) {
       const float* from = p.part + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * S::kPartFloats;
       float4 u[kVecs];
 #pragma unroll
-      for (int e = 0; e < kVecs; ++e) u[e] = __ldcg(reinterpret_cast<const float4*>(from) + e * 32 + lane);
-      const float m = __ldcg(from + R * D + row), l = __ldcg(from + R * D + R + row);
+      for (int e = 0; e < kVecs; ++e)  // rows behind the group's last are not written
+        if ((e * 32 + lane) / (D / 4) < rows) u[e] = __ldcg(reinterpret_cast<const float4*>(from) + e * 32 + lane);
+        else u[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float m = row < rows ? __ldcg(from + R * D + row) : -INFINITY, l = row < rows ? __ldcg(from + R * D + R + row) : 0.f;
       const float top = fmaxf(M, m), ref = from_minus_inf(top), old = ex2_approx_ftz(M - ref), f = ex2_approx_ftz(m - ref);
       M = top;
       L = L * old + l * f;
@@ -853,12 +870,10 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       for (int e = 0; e < kVecs; ++e) {
         const int r = (e * 32 + lane) / (D / 4);
         const float fr = __shfl_sync(0xffffffffu, f, r), of = __shfl_sync(0xffffffffu, old, r);
-        if (r < rows) {  // rows behind the group's last are not written
-          acc[e].x = acc[e].x * of + u[e].x * fr;
-          acc[e].y = acc[e].y * of + u[e].y * fr;
-          acc[e].z = acc[e].z * of + u[e].z * fr;
-          acc[e].w = acc[e].w * of + u[e].w * fr;
-        }
+        acc[e].x = acc[e].x * of + u[e].x * fr;
+        acc[e].y = acc[e].y * of + u[e].y * fr;
+        acc[e].z = acc[e].z * of + u[e].z * fr;
+        acc[e].w = acc[e].w * of + u[e].w * fr;
       }
     }
     __syncthreads();  // the slots are free
@@ -873,7 +888,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       to[R * S::kPitch + R + lane] = L;
     }
     __syncthreads();
-    join(0, 2 * kWarps, [](int s) { return (s & 1) == 0; }, item, nullptr);
+    const uint32_t used = 0x55555555u & ((1ull << 2 * min(kWarps, c1 - c0 + 1)) - 1);
+    for (int r = warp; r < rows; r += kWarps) join_row(used, item.x, r, nullptr);
   }
 }
 
