@@ -21,7 +21,8 @@ enum Store { F16 = 0, BF16 = 1, E4M3 = 2, I8 = 3 };
 
 constexpr int kMaxBatch = 1024;  // sequences of a launch (their lengths lie in shared memory)
 constexpr int kMinTiles = 2;     // of a warp, where there is that much work
-constexpr unsigned kWholeItems = 40;  // tiles of the longest item up to which CTAs have whole items
+constexpr unsigned kItemCost = 1;  // tiles that an item counts more than it has
+constexpr unsigned kWholeItems = 80;  // tiles of the longest item up to which CTAs have whole items
 // Exponents' reference (in powers of two): it moves once a score stands kLazy above the largest that it knows.  What goes to f16 is lifted
 // by kLift, so that the largest is at most 2^(kLazy + kLift + 1) and what f16 pairs cannot tell from 0 is 2^-(25 + kLift) of it.
 constexpr int kLazy = 6, kLift = 8;
@@ -174,6 +175,7 @@ struct Shares {
 
 // A tile: the sequence, the row of heads, and the keys.
 struct Cursor {
+  unsigned x;                 // its place on the line
   int b, head, rt, key, len;  // head: of the keys and values
 };
 
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   unsigned longest;
   {
     const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-    auto tiles = [&](int n) { return (unsigned)(n + kTileKeys - 1) / kTileKeys; };
+    auto tiles = [&](int n) { return n ? (unsigned)(n + kTileKeys - 1) / kTileKeys + kItemCost : 0; };
     unsigned sum = 0, top = 0;
     for (int b = b0; b < b1; ++b) {
       const int n = min(max(__ldg(p.lengths + b), 0), most);
@@ -272,8 +274,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       const unsigned x = shares.first(i);
       if (x >= total) return total;
       const int b = sequence_of(x);
-      const unsigned tiles = (unsigned)(lens[b] + kTileKeys - 1) / kTileKeys;
-      return prefix[b] + (x - prefix[b] + tiles / 2) / tiles * tiles;
+      const unsigned n = (unsigned)(lens[b] + kTileKeys - 1) / kTileKeys + kItemCost;
+      return prefix[b] + (x - prefix[b] + n / 2) / n * n;
     };
     cta_lo = end_of(blockIdx.x);
     cta_hi = end_of(blockIdx.x + 1);
@@ -292,9 +294,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     if (p.lse) p.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
   };
   auto pack = [&](float x, float y) { return p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y); };
-  auto next = [&](Cursor& t) {
-    t.key += kTileKeys;
-    if (t.key < t.len) return;
+  auto next_item = [&](Cursor& t) {
+    t.x += kItemCost;
     t.key = 0;
     if (++t.rt < p.row_tiles) return;
     t.rt = 0;
@@ -303,14 +304,21 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     do ++t.b;
     while (t.b < p.batch && (t.len = lens[t.b]) <= 0);
   };
-  auto cursor_at = [&](unsigned x) {
+  auto next = [&](Cursor& t) {
+    ++t.x;
+    t.key += kTileKeys;
+    if (t.key >= t.len) next_item(t);
+  };
+  auto cursor_at = [&](unsigned x) {  // the first tile at x or behind it
     Cursor t;
     t.b = sequence_of(x);
     t.len = lens[t.b];
-    const unsigned tiles = (unsigned)(t.len + kTileKeys - 1) / kTileKeys, at = x - prefix[t.b], item = at / tiles;
+    const unsigned tiles = (unsigned)(t.len + kTileKeys - 1) / kTileKeys, n = tiles + kItemCost, at = x - prefix[t.b], item = at / n, tile = min(at - item * n, tiles);
     t.head = item / p.row_tiles;
     t.rt = item - t.head * p.row_tiles;
-    t.key = (int)(at - item * tiles) * kTileKeys;
+    t.key = (int)tile * kTileKeys;
+    t.x = prefix[t.b] + item * n + tile;
+    if (tile == tiles) next_item(t);
     return t;
   };
   if (lo < hi) {
@@ -320,19 +328,26 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     constexpr int kLanes = 32 / KT;  // of a group
     const int mine = lane / kLanes * 16;
     Cursor ahead = now;
-    unsigned ahead_x = lo, asked_x = lo;
+    unsigned looked = 0, asked = 0, done = 0;  // tiles
     int id[3] = {}, row[3] = {};
     uint32_t bad_pages = 0;  // a bit per tile that has been asked for
     bool seen_bad = false;
     auto look_ahead = [&](int& to_id, int& to_row) {
-      if (ahead_x >= hi) return;
+      if (ahead.x >= hi) return;
+      ++looked;
       const int key = ahead.key + mine;
       to_id = to_row = -1;
       if (key < ahead.len) {
         to_id = __ldg(p.table + ahead.b * p.table_ld + (key >> p.page_log2));
         to_row = (ahead.head << p.page_log2) + (key & ((1 << p.page_log2) - 1));
       }
-      if (++ahead_x < hi) next(ahead);
+      if (ahead.key == 0) {  // an item's queries are wanted at once when it is its turn
+        const int r = lane / (D / 64);
+        if (r < min(R, p.group - ahead.rt * R))
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint16_t*>(p.Q) + (int64_t)ahead.b * p.q_seq +
+                                                          ((int64_t)ahead.head * p.group + ahead.rt * R + r) * p.q_head + lane % (D / 64) * 64));
+      }
+      next(ahead);
     };
 #pragma unroll
     for (int i = 0; i < 3; ++i) look_ahead(id[i], row[i]);
@@ -348,7 +363,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
                                       : (lane >> 3) * 1024 + l * 16;
     auto ask = [&](auto values) {
       constexpr bool V = decltype(values)::value;
-      if (asked_x < hi) {
+      if (asked < looked) {
         const bool good = (unsigned)(id[0] - 1) < (unsigned)p.pages;
         const int64_t page = good ? id[0] - 1 : 0;  // the first one where there is none
         if (KT == 1 || row[0] >= 0) {
@@ -367,9 +382,9 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         }
         if constexpr (!V) {
           const bool wrong = __any_sync(0xffffffffu, row[0] >= 0 && !good);
-          bad_pages = (bad_pages & ~(1u << (asked_x & 31))) | ((uint32_t)wrong << (asked_x & 31));
+          bad_pages = (bad_pages & ~(1u << (asked & 31))) | ((uint32_t)wrong << (asked & 31));
         } else {
-          ++asked_x;
+          ++asked;
           id[0] = id[1];
           id[1] = id[2];
           row[0] = row[1];
@@ -404,11 +419,10 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
                           : kRow == 64 ? c * 128 + ((g >> 1) ^ c) * 16 + (g & 1) * 8
                                        : c * 256 + (g ^ (2 * c)) * 16;
 
-    for (unsigned x = lo; x < hi;) {
+    while (now.x < hi) {
       // ---- an item or the part of it that is this warp's
       const int b = now.b, head = now.head, rt = now.rt, len = now.len;
-      const unsigned tiles = (unsigned)(len + kTileKeys - 1) / kTileKeys;
-      const unsigned item_lo = x - (unsigned)now.key / kTileKeys, item_hi = item_lo + tiles, end = min(hi, item_hi);
+      const unsigned item_lo = now.x - (unsigned)now.key / kTileKeys, item_hi = item_lo + (unsigned)(len + kTileKeys - 1) / kTileKeys;
       const int rows = p.group - rt * R;  // live rows, at least one
       bool bad = __ldg(p.lengths + b) > most;
       uint32_t q[NT][QW];
@@ -472,7 +486,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       auto tile = [&](auto tail_tag) {  // TAIL: some of its keys are behind the last one
         constexpr bool tail = decltype(tail_tag)::value;
         copies_wait<kRing - 1>();
-        bad |= (bad_pages >> (x & 31)) & 1;
+        bad |= (bad_pages >> (done++ & 31)) & 1;
         float sc[KT][NT][4];
         [[maybe_unused]] float ks[KT][2];
         const uint32_t k_even = ring + slot * S::kEntry + k_at, k_odd = k_even ^ 16;
@@ -701,13 +715,12 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         });
         leave_entry(AfterValues());
       };
-      for (; x < end; ++x) {
+      const unsigned end = min(hi, item_hi);
+      for (; now.x < end; ++now.x, now.key += kTileKeys) {
         if (now.key + kTileKeys <= len) tile(std::false_type());
         else tile(std::true_type());
-        now.key += kTileKeys;
       }
-      now.key -= kTileKeys;
-      next(now);
+      if (now.x == item_hi) next_item(now);
       // ---- leaving the item
       seen_bad |= bad;
       const bool whole = item_lo >= lo && item_hi <= hi;
@@ -899,7 +912,7 @@ int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   static_assert(S::kSmem <= 227 * 1024, "shared memory of a CTA");
   p.row_tiles = (p.group + S::R - 1) / S::R;
   // of a sequence, at most; one where the page table is empty
-  const int64_t tiles = std::max<int64_t>(1, (((int64_t)p.width << p.page_log2) + 16 * S::KT - 1) / (16 * S::KT) * p.kv_heads * p.row_tiles);
+  const int64_t tiles = std::max<int64_t>(1, ((((int64_t)p.width << p.page_log2) + 16 * S::KT - 1) / (16 * S::KT) + kItemCost) * p.kv_heads * p.row_tiles);
   if (tiles > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: a sequence has too many keys");
   const int64_t chunk = std::min<int64_t>(kMaxBatch, INT32_MAX / tiles);
   if ((size_t)ctx->sm_count * 2 * S::kPartFloats * sizeof(float) > kSlotBytes || ctx->sm_count > kTickets)
@@ -919,8 +932,7 @@ int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
     q.lse = p.lse ? p.lse + b * p.heads : nullptr;
     q.table = p.table + b * p.table_ld;
     q.lengths = p.lengths + b;
-    const int64_t most = (tiles * q.batch + (int64_t)S::kWarps * kMinTiles - 1) / ((int64_t)S::kWarps * kMinTiles);
-    launch_kernel(kern, (unsigned)std::min<int64_t>(most, ctx->sm_count), S::kThreads, S::kSmem, st, 0, q, ctx->dev_status);
+    launch_kernel(kern, (unsigned)ctx->sm_count, S::kThreads, S::kSmem, st, 0, q, ctx->dev_status);
     CTB_CHECK_LAUNCH("ctb_fmha_paged launch");
   }
   return CTB_OK;
