@@ -15,8 +15,7 @@ using namespace ctb_internal;
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxTokens = 16;  // of a CTA that writes
+constexpr int kThreads = 256;
 constexpr float kSmallest = 7.888609052210118e-31f;  // 2^-100: rows below it are zeros in 8 bits
 
 enum Store { Same = 0, E4M3 = 1, I8 = 2 };
@@ -53,133 +52,197 @@ struct WriteParams {
   const void *slots, *q, *k, *v, *positions;
   void* q_out;
   const double* frequencies;
-  int64_t qo_t, qo_h, q_t, q_h, k_t, k_h, v_t, v_h, tokens;
+  int qo_t, qo_h, q_t, q_h, k_t, k_h, v_t, v_h;
+  int64_t rows_all;
   AngleTable table;
-  int q_heads, rows, pairs, per_cta, wide_slots, wide_positions, interleaved, vectors;  // q_heads: 0 without queries; pairs: 0 without angles
+  Divisor by_token;  // rows of a token: of queries, keys, values
+  int q_heads, pairs, wide_slots, wide_positions, interleaved, vectors;  // q_heads: 0 without queries; pairs: 0 without angles
   float scale;
 };
 
-template <typename T, int D, int STORE>
+// A warp has U groups of 32 / (D / 8) neighbouring rows: it asks for them, takes its share of the CTA's angles and slots while they come, and
+// stores them behind the barrier.
+template <typename T, int D, int STORE, int U>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteParams p, int* status) {
-  constexpr int L = D / 8, kRows = 32 / L;  // lanes of a row, rows of a warp
-  __shared__ float2 angles[kMaxTokens * (D / 2 + 8)];
+  constexpr int L = D / 8, kRows = kThreads / L;  // lanes of a row, rows at a time
+  constexpr int kMaxTokens = kRows * U / 2 + 1;   // a token has two rows at least
+  __shared__ __align__(16) float angles[kMaxTokens * D];
   __shared__ long long places[kMaxTokens];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunk = lane & (L - 1), e0 = chunk * 8;
-  const int64_t t0 = (int64_t)blockIdx.x * p.per_cta;
-  const int tokens = (int)min((int64_t)p.per_cta, p.tokens - t0);
+  const int lane = threadIdx.x & 31, chunk = lane & (L - 1), e0 = chunk * 8;
+  const int64_t row0 = (int64_t)blockIdx.x * (kRows * U), t0 = row0 / p.by_token.d;
+  const uint32_t local0 = (uint32_t)(row0 - t0 * p.by_token.d), n = (uint32_t)min((int64_t)(kRows * U), p.rows_all - row0);
+  const int kv_heads = p.cache.kv_heads;
   grid_dependency_sync();
-  if (p.pairs)
-    p.table.fill(angles, p.positions, p.wide_positions, t0, tokens, p.frequencies, p.scale, false, threadIdx.x, kThreads);
-  if (threadIdx.x < tokens) {
-    const long long slot = index_at(p.slots, p.wide_slots, t0 + threadIdx.x);
+  uint4 asked[U];
+  int token_of[U], row_of[U];  // -1: none
+  auto rows_of = [&](int k, const void*& base, int& head, int& t_stride, int& h_stride) {  // the array that row k is in
+    const int r = row_of[k];
+    const bool key = r < p.q_heads + kv_heads;
+    head = r - (key ? p.q_heads : p.q_heads + kv_heads);
+    base = key ? p.k : p.v;
+    t_stride = key ? p.k_t : p.v_t;
+    h_stride = key ? p.k_h : p.v_h;
+    if (r < p.q_heads) {
+      head = r;
+      base = p.q;
+      t_stride = p.q_t;
+      h_stride = p.q_h;
+    }
+  };
+  auto source = [&](int k) {
+    const void* base;
+    int head, t_stride, h_stride;
+    rows_of(k, base, head, t_stride, h_stride);
+    return static_cast<const T*>(base) + (t0 * t_stride + (int64_t)token_of[k] * t_stride + (int64_t)head * h_stride);
+  };
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = k * kRows + threadIdx.x / L;
+    asked[k] = make_uint4(0, 0, 0, 0);
+    token_of[k] = 0;
+    row_of[k] = -1;
+    if (i >= n) continue;
+    token_of[k] = p.by_token(local0 + i);
+    row_of[k] = (int)(local0 + i) - token_of[k] * (int)p.by_token.d;
+    const T* src = source(k);
+    if (p.vectors) asked[k] = __ldcs(reinterpret_cast<const uint4*>(src + e0));
+    else {
+      alignas(16) T x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = src[e0 + j];
+      asked[k] = *reinterpret_cast<const uint4*>(x);
+    }
+  }
+  const int tokens = (int)p.by_token(local0 + n - 1) + 1;
+  if (p.pairs) p.table.fill(angles, p.positions, p.wide_positions, t0, tokens, p.frequencies, p.scale, false, threadIdx.x, kThreads);
+  for (int t = threadIdx.x; t < tokens; t += kThreads) {
+    const long long slot = index_at(p.slots, p.wide_slots, t0 + t);
     const bool bad = slot < 0 || slot > p.cache.tokens;
     if (bad) atomicMax(status, (int)DEV_BAD_INDEX);
-    places[threadIdx.x] = bad ? -1 : slot - 1;
+    places[t] = bad ? -1 : slot - 1;
   }
   __syncthreads();
-  const int all = tokens * p.rows;
-  for (int i0 = warp * kRows; i0 < all; i0 += kWarps * kRows) {
-    const int i = i0 + lane / L;
-    const bool live = i < all;
-    const int t = live ? i / p.rows : 0, r = live ? i - t * p.rows : 0;
-    const bool query = r < p.q_heads, value = r >= p.q_heads + p.cache.kv_heads;
-    const int head = query ? r : value ? r - p.q_heads - p.cache.kv_heads : r - p.q_heads;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int t = token_of[k], r = row_of[k];
+    const bool live = r >= 0, query = r < p.q_heads, value = r >= p.q_heads + kv_heads;
+    const int head = query ? r : value ? r - p.q_heads - kv_heads : r - p.q_heads;
     const long long place = places[t];
-    const bool wanted = live && (query || place >= 0);
-    const T* src = query ? static_cast<const T*>(p.q) + (t0 + t) * p.q_t + head * p.q_h
-                         : value ? static_cast<const T*>(p.v) + (t0 + t) * p.v_t + head * p.v_h
-                                 : static_cast<const T*>(p.k) + (t0 + t) * p.k_t + head * p.k_h;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (wanted) {
-      if (p.vectors) w = __ldcs(reinterpret_cast<const uint4*>(src + e0));
-      else {
-        alignas(16) T x[8];
+    const bool stored = live && !query && place >= 0;
+    uint32_t w[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
+    Pair x[4];  // the elements in f32, for 8 bits
+    const bool turned = live && !value && e0 < 2 * p.pairs;
+    const float* table = angles + t * 2 * p.pairs;
+    if (p.pairs) {
+      if (p.interleaved || p.pairs % 8 == 0) {
+        // with pairs (i, i + pairs), a pair's other elements are another lane's eight
+        const int half = p.pairs / 8;
+        const bool second = chunk >= half;
+        uint32_t o[4];
+        if (!p.interleaved) {
+          const int other = turned ? (second ? lane - half : lane + half) : lane;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = src[e0 + j];
-        w = *reinterpret_cast<const uint4*>(x);
-      }
-    }
-    float x[8];
-    unpack_row<T>(w, x);
-    const bool turned = !value && e0 < 2 * p.pairs;
-    const float2* a = angles + t * p.table.size();
-    if (p.pairs && p.interleaved) {
-      if (turned) {
+          for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, w[i], other) ^ (second ? 0u : 0x80008000u);
+        }
+        if (turned) {
+          if (!p.interleaved) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (e0 + 2 * j < 2 * p.pairs) {
-            const float2 cs = a[p.table.at(chunk, j)];
-            const float y = x[2 * j] * cs.x - x[2 * j + 1] * cs.y;
-            x[2 * j + 1] = x[2 * j] * cs.y + x[2 * j + 1] * cs.x;
-            x[2 * j] = y;
+            for (int i = 0; i < 4; ++i) {
+              const TwoAngles a = angles_of(table, p.table.runs, second ? chunk - half : chunk, i);
+              x[i] = fma2(vec_pair<T>(o, i), a.sin, mul2(vec_pair<T>(w, i), a.cos));
+            }
+          } else if (p.table.step == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const TwoAngles a = angles_of(table, p.table.runs, chunk, i);
+              Pair u, v;
+              split_pairs<T>(w, i, u, v);
+              const float2 f = halves(fma2(v, minus(a.sin), mul2(u, a.cos))), g = halves(fma2(v, a.cos, mul2(u, a.sin)));
+              x[2 * i] = pair(f.x, g.x);
+              x[2 * i + 1] = pair(f.y, g.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[i] = vec_pair<T>(w, i);
+              if (e0 + 2 * i < 2 * p.pairs) {
+                const float2 f = halves(x[i]);
+                const float c = table[e0 + 2 * i], d = table[e0 + 2 * i + 1];
+                x[i] = pair(f.x * c - f.y * d, f.x * d + f.y * c);
+              }
+            }
           }
+        }
+      } else {
+        if (turned) {
+          const T* src = source(k);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int e = e0 + 2 * i + j;
+              const bool second = e >= p.pairs;
+              const int at = second ? e - p.pairs : e;
+              f[j] = to_float(reinterpret_cast<const T*>(&asked[k])[2 * i + j]);
+              if (e >= 2 * p.pairs) continue;
+              const float y = to_float(src[second ? at : e + p.pairs]);
+              f[j] = f[j] * table[2 * at] + (second ? y : -y) * table[2 * at + 1];
+            }
+            x[i] = pair(f[0], f[1]);
+          }
+        }
+        __syncwarp();  // queries in place: what other lanes read here is written below
       }
-    } else if (p.pairs && p.pairs % 8 == 0) {  // the pair's other elements are another lane's eight
-      const int half = p.pairs / 8;
-      const bool second = chunk >= half;
-      const int other = turned ? (second ? lane - half : lane + half) : lane;
-      const uint4 o = make_uint4(__shfl_sync(0xffffffffu, w.x, other), __shfl_sync(0xffffffffu, w.y, other),
-                                 __shfl_sync(0xffffffffu, w.z, other), __shfl_sync(0xffffffffu, w.w, other));
       if (turned) {
-        float y[8];
-        unpack_row<T>(o, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 cs = a[p.table.at(second ? chunk - half : chunk, j)];
-          x[j] = x[j] * cs.x + (second ? y[j] * cs.y : -y[j] * cs.y);
-        }
-      }
-    } else if (p.pairs) {
-      if (turned && wanted) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int e = e0 + j;
-          if (e >= 2 * p.pairs) continue;
-          const bool second = e >= p.pairs;
-          const int pair = second ? e - p.pairs : e;
-          const float2 cs = a[p.table.at(pair / p.table.step, pair % p.table.step)];
-          const float y = to_float(src[second ? pair : e + p.pairs]);
-          x[j] = x[j] * cs.x + (second ? y * cs.y : -y * cs.y);
-        }
-      }
-      __syncwarp();  // queries in place: what other lanes read here is written below
-    }
-    if (turned) w = pack_row<T>(x);
-    if (query) {
-      if (live) {
-        T* to = static_cast<T*>(p.q_out) + (t0 + t) * p.qo_t + head * p.qo_h + e0;
-        if (p.vectors) *reinterpret_cast<uint4*>(to) = w;
-        else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) to[j] = reinterpret_cast<const T*>(&w)[j];
-        }
+        for (int i = 0; i < 4; ++i) put_pair<T>(w, i, x[i]);
       }
     }
+    const uint4 words = make_uint4(w[0], w[1], w[2], w[3]);
+    if (live && query) {
+      T* to = static_cast<T*>(p.q_out) + (t0 * p.qo_t + (int64_t)t * p.qo_t + (int64_t)head * p.qo_h) + e0;
+      if (p.vectors) *reinterpret_cast<uint4*>(to) = words;
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j] = reinterpret_cast<const T*>(&words)[j];
+      }
+    }
+    if (!__any_sync(0xffffffffu, stored)) continue;
     const int64_t page = place >> p.cache.page_log2;
-    const int64_t row = ((int64_t)head << p.cache.page_log2) + (place & ((1 << p.cache.page_log2) - 1));
+    const int64_t row = (head << p.cache.page_log2) + (int)(place & ((1 << p.cache.page_log2) - 1));
     if constexpr (STORE == Same) {
-      if (wanted && !query) {
+      if (stored) {
         T* to = static_cast<T*>(value ? p.cache.v : p.cache.k) + page * (value ? p.cache.v_page : p.cache.k_page) + row * D + e0;
-        *reinterpret_cast<uint4*>(to) = w;
+        *reinterpret_cast<uint4*>(to) = words;
       }
     } else {
       constexpr float kMost = STORE == I8 ? 127.f : 448.f;
-      uint32_t top = 0;  // magnitudes as whole numbers: NaN is above infinity
+      if (!turned) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+        for (int i = 0; i < 4; ++i) x[i] = vec_pair<T>(w, i);
+      }
+      float peak = 0.f;  // NaN where there is one
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (wanted && !query) {
-        const float peak = __uint_as_float(top);
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = halves(x[i]);
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(peak) : "f"(peak), "f"(f.x), "f"(f.y));
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) asm("max.NaN.f32 %0, %1, %2;" : "=f"(peak) : "f"(peak), "f"(__shfl_xor_sync(0xffffffffu, peak, o)));
+      if (stored) {
         const bool fine = peak >= kSmallest && peak < INFINITY;
         // x c / a with one Newton step behind the product with 1 / a: a quotient that is a number of f32 comes out as it is, so ties are ties
         const float pre = peak > 1.2676506e30f ? 5.9604645e-8f : 1.f;  // beyond 2^100 in units of 2^24: x c is finite
-        const float a = peak * pre, inv = fine ? __frcp_rn(a) : 0.f;
+        const float a = peak * pre, inv = fine ? __frcp_rn(a) : 0.f, most = pre * kMost;
+        const Pair inv2 = pair(inv, inv), a2 = pair(-a, -a), most2 = pair(most, most);
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float n = x[j] * pre * kMost, z = n * inv;
-          y[j] = fine ? fmaf(fmaf(-z, a, n), inv, z) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const Pair m = mul2(x[i], most2), z = mul2(m, inv2);
+          const float2 f = halves(fma2(fma2(z, a2, m), inv2, z));
+          y[2 * i] = fine ? f.x : 0.f;
+          y[2 * i + 1] = fine ? f.y : 0.f;
         }
         uint2 codes;
         if constexpr (STORE == I8) codes = make_uint2(i8x4(y[0], y[1], y[2], y[3]), i8x4(y[4], y[5], y[6], y[7]));
@@ -271,7 +334,10 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadParams p, i
       else {
         float x[8];
         values8<STORE>(w[i][s], scale[i][s], x);
-        out = pack_row<T>(x);
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put_pair<T>(u, j, ctb::pair(x[2 * j], x[2 * j + 1]));
+        out = make_uint4(u[0], u[1], u[2], u[3]);
       }
       __stcs(reinterpret_cast<uint4*>(static_cast<T*>(s ? p.V : p.K) + (pair * p.seq + at) * D) + chunk, out);
     }
@@ -294,10 +360,18 @@ int by_type(int dtype, int64_t D, int store, A&&... args) {
 }
 template <typename T, int D, int STORE>
 struct Write {
-  static int run(ctb_ctx* ctx, cudaStream_t st, unsigned grid, const WriteParams& p) {
-    launch_kernel(kv_write_kernel<T, D, STORE>, grid, kThreads, 0, st, 0, p, ctx->dev_status);
+  template <int U>
+  static int launch(ctb_ctx* ctx, cudaStream_t st, const WriteParams& p) {
+    constexpr int kRows = kThreads / (D / 8) * U;
+    const int64_t grid = (p.rows_all + kRows - 1) / kRows;
+    if (grid > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: shape too large");
+    launch_kernel(kv_write_kernel<T, D, STORE, U>, (unsigned)grid, kThreads, 0, st, 0, p, ctx->dev_status);
     CTB_CHECK_LAUNCH("ctb_kv_write launch");
     return CTB_OK;
+  }
+  static int run(ctb_ctx* ctx, cudaStream_t st, const WriteParams& p) {
+    const int64_t ctas = p.rows_all / (kThreads / (D / 8));
+    return ctas >= 4ll * ctx->sm_count ? launch<4>(ctx, st, p) : launch<1>(ctx, st, p);  // four groups per warp still give every SM a CTA
   }
 };
 template <typename T, int D, int STORE>
@@ -376,21 +450,23 @@ extern "C" int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cach
   WriteParams p = {};
   p.cache = cache_of(cache);
   p.slots = slots; p.q = q; p.k = k; p.v = v; p.positions = positions; p.q_out = q_out; p.frequencies = frequencies;
-  p.qo_t = strides[0]; p.qo_h = strides[1]; p.q_t = strides[2]; p.q_h = strides[3];
-  p.k_t = strides[4]; p.k_h = strides[5]; p.v_t = strides[6]; p.v_h = strides[7];
-  p.tokens = tokens;
+  for (int i = 0; i < 8; ++i)
+    if (strides[i] < 0 || strides[i] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: strides too large");
+  p.qo_t = (int)strides[0]; p.qo_h = (int)strides[1]; p.q_t = (int)strides[2]; p.q_h = (int)strides[3];
+  p.k_t = (int)strides[4]; p.k_h = (int)strides[5]; p.v_t = (int)strides[6]; p.v_h = (int)strides[7];
+  const int64_t rows = heads + 2 * cache->kv_heads;
   p.q_heads = (int)heads;
-  p.rows = (int)(heads + 2 * cache->kv_heads);
+  p.by_token = Divisor((uint32_t)rows);
+  p.rows_all = tokens * rows;
   p.pairs = frequencies ? (int)(rotary / 2) : 0;
+  // runs of pairs that lie in the eight elements of a lane; where those would not all be full, single ones
   const int step = interleaved ? 4 : 8;
-  p.table = AngleTable{p.pairs, step, (p.pairs + step - 1) / step};
+  p.table = p.pairs % step ? AngleTable{p.pairs, 1, p.pairs} : AngleTable{p.pairs, step, p.pairs / step};
   p.wide_slots = slot_bits == 64; p.wide_positions = position_bits == 64; p.interleaved = interleaved != 0;
   p.scale = scale;
   p.vectors = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (!heads || ((uintptr_t)q % 16 == 0 && (uintptr_t)q_out % 16 == 0));
   for (int i = heads ? 0 : 4; i < 8; ++i) p.vectors &= strides[i] % 8 == 0;
-  p.per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, tokens / (ctx->sm_count * 8)));
-  return by_type<Write>(dtype, cache->head_dim, cache->dtype, ctx, static_cast<cudaStream_t>(stream), (unsigned)((tokens + p.per_cta - 1) / p.per_cta),
-                        p);
+  return by_type<Write>(dtype, cache->head_dim, cache->dtype, ctx, static_cast<cudaStream_t>(stream), p);
 }
 
 extern "C" int ctb_kv_read(ctb_ctx* ctx, void* stream, void* K, void* V, const ctb_kv_cache* cache, const int32_t* page_table,

@@ -1,8 +1,8 @@
 // Rotary positions (ctb_rope): pairs of elements of every head turned by the angle of their token.
 //
 // What bounds it is HBM: every element is read and written once, for three operations.  The angles are the only arithmetic of note (an f64
-// product, a reduction and a sincospif, about 60 instructions), and all heads of a token share them: a CTA takes a few tokens, works out their
-// angles once, a thread each, into shared memory, and then walks over the tokens' heads.
+// product, a reduction and a sincospif, about 60 instructions), and all heads of a token share them: a CTA takes a run of heads, asks for
+// them, works out the angles of their tokens, a thread each, into shared memory while they come, and turns them.
 #include <math.h>
 
 #include <algorithm>
@@ -16,116 +16,138 @@ using namespace ctb_internal;
 
 namespace {
 
-constexpr int kThreads = 256, kMaxPairs = 2048;  // angles of a CTA
+constexpr int kThreads = 256;
 
 struct Side {
   const void* src;
   void* dst;
-  int64_t src_b, src_s, src_h, dst_b, dst_s, dst_h;
+  int src_b, src_s, src_h, dst_b, dst_s, dst_h;
 };
 struct Params {
   Side side[2];
   const void* positions;
   const double* frequencies;
-  int64_t tokens;
   AngleTable table;
-  int seq, q_heads, heads, pairs, dim, turned, units, per_cta, wide, interleaved, inverse;
+  Divisor by_seq, by_token, by_units;  // units of a token, of a head
+  int64_t units_all;
+  int tokens, seq, q_heads, dim, turned, wide, interleaved, inverse;
   float scale;
 };
 
 // V: elements of a vector (16 bytes), or 1 where something does not lie on the 16-byte grid.  A unit of a head is V pairs (two
-// vectors, or with interleaved pairs two neighbouring ones), or for what is only copied two vectors.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const Params p) {
-  __shared__ float2 angles[kMaxPairs];
-  const int64_t t0 = (int64_t)blockIdx.x * p.per_cta;
-  const int tokens = (int)min((int64_t)p.per_cta, p.tokens - t0);
+// vectors, or with interleaved pairs two neighbouring ones), or for what is only copied two vectors.  A thread asks for its U units, then
+// takes its share of the CTA's angles, and turns the units behind the barrier.
+template <typename T, int V, int U>
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const Params p) {
+  using Vec = std::conditional_t<V == 1, T, uint4>;
+  extern __shared__ __align__(16) float angles[];
+  const int64_t unit0 = (int64_t)blockIdx.x * (kThreads * U);
+  const int t0 = (int)(unit0 / p.by_token.d);
+  const uint32_t local0 = (uint32_t)(unit0 - (int64_t)t0 * p.by_token.d), n = (uint32_t)min((int64_t)(kThreads * U), p.units_all - unit0);
   grid_dependency_sync();
-  p.table.fill(angles, p.positions, p.wide, t0, tokens, p.frequencies, p.scale, p.inverse, threadIdx.x, kThreads);
-  __syncthreads();
-  const int per_token = p.heads * p.units;
-  for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
-    const int t = i / per_token, r = i - t * per_token, h = r / p.units, u = r - h * p.units;
-    const bool second = h >= p.q_heads;
+  Vec x[U], y[U];
+  T* to[U];
+  int at[U], run[U], e0[U], e1[U];  // angles of the unit's token (-1: none) and run, the first elements of its vectors
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = threadIdx.x + k * kThreads;
+    to[k] = nullptr;
+    if (i >= n) continue;
+    const uint32_t t = p.by_token(local0 + i), r = local0 + i - t * p.by_token.d, h = p.by_units(r), u = r - h * p.by_units.d;
+    const bool second = (int)h >= p.q_heads;
     const Side& s = p.side[second];
     const int head = second ? h - p.q_heads : h;
-    const int64_t token = t0 + t, b = token / p.seq, n = token - b * p.seq;
-    const T* src = static_cast<const T*>(s.src) + b * s.src_b + n * s.src_s + head * s.src_h;
-    T* dst = static_cast<T*>(s.dst) + b * s.dst_b + n * s.dst_s + head * s.dst_h;
-    const float2* a = angles + t * p.table.size();
-    auto angle = [&](int k) { return a[p.table.at(u, k)]; };  // of pair u * V + k
-    const bool turned = u < p.turned;
-    // the unit's two vectors
-    int e0, e1;
-    if (!turned) {
-      e0 = 2 * p.pairs + (u - p.turned) * 2 * V;
-      e1 = e0 + V;
-    } else if (p.interleaved) {
-      e0 = u * 2 * V;
-      e1 = e0 + V;
-    } else {
-      e0 = u * V;
-      e1 = p.pairs + u * V;
-    }
+    const int token = t0 + t, b = p.by_seq(token), place = token - b * (int)p.by_seq.d;
+    const T* src = static_cast<const T*>(s.src) + ((int64_t)b * s.src_b + (int64_t)place * s.src_s + (int64_t)head * s.src_h);
+    to[k] = static_cast<T*>(s.dst) + ((int64_t)b * s.dst_b + (int64_t)place * s.dst_s + (int64_t)head * s.dst_h);
+    const bool turned = (int)u < p.turned;
+    at[k] = turned ? (int)t * 2 * p.table.pairs : -1;
+    run[k] = u;
+    e0[k] = !turned ? 2 * p.table.pairs + (u - p.turned) * 2 * V : p.interleaved ? u * 2 * V : u * V;
+    e1[k] = turned && !p.interleaved ? p.table.pairs + u * V : e0[k] + V;
     if constexpr (V == 1) {
-      float x = to_float(src[e0]), y = e1 < p.dim ? to_float(src[e1]) : 0.f;
-      if (turned) {
-        const float2 cs = angle(0);
-        const float x1 = x * cs.x - y * cs.y, y1 = x * cs.y + y * cs.x;
-        dst[e0] = from_float<T>(x1);
-        dst[e1] = from_float<T>(y1);
-      } else {
-        dst[e0] = src[e0];
-        if (e1 < p.dim) dst[e1] = src[e1];
-      }
+      x[k] = src[e0[k]];
+      y[k] = e1[k] < p.dim ? src[e1[k]] : T(0.f);
     } else {
-      uint4 q0 = __ldcs(reinterpret_cast<const uint4*>(src + e0));
-      uint4 q1 = e1 < p.dim ? __ldcs(reinterpret_cast<const uint4*>(src + e1)) : make_uint4(0, 0, 0, 0);
-      if (turned) {
-        float x[V], y[V];
-        unpack_row<T>(q0, x);
-        unpack_row<T>(q1, y);
-        if (p.interleaved) {
+      x[k] = __ldcs(reinterpret_cast<const uint4*>(src + e0[k]));
+      y[k] = e1[k] < p.dim ? __ldcs(reinterpret_cast<const uint4*>(src + e1[k])) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int tokens = (int)p.by_token(local0 + n - 1) + 1;
+  p.table.fill(angles, p.positions, p.wide, t0, tokens, p.frequencies, p.scale, p.inverse, threadIdx.x, kThreads);
+  __syncthreads();
 #pragma unroll
-          for (int k = 0; k < V; k += 2) {
-            const float2 c0 = angle(k / 2), c1 = angle(V / 2 + k / 2);
-            const float x0 = x[k] * c0.x - x[k + 1] * c0.y, y0 = y[k] * c1.x - y[k + 1] * c1.y;
-            x[k + 1] = x[k] * c0.y + x[k + 1] * c0.x;
-            y[k + 1] = y[k] * c1.y + y[k + 1] * c1.x;
-            x[k] = x0;
-            y[k] = y0;
-          }
-        } else {
+  for (int k = 0; k < U; ++k) {
+    if (!to[k]) continue;
+    if (at[k] >= 0) {
+      const float* table = angles + at[k];
+      if constexpr (V == 1) {
+        const float a = to_float(x[k]), b = to_float(y[k]), c = table[2 * run[k]], d = table[2 * run[k] + 1];
+        x[k] = from_float<T>(a * c - b * d);
+        y[k] = from_float<T>(a * d + b * c);
+      } else {
+        uint32_t a[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, b[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float2 cs = angle(k);
-            const float x0 = x[k] * cs.x - y[k] * cs.y;
-            y[k] = x[k] * cs.y + y[k] * cs.x;
-            x[k] = x0;
+        for (int i = 0; i < V / 2; ++i) {
+          const TwoAngles t = angles_of(table, p.turned, run[k], i);
+          auto turned = [&](Pair& u, Pair& v) {
+            const Pair first = fma2(v, minus(t.sin), mul2(u, t.cos));
+            v = fma2(v, t.cos, mul2(u, t.sin));
+            u = first;
+          };
+          Pair u, v;
+          if (p.interleaved) {
+            uint32_t (&w)[4] = i < V / 4 ? a : b;
+            split_pairs<T>(w, i % (V / 4), u, v);
+            turned(u, v);
+            join_pairs<T>(w, i % (V / 4), u, v);
+          } else {
+            u = vec_pair<T>(a, i);
+            v = vec_pair<T>(b, i);
+            turned(u, v);
+            put_pair<T>(a, i, u);
+            put_pair<T>(b, i, v);
           }
         }
-        q0 = pack_row<T>(x);
-        q1 = pack_row<T>(y);
+        x[k] = make_uint4(a[0], a[1], a[2], a[3]);
+        y[k] = make_uint4(b[0], b[1], b[2], b[3]);
       }
-      *reinterpret_cast<uint4*>(dst + e0) = q0;
-      if (e1 < p.dim) *reinterpret_cast<uint4*>(dst + e1) = q1;
     }
+    *reinterpret_cast<Vec*>(to[k] + e0[k]) = x[k];
+    if (e1[k] < p.dim) *reinterpret_cast<Vec*>(to[k] + e1[k]) = y[k];
   }
 }
 
-template <typename T>
-int launch(ctb_ctx* ctx, cudaStream_t st, Params p, bool vectors) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int v = vectors ? V : 1;
-  p.turned = p.pairs / v;
-  p.table = AngleTable{p.pairs, v, p.turned};
-  p.units = p.turned + (p.dim - 2 * p.pairs + 2 * v - 1) / (2 * v);
-  p.per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPairs / p.pairs, p.tokens / (ctx->sm_count * 8)));
-  const int64_t grid = (p.tokens + p.per_cta - 1) / p.per_cta;
+template <typename T, int V, int U>
+int launch(ctb_ctx*, cudaStream_t st, const Params& p) {
+  const int64_t grid = (p.units_all + kThreads * U - 1) / (kThreads * U);
   if (grid > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_rope: shape too large");
-  launch_kernel(vectors ? rope_kernel<T, V> : rope_kernel<T, 1>, (unsigned)grid, kThreads, 0, st, 0, p);
+  const int64_t tokens = std::min<int64_t>(p.tokens, kThreads * U / p.by_token.d + 2);  // that a CTA has units of
+  const size_t smem = tokens * 2 * p.table.pairs * sizeof(float), most = 200 * 1024;
+  if (smem > most) return fail(CTB_UNSUPPORTED, "ctb_rope: shape too large");
+  auto kern = rope_kernel<T, V, U>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = allow_smem(kern, most);
+    if (e != cudaSuccess) return cuda_fail(e, "ctb_rope: shared memory opt-in");
+  }
+  launch_kernel(kern, (unsigned)grid, kThreads, smem, st, 0, p);
   CTB_CHECK_LAUNCH("ctb_rope launch");
   return CTB_OK;
+}
+
+template <typename T>
+int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int heads, bool vectors) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int v = vectors ? V : 1;
+  p.turned = p.table.pairs / v;
+  p.table = AngleTable{p.table.pairs, v, p.turned};
+  const int units = p.turned + (p.dim - 2 * p.table.pairs + 2 * v - 1) / (2 * v);
+  p.by_units = Divisor(units);
+  p.by_token = Divisor(units * heads);
+  p.units_all = (int64_t)p.tokens * units * heads;
+  const bool many = p.units_all >= (int64_t)kThreads * 8 * ctx->sm_count;  // two units per thread still give every SM four CTAs
+  if (vectors) return many ? launch<T, V, 2>(ctx, st, p) : launch<T, V, 1>(ctx, st, p);
+  return many ? launch<T, 1, 2>(ctx, st, p) : launch<T, 1, 1>(ctx, st, p);
 }
 
 }  // namespace
@@ -164,7 +186,7 @@ extern "C" int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, 
   if (position_bits != 32 && position_bits != 64) return fail(CTB_BAD_ARG, "ctb_rope: positions are 32- or 64-bit");
   if (dtype != CTB_F32 && dtype != CTB_F16 && dtype != CTB_BF16) return fail(CTB_UNSUPPORTED, "ctb_rope: f32, f16 and bf16 are implemented");
   if (!isfinite(scale)) return fail(CTB_BAD_ARG, "ctb_rope: scale is not finite");
-  if (D > 4096 || q_heads + k_heads > 65536 || seq > INT32_MAX || (seq && batch > INT64_MAX / seq))
+  if (D > 4096 || q_heads + k_heads > 65536 || seq > INT32_MAX || (seq && batch > INT32_MAX / seq))
     return fail(CTB_UNSUPPORTED, "ctb_rope: shape too large");
   if (batch * seq == 0) return CTB_OK;
   CTB_CHECK_DEV(q); CTB_CHECK_DEV(q_out); CTB_CHECK_DEV(positions); CTB_CHECK_DEV(frequencies);
@@ -174,7 +196,9 @@ extern "C" int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, 
   bool vectors = rotary % (2 * V) == 0 && D % V == 0;
   for (int i = 0; i < (k_heads ? 2 : 1); ++i) {
     const int64_t* s = strides + 6 * i;
-    p.side[i] = Side{i ? k : q, i ? k_out : q_out, s[3], s[4], s[5], s[0], s[1], s[2]};
+    for (int j = 0; j < 6; ++j)
+      if (s[j] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_rope: strides too large");
+    p.side[i] = Side{i ? k : q, i ? k_out : q_out, (int)s[3], (int)s[4], (int)s[5], (int)s[0], (int)s[1], (int)s[2]};
     const int64_t extents[3] = {batch, seq, i ? k_heads : q_heads};
     const int r = check_turned_in_place("ctb_rope", p.side[i].src, s + 3, p.side[i].dst, s, extents, D, size);
     if (r) return r;
@@ -183,12 +207,14 @@ extern "C" int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, 
   }
   p.positions = positions;
   p.frequencies = frequencies;
-  p.tokens = batch * seq;
-  p.seq = (int)seq; p.q_heads = (int)q_heads; p.heads = (int)(q_heads + k_heads); p.pairs = (int)(rotary / 2); p.dim = (int)D;
+  p.tokens = (int)(batch * seq);
+  p.by_seq = Divisor((uint32_t)seq);
+  p.seq = (int)seq; p.q_heads = (int)q_heads; p.table.pairs = (int)(rotary / 2); p.dim = (int)D;
   p.wide = position_bits == 64; p.interleaved = interleaved != 0; p.inverse = inverse != 0;
   p.scale = scale;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == CTB_F32) return launch<float>(ctx, st, p, vectors);
-  if (dtype == CTB_F16) return launch<__half>(ctx, st, p, vectors);
-  return launch<__nv_bfloat16>(ctx, st, p, vectors);
+  const int heads = (int)(q_heads + k_heads);
+  if (dtype == CTB_F32) return launch<float>(ctx, st, p, heads, vectors);
+  if (dtype == CTB_F16) return launch<__half>(ctx, st, p, heads, vectors);
+  return launch<__nv_bfloat16>(ctx, st, p, heads, vectors);
 }

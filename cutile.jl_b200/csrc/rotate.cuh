@@ -8,6 +8,18 @@ __device__ __forceinline__ long long index_at(const void* p, bool wide, int64_t 
   return wide ? __ldg(static_cast<const long long*>(p) + i) : (long long)__ldg(static_cast<const int*>(p) + i);
 }
 
+// n / d for n < 2^31 and 1 <= d < 2^31 by a multiplication (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994):
+// with 2^(s - 1) < d <= 2^s and m = floor(2^32 (2^s - d) / d) + 1, n / d = (n + (m n >> 32)) >> s.
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (n + __umulhi(n, m)) >> s; }
+};
+
 // scale * (cos, sin) of position * frequency.  The product and its reduction to a turn are in f64: an f32 angle of a far position
 // (1e6 radians) has no digits left behind the point.  sincospif then takes half turns in [-1, 1], where its argument is off by
 // 2^-25 at most.
@@ -19,28 +31,49 @@ __device__ __forceinline__ float2 turn(long long position, double frequency, flo
   return make_float2(c * scale, s * scale);
 }
 
-// Threads that work on neighbouring runs of `step` pairs read the k-th pair of their runs at the same time: it lies next to its like.
+// The angles of a few tokens in shared memory.  Threads take neighbouring runs of `step` pairs and read the k-th and (k + 1)-th pair of
+// their runs at the same time, so these lie together, as (cos, cos, sin, sin), next to those of the other runs.  step 1: (cos, sin).
 struct AngleTable {
-  int pairs, step, runs;  // runs = ceil(pairs / step)
-  __host__ __device__ int size() const { return step * runs; }
-  __device__ __forceinline__ int at(int run, int k) const { return k * runs + run; }
-  __device__ __forceinline__ void fill(float2* table, const void* positions, bool wide, int64_t t0, int tokens, const double* frequencies,
+  int pairs, step, runs;  // runs * step = pairs
+  __device__ __forceinline__ void fill(float* table, const void* positions, bool wide, int64_t t0, int tokens, const double* frequencies,
                                        float scale, bool inverse, int thread, int threads) const {
     for (int i = thread; i < tokens * pairs; i += threads) {
       const int t = i / pairs, pair = i - t * pairs;
-      float2 a = turn(index_at(positions, wide, t0 + t), __ldg(frequencies + pair), scale);
-      if (inverse) a.y = -a.y;
-      table[t * size() + at(pair / step, pair % step)] = a;
+      const float2 a = turn(index_at(positions, wide, t0 + t), __ldg(frequencies + pair), scale);
+      const int run = pair / step, k = pair - run * step;
+      float* to = table + 2 * t * pairs + (step == 1 ? 2 * pair : ((k >> 1) * runs + run) * 4 + (k & 1));
+      to[0] = a.x;
+      to[step == 1 ? 1 : 2] = inverse ? -a.y : a.y;
     }
   }
 };
+// Pairs 2 i and 2 i + 1 of a run, step > 1; table: of the token.
+struct TwoAngles {
+  Pair cos, sin;
+};
+__device__ __forceinline__ TwoAngles angles_of(const float* table, int runs, int run, int i) {
+  const float4 a = reinterpret_cast<const float4*>(table)[i * runs + run];
+  return {pair(a.x, a.y), pair(a.z, a.w)};
+}
+__device__ __forceinline__ Pair minus(Pair a) { return a ^ 0x8000000080000000ull; }
 
+// Words 2 i and 2 i + 1 of interleaved pairs in 16 bits, or a vector's two pairs in f32, as (x, x) and (y, y), and back.
 template <typename T>
-__device__ __forceinline__ uint4 pack_row(const float (&f)[16 / sizeof(T)]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 8 / (int)sizeof(T); ++i) put_pair<T>(w, i, pair(f[2 * i], f[2 * i + 1]));
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ void split_pairs(const uint32_t (&w)[4], int i, Pair& x, Pair& y) {
+  if constexpr (sizeof(T) == 4) {
+    x = pair(__uint_as_float(w[0]), __uint_as_float(w[2]));
+    y = pair(__uint_as_float(w[1]), __uint_as_float(w[3]));
+  } else {
+    const float2 a = word_pair<T>(w[2 * i]), b = word_pair<T>(w[2 * i + 1]);
+    x = pair(a.x, b.x);
+    y = pair(a.y, b.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void join_pairs(uint32_t (&w)[4], int i, Pair x, Pair y) {
+  const float2 a = halves(x), b = halves(y);
+  put_pair<T>(w, 2 * i, pair(a.x, b.x));
+  put_pair<T>(w, 2 * i + 1, pair(a.y, b.y));
 }
 
 }  // namespace ctb
