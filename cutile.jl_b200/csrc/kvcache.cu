@@ -15,7 +15,8 @@ using namespace ctb_internal;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;       // of a CTA that reads
+constexpr int kMaxWarps = 8;        // of one that writes
 constexpr float kSmallest = 7.888609052210118e-31f;  // 2^-100: rows below it are zeros in 8 bits
 
 enum Store { Same = 0, E4M3 = 1, I8 = 2 };
@@ -47,210 +48,217 @@ __device__ __forceinline__ uint32_t i8x4(float a, float b, float c, float d) {  
   return __byte_perm(u, w, 0x5410);
 }
 
+enum Kind { Query = 0, Key = 1, Value = 2 };
+struct Side {
+  const void* src;
+  void* dst;           // of queries, or pages
+  float* scales;
+  int64_t page, scale_page;
+  int t_stride, h_stride, heads, tasks;  // tasks of a token
+};
 struct WriteParams {
-  Cache cache;
-  const void *slots, *q, *k, *v, *positions;
-  void* q_out;
+  Side side[3];
+  const void *slots, *positions;
   const double* frequencies;
-  int qo_t, qo_h, q_t, q_h, k_t, k_h, v_t, v_h;
-  int64_t rows_all;
+  int64_t tokens, places;  // places: of the cache
+  int qo_t, qo_h, page_log2;
   AngleTable table;
-  Divisor by_token;  // rows of a token: of queries, keys, values
-  int q_heads, pairs, wide_slots, wide_positions, interleaved, vectors;  // q_heads: 0 without queries; pairs: 0 without angles
+  Divisor by_token;  // tasks of a token
+  int span;          // tokens of a CTA; 0: parts of tokens
+  int pairs, wide_slots, wide_positions, interleaved, vectors;  // pairs: 0 without angles
   float scale;
 };
 
-// A warp has U groups of 32 / (D / 8) neighbouring rows: it asks for them, takes its share of the CTA's angles and slots while they come, and
-// stores them behind the barrier.
+// The largest magnitude of 8 elements, NaN where there is one.
+__device__ __forceinline__ float peak_of(const Pair (&x)[4]) {
+  float peak = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = halves(x[i]);
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(peak) : "f"(peak), "f"(f.x), "f"(f.y));
+  }
+  return peak;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// A warp's task is U groups of 32 / (D / 8) neighbouring heads of one token's queries, keys or values: it asks for them, takes its
+// share of the CTA's angles and slots while they come, and behind the barrier turns all of them by the angles that it reads once.
 template <typename T, int D, int STORE, int U>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteParams p, int* status) {
-  constexpr int L = D / 8, kRows = kThreads / L;  // lanes of a row, rows at a time
-  constexpr int kMaxTokens = kRows * U / 2 + 1;   // a token has two rows at least
-  __shared__ __align__(16) float angles[kMaxTokens * D];
-  __shared__ long long places[kMaxTokens];
-  const int lane = threadIdx.x & 31, chunk = lane & (L - 1), e0 = chunk * 8;
-  const int64_t row0 = (int64_t)blockIdx.x * (kRows * U), t0 = row0 / p.by_token.d;
-  const uint32_t local0 = (uint32_t)(row0 - t0 * p.by_token.d), n = (uint32_t)min((int64_t)(kRows * U), p.rows_all - row0);
-  const int kv_heads = p.cache.kv_heads;
+__global__ void __launch_bounds__(kMaxWarps * 32, U == 1 ? 1 : 4) kv_write_kernel(const WriteParams p, int* status) {
+  constexpr int L = D / 8, kRows = 32 / L;  // lanes of a row, rows of a group
+  extern __shared__ __align__(16) float angles[];
+  __shared__ long long places[kMaxWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, chunk = lane & (L - 1), e0 = chunk * 8;
+  const int per_token = p.by_token.d;
+  const int64_t task0 = (int64_t)blockIdx.x * (p.span ? p.span * per_token : warps), t0 = p.span ? (int64_t)blockIdx.x * p.span : task0 / per_token;
+  const int local0 = (int)(task0 - t0 * per_token);
+  const int n = (int)min((int64_t)(p.span ? p.span * per_token : warps), p.tokens * per_token - task0);  // tasks of the CTA
+  const int i = min(warp, n - 1), token = p.by_token(local0 + i);
+  const bool busy = warp < n;
+  int r = local0 + i - token * per_token;
+  const int queries = p.side[Query].tasks, keys = p.side[Key].tasks;
+  const int kind = r < queries ? Query : r < queries + keys ? Key : Value;
+  r -= kind == Query ? 0 : kind == Key ? queries : queries + keys;
+  const Side& side = p.side[kind];
+  const int head0 = r * (kRows * U) + lane / L, heads = busy ? side.heads : 0;  // the lane's heads: head0 + k kRows
   grid_dependency_sync();
+  const T* src = static_cast<const T*>(side.src) + ((t0 + token) * side.t_stride + (int64_t)head0 * side.h_stride) + e0;
+  const int64_t next_src = (int64_t)kRows * side.h_stride;
   uint4 asked[U];
-  int token_of[U], row_of[U];  // -1: none
-  auto rows_of = [&](int k, const void*& base, int& head, int& t_stride, int& h_stride) {  // the array that row k is in
-    const int r = row_of[k];
-    const bool key = r < p.q_heads + kv_heads;
-    head = r - (key ? p.q_heads : p.q_heads + kv_heads);
-    base = key ? p.k : p.v;
-    t_stride = key ? p.k_t : p.v_t;
-    h_stride = key ? p.k_h : p.v_h;
-    if (r < p.q_heads) {
-      head = r;
-      base = p.q;
-      t_stride = p.q_t;
-      h_stride = p.q_h;
-    }
-  };
-  auto source = [&](int k) {
-    const void* base;
-    int head, t_stride, h_stride;
-    rows_of(k, base, head, t_stride, h_stride);
-    return static_cast<const T*>(base) + (t0 * t_stride + (int64_t)token_of[k] * t_stride + (int64_t)head * h_stride);
-  };
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const uint32_t i = k * kRows + threadIdx.x / L;
     asked[k] = make_uint4(0, 0, 0, 0);
-    token_of[k] = 0;
-    row_of[k] = -1;
-    if (i >= n) continue;
-    token_of[k] = p.by_token(local0 + i);
-    row_of[k] = (int)(local0 + i) - token_of[k] * (int)p.by_token.d;
-    const T* src = source(k);
-    if (p.vectors) asked[k] = __ldcs(reinterpret_cast<const uint4*>(src + e0));
+    if (head0 + k * kRows >= heads) continue;
+    if (p.vectors) asked[k] = __ldcs(reinterpret_cast<const uint4*>(src + k * next_src));
     else {
       alignas(16) T x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = src[e0 + j];
+      for (int j = 0; j < 8; ++j) x[j] = src[k * next_src + j];
       asked[k] = *reinterpret_cast<const uint4*>(x);
     }
   }
   const int tokens = (int)p.by_token(local0 + n - 1) + 1;
-  if (p.pairs) p.table.fill(angles, p.positions, p.wide_positions, t0, tokens, p.frequencies, p.scale, false, threadIdx.x, kThreads);
-  for (int t = threadIdx.x; t < tokens; t += kThreads) {
+  if (p.pairs) p.table.fill(angles, p.positions, p.wide_positions, t0, tokens, p.frequencies, p.scale, false, threadIdx.x, blockDim.x);
+  for (int t = threadIdx.x; t < tokens; t += blockDim.x) {
     const long long slot = index_at(p.slots, p.wide_slots, t0 + t);
-    const bool bad = slot < 0 || slot > p.cache.tokens;
+    const bool bad = slot < 0 || slot > p.places;
     if (bad) atomicMax(status, (int)DEV_BAD_INDEX);
     places[t] = bad ? -1 : slot - 1;
   }
   __syncthreads();
+  if (!busy) return;
+
+  const float* table = angles + token * 2 * p.pairs;
+  const bool turns = p.pairs && kind != Value, mine = turns && e0 < 2 * p.pairs;  // the lane's elements are turned
+  const bool halves_apart = !p.interleaved && p.pairs % 8 == 0, side_by_side = p.interleaved && p.table.step_log2 == 2;
+  const int half = p.pairs / 8;
+  const bool second = chunk >= half;
+  const int other = mine ? (second ? lane - half : lane + half) : lane;
+  TwoAngles a[4];
+  if (mine && (halves_apart || side_by_side)) {
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int t = token_of[k], r = row_of[k];
-    const bool live = r >= 0, query = r < p.q_heads, value = r >= p.q_heads + kv_heads;
-    const int head = query ? r : value ? r - p.q_heads - kv_heads : r - p.q_heads;
-    const long long place = places[t];
-    const bool stored = live && !query && place >= 0;
-    uint32_t w[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
-    Pair x[4];  // the elements in f32, for 8 bits
-    const bool turned = live && !value && e0 < 2 * p.pairs;
-    const float* table = angles + t * 2 * p.pairs;
-    if (p.pairs) {
-      if (p.interleaved || p.pairs % 8 == 0) {
-        // with pairs (i, i + pairs), a pair's other elements are another lane's eight
-        const int half = p.pairs / 8;
-        const bool second = chunk >= half;
-        uint32_t o[4];
-        if (!p.interleaved) {
-          const int other = turned ? (second ? lane - half : lane + half) : lane;
+    for (int j = 0; j < 4; ++j)
+      if (halves_apart || j < 2) a[j] = angles_of(table, p.table.runs, halves_apart && second ? chunk - half : chunk, j);
+    if (halves_apart && !second) {  // x cos - y sin, and y cos + x sin
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, w[i], other) ^ (second ? 0u : 0x80008000u);
-        }
-        if (turned) {
-          if (!p.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const TwoAngles a = angles_of(table, p.table.runs, second ? chunk - half : chunk, i);
-              x[i] = fma2(vec_pair<T>(o, i), a.sin, mul2(vec_pair<T>(w, i), a.cos));
-            }
-          } else if (p.table.step == 4) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const TwoAngles a = angles_of(table, p.table.runs, chunk, i);
-              Pair u, v;
-              split_pairs<T>(w, i, u, v);
-              const float2 f = halves(fma2(v, minus(a.sin), mul2(u, a.cos))), g = halves(fma2(v, a.cos, mul2(u, a.sin)));
-              x[2 * i] = pair(f.x, g.x);
-              x[2 * i + 1] = pair(f.y, g.y);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[i] = vec_pair<T>(w, i);
-              if (e0 + 2 * i < 2 * p.pairs) {
-                const float2 f = halves(x[i]);
-                const float c = table[e0 + 2 * i], d = table[e0 + 2 * i + 1];
-                x[i] = pair(f.x * c - f.y * d, f.x * d + f.y * c);
-              }
-            }
-          }
-        }
-      } else {
-        if (turned) {
-          const T* src = source(k);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int e = e0 + 2 * i + j;
-              const bool second = e >= p.pairs;
-              const int at = second ? e - p.pairs : e;
-              f[j] = to_float(reinterpret_cast<const T*>(&asked[k])[2 * i + j]);
-              if (e >= 2 * p.pairs) continue;
-              const float y = to_float(src[second ? at : e + p.pairs]);
-              f[j] = f[j] * table[2 * at] + (second ? y : -y) * table[2 * at + 1];
-            }
-            x[i] = pair(f[0], f[1]);
-          }
-        }
-        __syncwarp();  // queries in place: what other lanes read here is written below
-      }
-      if (turned) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put_pair<T>(w, i, x[i]);
-      }
+      for (int j = 0; j < 4; ++j) a[j].sin = minus(a[j].sin);
     }
-    const uint4 words = make_uint4(w[0], w[1], w[2], w[3]);
-    if (live && query) {
-      T* to = static_cast<T*>(p.q_out) + (t0 * p.qo_t + (int64_t)t * p.qo_t + (int64_t)head * p.qo_h) + e0;
-      if (p.vectors) *reinterpret_cast<uint4*>(to) = words;
-      else {
+  }
+  // Turns the eight elements w of a row; x has them in f32.
+  auto turn_row = [&](int k, uint32_t (&w)[4], Pair (&x)[4]) {
+    if (halves_apart) {  // a pair's other elements are another lane's eight
+      uint32_t o[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) to[j] = reinterpret_cast<const T*>(&words)[j];
+      for (int j = 0; j < 4; ++j) o[j] = __shfl_sync(0xffffffffu, w[j], other);
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fma2(vec_pair<T>(o, j), a[j].sin, mul2(x[j], a[j].cos));
       }
-    }
-    if (!__any_sync(0xffffffffu, stored)) continue;
-    const int64_t page = place >> p.cache.page_log2;
-    const int64_t row = (head << p.cache.page_log2) + (int)(place & ((1 << p.cache.page_log2) - 1));
-    if constexpr (STORE == Same) {
-      if (stored) {
-        T* to = static_cast<T*>(value ? p.cache.v : p.cache.k) + page * (value ? p.cache.v_page : p.cache.k_page) + row * D + e0;
-        *reinterpret_cast<uint4*>(to) = words;
+    } else if (side_by_side) {
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          Pair u, v;
+          split_pairs<T>(w, j, u, v);
+          const float2 f = halves(fma2(v, minus(a[j].sin), mul2(u, a[j].cos))), g = halves(fma2(v, a[j].cos, mul2(u, a[j].sin)));
+          x[2 * j] = pair(f.x, g.x);
+          x[2 * j + 1] = pair(f.y, g.y);
+        }
       }
     } else {
+      if (mine && head0 + k * kRows < heads) {  // element by element
+        const T* row = src + k * next_src - e0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int e = e0 + 2 * j + h;
+            const bool later = p.interleaved ? e & 1 : e >= p.pairs;
+            const int at = p.interleaved ? e >> 1 : later ? e - p.pairs : e;
+            f[h] = to_float(reinterpret_cast<const T*>(w)[2 * j + h]);
+            if (e >= 2 * p.pairs) continue;
+            const float y = to_float(row[p.interleaved ? e ^ 1 : later ? at : e + p.pairs]);
+            f[h] = f[h] * table[2 * at] + (later ? y : -y) * table[2 * at + 1];
+          }
+          x[j] = pair(f[0], f[1]);
+        }
+      }
+      __syncwarp();  // queries in place: what other lanes read here is written below
+    }
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put_pair<T>(w, j, x[j]);
+    }
+  };
+  if (kind == Query) {
+    T* to = static_cast<T*>(side.dst) + ((t0 + token) * p.qo_t + (int64_t)head0 * p.qo_h) + e0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      uint32_t w[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
+      Pair x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = vec_pair<T>(w, j);
+      turn_row(k, w, x);
+      if (head0 + k * kRows >= heads) continue;
+      const uint4 words = make_uint4(w[0], w[1], w[2], w[3]);
+      if (p.vectors) *reinterpret_cast<uint4*>(to + (int64_t)k * kRows * p.qo_h) = words;
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[(int64_t)k * kRows * p.qo_h + j] = reinterpret_cast<const T*>(&words)[j];
+      }
+    }
+    return;
+  }
+  const long long place = places[token];
+  if (place < 0) return;
+  const int64_t page = place >> p.page_log2;
+  const int row0 = (head0 << p.page_log2) + (int)(place & ((1 << p.page_log2) - 1)), next_row = kRows << p.page_log2;
+  const int64_t to = page * side.page + (int64_t)row0 * D + e0;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const bool live = head0 + k * kRows < heads;
+    uint32_t w[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
+    Pair x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = vec_pair<T>(w, j);
+    if (turns) turn_row(k, w, x);
+    const int64_t at = to + (int64_t)k * next_row * D;
+    if constexpr (STORE == Same) {
+      if (live) *reinterpret_cast<uint4*>(static_cast<T*>(side.dst) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
       constexpr float kMost = STORE == I8 ? 127.f : 448.f;
-      if (!turned) {
+      float peak = peak_of(x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = vec_pair<T>(w, i);
-      }
-      float peak = 0.f;  // NaN where there is one
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = halves(x[i]);
-        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(peak) : "f"(peak), "f"(f.x), "f"(f.y));
-      }
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) asm("max.NaN.f32 %0, %1, %2;" : "=f"(peak) : "f"(peak), "f"(__shfl_xor_sync(0xffffffffu, peak, o)));
-      if (stored) {
-        const bool fine = peak >= kSmallest && peak < INFINITY;
-        // x c / a with one Newton step behind the product with 1 / a: a quotient that is a number of f32 comes out as it is, so ties are ties
-        const float pre = peak > 1.2676506e30f ? 5.9604645e-8f : 1.f;  // beyond 2^100 in units of 2^24: x c is finite
-        const float a = peak * pre, inv = fine ? __frcp_rn(a) : 0.f, most = pre * kMost;
-        const Pair inv2 = pair(inv, inv), a2 = pair(-a, -a), most2 = pair(most, most);
+      for (int o = L / 2; o > 0; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+      if (!live) continue;
+      // x c / a (and a / c) with a Newton step behind the product with a reciprocal: quotients that are numbers of f32 come out as they are,
+      // so ties are ties
+      const bool fine = peak >= kSmallest && peak < INFINITY;
+      const float pre = peak > 1.2676506e30f ? 5.9604645e-8f : 1.f;  // beyond 2^100 in units of 2^24: x c is finite
+      const float top = peak * pre, inv = rcp_approx_ftz(top), most = pre * kMost;
+      const Pair inv2 = pair(inv, inv), top2 = pair(-top, -top), most2 = pair(most, most);
+      uint2 codes = make_uint2(0, 0);
+      if (fine) {
         float y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const Pair m = mul2(x[i], most2), z = mul2(m, inv2);
-          const float2 f = halves(fma2(fma2(z, a2, m), inv2, z));
-          y[2 * i] = fine ? f.x : 0.f;
-          y[2 * i + 1] = fine ? f.y : 0.f;
+        for (int j = 0; j < 4; ++j) {
+          const Pair m = mul2(x[j], most2), z = mul2(m, inv2);
+          const float2 f = halves(fma2(fma2(z, top2, m), inv2, z));
+          y[2 * j] = f.x;
+          y[2 * j + 1] = f.y;
         }
-        uint2 codes;
         if constexpr (STORE == I8) codes = make_uint2(i8x4(y[0], y[1], y[2], y[3]), i8x4(y[4], y[5], y[6], y[7]));
         else codes = make_uint2(e4m3x4(y[0], y[1], y[2], y[3]), e4m3x4(y[4], y[5], y[6], y[7]));
-        uint8_t* to = static_cast<uint8_t*>(value ? p.cache.v : p.cache.k) + page * (value ? p.cache.v_page : p.cache.k_page) + row * D + e0;
-        *reinterpret_cast<uint2*>(to) = codes;
-        if (chunk == 0)
-          (value ? p.cache.vs : p.cache.ks)[page * (value ? p.cache.vs_page : p.cache.ks_page) + row] = peak < kSmallest ? 0.f : __fdiv_rn(peak, kMost);
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side.dst) + at) = codes;
+      if (chunk == 0) {
+        const float scale = peak * (1.f / kMost);
+        side.scales[page * side.scale_page + row0 + k * next_row] = fine ? fmaf(fmaf(-scale, kMost, peak), 1.f / kMost, scale) : peak < kSmallest ? 0.f : peak;
       }
     }
   }
@@ -361,17 +369,27 @@ int by_type(int dtype, int64_t D, int store, A&&... args) {
 template <typename T, int D, int STORE>
 struct Write {
   template <int U>
-  static int launch(ctb_ctx* ctx, cudaStream_t st, const WriteParams& p) {
-    constexpr int kRows = kThreads / (D / 8) * U;
-    const int64_t grid = (p.rows_all + kRows - 1) / kRows;
+  static int launch(ctb_ctx* ctx, cudaStream_t st, WriteParams p) {
+    int64_t per_token = 0;
+    for (Side& s : p.side) {
+      s.tasks = (s.heads + 256 / D * U - 1) / (256 / D * U);
+      per_token += s.tasks;
+    }
+    p.by_token = Divisor((uint32_t)per_token);
+    p.span = (int)std::min<int64_t>(kMaxWarps / per_token, p.tokens);
+    const int warps = p.span ? (int)(p.span * per_token) : kMaxWarps;
+    const int64_t grid = p.span ? (p.tokens + p.span - 1) / p.span : (p.tokens * per_token + warps - 1) / warps;
     if (grid > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: shape too large");
-    launch_kernel(kv_write_kernel<T, D, STORE, U>, (unsigned)grid, kThreads, 0, st, 0, p, ctx->dev_status);
+    // a CTA has parts of at most two tokens where it cannot have a whole one
+    const size_t smem = (size_t)(p.span ? p.span : 2) * 2 * p.pairs * sizeof(float);
+    launch_kernel(kv_write_kernel<T, D, STORE, U>, (unsigned)grid, warps * 32, smem, st, 0, p, ctx->dev_status);
     CTB_CHECK_LAUNCH("ctb_kv_write launch");
     return CTB_OK;
   }
   static int run(ctb_ctx* ctx, cudaStream_t st, const WriteParams& p) {
-    const int64_t ctas = p.rows_all / (kThreads / (D / 8));
-    return ctas >= 4ll * ctx->sm_count ? launch<4>(ctx, st, p) : launch<1>(ctx, st, p);  // four groups per warp still give every SM a CTA
+    const int64_t heads = p.side[Query].heads + p.side[Key].heads + p.side[Value].heads;
+    // four groups per warp where that still gives every SM 16 warps
+    return p.tokens * heads * D >= 256ll * 4 * 16 * ctx->sm_count ? launch<4>(ctx, st, p) : launch<1>(ctx, st, p);
   }
 };
 template <typename T, int D, int STORE>
@@ -447,21 +465,21 @@ extern "C" int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cach
     const int64_t extents[3] = {1, tokens, heads}, out[3] = {0, strides[0], strides[1]}, in[3] = {0, strides[2], strides[3]};
     if ((r = check_turned_in_place("ctb_kv_write", q, in, q_out, out, extents, cache->head_dim, 2))) return r;
   }
-  WriteParams p = {};
-  p.cache = cache_of(cache);
-  p.slots = slots; p.q = q; p.k = k; p.v = v; p.positions = positions; p.q_out = q_out; p.frequencies = frequencies;
   for (int i = 0; i < 8; ++i)
     if (strides[i] < 0 || strides[i] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: strides too large");
-  p.qo_t = (int)strides[0]; p.qo_h = (int)strides[1]; p.q_t = (int)strides[2]; p.q_h = (int)strides[3];
-  p.k_t = (int)strides[4]; p.k_h = (int)strides[5]; p.v_t = (int)strides[6]; p.v_h = (int)strides[7];
-  const int64_t rows = heads + 2 * cache->kv_heads;
-  p.q_heads = (int)heads;
-  p.by_token = Divisor((uint32_t)rows);
-  p.rows_all = tokens * rows;
+  WriteParams p = {};
+  p.side[Query] = Side{q, q_out, nullptr, 0, 0, (int)strides[2], (int)strides[3], (int)heads, 0};
+  p.side[Key] = Side{k, cache->k, cache->k_scale, cache->k_page_stride, cache->k_scale_page_stride, (int)strides[4], (int)strides[5], (int)cache->kv_heads, 0};
+  p.side[Value] = Side{v, cache->v, cache->v_scale, cache->v_page_stride, cache->v_scale_page_stride, (int)strides[6], (int)strides[7], (int)cache->kv_heads, 0};
+  p.slots = slots; p.positions = positions; p.frequencies = frequencies;
+  p.tokens = tokens;
+  p.places = cache->pages * cache->page_size;
+  p.qo_t = (int)strides[0]; p.qo_h = (int)strides[1];
+  while ((1ll << p.page_log2) < cache->page_size) ++p.page_log2;
   p.pairs = frequencies ? (int)(rotary / 2) : 0;
   // runs of pairs that lie in the eight elements of a lane; where those would not all be full, single ones
-  const int step = interleaved ? 4 : 8;
-  p.table = p.pairs % step ? AngleTable{p.pairs, 1, p.pairs} : AngleTable{p.pairs, step, p.pairs / step};
+  const int step_log2 = interleaved ? 2 : 3;
+  p.table = AngleTable(p.pairs, p.pairs % (1 << step_log2) ? 0 : step_log2);
   p.wide_slots = slot_bits == 64; p.wide_positions = position_bits == 64; p.interleaved = interleaved != 0;
   p.scale = scale;
   p.vectors = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (!heads || ((uintptr_t)q % 16 == 0 && (uintptr_t)q_out % 16 == 0));

@@ -16,7 +16,7 @@ using namespace ctb_internal;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMaxThreads = 256;
 
 struct Side {
   const void* src;
@@ -30,6 +30,7 @@ struct Params {
   AngleTable table;
   Divisor by_seq, by_token, by_units;  // units of a token, of a head
   int64_t units_all;
+  int span;  // units of a CTA
   int tokens, seq, q_heads, dim, turned, wide, interleaved, inverse;
   float scale;
 };
@@ -38,19 +39,19 @@ struct Params {
 // vectors, or with interleaved pairs two neighbouring ones), or for what is only copied two vectors.  A thread asks for its U units, then
 // takes its share of the CTA's angles, and turns the units behind the barrier.
 template <typename T, int V, int U>
-__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const Params p) {
+__global__ void __launch_bounds__(kMaxThreads, 4) rope_kernel(const Params p) {
   using Vec = std::conditional_t<V == 1, T, uint4>;
   extern __shared__ __align__(16) float angles[];
-  const int64_t unit0 = (int64_t)blockIdx.x * (kThreads * U);
+  const int64_t unit0 = (int64_t)blockIdx.x * p.span;
   const int t0 = (int)(unit0 / p.by_token.d);
-  const uint32_t local0 = (uint32_t)(unit0 - (int64_t)t0 * p.by_token.d), n = (uint32_t)min((int64_t)(kThreads * U), p.units_all - unit0);
+  const uint32_t local0 = (uint32_t)(unit0 - (int64_t)t0 * p.by_token.d), n = (uint32_t)min((int64_t)p.span, p.units_all - unit0);
   grid_dependency_sync();
   Vec x[U], y[U];
   T* to[U];
   int at[U], run[U], e0[U], e1[U];  // angles of the unit's token (-1: none) and run, the first elements of its vectors
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const uint32_t i = threadIdx.x + k * kThreads;
+    const uint32_t i = threadIdx.x + k * blockDim.x;
     to[k] = nullptr;
     if (i >= n) continue;
     const uint32_t t = p.by_token(local0 + i), r = local0 + i - t * p.by_token.d, h = p.by_units(r), u = r - h * p.by_units.d;
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const Params p) {
     }
   }
   const int tokens = (int)p.by_token(local0 + n - 1) + 1;
-  p.table.fill(angles, p.positions, p.wide, t0, tokens, p.frequencies, p.scale, p.inverse, threadIdx.x, kThreads);
+  p.table.fill(angles, p.positions, p.wide, t0, tokens, p.frequencies, p.scale, p.inverse, threadIdx.x, blockDim.x);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < U; ++k) {
@@ -119,18 +120,16 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const Params p) {
 }
 
 template <typename T, int V, int U>
-int launch(ctb_ctx*, cudaStream_t st, const Params& p) {
-  const int64_t grid = (p.units_all + kThreads * U - 1) / (kThreads * U);
+int launch(cudaStream_t st, Params p) {
+  const int64_t per_token = p.by_token.d;
+  // Whole tokens where one fits: their angles are worked out once.
+  p.span = (int)(kMaxThreads * U >= per_token ? kMaxThreads * U / per_token * per_token : kMaxThreads * U);
+  const int threads = (p.span + 32 * U - 1) / (32 * U) * 32;
+  const int64_t grid = (p.units_all + p.span - 1) / p.span, tokens = std::max<int64_t>(p.span / per_token, 1) + (p.span % per_token != 0);  // that a CTA has units of
   if (grid > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_rope: shape too large");
-  const int64_t tokens = std::min<int64_t>(p.tokens, kThreads * U / p.by_token.d + 2);  // that a CTA has units of
-  const size_t smem = tokens * 2 * p.table.pairs * sizeof(float), most = 200 * 1024;
-  if (smem > most) return fail(CTB_UNSUPPORTED, "ctb_rope: shape too large");
+  const size_t smem = tokens * 2 * p.table.pairs * sizeof(float);
   auto kern = rope_kernel<T, V, U>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = allow_smem(kern, most);
-    if (e != cudaSuccess) return cuda_fail(e, "ctb_rope: shared memory opt-in");
-  }
-  launch_kernel(kern, (unsigned)grid, kThreads, smem, st, 0, p);
+  launch_kernel(kern, (unsigned)grid, threads, smem, st, 0, p);
   CTB_CHECK_LAUNCH("ctb_rope launch");
   return CTB_OK;
 }
@@ -138,16 +137,16 @@ int launch(ctb_ctx*, cudaStream_t st, const Params& p) {
 template <typename T>
 int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int heads, bool vectors) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int v = vectors ? V : 1;
-  p.turned = p.table.pairs / v;
-  p.table = AngleTable{p.table.pairs, v, p.turned};
-  const int units = p.turned + (p.dim - 2 * p.table.pairs + 2 * v - 1) / (2 * v);
+  const int v = vectors ? V : 1, pairs = p.table.pairs;
+  p.turned = pairs / v;
+  p.table = AngleTable(pairs, v == 8 ? 3 : v == 4 ? 2 : 0);
+  const int units = p.turned + (p.dim - 2 * pairs + 2 * v - 1) / (2 * v);
   p.by_units = Divisor(units);
   p.by_token = Divisor(units * heads);
   p.units_all = (int64_t)p.tokens * units * heads;
-  const bool many = p.units_all >= (int64_t)kThreads * 8 * ctx->sm_count;  // two units per thread still give every SM four CTAs
-  if (vectors) return many ? launch<T, V, 2>(ctx, st, p) : launch<T, V, 1>(ctx, st, p);
-  return many ? launch<T, 1, 2>(ctx, st, p) : launch<T, 1, 1>(ctx, st, p);
+  const bool many = p.units_all >= (int64_t)kMaxThreads * 2 * 4 * ctx->sm_count;  // two units per thread still give every SM four CTAs
+  if (vectors) return many ? launch<T, V, 2>(st, p) : launch<T, V, 1>(st, p);
+  return many ? launch<T, 1, 2>(st, p) : launch<T, 1, 1>(st, p);
 }
 
 }  // namespace

@@ -31,19 +31,22 @@ __device__ __forceinline__ float2 turn(long long position, double frequency, flo
   return make_float2(c * scale, s * scale);
 }
 
-// The angles of a few tokens in shared memory.  Threads take neighbouring runs of `step` pairs and read the k-th and (k + 1)-th pair of
-// their runs at the same time, so these lie together, as (cos, cos, sin, sin), next to those of the other runs.  step 1: (cos, sin).
+// The angles of a few tokens in shared memory.  Threads take neighbouring runs of 2^step_log2 pairs and read the k-th and (k + 1)-th pair of
+// their runs at the same time, so these lie together, as (cos, cos, sin, sin), next to those of the other runs.  A step of 1: (cos, sin).
 struct AngleTable {
-  int pairs, step, runs;  // runs * step = pairs
+  int pairs, step_log2, runs;  // runs << step_log2 = pairs
+  Divisor by_pairs;
+  AngleTable() = default;
+  AngleTable(int pairs, int step_log2) : pairs(pairs), step_log2(step_log2), runs(pairs >> step_log2), by_pairs(pairs ? pairs : 1) {}
   __device__ __forceinline__ void fill(float* table, const void* positions, bool wide, int64_t t0, int tokens, const double* frequencies,
                                        float scale, bool inverse, int thread, int threads) const {
     for (int i = thread; i < tokens * pairs; i += threads) {
-      const int t = i / pairs, pair = i - t * pairs;
+      const int t = by_pairs(i), pair = i - t * pairs;
       const float2 a = turn(index_at(positions, wide, t0 + t), __ldg(frequencies + pair), scale);
-      const int run = pair / step, k = pair - run * step;
-      float* to = table + 2 * t * pairs + (step == 1 ? 2 * pair : ((k >> 1) * runs + run) * 4 + (k & 1));
+      const int run = pair >> step_log2, k = pair - (run << step_log2);
+      float* to = table + 2 * t * pairs + (step_log2 == 0 ? 2 * pair : ((k >> 1) * runs + run) * 4 + (k & 1));
       to[0] = a.x;
-      to[step == 1 ? 1 : 2] = inverse ? -a.y : a.y;
+      to[step_log2 == 0 ? 1 : 2] = inverse ? -a.y : a.y;
     }
   }
 };
