@@ -8,7 +8,7 @@
 
 #include "ctx.h"
 #include "ptx.cuh"
-#include "rotate.cuh"
+#include "rope.cuh"
 
 using namespace ctb;
 using namespace ctb_internal;
@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;       // of a CTA that reads
 constexpr int kMaxWarps = 8;        // of one that writes
+static_assert(kMaxWarps * 32 == kRopeThreads, "CTAs of both kinds in one launch");
 constexpr float kSmallest = 7.888609052210118e-31f;  // 2^-100: rows below it are zeros in 8 bits
 
 enum Store { Same = 0, E4M3 = 1, I8 = 2 };
@@ -67,6 +68,8 @@ struct WriteParams {
   int span;          // tokens of a CTA; 0: parts of tokens
   int pairs, wide_slots, wide_positions, interleaved, vectors;  // pairs: 0 without angles
   float scale;
+  int rope_vectors, ctas, period;  // CTAs with tasks, one in `period`; the others turn queries
+  RopeParams rope;
 };
 
 // The largest magnitude of 8 elements, NaN where there is one.
@@ -87,14 +90,27 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // A warp's task is U groups of 32 / (D / 8) neighbouring heads of one token's queries, keys or values: it asks for them, takes its
 // share of the CTA's angles and slots while they come, and behind the barrier turns all of them by the angles that it reads once.
+// U > 1: many tokens, whose queries are other CTAs' of the same launch, in between: turning them is bound by HBM, rounding to codes by the
+// issue of instructions.
 template <typename T, int D, int STORE, int U>
 __global__ void __launch_bounds__(kMaxWarps * 32, U == 1 ? 1 : 4) kv_write_kernel(const WriteParams p, int* status) {
   constexpr int L = D / 8, kRows = 32 / L;  // lanes of a row, rows of a group
   extern __shared__ __align__(16) float angles[];
   __shared__ long long places[kMaxWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, chunk = lane & (L - 1), e0 = chunk * 8;
+  int cta = blockIdx.x;
+  if constexpr (U > 1) {
+    if (cta >= p.ctas * p.period || cta % p.period) {
+      grid_dependency_sync();
+      cta -= cta >= p.ctas * p.period ? p.ctas : cta / p.period + 1;
+      if (p.rope_vectors) rope_cta<T, 8, 2>(p.rope, cta, angles);
+      else rope_cta<T, 1, 2>(p.rope, cta, angles);
+      return;
+    }
+    cta /= p.period;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kMaxWarps, chunk = lane & (L - 1), e0 = chunk * 8;
   const int per_token = p.by_token.d;
-  const int64_t task0 = (int64_t)blockIdx.x * (p.span ? p.span * per_token : warps), t0 = p.span ? (int64_t)blockIdx.x * p.span : task0 / per_token;
+  const int64_t task0 = (int64_t)cta * (p.span ? p.span * per_token : warps), t0 = p.span ? (int64_t)cta * p.span : task0 / per_token;
   const int local0 = (int)(task0 - t0 * per_token);
   const int n = (int)min((int64_t)(p.span ? p.span * per_token : warps), p.tokens * per_token - task0);  // tasks of the CTA
   const int i = min(warp, n - 1), token = p.by_token(local0 + i);
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, U == 1 ? 1 : 4) kv_write_kerne
       for (int j = 0; j < 4; ++j) put_pair<T>(w, j, x[j]);
     }
   };
-  if (kind == Query) {
+  if (U == 1 && kind == Query) {
     T* to = static_cast<T*>(side.dst) + ((t0 + token) * p.qo_t + (int64_t)head0 * p.qo_h) + e0;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -242,20 +258,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32, U == 1 ? 1 : 4) kv_write_kerne
       const float pre = peak > 1.2676506e30f ? 5.9604645e-8f : 1.f;  // beyond 2^100 in units of 2^24: x c is finite
       const float top = peak * pre, inv = rcp_approx_ftz(top), most = pre * kMost;
       const Pair inv2 = pair(inv, inv), top2 = pair(-top, -top), most2 = pair(most, most);
-      uint2 codes = make_uint2(0, 0);
-      if (fine) {
-        float y[8];
+      float y[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Pair m = mul2(x[j], most2), z = mul2(m, inv2);
-          const float2 f = halves(fma2(fma2(z, top2, m), inv2, z));
-          y[2 * j] = f.x;
-          y[2 * j + 1] = f.y;
-        }
-        if constexpr (STORE == I8) codes = make_uint2(i8x4(y[0], y[1], y[2], y[3]), i8x4(y[4], y[5], y[6], y[7]));
-        else codes = make_uint2(e4m3x4(y[0], y[1], y[2], y[3]), e4m3x4(y[4], y[5], y[6], y[7]));
+      for (int j = 0; j < 4; ++j) {
+        const Pair m = mul2(x[j], most2), z = mul2(m, inv2);
+        const float2 f = halves(fma2(fma2(z, top2, m), inv2, z));
+        y[2 * j] = f.x;
+        y[2 * j + 1] = f.y;
       }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side.dst) + at) = codes;
+      uint2 codes;
+      if constexpr (STORE == I8) codes = make_uint2(i8x4(y[0], y[1], y[2], y[3]), i8x4(y[4], y[5], y[6], y[7]));
+      else codes = make_uint2(e4m3x4(y[0], y[1], y[2], y[3]), e4m3x4(y[4], y[5], y[6], y[7]));
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side.dst) + at) = fine ? codes : make_uint2(0, 0);
       if (chunk == 0) {
         const float scale = peak * (1.f / kMost);
         side.scales[page * side.scale_page + row0 + k * next_row] = fine ? fmaf(fmaf(-scale, kMost, peak), 1.f / kMost, scale) : peak < kSmallest ? 0.f : peak;
@@ -370,26 +384,34 @@ template <typename T, int D, int STORE>
 struct Write {
   template <int U>
   static int launch(ctb_ctx* ctx, cudaStream_t st, WriteParams p) {
-    int64_t per_token = 0;
+    int64_t per_token = 0, queries = 0;
+    int threads = kMaxWarps * 32;
+    size_t rope_smem = 0;
+    if (U > 1 && p.side[Query].heads) {
+      queries = p.rope_vectors ? rope_shares<8, 2>(p.rope, &threads, &rope_smem) : rope_shares<1, 2>(p.rope, &threads, &rope_smem);
+      p.side[Query].heads = 0;
+    }
     for (Side& s : p.side) {
       s.tasks = (s.heads + 256 / D * U - 1) / (256 / D * U);
       per_token += s.tasks;
     }
     p.by_token = Divisor((uint32_t)per_token);
     p.span = (int)std::min<int64_t>(kMaxWarps / per_token, p.tokens);
-    const int warps = p.span ? (int)(p.span * per_token) : kMaxWarps;
-    const int64_t grid = p.span ? (p.tokens + p.span - 1) / p.span : (p.tokens * per_token + warps - 1) / warps;
-    if (grid > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: shape too large");
+    const int64_t ctas = p.span ? (p.tokens + p.span - 1) / p.span : (p.tokens * per_token + kMaxWarps - 1) / kMaxWarps;
+    if (ctas + queries > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: shape too large");
+    p.ctas = (int)ctas;
+    p.period = (int)((ctas + queries) / ctas);
     // a CTA has parts of at most two tokens where it cannot have a whole one
-    const size_t smem = (size_t)(p.span ? p.span : 2) * 2 * p.pairs * sizeof(float);
-    launch_kernel(kv_write_kernel<T, D, STORE, U>, (unsigned)grid, warps * 32, smem, st, 0, p, ctx->dev_status);
+    const size_t smem = std::max(rope_smem, (size_t)(p.span ? p.span : 2) * 2 * p.pairs * sizeof(float));
+    launch_kernel(kv_write_kernel<T, D, STORE, U>, (unsigned)(ctas + queries), kMaxWarps * 32, smem, st, 0, p, ctx->dev_status);
     CTB_CHECK_LAUNCH("ctb_kv_write launch");
     return CTB_OK;
   }
   static int run(ctb_ctx* ctx, cudaStream_t st, const WriteParams& p) {
     const int64_t heads = p.side[Query].heads + p.side[Key].heads + p.side[Value].heads;
-    // four groups per warp where that still gives every SM 16 warps
-    return p.tokens * heads * D >= 256ll * 4 * 16 * ctx->sm_count ? launch<4>(ctx, st, p) : launch<1>(ctx, st, p);
+    // four groups per warp (two where a token's keys have no more) where that still gives every SM 16 warps
+    if (p.tokens * heads * D < 256ll * 4 * 16 * ctx->sm_count) return launch<1>(ctx, st, p);
+    return p.side[Key].heads * D > 256 * 2 ? launch<4>(ctx, st, p) : launch<2>(ctx, st, p);
   }
 };
 template <typename T, int D, int STORE>
@@ -484,6 +506,15 @@ extern "C" int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cach
   p.scale = scale;
   p.vectors = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (!heads || ((uintptr_t)q % 16 == 0 && (uintptr_t)q_out % 16 == 0));
   for (int i = heads ? 0 : 4; i < 8; ++i) p.vectors &= strides[i] % 8 == 0;
+  if (heads) {
+    p.rope.side[0] = RopeSide{q, q_out, 0, p.side[Query].t_stride, p.side[Query].h_stride, 0, p.qo_t, p.qo_h, (int)heads};
+    p.rope.positions = positions; p.rope.frequencies = frequencies;
+    p.rope.table.pairs = p.pairs;
+    p.rope.by_seq = Divisor((uint32_t)tokens);
+    p.rope.tokens = (int)tokens; p.rope.q_heads = (int)heads; p.rope.dim = (int)cache->head_dim;
+    p.rope.wide = p.wide_positions; p.rope.interleaved = p.interleaved; p.rope.scale = scale;
+    p.rope_vectors = p.vectors && rotary % 16 == 0;
+  }
   return by_type<Write>(dtype, cache->head_dim, cache->dtype, ctx, static_cast<cudaStream_t>(stream), p);
 }
 
