@@ -20,7 +20,6 @@ namespace {
 enum Store { F16 = 0, BF16 = 1, E4M3 = 2, I8 = 3 };
 
 constexpr int kMaxBatch = 1024;  // sequences of a launch (their lengths lie in shared memory)
-constexpr int kMinTiles = 2;     // of a warp, where there is that much work
 constexpr unsigned kItemCost = 1;  // tiles that an item counts more than it has
 constexpr unsigned kWholeItems = 80;  // tiles of the longest item up to which CTAs have whole items
 // Exponents' reference (in powers of two): it moves once a score stands kLazy above the largest that it knows.  What goes to f16 is lifted
@@ -179,7 +178,8 @@ struct Cursor {
   int b, head, rt, key, len;  // head: of the keys and values
 };
 
-template <int STORE, int D, int NT>
+// PAIR: probabilities go to the product as two 16-bit numbers.
+template <int STORE, int D, int NT, bool PAIR>
 __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     fmha_paged_kernel(const Params p, int* status) {
   using S = Shape<STORE, D, NT>;
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   // Ranges of the line of tiles: equal ones for all warps of the grid, or, where items are short, for the warps of a CTA, whose range
   // ends where an item ends.
   const bool whole_items = longest <= kWholeItems;
-  const Shares shares(total, whole_items ? gridDim.x : min(gridDim.x * kWarps, (total + kMinTiles - 1) / kMinTiles));
+  const Shares shares(total, whole_items ? gridDim.x : min(gridDim.x * kWarps, total));
   unsigned cta_lo, cta_hi, lo, hi;
   if (whole_items) {
     auto end_of = [&](unsigned i) {  // the end of an item that is next to the end of an equal range
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
               }
           }
         }
-        // ---- O += V P.  Probabilities are the sum of two 16-bit numbers beside 16-bit values, one f16 beside 8-bit ones.
+        // ---- O += V P
         const uint32_t v_even = ring + slot * S::kEntry + v_at;
         [[maybe_unused]] const uint32_t v_odd = v_even ^ 16;
         unrolled<KT>([&](auto tag) {
@@ -649,12 +649,12 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if constexpr (S::kBytes) hi_[n][h] = transposed(pack2<false>(sc[s][n][2 * h], sc[s][n][2 * h + 1]));
-              else {
-                const uint32_t w = pack2<BF>(d[s][n][2 * h], d[s][n][2 * h + 1]);
+              const float a = S::kBytes ? sc[s][n][2 * h] : d[s][n][2 * h], z = S::kBytes ? sc[s][n][2 * h + 1] : d[s][n][2 * h + 1];
+              const uint32_t w = pack2<BF>(a, z);
+              hi_[n][h] = transposed(w);
+              if constexpr (PAIR) {
                 const float2 f = unpack2<BF>(w);
-                hi_[n][h] = transposed(w);
-                lo_[n][h] = transposed(pack2<BF>(d[s][n][2 * h] - f.x, d[s][n][2 * h + 1] - f.y));
+                lo_[n][h] = transposed(pack2<BF>(a - f.x, z - f.y));
               }
             }
           // rows behind the last key may hold anything: 0 x NaN is NaN
@@ -690,7 +690,10 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], hi_[n][0], hi_[n][1]);
+                for (int n = 0; n < NT; ++n) {
+                  mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], hi_[n][0], hi_[n][1]);
+                  if constexpr (PAIR) mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], lo_[n][0], lo_[n][1]);
+                }
             }
           } else {
             const uint32_t mask0 = (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   const uint32_t marked = __ballot_sync(0xffffffffu, seg.x != ~0u), below = marked & ((1u << lane) - 1);
   const uint32_t item_below = __shfl_sync(0xffffffffu, seg.x, below ? 31 - __clz(below) : 0);
   uint32_t leaders = __ballot_sync(0xffffffffu, seg.x != ~0u && (!below || item_below != seg.x));
-  uint4 shared_item[2] = {make_uint4(~0u, 0, 0, 0), make_uint4(~0u, 0, 0, 0)};  // that other CTAs have a part of: the first and the last of the range
+  uint4 shared_first = make_uint4(~0u, 0, 0, 0), shared_last = shared_first;  // that other CTAs have a part of: the first and the last of the range
   for (int task = 0; leaders; leaders &= leaders - 1) {
     const int s = __ffs(leaders) - 1;
     const uint32_t later = leaders & (leaders - 1), members = marked & ~((1u << s) - 1) & (later ? (later & -later) - 1 : ~0u);
@@ -835,23 +838,24 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
                                   __shfl_sync(0xffffffffu, seg.w, s));
     const bool inside = item.z >= cta_lo && item.w <= cta_hi;
     const int which = item.z < cta_lo ? 0 : 1;
-    if (!inside) shared_item[which] = item;
+    if (!inside && which == 0) shared_first = item;
+    if (!inside && which == 1) shared_last = item;
     float* part = inside ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + which) * S::kPartFloats;
     for (int row = (warp + kWarps - task % kWarps) % kWarps; row < (int)item.y; row += kWarps) join_row(members, item.x, row, part);
     task += item.y;
   }
-  if (shared_item[0].x == ~0u && shared_item[1].x == ~0u) return;
+  if (shared_first.x == ~0u && shared_last.x == ~0u) return;
   // ---- Items that several CTAs had: the one that is done last adds the parts.
   auto cta_of = [&](unsigned x) { return (int)(shares.owner(x) / kWarps); };
   __syncthreads();
   if (tid < 2) {
     last_s[tid] = 0;
-    const uint4 item = tid ? shared_item[1] : shared_item[0];
+    const uint4 item = tid ? shared_last : shared_first;
     if (item.x != ~0u) {
       const int c0 = cta_of(item.z), parts = cta_of(item.w - 1) - c0;
-      __threadfence();
-      last_s[tid] = atomicInc(&p.tickets[c0], parts) == parts;  // back to zero by the last
-      __threadfence();
+      unsigned before;  // back to zero by the last; what the CTA has written (it met above) comes before, what it reads below behind
+      asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(before) : "l"(p.tickets + c0), "r"(parts) : "memory");
+      last_s[tid] = before == (unsigned)parts;
     }
   }
   __syncthreads();
@@ -859,7 +863,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (!last[which]) continue;
-    const uint4 item = shared_item[which];
+    const uint4 item = which ? shared_last : shared_first;
     // warp w takes the parts c0 + w, c0 + w + kWarps, ...: vector i of a lane is number i * 32 + lane of the part's rows
     const int c0 = cta_of(item.z), c1 = cta_of(item.w - 1), rows = item.y;
     constexpr int kVecs = R * D / 4 / 32;
@@ -906,8 +910,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   }
 }
 
-template <int STORE, int D, int NT>
-int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
+template <int STORE, int D, int NT, bool PAIR>
+int launch_as(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   using S = Shape<STORE, D, NT>;
   static_assert(S::kSmem <= 227 * 1024, "shared memory of a CTA");
   p.row_tiles = (p.group + S::R - 1) / S::R;
@@ -917,7 +921,7 @@ int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   const int64_t chunk = std::min<int64_t>(kMaxBatch, INT32_MAX / tiles);
   if ((size_t)ctx->sm_count * 2 * S::kPartFloats * sizeof(float) > kSlotBytes || ctx->sm_count > kTickets)
     return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: more SMs than the split over keys has scratch for");
-  auto kern = fmha_paged_kernel<STORE, D, NT>;
+  auto kern = fmha_paged_kernel<STORE, D, NT, PAIR>;
   cudaError_t e = allow_smem(kern, S::kSmem);
   if (e != cudaSuccess) return cuda_fail(e, "ctb_fmha_paged: shared memory opt-in");
   const StreamScratch scratch(ctx, st);
@@ -936,6 +940,16 @@ int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
     CTB_CHECK_LAUNCH("ctb_fmha_paged launch");
   }
   return CTB_OK;
+}
+
+// One f16 (2^-11 of a probability) is enough for results in bf16 from 8-bit values; results in f16 would be half as far off again as
+// their own rounding makes them (3.0e-4 for 2.0e-4).
+template <int STORE, int D, int NT>
+int launch(ctb_ctx* ctx, cudaStream_t st, const Params& p, int64_t batch) {
+  if constexpr (STORE >= E4M3) {
+    if (p.q_bf16) return launch_as<STORE, D, NT, false>(ctx, st, p, batch);
+  }
+  return launch_as<STORE, D, NT, true>(ctx, st, p, batch);
 }
 
 template <int STORE>

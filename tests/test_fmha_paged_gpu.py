@@ -4,7 +4,7 @@ With c the scale, S = c max_j sum_i |q_i k_ji| and W = sum_j p_j |v_j| (for one 
 sums lose, 2^-19 S at most (sums of 16 products at a time, each rounded or cut off to 24 bits), and by the roundings of its scale, its 8-bit
 scale and its distance from the reference (2^-21 of the score, again below S); queries in bf16 over 8-bit keys lose 2^-33 of a row's
 largest element.  Probabilities are therefore off by 2^-18 S + 2^-22 (ex2) relative to each other, which moves o by twice that of W; they
-enter as two 16-bit numbers (2^-17), beside 8-bit values as one f16 (2^-11), and the sums over keys and over parts take 24-bit roundings, 2^-17 W for up to 2^7 of them in a
+enter as two 16-bit numbers (2^-17), in bf16 beside 8-bit values as one f16 (2^-11), and the sums over keys and over parts take 24-bit roundings, 2^-17 W for up to 2^7 of them in a
 row (a tile of a part adds one; longer parts are averages).  Pairs of f16 numbers, where the type or the cache's eight bits ask for them, have a
 smallest step, 2^-24, and hold numbers whose largest is brought to 2^8 or more: a probability (with its value's scale) is off by 2^-33 of
 the largest of the row besides, F = 2^-33 max_j (p_j s_j) sum_j |v_j| / s_j, s = 1 without scales.  One rounding to the type at the end.  lse: the scores' part, and 2^-20 of
@@ -91,7 +91,7 @@ class Case:
             S = (torch.einsum("hgd,hnd->hgn", q.abs(), k.abs()).amax(-1) * abs(scale))[..., None]
             p = torch.softmax(s, -1)
             o, W = torch.einsum("hgn,hnd->hgd", p, v), torch.einsum("hgn,hnd->hgd", p, v.abs())
-            F, P = torch.zeros_like(o), 2.0 ** -17 if self.cache.v_scale is None else 2.0 ** -11
+            F, P = torch.zeros_like(o), 2.0 ** -17 if self.cache.v_scale is None or self.dtype == torch.float16 else 2.0 ** -11
             if self.cache.v_scale is not None:
                 at = self.table[b, :-(-k.shape[1] // self.page)].long() - 1
                 codes = self.cache.v[at].float().double().transpose(0, 1).flatten(1, 2)[:, :k.shape[1]].abs().sum(1)
