@@ -2,6 +2,32 @@
 // query head, with the heads of a group as rows of one operand.
 //
 // What bounds it is HBM: every stored key and value is read once, 2 D bytes times the element's size, against 4 D operations per row.
+// 64 sequences of up to 8000 tokens, 64 heads over 8 of 128 in bf16 (1018 MB): 161 us, 6.3 TB/s, 0.97 of the copy rate; one sequence of
+// 131072 in f16 89 us (0.92); 128 of up to 4096 in e4m3 (560 MB) 102 us (0.84); 4 of up to 500 9 us, which are latencies: lengths (0.9 us),
+// ranges (0.5), page numbers (1.1), the first keys (0.6), tiles, meeting (1) and joining (1).
+//
+// Work is cut into tiles of 16 to 64 keys of one item (a sequence, a key/value head, a row of up to 16 heads of its group); 4 KB of keys and
+// 4 KB of values each.  The tiles of all items form one line that the warps of the grid share out in equal contiguous ranges, whatever the
+// lengths are: every CTA finds the tiles before every sequence by a scan over the lengths, which only the device knows.  An item counts a
+// tile more than it has, for its queries and results (attend 64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
+// longest item has at most kWholeItems tiles, ranges of CTAs end where items end, so that no CTA has to wait for another's part (16
+// x 1000 keys 15.9 us with parts, 12.8 with whole items; 8 x 4000 in e4m3, 125 tiles, 20.1 and 25.6 us).  A warp leaves an item that it has
+// as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
+// takes rows of parts to join, and items that several CTAs have are joined by the one that arrives last, in ascending order of the parts.  The
+// ranges hang on the lengths alone, so that results are the same from run to run.
+//
+// A warp streams its range for itself: it asks for keys and values in turn, an entry of 4 KB of its ring in shared memory each, three
+// entries ahead of the one that it reads (144 KB on the way per SM), by asynchronous copies of 16 bytes per lane.  Rows are exchanged in chunks
+// as they are copied, so that no read meets a bank conflict.  Ways that were slower: keys and values straight into registers, 12 warps
+// (attend_batch 169 us, 8-bit caches 151 for 102); bulk and tensor copies by a lane of every warp (177, 154) or by a warp for all
+// (181, 206): a copy costs its warp about 100 clocks, and pages of 16 tokens make many small ones; 8 or 10 warps with longer rings, 16 with
+// shorter ones (8-bit caches 115, 112, 120).
+//
+// S^T = K Q^T and O^T += V^T P^T are m16n8k16 tensor-core instructions with the keys (the dimensions) as the 16 rows and up to eight heads as
+// the columns: a tcgen05 tile of 128 rows would be 94 % padding, and the tensor work is an eighth of what this path delivers.
+// A lane reads 16-byte chunks of a key and takes its dimensions in the order in which they come, queries accordingly.  Probabilities go from the
+// accumulators' layout into the operand's by a transposition in registers, 16-bit values by transposing loads, 8-bit codes by byte
+// permutes; codes become f16 as they are read (exact), their scales multiply scores and probabilities.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -20,7 +46,7 @@ namespace {
 enum Store { F16 = 0, BF16 = 1, E4M3 = 2, I8 = 3 };
 
 constexpr int kMaxBatch = 1024;  // sequences of a launch (their lengths lie in shared memory)
-constexpr unsigned kItemCost = 1;  // tiles that an item counts more than it has
+constexpr unsigned kItemCost = 1;     // tiles that an item counts more than it has
 constexpr unsigned kWholeItems = 80;  // tiles of the longest item up to which CTAs have whole items
 // Exponents' reference (in powers of two): it moves once a score stands kLazy above the largest that it knows.  What goes to f16 is lifted
 // by kLift, so that the largest is at most 2^(kLazy + kLift + 1) and what f16 pairs cannot tell from 0 is 2^-(25 + kLift) of it.

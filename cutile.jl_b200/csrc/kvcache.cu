@@ -1,7 +1,12 @@
 // The paged key-value cache: writing new tokens to it (turned by their positions and rounded to 8 bits on the way) and reading sequences back.
 //
-// What bounds both is HBM.  A row (one head of one token) is the work of D / 8 neighbouring lanes, eight elements each, so that its
-// largest magnitude is found by a few shuffles and its pairs (i, i + rotary / 2) meet by one.
+// Reading is bound by HBM: 4 x 4096 tokens of 8 heads of 128 from e4m3 (101 MB) 15.2 us, the copy rate.
+// Writing: by HBM in 16 bits (10240 tokens with 32 + 8 + 8 heads of 128 in bf16, 252 MB, 48 us for 38), by the issue of instructions in 8
+// (in e4m3 51 us for 35; int8, keys and values alone, without angles, 20 for 10: a row's maximum, two products and a Newton step per
+// element, and the codes, 180 instructions per 256 elements); few tokens by latencies (64: 2.3 us).  A row (one head of one token) is the
+// work of D / 8 neighbouring lanes, eight elements each, so that its largest magnitude is found by a few shuffles and its pairs (i, i +
+// rotary / 2) meet by one.  Slower: all kinds of rows in the same warps (84 to 98 us for the 51), CTAs that walk over the tokens and ask a
+// round ahead (96: registers), one group of rows per warp (110).
 #include <math.h>
 
 #include <algorithm>

@@ -20,14 +20,14 @@ struct Divisor {
   __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (n + __umulhi(n, m)) >> s; }
 };
 
-// scale * (cos, sin) of position * frequency.  The product and its reduction to a turn are in f64: an f32 angle of a far position
-// (1e6 radians) has no digits left behind the point.  sincospif then takes half turns in [-1, 1], where its argument is off by
-// 2^-25 at most.
+// scale * (cos, sin) of position * frequency.  The product and its reduction to half a turn are in f64, the latter by 2 pi in two
+// numbers: an f32 angle of a far position (1e6 radians) has no digits left behind the point.  sincospif then takes half turns in [-1, 1], where
+// its argument is off by 2^-25 at most.
 __device__ __forceinline__ float2 turn(long long position, double frequency, float scale) {
-  double t = (double)position * (frequency * 0.15915494309189535);  // turns
-  t -= rint(t);
+  const double a = (double)position * frequency, n = rint(a * 0.15915494309189535);
+  const double r = fma(n, -2.4492935982947064e-16, fma(n, -6.283185307179586, a));
   float s, c;
-  sincospif((float)(2.0 * t), &s, &c);
+  sincospif((float)(r * 0.3183098861837907), &s, &c);
   return make_float2(c * scale, s * scale);
 }
 
