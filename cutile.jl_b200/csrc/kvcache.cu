@@ -487,21 +487,24 @@ extern "C" int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cach
   if (tokens == 0) return CTB_OK;
   CTB_CHECK_DEV(slots); CTB_CHECK_DEV(k); CTB_CHECK_DEV(v);
   if (frequencies) { CTB_CHECK_DEV(positions); CTB_CHECK_DEV(frequencies); }
+  int64_t s[8];  // none along what has one element
+  for (int i = 0; i < 8; ++i) {
+    s[i] = (i & 1 ? (i < 4 ? heads : cache->kv_heads) : tokens) == 1 ? 0 : strides[i];
+    if ((heads || i >= 4) && (s[i] < 0 || s[i] > INT32_MAX)) return fail(CTB_UNSUPPORTED, "ctb_kv_write: strides too large");
+  }
   if (heads) {
     CTB_CHECK_DEV(q); CTB_CHECK_DEV(q_out);
-    const int64_t extents[3] = {1, tokens, heads}, out[3] = {0, strides[0], strides[1]}, in[3] = {0, strides[2], strides[3]};
+    const int64_t extents[3] = {1, tokens, heads}, out[3] = {0, s[0], s[1]}, in[3] = {0, s[2], s[3]};
     if ((r = check_turned_in_place("ctb_kv_write", q, in, q_out, out, extents, cache->head_dim, 2))) return r;
   }
-  for (int i = 0; i < 8; ++i)
-    if (strides[i] < 0 || strides[i] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_kv_write: strides too large");
   WriteParams p = {};
-  p.side[Query] = Side{q, q_out, nullptr, 0, 0, (int)strides[2], (int)strides[3], (int)heads, 0};
-  p.side[Key] = Side{k, cache->k, cache->k_scale, cache->k_page_stride, cache->k_scale_page_stride, (int)strides[4], (int)strides[5], (int)cache->kv_heads, 0};
-  p.side[Value] = Side{v, cache->v, cache->v_scale, cache->v_page_stride, cache->v_scale_page_stride, (int)strides[6], (int)strides[7], (int)cache->kv_heads, 0};
+  p.side[Query] = Side{q, q_out, nullptr, 0, 0, (int)s[2], (int)s[3], (int)heads, 0};
+  p.side[Key] = Side{k, cache->k, cache->k_scale, cache->k_page_stride, cache->k_scale_page_stride, (int)s[4], (int)s[5], (int)cache->kv_heads, 0};
+  p.side[Value] = Side{v, cache->v, cache->v_scale, cache->v_page_stride, cache->v_scale_page_stride, (int)s[6], (int)s[7], (int)cache->kv_heads, 0};
   p.slots = slots; p.positions = positions; p.frequencies = frequencies;
   p.tokens = tokens;
   p.places = cache->pages * cache->page_size;
-  p.qo_t = (int)strides[0]; p.qo_h = (int)strides[1];
+  p.qo_t = (int)s[0]; p.qo_h = (int)s[1];
   while ((1ll << p.page_log2) < cache->page_size) ++p.page_log2;
   p.pairs = frequencies ? (int)(rotary / 2) : 0;
   // runs of pairs that lie in the eight elements of a lane; where those would not all be full, single ones
@@ -510,9 +513,9 @@ extern "C" int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cach
   p.wide_slots = slot_bits == 64; p.wide_positions = position_bits == 64; p.interleaved = interleaved != 0;
   p.scale = scale;
   p.vectors = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (!heads || ((uintptr_t)q % 16 == 0 && (uintptr_t)q_out % 16 == 0));
-  for (int i = heads ? 0 : 4; i < 8; ++i) p.vectors &= strides[i] % 8 == 0;
+  for (int i = heads ? 0 : 4; i < 8; ++i) p.vectors &= s[i] % 8 == 0;
   if (heads) {
-    p.rope.side[0] = RopeSide{q, q_out, 0, p.side[Query].t_stride, p.side[Query].h_stride, 0, p.qo_t, p.qo_h, (int)heads};
+    p.rope.side[0] = RopeSide{q, q_out, 0, 0, p.side[Query].t_stride, p.side[Query].h_stride, p.qo_t, p.qo_h, (int)heads};
     p.rope.positions = positions; p.rope.frequencies = frequencies;
     p.rope.table.pairs = p.pairs;
     p.rope.by_seq = Divisor((uint32_t)tokens);

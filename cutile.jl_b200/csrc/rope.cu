@@ -93,15 +93,17 @@ extern "C" int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, 
   const int64_t size = dtype == CTB_F32 ? 4 : 2, V = 16 / size;
   bool vectors = rotary % (2 * V) == 0 && D % V == 0;
   for (int i = 0; i < (k_heads ? 2 : 1); ++i) {
-    const int64_t* s = strides + 6 * i;
-    for (int j = 0; j < 6; ++j)
-      if (s[j] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_rope: strides too large");
-    p.side[i] = RopeSide{i ? k : q, i ? k_out : q_out, (int)s[3], (int)s[4], (int)s[5], (int)s[0], (int)s[1], (int)s[2], (int)(i ? k_heads : q_heads)};
     const int64_t extents[3] = {batch, seq, i ? k_heads : q_heads};
+    int64_t s[6];
+    for (int j = 0; j < 6; ++j) {
+      s[j] = extents[j % 3] == 1 ? 0 : strides[6 * i + j];
+      if (j % 3 && s[j] > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_rope: strides too large");
+    }
+    p.side[i] = RopeSide{i ? k : q, i ? k_out : q_out, s[3], s[0], (int)s[4], (int)s[5], (int)s[1], (int)s[2], (int)extents[2]};
     const int r = check_turned_in_place("ctb_rope", p.side[i].src, s + 3, p.side[i].dst, s, extents, D, size);
     if (r) return r;
     vectors &= (uintptr_t)p.side[i].src % 16 == 0 && (uintptr_t)p.side[i].dst % 16 == 0;
-    for (int j = 0; j < 6; ++j) vectors &= extents[j % 3] == 1 || s[j] % V == 0;
+    for (int j = 0; j < 6; ++j) vectors &= s[j] % V == 0;
   }
   p.positions = positions;
   p.frequencies = frequencies;

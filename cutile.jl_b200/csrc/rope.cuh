@@ -11,7 +11,8 @@ constexpr int kRopeThreads = 256;
 struct RopeSide {
   const void* src;
   void* dst;
-  int src_b, src_s, src_h, dst_b, dst_s, dst_h, heads;
+  int64_t src_b, dst_b;
+  int src_s, src_h, dst_s, dst_h, heads;
 };
 struct RopeParams {
   RopeSide side[2];
@@ -47,8 +48,8 @@ __device__ __forceinline__ void rope_cta(const RopeParams& p, int cta, float* an
     const RopeSide& s = p.side[second];
     const int head = second ? h - p.q_heads : h;
     const int token = t0 + t, b = p.by_seq(token), place = token - b * (int)p.by_seq.d;
-    const T* src = static_cast<const T*>(s.src) + ((int64_t)b * s.src_b + (int64_t)place * s.src_s + (int64_t)head * s.src_h);
-    to[k] = static_cast<T*>(s.dst) + ((int64_t)b * s.dst_b + (int64_t)place * s.dst_s + (int64_t)head * s.dst_h);
+    const T* src = static_cast<const T*>(s.src) + (b * s.src_b + (int64_t)place * s.src_s + (int64_t)head * s.src_h);
+    to[k] = static_cast<T*>(s.dst) + (b * s.dst_b + (int64_t)place * s.dst_s + (int64_t)head * s.dst_h);
     const bool turned = (int)u < p.turned;
     at[k] = turned ? (int)t * 2 * p.table.pairs : -1;
     run[k] = u;

@@ -248,6 +248,65 @@ def test_pages_of_one_allocation(cuda):
     assert V[0].equal(want)
 
 
+def test_one_token_of_any_stride(cuda):
+    import torch
+    from test_rope_gpu import close
+    x = torch.randn(1, 3, 64, device="cuda").half()
+    far = x.as_strided((1, 3, 64), (2 ** 40, 64, 1))
+    cache = cuda.kvcache.kv_cache(1, 3, 16, 64, torch.float16)
+    f, one = cuda.rope.rope_frequencies(64).cuda(), torch.ones(1, device="cuda", dtype=torch.int32)
+    out = cuda.kvcache.kv_write(cache, one, far, far, q=far, positions=one, frequencies=f)
+    close(out, x, one, f.cpu())
+    close(cache.k[0, :, 0][None], x, one, f.cpu())
+    assert cache.v[0, :, 0].equal(x[0])
+
+
+@pytest.mark.parametrize("store", STORES)
+def test_streams_and_graphs(cuda, store):
+    """Writes and reads of caches of their own on several streams, captured ones among them: each gives what it gives alone."""
+    import torch
+    f = cuda.rope.rope_frequencies(128).cuda()
+    cases = []
+    for T in (5, 900, 2100):
+        q, k, v = (torch.randn(T, h, 128, device="cuda").bfloat16() for h in (8, 2, 2))
+        pages = -(-T // 32)
+        cache = cuda.kvcache.kv_cache(pages, 2, 32, 128, getattr(torch, store if store != "float16" else "bfloat16"))
+        args = dict(slots=torch.arange(1, T + 1, device="cuda"), k=k, v=v, q=q, positions=torch.arange(T, device="cuda"), frequencies=f, out_q=torch.empty_like(q))
+        cases.append((cache, args, torch.arange(1, pages + 1, device="cuda", dtype=torch.int32)[None], torch.tensor([T], device="cuda", dtype=torch.int32), T))
+
+    def run(cache, args, table, length, T):
+        out = cuda.kvcache.kv_write(cache, **args)
+        return (out, *cuda.kvcache.kv_read(cache, table, length, T, dtype=torch.bfloat16))
+
+    want = [[t.clone() for t in run(*c)] for c in cases]
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(*c))
+        graphs.append(g)
+    for cache, args, *_ in cases:
+        for t in (*cache, args["out_q"]):
+            if t is not None:
+                t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+                got.append((i, run(*cases[i])))
+    torch.cuda.synchronize()
+    for i, parts in got + list(enumerate(outs)):
+        assert all(a.equal(b) for a, b in zip(parts, want[i]))
+    cases[0][1]["k"].normal_()  # a graph goes by what its inputs hold at its replay
+    cases[0][1]["positions"].add_(100)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(a.equal(b) for a, b in zip([t.clone() for t in outs[0]], run(*cases[0])))
+
+
 def test_refusals(cuda):
     import torch
     kc = cuda.kvcache

@@ -166,6 +166,24 @@ def test_captured(cuda):
     close(ok, k, positions, f.cpu())
 
 
+def test_large_strides(cuda):
+    """Sequences more than 2^31 elements apart, and strides along dimensions of one element, which mean nothing."""
+    import torch
+    apart = 2 ** 31 + 64
+    f, positions = cuda.rope.rope_frequencies(64).cuda(), torch.tensor([[3, 4], [70, 5]], device="cuda")
+    store = torch.empty(apart + 2 * 3 * 64, device="cuda", dtype=torch.float16)
+    q = store.as_strided((2, 2, 3, 64), (apart, 3 * 64, 64, 1))
+    q.copy_(make(4, 3, 64, "float16", 3).view(2, 2, 3, 64))
+    before = q.clone()
+    close(cuda.rope.rope_fwd(q, None, positions, f)[0], before, positions, f.cpu())
+    cuda.rope.rope_fwd(q, None, positions, f, out_q=q)
+    close(q, before, positions, f.cpu())
+    one = before[:1, :1].as_strided((1, 1, 3, 64), (2 ** 40, 2 ** 40, 64, 1))
+    close(cuda.rope.rope_fwd(one, None, positions[:1, :1], f)[0], before[:1, :1], positions[:1, :1], f.cpu())
+    with pytest.raises(cuda.CtbError, match="strides too large"):
+        cuda.rope.rope_fwd(store.as_strided((1, 2, 3, 64), (apart, apart, 64, 1)), None, positions[:1], f)
+
+
 def test_refusals(cuda):
     import torch
     q, k = make(4, 2, 64, "float16"), make(4, 1, 64, "float16")
