@@ -272,6 +272,82 @@ function distill_fwd_bwd(logits::CuArray{X,2}, teacher_ids::CuArray, teacher_val
     return loss, d
 end
 
+# ---- rotary positions and a paged key-value cache (no example in the reference) -------
+"Pairs of the heads (D, heads, seq, batch) of q and k (or nothing) turned by positions (seq, batch) times `frequencies` (Float64); `inverse` for gradients."
+function rope(q::CuArray{X,4}, k, positions::CuArray, frequencies::CuArray{Float64,1}; interleaved::Bool=false, scale::Real=1,
+              inverse::Bool=false) where {X}
+    D, heads, seq, batch = size(q)
+    oq = similar(q); ok = k === nothing ? nothing : similar(k)
+    three(a) = a === nothing ? Int64[0, 0, 0] : Int64[stride(a, 4), stride(a, 3), stride(a, 2)]
+    strides = vcat(three(oq), three(q), three(ok), three(k))
+    check(ccall((:ctb_rope, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Int64, Int64, Int64, Int64,
+         Int64, Int64, Ptr{Int64}, Cint, Cint, Cfloat, Cint),
+        context(), stream(), dptr(oq), dptr(q), or_null(ok), or_null(k), dptr(positions), ids_bits(positions), dptr(frequencies), batch, seq,
+        heads, k === nothing ? 0 : size(k, 2), D, 2 * length(frequencies), strides, interleaved, inverse, scale, dtype(X)))
+    return oq, ok
+end
+
+"Keys and values (D, page, heads, pages) in Float16, BFloat16, Int8 or (as UInt8) e4m3 codes; the latter two with scales (page, heads, pages)."
+struct KvCache{T}
+    k::CuArray{T,4}
+    v::CuArray{T,4}
+    k_scale::Union{CuArray{Float32,3},Nothing}
+    v_scale::Union{CuArray{Float32,3},Nothing}
+end
+struct KvCacheArrays # ctb_kv_cache
+    k::Ptr{Cvoid}; v::Ptr{Cvoid}; k_scale::Ptr{Cvoid}; v_scale::Ptr{Cvoid}
+    pages::Int64; kv_heads::Int64; page_size::Int64; head_dim::Int64
+    k_page_stride::Int64; v_page_stride::Int64; k_scale_page_stride::Int64; v_scale_page_stride::Int64
+    dtype::Cint
+end
+cache_dtype(::Type{T}) where {T} = T === UInt8 ? Cint(3) : T === Int8 ? Cint(4) : dtype(T)
+function arrays(c::KvCache{T}) where {T}
+    D, page, heads, pages = size(c.k)
+    s(a) = a === nothing ? 0 : stride(a, 3)
+    p(a) = a === nothing ? C_NULL : dptr(a)
+    return KvCacheArrays(dptr(c.k), dptr(c.v), p(c.k_scale), p(c.v_scale), pages, heads, page, D, stride(c.k, 4), stride(c.v, 4),
+                         s(c.k_scale), s(c.v_scale), cache_dtype(T))
+end
+
+"k and v (D, heads, tokens) to `slots` (1-based, 0: none); with positions and frequencies k is turned before, and so is q, which is returned."
+function kv_write(cache::KvCache, slots::CuArray, k::CuArray{X,3}, v::CuArray{X,3}; q=nothing, positions=nothing, frequencies=nothing,
+                  interleaved::Bool=false, scale::Real=1) where {X}
+    oq = q === nothing ? nothing : similar(q)
+    two(a) = a === nothing ? Int64[0, 0] : Int64[stride(a, 3), stride(a, 2)]
+    strides = vcat(two(oq), two(q), two(k), two(v))
+    check(ccall((:ctb_kv_write, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ref{KvCacheArrays}, Ptr{Cvoid}, Cint, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Int64},
+         Ptr{Cvoid}, Cint, Ptr{Cvoid}, Int64, Int64, Int64, Cint, Cfloat, Cint),
+        context(), stream(), arrays(cache), dptr(slots), ids_bits(slots), or_null(oq), or_null(q), dptr(k), dptr(v), strides,
+        or_null(positions), positions === nothing ? 32 : ids_bits(positions), or_null(frequencies), size(k, 3),
+        q === nothing ? 0 : size(q, 2), frequencies === nothing ? 0 : 2 * length(frequencies), interleaved, scale, dtype(X)))
+    return oq
+end
+
+"The first tokens of every sequence (table (width, batch), lengths (batch), Int32) as dense (D, seq, heads, batch) K and V: what `cutile_fmha` takes."
+function kv_read(cache::KvCache, page_table::CuArray{Int32,2}, lengths::CuArray{Int32,1}, seq::Int, X::Type)
+    D, _, heads, _ = size(cache.k); width, batch = size(page_table)
+    K = CuArray{X}(undef, D, seq, heads, batch); V = similar(K)
+    check(ccall((:ctb_kv_read, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ref{KvCacheArrays}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Cint),
+        context(), stream(), dptr(K), dptr(V), arrays(cache), dptr(page_table), dptr(lengths), batch, seq, width, stride(page_table, 2), dtype(X)))
+    return K, V
+end
+
+"Attention of a token per sequence, Q (D, heads, batch), over the cache: (Out, lse)."
+function fmha_paged(Q::CuArray{X,3}, cache::KvCache, page_table::CuArray{Int32,2}, lengths::CuArray{Int32,1};
+                    qk_scale::Real=1 / sqrt(size(Q, 1))) where {X}
+    D, heads, batch = size(Q)
+    Out = similar(Q); lse = CuArray{Float32}(undef, heads, batch)
+    check(ccall((:ctb_fmha_paged, LIB), Cint,
+        (Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ref{KvCacheArrays}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64,
+         Int64, Int64, Cfloat, Cint),
+        context(), stream(), dptr(Out), dptr(lse), dptr(Q), arrays(cache), dptr(page_table), dptr(lengths), batch, heads, stride(Q, 3),
+        stride(Q, 2), size(page_table, 1), stride(page_table, 2), qk_scale, dtype(X)))
+    return Out, lse
+end
+
 function moe_align_tile_size(topk_ids::CuArray, tile_m::Int, num_experts::Int)
     T, topk = size(topk_ids)
     cap = ccall((:ctb_moe_max_blocks, LIB), Int64, (Int64, Int64, Int64, Cint), T, topk, num_experts, tile_m)
