@@ -100,7 +100,7 @@ def build_host(force=False, verbose=False):
            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(env["dir"], "include"),
            "-I", os.path.join(env["dir"], "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
            src, "-o", HOST, "-L", OUT_DIR, "-l:libcutile_b200.so", "-L", os.path.join(env["dir"], "lib"),
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode:
         sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)

@@ -11,6 +11,7 @@
 // checks, which either raise the precise error or make the call themselves.  A status other than CTB_OK raises CtbError
 // (through the Python function installed by setup()).
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -327,10 +328,20 @@ int index_bits(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : t.sc
 bool frequencies_of(const Tensor* f, const Tensor& like) {
   return f && f->scalar_type() == at::kDouble && f->dim() == 1 && f->is_contiguous() && f->device() == like.device();
 }
-// A result where one is given, else a new array with the strides of its input.
+// A new array, without the dispatcher: at::empty takes 0.6 us more.
+Tensor new_array(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+// at::empty_like's layout: the order of the dimensions in memory stays.
+Tensor new_like(const Tensor& x) {
+  for (int64_t i = 1; i < x.dim(); ++i)
+    if (x.stride(i - 1) < x.stride(i)) return at::empty_like(x);
+  return new_array(x.sizes(), x.scalar_type(), x);
+}
+// A result where one is given, else a new array with the layout of its input.
 const Tensor* result_like(PyObject* given, const Tensor& x, Tensor* made) {
   if (given == Py_None) {
-    *made = at::empty_like(x);
+    *made = new_like(x);
     return made;
   }
   const Tensor* out = cuda_tensor(given);
@@ -477,8 +488,7 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (type != at::kHalf && type != at::kBFloat16) return decline();
   Call c(*table);
   if (!c.ok()) return nullptr;
-  const auto options = table->options().dtype(type);
-  Tensor K = at::empty({table->size(0), cache.kv_heads, seq, cache.head_dim}, options), V = at::empty_like(K);
+  Tensor K = new_array({table->size(0), cache.kv_heads, seq, cache.head_dim}, type, *table), V = new_array(K.sizes(), type, *table);
   const int r = without_gil([&] {
     return ctb_kv_read(c.ctx, c.stream, K.data_ptr(), V.data_ptr(), &cache, static_cast<const int32_t*>(table->data_ptr()),
                        static_cast<const int32_t*>(lengths->data_ptr()), table->size(0), seq, table->size(1), ld,
@@ -503,9 +513,9 @@ PyObject* fmha_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Call c(*q);
   if (!c.ok()) return nullptr;
   const int64_t B = q->size(0), H = q->size(1);
-  Tensor out = at::empty({B, H, cache.head_dim}, q->options()), lse;
+  Tensor out = new_array({B, H, cache.head_dim}, q->scalar_type(), *q), lse;
   const bool with_lse = a[5] == Py_True;
-  if (with_lse) lse = at::empty({B, H}, q->options().dtype(at::kFloat));
+  if (with_lse) lse = new_array({B, H}, at::kFloat, *q);
   const int r = without_gil([&] {
     return ctb_fmha_paged(c.ctx, c.stream, out.data_ptr(), with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, q->data_ptr(), &cache,
                           static_cast<const int32_t*>(table->data_ptr()), static_cast<const int32_t*>(lengths->data_ptr()), B, H, s[0], s[1],
