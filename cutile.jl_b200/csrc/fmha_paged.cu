@@ -3,13 +3,14 @@
 //
 // What bounds it is HBM: every stored key and value is read once, 2 D bytes times the element's size, against 4 D operations per row.
 // 64 sequences of up to 8000 tokens, 64 heads over 8 of 128 in bf16 (1018 MB): 161 us, 6.3 TB/s, 0.97 of the copy rate; one sequence of
-// 131072 in f16 89 us (0.92); 128 of up to 4096 in e4m3 (560 MB) 102 us (0.84); 4 of up to 500 9 us, which are latencies: lengths (0.9 us),
-// ranges (0.5), page numbers (1.1), the first keys (0.6), tiles, meeting (1) and joining (1).
+// 131072 in f16 89 us (0.92); 128 of up to 4096 in e4m3 (560 MB) 100 us (0.85); 4 of up to 500 8.6 us, which are latencies: lengths (0.9 us),
+// ranges (0.3), page numbers (1.1), the first keys (0.6), tiles, meeting (1) and joining (1).
+// In 8 bits the 670 (e4m3) or 870 (int8) instructions of a tile of 32 keys come next to HBM: with pages out of L2 the same keys take 76 or 86 us.
 //
 // Work is cut into tiles of 16 to 64 keys of one item (a sequence, a key/value head, a row of up to 16 heads of its group); 4 KB of keys and
 // 4 KB of values each.  The tiles of all items form one line that the warps of the grid share out in equal contiguous ranges, whatever the
 // lengths are: every CTA finds the tiles before every sequence by a scan over the lengths, which only the device knows.  An item counts a
-// tile more than it has, for its queries and results (attend 64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
+// tile more than it has, for its queries and results (64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
 // longest item has at most kWholeItems tiles, ranges of CTAs end where items end, so that no CTA has to wait for another's part (16
 // x 1000 keys 15.9 us with parts, 12.8 with whole items; 8 x 4000 in e4m3, 125 tiles, 20.1 and 25.6 us).  A warp leaves an item that it has
 // as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
@@ -19,7 +20,7 @@
 // A warp streams its range for itself: it asks for keys and values in turn, an entry of 4 KB of its ring in shared memory each, three
 // entries ahead of the one that it reads (144 KB on the way per SM), by asynchronous copies of 16 bytes per lane.  Rows are exchanged in chunks
 // as they are copied, so that no read meets a bank conflict.  Ways that were slower: keys and values straight into registers, 12 warps
-// (attend_batch 169 us, 8-bit caches 151 for 102); bulk and tensor copies by a lane of every warp (177, 154) or by a warp for all
+// (the first of these 169 us, 8-bit caches 151 for 100); bulk and tensor copies by a lane of every warp (177, 154) or by a warp for all
 // (181, 206): a copy costs its warp about 100 clocks, and pages of 16 tokens make many small ones; 8 or 10 warps with longer rings, 16 with
 // shorter ones (8-bit caches 115, 112, 120).
 //
@@ -85,7 +86,7 @@ struct Shape {
   static constexpr int kPartFloats = R * D + 2 * R;
   static constexpr int kScales = kBytes ? 16 * KT : 0;  // of an entry
   static constexpr size_t kSmem =
-      128 + (size_t)kWarps * (kRing * (kEntry + kScales * 4) + kSlotFloats * 4) + (2 * kMaxBatch + 1) * 4;
+      128 + (size_t)kWarps * (kRing * (kEntry + kScales * 4) + kSlotFloats * 4) + 2 * kMaxBatch * 4;
 };
 
 template <int OFFSET>
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   float* firsts = all_scales + kWarps * kRing * S::kScales;
   int* lens = reinterpret_cast<int*>(firsts + kWarps * S::kSlotFloats);
   unsigned* prefix = reinterpret_cast<unsigned*>(lens + kMaxBatch);
-  __shared__ unsigned warp_sum[kWarps], warp_most[kWarps];
+  __shared__ unsigned warp_sum[kWarps], warp_most[kWarps], ends[2];
   __shared__ uint4 segs[2 * kWarps];  // parts of items: first output row of the item (-1: no part), its live rows, its first tile, its last one's end
   __shared__ int last_s[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   // ---- tiles before every sequence
   const int most = p.width << p.page_log2;
   const unsigned per_tile = (unsigned)p.kv_heads * p.row_tiles;
-  unsigned longest;
+  unsigned longest, total = 0;
   {
     const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
     auto tiles = [&](int n) { return n ? (unsigned)(n + kTileKeys - 1) / kTileKeys + kItemCost : 0; };
@@ -261,17 +262,33 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     longest = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
+      total += warp_sum[w];
       before += w < warp ? warp_sum[w] : 0;
       longest = max(longest, warp_most[w]);
     }
-    for (int b = b0; b < b1; ++b) {
-      prefix[b] = before;
-      before += tiles(lens[b]) * per_tile;
+    auto place = [&](auto&& at_sequence) {  // at_sequence(an item's tiles, the first one of all items, their end)
+      for (int b = b0; b < b1; ++b) {
+        const unsigned n = tiles(lens[b]), behind = before + n * per_tile;
+        prefix[b] = before;
+        at_sequence(n, before, behind);
+        before = behind;
+      }
+    };
+    if (longest <= kWholeItems) {
+      // Whole items: a CTA's range ends where an item does that is next to the end of an equal range.  Whoever has that sequence says where.
+      const Shares equal(total, gridDim.x);
+      const unsigned at[2] = {equal.first(blockIdx.x), equal.first(blockIdx.x + 1)};
+      if (tid < 2 && at[tid] >= total) ends[tid] = total;
+      place([&](unsigned n, unsigned first, unsigned behind) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (first <= at[i] && at[i] < behind) ends[i] = first + (at[i] - first + n / 2) / n * n;
+      });
+    } else {
+      place([](unsigned, unsigned, unsigned) {});
     }
-    if (tid == kThreads - 1) prefix[p.batch] = before;
     __syncthreads();
   }
-  const unsigned total = prefix[p.batch];
   // sequences without keys
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (lens[b] > 0) continue;
@@ -292,26 +309,16 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   };
   // Ranges of the line of tiles: equal ones for all warps of the grid, or, where items are short, for the warps of a CTA, whose range
   // ends where an item ends.
-  const bool whole_items = longest <= kWholeItems;
-  const Shares shares(total, whole_items ? gridDim.x : min(gridDim.x * kWarps, total));
-  unsigned cta_lo, cta_hi, lo, hi;
-  if (whole_items) {
-    auto end_of = [&](unsigned i) {  // the end of an item that is next to the end of an equal range
-      const unsigned x = shares.first(i);
-      if (x >= total) return total;
-      const int b = sequence_of(x);
-      const unsigned n = (unsigned)(lens[b] + kTileKeys - 1) / kTileKeys + kItemCost;
-      return prefix[b] + (x - prefix[b] + n / 2) / n * n;
-    };
-    cta_lo = end_of(blockIdx.x);
-    cta_hi = end_of(blockIdx.x + 1);
-    const unsigned n = cta_hi - cta_lo;
-    lo = cta_lo + warp * n / kWarps;
-    hi = cta_lo + (warp + 1) * n / kWarps;
+  auto warp_shares = [&] { return Shares(total, min(gridDim.x * kWarps, total)); };
+  unsigned lo, hi;
+  if (longest <= kWholeItems) {
+    const unsigned n = ends[1] - ends[0];
+    lo = ends[0] + warp * n / kWarps;
+    hi = ends[0] + (warp + 1) * n / kWarps;
   } else {
+    const Shares shares = warp_shares();
     auto range_of = [&](unsigned w) { return min(shares.first(w), total); };
-    cta_lo = range_of(blockIdx.x * kWarps);
-    cta_hi = range_of((blockIdx.x + 1) * kWarps);
+    if (tid < 2) ends[tid] = range_of((blockIdx.x + tid) * kWarps);
     lo = range_of(blockIdx.x * kWarps + warp);
     hi = range_of(blockIdx.x * kWarps + warp + 1);
   }
@@ -852,6 +859,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
       if (lane == 0) write_lse(out_row + row, M, L);
     }
   };
+  const unsigned cta_lo = ends[0], cta_hi = ends[1];
   const uint4 seg = lane < 2 * kWarps ? segs[lane] : make_uint4(~0u, 0, 0, 0);
   const uint32_t marked = __ballot_sync(0xffffffffu, seg.x != ~0u), below = marked & ((1u << lane) - 1);
   const uint32_t item_below = __shfl_sync(0xffffffffu, seg.x, below ? 31 - __clz(below) : 0);
@@ -872,6 +880,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   }
   if (shared_first.x == ~0u && shared_last.x == ~0u) return;
   // ---- Items that several CTAs had: the one that is done last adds the parts.
+  const Shares shares = warp_shares();
   auto cta_of = [&](unsigned x) { return (int)(shares.owner(x) / kWarps); };
   __syncthreads();
   if (tid < 2) {
