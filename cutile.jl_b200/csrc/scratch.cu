@@ -21,7 +21,7 @@ namespace ctb_internal {
 
 namespace {
 
-constexpr int kSlots = 96;     // eager slots of a context (1.25 MB each); torch has 32 streams per priority and the default
+constexpr int kSlots = 96;     // eager slots of a context (2.5 MB each); torch has 32 streams per priority and the default
 constexpr int kMarkFrom = 72;
 
 struct GraphHold {  // shared by a slot and the graph that uses it
