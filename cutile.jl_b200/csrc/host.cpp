@@ -430,7 +430,8 @@ bool token_rows(const Tensor* t, const Tensor& like, int64_t T, int64_t D, int64
   return true;
 }
 
-// kv_write(cache, slots, k, v, q, positions, frequencies, interleaved, scale, out_q) -> (out_q or None,); q .. frequencies, out_q: or None
+// kv_write(cache, slots, k, v, q, positions, frequencies, interleaved, scale, out_q) -> (out_q or None,); q .. frequencies, out_q: or None.
+// Positions without frequencies turn nothing.
 PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 10) return decline();
   const Tensor *slots = cuda_tensor(a[1]), *k = cuda_tensor(a[2]), *v = cuda_tensor(a[3]);
@@ -445,7 +446,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = k->size(0), D = cache.head_dim;
   auto list = [&](const Tensor& t) { return t.dim() == 1 && t.size(0) == T && t.is_contiguous() && t.device() == k->device() && index_bits(t); };
   if (!list(*slots) || !token_rows(k, *k, T, D, s + 4) || !token_rows(v, *k, T, D, s + 6) || k->size(1) != cache.kv_heads ||
-      v->size(1) != cache.kv_heads || (pos != nullptr) != (f != nullptr) || (f && (!frequencies_of(f, *k) || !list(*pos))) ||
+      v->size(1) != cache.kv_heads || (f && !pos) || (f && !frequencies_of(f, *k)) || (pos && !list(*pos)) ||
       (q && (!f || !token_rows(q, *k, T, D, s + 2))) || (!q && a[9] != Py_None))
     return decline();
   Call c(*k);
@@ -455,7 +456,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (q && (!(out = result_like(a[9], *q, &made)) || !token_rows(out, *k, T, D, s))) return decline();
   const int r = without_gil([&] {
     return ctb_kv_write(c.ctx, c.stream, &cache, slots->data_ptr(), index_bits(*slots), q ? out->data_ptr() : nullptr, q ? q->data_ptr() : nullptr,
-                        k->data_ptr(), v->data_ptr(), s, pos ? pos->data_ptr() : nullptr, pos ? index_bits(*pos) : 32,
+                        k->data_ptr(), v->data_ptr(), s, f ? pos->data_ptr() : nullptr, f ? index_bits(*pos) : 32,
                         f ? static_cast<const double*>(f->data_ptr()) : nullptr, T, q ? q->size(1) : 0, f ? 2 * f->size(0) : 0, a[7] == Py_True,
                         scale, dtype_of(*k));
   });

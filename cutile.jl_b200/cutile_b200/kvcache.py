@@ -78,11 +78,19 @@ def _rows_of(t, heads, D, T, what, like):
     return t
 
 
-def kv_write(cache, slots, k, v, q=None, positions=None, frequencies=None, interleaved=False, scale=1.0, out_q=None, **hints):
+_LEFT_OUT = object()
+
+
+def kv_write(cache, slots, k, v, q=None, positions=None, frequencies=_LEFT_OUT, interleaved=False, scale=1.0, out_q=None, **hints):
     """Writes k and v [tokens, KV_Heads, D] (f16 or bf16, any strides but contiguous heads) to slots [tokens] (int32 or int64; 0 writes
     nothing, the others must differ).  With positions [tokens] and frequencies, keys are turned as by `rope.rope_fwd` before they are stored,
-    and so are the queries q [tokens, Heads, D], if given: returns them turned (in out_q, which may be q), else None."""
-    if not hints:
+    and so are the queries q [tokens, Heads, D], if given: returns them turned (in out_q, which may be q), else None.  Frequencies of None, said
+    in so many words, turn nothing, whatever the positions (a model without rotary positions); positions whose frequencies are left
+    out are refused."""
+    forgotten = frequencies is _LEFT_OUT and positions is not None
+    if frequencies is _LEFT_OUT:
+        frequencies = None
+    if not hints and not forgotten:
         r = _host.kv_write(cache, slots, k, v, q, positions, frequencies, interleaved, scale, out_q)
         if r is not None:
             return r[0]
@@ -92,15 +100,16 @@ def kv_write(cache, slots, k, v, q=None, positions=None, frequencies=None, inter
     _rows_of(k, KVH, D, T, "k", k)
     _rows_of(v, KVH, D, T, "v", k)
     bits = ids_bits(dense(slots, (T,), "slots", k), "slots")
-    if (positions is None) != (frequencies is None):
+    if forgotten or (positions is None and frequencies is not None):
         raise _lib.CtbError(_lib.BAD_ARG, "kv_write: positions and frequencies come together")
     if frequencies is None and q is not None:
         raise _lib.CtbError(_lib.BAD_ARG, "kv_write: queries come with positions and frequencies")
     if q is None and out_q is not None:
         raise _lib.CtbError(_lib.BAD_ARG, "kv_write: out_q comes with q")
     position_bits, rotary, strides, heads = 32, 0, [0] * 4, 0
-    if frequencies is not None:
+    if positions is not None:
         position_bits = ids_bits(dense(positions, (T,), "positions", k), "positions")
+    if frequencies is not None:
         if not isinstance(frequencies, torch.Tensor) or frequencies.dim() != 1:
             raise _lib.CtbError(_lib.BAD_ARG, "frequencies: expected a tensor of one dimension")
         rotary = 2 * dense(frequencies, frequencies.shape, "frequencies", k, torch.float64).shape[0]
@@ -111,7 +120,7 @@ def kv_write(cache, slots, k, v, q=None, positions=None, frequencies=None, inter
         strides = [out_q.stride(0), out_q.stride(1), q.stride(0), q.stride(1)]
     strides += [k.stride(0), k.stride(1), v.stride(0), v.stride(1)]
     _lib.check(_lib.lib.ctb_kv_write(ctx, stream, C.byref(s), ptr(slots), bits, ptr(out_q), ptr(q), ptr(k), ptr(v), (C.c_int64 * 8)(*strides),
-                                     ptr(positions), position_bits, ptr(frequencies), T, heads, rotary, int(bool(interleaved)),
+                                     ptr(None if frequencies is None else positions), position_bits, ptr(frequencies), T, heads, rotary, int(bool(interleaved)),
                                      float(scale), dtype_code(k)))
     return out_q
 

@@ -1,0 +1,27 @@
+"""Cache writes and rotary positions of large calls, whose kernels take several rows and units at a time, against f64 as in test_kvcache_gpu and
+test_rope_gpu; calls that their documentation allows and those tests do not make."""
+import pytest
+
+from test_kvcache_gpu import STORES, places
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("bits", ["int32", "int64"])
+def test_rows_that_are_not_turned(cuda, store, bits):
+    """Positions beside frequencies of None, as of a model without rotary positions: rows are stored as they are."""
+    import torch
+    k, v = (torch.randn(9, 2, 64, device="cuda").to(torch.bfloat16 if store != "float16" else torch.float16) for _ in range(2))
+    slots, positions = places(2, 16, 9), torch.arange(9, device="cuda").to(getattr(torch, bits))
+    caches = [cuda.kvcache.kv_cache(2, 2, 16, 64, getattr(torch, store)) for _ in range(3)]
+    for cache, more in zip(caches, ({}, dict(positions=positions, frequencies=None), dict(positions=positions, frequencies=None, occupancy=1))):
+        assert cuda.kvcache.kv_write(cache, slots, k, v, q=None, interleaved=True, **more) is None
+    for other in caches[1:]:
+        for x, y in zip(caches[0], other):
+            assert x is y is None or x.view(torch.uint8).equal(y.view(torch.uint8))
+    for bad, word in ((positions[:8], "positions"), (positions.float(), "int32 or int64"), (positions.cpu(), "positions")):
+        with pytest.raises(cuda.CtbError, match=word):
+            cuda.kvcache.kv_write(caches[0], slots, k, v, positions=bad, frequencies=None)
+    with pytest.raises(cuda.CtbError, match="positions and frequencies"):
+        cuda.kvcache.kv_write(caches[0], slots, k, v, q=k, positions=positions, frequencies=None)
