@@ -275,8 +275,8 @@ def _prepare_write(c, g):
 
 
 def _own_write(s):
-    turned = dict(q=s["q"], positions=s["positions"], frequencies=s["frequencies"]) if s["frequencies"] is not None else {}
-    return _package().kvcache.kv_write(_own_cache(s), s["slots"], s["k_new"], s["v_new"], interleaved=s["interleaved"], **turned)
+    return _package().kvcache.kv_write(_own_cache(s), s["slots"], s["k_new"], s["v_new"], q=s["q"] if s["frequencies"] is not None else None,
+                                       positions=s["positions"], frequencies=s["frequencies"], interleaved=s["interleaved"])
 
 
 def _own_cached(s):
