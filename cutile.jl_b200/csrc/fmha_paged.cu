@@ -205,8 +205,7 @@ struct Cursor {
   int b, head, rt, key, len;  // head: of the keys and values
 };
 
-// PAIR: probabilities go to the product as two 16-bit numbers.
-template <int STORE, int D, int NT, bool PAIR>
+template <int STORE, int D, int NT>
 __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
     fmha_paged_kernel(const Params p, int* status) {
   using S = Shape<STORE, D, NT>;
@@ -677,7 +676,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         unrolled<KT>([&](auto tag) {
           constexpr int s = decltype(tag)::value;
           uint32_t hi_[NT][2];
-          [[maybe_unused]] uint32_t lo_[NT][2];
+          uint32_t lo_[NT][2];  // what is left of a probability: one 16-bit number each would show in results whose terms cancel
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -685,10 +684,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
               const float a = S::kBytes ? sc[s][n][2 * h] : d[s][n][2 * h], z = S::kBytes ? sc[s][n][2 * h + 1] : d[s][n][2 * h + 1];
               const uint32_t w = pack2<BF>(a, z);
               hi_[n][h] = transposed(w);
-              if constexpr (PAIR) {
-                const float2 f = unpack2<BF>(w);
-                lo_[n][h] = transposed(pack2<BF>(a - f.x, z - f.y));
-              }
+              const float2 f = unpack2<BF>(w);
+              lo_[n][h] = transposed(pack2<BF>(a - f.x, z - f.y));
             }
           // rows behind the last key may hold anything: 0 x NaN is NaN
           const int left = len - now.key - 16 * s;
@@ -725,7 +722,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], hi_[n][0], hi_[n][1]);
-                  if constexpr (PAIR) mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], lo_[n][0], lo_[n][1]);
+                  mma<false>(o[2 * i + h][n], a[h][0], a[h][1], a[h][2], a[h][3], lo_[n][0], lo_[n][1]);
                 }
             }
           } else {
@@ -945,8 +942,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   }
 }
 
-template <int STORE, int D, int NT, bool PAIR>
-int launch_as(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
+template <int STORE, int D, int NT>
+int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   using S = Shape<STORE, D, NT>;
   static_assert(S::kSmem <= 227 * 1024, "shared memory of a CTA");
   p.row_tiles = (p.group + S::R - 1) / S::R;
@@ -956,7 +953,7 @@ int launch_as(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   const int64_t chunk = std::min<int64_t>(kMaxBatch, INT32_MAX / tiles);
   if ((size_t)ctx->sm_count * 2 * S::kPartFloats * sizeof(float) > kSlotBytes || ctx->sm_count > kTickets)
     return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: more SMs than the split over keys has scratch for");
-  auto kern = fmha_paged_kernel<STORE, D, NT, PAIR>;
+  auto kern = fmha_paged_kernel<STORE, D, NT>;
   cudaError_t e = allow_smem(kern, S::kSmem);
   if (e != cudaSuccess) return cuda_fail(e, "ctb_fmha_paged: shared memory opt-in");
   const StreamScratch scratch(ctx, st);
@@ -975,16 +972,6 @@ int launch_as(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
     CTB_CHECK_LAUNCH("ctb_fmha_paged launch");
   }
   return CTB_OK;
-}
-
-// One f16 (2^-11 of a probability) is enough for results in bf16 from 8-bit values; results in f16 would be half as far off again as
-// their own rounding makes them (3.0e-4 for 2.0e-4).
-template <int STORE, int D, int NT>
-int launch(ctb_ctx* ctx, cudaStream_t st, const Params& p, int64_t batch) {
-  if constexpr (STORE >= E4M3) {
-    if (p.q_bf16) return launch_as<STORE, D, NT, false>(ctx, st, p, batch);
-  }
-  return launch_as<STORE, D, NT, true>(ctx, st, p, batch);
 }
 
 template <int STORE>

@@ -1,0 +1,90 @@
+"""Attention over a paged cache where one tile's contents or layout say little about the next one's.  Bounds as in test_fmha_paged_gpu,
+with probabilities as two 16-bit numbers for every type (2^-17)."""
+import math
+
+import pytest
+
+from test_fmha_paged_gpu import Case, same
+
+pytestmark = pytest.mark.gpu
+
+EIGHT = ("float8_e4m3fn", "int8")
+SIXTEEN = ("float16", "bfloat16")
+
+
+def case(*args, **kw):
+    """A Case without the NaN that its e4m3 codes of numbers beyond 4.64 are: in long sequences every row would have one."""
+    import torch
+    c = Case(*args, **kw)
+    if c.store == torch.float8_e4m3fn:
+        for i, (x, s) in enumerate(((c.cache.k, c.cache.k_scale), (c.cache.v, c.cache.v_scale))):
+            x.copy_(x.float().nan_to_num(448.0).to(c.store))
+            c.values[i] = x.float().double() * s.double()[..., None]
+    return c
+
+
+def bound_of(c, b, k, v, keys=None):
+    """(o, what it may be off by, lse, what that may be off by) of sequence b over its keys k and values v (f64), of which `keys` (a mask) are meant."""
+    import torch
+    D, info = c.q.shape[2], torch.finfo(c.dtype)
+    q = c.q[b].double().view(k.shape[0], -1, D)
+    if keys is not None:
+        k, v = k[:, keys], v[:, keys]
+    s = torch.einsum("hgd,hnd->hgn", q, k) / math.sqrt(D)
+    S = (torch.einsum("hgd,hnd->hgn", q.abs(), k.abs()).amax(-1) / math.sqrt(D))[..., None]
+    p = torch.softmax(s, -1)
+    o, W = torch.einsum("hgn,hnd->hgd", p, v), torch.einsum("hgn,hnd->hgd", p, v.abs())
+    F = torch.zeros_like(o)
+    if c.cache.v_scale is not None:
+        n = int(c.lengths[b])
+        at = c.table[b, :-(-n // c.page)].long() - 1
+        codes = c.cache.v[at].float().double().transpose(0, 1).flatten(1, 2)[:, :n].abs()
+        each = c.cache.v_scale[at].double().transpose(0, 1).flatten(1, 2)[:, :n].abs()
+        if keys is not None:
+            codes, each = codes[:, keys], each[:, keys]
+        F = 2.0 ** -33 * (p * each[:, None]).amax(-1)[..., None] * codes.sum(1)[:, None]
+    elif c.store == torch.float16:
+        F = 2.0 ** -33 * p.amax(-1)[..., None] * v.abs().sum(1)[:, None]
+    off = info.eps / 2 * o.abs() + W * (2 * (S * 2.0 ** -18 + 2.0 ** -22) + 2.0 ** -17 + 2.0 ** -17) + F + info.smallest_normal * info.eps / 2
+    lse = torch.logsumexp(s, -1)
+    return o, off, lse, S[..., 0] * 2.0 ** -18 + 2.0 ** -20 * (1 + lse.abs())
+
+
+def check(c, got, keys=None, sequences=None):
+    for b in range(c.q.shape[0]) if sequences is None else sequences:
+        o, off, lse, lse_off = bound_of(c, b, *c.sequence(b), None if keys is None else keys[b])
+        err = (got[0][b].double().view(o.shape) - o).abs()
+        assert (err <= off).all(), (b, float((err / off).max()))
+        err = (got[1][b].double().view(lse.shape) - lse).abs()
+        assert (err <= lse_off).all(), (b, float((err / lse_off).max()))
+
+
+def slots_of(c, b, keys):
+    """(pages, places) of keys of sequence b."""
+    return c.table[b].long()[keys // c.page] - 1, keys % c.page
+
+
+def runs(c, b, first, length, every):
+    """Keys of sequence b in runs: `length` of every `every` keys, from `first` on."""
+    import torch
+    n = torch.arange(int(c.lengths[b]), device="cuda")
+    return n[((n - first) % every < length) & (n >= first)]
+
+
+@pytest.mark.parametrize("store", EIGHT)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("heads", [4, 16])
+def test_values_that_cancel(cuda, store, D, heads):
+    """Neighbouring keys alike, their values opposite, from other codes and scales: what is left is small beside the terms, so that bf16 results
+    show how probabilities were rounded."""
+    import torch
+    c = case(cuda, [2, 64, 500], heads, 1, D, 16, store, "bfloat16", seed=31, q_size=0.01)  # scores add little to the bound
+    k, v, ks, vs = c.cache
+    first, second = slice(0, None, 2), slice(1, None, 2)
+    k[:, :, second], ks[:, :, second] = k[:, :, first], ks[:, :, first]
+    sign = torch.where(torch.rand(v[:, :, first].shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.5, -1.0, 1.0)
+    v[:, :, first], v[:, :, second] = (44 * sign).to(v.dtype), (-32 * sign).to(v.dtype)
+    vs[:, :, second] = vs[:, :, first] * (44 / 32)
+    for i, (x, s) in enumerate(((k, ks), (v, vs))):
+        c.values[i] = x.float().double() * s.double()[..., None]
+    check(c, c.run())
