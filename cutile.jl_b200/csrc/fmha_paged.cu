@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         for (int r = 0; r < 2; ++r) {
           m[n][r] = -INFINITY;
           ref[n][r] = l[n][r] = peak[n][r] = 0.f;
-          unit[n][r] = 1.f;
+          unit[n][r] = S::kBytes ? 8.507059e37f : 1.f;  // 2^126
         }
 #pragma unroll
       for (int j = 0; j < MT; ++j)
@@ -623,7 +623,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
             }
         if constexpr (S::kBytes) {
           // A probability times its value's scale goes to f16 in units of (about) the largest so far: scales differ from key to key by
-          // any factor.
+          // any factor.  While there was none above 0 (rows of zeros have scales of 0) the unit is 2^126, the largest there is, which the first
+          // that is more than 2^-111 exceeds.
           float vs[KT][2];
 #pragma unroll
           for (int s = 0; s < KT; ++s)
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
                 top = max_over_keys(top);
                 peak[n][r] = top;
                 const int e = (int)(__float_as_uint(top) >> 23);
-                const float u = top > 0.f && e < 255 ? __uint_as_float((uint32_t)min(max(254 + kLift - e, 1), 253) << 23) : unit[n][r];
+                const float u = e < 255 ? __uint_as_float((uint32_t)min(max(254 + kLift - e, 1), 253) << 23) : unit[n][r];
                 const float f = u / unit[n][r];
                 unit[n][r] = u;
 #pragma unroll

@@ -73,6 +73,24 @@ def runs(c, b, first, length, every):
 
 @pytest.mark.parametrize("store", EIGHT)
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("lead", [32, 64, 100])
+def test_runs_of_zero_values(cuda, store, D, dtype, lead):
+    """Values whose scales are zero, as an untouched cache has them and rows below 2^-100 are stored, before small ones: in the first tiles of a
+    sequence (whole items), and in stretches (items in parts)."""
+    for lengths, heads, kv_heads, every in (([400, lead + 1, lead + 90], 8, 1, 10 ** 6), ([300, 220], 6, 2, 10 ** 6), ([9000] * 8, 16, 8, 2 * lead)):
+        for size in (1.0, 1e-3, 1e-6, 1e-9):
+            c = case(cuda, lengths, heads, kv_heads, D, 16, store, dtype, seed=lead)
+            c.cache.v_scale.mul_(size)
+            for b in range(len(lengths)):
+                pages, places = slots_of(c, b, runs(c, b, 0, lead, every))
+                c.cache.v_scale[pages, :, places] = 0
+            c.values[1] = c.cache.v.float().double() * c.cache.v_scale.double()[..., None]
+            check(c, c.run(), sequences=range(min(len(lengths), 3)))
+
+
+@pytest.mark.parametrize("store", EIGHT)
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("heads", [4, 16])
 def test_values_that_cancel(cuda, store, D, heads):
     """Neighbouring keys alike, their values opposite, from other codes and scales: what is left is small beside the terms, so that bf16 results
