@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   constexpr int kTileKeys = 16 * KT, kRow = S::kRow, kRing = S::kRing;
   constexpr bool BF = STORE == BF16;
   constexpr float kAbove = STORE == F16 ? kLift : 0;  // what the known largest score stands above m
+  constexpr float kNone = -3.4028235e38f;  // the reference of a row whose keys so far score -inf: whatever comes stands far above it
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   // [warp][entries], [warp][entries' scales], [warp][R rows, maxima, sums], lengths, tiles before
@@ -500,13 +501,13 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         mult[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
       }
       float o[MT][NT][4], m[NT][2], ref[NT][2], l[NT][2], unit[NT][2], peak[NT][2];
-      bool fresh = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           m[n][r] = -INFINITY;
-          ref[n][r] = l[n][r] = peak[n][r] = 0.f;
+          ref[n][r] = kNone;
+          l[n][r] = peak[n][r] = 0.f;
           unit[n][r] = S::kBytes ? 8.507059e37f : 1.f;  // 2^126
         }
 #pragma unroll
@@ -580,9 +581,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
               d[s][n][e] = hidden(s, e) ? -INFINITY : fmaf(sc[s][n][e], times(s, n, e), -ref[n][e & 1]);
               top_d = fmaxf(top_d, d[s][n][e]);
             }
-        const bool grown = fresh || __any_sync(0xffffffffu, top_d > kAbove + kLazy);
+        const bool grown = __any_sync(0xffffffffu, top_d > kAbove + kLazy);
         if (grown) {
-          fresh = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
                 for (int e = r; e < 4; e += 2)
                   if (!hidden(s, e)) top = fmaxf(top, sc[s][n][e] * times(s, n, e));
               const float m_new = fmaxf(m[n][r], max_over_keys(top) - kAbove);
-              ref[n][r] = from_minus_inf(m_new);
+              ref[n][r] = m_new == -INFINITY ? kNone : m_new;
               const float alpha = ex2_approx_ftz(m[n][r] - ref[n][r]);
               m[n][r] = m_new;
               l[n][r] *= alpha;

@@ -106,3 +106,34 @@ def test_values_that_cancel(cuda, store, D, heads):
     for i, (x, s) in enumerate(((k, ks), (v, vs))):
         c.values[i] = x.float().double() * s.double()[..., None]
     check(c, c.run())
+
+
+@pytest.mark.parametrize("store", SIXTEEN)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lead", [16, 32, 100])
+@pytest.mark.parametrize("shift", [0.0, -300.0])
+def test_runs_of_keys_of_minus_infinity(cuda, store, D, lead, shift):
+    """Keys that score -inf throughout the first tiles of an item or a part do not count, before ordinary scores and before very low ones."""
+    import torch
+    for lengths, heads, kv_heads, every in (([400, lead + 1, lead + 90], 8, 1, 10 ** 6), ([300, 220], 6, 2, 10 ** 6), ([5000] * 8, 16, 8, 2 * lead)):
+        c = case(cuda, lengths, heads, kv_heads, D, 16, store, seed=lead + 1)
+        c.q.abs_().clamp_(min=0.25)
+        if shift:  # by shift or so: every query has 8 in one dimension
+            c.q[..., 0] = 8.0
+            c.cache.k[..., 0] += shift / 8 * math.sqrt(D)
+            c.values[0] = c.cache.k.double()
+        keep = []
+        for b, n in enumerate(lengths):
+            keys = runs(c, b, 0, lead, every)
+            pages, places = slots_of(c, b, keys)
+            c.cache.k[pages, :, places] = -math.inf
+            keep.append(torch.ones(n, device="cuda", dtype=torch.bool).index_fill_(0, keys, False))
+        out, lse = c.run()
+        check(c, (out, lse), keys=keep, sequences=range(min(len(lengths), 3)))
+    c = case(cuda, [lead, lead + 3000], 8, 1, D, 16, store, seed=2)  # all of one sequence's
+    c.q.abs_()
+    pages, places = slots_of(c, 0, torch.arange(lead, device="cuda"))
+    clean = c.run()
+    c.cache.k[pages, :, places] = -math.inf
+    out, lse = c.run()
+    assert out[0].isnan().all() and (lse[0] == -math.inf).all() and same(out[1], clean[0][1]) and same(lse[1], clean[1][1])
