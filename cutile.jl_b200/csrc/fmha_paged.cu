@@ -640,10 +640,12 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                sc[s][n][e] = d[s][n][e] * (vs[s][e >> 1] * unit[n][e & 1]);
+                sc[s][n][e] = d[s][n][e] * vs[s][e >> 1] * unit[n][e & 1];  // not d (vs unit), which is 0 inf for a large scale behind tiny ones
                 top_w = fmaxf(top_w, sc[s][n][e]);
               }
           if (grown || __any_sync(0xffffffffu, top_w > (float)(2 << (kLift + kLazy)))) {
+#pragma unroll
+            for (int s = 0; s < KT; ++s) asm volatile("" : "+f"(vs[s][0]), "+f"(vs[s][1]));  // products again, below: kept, they cost registers in every tile
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll

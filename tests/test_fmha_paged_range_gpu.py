@@ -90,6 +90,23 @@ def test_runs_of_zero_values(cuda, store, D, dtype, lead):
 
 
 @pytest.mark.parametrize("store", EIGHT)
+def test_large_scales_of_keys_that_do_not_count(cuda, store):
+    """Tiny values, and huge ones whose probabilities are zero in every row of the operand."""
+    import torch
+    c = case(cuda, [4000], 8, 1, 64, 16, store, "bfloat16", seed=29)
+    c.q.abs_()
+    c.cache.v_scale.mul_(1e-30)
+    keys = runs(c, 0, 150, 1, 200)
+    pages, places = slots_of(c, 0, keys)
+    c.cache.v_scale[pages, 0, places] = 1e12
+    c.cache.k[pages, 0, places] = -100
+    c.cache.k_scale[pages, 0, places] = 1.0  # scores of -100 sum |q| / 8, below -400
+    for i, (x, s) in enumerate(((c.cache.k, c.cache.k_scale), (c.cache.v, c.cache.v_scale))):
+        c.values[i] = x.float().double() * s.double()[..., None]
+    check(c, c.run(), keys=[torch.ones(4000, device="cuda", dtype=torch.bool).index_fill_(0, keys, False)])  # e^-400 1e14 is nothing beside 1e-30
+
+
+@pytest.mark.parametrize("store", EIGHT)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("heads", [4, 16])
 def test_values_that_cancel(cuda, store, D, heads):
