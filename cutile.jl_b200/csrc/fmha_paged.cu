@@ -623,8 +623,8 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
             }
         if constexpr (S::kBytes) {
           // A probability times its value's scale goes to f16 in units of (about) the largest so far: scales differ from key to key by
-          // any factor.  While there was none above 0 (rows of zeros have scales of 0) the unit is 2^126, the largest there is, which the first
-          // that is more than 2^-111 exceeds.
+          // any factor.  While all were 0 (rows of zeros have scales of 0) the unit is 2^126, the largest there is, with which the first
+          // beyond 2^-111 is too large.
           float vs[KT][2];
 #pragma unroll
           for (int s = 0; s < KT; ++s)
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 sc[s][n][e] = d[s][n][e] * vs[s][e >> 1] * unit[n][e & 1];  // not d (vs unit), which is 0 inf for a large scale behind tiny ones
-                top_w = fmaxf(top_w, sc[s][n][e]);
+                top_w = fmaxf(top_w, fabsf(sc[s][n][e]));
               }
           if (grown || __any_sync(0xffffffffu, top_w > (float)(2 << (kLift + kLazy)))) {
 #pragma unroll
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
 #pragma unroll
                 for (int s = 0; s < KT; ++s)
 #pragma unroll
-                  for (int e = r; e < 4; e += 2) top = fmaxf(top, d[s][n][e] * vs[s][e >> 1]);
+                  for (int e = r; e < 4; e += 2) top = fmaxf(top, fabsf(d[s][n][e] * vs[s][e >> 1]));
                 top = max_over_keys(top);
                 peak[n][r] = top;
                 const int e = (int)(__float_as_uint(top) >> 23);

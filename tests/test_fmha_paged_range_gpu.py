@@ -90,6 +90,22 @@ def test_runs_of_zero_values(cuda, store, D, dtype, lead):
 
 
 @pytest.mark.parametrize("store", EIGHT)
+@pytest.mark.parametrize("dtype", SIXTEEN)
+def test_negative_scales(cuda, store, dtype):
+    """A value is code * scale, whatever the scale's sign: all of them negative, or the large ones only, later than small positive ones."""
+    import torch
+    for every in (True, False):
+        c = case(cuda, [500, 70], 8, 1, 64, 16, store, dtype, seed=23)
+        c.cache.v_scale.mul_(-1e-4 if every else 1e-4)
+        if not every:
+            for b in (0, 1):
+                pages, places = slots_of(c, b, torch.arange(64, int(c.lengths[b]), device="cuda"))
+                c.cache.v_scale[pages, :, places] *= -1e5
+        c.values[1] = c.cache.v.float().double() * c.cache.v_scale.double()[..., None]
+        check(c, c.run())
+
+
+@pytest.mark.parametrize("store", EIGHT)
 def test_large_scales_of_keys_that_do_not_count(cuda, store):
     """Tiny values, and huge ones whose probabilities are zero in every row of the operand."""
     import torch
