@@ -199,6 +199,44 @@ struct Shares {
   }
 };
 
+// Of the dimensions 8 i + g of a lane, those (bit i) of which some value of a sequence's keys first .. end - 1 is infinite, with one sign (bit
+// 16 + i: minus) and no NaN beside it.  The four lanes of a dimension look at a key each.  A key that is not finite itself has a
+// probability of 0 or NaN in every row: its infinite values are as good as NaN.  Not inlined: seldom called, and in the way otherwise.
+template <bool BF, int D>
+__device__ __noinline__ uint32_t infinite_values(const uint16_t* K, const uint16_t* V, int64_t k_page, int64_t v_page, const int32_t* pages,
+                                                 int page_log2, int first, int end) {
+  constexpr uint32_t kInf = BF ? 0x7f80 : 0x7c00;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  uint32_t plus = 0, minus = 0, nan = 0;
+  for (int key = first + c; key < end; key += 4) {
+    const int64_t page = __ldg(pages + (key >> page_log2)) - 1, at = (key & ((1 << page_log2) - 1)) * D;
+    const uint16_t *v = V + page * v_page + at, *k = K + page * k_page + at;
+    uint32_t up = 0, down = 0;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const uint32_t x = __ldg(v + 8 * i + g);
+      up |= (uint32_t)(x == kInf) << i;
+      down |= (uint32_t)(x == (kInf | 0x8000)) << i;
+      nan |= (uint32_t)((x & 0x7fff) > kInf) << i;
+    }
+    if (up | down) {
+      bool finite = true;
+      for (int i = 0; i < D; ++i) finite &= (__ldg(k + i) & 0x7fff) < kInf;
+      if (!finite) nan |= up | down;
+    }
+    plus |= up;
+    minus |= down;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    plus |= __shfl_xor_sync(0xffffffffu, plus, x);
+    minus |= __shfl_xor_sync(0xffffffffu, minus, x);
+    nan |= __shfl_xor_sync(0xffffffffu, nan, x);
+  }
+  return ((plus ^ minus) & ~nan) | minus << 16;
+}
+
 // A tile: the sequence, the row of heads, and the keys.
 struct Cursor {
   unsigned x;                 // its place on the line
@@ -752,9 +790,35 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         leave_entry(AfterValues());
       };
       const unsigned end = min(hi, item_hi);
+      [[maybe_unused]] const int first_key = now.key;
       for (; now.x < end; ++now.x, now.key += kTileKeys) {
         if (now.key + kTileKeys <= len) tile(std::false_type());
         else tile(std::true_type());
+      }
+      if constexpr (!S::kBytes) {
+        // An infinite value: its product with the low half of a probability, zero or negative, is a NaN beside the one with the high
+        // half.  (8-bit rows with an infinity have a scale that is one, and codes of 0.)
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= o[j][n][e] != o[j][n][e];
+        if (__any_sync(0xffffffffu, odd) && !bad) {
+          const int64_t at = ((int64_t)head << p.page_log2) * D;
+          const uint32_t found = infinite_values<BF, D>(static_cast<const uint16_t*>(p.K) + at, static_cast<const uint16_t*>(p.V) + at, p.k_page, p.v_page,
+                                                        p.table + b * p.table_ld, p.page_log2, first_key, min(now.key, len));
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t here = found >> (2 * j + (e >> 1));
+                if (o[j][n][e] != o[j][n][e] && (here & 1)) o[j][n][e] = here & 0x10000 ? -INFINITY : INFINITY;
+              }
+        }
       }
       if (now.x == item_hi) next_item(now);
       // ---- leaving the item

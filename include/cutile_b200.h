@@ -332,7 +332,8 @@ int ctb_kv_read(ctb_ctx* ctx, void* stream, void* K, void* V, const ctb_kv_cache
  * cache's type if that has 16 bits), with strides from sequence to sequence and head to head (multiples of 8); Out (head_dim,
  * heads, batch) in the type of Q and lse (heads, batch) f32, dense.  heads is a multiple of kv_heads, and head h has the keys of
  * h / (heads / kv_heads).  A length of 0 gives zeros and -inf; bad lengths and pages as above make the sequence's (for a page, the
- * heads') results NaN.  What the cache holds behind a sequence's length does not matter.  Scores, sums and outputs are f32,
+ * heads') results NaN.  What the cache holds behind a sequence's length does not matter.  An infinite
+ * value makes its dimension infinite (NaN beside one of the other sign).  Scores, sums and outputs are f32,
  * probabilities enter the product with values as the sum of two 16-bit numbers.  Bitwise repeatable. */
 int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse, const void* Q, const ctb_kv_cache* cache,
                    const int32_t* page_table, const int32_t* lengths, int64_t batch, int64_t heads, int64_t q_seq_stride,

@@ -170,3 +170,27 @@ def test_runs_of_keys_of_minus_infinity(cuda, store, D, lead, shift):
     c.cache.k[pages, :, places] = -math.inf
     out, lse = c.run()
     assert out[0].isnan().all() and (lse[0] == -math.inf).all() and same(out[1], clean[0][1]) and same(lse[1], clean[1][1])
+
+
+@pytest.mark.parametrize("store", SIXTEEN)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([100, 37], 8, 1), ([9000], 4, 2), ([3000] * 3, 32, 2)])
+def test_infinite_values(cuda, store, D, lengths, heads, kv_heads):
+    """An infinite value makes its dimension infinite, infinities of both signs and a NaN make it NaN, and nothing else changes."""
+    import torch
+    c = case(cuda, lengths, heads, kv_heads, D, 16, store, seed=37)
+    clean = c.run()
+    inf, nan = math.inf, math.nan
+    b, h = len(lengths) - 1, kv_heads - 1
+    n = lengths[b]
+    marks = {0: [(3, inf)], 9: [(n - 1, -inf)], 17: [(0, inf), (n // 2, inf)], 25: [(1, inf), (n - 2, -inf)], 33: [(5, inf), (20, nan)], D - 1: [(n // 3, -inf)]}
+    for dim, at in marks.items():
+        for key, x in at:
+            (page,), (place,) = slots_of(c, b, torch.tensor([key], device="cuda"))
+            c.cache.v[page, h, place, dim] = x
+    out, lse = c.run()
+    group = heads // kv_heads
+    want = clean[0].clone()
+    for dim, at in marks.items():
+        want[b, h * group:(h + 1) * group, dim] = sum(x for _, x in at)
+    assert same(out, want) and same(lse, clean[1])
