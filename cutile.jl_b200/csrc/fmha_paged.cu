@@ -1072,6 +1072,8 @@ extern "C" int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse,
   if (lse) CTB_CHECK_DEV(lse);
   if (table_width) CTB_CHECK_DEV(page_table);
   if (table_stride < table_width && batch > 1) return fail(CTB_BAD_ARG, "ctb_fmha_paged: rows of the page table overlap");
+  if (batch == 1) q_seq_stride = 0;  // none along what has one element
+  if (heads == 1) q_head_stride = 0;
   if ((uintptr_t)Q % 16 || (uintptr_t)Out % 16 || q_seq_stride % 8 || q_head_stride % 8)
     return fail(CTB_BAD_ALIGN, "ctb_fmha_paged: Q and Out must be 16-byte aligned and the strides of Q multiples of 8 elements");
   Params p = {};

@@ -194,3 +194,17 @@ def test_infinite_values(cuda, store, D, lengths, heads, kv_heads):
     for dim, at in marks.items():
         want[b, h * group:(h + 1) * group, dim] = sum(x for _, x in at)
     assert same(out, want) and same(lse, clean[1])
+
+
+def test_strides_of_one_element(cuda):
+    """Strides along a dimension of one element mean nothing."""
+    import torch
+    c = case(cuda, [40], 4, 2, 64, 16, "float16", seed=41)
+    q = c.q.as_strided((1, 4, 64), (4 * 64 + 1, 64, 1))
+    want = c.run()
+    got = cuda.fmha.fmha_paged(q, c.cache, c.table, c.lengths, return_lse=True)
+    assert got[0].equal(want[0]) and got[1].equal(want[1])
+    assert cuda.fmha.fmha_paged(q, c.cache, c.table, c.lengths, occupancy=1).equal(want[0])
+    c = case(cuda, [40, 3], 1, 1, 64, 16, "bfloat16", seed=43)
+    q = c.q.as_strided((2, 1, 64), (64, 3, 1))
+    assert cuda.fmha.fmha_paged(q, c.cache, c.table, c.lengths).equal(c.run()[0])
