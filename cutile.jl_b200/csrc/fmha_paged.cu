@@ -11,7 +11,7 @@
 // 4 KB of values each.  The tiles of all items form one line that the warps of the grid share out in equal contiguous ranges, whatever the
 // lengths are: every CTA finds the tiles before every sequence by a scan over the lengths, which only the device knows.  An item counts a
 // tile more than it has, for its queries and results (64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
-// longest item has at most kWholeItems tiles, ranges of CTAs end where items end, so that no CTA has to wait for another's part (16
+// longest item has at most kWholeItems tiles (or there is no scratch for parts), ranges of CTAs end where items end, so that no CTA has to wait for another's part (16
 // x 1000 keys 15.9 us with parts, 12.8 with whole items; 8 x 4000 in e4m3, 125 tiles, 20.1 and 25.6 us).  A warp leaves an item that it has
 // as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
 // takes rows of parts to join, and items that several CTAs have are joined by the one that arrives last, in ascending order of the parts.  The
@@ -34,6 +34,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <optional>
 #include <type_traits>
 
 #include "ctx.h"
@@ -63,6 +64,7 @@ struct Params {
   int batch, heads, kv_heads, group, row_tiles, width, page_log2, pages;
   int q_bf16;
   float scale_log2;
+  unsigned whole_items;  // tiles of the longest item up to which CTAs have whole items: kWholeItems, or any number without scratch
   float* part;        // [CTA][first, last item of its range][rows x D, maxima, sums]
   unsigned* tickets;  // per CTA: parts left of the item that begins in its range and ends in another's
 };
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
         before = behind;
       }
     };
-    if (longest <= kWholeItems) {
+    if (longest <= p.whole_items) {
       // Whole items: a CTA's range ends where an item does that is next to the end of an equal range.  Whoever has that sequence says where.
       const Shares equal(total, gridDim.x);
       const unsigned at[2] = {equal.first(blockIdx.x), equal.first(blockIdx.x + 1)};
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(Shape<STORE, D, NT>::kThreads, 1)
   // ends where an item ends.
   auto warp_shares = [&] { return Shares(total, min(gridDim.x * kWarps, total)); };
   unsigned lo, hi;
-  if (longest <= kWholeItems) {
+  if (longest <= p.whole_items) {
     const unsigned n = ends[1] - ends[0];
     lo = ends[0] + warp * n / kWarps;
     hi = ends[0] + (warp + 1) * n / kWarps;
@@ -1015,18 +1017,25 @@ int launch(ctb_ctx* ctx, cudaStream_t st, Params p, int64_t batch) {
   static_assert(S::kSmem <= 227 * 1024, "shared memory of a CTA");
   p.row_tiles = (p.group + S::R - 1) / S::R;
   // of a sequence, at most; one where the page table is empty
-  const int64_t tiles = std::max<int64_t>(1, ((((int64_t)p.width << p.page_log2) + 16 * S::KT - 1) / (16 * S::KT) + kItemCost) * p.kv_heads * p.row_tiles);
+  const int64_t most = (((int64_t)p.width << p.page_log2) + 16 * S::KT - 1) / (16 * S::KT) + kItemCost;  // of an item
+  const int64_t tiles = std::max<int64_t>(1, most * p.kv_heads * p.row_tiles);
   if (tiles > INT32_MAX) return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: a sequence has too many keys");
   const int64_t chunk = std::min<int64_t>(kMaxBatch, INT32_MAX / tiles);
-  if ((size_t)ctx->sm_count * 2 * S::kPartFloats * sizeof(float) > kSlotBytes || ctx->sm_count > kTickets)
-    return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: more SMs than the split over keys has scratch for");
   auto kern = fmha_paged_kernel<STORE, D, NT>;
   cudaError_t e = allow_smem(kern, S::kSmem);
   if (e != cudaSuccess) return cuda_fail(e, "ctb_fmha_paged: shared memory opt-in");
-  const StreamScratch scratch(ctx, st);
-  if (!scratch.data) return fail(CTB_CUDA_ERROR, "ctb_fmha_paged: no scratch for the split over keys");
-  p.part = scratch.data;
-  p.tickets = scratch.tickets;
+  std::optional<StreamScratch> scratch;  // until the kernel is launched
+  p.whole_items = UINT32_MAX;            // no scratch, or more SMs than it has room for
+  if (most <= kWholeItems) {
+    p.whole_items = kWholeItems;  // none is used
+  } else if ((size_t)ctx->sm_count * 2 * S::kPartFloats * sizeof(float) <= kSlotBytes && ctx->sm_count <= kTickets) {
+    scratch.emplace(ctx, st);
+    if (scratch->data) {
+      p.part = scratch->data;
+      p.tickets = scratch->tickets;
+      p.whole_items = kWholeItems;
+    }
+  }
   for (int64_t b = 0; b < batch; b += chunk) {
     Params q = p;
     q.batch = (int)std::min(chunk, batch - b);

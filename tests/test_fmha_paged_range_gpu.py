@@ -208,3 +208,28 @@ def test_strides_of_one_element(cuda):
     c = case(cuda, [40, 3], 1, 1, 64, 16, "bfloat16", seed=43)
     q = c.q.as_strided((2, 1, 64), (64, 3, 1))
     assert cuda.fmha.fmha_paged(q, c.cache, c.table, c.lengths).equal(c.run()[0])
+
+
+def test_no_scratch_where_none_is_used(cuda):
+    """A page table too narrow for items that several CTAs share takes no scratch: neither a stream's nor a graph's."""
+    import torch
+    c = case(cuda, [700, 20], 8, 2, 128, 16, "bfloat16", seed=47)
+    want = c.run()
+    side, pool = torch.cuda.Stream(), torch.cuda.graph_pool_handle()
+    out = None
+
+    def capture():
+        nonlocal out
+        graph = torch.cuda.CUDAGraph()
+        out = None  # its place in the pool is the next one's
+        with torch.cuda.graph(graph, stream=side, pool=pool):
+            out = c.run()
+        return graph
+    graphs = [capture() for _ in range(4)]
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    graphs += [capture() for _ in range(60)]
+    assert free - torch.cuda.mem_get_info()[0] < 64 << 20  # 60 slots of 2.5 MB would be 150
+    graphs[-1].replay()
+    torch.cuda.synchronize()
+    assert out[0].equal(want[0]) and out[1].equal(want[1])
