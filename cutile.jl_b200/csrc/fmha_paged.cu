@@ -1072,9 +1072,10 @@ extern "C" int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse,
   if (dtype != CTB_F16 && dtype != CTB_BF16) return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: queries are f16 or bf16");
   if (cache->dtype != dtype && cache->dtype != CTB_E4M3 && cache->dtype != CTB_I8)
     return fail(CTB_BAD_ARG, "ctb_fmha_paged: a cache of 16-bit elements has the type of the queries");
-  if (!isfinite(qk_scale)) return fail(CTB_BAD_ARG, "ctb_fmha_paged: qk_scale is not finite");
+  const float scale_log2 = qk_scale * 1.4426950408889634f;
+  if (!isfinite(scale_log2)) return fail(CTB_BAD_ARG, "ctb_fmha_paged: qk_scale is not finite (in powers of two)");
   const int64_t D = cache->head_dim, page = cache->page_size;
-  if (heads > 65536 || table_width * page > (1 << 28) || table_width > (1 << 28))
+  if (heads > 65536 || table_width > (1 << 28) / page)
     return fail(CTB_UNSUPPORTED, "ctb_fmha_paged: shape too large");
   if (batch == 0) return CTB_OK;
   CTB_CHECK_DEV(Q); CTB_CHECK_DEV(Out); CTB_CHECK_DEV(lengths);
@@ -1096,7 +1097,7 @@ extern "C" int ctb_fmha_paged(ctb_ctx* ctx, void* stream, void* Out, float* lse,
   p.width = (int)table_width; p.pages = (int)cache->pages;
   while ((1ll << p.page_log2) < page) ++p.page_log2;
   p.q_bf16 = dtype == CTB_BF16;
-  p.scale_log2 = qk_scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (cache->dtype) {
     case CTB_F16: return pick<F16>(ctx, st, p, batch, D);

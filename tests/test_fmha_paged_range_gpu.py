@@ -233,3 +233,10 @@ def test_no_scratch_where_none_is_used(cuda):
     graphs[-1].replay()
     torch.cuda.synchronize()
     assert out[0].equal(want[0]) and out[1].equal(want[1])
+
+
+def test_scale_refused(cuda):
+    """A scale that is no f32 number in powers of two."""
+    c = case(cuda, [20], 2, 1, 64, 16, "float16")
+    with pytest.raises(cuda.CtbError, match="not finite"):
+        c.run(qk_scale=3e38)
