@@ -326,7 +326,7 @@ bool token_strides(const Tensor& t, int64_t* s) {
 }
 int index_bits(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : t.scalar_type() == at::kLong ? 64 : 0; }
 bool frequencies_of(const Tensor* f, const Tensor& like) {
-  return f && f->scalar_type() == at::kDouble && f->dim() == 1 && f->is_contiguous() && f->device() == like.device();
+  return f && f->scalar_type() == at::kDouble && f->dim() == 1 && f->size(0) > 0 && f->is_contiguous() && f->device() == like.device();
 }
 // A new array, without the dispatcher: at::empty takes 0.6 us more.
 Tensor new_array(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {

@@ -113,6 +113,8 @@ def kv_write(cache, slots, k, v, q=None, positions=None, frequencies=_LEFT_OUT, 
         if not isinstance(frequencies, torch.Tensor) or frequencies.dim() != 1:
             raise _lib.CtbError(_lib.BAD_ARG, "frequencies: expected a tensor of one dimension")
         rotary = 2 * dense(frequencies, frequencies.shape, "frequencies", k, torch.float64).shape[0]
+        if rotary == 0:
+            raise _lib.CtbError(_lib.BAD_ARG, "kv_write: frequencies of no pairs (rotary is 0); None turns nothing")
     if q is not None:
         _rows_of(q, None, D, T, "q", k)
         heads = q.shape[1]

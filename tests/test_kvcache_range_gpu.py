@@ -7,6 +7,20 @@ from test_kvcache_gpu import STORES, places
 pytestmark = pytest.mark.gpu
 
 
+def test_frequencies_of_no_pairs(cuda):
+    """An empty array, whose address is null, is not the same as none."""
+    import torch
+    cache = cuda.kvcache.kv_cache(1, 2, 16, 64, torch.float16)
+    k, positions = torch.ones(3, 2, 64, device="cuda").half(), torch.arange(1, 4, device="cuda")
+    none = torch.empty(0, device="cuda", dtype=torch.float64)
+    for more in ({}, dict(q=k), dict(occupancy=1)):
+        with pytest.raises(cuda.CtbError, match="rotary"):
+            cuda.kvcache.kv_write(cache, positions, k, k, positions=positions, frequencies=none, **more)
+    with pytest.raises(cuda.CtbError, match="rotary"):
+        cuda.rope.rope_fwd(k, None, positions, none)
+    assert (cache.k == 0).all()
+
+
 @pytest.mark.parametrize("store", STORES)
 @pytest.mark.parametrize("bits", ["int32", "int64"])
 def test_rows_that_are_not_turned(cuda, store, bits):
