@@ -60,11 +60,22 @@ int check_turned_in_place(const char* who, const void* in, const int64_t* in_str
     const int64_t n = extents[i] - 1;
     if (n == 0) continue;
     if (in_strides[i] < 0 || out_strides[i] < 0) return fail(CTB_BAD_ARG, "%s: negative strides", who);
-    if (out_strides[i] < D) return fail(CTB_BAD_ARG, "%s: the rows of a result overlap", who);
     if (in_strides[i] > INT64_MAX / 64 / n || out_strides[i] > INT64_MAX / 64 / n) return fail(CTB_UNSUPPORTED, "%s: strides too large", who);
     in_last += n * in_strides[i];
     out_last += n * out_strides[i];
     same &= in_strides[i] == out_strides[i];
+  }
+  // In the order of their strides, the rows of a dimension lie behind all that one of them has.
+  int64_t reach = D;
+  bool seen[3] = {};
+  for (int step = 0; step < 3; ++step) {
+    int next = -1;
+    for (int i = 0; i < 3; ++i)
+      if (!seen[i] && extents[i] > 1 && (next < 0 || out_strides[i] < out_strides[next])) next = i;
+    if (next < 0) break;
+    if (out_strides[next] < reach) return fail(CTB_BAD_ARG, "%s: the rows of a result overlap", who);
+    seen[next] = true;
+    reach += (extents[next] - 1) * out_strides[next];
   }
   const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out;
   if (same || a + in_last * elem_size <= b || b + out_last * elem_size <= a) return CTB_OK;

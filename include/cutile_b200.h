@@ -293,7 +293,8 @@ int ctb_fmha_fwd(ctb_ctx* ctx, void* stream, const void* Q, const void* K, const
  * k_heads, seq, batch) in CTB_F32, CTB_F16 or CTB_BF16, dimensions contiguous, with strides[12] (elements) of q_out, q, k_out, k:
  * batch, seq, head each.  positions (seq, batch), dense, 32- or 64-bit; frequencies (rotary / 2) f64, both device arrays.  Angles are
  * formed and reduced in f64 (|n| < 2^31), cosines and sines are within 2^-22, and results are rounded once.  A result may lie
- * where its rows lie (the same address and strides), and must not overlap them, or the other array, in any other way. */
+ * where its rows lie (the same address and strides) or apart from them, from its first element to its last; it must not overlap the other
+ * array, and its own rows must not overlap (in the order of their strides, those of a dimension lie behind all that one of them has). */
 int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, void* k_out, const void* k, const void* positions,
              int position_bits, const double* frequencies, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t D,
              int64_t rotary, const int64_t* strides, int interleaved, int inverse, float scale, int dtype);
@@ -315,8 +316,8 @@ typedef struct ctb_kv_cache {
 /* Writes k and v (head_dim, kv_heads, tokens), CTB_F16 or CTB_BF16 (the cache's type, or any of the two for 8 bits), to slots
  * (tokens) 32- or 64-bit; slot 0 writes nothing, a slot outside of the cache is a bad index (ctb_check_device_status) and writes
  * nothing either; slots that are not 0 must differ.  With frequencies, keys are turned by their positions as by ctb_rope before
- * they are stored (rounded once, when stored), and so are the queries q (head_dim, heads, tokens), if given, into q_out, for all tokens.
- * strides[8] (elements): of q_out, q, k, v: token, head each.
+ * they are stored (rounded once, when stored), and so are the queries q (head_dim, heads, tokens), if given, into q_out, for all tokens
+ * (q_out as a result of ctb_rope; it overlaps neither k, v nor the cache).  strides[8] (elements): of q_out, q, k, v: token, head each.
  * 8 bits: with a the largest magnitude of a row and c the largest code, scale = a / c and code = x c / a, rounded to the
  * nearest, ties to even.  Rows with a < 2^-100 are stored as zeros, rows with an infinity or NaN with a scale that is one. */
 int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cache, const void* slots, int slot_bits, void* q_out,

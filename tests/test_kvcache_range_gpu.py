@@ -3,6 +3,7 @@ test_rope_gpu; calls that their documentation allows and those tests do not make
 import pytest
 
 from test_kvcache_gpu import STORES, places
+from test_rope_gpu import close, make
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,26 @@ def test_rows_that_are_not_turned(cuda, store, bits):
             cuda.kvcache.kv_write(caches[0], slots, k, v, positions=bad, frequencies=None)
     with pytest.raises(cuda.CtbError, match="positions and frequencies"):
         cuda.kvcache.kv_write(caches[0], slots, k, v, q=k, positions=positions, frequencies=None)
+
+
+def test_results_whose_rows_overlap(cuda):
+    """Strides that are each as long as a row, but too short together."""
+    import torch
+    f, positions = cuda.rope.rope_frequencies(64).cuda(), torch.arange(3, device="cuda")
+    q = make(3, 2, 64, "float16")
+    store = torch.zeros(4096, device="cuda", dtype=torch.float16)
+    cache = cuda.kvcache.kv_cache(1, 2, 16, 64, torch.float16)
+    for strides in ((64, 64, 1), (96, 64, 1), (64, 96, 1), (64, 191, 1)):
+        out = store.as_strided((3, 2, 64), strides)
+        with pytest.raises(cuda.CtbError, match="rows of a result overlap"):
+            cuda.rope.rope_fwd(q, None, positions, f, out_q=out)
+        with pytest.raises(cuda.CtbError, match="rows of a result overlap"):
+            cuda.kvcache.kv_write(cache, positions, q, q, q=q, positions=positions, frequencies=f, out_q=out)
+    assert (store == 0).all() and (cache.k == 0).all()
+    for strides in ((128, 64, 1), (64, 192, 1), (200, 72, 1)):
+        out = store.as_strided((3, 2, 64), strides)
+        cuda.rope.rope_fwd(q, None, positions, f, out_q=out)
+        close(out, q, positions, f.cpu())
+    out = store.as_strided((1, 3, 2, 64), (1, 128, 64, 1))  # the batch of one has no stride
+    cuda.rope.rope_fwd(q[None], None, positions[None], f, out_q=out)
+    close(out[0], q, positions, f.cpu())
