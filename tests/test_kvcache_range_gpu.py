@@ -2,10 +2,80 @@
 test_rope_gpu; calls that their documentation allows and those tests do not make."""
 import pytest
 
-from test_kvcache_gpu import STORES, places
+from test_kvcache_gpu import STORES, filled, places, rows_at, stored_close, turned, untouched
 from test_rope_gpu import close, make
 
 pytestmark = pytest.mark.gpu
+
+
+# Tokens * heads * D is above what 148 SMs take one group per warp for (2.42 M elements); two groups per warp up to 512 elements of keys per token,
+# then four.  Heads that do not fill the groups of a task, tokens that do not fill the last CTA, and queries that are few or many beside the keys.
+@pytest.mark.parametrize("T,H,KVH,D,page,R,interleaved,shift", [
+    (2501, 8, 4, 128, 16, 128, False, 0), (10001, 0, 2, 64, 32, 64, False, 0), (4003, 3, 8, 64, 64, 32, True, 0), (3001, 40, 1, 128, 16, 24, False, 0),
+    (2000, 5, 5, 128, 128, 64, False, 1), (1701, 32, 8, 128, 16, 128, False, 0), (3001, 1, 9, 64, 1024, 64, True, 0), (2003, 0, 8, 128, 16, 0, False, 0),
+    (1999, 9, 9, 128, 32, 12, True, 1), (8200, 0, 9, 64, 16, 6, False, 0), (5003, 2, 5, 128, 64, 2, True, 0)])
+@pytest.mark.parametrize("store", STORES)
+def test_large_writes(cuda, T, H, KVH, D, page, R, interleaved, shift, store):
+    import torch
+    assert T * (H + 2 * KVH) * D >= 256 * 4 * 16 * 148
+    dtype = getattr(torch, store) if store.endswith("float16") else (torch.bfloat16 if T % 3 else torch.float16)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    base = torch.randn(T, (H + 2 * KVH) * D + 8 * shift + shift, device="cuda", generator=g).to(dtype)
+    q, k, v = base[:, shift:shift + (H + 2 * KVH) * D].unflatten(1, (H + 2 * KVH, D)).split((H, KVH, KVH), 1)
+    pages = -(-T // page) + 3
+    cache = filled(cuda, pages, KVH, page, D, store)
+    before = [None if t is None else t.clone() for t in cache]
+    slots = places(pages, page, T, T)
+    slots[::7] = 0
+    live = slots > 0
+    f = cuda.rope.rope_frequencies(R) if R else None
+    positions = torch.randint(0, 100000, (T,), device="cuda", generator=g)
+    more = dict(positions=positions, frequencies=f.cuda(), interleaved=interleaved, scale=0.75, q=q if H else None) if R else {}
+    out = cuda.kvcache.kv_write(cache, slots, k, v, **more)
+    untouched(before, cache, slots[live])
+    if H and R:
+        close(out, q, positions, f, interleaved=interleaved, scale=0.75)
+        was, kept = q.clone(), base.clone()
+        assert cuda.kvcache.kv_write(cache, slots, k, v, out_q=q, **more) is q  # in place
+        assert q.equal(out)
+        q.copy_(was)
+        assert base.equal(kept)
+    else:
+        assert out is None
+    for i, x in enumerate((k, v)):
+        got = rows_at(cache[i], slots[live])
+        want, off = turned(x, positions, f if i == 0 else None, interleaved)
+        if cache.k_scale is not None:
+            stored_close(got, rows_at(cache[2 + i], slots[live]), want[live], off[live] if torch.is_tensor(off) else off)
+        elif i == 1 or not R:
+            assert got.equal(x[live])
+        else:
+            close(got, x[live], positions[live], f, interleaved=interleaved, scale=0.75)
+
+
+# Two units per thread: from 4.85 M elements in 16-bit vectors, 2.42 M in f32 ones, 0.61 M off the grid of 16 bytes (148 SMs).
+@pytest.mark.parametrize("T,Hq,Hk,D,R,shift", [(4099, 8, 2, 128, 128, 0), (20001, 3, 1, 64, 32, 0), (16001, 2, 2, 80, 80, 0), (1201, 16, 1, 256, 64, 0),
+                                               (3001, 3, 1, 64, 64, 1), (1201, 5, 3, 66, 6, 0), (5001, 7, 0, 128, 24, 0), (150, 1, 1, 4096, 4096, 1)])
+@pytest.mark.parametrize("dtype", ("float32", "float16", "bfloat16"))
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_large_turns(cuda, T, Hq, Hk, D, R, shift, dtype, interleaved):
+    import torch
+    vector = 4 if dtype == "float32" else 8
+    assert T * (Hq + Hk) * D >= 2 * (vector if D % vector == 0 and R % (2 * vector) == 0 and not shift else 1) * 256 * 2 * 4 * 148
+    base = make(T, Hq + Hk + (1 if shift else 0), D, dtype, T).flatten(1)
+    q, k = base[:, shift:shift + (Hq + Hk) * D].unflatten(1, (Hq + Hk, D)).split((Hq, Hk), 1)
+    f = cuda.rope.rope_frequencies(R)
+    positions = torch.arange(T, device="cuda", dtype=torch.int32) * 37 + 5
+    for fn, inverse in ((cuda.rope.rope_fwd, False), (cuda.rope.rope_bwd, True)):
+        oq, ok = fn(q, k if Hk else None, positions, f.cuda(), interleaved=interleaved, scale=1.25)
+        close(oq, q, positions, f, interleaved=interleaved, scale=1.25, inverse=inverse)
+        if Hk:
+            close(ok, k, positions, f, interleaved=interleaved, scale=1.25, inverse=inverse)
+    kept = base.clone()
+    rq, rk = cuda.rope.rope_bwd(q, k if Hk else None, positions, f.cuda(), interleaved=interleaved, scale=1.25, out_q=q, out_k=k if Hk else None)
+    assert rq is q and q.equal(oq) and (not Hk or k.equal(ok))
+    base[:, shift:shift + (Hq + Hk) * D] = kept[:, shift:shift + (Hq + Hk) * D]
+    assert base.equal(kept)
 
 
 def test_frequencies_of_no_pairs(cuda):
