@@ -30,12 +30,12 @@ enum Store { Same = 0, E4M3 = 1, I8 = 2 };
 struct Cache {
   void *k, *v;
   float *ks, *vs;
-  int64_t k_page, v_page, ks_page, vs_page, tokens;  // tokens: pages * page_size
+  int64_t k_page, v_page, ks_page, vs_page;
   int kv_heads, page_log2, pages;
 };
 Cache cache_of(const ctb_kv_cache* c) {
   Cache d = {c->k, c->v, c->k_scale, c->v_scale, c->k_page_stride, c->v_page_stride, c->k_scale_page_stride, c->v_scale_page_stride,
-             c->pages * c->page_size, (int)c->kv_heads, 0, (int)c->pages};
+             (int)c->kv_heads, 0, (int)c->pages};
   while ((1ll << d.page_log2) < c->page_size) ++d.page_log2;
   return d;
 }

@@ -140,7 +140,8 @@ def page_table_of(page_table, lengths, like):
 
 def kv_read(cache, page_table, lengths, max_length, dtype=None, **hints):
     """The first lengths[b] tokens (int32) of every sequence's pages as dense K and V [Batch, KV_Heads, max_length, D], zeros behind them:
-    what `fmha.cutile_fmha` takes.  dtype f16 or bf16, for a 16-bit cache its own."""
+    the layout of `fmha.cutile_fmha`, which takes heads of 64 and sequences of one length (the zeros behind a shorter one would count).  dtype f16
+    or bf16, for a 16-bit cache its own."""
     if not hints:
         r = _host.kv_read(cache, page_table, lengths, max_length, dtype)
         if r is not None:

@@ -325,7 +325,7 @@ function kv_write(cache::KvCache, slots::CuArray, k::CuArray{X,3}, v::CuArray{X,
     return oq
 end
 
-"The first tokens of every sequence (table (width, batch), lengths (batch), Int32) as dense (D, seq, heads, batch) K and V: what `cutile_fmha` takes."
+"The first tokens of every sequence (table (width, batch), lengths (batch), Int32) as dense (D, seq, heads, batch) K and V: the layout of `cutile_fmha`, which takes heads of 64 and sequences of one length."
 function kv_read(cache::KvCache, page_table::CuArray{Int32,2}, lengths::CuArray{Int32,1}, seq::Int, X::Type)
     D, _, heads, _ = size(cache.k); width, batch = size(page_table)
     K = CuArray{X}(undef, D, seq, heads, batch); V = similar(K)

@@ -323,8 +323,9 @@ typedef struct ctb_kv_cache {
 int ctb_kv_write(ctb_ctx* ctx, void* stream, const ctb_kv_cache* cache, const void* slots, int slot_bits, void* q_out,
                  const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int position_bits,
                  const double* frequencies, int64_t tokens, int64_t heads, int64_t rotary, int interleaved, float scale, int dtype);
-/* Reads sequences back: K, V (head_dim, seq, kv_heads, batch) dense, CTB_F16 or CTB_BF16 (of a 16-bit cache its type): what
- * ctb_fmha_fwd takes.  Tokens behind a sequence's length are zeros.  A length outside of 0..table_width * page_size, or a page that a
+/* Reads sequences back: K, V (head_dim, seq, kv_heads, batch) dense, CTB_F16 or CTB_BF16 (of a 16-bit cache its type): the
+ * layout of ctb_fmha_fwd, which takes head_dim 64 and sequences of one length (zeros behind a shorter one would count).  Tokens behind a
+ * sequence's length are zeros.  A length outside of 0..table_width * page_size, or a page that a
  * length needs outside of 1..pages, is a bad index, and the tokens in question are NaN. */
 int ctb_kv_read(ctb_ctx* ctx, void* stream, void* K, void* V, const ctb_kv_cache* cache, const int32_t* page_table,
                 const int32_t* lengths, int64_t batch, int64_t seq, int64_t table_width, int64_t table_stride, int dtype);
