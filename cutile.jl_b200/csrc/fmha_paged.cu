@@ -3,17 +3,16 @@
 //
 // What bounds it is HBM: every stored key and value is read once, 2 D bytes times the element's size, against 4 D operations per row.
 // 64 sequences of up to 8000 tokens, 64 heads over 8 of 128 in bf16 (1018 MB): 161 us, 6.3 TB/s, 0.97 of the copy rate; one sequence of
-// 131072 in f16 89 us (0.92); 128 of up to 4096 in e4m3 (560 MB) 100 us (0.85); 4 of up to 500 8.6 us, which are latencies: lengths (0.9 us),
+// 131072 in f16 89 us (0.92); 128 of up to 4096 in e4m3 (560 MB) 102 us (0.84); 4 of up to 500 8.8 us, which are latencies: lengths (0.9 us),
 // ranges (0.3), page numbers (1.1), the first keys (0.6), tiles, meeting (1) and joining (1).
-// In 8 bits the 670 (e4m3) or 870 (int8) instructions of a tile of 32 keys come next to HBM: with pages out of L2 the same keys take 76 or 86 us.
+// In 8 bits the 630 (e4m3) or 820 (int8) instructions of a tile of 32 keys come next to HBM: with pages out of L2 the same keys take 80 or 91 us.
 //
 // Work is cut into tiles of 16 to 64 keys of one item (a sequence, a key/value head, a row of up to 16 heads of its group); 4 KB of keys and
 // 4 KB of values each.  The tiles of all items form one line that the warps of the grid share out in equal contiguous ranges, whatever the
 // lengths are: every CTA finds the tiles before every sequence by a scan over the lengths, which only the device knows.  An item counts a
 // tile more than it has, for its queries and results (64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
-// longest item has at most kWholeItems tiles (or there is no scratch for parts), ranges of CTAs end where items end, so that no CTA has to wait for another's part (16
-// x 1000 keys 15.9 us with parts, 12.8 with whole items; 8 x 4000 in e4m3, 125 tiles, 20.1 and 25.6 us).  A warp leaves an item that it has
-// as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
+// longest item has at most kWholeItems tiles (or there is no scratch for parts), ranges of CTAs end where items end, so that no CTA has to
+// wait for another's part (figures at kWholeItems).  A warp leaves an item that it has as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
 // takes rows of parts to join, and items that several CTAs have are joined by the one that arrives last, in ascending order of the parts.  The
 // ranges hang on the lengths alone, so that results are the same from run to run.
 //
@@ -28,7 +27,8 @@
 // the columns: a tcgen05 tile of 128 rows would be 94 % padding, and the tensor work is an eighth of what this path delivers.
 // A lane reads 16-byte chunks of a key and takes its dimensions in the order in which they come, queries accordingly.  Probabilities go from the
 // accumulators' layout into the operand's by a transposition in registers, 16-bit values by transposing loads, 8-bit codes by byte
-// permutes; codes become f16 as they are read (exact), their scales multiply scores and probabilities.
+// permutes; codes become f16 as they are read (exact), their scales multiply scores and probabilities.  Probabilities enter as two 16-bit
+// numbers, which leave 2^-16 of them at most: one f16 beside 8-bit codes (2^-11) took up to 7 % less time where a tile's instructions count.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
