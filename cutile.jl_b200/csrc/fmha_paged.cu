@@ -12,9 +12,10 @@
 // lengths are: every CTA finds the tiles before every sequence by a scan over the lengths, which only the device knows.  An item counts a
 // tile more than it has, for its queries and results (64 x 500 keys in bf16 19.5 us without, 18.0 with).  Where the
 // longest item has at most kWholeItems tiles (or there is no scratch for parts), ranges of CTAs end where items end, so that no CTA has to
-// wait for another's part (figures at kWholeItems).  A warp leaves an item that it has as a whole with the output, otherwise with its part in shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each
-// takes rows of parts to join, and items that several CTAs have are joined by the one that arrives last, in ascending order of the parts.  The
-// ranges hang on the lengths alone, so that results are the same from run to run.
+// wait for another's part (figures at kWholeItems).  A warp leaves an item that it has as a whole with the output, otherwise with its part in
+// shared memory (maxima, sums, unnormalised output); when the CTA's warps are done, each takes rows of parts to join, and items that several
+// CTAs have are joined by the one that arrives last, in ascending order of the parts.  The ranges hang on the lengths alone, so that
+// results are the same from run to run.
 //
 // A warp streams its range for itself: it asks for keys and values in turn, an entry of 4 KB of its ring in shared memory each, three
 // entries ahead of the one that it reads (144 KB on the way per SM), by asynchronous copies of 16 bytes per lane.  Rows are exchanged in chunks

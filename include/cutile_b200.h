@@ -292,9 +292,10 @@ int ctb_fmha_fwd(ctb_ctx* ctx, void* stream, const void* Q, const void* K, const
  * other dimensions are copied.  Up to two arrays of one call (queries and keys; k may be NULL): q (D, q_heads, seq, batch), k (D,
  * k_heads, seq, batch) in CTB_F32, CTB_F16 or CTB_BF16, dimensions contiguous, with strides[12] (elements) of q_out, q, k_out, k:
  * batch, seq, head each.  positions (seq, batch), dense, 32- or 64-bit; frequencies (rotary / 2) f64, both device arrays.  Angles are
- * formed and reduced in f64 (|n| < 2^31), cosines and sines are within 2^-22 of those of the f64 product, and results are rounded once.  A result may lie
- * where its rows lie (the same address and strides) or apart from them, from its first element to its last; it must not overlap the other
- * array, and its own rows must not overlap (in the order of their strides, those of a dimension lie behind all that one of them has). */
+ * formed and reduced in f64 (|n| < 2^31), cosines and sines are within 2^-22 of those of the f64 product, and results are rounded once.
+ * A result may lie where its rows lie (the same address and strides) or apart from them, from its first element to its last; it must not
+ * overlap the other array, and its own rows must not overlap (in the order of their strides, those of a dimension lie behind all that
+ * one of them has). */
 int ctb_rope(ctb_ctx* ctx, void* stream, void* q_out, const void* q, void* k_out, const void* k, const void* positions,
              int position_bits, const double* frequencies, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t D,
              int64_t rotary, const int64_t* strides, int interleaved, int inverse, float scale, int dtype);
